@@ -85,6 +85,17 @@ class HtgsFilterView(ctypes.Structure):
                 ("focal_y", ctypes.c_float), ("center_x", ctypes.c_float), ("center_y", ctypes.c_float), ("near_plane", ctypes.c_float)]
 
 
+class HtgsFp8Matrix(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("rows", ctypes.c_int64), ("width", ctypes.c_int64),
+                ("codes_stride", ctypes.c_int64), ("scales_stride", ctypes.c_int64), ("rows_per_scale", ctypes.c_int32)]
+
+
+class HtgsScan(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("initial", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64), ("rows", ctypes.c_int64), ("width", ctypes.c_int32),
+                ("n_sequences", ctypes.c_int32), ("type", ctypes.c_int32), ("reverse", ctypes.c_int32)]
+
+
 class HtgsError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(message)
@@ -178,6 +189,24 @@ def lib():
                                                           ctypes.c_int32, ctypes.c_float, ctypes.c_float, ctypes.c_void_p]
                 l.htgs_activate.argtypes = [ctypes.c_void_p] * 7 + [ctypes.c_int32, ctypes.c_void_p]
                 l.htgs_activate_backward.argtypes = [ctypes.c_void_p] * 10 + [ctypes.c_int32, ctypes.c_void_p]
+                pointer, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+                l.htgs_add_rms_norm.argtypes = [pointer, i64, pointer, i64, pointer, i32, i64, i32, ctypes.c_float, pointer, i64, pointer, i64, pointer,
+                                                pointer, i64, pointer, i64, pointer]
+                l.htgs_add_rms_norm_backward_scratch_bytes.restype = ctypes.c_size_t
+                l.htgs_add_rms_norm_backward_scratch_bytes.argtypes = [i64, i32]
+                l.htgs_add_rms_norm_backward.argtypes = [pointer, i64, pointer, i64, pointer, i64, pointer, pointer, i32, i64, i32, pointer, i64, pointer,
+                                                         pointer, ctypes.c_size_t, pointer]
+                l.htgs_quantize_fp8.argtypes = [pointer, i64, i32, i64, i64, i32] + [pointer, i64] * 4 + [pointer]
+                l.htgs_dequantize_fp8.argtypes = [ctypes.POINTER(HtgsFp8Matrix), pointer, i64, i32, pointer]
+                l.htgs_fp8_matmul.argtypes = [ctypes.POINTER(HtgsFp8Matrix)] * 2 + [pointer, i64, i32, pointer]
+                l.htgs_gated_scan_state_bytes.restype = ctypes.c_size_t
+                l.htgs_gated_scan_state_bytes.argtypes = [i64, i32]
+                l.htgs_gated_scan_workspace_bytes.restype = ctypes.c_size_t
+                l.htgs_gated_scan_workspace_bytes.argtypes = [i64, i32]
+                l.htgs_gated_scan.argtypes = [ctypes.POINTER(HtgsScan), pointer, i64, pointer, pointer, pointer, ctypes.c_size_t, pointer]
+                l.htgs_gated_scan_backward.argtypes = [ctypes.POINTER(HtgsScan), pointer, pointer, i64, pointer, pointer, i64, pointer, i64, pointer, pointer,
+                                                       ctypes.c_size_t, pointer]
+                l.htgs_gated_scan_step.argtypes = [pointer, i64, pointer, i64, pointer, i64, pointer, i64, i32, i64, i32, pointer]
                 l.htgs_set_profiling.argtypes = [ctypes.c_void_p, ctypes.c_int]
                 l.htgs_set_collect_stats.argtypes = [ctypes.c_void_p, ctypes.c_int]
                 l.htgs_set_fast_deterministic.argtypes = [ctypes.c_void_p, ctypes.c_int]

@@ -1,0 +1,341 @@
+// Root-mean-square norm of a residual stream, with the residual's addition, forward and backward, and with an 8-bit output.
+//
+//   u = x + residual;   rho = 1 / sqrt(mean(u^2) + eps);   y = u * rho * weight;   sum = u in the stream's type
+//   backward, with unit = u * rho and z = weight * grad_y:
+//       grad_x = grad_residual = rho * (z - unit * mean(z * unit)) + grad_sum;      grad_weight = sum over rows of grad_y * unit
+//
+// A row stays in registers between its statistics and its output, so every value crosses HBM once: read x and residual, write sum
+// and y (or 8-bit codes and a scale byte for each 128 columns); backward read grad_y, grad_sum and sum, write one gradient that
+// serves x and residual alike.  Bound by HBM.  A warp holds a row of up to 1024 columns (32 values a lane), eight warps a wider one.
+// Sums are 32-bit; y is computed from the unrounded u, the backward pass from the stream's rounded one, which is what is kept.
+#include "sequence.cuh"
+
+namespace htgs {
+
+namespace {
+
+constexpr int kNormBlock = 256;
+constexpr int kNormWarps = kNormBlock / 32;
+constexpr int kNormBackwardBlocks = 148 * 2;       // persistent: two blocks per SM, each with one partial sum of grad_weight
+constexpr int kMaxNormWidth = kNormBlock * 32;
+
+struct NormArgs {
+    const void* x; const void* residual; const void* weight;
+    int64_t x_stride, residual_stride;
+    void* y; void* sum; float* rstd; uint8_t* codes; uint8_t* scales;
+    int64_t y_stride, sum_stride, codes_stride, scales_stride;
+    int64_t rows;
+    int32_t width;
+    float eps;
+};
+
+struct NormBackwardArgs {
+    const void* grad_y; const void* grad_sum; const void* sum; const void* weight; const float* rstd;
+    int64_t grad_y_stride, grad_sum_stride, sum_stride, grad_x_stride;
+    void* grad_x; float* partial;
+    int64_t rows;
+    int32_t width;
+};
+
+// Sum over the WPR warps that share a row.
+template <int WPR> __device__ __forceinline__ float row_sum(float v, float* shared) {
+    v = warp_sum(v);
+    if (WPR == 1) return v;
+    __syncthreads();                    // the previous use of `shared` is over
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float total = 0.0f;
+    #pragma unroll
+    for (int w = 0; w < WPR; ++w) total += shared[w];
+    return total;
+}
+
+// E values a lane, in groups of VEC side by side; group j of a warp starts at column (32 * j + lane) * VEC of the warp's 32 * E, so
+// that a block of 128 columns is held by 16 or 32 lanes of one group (VEC 8, 4) or by four groups (VEC 1) of one warp.
+template <typename T, int VEC, int E, int WPR, bool FP8>
+__global__ void __launch_bounds__(kNormBlock) norm_kernel(const NormArgs a) {
+    __shared__ float shared[kNormWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = int64_t(blockIdx.x) * (kNormWarps / WPR) + (WPR == 1 ? warp : 0);
+    if (row >= a.rows) return;          // whole warps where WPR is 1, never where it is 8
+    const int base = WPR == 1 ? 0 : warp * 32 * E;
+    constexpr int G = E / VEC;
+    float u[G][VEC];
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* residual = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+    float squares = 0.0f;
+    #pragma unroll
+    for (int j = 0; j < G; ++j) {
+        const int column = base + (32 * j + lane) * VEC;
+        if (column < a.width) load_floats<T, VEC>(x + column, u[j]);
+        else {
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) u[j][i] = 0.0f;
+        }
+    }
+    if (residual) {
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int column = base + (32 * j + lane) * VEC;
+            if (column >= a.width) continue;
+            float r[VEC];
+            load_floats<T, VEC>(residual + column, r);
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) u[j][i] += r[i];
+        }
+    }
+    #pragma unroll
+    for (int j = 0; j < G; ++j) {
+        #pragma unroll
+        for (int i = 0; i < VEC; ++i) squares += u[j][i] * u[j][i];
+    }
+    const float rho = rsqrtf(row_sum<WPR>(squares, shared) / float(a.width) + a.eps);
+    if (a.rstd && threadIdx.x % (32 * WPR) == 0) a.rstd[row] = rho;
+    T* sum = a.sum ? static_cast<T*>(a.sum) + row * a.sum_stride : nullptr;
+    const T* weight = static_cast<const T*>(a.weight);
+    #pragma unroll
+    for (int j = 0; j < G; ++j) {
+        const int column = base + (32 * j + lane) * VEC;
+        if (column < a.width) {
+            if (sum) store_floats<T, VEC>(sum + column, u[j]);
+            float w[VEC];
+            load_floats<T, VEC>(weight + column, w);
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) u[j][i] = u[j][i] * rho * w[i];
+            if (!FP8) store_floats<T, VEC>(static_cast<T*>(a.y) + row * a.y_stride + column, u[j]);
+        }
+    }
+    if (FP8) {
+        uint8_t* codes = a.codes + row * a.codes_stride;
+        uint8_t* scales = a.scales + row * a.scales_stride;
+        constexpr int kGroups = VEC == 1 ? 4 : 1;                    // groups in a block of 128 columns
+        constexpr int kLanes = VEC == 8 ? 16 : 32;                   // lanes
+        #pragma unroll
+        for (int j = 0; j < G; j += kGroups) {
+            float largest = 0.0f;
+            #pragma unroll
+            for (int k = 0; k < kGroups; ++k) {
+                #pragma unroll
+                for (int i = 0; i < VEC; ++i) largest = fmaxf(largest, finite_magnitude(u[j + k][i]));
+            }
+            const int e = scale_exponent(lanes_max<kLanes>(largest));
+            const float inverse = inverse_scale(e);
+            #pragma unroll
+            for (int k = 0; k < kGroups; ++k) {
+                const int column = base + (32 * (j + k) + lane) * VEC;
+                if (column >= a.width) continue;
+                const float* v = u[j + k];
+                if (VEC == 8)
+                    *reinterpret_cast<uint2*>(codes + column) = make_uint2(encode4(v[0], v[1 % VEC], v[2 % VEC], v[3 % VEC], inverse),
+                                                                           encode4(v[4 % VEC], v[5 % VEC], v[6 % VEC], v[7 % VEC], inverse));
+                else if (VEC == 4)
+                    *reinterpret_cast<uint32_t*>(codes + column) = encode4(v[0], v[1 % VEC], v[2 % VEC], v[3 % VEC], inverse);
+                else
+                    codes[column] = uint8_t(encode2(v[0], 0.0f, inverse) & 0xffu);
+                if (k == 0 && lane % kLanes == 0) scales[column / kScaleBlock] = uint8_t(e + 127);
+            }
+        }
+    }
+}
+
+template <typename T, int VEC, int E, int WPR>
+__global__ void __launch_bounds__(kNormBlock) norm_backward_kernel(const NormBackwardArgs a) {
+    __shared__ float shared[WPR == 1 ? kNormWarps * 32 * E : kNormWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int G = E / VEC;
+    constexpr int kRows = kNormWarps / WPR;
+    const int base = WPR == 1 ? 0 : warp * 32 * E;
+    const T* weight = static_cast<const T*>(a.weight);
+    float grad_weight[G][VEC] = {};
+    for (int64_t row = int64_t(blockIdx.x) * kRows + (WPR == 1 ? warp : 0); row < a.rows; row += int64_t(gridDim.x) * kRows) {
+        const T* grad_y = static_cast<const T*>(a.grad_y) + row * a.grad_y_stride;
+        const T* sum = static_cast<const T*>(a.sum) + row * a.sum_stride;
+        const T* grad_sum = a.grad_sum ? static_cast<const T*>(a.grad_sum) + row * a.grad_sum_stride : nullptr;
+        Pack<T, VEC> g[G], u[G], d[G];          // as they are in memory: half the registers of 32-bit values
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int column = base + (32 * j + lane) * VEC;
+            if (column < a.width) {
+                g[j] = *reinterpret_cast<const Pack<T, VEC>*>(grad_y + column);
+                u[j] = *reinterpret_cast<const Pack<T, VEC>*>(sum + column);
+                if (grad_sum) d[j] = *reinterpret_cast<const Pack<T, VEC>*>(grad_sum + column);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < VEC; ++i) g[j].v[i] = u[j].v[i] = from_float<T>(0.0f);
+            }
+        }
+        const float rho = a.rstd[row];
+        float dot = 0.0f;
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int column = base + (32 * j + lane) * VEC;
+            float w[VEC] = {};
+            if (column < a.width) load_floats<T, VEC>(weight + column, w);
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float gy = to_float<T>(g[j].v[i]), unit = to_float<T>(u[j].v[i]) * rho;
+                grad_weight[j][i] += gy * unit;
+                dot += gy * w[i] * unit;
+            }
+        }
+        const float mean = row_sum<WPR>(dot, shared) / float(a.width);
+        T* grad_x = static_cast<T*>(a.grad_x) + row * a.grad_x_stride;
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int column = base + (32 * j + lane) * VEC;
+            if (column >= a.width) continue;
+            float w[VEC], out[VEC];
+            load_floats<T, VEC>(weight + column, w);
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                out[i] = rho * (to_float<T>(g[j].v[i]) * w[i] - to_float<T>(u[j].v[i]) * rho * mean);
+                if (grad_sum) out[i] += to_float<T>(d[j].v[i]);
+            }
+            store_floats<T, VEC>(grad_x + column, out);
+        }
+    }
+    float* partial = a.partial + int64_t(blockIdx.x) * a.width;
+    if (WPR == 1) {
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) shared[warp * 32 * E + (32 * j + lane) * VEC + i] = grad_weight[j][i];
+        }
+        __syncthreads();
+        for (int column = threadIdx.x; column < min(a.width, 32 * E); column += kNormBlock) {
+            float total = 0.0f;
+            #pragma unroll
+            for (int w = 0; w < kNormWarps; ++w) total += shared[w * 32 * E + column];
+            partial[column] = total;
+        }
+    } else {
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int column = base + (32 * j + lane) * VEC;
+            if (column >= a.width) continue;
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) partial[column + i] = grad_weight[j][i];
+        }
+    }
+}
+
+// Sums the blocks' partial gradients of the weight, always in the same order.  32 columns by 8 slices of the blocks.
+template <typename T> __global__ void __launch_bounds__(kNormBlock) norm_weight_kernel(const float* partial, int blocks, int width, T* grad_weight) {
+    __shared__ float shared[kNormWarps][32];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, column = blockIdx.x * 32 + lane;
+    float total = 0.0f;
+    if (column < width)
+        for (int b = slice; b < blocks; b += kNormWarps) total += partial[int64_t(b) * width + column];
+    shared[slice][lane] = total;
+    __syncthreads();
+    if (slice == 0 && column < width) {
+        total = 0.0f;
+        #pragma unroll
+        for (int s = 0; s < kNormWarps; ++s) total += shared[s][lane];
+        grad_weight[column] = from_float<T>(total);
+    }
+}
+
+int backward_blocks(int64_t rows, int width) {
+    const int64_t rows_per_block = width <= 32 * 32 ? kNormWarps : 1;
+    const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
+    return int(blocks < kNormBackwardBlocks ? blocks : kNormBackwardBlocks);
+}
+
+template <typename T, int VEC, int E, int WPR> void launch_norm(const NormArgs& a, cudaStream_t stream) {
+    const unsigned int blocks = unsigned((a.rows + kNormWarps / WPR - 1) / (kNormWarps / WPR));
+    if (a.codes) norm_kernel<T, VEC, E, WPR, true><<<blocks, kNormBlock, 0, stream>>>(a);
+    else norm_kernel<T, VEC, E, WPR, false><<<blocks, kNormBlock, 0, stream>>>(a);
+}
+template <typename T, int VEC, int E, int WPR> void launch_backward(const NormBackwardArgs& a, cudaStream_t stream) {
+    norm_backward_kernel<T, VEC, E, WPR><<<backward_blocks(a.rows, a.width), kNormBlock, 0, stream>>>(a);
+}
+
+// The fewest values a lane that hold a row: one warp up to 1024 columns, then eight.
+#define HTGS_NORM_WIDTHS(launch, args)                                                              \
+    do {                                                                                            \
+        if (args.width <= 32 * 8) launch<T, VEC, 8, 1>(args, stream);                               \
+        else if (args.width <= 32 * 16) launch<T, VEC, 16, 1>(args, stream);                        \
+        else if (args.width <= 32 * 32) launch<T, VEC, 32, 1>(args, stream);                        \
+        else if (args.width <= 256 * 8) launch<T, VEC, 8, 8>(args, stream);                         \
+        else if (args.width <= 256 * 16) launch<T, VEC, 16, 8>(args, stream);                       \
+        else launch<T, VEC, 32, 8>(args, stream);                                                   \
+    } while (0)
+
+template <typename T, int VEC> void norm_widths(const NormArgs& a, cudaStream_t stream) { HTGS_NORM_WIDTHS(launch_norm, a); }
+template <typename T, int VEC> void backward_widths(const NormBackwardArgs& a, cudaStream_t stream) { HTGS_NORM_WIDTHS(launch_backward, a); }
+
+// 16-byte groups where every row of every tensor allows them, single values otherwise.
+template <typename T> void norm_typed(const NormArgs& a, cudaStream_t stream) {
+    constexpr int V = 16 / int(sizeof(T));
+    const size_t e = sizeof(T);
+    const bool wide = a.width % V == 0 && rows_aligned(a.x, a.x_stride, a.rows, e, 16) && rows_aligned(a.residual, a.residual_stride, a.rows, e, 16) &&
+                      aligned(a.weight, 16) && rows_aligned(a.y, a.y_stride, a.rows, e, 16) && rows_aligned(a.sum, a.sum_stride, a.rows, e, 16) &&
+                      rows_aligned(a.codes, a.codes_stride, a.rows, 1, 8);
+    if (wide) norm_widths<T, V>(a, stream); else norm_widths<T, 1>(a, stream);
+}
+template <typename T> void backward_typed(const NormBackwardArgs& a, void* grad_weight, cudaStream_t stream) {
+    constexpr int V = 16 / int(sizeof(T));
+    const size_t e = sizeof(T);
+    const bool wide = a.width % V == 0 && rows_aligned(a.grad_y, a.grad_y_stride, a.rows, e, 16) && rows_aligned(a.grad_sum, a.grad_sum_stride, a.rows, e, 16) &&
+                      rows_aligned(a.sum, a.sum_stride, a.rows, e, 16) && aligned(a.weight, 16) && rows_aligned(a.grad_x, a.grad_x_stride, a.rows, e, 16);
+    if (wide) backward_widths<T, V>(a, stream); else backward_widths<T, 1>(a, stream);
+    norm_weight_kernel<T><<<(a.width + 31) / 32, kNormBlock, 0, stream>>>(a.partial, backward_blocks(a.rows, a.width), a.width, static_cast<T*>(grad_weight));
+}
+
+}  // namespace
+
+}  // namespace htgs
+
+extern "C" {
+
+int htgs_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int type, int64_t rows,
+                      int32_t width, float eps, void* y, int64_t y_stride, void* sum, int64_t sum_stride, float* rstd, uint8_t* codes,
+                      int64_t codes_stride, uint8_t* scales, int64_t scales_stride, void* stream) {
+    using namespace htgs;
+    if (!known_type(type)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm: unknown element type");
+    if (rows < 0 || rows > 0x7fffffff || width < 1 || width > kMaxNormWidth)
+        return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm: rows must be in [0, 2^31), width in [1, 8192]");
+    if (!(eps >= 0.0f)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm: eps must be >= 0");
+    if (rows == 0) return HTGS_OK;
+    if (!x || !weight || (y != nullptr) == (codes != nullptr) || (codes != nullptr) != (scales != nullptr))
+        return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm: x, weight and either y or codes with scales must be given");
+    const NormArgs a{x, residual, weight, x_stride, residual_stride, y, sum, rstd, codes, scales, y_stride, sum_stride, codes_stride, scales_stride,
+                     rows, width, eps};
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (type == HTGS_FLOAT32) norm_typed<float>(a, s);
+    else if (type == HTGS_FLOAT16) norm_typed<__half>(a, s);
+    else norm_typed<__nv_bfloat16>(a, s);
+    return sequence_status("htgs_add_rms_norm");
+}
+
+size_t htgs_add_rms_norm_backward_scratch_bytes(int64_t rows, int32_t width) {
+    if (rows <= 0 || width <= 0) return 0;
+    return size_t(htgs::backward_blocks(rows, width)) * size_t(width) * sizeof(float);
+}
+
+int htgs_add_rms_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride, const void* sum,
+                               int64_t sum_stride, const void* weight, const float* rstd, int type, int64_t rows, int32_t width, void* grad_x,
+                               int64_t grad_x_stride, void* grad_weight, void* scratch, size_t scratch_bytes, void* stream) {
+    using namespace htgs;
+    if (!known_type(type)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm_backward: unknown element type");
+    if (rows < 0 || rows > 0x7fffffff || width < 1 || width > kMaxNormWidth)
+        return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm_backward: rows must be in [0, 2^31), width in [1, 8192]");
+    if (!grad_weight) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm_backward: grad_weight must not be null");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        const cudaError_t err = cudaMemsetAsync(grad_weight, 0, size_t(width) * type_bytes(type), s);
+        return err == cudaSuccess ? HTGS_OK : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+    }
+    if (!grad_y || !sum || !weight || !rstd || !grad_x) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm_backward: null pointer");
+    if (!scratch || !aligned(scratch, 16) || scratch_bytes < htgs_add_rms_norm_backward_scratch_bytes(rows, width))
+        return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_add_rms_norm_backward: scratch too small or not 16-byte aligned");
+    const NormBackwardArgs a{grad_y, grad_sum, sum, weight, rstd, grad_y_stride, grad_sum_stride, sum_stride, grad_x_stride, grad_x,
+                             static_cast<float*>(scratch), rows, width};
+    if (type == HTGS_FLOAT32) backward_typed<float>(a, grad_weight, s);
+    else if (type == HTGS_FLOAT16) backward_typed<__half>(a, grad_weight, s);
+    else backward_typed<__nv_bfloat16>(a, grad_weight, s);
+    return sequence_status("htgs_add_rms_norm_backward");
+}
+
+}  // extern "C"

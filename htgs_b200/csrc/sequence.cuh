@@ -1,0 +1,96 @@
+// Shared by the sequence operators (norm.cu, fp8.cu, fp8_matmul.cu, scan.cu): element types, vector loads and stores, and the 8-bit
+// format: blocks of 128 columns (of 1 or 128 rows) share a scale, a power of two kept as the byte e + 127 (E8M0), and hold codes of
+// type E4M3.  With a power of two nothing is rounded by the scale, neither when it is taken out nor when it is put back.
+#pragma once
+
+#include "kernels.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+namespace htgs {
+
+constexpr int kScaleBlock = 128;      // columns (and, for weights, rows) that share a scale
+
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N elements side by side, moved by one load or store (N * sizeof(T) is 2, 4, 8 or 16 bytes, and the address a multiple of that).
+template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T v[N]; };
+template <typename T, int N> __device__ __forceinline__ void load_floats(const T* p, float (&out)[N]) {
+    const Pack<T, N> pack = *reinterpret_cast<const Pack<T, N>*>(p);
+    #pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = to_float<T>(pack.v[i]);
+}
+template <typename T, int N> __device__ __forceinline__ void store_floats(T* p, const float (&in)[N]) {
+    Pack<T, N> pack;
+    #pragma unroll
+    for (int i = 0; i < N; ++i) pack.v[i] = from_float<T>(in[i]);
+    *reinterpret_cast<Pack<T, N>*>(p) = pack;
+}
+
+// Magnitude that counts for a block's scale: infinities and NaN do not, their codes are NaN whatever the scale.
+__device__ __forceinline__ float finite_magnitude(float v) { const float m = fabsf(v); return m <= FLT_MAX ? m : 0.0f; }
+
+// Least e in [-127, 120] with largest <= 448 * 2^e (448 = 1.75 * 2^8 is the largest finite E4M3 value); 0 for a block of zeros.
+__device__ __forceinline__ int scale_exponent(float largest) {
+    if (largest == 0.0f) return 0;
+    const uint32_t bits = __float_as_uint(largest);
+    const int e = int(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return max(e, -127);
+}
+__device__ __forceinline__ float inverse_scale(int e) { return __uint_as_float(uint32_t(127 - e) << 23); }      // 2^-e
+__device__ __forceinline__ float scale_value(uint32_t byte) {                                                     // 2^(byte - 127); 255 is NaN
+    return byte == 255u ? __uint_as_float(0x7fffffffu) : byte == 0u ? __uint_as_float(0x400000u) : __uint_as_float(byte << 23);
+}
+
+// Two codes in one: v * 2^-e to the nearest E4M3 value, ties to even; what is not finite becomes NaN.
+__device__ __forceinline__ uint32_t encode2(float lo, float hi, float inverse) {
+    lo = fabsf(lo) <= FLT_MAX ? lo * inverse : __uint_as_float(0x7fffffffu);
+    hi = fabsf(hi) <= FLT_MAX ? hi * inverse : __uint_as_float(0x7fffffffu);
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inverse) {
+    return encode2(a, b, inverse) | encode2(c, d, inverse) << 16;
+}
+__device__ __forceinline__ float2 decode2(uint32_t codes) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3);
+    return __half22float2(__half2(h));
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+template <int LANES> __device__ __forceinline__ float lanes_max(float v) {
+    #pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+}
+
+// ---- host side of the entry points ----------------------------------------------------------------------------------------
+
+inline int sequence_fail(int code, const char* message) { set_last_error(message); return code; }
+inline int sequence_status(const char* what) {
+    const cudaError_t err = cudaGetLastError();
+    if (err == cudaSuccess) return HTGS_OK;
+    (void)what;
+    return sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
+inline bool known_type(int type) { return type == HTGS_FLOAT32 || type == HTGS_FLOAT16 || type == HTGS_BFLOAT16; }
+inline size_t type_bytes(int type) { return type == HTGS_FLOAT32 ? 4 : 2; }
+inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// A row-major matrix whose rows all begin on a multiple of `bytes`.
+inline bool rows_aligned(const void* p, int64_t stride, int64_t rows, size_t element, size_t bytes) {
+    return aligned(p, bytes) && (rows <= 1 || (uint64_t(stride) * element) % bytes == 0);
+}
+
+}  // namespace htgs

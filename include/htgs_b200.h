@@ -440,6 +440,80 @@ int htgs_activate_backward(const float* raw_scales, const float* raw_rotations, 
                            const float* grad_scales, const float* grad_rotations, const float* grad_opacities, float* grad_raw_scales,
                            float* grad_raw_rotations, float* grad_raw_opacities, int32_t n_primitives, void* stream);
 
+/*
+ * Operators for networks over sequences of Gaussians (no counterpart in the reference): what reads or refines a scene's Gaussians, one
+ * row each in the order of a space-filling curve.  All are stream-ordered without host synchronisation, take no context, allocate
+ * nothing, and give the same bits for the same inputs.  Matrices are row-major with a stride in elements (codes and scales: bytes) from row to row; `type` is an
+ * HtgsElementType.  Sums, statistics and states are 32-bit whatever the type.
+ */
+enum HtgsElementType { HTGS_FLOAT32 = 0, HTGS_FLOAT16 = 1, HTGS_BFLOAT16 = 2 };
+
+/*
+ * Root-mean-square norm of x + residual (residual may be NULL):
+ *   u = x + residual;  rho = 1 / sqrt(mean(u^2) + eps);  y = u * rho * weight;  sum = u in the stream's type.
+ * Either y, or codes and scales (the 8-bit format below, one scale per row and 128 columns; rows of codes begin on 8 bytes for the
+ * fast path) must be given.  sum [rows, width] and rstd [rows] (rho) may be NULL; the backward pass needs both.  1 <= width <= 8192.
+ * The backward pass takes grad_sum == NULL for zeros; grad_x is the gradient of x and of residual; scratch as the size function says, 16-byte aligned.
+ */
+int htgs_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int type, int64_t rows,
+                      int32_t width, float eps, void* y, int64_t y_stride, void* sum, int64_t sum_stride, float* rstd, uint8_t* codes,
+                      int64_t codes_stride, uint8_t* scales, int64_t scales_stride, void* stream);
+size_t htgs_add_rms_norm_backward_scratch_bytes(int64_t rows, int32_t width);
+int htgs_add_rms_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride, const void* sum,
+                               int64_t sum_stride, const void* weight, const float* rstd, int type, int64_t rows, int32_t width, void* grad_x,
+                               int64_t grad_x_stride, void* grad_weight, void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * 8-bit matrices: codes [rows, width] of type E4M3, and one power-of-two scale, the byte e + 127 (E8M0), for each block of 128 columns and
+ * rows_per_scale rows (1 or 128): scales [ceil(rows / rows_per_scale), ceil(width / 128)].  A block's scale is the least 2^e with
+ * |v| <= 448 * 2^e for its finite values (2^-127 at least; 1 for zeros); a code is v * 2^-e rounded to nearest even; infinities and NaN become NaN.
+ * `htgs_quantize_fp8` writes the matrix as it lies (codes, scales), its transpose (codes_t [width, rows], scales_t), or both from one read.
+ */
+typedef struct HtgsFp8Matrix {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    int64_t rows, width, codes_stride, scales_stride;
+    int32_t rows_per_scale;
+} HtgsFp8Matrix;
+int htgs_quantize_fp8(const void* x, int64_t x_stride, int type, int64_t rows, int64_t width, int rows_per_scale, uint8_t* codes, int64_t codes_stride,
+                      uint8_t* scales, int64_t scales_stride, uint8_t* codes_t, int64_t codes_t_stride, uint8_t* scales_t, int64_t scales_t_stride,
+                      void* stream);
+int htgs_dequantize_fp8(const HtgsFp8Matrix* matrix, void* out, int64_t out_stride, int out_type, void* stream);
+
+/*
+ * out [a.rows, b.rows] = a * b^T, products of codes and scales summed in 32 bits and rounded once.  a.width == b.width; codes begin on 16 bytes
+ * and have a stride that is a multiple of 16; scales begin on 4 bytes with a stride that is a multiple of 4.
+ */
+int htgs_fp8_matmul(const HtgsFp8Matrix* a, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream);
+
+/*
+ * Gated linear recurrence along the rows, per channel:
+ *   a = 1 / (1 + exp(-gate));  h_t = a_t h_{t-1} + (1 - a_t) x_t,
+ * for n_sequences sequences that lie one behind the other: of rows / n_sequences rows each (offsets == NULL), or from row
+ * offsets[s] to offsets[s + 1] (device memory, n_sequences + 1 ascending numbers from 0 to rows; sequences may be empty).
+ * initial [n_sequences, width] is the state in front of each sequence (NULL: zeros), last [n_sequences, width] the one behind it (that of an
+ * empty sequence is its initial state).  reverse != 0 goes through each sequence from its last row to its first.
+ * states (htgs_gated_scan_state_bytes) keeps what the backward pass needs and may be NULL where there is none.
+ * The backward pass takes grad_last == NULL for zeros; grad_initial may be NULL.  1 <= width <= 65536.
+ * htgs_gated_scan_step does one step for each row and updates state [rows, width] in place.
+ */
+typedef struct HtgsScan {
+    const void* x;
+    const void* gate;
+    const float* initial;
+    const int32_t* offsets;
+    int64_t x_stride, gate_stride, rows;
+    int32_t width, n_sequences, type, reverse;
+} HtgsScan;
+size_t htgs_gated_scan_state_bytes(int64_t rows, int32_t width);
+size_t htgs_gated_scan_workspace_bytes(int64_t rows, int32_t width);
+int htgs_gated_scan(const HtgsScan* scan, void* h, int64_t h_stride, float* last, float* states, void* workspace, size_t workspace_bytes, void* stream);
+int htgs_gated_scan_backward(const HtgsScan* scan, const float* states, const void* grad_h, int64_t grad_h_stride, const float* grad_last, void* grad_x,
+                             int64_t grad_x_stride, void* grad_gate, int64_t grad_gate_stride, float* grad_initial, void* workspace, size_t workspace_bytes,
+                             void* stream);
+int htgs_gated_scan_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride, float* state, int64_t state_stride, void* h,
+                         int64_t h_stride, int type, int64_t rows, int32_t width, void* stream);
+
 /* Measurement aids (off by default; they do not change results).
  * Profiling: CUDA events are recorded on the frame's stream between the stages; after the call
  * htgs_get_stage_ms fills out_ms[0..HTGS_N_STAGES) with the device time of each stage in ms.
