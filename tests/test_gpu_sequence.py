@@ -215,6 +215,18 @@ def test_product(kind, rows, out, width):
     near(seq.fp8_matmul(seq.quantize_fp8(x, 128), wq, torch.float32), *product_bound(ref.dequantize(*ref.quantize(f64(x), 128), 128), b, "fp32"), "block scales")
 
 
+@pytest.mark.parametrize("rows,out,width", [(2500, 2301, 640), (40_001, 200, 129), (385, 4100, 1030)])
+def test_product_of_many_tiles(rows, out, width):
+    """More tiles than SMs, so that each block computes several; sizes that leave the last tiles ragged."""
+    import torch
+    from htgs_b200 import sequence as seq
+    x, w = draw((rows, width), 3, "bf16"), draw((out, width), 4, "bf16", width ** -0.5)
+    y = seq.fp8_matmul(x, seq.quantize_fp8(w, 128))
+    a, b = ref.dequantize(*ref.quantize(f64(x))), ref.dequantize(*ref.quantize(f64(w), 128), 128)
+    near(y, *product_bound(a, b, "bf16"))
+    assert torch.equal(y, seq.fp8_matmul(x, seq.quantize_fp8(w, 128)))
+
+
 def test_product_of_views_strides_and_empty_matrices():
     import torch
     from htgs_b200 import sequence as seq
