@@ -168,17 +168,6 @@ __device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uin
                  ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(scale_a), "r"(scale_b), "r"(uint32_t(add)) : "memory");
 }
 
-__device__ __forceinline__ float peer_float(uint32_t address, uint32_t block) {       // of the cluster's block `block`, at this block's shared address
-    uint32_t there;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(block));
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-    return v;
-}
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // One row's 32 columns, rounded and stored.
 template <typename T> __device__ __forceinline__ void store_row(T* row, int column, int columns, const uint32_t (&v)[32], bool wide) {
     constexpr int V = 16 / int(sizeof(T));

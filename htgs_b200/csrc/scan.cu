@@ -34,10 +34,58 @@ struct ScanArgs {
     float* grad_states;                      // [chunks, width] E behind each chunk; that of the last is not kept
 };
 
-struct Gate { float a, rest; };              // a and 1 - a
-// exp(80) is far from the end of the range, and a below 2e-35 tells nothing from zero.
-__device__ __forceinline__ float gate_exp(float g) { return __expf(g < -80.0f ? 80.0f : -g); }
-__device__ __forceinline__ Gate gate_of(float t) { const float a = __fdividef(1.0f, 1.0f + t); return {a, t * a}; }
+// V channels side by side: one float, or two in a register pair (one instruction for both).
+template <int V> struct Num;
+template <> struct Num<1> {
+    float v;
+    __device__ __forceinline__ static Num make(const float (&f)[1]) { return {f[0]}; }
+    __device__ __forceinline__ static Num all(float f) { return {f}; }
+    __device__ __forceinline__ float operator[](int) const { return v; }
+};
+template <> struct Num<2> {
+    f32x2 v;
+    __device__ __forceinline__ static Num make(const float (&f)[2]) { return {pack2(f[0], f[1])}; }
+    __device__ __forceinline__ static Num all(float f) { return {pack2(f, f)}; }
+    __device__ __forceinline__ float operator[](int i) const { const float2 f = unpack2(v); return i ? f.y : f.x; }
+};
+__device__ __forceinline__ Num<1> operator*(Num<1> a, Num<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Num<1> operator+(Num<1> a, Num<1> b) { return {a.v + b.v}; }
+__device__ __forceinline__ Num<1> madd(Num<1> a, Num<1> b, Num<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Num<2> operator*(Num<2> a, Num<2> b) { return {mul2(a.v, b.v)}; }
+__device__ __forceinline__ Num<2> operator+(Num<2> a, Num<2> b) { return {add2(a.v, b.v)}; }
+__device__ __forceinline__ Num<2> madd(Num<2> a, Num<2> b, Num<2> c) { return {fma2(a.v, b.v, c.v)}; }
+
+// exp(-g), from the hardware's 2^x (2 units); above exp(80), where a < 2e-35 tells nothing from zero, it stays; a NaN stays one.
+__device__ __forceinline__ float exp_negated(float scaled) {        // scaled = -g / ln 2
+    float t;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(scaled), "f"(115.4f));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t));
+    return t;
+}
+__device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+template <int V> __device__ __forceinline__ Num<V> gate_exp(Num<V> g) {
+    const Num<V> scaled = g * Num<V>::all(-1.4426950408889634f);
+    float t[V];
+    #pragma unroll
+    for (int k = 0; k < V; ++k) t[k] = exp_negated(scaled[k]);
+    return Num<V>::make(t);
+}
+template <int V> struct Gate { Num<V> a, rest; };                    // a and 1 - a
+template <int V> __device__ __forceinline__ Gate<V> gate_of(Num<V> t) {
+    const Num<V> sum = t + Num<V>::all(1.0f);
+    float a[V];
+    #pragma unroll
+    for (int k = 0; k < V; ++k) a[k] = rcp_approx(sum[k]);
+    const Num<V> A = Num<V>::make(a);
+    return {A, t * A};
+}
+template <typename T, int V> __device__ __forceinline__ Num<V> number(const Pack<T, V>& p) { float f[V]; to_floats<T, V>(p, f); return Num<V>::make(f); }
+template <typename T, int V> __device__ __forceinline__ void store_number(T* p, Num<V> n) {
+    float f[V];
+    #pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = n[k];
+    store_floats<T, V>(p, f);
+}
 
 // The map of a sequence's first step takes nothing from the state in front of it: A is -0, which no product of gates is.
 constexpr float kCut = -0.0f;
@@ -46,6 +94,16 @@ __device__ __forceinline__ float follow(float2 m, float state) { return is_cut(m
 __device__ __forceinline__ void compose(float& A, float& H, float2 next) {
     H = follow(next, H);
     A = is_cut(next.x) ? next.x : A * next.x;
+}
+template <int V> __device__ __forceinline__ Num<V> follow(const float2* maps, Num<V> state) {
+    float f[V];
+    #pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = follow(maps[k], state[k]);
+    return Num<V>::make(f);
+}
+template <int V> __device__ __forceinline__ void leave_map(float2* to, Num<V> A, Num<V> H) {
+    #pragma unroll
+    for (int k = 0; k < V; ++k) to[k] = make_float2(A[k], H[k]);
 }
 
 // Which of the warp's `STEPS` steps are the first or last of their sequence (bits), and in lane i the sequence of step i.
@@ -64,6 +122,8 @@ template <int STEPS> __device__ __forceinline__ Edges find_edges(const HtgsScan&
                 if (__ldg(in.offsets + mid) <= row) s = mid; else hi = mid;
             }
             begin = __ldg(in.offsets + s); end = __ldg(in.offsets + s + 1);
+        } else if (in.n_sequences == 1) {
+            begin = 0; end = in.rows;
         } else {
             const int64_t length = in.rows / in.n_sequences;
             s = int(row / length);
@@ -75,15 +135,22 @@ template <int STEPS> __device__ __forceinline__ Edges find_edges(const HtgsScan&
     return {__ballot_sync(0xffffffffu, first), __ballot_sync(0xffffffffu, last), s};
 }
 
-template <int V> __device__ __forceinline__ void load_state(const float* states, int64_t at, float (&v)[V]) {
+template <int V> __device__ __forceinline__ Num<V> load_state(const float* states, int64_t at) {
+    float f[V];
     #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = states ? states[at + k] : 0.0f;
+    for (int k = 0; k < V; ++k) f[k] = states ? states[at + k] : 0.0f;
+    return Num<V>::make(f);
+}
+template <int V> __device__ __forceinline__ void store_state(float* states, int64_t at, Num<V> n) {
+    #pragma unroll
+    for (int k = 0; k < V; ++k) states[at + k] = n[k];
 }
 
-// Where a thread works: V channels side by side, STEPS rows.
+// Where a thread works: V channels side by side, STEPS rows from p0 on, `count` of which exist; row r of them is r * step rows behind the first.
 template <int V, int STEPS> struct Place {
-    int lane, warp, channel;
-    int64_t chunk, p0;
+    int lane, warp, channel, count;
+    int64_t chunk, p0, row0;
+    int step;
     bool inside;
     __device__ __forceinline__ explicit Place(const ScanArgs& a) {
         lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
@@ -91,110 +158,124 @@ template <int V, int STEPS> struct Place {
         channel = (int(blockIdx.x % unsigned(a.channel_tiles)) * 32 + lane) * V;
         inside = channel < a.in.width;
         p0 = chunk * kChunk + warp * STEPS;
+        count = int(max(int64_t(0), min(int64_t(STEPS), a.in.rows - p0)));
+        row0 = a.in.reverse ? a.in.rows - 1 - p0 : p0;
+        step = a.in.reverse ? -1 : 1;
     }
+    __device__ __forceinline__ int64_t state_at(const ScanArgs& a, int sequence) const { return int64_t(sequence) * a.in.width + channel; }
 };
 
 template <typename T, int V, int STEPS>
-__device__ __forceinline__ void load_rows(const void* base, int64_t stride, const HtgsScan& in, int64_t p0, int channel, bool inside, Pack<T, V> (&out)[STEPS]) {
-    #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const int64_t p = p0 + i;
-        if (inside && p < in.rows) {
-            const int64_t row = in.reverse ? in.rows - 1 - p : p;
-            out[i] = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(base) + row * stride + channel);
-        } else {
-            #pragma unroll
-            for (int k = 0; k < V; ++k) out[i].v[k] = from_float<T>(0.0f);
+__device__ __forceinline__ void load_rows(const void* base, int64_t stride, const Place<V, STEPS>& at, Pack<T, V> (&out)[STEPS]) {
+    const T* p = static_cast<const T*>(base) + at.row0 * stride + at.channel;
+    const int64_t step = at.step * stride;
+    if (at.count == STEPS && at.inside) {
+        #pragma unroll
+        for (int i = 0; i < STEPS; ++i) out[i] = *reinterpret_cast<const Pack<T, V>*>(p + i * step);
+    } else {
+        #pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            if (at.inside && i < at.count) out[i] = *reinterpret_cast<const Pack<T, V>*>(p + i * step);
+            else {
+                #pragma unroll
+                for (int k = 0; k < V; ++k) out[i].v[k] = from_float<T>(0.0f);
+            }
         }
     }
 }
 
-// The warp's steps as (a, b), h -> a h + b, from the loaded rows.
+// The warp's steps as h -> a h + b, and all of them composed (A, H).  The loop for rows in the middle of a sequence asks for nothing else.
 template <typename T, int V, int STEPS>
 __device__ __forceinline__ void forward_steps(const ScanArgs& args, const Place<V, STEPS>& at, const Edges& edges, const Pack<T, V> (&x)[STEPS],
-                                              const Pack<T, V> (&g)[STEPS], float (&a)[STEPS][V], float (&b)[STEPS][V]) {
+                                              const Pack<T, V> (&g)[STEPS], Num<V> (&a)[STEPS], Num<V> (&b)[STEPS], Num<V>& A, Num<V>& H) {
+    A = Num<V>::all(1.0f); H = Num<V>::all(0.0f);
     #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-        const bool real = at.p0 + i < args.in.rows;
+        const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
+        a[i] = gate.a;
+        b[i] = gate.rest * number<T, V>(x[i]);
+    }
+    if (edges.first == 0 && at.count == STEPS) {
         #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const Gate gate = gate_of(gate_exp(to_float<T>(g[i].v[k])));
-            a[i][k] = real ? gate.a : 1.0f;
-            b[i][k] = real ? gate.rest * to_float<T>(x[i].v[k]) : 0.0f;
-        }
+        for (int i = 0; i < STEPS; ++i) { A = A * a[i]; H = madd(a[i], H, b[i]); }
+        return;
+    }
+    #pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        if (i >= at.count) { a[i] = Num<V>::all(1.0f); b[i] = Num<V>::all(0.0f); }
         if (edges.first >> i & 1u) {
             const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            float initial[V];
-            load_state<V>(at.inside ? args.in.initial : nullptr, int64_t(s) * args.in.width + at.channel, initial);
-            #pragma unroll
-            for (int k = 0; k < V; ++k) { b[i][k] = fmaf(a[i][k], initial[k], b[i][k]); a[i][k] = kCut; }
-        }
+            b[i] = madd(a[i], load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s)), b[i]);
+            A = a[i] = Num<V>::all(kCut); H = b[i];
+        } else { A = A * a[i]; H = madd(a[i], H, b[i]); }
     }
 }
 
 // First pass, forward: the composition of each chunk.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kForwardSteps * 32) scan_compose_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 4) scan_compose_kernel(const ScanArgs args) {
     constexpr int S = kForwardSteps, W = kChunk / S;
     __shared__ float2 shared[W][32 * V];
     const Place<V, S> at(args);
     Pack<T, V> x[S], g[S];
-    load_rows<T, V, S>(args.in.x, args.in.x_stride, args.in, at.p0, at.channel, at.inside, x);
-    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, args.in, at.p0, at.channel, at.inside, g);
+    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
+    load_rows<T, V, S>(args.in.x, args.in.x_stride, at, x);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
-    float a[S][V], b[S][V];
-    forward_steps<T, V, S>(args, at, edges, x, g, a, b);
+    Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
+    const bool plain = edges.first == 0 && at.count == S;
     #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        float A = 1.0f, H = 0.0f;
-        #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (edges.first >> i & 1u) { A = kCut; H = b[i][k]; }
-            else { A *= a[i][k]; H = fmaf(a[i][k], H, b[i][k]); }
+    for (int i = 0; i < S; ++i) {
+        const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
+        if (!plain) {
+            if (i >= at.count) continue;
+            if (edges.first >> i & 1u) {
+                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
+                A = Num<V>::all(kCut);
+                H = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
+            }
         }
-        shared[at.warp][at.lane * V + k] = make_float2(A, H);
+        H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
+        A = A * gate.a;
     }
+    leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
     if (at.warp != 0 || !at.inside) return;
     #pragma unroll
     for (int k = 0; k < V; ++k) {
-        float A = 1.0f, H = 0.0f;
+        float P = 1.0f, Q = 0.0f;
         #pragma unroll
-        for (int w = 0; w < W; ++w) compose(A, H, shared[w][at.lane * V + k]);
-        args.composed[at.chunk * args.in.width + at.channel + k] = make_float2(A, H);
+        for (int w = 0; w < W; ++w) compose(P, Q, shared[w][at.lane * V + k]);
+        args.composed[at.chunk * args.in.width + at.channel + k] = make_float2(P, Q);
     }
 }
 
 // First pass, backward: E in front of a chunk as a map of E behind it.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kForwardSteps * 32) scan_compose_backward_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 4) scan_compose_backward_kernel(const ScanArgs args) {
     constexpr int S = kForwardSteps, W = kChunk / S;
     __shared__ float2 shared[W][32 * V];
     const Place<V, S> at(args);
     Pack<T, V> d[S], g[S];
-    load_rows<T, V, S>(args.grad_h, args.grad_h_stride, args.in, at.p0, at.channel, at.inside, d);
-    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, args.in, at.p0, at.channel, at.inside, g);
+    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
+    load_rows<T, V, S>(args.grad_h, args.grad_h_stride, at, d);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
-    float A[V], H[V];
-    #pragma unroll
-    for (int k = 0; k < V; ++k) { A[k] = 1.0f; H[k] = 0.0f; }
+    Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
+    const bool plain = edges.last == 0 && at.count == S;
     #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
-        float behind[V] = {};
-        const bool last = edges.last >> i & 1u, real = at.p0 + i < args.in.rows;
-        if (last) {
-            const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            load_state<V>(at.inside ? args.grad_last : nullptr, int64_t(s) * args.in.width + at.channel, behind);
+        const Num<V> a = gate_of<V>(gate_exp<V>(number<T, V>(g[i]))).a;
+        if (!plain) {
+            if (i >= at.count) continue;
+            if (edges.last >> i & 1u) {
+                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
+                A = Num<V>::all(kCut);
+                H = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
+            }
         }
-        #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float a = gate_of(gate_exp(to_float<T>(g[i].v[k]))).a;
-            if (last) { A[k] = kCut; H[k] = behind[k]; }
-            if (real) { H[k] = a * (H[k] + to_float<T>(d[i].v[k])); A[k] *= a; }
-        }
+        H = a * (H + number<T, V>(d[i]));
+        A = A * a;
     }
-    #pragma unroll
-    for (int k = 0; k < V; ++k) shared[at.warp][at.lane * V + k] = make_float2(A[k], H[k]);
+    leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
     if (at.warp != 0 || !at.inside) return;
     #pragma unroll
@@ -206,28 +287,43 @@ __global__ void __launch_bounds__(kChunk / kForwardSteps * 32) scan_compose_back
     }
 }
 
-// Second pass: the state at each chunk's beginning (from_end: behind each chunk, walking from the last to the first).  A block takes 32
-// channels; each of its warps composes a run of chunks, then walks through it again from the state in front of the run.
+// Second pass: the state at each chunk's beginning (from_end: behind each chunk, walking from the last to the first).  A cluster of `parts` blocks takes 32
+// channels; each of its warps composes a run of chunks, then walks through it again from the state in front of the run, which
+// it has from the warps before it and the blocks before its own.
 __global__ void __launch_bounds__(kCarryWarps * 32) scan_carry_kernel(const float2* __restrict__ composed, float* __restrict__ states, int64_t chunks, int width,
-                                                                    bool from_end) {
+                                                                    bool from_end, int parts) {
     __shared__ float2 shared[kCarryWarps][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, channel = blockIdx.x * 32 + lane;
-    const int64_t run = (chunks + kCarryWarps - 1) / kCarryWarps, begin = min(warp * run, chunks), end = min(begin + run, chunks);
+    __shared__ float2 whole[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, channel = int(blockIdx.x) / parts * 32 + lane, part = int(blockIdx.x) % parts;
+    const int64_t warps = int64_t(kCarryWarps) * parts, run = (chunks + warps - 1) / warps;
+    const int64_t begin = min((int64_t(part) * kCarryWarps + warp) * run, chunks), end = min(begin + run, chunks);
+    const int64_t first = (from_end ? chunks - 1 - begin : begin) * width + channel, step = from_end ? -int64_t(width) : width;
     float A = 1.0f, H = 0.0f;
     if (channel < width) {
         #pragma unroll 8
-        for (int64_t c = begin; c < end; ++c) compose(A, H, composed[(from_end ? chunks - 1 - c : c) * width + channel]);
+        for (int64_t c = 0; c < end - begin; ++c) compose(A, H, composed[first + c * step]);
     }
     shared[warp][lane] = make_float2(A, H);
     __syncthreads();
-    if (channel >= width) return;
     float state = 0.0f;
+    if (parts > 1) {
+        if (warp == 0) {
+            float P = 1.0f, Q = 0.0f;
+            #pragma unroll
+            for (int w = 0; w < kCarryWarps; ++w) compose(P, Q, shared[w][lane]);
+            whole[lane] = make_float2(P, Q);
+        }
+        cluster_barrier();
+        const uint32_t at = smem_u32(&whole[lane]);
+        for (int p = 0; p < part; ++p) state = follow(make_float2(peer_float(at, p), peer_float(at + 4, p)), state);
+        cluster_barrier();               // no block's shared memory goes before the others have read it
+    }
+    if (channel >= width) return;
     for (int w = 0; w < warp; ++w) state = follow(shared[w][lane], state);
     #pragma unroll 8
-    for (int64_t c = begin; c < end; ++c) {
-        const int64_t at = (from_end ? chunks - 1 - c : c) * width + channel;
-        const float2 m = composed[at];
-        states[at] = state;
+    for (int64_t c = 0; c < end - begin; ++c) {
+        const float2 m = composed[first + c * step];
+        states[first + c * step] = state;
         state = follow(m, state);
     }
 }
@@ -242,148 +338,134 @@ __device__ __forceinline__ void pass_empty_sequences(const ScanArgs& args, const
 
 // Third pass, forward.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kForwardSteps * 32) scan_apply_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 2) scan_apply_kernel(const ScanArgs args) {
     constexpr int S = kForwardSteps, W = kChunk / S;
     __shared__ float2 shared[W][32 * V];
     const Place<V, S> at(args);
     Pack<T, V> x[S], g[S];
-    load_rows<T, V, S>(args.in.x, args.in.x_stride, args.in, at.p0, at.channel, at.inside, x);
-    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, args.in, at.p0, at.channel, at.inside, g);
+    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
+    load_rows<T, V, S>(args.in.x, args.in.x_stride, at, x);
+    Num<V> h = load_state<V>(at.chunk > 0 && at.inside ? args.states : nullptr, at.chunk * args.in.width + at.channel);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
-    float h[V];
-    load_state<V>(at.chunk > 0 && at.inside ? args.states : nullptr, at.chunk * args.in.width + at.channel, h);
-    float a[S][V], b[S][V];
-    forward_steps<T, V, S>(args, at, edges, x, g, a, b);
-    #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        float A = 1.0f, H = 0.0f;
+    Num<V> a[S], b[S], A, H;
+    forward_steps<T, V, S>(args, at, edges, x, g, a, b, A, H);
+    leave_map<V>(&shared[at.warp][at.lane * V], A, H);
+    __syncthreads();
+    for (int w = 0; w < at.warp; ++w) h = follow<V>(&shared[w][at.lane * V], h);
+    T* to = static_cast<T*>(args.h) + at.row0 * args.h_stride + at.channel;
+    const int64_t step = at.step * args.h_stride;
+    if (at.inside && at.count == S && (edges.first | edges.last) == 0) {
         #pragma unroll
         for (int i = 0; i < S; ++i) {
-            if (edges.first >> i & 1u) { A = kCut; H = b[i][k]; }
-            else { A *= a[i][k]; H = fmaf(a[i][k], H, b[i][k]); }
+            h = madd(a[i], h, b[i]);
+            store_number<T, V>(to + i * step, h);
         }
-        shared[at.warp][at.lane * V + k] = make_float2(A, H);
-    }
-    __syncthreads();
-    for (int w = 0; w < at.warp; ++w) {
+    } else {
         #pragma unroll
-        for (int k = 0; k < V; ++k) h[k] = follow(shared[w][at.lane * V + k], h[k]);
-    }
-    #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        const int64_t p = at.p0 + i;
-        #pragma unroll
-        for (int k = 0; k < V; ++k) h[k] = edges.first >> i & 1u ? b[i][k] : fmaf(a[i][k], h[k], b[i][k]);
-        if (at.inside && p < args.in.rows) {
-            const int64_t row = args.in.reverse ? args.in.rows - 1 - p : p;
-            store_floats<T, V>(static_cast<T*>(args.h) + row * args.h_stride + at.channel, h);
-        }
-        if (edges.last >> i & 1u) {
-            const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            if (at.inside) {
-                #pragma unroll
-                for (int k = 0; k < V; ++k) args.last[int64_t(s) * args.in.width + at.channel + k] = h[k];
+        for (int i = 0; i < S; ++i) {
+            h = edges.first >> i & 1u ? b[i] : madd(a[i], h, b[i]);
+            if (at.inside && i < at.count) store_number<T, V>(to + i * step, h);
+            if (edges.last >> i & 1u) {
+                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
+                if (at.inside) store_state<V>(args.last, at.state_at(args, s), h);
             }
         }
     }
     if (at.warp == 0 && at.inside) pass_empty_sequences(args, args.in.initial, args.last, at.chunk, at.channel, V);
 }
 
-// Third pass, backward.
+// Third pass, backward.  exp(-gate) is kept from step to step and a computed from it again: with both there were too many registers for two blocks per SM.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kBackwardSteps * 32) scan_apply_backward_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kChunk / kBackwardSteps * 32, 2) scan_apply_backward_kernel(const ScanArgs args) {
     constexpr int S = kBackwardSteps, W = kChunk / S;
     __shared__ float2 ahead[W][32 * V], back[W][32 * V];
     const Place<V, S> at(args);
-    Pack<T, V> x[S], g[S], d[S];
-    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, args.in, at.p0, at.channel, at.inside, g);
-    load_rows<T, V, S>(args.in.x, args.in.x_stride, args.in, at.p0, at.channel, at.inside, x);
-    load_rows<T, V, S>(args.grad_h, args.grad_h_stride, args.in, at.p0, at.channel, at.inside, d);
-    const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
-    float h[V], E[V];
-    load_state<V>(at.chunk > 0 && at.inside ? args.states : nullptr, at.chunk * args.in.width + at.channel, h);
-    load_state<V>(at.chunk + 1 < args.chunks && at.inside ? args.grad_states : nullptr, at.chunk * args.in.width + at.channel, E);
-    float t[S][V];                            // exp(-gate)
-    float A[V], H[V], P[V], Q[V];             // h behind the warp's rows is A h + H; E in front of them is P E + Q
-    #pragma unroll
-    for (int k = 0; k < V; ++k) { A[k] = P[k] = 1.0f; H[k] = Q[k] = 0.0f; }
-    bool cut = false;                         // the rows so far hold the end of a sequence
-    #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        const bool real = at.p0 + i < args.in.rows, first = edges.first >> i & 1u, last = edges.last >> i & 1u;
-        float initial[V] = {}, behind[V] = {};
-        if (first || last) {
-            const int64_t s = int64_t(__shfl_sync(0xffffffffu, edges.sequence, i)) * args.in.width + at.channel;
-            load_state<V>(first && at.inside ? args.in.initial : nullptr, s, initial);
-            load_state<V>(last && at.inside ? args.grad_last : nullptr, s, behind);
-        }
+    Pack<T, V> x[S], d[S];
+    Num<V> t[S];                              // exp(-gate)
+    {
+        Pack<T, V> g[S];
+        load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
+        load_rows<T, V, S>(args.in.x, args.in.x_stride, at, x);
+        load_rows<T, V, S>(args.grad_h, args.grad_h_stride, at, d);
         #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            t[i][k] = gate_exp(to_float<T>(g[i].v[k]));
-            if (!real) continue;
-            const Gate gate = gate_of(t[i][k]);
-            if (first) { A[k] = kCut; H[k] = initial[k]; }
-            A[k] *= gate.a;
-            H[k] = fmaf(gate.a, H[k], gate.rest * to_float<T>(x[i].v[k]));
-            if (cut) continue;
-            Q[k] = fmaf(P[k], gate.a * (to_float<T>(d[i].v[k]) + behind[k]), Q[k]);
-            P[k] = last ? kCut : P[k] * gate.a;
-        }
-        cut |= last;
+        for (int i = 0; i < S; ++i) t[i] = gate_exp<V>(number<T, V>(g[i]));
     }
-    #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        ahead[at.warp][at.lane * V + k] = make_float2(A[k], H[k]);
-        back[at.warp][at.lane * V + k] = make_float2(P[k], Q[k]);
+    const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
+    const int64_t state_at = at.chunk * args.in.width + at.channel;
+    Num<V> h = load_state<V>(at.chunk > 0 && at.inside ? args.states : nullptr, state_at);
+    Num<V> E = load_state<V>(at.chunk + 1 < args.chunks && at.inside ? args.grad_states : nullptr, state_at);
+    const bool plain = (edges.first | edges.last) == 0 && at.count == S;
+    const Num<V> one = Num<V>::all(1.0f), zero = Num<V>::all(0.0f);
+    {                                         // h behind the warp's rows is A h + H; E in front of them is P E + Q
+        Num<V> A = one, H = zero, P = one, Q = zero;
+        if (plain) {
+            #pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const Gate<V> gate = gate_of<V>(t[i]);
+                H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
+                A = A * gate.a;
+                Q = madd(A, number<T, V>(d[i]), Q);
+            }
+            P = A;
+        } else {
+            bool cut = false;                 // the rows so far hold the end of a sequence
+            #pragma unroll
+            for (int i = 0; i < S; ++i) {
+                if (i >= at.count) continue;
+                const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u;
+                const int64_t s = first || last ? at.state_at(args, __shfl_sync(0xffffffffu, edges.sequence, i)) : 0;
+                const Gate<V> gate = gate_of<V>(t[i]);
+                if (first) { A = Num<V>::all(kCut); H = load_state<V>(at.inside ? args.in.initial : nullptr, s); }
+                A = A * gate.a;
+                H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
+                if (cut) continue;
+                Num<V> own = number<T, V>(d[i]);
+                if (last) own = own + load_state<V>(at.inside ? args.grad_last : nullptr, s);
+                P = P * gate.a;
+                Q = madd(P, own, Q);
+                if (last) { P = Num<V>::all(kCut); cut = true; }
+            }
+        }
+        leave_map<V>(&ahead[at.warp][at.lane * V], A, H);
+        leave_map<V>(&back[at.warp][at.lane * V], P, Q);
     }
     __syncthreads();
-    for (int w = 0; w < at.warp; ++w) {
-        #pragma unroll
-        for (int k = 0; k < V; ++k) h[k] = follow(ahead[w][at.lane * V + k], h[k]);
-    }
-    for (int w = W - 1; w > at.warp; --w) {
-        #pragma unroll
-        for (int k = 0; k < V; ++k) E[k] = follow(back[w][at.lane * V + k], E[k]);
-    }
-    float slope[S][V];                        // (h_{t-1} - x) a (1 - a)
+    for (int w = 0; w < at.warp; ++w) h = follow<V>(&ahead[w][at.lane * V], h);
+    for (int w = W - 1; w > at.warp; --w) E = follow<V>(&back[w][at.lane * V], E);
+    Num<V> slope[S];                          // (h_{t-1} - x) a (1 - a)
     #pragma unroll
     for (int i = 0; i < S; ++i) {
-        const bool first = edges.first >> i & 1u;
-        if (first) {
+        if (!plain && (edges.first >> i & 1u)) {
             const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            load_state<V>(at.inside ? args.in.initial : nullptr, int64_t(s) * args.in.width + at.channel, h);
+            h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
         }
-        #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const Gate gate = gate_of(t[i][k]);
-            const float value = to_float<T>(x[i].v[k]);
-            slope[i][k] = (h[k] - value) * gate.a * gate.rest;
-            h[k] = fmaf(gate.a, h[k], gate.rest * value);
-        }
+        const Gate<V> gate = gate_of<V>(t[i]);
+        const Num<V> value = number<T, V>(x[i]);
+        slope[i] = madd(Num<V>::all(-1.0f), value, h) * (gate.a * gate.rest);
+        h = madd(gate.a, h, gate.rest * value);
     }
+    T* to_x = static_cast<T*>(args.grad_x) + at.row0 * args.grad_x_stride + at.channel;
+    T* to_gate = static_cast<T*>(args.grad_gate) + at.row0 * args.grad_gate_stride + at.channel;
+    const int64_t step_x = at.step * args.grad_x_stride, step_gate = at.step * args.grad_gate_stride;
     #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
-        const int64_t p = at.p0 + i;
-        const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u, real = p < args.in.rows;
-        int s = 0;
-        if (first || last) s = __shfl_sync(0xffffffffu, edges.sequence, i);
-        if (last) load_state<V>(at.inside ? args.grad_last : nullptr, int64_t(s) * args.in.width + at.channel, E);
-        float grad_x[V], grad_gate[V];
-        #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const Gate gate = gate_of(t[i][k]);
-            const float D = to_float<T>(d[i].v[k]) + E[k];
-            grad_x[k] = gate.rest * D;
-            grad_gate[k] = slope[i][k] * D;
-            if (real) E[k] = gate.a * D;
-        }
-        if (real && at.inside) {
-            const int64_t row = args.in.reverse ? args.in.rows - 1 - p : p;
-            store_floats<T, V>(static_cast<T*>(args.grad_x) + row * args.grad_x_stride + at.channel, grad_x);
-            store_floats<T, V>(static_cast<T*>(args.grad_gate) + row * args.grad_gate_stride + at.channel, grad_gate);
-            if (first && args.grad_initial) {
-                #pragma unroll
-                for (int k = 0; k < V; ++k) args.grad_initial[int64_t(s) * args.in.width + at.channel + k] = E[k];
+        const Gate<V> gate = gate_of<V>(t[i]);
+        if (plain && at.inside) {
+            const Num<V> D = number<T, V>(d[i]) + E;
+            store_number<T, V>(to_x + i * step_x, gate.rest * D);
+            store_number<T, V>(to_gate + i * step_gate, slope[i] * D);
+            E = gate.a * D;
+        } else if (i < at.count) {
+            const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u;
+            int s = 0;
+            if (first || last) s = __shfl_sync(0xffffffffu, edges.sequence, i);
+            if (last) E = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
+            const Num<V> D = number<T, V>(d[i]) + E;
+            E = gate.a * D;
+            if (at.inside) {
+                store_number<T, V>(to_x + i * step_x, gate.rest * D);
+                store_number<T, V>(to_gate + i * step_gate, slope[i] * D);
+                if (first && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, s), E);
             }
         }
     }
@@ -397,9 +479,9 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const T* __restrict__ x,
     const int64_t total = rows * width, step = int64_t(gridDim.x) * 256;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
         const int64_t row = i / width, channel = i - row * width;
-        const Gate g = gate_of(gate_exp(to_float<T>(gate[row * gate_stride + channel])));
+        const Gate<1> g = gate_of<1>(gate_exp<1>({to_float<T>(gate[row * gate_stride + channel])}));
         float* s = state + row * state_stride + channel;
-        const float next = fmaf(g.a, *s, g.rest * to_float<T>(x[row * x_stride + channel]));
+        const float next = fmaf(g.a.v, *s, g.rest.v * to_float<T>(x[row * x_stride + channel]));
         *s = next;
         h[row * h_stride + channel] = from_float<T>(next);
     }
@@ -408,7 +490,19 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const T* __restrict__ x,
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 int64_t chunk_count(int64_t rows) { return (rows + kChunk - 1) / kChunk; }
 
-bool pairs_possible(const void* p, int64_t stride, int64_t rows) { return !p || rows_aligned(p, stride, rows, 2, 4); }
+bool pairs_possible(const void* p, int64_t stride, int64_t rows, size_t element) { return !p || rows_aligned(p, stride, rows, element, 2 * element); }
+
+void launch_carry(const ScanArgs& args, float* states, bool from_end, cudaStream_t stream) {
+    int parts = 1;                             // eight chunks a warp, and at most eight blocks
+    while (parts < 8 && args.chunks > int64_t(kCarryWarps) * 8 * parts) parts *= 2;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = unsigned(parts); attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = unsigned((args.in.width + 31) / 32 * parts); config.blockDim = kCarryWarps * 32; config.stream = stream;
+    config.attrs = &attribute; config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, scan_carry_kernel, static_cast<const float2*>(args.composed), states, args.chunks, int(args.in.width), from_end, parts);
+}
 
 template <typename T, int V> void forward_launch(ScanArgs& args, cudaStream_t stream) {
     constexpr int threads = kChunk / kForwardSteps * 32;
@@ -416,7 +510,7 @@ template <typename T, int V> void forward_launch(ScanArgs& args, cudaStream_t st
     const unsigned int blocks = unsigned(args.chunks * args.channel_tiles);
     if (args.chunks > 1) {
         scan_compose_kernel<T, V><<<blocks, threads, 0, stream>>>(args);
-        scan_carry_kernel<<<(args.in.width + 31) / 32, kCarryWarps * 32, 0, stream>>>(args.composed, args.states, args.chunks, args.in.width, false);
+        launch_carry(args, args.states, false, stream);
     }
     scan_apply_kernel<T, V><<<blocks, threads, 0, stream>>>(args);
 }
@@ -425,17 +519,18 @@ template <typename T, int V> void backward_launch(ScanArgs& args, cudaStream_t s
     const unsigned int blocks = unsigned(args.chunks * args.channel_tiles);
     if (args.chunks > 1) {
         scan_compose_backward_kernel<T, V><<<blocks, kChunk / kForwardSteps * 32, 0, stream>>>(args);
-        scan_carry_kernel<<<(args.in.width + 31) / 32, kCarryWarps * 32, 0, stream>>>(args.composed, args.grad_states, args.chunks, args.in.width, true);
+        launch_carry(args, args.grad_states, true, stream);
     }
     scan_apply_backward_kernel<T, V><<<blocks, kChunk / kBackwardSteps * 32, 0, stream>>>(args);
 }
 
-// Two 16-bit channels a lane where every row allows it.
+// Two channels a lane where every row allows it.
 template <typename T> void scan_typed(ScanArgs& a, bool backward, cudaStream_t stream) {
     const int64_t rows = a.in.rows;
-    const bool pairs = sizeof(T) == 2 && a.in.width % 2 == 0 && pairs_possible(a.in.x, a.in.x_stride, rows) && pairs_possible(a.in.gate, a.in.gate_stride, rows) &&
-                       pairs_possible(a.h, a.h_stride, rows) && pairs_possible(a.grad_h, a.grad_h_stride, rows) &&
-                       pairs_possible(a.grad_x, a.grad_x_stride, rows) && pairs_possible(a.grad_gate, a.grad_gate_stride, rows);
+    const size_t e = sizeof(T);
+    const bool pairs = a.in.width % 2 == 0 && pairs_possible(a.in.x, a.in.x_stride, rows, e) && pairs_possible(a.in.gate, a.in.gate_stride, rows, e) &&
+                       pairs_possible(a.h, a.h_stride, rows, e) && pairs_possible(a.grad_h, a.grad_h_stride, rows, e) &&
+                       pairs_possible(a.grad_x, a.grad_x_stride, rows, e) && pairs_possible(a.grad_gate, a.grad_gate_stride, rows, e);
     if (pairs) { if (backward) backward_launch<T, 2>(a, stream); else forward_launch<T, 2>(a, stream); }
     else { if (backward) backward_launch<T, 1>(a, stream); else forward_launch<T, 1>(a, stream); }
 }

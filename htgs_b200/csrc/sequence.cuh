@@ -24,15 +24,44 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 
 // N elements side by side, moved by one load or store (N * sizeof(T) is 2, 4, 8 or 16 bytes, and the address a multiple of that).
 template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T v[N]; };
+
+// Two 16-bit values of one 32-bit word as floats, and back: one conversion for both.
+template <typename T> __device__ __forceinline__ float2 pair_floats(uint32_t word);
+template <> __device__ __forceinline__ float2 pair_floats<__nv_bfloat16>(uint32_t word) { return make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 pair_floats<__half>(uint32_t word) { return __half22float2(*reinterpret_cast<const __half2*>(&word)); }
+template <typename T> __device__ __forceinline__ uint32_t floats_pair(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t floats_pair<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t floats_pair<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int N> __device__ __forceinline__ void to_floats(const Pack<T, N>& pack, float (&out)[N]) {
+    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(&pack);
+        #pragma unroll
+        for (int i = 0; i < N / 2; ++i) { const float2 f = pair_floats<T>(words[i]); out[2 * i] = f.x; out[2 * i + 1] = f.y; }
+    } else {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = to_float<T>(pack.v[i]);
+    }
+}
 template <typename T, int N> __device__ __forceinline__ void load_floats(const T* p, float (&out)[N]) {
-    const Pack<T, N> pack = *reinterpret_cast<const Pack<T, N>*>(p);
-    #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = to_float<T>(pack.v[i]);
+    to_floats<T, N>(*reinterpret_cast<const Pack<T, N>*>(p), out);
 }
 template <typename T, int N> __device__ __forceinline__ void store_floats(T* p, const float (&in)[N]) {
     Pack<T, N> pack;
-    #pragma unroll
-    for (int i = 0; i < N; ++i) pack.v[i] = from_float<T>(in[i]);
+    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+        uint32_t* words = reinterpret_cast<uint32_t*>(&pack);
+        #pragma unroll
+        for (int i = 0; i < N / 2; ++i) words[i] = floats_pair<T>(in[2 * i], in[2 * i + 1]);
+    } else {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) pack.v[i] = from_float<T>(in[i]);
+    }
     *reinterpret_cast<Pack<T, N>*>(p) = pack;
 }
 
@@ -74,6 +103,18 @@ template <int LANES> __device__ __forceinline__ float lanes_max(float v) {
     #pragma unroll
     for (int d = LANES / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
+}
+
+// Blocks of a cluster: the float at this block's shared address in block `block`, and a barrier of all their threads.
+__device__ __forceinline__ float peer_float(uint32_t address, uint32_t block) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(block));
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---- host side of the entry points ----------------------------------------------------------------------------------------
