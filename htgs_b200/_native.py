@@ -194,7 +194,7 @@ def lib():
                                                 pointer, i64, pointer, i64, pointer]
                 l.htgs_add_rms_norm_backward_scratch_bytes.restype = ctypes.c_size_t
                 l.htgs_add_rms_norm_backward_scratch_bytes.argtypes = [i64, i32]
-                l.htgs_add_rms_norm_backward.argtypes = [pointer, i64, pointer, i64, pointer, i64, pointer, pointer, i32, i64, i32, pointer, i64, pointer,
+                l.htgs_add_rms_norm_backward.argtypes = [pointer, i64] * 4 + [pointer, pointer, i32, i64, i32, pointer, i64, pointer,
                                                          pointer, ctypes.c_size_t, pointer]
                 l.htgs_quantize_fp8.argtypes = [pointer, i64, i32, i64, i64, i32] + [pointer, i64] * 4 + [pointer]
                 l.htgs_dequantize_fp8.argtypes = [ctypes.POINTER(HtgsFp8Matrix), pointer, i64, i32, pointer]

@@ -2,8 +2,8 @@
 // (activations, gradients) or of 128 rows (weights).  For a block with largest finite magnitude m the scale is 2^e with the least e that has
 // m <= 448 * 2^e, and a code is v * 2^-e rounded to nearest, ties to even.  Infinities and NaN become NaN codes and leave the scale alone.
 //
-// `quantize_rows_kernel` codes a matrix as it lies; `quantize_tiles_kernel` codes it, its transpose or both from one read through
-// shared memory: the two gradients of a product sum over other axes than the product, and their operands' blocks run along those.
+// `quantize_rows_kernel` codes a matrix as it lies; `quantize_tiles_kernel` codes it, its transpose or both from one
+// read: the two gradients of a product sum over other axes than the product, and their operands' blocks run along those.
 // Both are bound by HBM: 2 bytes read (16-bit input) and 1 written per value and orientation.
 #include "sequence.cuh"
 
@@ -20,121 +20,173 @@ struct QuantArgs {
     uint8_t* codes_t; uint8_t* scales_t; int64_t codes_t_stride, scales_t_stride; // transposed; may be null
 };
 
-// A warp takes 32 * VEC columns of a row at a time, VEC side by side in a lane; VEC 1: 128 columns, four of them 32 apart in a lane.
+// N (4 or 8) codes side by side.
+template <int N> __device__ __forceinline__ void store_codes(uint8_t* to, const float (&v)[N], float inverse) {
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(encode4(v[0], v[1], v[2], v[3], inverse), encode4(v[4], v[5], v[6], v[7], inverse));
+    else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = encode4(v[0], v[1], v[2], v[3], inverse);
+}
+
+// A warp takes 32 * VEC columns, VEC side by side in a lane (VEC 1: 128 columns, four of them 32 apart in a lane), of several rows, four at a
+// time, so that enough loads are on their way.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantArgs a) {
     const int lane = threadIdx.x & 31;
-    constexpr int kColumns = VEC == 1 ? kScaleBlock : 32 * VEC, kValues = VEC == 1 ? 4 : VEC, kLanes = VEC == 8 ? 16 : 32;
-    const int64_t units_per_row = (a.width + kColumns - 1) / kColumns, units = units_per_row * a.rows;
-    const int64_t step = int64_t(gridDim.x) * (kQuantBlock / 32);
-    for (int64_t unit = int64_t(blockIdx.x) * (kQuantBlock / 32) + (threadIdx.x >> 5); unit < units; unit += step) {
-        const int64_t row = unit / units_per_row, first = (unit - row * units_per_row) * kColumns;
-        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-        uint8_t* codes = a.codes + row * a.codes_stride;
-        float v[kValues];
-        float largest = 0.0f;
-        if (VEC == 1) {
-            #pragma unroll
-            for (int i = 0; i < kValues; ++i) v[i] = first + 32 * i + lane < a.width ? to_float<T>(x[first + 32 * i + lane]) : 0.0f;
-        } else if (first + lane * VEC < a.width) {
-            load_floats<T, kValues>(x + first + lane * VEC, v);
-        } else {
-            #pragma unroll
-            for (int i = 0; i < kValues; ++i) v[i] = 0.0f;
+    constexpr int kColumns = VEC == 1 ? kScaleBlock : 32 * VEC, kValues = VEC == 1 ? 4 : VEC, kLanes = VEC == 8 ? 16 : 32, R = 4;
+    const uint32_t across = uint32_t((a.width + kColumns - 1) / kColumns), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
+    const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;        // rows that are begun side by side
+    if (warp >= across * down) return;
+    const int64_t first = int64_t(warp % across) * kColumns, at = first + (lane / kLanes) * kScaleBlock;
+    for (int64_t row0 = warp / across; row0 < a.rows; row0 += int64_t(down) * R) {
+        float v[R][kValues];
+        #pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + int64_t(down) * r;
+            const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+            if (VEC == 1) {
+                #pragma unroll
+                for (int i = 0; i < kValues; ++i) v[r][i] = row < a.rows && first + 32 * i + lane < a.width ? to_float<T>(x[first + 32 * i + lane]) : 0.0f;
+            } else if (row < a.rows && first + lane * VEC < a.width) {
+                load_floats<T, kValues>(x + first + lane * VEC, v[r]);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < kValues; ++i) v[r][i] = 0.0f;
+            }
         }
         #pragma unroll
-        for (int i = 0; i < kValues; ++i) largest = fmaxf(largest, finite_magnitude(v[i]));
-        const int e = scale_exponent(lanes_max<kLanes>(largest));
-        const float inverse = inverse_scale(e);
-        if (VEC == 1) {
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + int64_t(down) * r;
+            if (row >= a.rows) break;
+            uint8_t* codes = a.codes + row * a.codes_stride;
+            float largest = 0.0f;
             #pragma unroll
-            for (int i = 0; i < kValues; ++i)
-                if (first + 32 * i + lane < a.width) codes[first + 32 * i + lane] = uint8_t(encode2(v[i], 0.0f, inverse) & 0xffu);
-        } else if (first + lane * VEC < a.width) {
-            if (VEC == 8)
-                *reinterpret_cast<uint2*>(codes + first + lane * VEC) =
-                    make_uint2(encode4(v[0], v[1], v[2], v[3], inverse), encode4(v[4 % kValues], v[5 % kValues], v[6 % kValues], v[7 % kValues], inverse));
-            else
-                *reinterpret_cast<uint32_t*>(codes + first + lane * VEC) = encode4(v[0], v[1], v[2], v[3], inverse);
+            for (int i = 0; i < kValues; ++i) largest = fmaxf(largest, finite_magnitude(v[r][i]));
+            const int e = scale_exponent(lanes_max<kLanes>(largest));
+            const float inverse = inverse_scale(e);
+            if (VEC == 1) {
+                #pragma unroll
+                for (int i = 0; i < kValues; ++i)
+                    if (first + 32 * i + lane < a.width) codes[first + 32 * i + lane] = uint8_t(encode2(v[r][i], 0.0f, inverse) & 0xffu);
+            } else if (first + lane * VEC < a.width) {
+                store_codes<kValues>(codes + first + lane * VEC, v[r], inverse);
+            }
+            if (lane % kLanes == 0 && at < a.width) a.scales[row * a.scales_stride + at / kScaleBlock] = uint8_t(e + 127);
         }
-        const int64_t at = first + (lane / kLanes) * kScaleBlock;
-        if (lane % kLanes == 0 && at < a.width) a.scales[row * a.scales_stride + at / kScaleBlock] = uint8_t(e + 127);
     }
 }
 
-// One block per 128 x 128 values.  The tile lies in shared memory with a row pitch of an odd number of words, so that the 32 rows that a
-// warp reads of one column come from 32 banks.  PER_TILE: one scale for the whole tile.
-template <typename T, bool PER_TILE>
+// One block per 128 x 128 values.  A thread holds eight rows by eight columns: half a warp has the 128 columns of its eight rows, so a row's
+// largest value is found by shuffles, a column's through shared memory.  The transposed codes go through shared memory too, so that they leave as rows of
+// 128: the eight bytes of half-warp h and column c lie in slot h ^ (c / 8 % 16) of the column's sixteen, which spreads the 16
+// lanes of a store over all banks.  PER_TILE: one scale for the whole tile.  VEC: columns a load takes; a thread's eight are (8 / VEC) groups 16 * VEC apart.
+template <typename T, int VEC, bool PER_TILE>
 __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const QuantArgs a) {
-    extern __shared__ unsigned char raw[];
-    T* tile = reinterpret_cast<T*>(raw);
-    constexpr int kPitch = sizeof(T) == 4 ? 129 : 130;
-    __shared__ float block_largest[kQuantBlock / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ float column_largest[16][kScaleBlock];
+    __shared__ float column_all[kScaleBlock];
+    __shared__ __align__(16) uint2 turned[kScaleBlock][16];
+    constexpr int G = 8 / VEC;
+    const int l = threadIdx.x & 15, h = threadIdx.x >> 4;
     const int64_t row0 = int64_t(blockIdx.y) * kScaleBlock, column0 = int64_t(blockIdx.x) * kScaleBlock;
-    float largest = 0.0f;
-    for (int r = warp; r < kScaleBlock; r += kQuantBlock / 32) {
-        const int64_t row = row0 + r;
-        const T* x = static_cast<const T*>(a.x) + row * a.x_stride + column0;
-        float v[4];
+    const int rows = int(min(int64_t(kScaleBlock), a.rows - row0)), columns = int(min(int64_t(kScaleBlock), a.width - column0));
+    const auto column = [&](int c) { return c / VEC * 16 * VEC + l * VEC + c % VEC; };      // of the thread's c-th value in the tile
+    Pack<T, VEC> raw[8][G];
+    const T* x = static_cast<const T*>(a.x) + (row0 + h * 8) * a.x_stride + column0;
+    #pragma unroll
+    for (int r = 0; r < 8; ++r) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = lane + 32 * i;
-            const T value = row < a.rows && column0 + c < a.width ? x[c] : from_float<T>(0.0f);
-            tile[r * kPitch + c] = value;
-            v[i] = to_float<T>(value);
+        for (int j = 0; j < G; ++j) {
+            if (h * 8 + r < rows && column(j * VEC) < columns) raw[r][j] = *reinterpret_cast<const Pack<T, VEC>*>(x + r * a.x_stride + column(j * VEC));
+            else {
+                #pragma unroll
+                for (int i = 0; i < VEC; ++i) raw[r][j].v[i] = from_float<T>(0.0f);
+            }
         }
-        float most = fmaxf(fmaxf(finite_magnitude(v[0]), finite_magnitude(v[1])), fmaxf(finite_magnitude(v[2]), finite_magnitude(v[3])));
-        if (PER_TILE) { largest = fmaxf(largest, most); continue; }
-        if (!a.codes || row >= a.rows) continue;
-        const int e = scale_exponent(lanes_max<32>(most));
-        const float inverse = inverse_scale(e);
-        uint8_t* codes = a.codes + row * a.codes_stride + column0;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (column0 + lane + 32 * i < a.width) codes[lane + 32 * i] = uint8_t(encode2(v[i], 0.0f, inverse) & 0xffu);
-        if (lane == 0) a.scales[row * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
     }
-    int tile_e = 0;
-    if (PER_TILE) {
-        largest = lanes_max<32>(largest);
-        if (lane == 0) block_largest[warp] = largest;
+    const auto values = [&](int r, float (&v)[8]) {
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            float f[VEC];
+            to_floats<T, VEC>(raw[r][j], f);
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) v[j * VEC + i] = f[i];
+        }
+    };
+    const auto store_row_codes = [&](int r, const float (&v)[8], float inverse) {
+        uint8_t* codes = a.codes + (row0 + h * 8 + r) * a.codes_stride + column0;
+        #pragma unroll
+        for (int j = 0; j < G; ++j) {
+            if (column(j * VEC) >= columns) continue;
+            float f[VEC];
+            #pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = v[j * VEC + i];
+            if (VEC == 1) codes[column(j)] = uint8_t(encode2(f[0], 0.0f, inverse) & 0xffu);
+            else store_codes<VEC>(codes + column(j * VEC), f, inverse);
+        }
+    };
+    float most[8] = {};                      // of the thread's columns
+    #pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        float v[8], largest = 0.0f;
+        values(r, v);
+        #pragma unroll
+        for (int c = 0; c < 8; ++c) { const float m = finite_magnitude(v[c]); largest = fmaxf(largest, m); most[c] = fmaxf(most[c], m); }
+        if (PER_TILE || !a.codes) continue;
+        const int e = scale_exponent(lanes_max<16>(largest));
+        if (h * 8 + r >= rows) continue;
+        store_row_codes(r, v, inverse_scale(e));
+        if (l == 0) a.scales[(row0 + h * 8 + r) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
+    }
+    if (!PER_TILE && !a.codes_t) return;
+    #pragma unroll
+    for (int c = 0; c < 8; ++c) column_largest[h][column(c)] = most[c];
+    __syncthreads();
+    if (threadIdx.x < kScaleBlock) {
+        float largest = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) largest = fmaxf(largest, column_largest[i][threadIdx.x]);
+        if (PER_TILE) largest = lanes_max<32>(largest);
+        column_all[threadIdx.x] = largest;
+        if (!PER_TILE && int(threadIdx.x) < columns) a.scales_t[(column0 + threadIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(scale_exponent(largest) + 127);
     }
     __syncthreads();
     if (PER_TILE) {
-        #pragma unroll
-        for (int w = 0; w < kQuantBlock / 32; ++w) largest = fmaxf(largest, block_largest[w]);
-        tile_e = scale_exponent(largest);
+        const int e = scale_exponent(fmaxf(fmaxf(column_all[0], column_all[32]), fmaxf(column_all[64], column_all[96])));
         if (a.codes) {
-            const float inverse = inverse_scale(tile_e);
-            for (int r = warp; r < kScaleBlock && row0 + r < a.rows; r += kQuantBlock / 32) {
-                uint8_t* codes = a.codes + (row0 + r) * a.codes_stride + column0;
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = lane + 32 * i;
-                    if (column0 + c < a.width) codes[c] = uint8_t(encode2(to_float<T>(tile[r * kPitch + c]), 0.0f, inverse) & 0xffu);
-                }
+            #pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                if (h * 8 + r >= rows) break;
+                float v[8];
+                values(r, v);
+                store_row_codes(r, v, inverse_scale(e));
             }
-            if (threadIdx.x == 0) a.scales[int64_t(blockIdx.y) * a.scales_stride + blockIdx.x] = uint8_t(tile_e + 127);
+            if (threadIdx.x == 0) a.scales[int64_t(blockIdx.y) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
         }
-        if (a.codes_t && threadIdx.x == 0) a.scales_t[int64_t(blockIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(tile_e + 127);
+        if (!a.codes_t) return;
+        if (threadIdx.x == 0) a.scales_t[int64_t(blockIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(e + 127);
+        #pragma unroll
+        for (int c = 0; c < 8; ++c) most[c] = inverse_scale(e);
+    } else {
+        #pragma unroll
+        for (int c = 0; c < 8; ++c) most[c] = inverse_scale(scale_exponent(column_all[column(c)]));
     }
-    if (!a.codes_t) return;
-    for (int c = warp; c < kScaleBlock && column0 + c < a.width; c += kQuantBlock / 32) {
-        float v[4];
+    {
+        float v[8][8];
         #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = to_float<T>(tile[(lane + 32 * i) * kPitch + c]);
-        int e = tile_e;
-        if (!PER_TILE) {
-            const float most = fmaxf(fmaxf(finite_magnitude(v[0]), finite_magnitude(v[1])), fmaxf(finite_magnitude(v[2]), finite_magnitude(v[3])));
-            e = scale_exponent(lanes_max<32>(most));
-            if (lane == 0) a.scales_t[(column0 + c) * a.scales_t_stride + blockIdx.y] = uint8_t(e + 127);
+        for (int r = 0; r < 8; ++r) values(r, v[r]);
+        #pragma unroll
+        for (int c = 0; c < 8; ++c)
+            turned[column(c)][h ^ (column(c) / 8 % 16)] = make_uint2(encode4(v[0][c], v[1][c], v[2][c], v[3][c], most[c]), encode4(v[4][c], v[5][c], v[6][c], v[7][c], most[c]));
+    }
+    __syncthreads();
+    const bool whole = rows == kScaleBlock && a.codes_t_stride % 16 == 0 && reinterpret_cast<uintptr_t>(a.codes_t) % 16 == 0;
+    for (int i = threadIdx.x; i < columns * 8; i += kQuantBlock) {
+        const int c = i >> 3, s = i & 7;                  // rows 16 s .. 16 s + 15 of column c
+        const uint2 lo = turned[c][(2 * s) ^ (c / 8 % 16)], hi = turned[c][(2 * s + 1) ^ (c / 8 % 16)];
+        uint8_t* to = a.codes_t + (column0 + c) * a.codes_t_stride + row0 + 16 * s;
+        if (whole) *reinterpret_cast<uint4*>(to) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        else {
+            const uint32_t words[4] = {lo.x, lo.y, hi.x, hi.y};
+            for (int k = 0; k < 16 && 16 * s + k < rows; ++k) to[k] = uint8_t(words[k >> 2] >> (8 * (k & 3)));
         }
-        const float inverse = inverse_scale(e);
-        uint8_t* codes = a.codes_t + (column0 + c) * a.codes_t_stride + row0;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (row0 + lane + 32 * i < a.rows) codes[lane + 32 * i] = uint8_t(encode2(v[i], 0.0f, inverse) & 0xffu);
     }
 }
 
@@ -167,26 +219,24 @@ unsigned int capped_blocks(int64_t work, int64_t per_block) {
     return unsigned(blocks < 148 * 8 ? blocks : 148 * 8);
 }
 
-template <typename T> void quantize_typed(const QuantArgs& a, int rows_per_scale, cudaStream_t stream) {
-    if (rows_per_scale == 1 && !a.codes_t) {
-        constexpr int V = 16 / int(sizeof(T));
-        if (a.width % V == 0 && rows_aligned(a.x, a.x_stride, a.rows, sizeof(T), 16) && rows_aligned(a.codes, a.codes_stride, a.rows, 1, V))
-            quantize_rows_kernel<T, V><<<capped_blocks(a.rows * ((a.width + 32 * V - 1) / (32 * V)), kQuantBlock / 32), kQuantBlock, 0, stream>>>(a);
-        else
-            quantize_rows_kernel<T, 1><<<capped_blocks(a.rows * ((a.width + kScaleBlock - 1) / kScaleBlock), kQuantBlock / 32), kQuantBlock, 0, stream>>>(a);
-        return;
-    }
+template <typename T, int VEC> void launch_rows(const QuantArgs& a, cudaStream_t stream) {
+    constexpr int kColumns = VEC == 1 ? kScaleBlock : 32 * VEC;
+    const int64_t across = (a.width + kColumns - 1) / kColumns, warps = across * ((a.rows + 3) / 4);
+    int64_t blocks = (warps + kQuantBlock / 32 - 1) / (kQuantBlock / 32);
+    if (blocks > 148 * 8) blocks = 148 * 8;
+    if (blocks * (kQuantBlock / 32) < across) blocks = (across + kQuantBlock / 32 - 1) / (kQuantBlock / 32);     // at least one row at a time
+    quantize_rows_kernel<T, VEC><<<unsigned(blocks), kQuantBlock, 0, stream>>>(a);
+}
+template <typename T, int VEC> void launch_tiles(const QuantArgs& a, int rows_per_scale, cudaStream_t stream) {
     const dim3 grid(unsigned((a.width + kScaleBlock - 1) / kScaleBlock), unsigned((a.rows + kScaleBlock - 1) / kScaleBlock));
-    constexpr size_t smem = size_t(kScaleBlock) * (sizeof(T) == 4 ? 129 : 130) * sizeof(T);
-    if (rows_per_scale == 1) {
-        static PerDeviceOnce once;
-        once.run([] { return cudaFuncSetAttribute(quantize_tiles_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)); });
-        quantize_tiles_kernel<T, false><<<grid, kQuantBlock, smem, stream>>>(a);
-    } else {
-        static PerDeviceOnce once;
-        once.run([] { return cudaFuncSetAttribute(quantize_tiles_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)); });
-        quantize_tiles_kernel<T, true><<<grid, kQuantBlock, smem, stream>>>(a);
-    }
+    if (rows_per_scale == 1) quantize_tiles_kernel<T, VEC, false><<<grid, kQuantBlock, 0, stream>>>(a);
+    else quantize_tiles_kernel<T, VEC, true><<<grid, kQuantBlock, 0, stream>>>(a);
+}
+template <typename T> void quantize_typed(const QuantArgs& a, int rows_per_scale, cudaStream_t stream) {
+    constexpr int V = 16 / int(sizeof(T));
+    const bool wide = a.width % V == 0 && rows_aligned(a.x, a.x_stride, a.rows, sizeof(T), 16) && rows_aligned(a.codes, a.codes_stride, a.rows, 1, V);
+    if (rows_per_scale == 1 && !a.codes_t) { if (wide) launch_rows<T, V>(a, stream); else launch_rows<T, 1>(a, stream); }
+    else { if (wide) launch_tiles<T, V>(a, rows_per_scale, stream); else launch_tiles<T, 1>(a, rows_per_scale, stream); }
 }
 
 template <typename T> void dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {

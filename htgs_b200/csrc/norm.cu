@@ -5,9 +5,10 @@
 //       grad_x = grad_residual = rho * (z - unit * mean(z * unit)) + grad_sum;      grad_weight = sum over rows of grad_y * unit
 //
 // A row stays in registers between its statistics and its output, so every value crosses HBM once: read x and residual, write sum
-// and y (or 8-bit codes and a scale byte for each 128 columns); backward read grad_y, grad_sum and sum, write one gradient that
-// serves x and residual alike.  Bound by HBM.  A warp holds a row of up to 1024 columns (32 values a lane), eight warps a wider one.
-// Sums are 32-bit; y is computed from the unrounded u, the backward pass from the stream's rounded one, which is what is kept.
+// and y (or 8-bit codes and a scale byte for each 128 columns); backward read grad_y, grad_sum, x and residual, write one gradient that
+// serves x and residual alike.  Bound by HBM.  Forward, a warp holds a row of up to 1024 columns (32 values a lane), eight warps a wider one.
+// Sums are 32-bit and u is never rounded where it is computed with: the backward pass adds x and residual again rather than read the stream, whose
+// rounding to 16 bits would show in grad_weight (relative error 0.0028 instead of 0.0018 at 65537 x 1024 in bf16) for 2 bytes less of 16 a value.
 #include "sequence.cuh"
 
 namespace htgs {
@@ -16,7 +17,8 @@ namespace {
 
 constexpr int kNormBlock = 256;
 constexpr int kNormWarps = kNormBlock / 32;
-constexpr int kNormBackwardBlocks = 148 * 2;       // persistent: two blocks per SM, each with one partial sum of grad_weight
+constexpr int kBackwardColumns = 8;                // a thread
+constexpr int kNarrowBlock = 128, kNarrowBlocks = 4, kWideBlock = 1024;
 constexpr int kMaxNormWidth = kNormBlock * 32;
 
 struct NormArgs {
@@ -30,8 +32,8 @@ struct NormArgs {
 };
 
 struct NormBackwardArgs {
-    const void* grad_y; const void* grad_sum; const void* sum; const void* weight; const float* rstd;
-    int64_t grad_y_stride, grad_sum_stride, sum_stride, grad_x_stride;
+    const void* grad_y; const void* grad_sum; const void* x; const void* residual; const void* weight; const float* rstd;
+    int64_t grad_y_stride, grad_sum_stride, x_stride, residual_stride, grad_x_stride;
     void* grad_x; float* partial;
     int64_t rows;
     int32_t width;
@@ -138,84 +140,118 @@ __global__ void __launch_bounds__(kNormBlock) norm_kernel(const NormArgs a) {
     }
 }
 
-template <typename T, int VEC, int E, int WPR>
-__global__ void __launch_bounds__(kNormBlock) norm_backward_kernel(const NormBackwardArgs a) {
-    __shared__ float shared[WPR == 1 ? kNormWarps * 32 * E : kNormWarps];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int G = E / VEC;
-    constexpr int kRows = kNormWarps / WPR;
-    const int base = WPR == 1 ? 0 : warp * 32 * E;
-    const T* weight = static_cast<const T*>(a.weight);
-    float grad_weight[G][VEC] = {};
-    for (int64_t row = int64_t(blockIdx.x) * kRows + (WPR == 1 ? warp : 0); row < a.rows; row += int64_t(gridDim.x) * kRows) {
-        const T* grad_y = static_cast<const T*>(a.grad_y) + row * a.grad_y_stride;
-        const T* sum = static_cast<const T*>(a.sum) + row * a.sum_stride;
-        const T* grad_sum = a.grad_sum ? static_cast<const T*>(a.grad_sum) + row * a.grad_sum_stride : nullptr;
-        Pack<T, VEC> g[G], u[G], d[G];          // as they are in memory: half the registers of 32-bit values
+// A block holds whole rows, eight columns a thread, and takes R of them at a time, so that enough loads are on their way; persistent, with
+// each thread's part of grad_weight in registers until the end.  Groups of VEC columns as in norm_kernel, 256 columns a warp.
+// Blocks of up to 128 threads (1024 columns), four per SM, have registers for four rows of 16-byte groups (two of other types); wider ones take one.
+template <typename T, int VEC, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == kNarrowBlock ? kNarrowBlocks : 1) norm_backward_kernel(const NormBackwardArgs a) {
+    constexpr int G = kBackwardColumns / VEC, R = MOST != kNarrowBlock ? 1 : VEC * sizeof(T) == 16 && sizeof(T) == 2 ? 4 : 2;
+    __shared__ float shared[2][32][R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int base = warp * 32 * kBackwardColumns;
+    float w[G][VEC] = {}, grad_weight[G][VEC] = {};
+    #pragma unroll
+    for (int j = 0; j < G; ++j) {
+        const int column = base + (32 * j + lane) * VEC;
+        if (column < a.width) load_floats<T, VEC>(static_cast<const T*>(a.weight) + column, w[j]);
+    }
+    const float per_width = 1.0f / float(a.width);
+    int buffer = 0;
+    for (int64_t row0 = int64_t(blockIdx.x) * R; row0 < a.rows; row0 += int64_t(gridDim.x) * R, buffer ^= 1) {
+        Pack<T, VEC> g[R][G], x[R][G], r[R][G], d[R][G];          // as they are in memory: half the registers of 32-bit values
+        float rho[R];
         #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const int column = base + (32 * j + lane) * VEC;
-            if (column < a.width) {
-                g[j] = *reinterpret_cast<const Pack<T, VEC>*>(grad_y + column);
-                u[j] = *reinterpret_cast<const Pack<T, VEC>*>(sum + column);
-                if (grad_sum) d[j] = *reinterpret_cast<const Pack<T, VEC>*>(grad_sum + column);
-            } else {
+        for (int k = 0; k < R; ++k) {
+            const int64_t row = min(row0 + k, a.rows - 1);
+            rho[k] = row0 + k < a.rows ? a.rstd[row] : 0.0f;
+            #pragma unroll
+            for (int j = 0; j < G; ++j) {
+                const int column = base + (32 * j + lane) * VEC;
+                if (column < a.width && row0 + k < a.rows) {
+                    g[k][j] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.grad_y) + row * a.grad_y_stride + column);
+                    x[k][j] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + row * a.x_stride + column);
+                    if (a.residual) r[k][j] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.residual) + row * a.residual_stride + column);
+                    if (a.grad_sum) d[k][j] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.grad_sum) + row * a.grad_sum_stride + column);
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < VEC; ++i) g[k][j].v[i] = x[k][j].v[i] = r[k][j].v[i] = from_float<T>(0.0f);
+                }
+            }
+        }
+        float mean[R];
+        #pragma unroll
+        for (int k = 0; k < R; ++k) {
+            float dot = 0.0f;
+            #pragma unroll
+            for (int j = 0; j < G; ++j) {
+                float gy[VEC], u[VEC];
+                to_floats<T, VEC>(g[k][j], gy);
+                to_floats<T, VEC>(x[k][j], u);
+                if (a.residual) {
+                    float v[VEC];
+                    to_floats<T, VEC>(r[k][j], v);
+                    #pragma unroll
+                    for (int i = 0; i < VEC; ++i) u[i] += v[i];
+                }
                 #pragma unroll
-                for (int i = 0; i < VEC; ++i) g[j].v[i] = u[j].v[i] = from_float<T>(0.0f);
+                for (int i = 0; i < VEC; ++i) {
+                    const float term = gy[i] * (u[i] * rho[k]);
+                    grad_weight[j][i] += term;
+                    dot = fmaf(term, w[j][i], dot);
+                }
+            }
+            mean[k] = warp_sum(dot);
+        }
+        if (warps > 1) {
+            if (lane == 0) {
+                #pragma unroll
+                for (int k = 0; k < R; ++k) shared[buffer][warp][k] = mean[k];
+            }
+            __syncthreads();            // one per trip: the other buffer is read before the next one
+            #pragma unroll
+            for (int k = 0; k < R; ++k) mean[k] = 0.0f;
+            for (int v = 0; v < warps; ++v) {
+                #pragma unroll
+                for (int k = 0; k < R; ++k) mean[k] += shared[buffer][v][k];
             }
         }
-        const float rho = a.rstd[row];
-        float dot = 0.0f;
         #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const int column = base + (32 * j + lane) * VEC;
-            float w[VEC] = {};
-            if (column < a.width) load_floats<T, VEC>(weight + column, w);
+        for (int k = 0; k < R; ++k) {
+            if (row0 + k >= a.rows) break;
+            T* grad_x = static_cast<T*>(a.grad_x) + (row0 + k) * a.grad_x_stride;
+            const float slope = mean[k] * per_width * rho[k];
             #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float gy = to_float<T>(g[j].v[i]), unit = to_float<T>(u[j].v[i]) * rho;
-                grad_weight[j][i] += gy * unit;
-                dot += gy * w[i] * unit;
+            for (int j = 0; j < G; ++j) {
+                const int column = base + (32 * j + lane) * VEC;
+                if (column >= a.width) continue;
+                float gy[VEC], u[VEC], out[VEC];
+                to_floats<T, VEC>(g[k][j], gy);
+                to_floats<T, VEC>(x[k][j], u);
+                if (a.residual) {
+                    float v[VEC];
+                    to_floats<T, VEC>(r[k][j], v);
+                    #pragma unroll
+                    for (int i = 0; i < VEC; ++i) u[i] += v[i];
+                }
+                #pragma unroll
+                for (int i = 0; i < VEC; ++i) out[i] = rho[k] * (gy[i] * w[j][i] - u[i] * slope);
+                if (a.grad_sum) {
+                    float v[VEC];
+                    to_floats<T, VEC>(d[k][j], v);
+                    #pragma unroll
+                    for (int i = 0; i < VEC; ++i) out[i] += v[i];
+                }
+                store_floats<T, VEC>(grad_x + column, out);
             }
-        }
-        const float mean = row_sum<WPR>(dot, shared) / float(a.width);
-        T* grad_x = static_cast<T*>(a.grad_x) + row * a.grad_x_stride;
-        #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const int column = base + (32 * j + lane) * VEC;
-            if (column >= a.width) continue;
-            float w[VEC], out[VEC];
-            load_floats<T, VEC>(weight + column, w);
-            #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                out[i] = rho * (to_float<T>(g[j].v[i]) * w[i] - to_float<T>(u[j].v[i]) * rho * mean);
-                if (grad_sum) out[i] += to_float<T>(d[j].v[i]);
-            }
-            store_floats<T, VEC>(grad_x + column, out);
         }
     }
     float* partial = a.partial + int64_t(blockIdx.x) * a.width;
-    if (WPR == 1) {
+    #pragma unroll
+    for (int j = 0; j < G; ++j) {
+        const int column = base + (32 * j + lane) * VEC;
+        if (column >= a.width) continue;
         #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            #pragma unroll
-            for (int i = 0; i < VEC; ++i) shared[warp * 32 * E + (32 * j + lane) * VEC + i] = grad_weight[j][i];
-        }
-        __syncthreads();
-        for (int column = threadIdx.x; column < min(a.width, 32 * E); column += kNormBlock) {
-            float total = 0.0f;
-            #pragma unroll
-            for (int w = 0; w < kNormWarps; ++w) total += shared[w * 32 * E + column];
-            partial[column] = total;
-        }
-    } else {
-        #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            const int column = base + (32 * j + lane) * VEC;
-            if (column >= a.width) continue;
-            #pragma unroll
-            for (int i = 0; i < VEC; ++i) partial[column + i] = grad_weight[j][i];
-        }
+        for (int i = 0; i < VEC; ++i) partial[column + i] = grad_weight[j][i];
     }
 }
 
@@ -236,19 +272,18 @@ template <typename T> __global__ void __launch_bounds__(kNormBlock) norm_weight_
     }
 }
 
+int backward_threads(int width) { return (width + 32 * kBackwardColumns - 1) / (32 * kBackwardColumns) * 32; }
+// Persistent blocks, each with one partial sum of grad_weight: as many threads per SM as their registers allow.
 int backward_blocks(int64_t rows, int width) {
-    const int64_t rows_per_block = width <= 32 * 32 ? kNormWarps : 1;
-    const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
-    return int(blocks < kNormBackwardBlocks ? blocks : kNormBackwardBlocks);
+    const int threads = backward_threads(width), per_sm = (threads <= kNarrowBlock ? kNarrowBlock * kNarrowBlocks : kWideBlock) / threads;
+    const int64_t blocks = (rows + 1) / 2, most = 148 * per_sm;
+    return int(blocks < most ? blocks : most);
 }
 
 template <typename T, int VEC, int E, int WPR> void launch_norm(const NormArgs& a, cudaStream_t stream) {
     const unsigned int blocks = unsigned((a.rows + kNormWarps / WPR - 1) / (kNormWarps / WPR));
     if (a.codes) norm_kernel<T, VEC, E, WPR, true><<<blocks, kNormBlock, 0, stream>>>(a);
     else norm_kernel<T, VEC, E, WPR, false><<<blocks, kNormBlock, 0, stream>>>(a);
-}
-template <typename T, int VEC, int E, int WPR> void launch_backward(const NormBackwardArgs& a, cudaStream_t stream) {
-    norm_backward_kernel<T, VEC, E, WPR><<<backward_blocks(a.rows, a.width), kNormBlock, 0, stream>>>(a);
 }
 
 // The fewest values a lane that hold a row: one warp up to 1024 columns, then eight.
@@ -263,7 +298,11 @@ template <typename T, int VEC, int E, int WPR> void launch_backward(const NormBa
     } while (0)
 
 template <typename T, int VEC> void norm_widths(const NormArgs& a, cudaStream_t stream) { HTGS_NORM_WIDTHS(launch_norm, a); }
-template <typename T, int VEC> void backward_widths(const NormBackwardArgs& a, cudaStream_t stream) { HTGS_NORM_WIDTHS(launch_backward, a); }
+template <typename T, int VEC> void backward_launch(const NormBackwardArgs& a, cudaStream_t stream) {
+    const int threads = backward_threads(a.width), blocks = backward_blocks(a.rows, a.width);
+    if (threads <= kNarrowBlock) norm_backward_kernel<T, VEC, kNarrowBlock><<<blocks, threads, 0, stream>>>(a);
+    else norm_backward_kernel<T, VEC, kWideBlock><<<blocks, threads, 0, stream>>>(a);
+}
 
 // 16-byte groups where every row of every tensor allows them, single values otherwise.
 template <typename T> void norm_typed(const NormArgs& a, cudaStream_t stream) {
@@ -278,8 +317,9 @@ template <typename T> void backward_typed(const NormBackwardArgs& a, void* grad_
     constexpr int V = 16 / int(sizeof(T));
     const size_t e = sizeof(T);
     const bool wide = a.width % V == 0 && rows_aligned(a.grad_y, a.grad_y_stride, a.rows, e, 16) && rows_aligned(a.grad_sum, a.grad_sum_stride, a.rows, e, 16) &&
-                      rows_aligned(a.sum, a.sum_stride, a.rows, e, 16) && aligned(a.weight, 16) && rows_aligned(a.grad_x, a.grad_x_stride, a.rows, e, 16);
-    if (wide) backward_widths<T, V>(a, stream); else backward_widths<T, 1>(a, stream);
+                      rows_aligned(a.x, a.x_stride, a.rows, e, 16) && rows_aligned(a.residual, a.residual_stride, a.rows, e, 16) && aligned(a.weight, 16) &&
+                      rows_aligned(a.grad_x, a.grad_x_stride, a.rows, e, 16);
+    if (wide) backward_launch<T, V>(a, stream); else backward_launch<T, 1>(a, stream);
     norm_weight_kernel<T><<<(a.width + 31) / 32, kNormBlock, 0, stream>>>(a.partial, backward_blocks(a.rows, a.width), a.width, static_cast<T*>(grad_weight));
 }
 
@@ -314,9 +354,9 @@ size_t htgs_add_rms_norm_backward_scratch_bytes(int64_t rows, int32_t width) {
     return size_t(htgs::backward_blocks(rows, width)) * size_t(width) * sizeof(float);
 }
 
-int htgs_add_rms_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride, const void* sum,
-                               int64_t sum_stride, const void* weight, const float* rstd, int type, int64_t rows, int32_t width, void* grad_x,
-                               int64_t grad_x_stride, void* grad_weight, void* scratch, size_t scratch_bytes, void* stream) {
+int htgs_add_rms_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride, const void* x, int64_t x_stride,
+                               const void* residual, int64_t residual_stride, const void* weight, const float* rstd, int type, int64_t rows, int32_t width,
+                               void* grad_x, int64_t grad_x_stride, void* grad_weight, void* scratch, size_t scratch_bytes, void* stream) {
     using namespace htgs;
     if (!known_type(type)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm_backward: unknown element type");
     if (rows < 0 || rows > 0x7fffffff || width < 1 || width > kMaxNormWidth)
@@ -327,10 +367,10 @@ int htgs_add_rms_norm_backward(const void* grad_y, int64_t grad_y_stride, const 
         const cudaError_t err = cudaMemsetAsync(grad_weight, 0, size_t(width) * type_bytes(type), s);
         return err == cudaSuccess ? HTGS_OK : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
     }
-    if (!grad_y || !sum || !weight || !rstd || !grad_x) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm_backward: null pointer");
+    if (!grad_y || !x || !weight || !rstd || !grad_x) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_add_rms_norm_backward: null pointer");
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < htgs_add_rms_norm_backward_scratch_bytes(rows, width))
         return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_add_rms_norm_backward: scratch too small or not 16-byte aligned");
-    const NormBackwardArgs a{grad_y, grad_sum, sum, weight, rstd, grad_y_stride, grad_sum_stride, sum_stride, grad_x_stride, grad_x,
+    const NormBackwardArgs a{grad_y, grad_sum, x, residual, weight, rstd, grad_y_stride, grad_sum_stride, x_stride, residual_stride, grad_x_stride, grad_x,
                              static_cast<float*>(scratch), rows, width};
     if (type == HTGS_FLOAT32) backward_typed<float>(a, grad_weight, s);
     else if (type == HTGS_FLOAT16) backward_typed<__half>(a, grad_weight, s);

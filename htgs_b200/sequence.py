@@ -103,32 +103,30 @@ class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         ctx.set_materialize_grads(False)
-        xm = _rows(x)
-        y, total, rstd = _norm_forward(xm, weight, None if residual is None else _rows(residual), eps, True, False)
-        ctx.save_for_backward(xm if total is None else total, weight, rstd)
-        ctx.with_residual = residual is not None
-        return (y.view(x.shape), total.view(x.shape)) if ctx.with_residual else y.view(x.shape)
+        xm, rm = _rows(x), None if residual is None else _rows(residual)
+        y, total, rstd = _norm_forward(xm, weight, rm, eps, True, False)
+        ctx.save_for_backward(xm, rm, weight, rstd)
+        return (y.view(x.shape), total.view(x.shape)) if residual is not None else y.view(x.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_sum=None):
-        total, weight, rstd = ctx.saved_tensors
+        x, residual, weight, rstd = ctx.saved_tensors
         if grad_y is None:
-            if grad_sum is None:
-                return None, None, None, None
             return grad_sum, torch.zeros_like(weight), grad_sum, None
         shape = grad_y.shape
-        rows, width = total.shape
+        rows, width = x.shape
         gy, gs = _rows(grad_y), None if grad_sum is None else _rows(grad_sum)
-        grad_x = torch.empty((rows, width), dtype=total.dtype, device=total.device)
-        grad_weight = torch.empty(width, dtype=total.dtype, device=total.device)
+        grad_x = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+        grad_weight = torch.empty(width, dtype=x.dtype, device=x.device)
         size = _native.lib().htgs_add_rms_norm_backward_scratch_bytes(rows, width)
-        scratch = torch.empty(size, dtype=torch.uint8, device=total.device)
-        _call(total.device, "htgs_add_rms_norm_backward", gy.data_ptr(), gy.stride(0), None if gs is None else gs.data_ptr(),
-              0 if gs is None else gs.stride(0), total.data_ptr(), total.stride(0), weight.contiguous().data_ptr(), rstd.data_ptr(), _TYPES[total.dtype],
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+        _call(x.device, "htgs_add_rms_norm_backward", gy.data_ptr(), gy.stride(0), None if gs is None else gs.data_ptr(),
+              0 if gs is None else gs.stride(0), x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(),
+              0 if residual is None else residual.stride(0), weight.contiguous().data_ptr(), rstd.data_ptr(), _TYPES[x.dtype],
               rows, width, grad_x.data_ptr(), width, grad_weight.data_ptr(), scratch.data_ptr(), size)
         grad_x = grad_x.view(shape)
-        return grad_x, grad_weight, grad_x if ctx.with_residual else None, None
+        return grad_x, grad_weight, None if residual is None else grad_x, None
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:

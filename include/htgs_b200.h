@@ -452,16 +452,17 @@ enum HtgsElementType { HTGS_FLOAT32 = 0, HTGS_FLOAT16 = 1, HTGS_BFLOAT16 = 2 };
  * Root-mean-square norm of x + residual (residual may be NULL):
  *   u = x + residual;  rho = 1 / sqrt(mean(u^2) + eps);  y = u * rho * weight;  sum = u in the stream's type.
  * Either y, or codes and scales (the 8-bit format below, one scale per row and 128 columns; rows of codes begin on 8 bytes for the
- * fast path) must be given.  sum [rows, width] and rstd [rows] (rho) may be NULL; the backward pass needs both.  1 <= width <= 8192.
- * The backward pass takes grad_sum == NULL for zeros; grad_x is the gradient of x and of residual; scratch as the size function says, 16-byte aligned.
+ * fast path) must be given.  sum [rows, width] and rstd [rows] (rho) may be NULL; the backward pass needs rstd.  1 <= width <= 8192.
+ * The backward pass takes the forward's x and residual, and grad_sum == NULL for zeros; grad_x is the gradient of x and of residual; scratch as the size
+ * function says, 16-byte aligned.
  */
 int htgs_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int type, int64_t rows,
                       int32_t width, float eps, void* y, int64_t y_stride, void* sum, int64_t sum_stride, float* rstd, uint8_t* codes,
                       int64_t codes_stride, uint8_t* scales, int64_t scales_stride, void* stream);
 size_t htgs_add_rms_norm_backward_scratch_bytes(int64_t rows, int32_t width);
-int htgs_add_rms_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride, const void* sum,
-                               int64_t sum_stride, const void* weight, const float* rstd, int type, int64_t rows, int32_t width, void* grad_x,
-                               int64_t grad_x_stride, void* grad_weight, void* scratch, size_t scratch_bytes, void* stream);
+int htgs_add_rms_norm_backward(const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride, const void* x, int64_t x_stride,
+                               const void* residual, int64_t residual_stride, const void* weight, const float* rstd, int type, int64_t rows, int32_t width,
+                               void* grad_x, int64_t grad_x_stride, void* grad_weight, void* scratch, size_t scratch_bytes, void* stream);
 
 /*
  * 8-bit matrices: codes [rows, width] of type E4M3, and one power-of-two scale, the byte e + 127 (E8M0), for each block of 128 columns and

@@ -34,8 +34,8 @@ def test_c_entries_check_their_arguments():
         _refused(BAD, norm(**k))
     assert norm(rows=0) == 0
     assert lib.htgs_add_rms_norm_backward_scratch_bytes(0, 8) == 0 and lib.htgs_add_rms_norm_backward_scratch_bytes(100, 8) >= 32
-    _refused(SMALL, lib.htgs_add_rms_norm_backward(64, 8, None, 0, 64, 8, 64, 64, 0, 4, 8, 64, 8, 64, 64, 8, None))
-    _refused(BAD, lib.htgs_add_rms_norm_backward(64, 8, None, 0, 64, 8, 64, 64, 0, 4, 8, 64, 8, None, 64, 1 << 20, None))
+    _refused(SMALL, lib.htgs_add_rms_norm_backward(64, 8, None, 0, 64, 8, None, 0, 64, 64, 0, 4, 8, 64, 8, 64, 64, 8, None))
+    _refused(BAD, lib.htgs_add_rms_norm_backward(64, 8, None, 0, 64, 8, None, 0, 64, 64, 0, 4, 8, 64, 8, None, 64, 1 << 20, None))
     quantize = lambda rps=1, rows=4, codes=64, scales=64, t=0: lib.htgs_quantize_fp8(64, 8, t, rows, 8, rps, codes, 16, scales, 4, None, 0, None, 0, None)  # noqa: E731
     for k in ({"rps": 2}, {"rows": -1}, {"codes": None}, {"scales": None}, {"t": 7}):
         _refused(BAD, quantize(**k))
