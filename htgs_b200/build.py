@@ -114,7 +114,7 @@ def build_bindings(force: bool = False) -> tuple:
     targets = binding_paths()
     jobs = []
     for target, name, extra in ((targets[0], "_C", []), (targets[1], "_C_benchmarking", ["-DHTGS_BINDINGS_BENCHMARKING"])):
-        if force or _stale(target, [BINDINGS_SRC, lib, os.path.normpath(os.path.join(CSRC, "..", "..", "include", "htgs_b200.h"))]):
+        if force or _stale(target, [BINDINGS_SRC, os.path.join(CSRC, "bindings_sequence.h"), lib, os.path.normpath(os.path.join(CSRC, "..", "..", "include", "htgs_b200.h"))]):
             jobs.append((name, [cxx] + flags + extra + [f"-DTORCH_EXTENSION_NAME={name}"] + [f"-I{d}" for d in includes] + [BINDINGS_SRC, "-o", target] + link))
     if jobs:
         os.makedirs(PYBIND_DIR, exist_ok=True)

@@ -15,6 +15,8 @@
 #include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/graph_task.h>
 
@@ -407,6 +409,8 @@ struct ReadyEvent {     // what `torch.cuda.Stream.wait_event` needs: an object 
     void synchronize() const { event->synchronize(); }
 };
 
+#include "bindings_sequence.h"
+
 #endif  // !HTGS_BINDINGS_BENCHMARKING
 
 }  // namespace
@@ -459,5 +463,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         for (auto& entry : tls.contexts) if (device < 0 || entry.first.first == device) out.push_back(reinterpret_cast<uintptr_t>(entry.second));
         return out;
     }, py::arg("device") = -1);
+    sequence::define(m);
 #endif
 }

@@ -20,12 +20,6 @@ struct QuantArgs {
     uint8_t* codes_t; uint8_t* scales_t; int64_t codes_t_stride, scales_t_stride; // transposed; may be null
 };
 
-// N (4 or 8) codes side by side.
-template <int N> __device__ __forceinline__ void store_codes(uint8_t* to, const float (&v)[N], float inverse) {
-    if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(encode4(v[0], v[1], v[2], v[3], inverse), encode4(v[4], v[5], v[6], v[7], inverse));
-    else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = encode4(v[0], v[1], v[2], v[3], inverse);
-}
-
 // A warp takes 32 * VEC columns, VEC side by side in a lane (VEC 1: 128 columns, four of them 32 apart in a lane), of several rows, four at a
 // time, so that enough loads are on their way.
 template <typename T, int VEC>
@@ -57,17 +51,18 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantA
             const int64_t row = row0 + int64_t(down) * r;
             if (row >= a.rows) break;
             uint8_t* codes = a.codes + row * a.codes_stride;
-            float largest = 0.0f;
-            #pragma unroll
-            for (int i = 0; i < kValues; ++i) largest = fmaxf(largest, finite_magnitude(v[r][i]));
+            float largest = largest_magnitude(v[r]);
+            const bool careful = __any_sync(0xffffffffu, largest > FLT_MAX);
+            if (careful) largest = largest_finite(v[r]);
             const int e = scale_exponent(lanes_max<kLanes>(largest));
             const float inverse = inverse_scale(e);
             if (VEC == 1) {
                 #pragma unroll
                 for (int i = 0; i < kValues; ++i)
-                    if (first + 32 * i + lane < a.width) codes[first + 32 * i + lane] = uint8_t(encode2(v[r][i], 0.0f, inverse) & 0xffu);
+                    if (first + 32 * i + lane < a.width) codes[first + 32 * i + lane] = uint8_t(encode2<true>(v[r][i], 0.0f, inverse) & 0xffu);
             } else if (first + lane * VEC < a.width) {
-                store_codes<kValues>(codes + first + lane * VEC, v[r], inverse);
+                if (careful) store_codes<true>(codes + first + lane * VEC, v[r], inverse);
+                else store_codes<false>(codes + first + lane * VEC, v[r], inverse);
             }
             if (lane % kLanes == 0 && at < a.width) a.scales[row * a.scales_stride + at / kScaleBlock] = uint8_t(e + 127);
         }
@@ -110,7 +105,7 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const Quant
             for (int i = 0; i < VEC; ++i) v[j * VEC + i] = f[i];
         }
     };
-    const auto store_row_codes = [&](int r, const float (&v)[8], float inverse) {
+    const auto store_row_codes = [&](int r, const float (&v)[8], float inverse, bool careful) {
         uint8_t* codes = a.codes + (row0 + h * 8 + r) * a.codes_stride + column0;
         #pragma unroll
         for (int j = 0; j < G; ++j) {
@@ -118,22 +113,40 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const Quant
             float f[VEC];
             #pragma unroll
             for (int i = 0; i < VEC; ++i) f[i] = v[j * VEC + i];
-            if (VEC == 1) codes[column(j)] = uint8_t(encode2(f[0], 0.0f, inverse) & 0xffu);
-            else store_codes<VEC>(codes + column(j * VEC), f, inverse);
+            if (careful) store_codes<true>(codes + column(j * VEC), f, inverse);
+            else store_codes<false>(codes + column(j * VEC), f, inverse);
         }
     };
     float most[8] = {};                      // of the thread's columns
     #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        float v[8], largest = 0.0f;
+        float v[8];
         values(r, v);
         #pragma unroll
-        for (int c = 0; c < 8; ++c) { const float m = finite_magnitude(v[c]); largest = fmaxf(largest, m); most[c] = fmaxf(most[c], m); }
-        if (PER_TILE || !a.codes) continue;
-        const int e = scale_exponent(lanes_max<16>(largest));
-        if (h * 8 + r >= rows) continue;
-        store_row_codes(r, v, inverse_scale(e));
-        if (l == 0) a.scales[(row0 + h * 8 + r) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
+        for (int c = 0; c < 8; ++c) most[c] = fmaxf(most[c], fabsf(v[c]));
+    }
+    const bool careful = __syncthreads_or(largest_magnitude(most) > FLT_MAX) != 0;      // an infinity in the tile
+    if (careful) {
+        #pragma unroll
+        for (int c = 0; c < 8; ++c) most[c] = 0.0f;
+        #pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            float v[8];
+            values(r, v);
+            #pragma unroll
+            for (int c = 0; c < 8; ++c) most[c] = fmaxf(most[c], finite_magnitude(v[c]));
+        }
+    }
+    if (!PER_TILE && a.codes) {
+        #pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            float v[8];
+            values(r, v);
+            const int e = scale_exponent(lanes_max<16>(careful ? largest_finite(v) : largest_magnitude(v)));
+            if (h * 8 + r >= rows) continue;
+            store_row_codes(r, v, inverse_scale(e), careful);
+            if (l == 0) a.scales[(row0 + h * 8 + r) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
+        }
     }
     if (!PER_TILE && !a.codes_t) return;
     #pragma unroll
@@ -156,7 +169,7 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const Quant
                 if (h * 8 + r >= rows) break;
                 float v[8];
                 values(r, v);
-                store_row_codes(r, v, inverse_scale(e));
+                store_row_codes(r, v, inverse_scale(e), careful);
             }
             if (threadIdx.x == 0) a.scales[int64_t(blockIdx.y) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
         }
@@ -172,9 +185,15 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const Quant
         float v[8][8];
         #pragma unroll
         for (int r = 0; r < 8; ++r) values(r, v[r]);
-        #pragma unroll
-        for (int c = 0; c < 8; ++c)
-            turned[column(c)][h ^ (column(c) / 8 % 16)] = make_uint2(encode4(v[0][c], v[1][c], v[2][c], v[3][c], most[c]), encode4(v[4][c], v[5][c], v[6][c], v[7][c], most[c]));
+        if (careful) {
+            #pragma unroll
+            for (int c = 0; c < 8; ++c)
+                turned[column(c)][h ^ (column(c) / 8 % 16)] = make_uint2(encode4<true>(v[0][c], v[1][c], v[2][c], v[3][c], most[c]), encode4<true>(v[4][c], v[5][c], v[6][c], v[7][c], most[c]));
+        } else {
+            #pragma unroll
+            for (int c = 0; c < 8; ++c)
+                turned[column(c)][h ^ (column(c) / 8 % 16)] = make_uint2(encode4<false>(v[0][c], v[1][c], v[2][c], v[3][c], most[c]), encode4<false>(v[4][c], v[5][c], v[6][c], v[7][c], most[c]));
+        }
     }
     __syncthreads();
     const bool whole = rows == kScaleBlock && a.codes_t_stride % 16 == 0 && reinterpret_cast<uintptr_t>(a.codes_t) % 16 == 0;
@@ -193,39 +212,55 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const Quant
 // Codes back to values: exact in every output type, except that what leaves the range of 16-bit floats becomes infinite or zero.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kQuantBlock) dequantize_kernel(const uint8_t* codes, int64_t codes_stride, const uint8_t* scales, int64_t scales_stride,
-                                                                int rows_per_scale, int64_t rows, int64_t width, T* out, int64_t out_stride) {
-    const int64_t per_row = (width + VEC - 1) / VEC, total = per_row * rows, step = int64_t(gridDim.x) * kQuantBlock;
-    for (int64_t i = int64_t(blockIdx.x) * kQuantBlock + threadIdx.x; i < total; i += step) {
-        const int64_t row = i / per_row, column = (i - row * per_row) * VEC;
-        const float scale = scale_value(scales[row / rows_per_scale * scales_stride + column / kScaleBlock]);
-        const uint8_t* at = codes + row * codes_stride + column;
-        if (VEC == 8) {
-            const uint2 packed = *reinterpret_cast<const uint2*>(at);
-            const float2 a = decode2(packed.x), b = decode2(packed.x >> 16), c = decode2(packed.y), d = decode2(packed.y >> 16);
-            const float v[8] = {a.x * scale, a.y * scale, b.x * scale, b.y * scale, c.x * scale, c.y * scale, d.x * scale, d.y * scale};
-            if (sizeof(T) == 2) store_floats<T, 8>(out + row * out_stride + column, v);
-            else {
-                *reinterpret_cast<float4*>(out + row * out_stride + column) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4*>(out + row * out_stride + column + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                                                                int shift, int64_t rows, int64_t width, T* out, int64_t out_stride) {
+    const int lane = threadIdx.x & 31;
+    constexpr int R = 4;
+    const uint32_t across = uint32_t((width + 32 * VEC - 1) / (32 * VEC)), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
+    const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;
+    const int64_t column = int64_t(warp % across) * (32 * VEC) + lane * VEC;
+    if (warp >= across * down || column >= width) return;
+    for (int64_t row0 = warp / across; row0 < rows; row0 += int64_t(down) * R) {
+        Pack<uint8_t, VEC> packed[R];
+        uint32_t exponent[R];
+        #pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + int64_t(down) * r;
+            if (row >= rows) break;
+            packed[r] = *reinterpret_cast<const Pack<uint8_t, VEC>*>(codes + row * codes_stride + column);
+            exponent[r] = scales[(row >> shift) * scales_stride + column / kScaleBlock];
+        }
+        #pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + int64_t(down) * r;
+            if (row >= rows) break;
+            const float scale = scale_value(exponent[r]);
+            T* to = out + row * out_stride + column;
+            if constexpr (VEC == 8) {
+                const uint32_t* words = reinterpret_cast<const uint32_t*>(&packed[r]);
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 lo = decode2(words[i]), hi = decode2(words[i] >> 16);
+                    const float v[4] = {lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale};
+                    store_floats<T, 4>(to + 4 * i, v);
+                }
+            } else {
+                *to = from_float<T>(decode2(packed[r].v[0]).x * scale);
             }
-        } else {
-            out[row * out_stride + column] = from_float<T>(decode2(*at).x * scale);
         }
     }
 }
 
-unsigned int capped_blocks(int64_t work, int64_t per_block) {
-    const int64_t blocks = (work + per_block - 1) / per_block;
-    return unsigned(blocks < 148 * 8 ? blocks : 148 * 8);
+// Blocks for warps that take `columns` columns of four rows each: eight per SM at most, and at least one row's worth.
+unsigned int blocks_for(int64_t rows, int64_t width, int columns) {
+    const int64_t across = (width + columns - 1) / columns, per_block = kQuantBlock / 32;
+    int64_t blocks = (across * ((rows + 3) / 4) + per_block - 1) / per_block;
+    if (blocks > 148 * 8) blocks = 148 * 8;
+    const int64_t least = (across + per_block - 1) / per_block;
+    return unsigned(blocks > least ? blocks : least);
 }
 
 template <typename T, int VEC> void launch_rows(const QuantArgs& a, cudaStream_t stream) {
-    constexpr int kColumns = VEC == 1 ? kScaleBlock : 32 * VEC;
-    const int64_t across = (a.width + kColumns - 1) / kColumns, warps = across * ((a.rows + 3) / 4);
-    int64_t blocks = (warps + kQuantBlock / 32 - 1) / (kQuantBlock / 32);
-    if (blocks > 148 * 8) blocks = 148 * 8;
-    if (blocks * (kQuantBlock / 32) < across) blocks = (across + kQuantBlock / 32 - 1) / (kQuantBlock / 32);     // at least one row at a time
-    quantize_rows_kernel<T, VEC><<<unsigned(blocks), kQuantBlock, 0, stream>>>(a);
+    quantize_rows_kernel<T, VEC><<<blocks_for(a.rows, a.width, VEC == 1 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream>>>(a);
 }
 template <typename T, int VEC> void launch_tiles(const QuantArgs& a, int rows_per_scale, cudaStream_t stream) {
     const dim3 grid(unsigned((a.width + kScaleBlock - 1) / kScaleBlock), unsigned((a.rows + kScaleBlock - 1) / kScaleBlock));
@@ -239,13 +274,13 @@ template <typename T> void quantize_typed(const QuantArgs& a, int rows_per_scale
     else { if (wide) launch_tiles<T, V>(a, rows_per_scale, stream); else launch_tiles<T, 1>(a, rows_per_scale, stream); }
 }
 
+template <typename T, int VEC> void launch_dequantize(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
+    dequantize_kernel<T, VEC><<<blocks_for(m.rows, m.width, 32 * VEC), kQuantBlock, 0, stream>>>(
+        m.codes, m.codes_stride, m.scales, m.scales_stride, m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);
+}
 template <typename T> void dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
-    if (m.width % 8 == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, 8) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16))
-        dequantize_kernel<T, 8><<<capped_blocks(m.rows * (m.width / 8), kQuantBlock), kQuantBlock, 0, stream>>>(
-            m.codes, m.codes_stride, m.scales, m.scales_stride, m.rows_per_scale, m.rows, m.width, static_cast<T*>(out), out_stride);
-    else
-        dequantize_kernel<T, 1><<<capped_blocks(m.rows * m.width, kQuantBlock), kQuantBlock, 0, stream>>>(
-            m.codes, m.codes_stride, m.scales, m.scales_stride, m.rows_per_scale, m.rows, m.width, static_cast<T*>(out), out_stride);
+    if (m.width % 8 == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, 8) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16)) launch_dequantize<T, 8>(m, out, out_stride, stream);
+    else launch_dequantize<T, 1>(m, out, out_stride, stream);
 }
 
 }  // namespace

@@ -116,9 +116,12 @@ __global__ void __launch_bounds__(kNormBlock) norm_kernel(const NormArgs a) {
         for (int j = 0; j < G; j += kGroups) {
             float largest = 0.0f;
             #pragma unroll
-            for (int k = 0; k < kGroups; ++k) {
+            for (int k = 0; k < kGroups; ++k) largest = largest_magnitude(u[j + k], largest);
+            const bool careful = __any_sync(0xffffffffu, largest > FLT_MAX);
+            if (careful) {
+                largest = 0.0f;
                 #pragma unroll
-                for (int i = 0; i < VEC; ++i) largest = fmaxf(largest, finite_magnitude(u[j + k][i]));
+                for (int k = 0; k < kGroups; ++k) largest = largest_finite(u[j + k], largest);
             }
             const int e = scale_exponent(lanes_max<kLanes>(largest));
             const float inverse = inverse_scale(e);
@@ -126,14 +129,8 @@ __global__ void __launch_bounds__(kNormBlock) norm_kernel(const NormArgs a) {
             for (int k = 0; k < kGroups; ++k) {
                 const int column = base + (32 * (j + k) + lane) * VEC;
                 if (column >= a.width) continue;
-                const float* v = u[j + k];
-                if (VEC == 8)
-                    *reinterpret_cast<uint2*>(codes + column) = make_uint2(encode4(v[0], v[1 % VEC], v[2 % VEC], v[3 % VEC], inverse),
-                                                                           encode4(v[4 % VEC], v[5 % VEC], v[6 % VEC], v[7 % VEC], inverse));
-                else if (VEC == 4)
-                    *reinterpret_cast<uint32_t*>(codes + column) = encode4(v[0], v[1 % VEC], v[2 % VEC], v[3 % VEC], inverse);
-                else
-                    codes[column] = uint8_t(encode2(v[0], 0.0f, inverse) & 0xffu);
+                if (careful) store_codes<true>(codes + column, u[j + k], inverse);
+                else store_codes<false>(codes + column, u[j + k], inverse);
                 if (k == 0 && lane % kLanes == 0) scales[column / kScaleBlock] = uint8_t(e + 127);
             }
         }

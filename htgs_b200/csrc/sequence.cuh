@@ -80,14 +80,33 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {                   
     return byte == 255u ? __uint_as_float(0x7fffffffu) : byte == 0u ? __uint_as_float(0x400000u) : __uint_as_float(byte << 23);
 }
 
-// Two codes in one: v * 2^-e to the nearest E4M3 value, ties to even; what is not finite becomes NaN.
-__device__ __forceinline__ uint32_t encode2(float lo, float hi, float inverse) {
-    lo = fabsf(lo) <= FLT_MAX ? lo * inverse : __uint_as_float(0x7fffffffu);
-    hi = fabsf(hi) <= FLT_MAX ? hi * inverse : __uint_as_float(0x7fffffffu);
-    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+// Codes v * 2^-e to the nearest E4M3 value, ties to even; NaN becomes NaN.  CAREFUL: infinities do too (the conversion takes them for 448).
+template <bool CAREFUL> __device__ __forceinline__ uint32_t encode2(float lo, float hi, float inverse) {
+    if (CAREFUL) {
+        lo = fabsf(lo) <= FLT_MAX ? lo : __uint_as_float(0x7fffffffu);
+        hi = fabsf(hi) <= FLT_MAX ? hi : __uint_as_float(0x7fffffffu);
+    }
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo * inverse, hi * inverse), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inverse) {
-    return encode2(a, b, inverse) | encode2(c, d, inverse) << 16;
+template <bool CAREFUL> __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inverse) {
+    return encode2<CAREFUL>(a, b, inverse) | encode2<CAREFUL>(c, d, inverse) << 16;
+}
+// N codes side by side (N 1, 4 or 8).
+template <bool CAREFUL, int N> __device__ __forceinline__ void store_codes(uint8_t* to, const float (&v)[N], float inverse) {
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(encode4<CAREFUL>(v[0], v[1], v[2], v[3], inverse), encode4<CAREFUL>(v[4], v[5], v[6], v[7], inverse));
+    else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = encode4<CAREFUL>(v[0], v[1], v[2], v[3], inverse);
+    else *to = uint8_t(encode2<CAREFUL>(v[0], 0.0f, inverse) & 0xffu);
+}
+// Largest magnitude; a NaN says nothing.  Infinite where one is, which is when the maximum is taken again over finite_magnitude, and CAREFUL codes follow.
+template <int N> __device__ __forceinline__ float largest_magnitude(const float (&v)[N], float so_far = 0.0f) {
+    #pragma unroll
+    for (int i = 0; i < N; ++i) so_far = fmaxf(so_far, fabsf(v[i]));
+    return so_far;
+}
+template <int N> __device__ __forceinline__ float largest_finite(const float (&v)[N], float so_far = 0.0f) {
+    #pragma unroll
+    for (int i = 0; i < N; ++i) so_far = fmaxf(so_far, finite_magnitude(v[i]));
+    return so_far;
 }
 __device__ __forceinline__ float2 decode2(uint32_t codes) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3);

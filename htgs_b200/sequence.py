@@ -25,6 +25,12 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _BLOCK = 128
 
 
+def _compiled():
+    """The compiled extension module where it is the active binding, else None: the functions here then do its work over ctypes."""
+    mods = _native.pybind_modules()
+    return mods[0] if mods else None
+
+
 def _check(t, name: str, dtype=None, device=None) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -133,6 +139,9 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     """(y, stream) with stream = x + residual and y = stream / sqrt(mean(stream^2) + eps) * weight over the last dimension (1 to 8192
     values).  Without a residual the stream is x itself.  x, weight and residual have one type.  y is computed from the
     unrounded sum.  Differentiable in x, weight and residual."""
+    compiled = _compiled()
+    if compiled:
+        return compiled.add_rms_norm(x, weight, residual, eps)
     _check_norm(x, weight, residual)
     if _wants_grad(x, weight, residual):
         return _AddRmsNorm.apply(x, weight, residual, float(eps)) if residual is not None else (_AddRmsNorm.apply(x, weight, None, float(eps)), x)
@@ -144,6 +153,10 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
                      eps: float = 1e-6) -> Tuple["Fp8Matrix", torch.Tensor]:
     """`add_rms_norm` whose y leaves as an `Fp8Matrix` of x.shape[:-1].numel() rows, quantised from 32-bit values with a scale for each row and
     128 columns: what `fp8_matmul` takes.  For inference: it has no gradient and refuses inputs that want one."""
+    compiled = _compiled()
+    if compiled:
+        codes, scales, total = compiled.add_rms_norm_fp8(x, weight, residual, eps)
+        return _fp8(codes, scales, 1), total
     _check_norm(x, weight, residual)
     if _wants_grad(x, weight, residual):
         raise RuntimeError("add_rms_norm_fp8 has no gradient: use add_rms_norm and fp8_linear in training, or torch.no_grad()")
@@ -161,6 +174,11 @@ class Fp8Matrix:
     __slots__ = ("codes", "scales", "rows_per_scale")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows_per_scale: int = 1):
+        compiled = _compiled()
+        if compiled:
+            compiled.check_fp8_matrix(codes, scales, rows_per_scale)
+            self.codes, self.scales, self.rows_per_scale = codes, scales, rows_per_scale
+            return
         _check(codes, "codes", torch.float8_e4m3fn)
         _check(scales, "scales", torch.float8_e8m0fnu, codes.device)
         if rows_per_scale not in (1, _BLOCK):
@@ -194,6 +212,9 @@ class Fp8Matrix:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values that the codes stand for; bfloat16 and float32 hold all of them exactly, except that float32's and
         bfloat16's largest exponent bounds them."""
+        compiled = _compiled()
+        if compiled:
+            return compiled.dequantize_fp8(self.codes, self.scales, self.rows_per_scale, dtype)
         if dtype not in _TYPES:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
         out = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
@@ -201,13 +222,17 @@ class Fp8Matrix:
         return out
 
 
-def _empty_fp8(rows: int, width: int, rows_per_scale: int, device) -> Fp8Matrix:
+def _fp8(codes: torch.Tensor, scales: torch.Tensor, rows_per_scale: int) -> Fp8Matrix:
+    """An `Fp8Matrix` of tensors that need no check."""
     m = Fp8Matrix.__new__(Fp8Matrix)
-    blocks = -(-width // _BLOCK)
-    m.codes = torch.empty_strided((rows, width), (-(-width // 16) * 16, 1), dtype=torch.float8_e4m3fn, device=device)
-    m.scales = torch.empty_strided((-(-rows // rows_per_scale), blocks), (-(-blocks // 4) * 4, 1), dtype=torch.float8_e8m0fnu, device=device)
-    m.rows_per_scale = rows_per_scale
+    m.codes, m.scales, m.rows_per_scale = codes, scales, rows_per_scale
     return m
+
+
+def _empty_fp8(rows: int, width: int, rows_per_scale: int, device) -> Fp8Matrix:
+    blocks = -(-width // _BLOCK)
+    return _fp8(torch.empty_strided((rows, width), (-(-width // 16) * 16, 1), dtype=torch.float8_e4m3fn, device=device),
+                torch.empty_strided((-(-rows // rows_per_scale), blocks), (-(-blocks // 4) * 4, 1), dtype=torch.float8_e8m0fnu, device=device), rows_per_scale)
 
 
 def _quantize(x: torch.Tensor, rows_per_scale: int, straight: bool, transposed: bool):
@@ -224,6 +249,9 @@ def quantize_fp8(x: torch.Tensor, rows_per_scale: int = 1, transpose: bool = Fal
     """The last dimension's rows of x (or, with `transpose`, the columns of the matrix x) as 8-bit codes: each block of 128 columns and
     `rows_per_scale` rows (1: activations, 128: weights) gets the least power of two with which its largest finite value is at most 448, and values are
     rounded to nearest even.  Infinities and NaN become NaN.  No gradient flows through it."""
+    compiled = _compiled()
+    if compiled:
+        return _fp8(*compiled.quantize_fp8(x, rows_per_scale, transpose), rows_per_scale)
     _check(x, "x")
     if rows_per_scale not in (1, _BLOCK):
         raise ValueError("rows_per_scale must be 1 or 128")
@@ -245,6 +273,11 @@ def fp8_matmul(x, weight: Fp8Matrix, dtype: Optional[torch.dtype] = None) -> tor
     inference: it refuses an x that wants a gradient (`fp8_linear` has one)."""
     if not isinstance(weight, Fp8Matrix):
         raise TypeError("weight must be an Fp8Matrix")
+    compiled = _compiled()
+    if compiled:
+        if isinstance(x, Fp8Matrix):
+            return compiled.fp8_matmul(x.codes, x.scales, x.rows_per_scale, weight.codes, weight.scales, weight.rows_per_scale, dtype)
+        return compiled.fp8_matmul(x, None, 1, weight.codes, weight.scales, weight.rows_per_scale, dtype)
     if dtype is not None and dtype not in _TYPES:
         raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     if isinstance(x, Fp8Matrix):
@@ -287,6 +320,9 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """x [..., width] times the transpose of weight [out, width], with 8-bit operands: x quantised per row and 128 columns, weight per block of
     128 x 128.  Differentiable: grad_y is quantised along `out` for the gradient of x, and grad_y and x along the rows for the gradient of
     weight; quantisation itself counts as the identity."""
+    compiled = _compiled()
+    if compiled:
+        return compiled.fp8_linear(x, weight)
     _check(x, "x")
     _check(weight, "weight", x.dtype, x.device)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
@@ -355,6 +391,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, initial: Optional[torch.Tens
     begin the sequences (sequences may be empty).  `initial` [sequences, width] float32 is the state in front of each sequence (default zeros), `last` the float32
     state behind it.  With `reverse` each sequence is gone through from its last row to its first.  States are 32-bit; h has x's
     type.  Differentiable in x, gate and initial."""
+    compiled = _compiled()
+    if compiled:
+        return compiled.gated_scan(x, gate, initial, offsets, reverse)
     _check(x, "x")
     _check(gate, "gate", x.dtype, x.device)
     if gate.shape != x.shape or x.dim() not in (2, 3):
@@ -385,6 +424,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, initial: Optional[torch.Tens
 def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
     """One step of `gated_scan` for each row: `state` [rows, width] float32 becomes a * state + (1 - a) * x, in place, and is returned in x's type.  For
     inference: it refuses inputs that want a gradient."""
+    compiled = _compiled()
+    if compiled:
+        return compiled.gated_scan_step(x, gate, state)
     _check(x, "x")
     _check(gate, "gate", x.dtype, x.device)
     _check(state, "state", torch.float32, x.device)
