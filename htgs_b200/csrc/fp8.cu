@@ -23,7 +23,7 @@ struct QuantArgs {
 // A warp takes 32 * VEC columns, VEC side by side in a lane (VEC 1: 128 columns, four of them 32 apart in a lane), of several rows, four at a
 // time, so that enough loads are on their way.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const QuantArgs a) {
     const int lane = threadIdx.x & 31;
     constexpr int kColumns = VEC == 1 ? kScaleBlock : 32 * VEC, kValues = VEC == 1 ? 4 : VEC, kLanes = VEC == 8 ? 16 : 32, R = 4;
     const uint32_t across = uint32_t((a.width + kColumns - 1) / kColumns), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
@@ -31,19 +31,18 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantA
     if (warp >= across * down) return;
     const int64_t first = int64_t(warp % across) * kColumns, at = first + (lane / kLanes) * kScaleBlock;
     for (int64_t row0 = warp / across; row0 < a.rows; row0 += int64_t(down) * R) {
-        float v[R][kValues];
+        Pack<T, VEC> raw[R][kValues / VEC];          // as they are in memory: half the registers of 32-bit values
         #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + int64_t(down) * r;
-            const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-            if (VEC == 1) {
-                #pragma unroll
-                for (int i = 0; i < kValues; ++i) v[r][i] = row < a.rows && first + 32 * i + lane < a.width ? to_float<T>(x[first + 32 * i + lane]) : 0.0f;
-            } else if (row < a.rows && first + lane * VEC < a.width) {
-                load_floats<T, kValues>(x + first + lane * VEC, v[r]);
-            } else {
-                #pragma unroll
-                for (int i = 0; i < kValues; ++i) v[r][i] = 0.0f;
+            const T* x = static_cast<const T*>(a.x) + row * a.x_stride + first + lane * VEC;
+            #pragma unroll
+            for (int i = 0; i < kValues / VEC; ++i) {
+                if (row < a.rows && first + 32 * i + lane * VEC < a.width) raw[r][i] = *reinterpret_cast<const Pack<T, VEC>*>(x + 32 * i);
+                else {
+                    #pragma unroll
+                    for (int k = 0; k < VEC; ++k) raw[r][i].v[k] = from_float<T>(0.0f);
+                }
             }
         }
         #pragma unroll
@@ -51,18 +50,26 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantA
             const int64_t row = row0 + int64_t(down) * r;
             if (row >= a.rows) break;
             uint8_t* codes = a.codes + row * a.codes_stride;
-            float largest = largest_magnitude(v[r]);
+            float v[kValues];
+            #pragma unroll
+            for (int i = 0; i < kValues / VEC; ++i) {
+                float f[VEC];
+                to_floats<T, VEC>(raw[r][i], f);
+                #pragma unroll
+                for (int k = 0; k < VEC; ++k) v[i * VEC + k] = f[k];
+            }
+            float largest = largest_magnitude(v);
             const bool careful = __any_sync(0xffffffffu, largest > FLT_MAX);
-            if (careful) largest = largest_finite(v[r]);
+            if (careful) largest = largest_finite(v);
             const int e = scale_exponent(lanes_max<kLanes>(largest));
             const float inverse = inverse_scale(e);
             if (VEC == 1) {
                 #pragma unroll
                 for (int i = 0; i < kValues; ++i)
-                    if (first + 32 * i + lane < a.width) codes[first + 32 * i + lane] = uint8_t(encode2<true>(v[r][i], 0.0f, inverse) & 0xffu);
+                    if (first + 32 * i + lane < a.width) codes[first + 32 * i + lane] = uint8_t(encode2<true>(v[i], 0.0f, inverse) & 0xffu);
             } else if (first + lane * VEC < a.width) {
-                if (careful) store_codes<true>(codes + first + lane * VEC, v[r], inverse);
-                else store_codes<false>(codes + first + lane * VEC, v[r], inverse);
+                if (careful) store_codes<true>(codes + first + lane * VEC, v, inverse);
+                else store_codes<false>(codes + first + lane * VEC, v, inverse);
             }
             if (lane % kLanes == 0 && at < a.width) a.scales[row * a.scales_stride + at / kScaleBlock] = uint8_t(e + 127);
         }
@@ -211,7 +218,7 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const Quant
 
 // Codes back to values: exact in every output type, except that what leaves the range of 16-bit floats becomes infinite or zero.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kQuantBlock) dequantize_kernel(const uint8_t* codes, int64_t codes_stride, const uint8_t* scales, int64_t scales_stride,
+__global__ void __launch_bounds__(kQuantBlock, 6) dequantize_kernel(const uint8_t* codes, int64_t codes_stride, const uint8_t* scales, int64_t scales_stride,
                                                                 int shift, int64_t rows, int64_t width, T* out, int64_t out_stride) {
     const int lane = threadIdx.x & 31;
     constexpr int R = 4;
@@ -235,13 +242,18 @@ __global__ void __launch_bounds__(kQuantBlock) dequantize_kernel(const uint8_t* 
             if (row >= rows) break;
             const float scale = scale_value(exponent[r]);
             T* to = out + row * out_stride + column;
-            if constexpr (VEC == 8) {
+            if constexpr (VEC == 16) {
+                constexpr int V = 16 / int(sizeof(T));
                 const uint32_t* words = reinterpret_cast<const uint32_t*>(&packed[r]);
                 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float2 lo = decode2(words[i]), hi = decode2(words[i] >> 16);
-                    const float v[4] = {lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale};
-                    store_floats<T, 4>(to + 4 * i, v);
+                for (int i = 0; i < 16; i += V) {
+                    float v[V];
+                    #pragma unroll
+                    for (int k = 0; k < V; k += 2) {
+                        const float2 f = decode2(words[(i + k) / 4] >> ((i + k) % 4 * 8));
+                        v[k] = f.x * scale; v[k + 1] = f.y * scale;
+                    }
+                    store_floats<T, V>(to + i, v);
                 }
             } else {
                 *to = from_float<T>(decode2(packed[r].v[0]).x * scale);
@@ -250,11 +262,11 @@ __global__ void __launch_bounds__(kQuantBlock) dequantize_kernel(const uint8_t* 
     }
 }
 
-// Blocks for warps that take `columns` columns of four rows each: eight per SM at most, and at least one row's worth.
+// Blocks for warps that take `columns` columns of four rows each: as many as the SMs hold at once, and at least one row's worth.
 unsigned int blocks_for(int64_t rows, int64_t width, int columns) {
     const int64_t across = (width + columns - 1) / columns, per_block = kQuantBlock / 32;
     int64_t blocks = (across * ((rows + 3) / 4) + per_block - 1) / per_block;
-    if (blocks > 148 * 8) blocks = 148 * 8;
+    if (blocks > 148 * 6) blocks = 148 * 6;
     const int64_t least = (across + per_block - 1) / per_block;
     return unsigned(blocks > least ? blocks : least);
 }
@@ -279,7 +291,7 @@ template <typename T, int VEC> void launch_dequantize(const HtgsFp8Matrix& m, vo
         m.codes, m.codes_stride, m.scales, m.scales_stride, m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);
 }
 template <typename T> void dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
-    if (m.width % 8 == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, 8) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16)) launch_dequantize<T, 8>(m, out, out_stride, stream);
+    if (m.width % 16 == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, 16) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16)) launch_dequantize<T, 16>(m, out, out_stride, stream);
     else launch_dequantize<T, 1>(m, out, out_stride, stream);
 }
 

@@ -124,12 +124,20 @@ template <int LANES> __device__ __forceinline__ float lanes_max(float v) {
     return v;
 }
 
-// Blocks of a cluster: the float at this block's shared address in block `block`, and a barrier of all their threads.
-__device__ __forceinline__ float peer_float(uint32_t address, uint32_t block) {
+// Blocks of a cluster: what block `block` has at this block's shared address `address`, and a barrier of all their threads.
+__device__ __forceinline__ uint32_t peer_address(uint32_t address, uint32_t block) {
     uint32_t there;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(block));
+    return there;
+}
+__device__ __forceinline__ float peer_float(uint32_t address, uint32_t block) {
     float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_address(address, block)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_float4(uint32_t address, uint32_t block) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_address(address, block)) : "memory");
     return v;
 }
 __device__ __forceinline__ void cluster_barrier() {
