@@ -286,6 +286,11 @@ Tensor fp8_linear(const Tensor& x, const Tensor& weight) {
 
 // ---- recurrence -------------------------------------------------------------------------------------------------------------------
 
+Tensor scan_rows(const Tensor& t) {           // row strides are at most 2^22
+    const Tensor m = rows_of(t);
+    return m.stride(0) > (1 << 22) ? m.clone(at::MemoryFormat::Contiguous) : m;
+}
+
 HtgsScan scan_of(const Tensor& x, const Tensor& gate, const Tensor& initial, const Tensor& offsets, int64_t sequences, bool reverse) {
     return {x.data_ptr(), gate.data_ptr(), initial.defined() ? initial.data_ptr<float>() : nullptr, offsets.defined() ? offsets.data_ptr<int32_t>() : nullptr, x.stride(0),
             gate.stride(0), x.size(0), int32_t(x.size(1)), int32_t(sequences), type_of(x.scalar_type()), reverse ? 1 : 0};
@@ -305,7 +310,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
         const Tensor initial = given_initial ? *given_initial : Tensor(), offsets = given_offsets ? *given_offsets : Tensor();
         const c10::cuda::CUDAGuard guard(x.device());
         ctx->set_materialize_grads(false);
-        const Tensor xm = rows_of(x), gm = rows_of(gate), start = initial.defined() ? initial.contiguous() : Tensor();
+        const Tensor xm = scan_rows(x), gm = scan_rows(gate), start = initial.defined() ? initial.contiguous() : Tensor();
         Tensor h = torch::empty(x.sizes(), x.options().requires_grad(false)), last = floats(x, {sequences, xm.size(1)});
         Tensor states = floats(x, {int64_t(htgs_gated_scan_state_bytes(xm.size(0), int32_t(xm.size(1))) / 4)});
         scan_into(xm, gm, start, offsets, sequences, reverse, h, last, &states);
@@ -323,7 +328,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
         const auto sizes = ctx->saved_data["sizes"].toIntVector();
         const c10::cuda::CUDAGuard guard(x.device());
         const int64_t rows = x.size(0), width = x.size(1);
-        const Tensor gh = grads[0].defined() ? rows_of(grads[0]) : torch::zeros({rows, width}, x.options());
+        const Tensor gh = grads[0].defined() ? scan_rows(grads[0]) : torch::zeros({rows, width}, x.options());
         const Tensor gl = grads[1].defined() ? grads[1].contiguous() : Tensor();
         Tensor grad_x = torch::empty(sizes, x.options()), grad_gate = torch::empty(sizes, x.options()), grad_initial;
         if (ctx->saved_data["initial"].toBool()) grad_initial = torch::empty_like(initial);
@@ -362,7 +367,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const
     }
     const c10::cuda::CUDAGuard guard(x.device());
     Tensor h = torch::empty(x.sizes(), x.options().requires_grad(false)), last = floats(x, {sequences, width});
-    scan_into(rows_of(x), rows_of(gate), start.defined() ? start.contiguous() : start, off, sequences, reverse, h, last, nullptr);
+    scan_into(scan_rows(x), scan_rows(gate), start.defined() ? start.contiguous() : start, off, sequences, reverse, h, last, nullptr);
     return {h, last};
 }
 

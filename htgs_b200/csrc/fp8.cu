@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const Qua
 // 128: the eight bytes of half-warp h and column c lie in slot h ^ (c / 8 % 16) of the column's sixteen, which spreads the 16
 // lanes of a store over all banks.  PER_TILE: one scale for the whole tile.  VEC: columns a load takes; a thread's eight are (8 / VEC) groups 16 * VEC apart.
 template <typename T, int VEC, bool PER_TILE>
-__global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(kQuantBlock, 2) quantize_tiles_kernel(const QuantArgs a) {
     __shared__ float column_largest[16][kScaleBlock];
     __shared__ float column_all[kScaleBlock];
     __shared__ __align__(16) uint2 turned[kScaleBlock][16];
@@ -189,17 +189,12 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_tiles_kernel(const Quant
         for (int c = 0; c < 8; ++c) most[c] = inverse_scale(scale_exponent(column_all[column(c)]));
     }
     {
-        float v[8][8];
+        const auto one = [&](int r, int c) { return to_float<T>(raw[r][c / VEC].v[c % VEC]); };
         #pragma unroll
-        for (int r = 0; r < 8; ++r) values(r, v[r]);
-        if (careful) {
-            #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                turned[column(c)][h ^ (column(c) / 8 % 16)] = make_uint2(encode4<true>(v[0][c], v[1][c], v[2][c], v[3][c], most[c]), encode4<true>(v[4][c], v[5][c], v[6][c], v[7][c], most[c]));
-        } else {
-            #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                turned[column(c)][h ^ (column(c) / 8 % 16)] = make_uint2(encode4<false>(v[0][c], v[1][c], v[2][c], v[3][c], most[c]), encode4<false>(v[4][c], v[5][c], v[6][c], v[7][c], most[c]));
+        for (int c = 0; c < 8; ++c) {
+            uint2& to = turned[column(c)][h ^ (column(c) / 8 % 16)];
+            if (careful) to = make_uint2(encode4<true>(one(0, c), one(1, c), one(2, c), one(3, c), most[c]), encode4<true>(one(4, c), one(5, c), one(6, c), one(7, c), most[c]));
+            else to = make_uint2(encode4<false>(one(0, c), one(1, c), one(2, c), one(3, c), most[c]), encode4<false>(one(4, c), one(5, c), one(6, c), one(7, c), most[c]));
         }
     }
     __syncthreads();

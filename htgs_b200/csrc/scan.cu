@@ -17,21 +17,23 @@ namespace htgs {
 
 namespace {
 
-constexpr int kChunk = 128;                  // rows
-constexpr int kForwardSteps = 16;            // rows a warp takes, one after the other
-constexpr int kBackwardSteps = 8;
-constexpr int kCarryWarps = 32;
+// A block takes a chunk of 32 or 64 channels; each of its warps takes some rows of it.
+constexpr int kChunk = 64;                                                       // rows
+constexpr int kComposeSteps = 16, kComposeWarps = kChunk / kComposeSteps;
+constexpr int kApplySteps = 8, kApplyWarps = kChunk / kApplySteps;
+constexpr int kKept = 8;                     // a state for every so many rows is kept for the backward pass
+constexpr int kCarryWarps = 32, kCarryChannels = 8, kCarryRun = 16;
+static_assert(kApplySteps == kKept, "a warp of the backward pass begins with a state that was kept");
 
 struct ScanArgs {
     HtgsScan in;
-    int64_t chunks;
-    int channel_tiles;
+    int chunks, channel_tiles;
     float2* composed;                        // [chunks, width]
-    float* states;                           // [chunks, width] state in front of each chunk; the first is not kept
+    float* carried;                          // [chunks, width] state in front of each chunk (backward: E behind it); nothing where there is one chunk
+    float* states;                           // [ceil(rows / 8), width] state in front of every eight rows, or null
     void* h; int64_t h_stride; float* last;
     const void* grad_h; int64_t grad_h_stride; const float* grad_last;
     void* grad_x; int64_t grad_x_stride; void* grad_gate; int64_t grad_gate_stride; float* grad_initial;
-    float* grad_states;                      // [chunks, width] E behind each chunk; that of the last is not kept
 };
 
 // V channels side by side: one float, or two in a register pair (one instruction for both).
@@ -146,47 +148,62 @@ template <int V> __device__ __forceinline__ void store_state(float* states, int6
     for (int k = 0; k < V; ++k) states[at + k] = n[k];
 }
 
-// Where a thread works: V channels side by side, STEPS rows from p0 on, `count` of which exist; row r of them is r * step rows behind the first.
-template <int V, int STEPS> struct Place {
-    int lane, warp, channel, count;
-    int64_t chunk, p0, row0;
-    int step;
-    bool inside;
-    __device__ __forceinline__ explicit Place(const ScanArgs& a) {
+// Where a thread works: V channels side by side, STEPS rows from position p0 on (positions count rows in the order of the recurrence), `count` of which exist.
+// Addresses are a pointer to the chunk's row i, the same for the whole block, and the thread's own 32-bit offset to its warp's rows and channel.
+template <int V, int STEPS, int WARPS> struct Place {
+    int lane, warp, channel, count, p0, chunk, lowest, row;       // lowest: the chunk's lowest row (it may lie in front of the first); row: the warp's lowest, from there
+    bool inside, reverse;
+    __device__ __forceinline__ explicit Place(const ScanArgs& a, bool from_end = false) {
+        constexpr int kRows = STEPS * WARPS;
         lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
-        chunk = blockIdx.x / unsigned(a.channel_tiles);
+        const int at = int(blockIdx.x / unsigned(a.channel_tiles));
+        chunk = from_end ? a.chunks - 1 - at : at;
         channel = (int(blockIdx.x % unsigned(a.channel_tiles)) * 32 + lane) * V;
         inside = channel < a.in.width;
-        p0 = chunk * kChunk + warp * STEPS;
-        count = int(max(int64_t(0), min(int64_t(STEPS), a.in.rows - p0)));
-        row0 = a.in.reverse ? a.in.rows - 1 - p0 : p0;
-        step = a.in.reverse ? -1 : 1;
+        reverse = a.in.reverse != 0;
+        const int rows = int(a.in.rows), begin = chunk * kRows;
+        p0 = begin + warp * STEPS;
+        count = max(0, min(STEPS, rows - p0));
+        lowest = reverse ? rows - begin - kRows : begin;
+        row = reverse ? kRows - STEPS - warp * STEPS : warp * STEPS;
     }
+    __device__ __forceinline__ bool whole() const { return count == STEPS && inside; }
     __device__ __forceinline__ int64_t state_at(const ScanArgs& a, int sequence) const { return int64_t(sequence) * a.in.width + channel; }
 };
 
-template <typename T, int V, int STEPS>
-__device__ __forceinline__ void load_rows(const void* base, int64_t stride, const Place<V, STEPS>& at, Pack<T, V> (&out)[STEPS]) {
-    const T* p = static_cast<const T*>(base) + at.row0 * stride + at.channel;
-    const int64_t step = at.step * stride;
-    if (at.count == STEPS && at.inside) {
-        #pragma unroll
-        for (int i = 0; i < STEPS; ++i) out[i] = *reinterpret_cast<const Pack<T, V>*>(p + i * step);
-    } else {
-        #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            if (at.inside && i < at.count) out[i] = *reinterpret_cast<const Pack<T, V>*>(p + i * step);
-            else {
-                #pragma unroll
-                for (int k = 0; k < V; ++k) out[i].v[k] = from_float<T>(0.0f);
+// A matrix's values at a place.
+template <typename T, int V> struct Rows {
+    char* chunk;                              // its lowest row
+    int64_t stride;                           // bytes
+    uint32_t offset;                          // of the thread's channel in the warp's lowest row
+    template <typename P> __device__ __forceinline__ Rows(const void* base, int64_t row_stride, const P& at) : stride(row_stride * int64_t(sizeof(T))) {
+        chunk = static_cast<char*>(const_cast<void*>(base)) + at.lowest * stride;
+        offset = uint32_t(at.row) * uint32_t(stride) + uint32_t(at.channel) * uint32_t(sizeof(T));
+    }
+    template <int STEPS> __device__ __forceinline__ Pack<T, V>* at(int i, bool reverse) const {
+        return reinterpret_cast<Pack<T, V>*>(chunk + (reverse ? STEPS - 1 - i : i) * stride + offset);
+    }
+    template <typename P, int STEPS> __device__ __forceinline__ void load(const P& place, Pack<T, V> (&out)[STEPS]) const {
+        if (place.whole()) {
+            #pragma unroll
+            for (int i = 0; i < STEPS; ++i) out[i] = *at<STEPS>(i, place.reverse);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                if (place.inside && i < place.count) out[i] = *at<STEPS>(i, place.reverse);
+                else {
+                    #pragma unroll
+                    for (int k = 0; k < V; ++k) out[i].v[k] = from_float<T>(0.0f);
+                }
             }
         }
     }
-}
+    template <int STEPS> __device__ __forceinline__ void store(int i, bool reverse, Num<V> n) const { store_number<T, V>(reinterpret_cast<T*>(at<STEPS>(i, reverse)), n); }
+};
 
 // The warp's steps as h -> a h + b, and all of them composed (A, H).  The loop for rows in the middle of a sequence asks for nothing else.
-template <typename T, int V, int STEPS>
-__device__ __forceinline__ void forward_steps(const ScanArgs& args, const Place<V, STEPS>& at, const Edges& edges, const Pack<T, V> (&x)[STEPS],
+template <typename T, int V, int STEPS, typename P>
+__device__ __forceinline__ void forward_steps(const ScanArgs& args, const P& at, const Edges& edges, const Pack<T, V> (&x)[STEPS],
                                               const Pack<T, V> (&g)[STEPS], Num<V> (&a)[STEPS], Num<V> (&b)[STEPS], Num<V>& A, Num<V>& H) {
     A = Num<V>::all(1.0f); H = Num<V>::all(0.0f);
     #pragma unroll
@@ -213,13 +230,13 @@ __device__ __forceinline__ void forward_steps(const ScanArgs& args, const Place<
 
 // First pass, forward: the composition of each chunk.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 4) scan_compose_kernel(const ScanArgs args) {
-    constexpr int S = kForwardSteps, W = kChunk / S;
+__global__ void __launch_bounds__(kComposeWarps * 32, 8) scan_compose_kernel(const ScanArgs args) {
+    constexpr int S = kComposeSteps, W = kComposeWarps;
     __shared__ float2 shared[W][32 * V];
-    const Place<V, S> at(args);
+    const Place<V, S, W> at(args);
     Pack<T, V> x[S], g[S];
-    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
-    load_rows<T, V, S>(args.in.x, args.in.x_stride, at, x);
+    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
+    Rows<T, V>(args.in.x, args.in.x_stride, at).load(at, x);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
     const bool plain = edges.first == 0 && at.count == S;
@@ -245,19 +262,19 @@ __global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 4) scan_compose_k
         float P = 1.0f, Q = 0.0f;
         #pragma unroll
         for (int w = 0; w < W; ++w) compose(P, Q, shared[w][at.lane * V + k]);
-        args.composed[at.chunk * args.in.width + at.channel + k] = make_float2(P, Q);
+        args.composed[int64_t(at.chunk) * args.in.width + at.channel + k] = make_float2(P, Q);
     }
 }
 
 // First pass, backward: E in front of a chunk as a map of E behind it.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 4) scan_compose_backward_kernel(const ScanArgs args) {
-    constexpr int S = kForwardSteps, W = kChunk / S;
+__global__ void __launch_bounds__(kComposeWarps * 32, 8) scan_compose_backward_kernel(const ScanArgs args) {
+    constexpr int S = kComposeSteps, W = kComposeWarps;
     __shared__ float2 shared[W][32 * V];
-    const Place<V, S> at(args);
+    const Place<V, S, W> at(args);
     Pack<T, V> d[S], g[S];
-    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
-    load_rows<T, V, S>(args.grad_h, args.grad_h_stride, at, d);
+    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
+    Rows<T, V>(args.grad_h, args.grad_h_stride, at).load(at, d);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
     const bool plain = edges.last == 0 && at.count == S;
@@ -283,88 +300,107 @@ __global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 4) scan_compose_b
         float P = 1.0f, Q = 0.0f;
         #pragma unroll
         for (int w = W - 1; w >= 0; --w) compose(P, Q, shared[w][at.lane * V + k]);
-        args.composed[at.chunk * args.in.width + at.channel + k] = make_float2(P, Q);
+        args.composed[int64_t(at.chunk) * args.in.width + at.channel + k] = make_float2(P, Q);
     }
 }
 
-// Second pass: the state at each chunk's beginning (from_end: behind each chunk, walking from the last to the first).  A cluster of `parts` blocks takes 32
-// channels; each of its warps composes a run of chunks, then walks through it again from the state in front of the run, which
-// it has from the warps before it and the blocks before its own.
-__global__ void __launch_bounds__(kCarryWarps * 32) scan_carry_kernel(const float2* __restrict__ composed, float* __restrict__ states, int64_t chunks, int width,
+// Second pass: the state at each chunk's beginning (from_end: behind each chunk, walking from the last to the first).  A cluster of `parts` blocks takes eight
+// channels.  Each quarter of a warp composes a run of chunks, learns the state in front of it from the quarters, warps and blocks before, and
+// goes through its run again.  Up to 16 maps of a run stay in registers, all of them on their way at once; a longer run is read twice.
+__global__ void __launch_bounds__(kCarryWarps * 32) scan_carry_kernel(const float2* __restrict__ composed, float* __restrict__ states, int chunks, int width,
                                                                     bool from_end, int parts) {
-    __shared__ float2 shared[kCarryWarps][32];
-    __shared__ float2 whole[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, channel = int(blockIdx.x) / parts * 32 + lane, part = int(blockIdx.x) % parts;
-    const int64_t warps = int64_t(kCarryWarps) * parts, run = (chunks + warps - 1) / warps;
-    const int64_t begin = min((int64_t(part) * kCarryWarps + warp) * run, chunks), end = min(begin + run, chunks);
-    const int64_t first = (from_end ? chunks - 1 - begin : begin) * width + channel, step = from_end ? -int64_t(width) : width;
+    constexpr int kQuarters = 32 / kCarryChannels;
+    __shared__ float2 shared[kCarryWarps][kCarryChannels];
+    __shared__ float2 whole[kCarryChannels];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = lane % kCarryChannels, quarter = lane / kCarryChannels;
+    const int channel = int(blockIdx.x) / parts * kCarryChannels + at, part = int(blockIdx.x) % parts;
+    const bool inside = channel < width;
+    const int runs = kCarryWarps * kQuarters * parts, run = (chunks + runs - 1) / runs;
+    const int begin = int(min(int64_t((part * kCarryWarps + warp) * kQuarters + quarter) * run, int64_t(chunks))), count = inside ? min(run, chunks - begin) : 0;
+    const int64_t first = int64_t(from_end ? chunks - 1 - begin : begin) * width + channel, step = from_end ? -int64_t(width) : width;
+    float2 maps[kCarryRun];
     float A = 1.0f, H = 0.0f;
-    if (channel < width) {
-        #pragma unroll 8
-        for (int64_t c = 0; c < end - begin; ++c) compose(A, H, composed[first + c * step]);
+    for (int c0 = 0; c0 < run; c0 += kCarryRun) {
+        #pragma unroll
+        for (int c = 0; c < kCarryRun; ++c) maps[c] = c0 + c < count ? composed[first + (c0 + c) * step] : make_float2(1.0f, 0.0f);
+        #pragma unroll
+        for (int c = 0; c < kCarryRun; ++c) compose(A, H, maps[c]);
     }
-    shared[warp][lane] = make_float2(A, H);
+    #pragma unroll
+    for (int d = 1; d < kQuarters; d *= 2) {                  // of this quarter and those before
+        float P = __shfl_up_sync(0xffffffffu, A, d * kCarryChannels), Q = __shfl_up_sync(0xffffffffu, H, d * kCarryChannels);
+        if (quarter >= d) { compose(P, Q, make_float2(A, H)); A = P; H = Q; }
+    }
+    if (quarter == kQuarters - 1) shared[warp][at] = make_float2(A, H);
+    float2 before = make_float2(__shfl_up_sync(0xffffffffu, A, kCarryChannels), __shfl_up_sync(0xffffffffu, H, kCarryChannels));
+    if (quarter == 0) before = make_float2(1.0f, 0.0f);
     __syncthreads();
     float state = 0.0f;
     if (parts > 1) {
-        if (warp == 0) {
+        if (threadIdx.x < kCarryChannels) {
             float P = 1.0f, Q = 0.0f;
             #pragma unroll
-            for (int w = 0; w < kCarryWarps; ++w) compose(P, Q, shared[w][lane]);
-            whole[lane] = make_float2(P, Q);
+            for (int w = 0; w < kCarryWarps; ++w) compose(P, Q, shared[w][threadIdx.x]);
+            whole[threadIdx.x] = make_float2(P, Q);
         }
         cluster_barrier();
-        const uint32_t at = smem_u32(&whole[lane]);
-        for (int p = 0; p < part; ++p) state = follow(make_float2(peer_float(at, p), peer_float(at + 4, p)), state);
+        const uint32_t there = smem_u32(&whole[at]);
+        for (int p = 0; p < part; ++p) state = follow(make_float2(peer_float(there, p), peer_float(there + 4, p)), state);
         cluster_barrier();               // no block's shared memory goes before the others have read it
     }
-    if (channel >= width) return;
-    for (int w = 0; w < warp; ++w) state = follow(shared[w][lane], state);
-    #pragma unroll 8
-    for (int64_t c = 0; c < end - begin; ++c) {
-        const float2 m = composed[first + c * step];
-        states[first + c * step] = state;
-        state = follow(m, state);
+    for (int w = 0; w < warp; ++w) state = follow(shared[w][at], state);
+    state = follow(before, state);
+    for (int c0 = 0; c0 < run; c0 += kCarryRun) {
+        if (run > kCarryRun) {
+            #pragma unroll
+            for (int c = 0; c < kCarryRun; ++c) maps[c] = c0 + c < count ? composed[first + (c0 + c) * step] : make_float2(1.0f, 0.0f);
+        }
+        #pragma unroll
+        for (int c = 0; c < kCarryRun; ++c) {
+            if (c0 + c < count) states[first + (c0 + c) * step] = state;
+            state = follow(maps[c], state);
+        }
     }
 }
 
 // Sequences without rows: their last state is the initial one, and so are the gradients.
-__device__ __forceinline__ void pass_empty_sequences(const ScanArgs& args, const float* from, float* to, int64_t chunk, int channel, int v) {
+__device__ __forceinline__ void pass_empty_sequences(const ScanArgs& args, const float* from, float* to, int chunk, int channel, int v) {
     if (!args.in.offsets || !to) return;
     for (int64_t s = chunk; s < args.in.n_sequences; s += args.chunks)
         if (args.in.offsets[s + 1] <= args.in.offsets[s])
             for (int k = 0; k < v; ++k) to[s * args.in.width + channel + k] = from ? from[s * args.in.width + channel + k] : 0.0f;
 }
 
-// Third pass, forward.
+// Third pass, forward; from the end, where the first pass has left the rows in L2.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 2) scan_apply_kernel(const ScanArgs args) {
-    constexpr int S = kForwardSteps, W = kChunk / S;
+__global__ void __launch_bounds__(kApplyWarps * 32, 4) scan_apply_kernel(const ScanArgs args) {
+    constexpr int S = kApplySteps, W = kApplyWarps;
     __shared__ float2 shared[W][32 * V];
-    const Place<V, S> at(args);
+    const Place<V, S, W> at(args, true);
     Pack<T, V> x[S], g[S];
-    load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
-    load_rows<T, V, S>(args.in.x, args.in.x_stride, at, x);
-    Num<V> h = load_state<V>(at.chunk > 0 && at.inside ? args.states : nullptr, at.chunk * args.in.width + at.channel);
+    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
+    Rows<T, V>(args.in.x, args.in.x_stride, at).load(at, x);
+    Num<V> h = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
     Num<V> a[S], b[S], A, H;
     forward_steps<T, V, S>(args, at, edges, x, g, a, b, A, H);
     leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
     for (int w = 0; w < at.warp; ++w) h = follow<V>(&shared[w][at.lane * V], h);
-    T* to = static_cast<T*>(args.h) + at.row0 * args.h_stride + at.channel;
-    const int64_t step = at.step * args.h_stride;
-    if (at.inside && at.count == S && (edges.first | edges.last) == 0) {
+    const Rows<T, V> to(args.h, args.h_stride, at);
+    if ((edges.first | edges.last) == 0 && at.whole()) {
         #pragma unroll
         for (int i = 0; i < S; ++i) {
+            if (i % kKept == 0 && args.states) store_state<V>(args.states, int64_t((at.p0 + i) / kKept) * args.in.width + at.channel, h);
             h = madd(a[i], h, b[i]);
-            store_number<T, V>(to + i * step, h);
+            to.template store<S>(i, at.reverse, h);
         }
     } else {
         #pragma unroll
         for (int i = 0; i < S; ++i) {
+            if (i % kKept == 0 && args.states && at.inside && i < at.count) store_state<V>(args.states, int64_t((at.p0 + i) / kKept) * args.in.width + at.channel, h);
             h = edges.first >> i & 1u ? b[i] : madd(a[i], h, b[i]);
-            if (at.inside && i < at.count) store_number<T, V>(to + i * step, h);
+            if (at.inside && i < at.count) to.template store<S>(i, at.reverse, h);
             if (edges.last >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 if (at.inside) store_state<V>(args.last, at.state_at(args, s), h);
@@ -374,64 +410,44 @@ __global__ void __launch_bounds__(kChunk / kForwardSteps * 32, 2) scan_apply_ker
     if (at.warp == 0 && at.inside) pass_empty_sequences(args, args.in.initial, args.last, at.chunk, at.channel, V);
 }
 
-// Third pass, backward.  exp(-gate) is kept from step to step and a computed from it again: with both there were too many registers for two blocks per SM.
+// Third pass, backward: each warp goes eight rows forward from the state that was kept, and back from the E that the warps behind it leave.
 template <typename T, int V>
-__global__ void __launch_bounds__(kChunk / kBackwardSteps * 32, 2) scan_apply_backward_kernel(const ScanArgs args) {
-    constexpr int S = kBackwardSteps, W = kChunk / S;
-    __shared__ float2 ahead[W][32 * V], back[W][32 * V];
-    const Place<V, S> at(args);
-    Pack<T, V> x[S], d[S];
-    Num<V> t[S];                              // exp(-gate)
-    {
-        Pack<T, V> g[S];
-        load_rows<T, V, S>(args.in.gate, args.in.gate_stride, at, g);
-        load_rows<T, V, S>(args.in.x, args.in.x_stride, at, x);
-        load_rows<T, V, S>(args.grad_h, args.grad_h_stride, at, d);
-        #pragma unroll
-        for (int i = 0; i < S; ++i) t[i] = gate_exp<V>(number<T, V>(g[i]));
-    }
+__global__ void __launch_bounds__(kApplyWarps * 32, 3) scan_apply_backward_kernel(const ScanArgs args) {
+    constexpr int S = kApplySteps, W = kApplyWarps;
+    __shared__ float2 shared[W][32 * V];
+    const Place<V, S, W> at(args, true);
+    Pack<T, V> x[S], d[S], g[S];
+    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
+    Rows<T, V>(args.grad_h, args.grad_h_stride, at).load(at, d);
+    Rows<T, V>(args.in.x, args.in.x_stride, at).load(at, x);
+    Num<V> h = load_state<V>(at.count > 0 && at.inside ? args.states : nullptr, int64_t(at.p0 / kKept) * args.in.width + at.channel);
+    Num<V> E = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
-    const int64_t state_at = at.chunk * args.in.width + at.channel;
-    Num<V> h = load_state<V>(at.chunk > 0 && at.inside ? args.states : nullptr, state_at);
-    Num<V> E = load_state<V>(at.chunk + 1 < args.chunks && at.inside ? args.grad_states : nullptr, state_at);
     const bool plain = (edges.first | edges.last) == 0 && at.count == S;
-    const Num<V> one = Num<V>::all(1.0f), zero = Num<V>::all(0.0f);
-    {                                         // h behind the warp's rows is A h + H; E in front of them is P E + Q
-        Num<V> A = one, H = zero, P = one, Q = zero;
-        if (plain) {
-            #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const Gate<V> gate = gate_of<V>(t[i]);
-                H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
-                A = A * gate.a;
-                Q = madd(A, number<T, V>(d[i]), Q);
-            }
-            P = A;
-        } else {
-            bool cut = false;                 // the rows so far hold the end of a sequence
-            #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                if (i >= at.count) continue;
-                const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u;
-                const int64_t s = first || last ? at.state_at(args, __shfl_sync(0xffffffffu, edges.sequence, i)) : 0;
-                const Gate<V> gate = gate_of<V>(t[i]);
-                if (first) { A = Num<V>::all(kCut); H = load_state<V>(at.inside ? args.in.initial : nullptr, s); }
-                A = A * gate.a;
-                H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
-                if (cut) continue;
-                Num<V> own = number<T, V>(d[i]);
-                if (last) own = own + load_state<V>(at.inside ? args.grad_last : nullptr, s);
-                P = P * gate.a;
-                Q = madd(P, own, Q);
-                if (last) { P = Num<V>::all(kCut); cut = true; }
-            }
-        }
-        leave_map<V>(&ahead[at.warp][at.lane * V], A, H);
-        leave_map<V>(&back[at.warp][at.lane * V], P, Q);
+    Num<V> a[S], rest[S];
+    Num<V> P = Num<V>::all(1.0f), Q = Num<V>::all(0.0f);             // E in front of the warp's rows is P E + Q
+    #pragma unroll
+    for (int i = 0; i < S; ++i) {
+        const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
+        a[i] = gate.a; rest[i] = gate.rest;
     }
-    __syncthreads();
-    for (int w = 0; w < at.warp; ++w) h = follow<V>(&ahead[w][at.lane * V], h);
-    for (int w = W - 1; w > at.warp; --w) E = follow<V>(&back[w][at.lane * V], E);
+    if (plain) {
+        #pragma unroll
+        for (int i = S - 1; i >= 0; --i) { Q = a[i] * (Q + number<T, V>(d[i])); P = P * a[i]; }
+    } else {
+        #pragma unroll
+        for (int i = S - 1; i >= 0; --i) {
+            if (i >= at.count) continue;
+            if (edges.last >> i & 1u) {
+                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
+                P = Num<V>::all(kCut);
+                Q = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
+            }
+            Q = a[i] * (Q + number<T, V>(d[i]));
+            P = P * a[i];
+        }
+    }
+    leave_map<V>(&shared[at.warp][at.lane * V], P, Q);
     Num<V> slope[S];                          // (h_{t-1} - x) a (1 - a)
     #pragma unroll
     for (int i = 0; i < S; ++i) {
@@ -439,32 +455,30 @@ __global__ void __launch_bounds__(kChunk / kBackwardSteps * 32, 2) scan_apply_ba
             const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
             h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
         }
-        const Gate<V> gate = gate_of<V>(t[i]);
         const Num<V> value = number<T, V>(x[i]);
-        slope[i] = madd(Num<V>::all(-1.0f), value, h) * (gate.a * gate.rest);
-        h = madd(gate.a, h, gate.rest * value);
+        slope[i] = madd(Num<V>::all(-1.0f), value, h) * (a[i] * rest[i]);
+        h = madd(a[i], h, rest[i] * value);
     }
-    T* to_x = static_cast<T*>(args.grad_x) + at.row0 * args.grad_x_stride + at.channel;
-    T* to_gate = static_cast<T*>(args.grad_gate) + at.row0 * args.grad_gate_stride + at.channel;
-    const int64_t step_x = at.step * args.grad_x_stride, step_gate = at.step * args.grad_gate_stride;
+    __syncthreads();
+    for (int w = W - 1; w > at.warp; --w) E = follow<V>(&shared[w][at.lane * V], E);
+    const Rows<T, V> to_x(args.grad_x, args.grad_x_stride, at), to_gate(args.grad_gate, args.grad_gate_stride, at);
     #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
-        const Gate<V> gate = gate_of<V>(t[i]);
         if (plain && at.inside) {
             const Num<V> D = number<T, V>(d[i]) + E;
-            store_number<T, V>(to_x + i * step_x, gate.rest * D);
-            store_number<T, V>(to_gate + i * step_gate, slope[i] * D);
-            E = gate.a * D;
+            to_x.template store<S>(i, at.reverse, rest[i] * D);
+            to_gate.template store<S>(i, at.reverse, slope[i] * D);
+            E = a[i] * D;
         } else if (i < at.count) {
             const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u;
             int s = 0;
             if (first || last) s = __shfl_sync(0xffffffffu, edges.sequence, i);
             if (last) E = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
             const Num<V> D = number<T, V>(d[i]) + E;
-            E = gate.a * D;
+            E = a[i] * D;
             if (at.inside) {
-                store_number<T, V>(to_x + i * step_x, gate.rest * D);
-                store_number<T, V>(to_gate + i * step_gate, slope[i] * D);
+                to_x.template store<S>(i, at.reverse, rest[i] * D);
+                to_gate.template store<S>(i, at.reverse, slope[i] * D);
                 if (first && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, s), E);
             }
         }
@@ -488,40 +502,33 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const T* __restrict__ x,
 }
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
-int64_t chunk_count(int64_t rows) { return (rows + kChunk - 1) / kChunk; }
+int64_t pieces(int64_t rows, int piece) { return (rows + piece - 1) / piece; }
 
 bool pairs_possible(const void* p, int64_t stride, int64_t rows, size_t element) { return !p || rows_aligned(p, stride, rows, element, 2 * element); }
 
-void launch_carry(const ScanArgs& args, float* states, bool from_end, cudaStream_t stream) {
-    int parts = 1;                             // eight chunks a warp, and at most eight blocks
-    while (parts < 8 && args.chunks > int64_t(kCarryWarps) * 8 * parts) parts *= 2;
+void launch_carry(const ScanArgs& args, bool from_end, cudaStream_t stream) {
+    int parts = 1;                             // eight chunks in a run, and at most eight blocks
+    while (parts < 8 && args.chunks > kCarryWarps * (32 / kCarryChannels) * 8 * parts) parts *= 2;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = unsigned(parts); attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = unsigned((args.in.width + 31) / 32 * parts); config.blockDim = kCarryWarps * 32; config.stream = stream;
+    config.gridDim = unsigned((args.in.width + kCarryChannels - 1) / kCarryChannels * parts); config.blockDim = kCarryWarps * 32; config.stream = stream;
     config.attrs = &attribute; config.numAttrs = 1;
-    cudaLaunchKernelEx(&config, scan_carry_kernel, static_cast<const float2*>(args.composed), states, args.chunks, int(args.in.width), from_end, parts);
+    cudaLaunchKernelEx(&config, scan_carry_kernel, static_cast<const float2*>(args.composed), args.carried, args.chunks, int(args.in.width), from_end, parts);
 }
 
-template <typename T, int V> void forward_launch(ScanArgs& args, cudaStream_t stream) {
-    constexpr int threads = kChunk / kForwardSteps * 32;
+template <typename T, int V> void scan_launch(ScanArgs& args, bool backward, cudaStream_t stream) {
     args.channel_tiles = (args.in.width + 32 * V - 1) / (32 * V);
-    const unsigned int blocks = unsigned(args.chunks * args.channel_tiles);
+    args.chunks = int(pieces(args.in.rows, kChunk));
+    const unsigned int blocks = unsigned(int64_t(args.chunks) * args.channel_tiles);
     if (args.chunks > 1) {
-        scan_compose_kernel<T, V><<<blocks, threads, 0, stream>>>(args);
-        launch_carry(args, args.states, false, stream);
+        if (backward) scan_compose_backward_kernel<T, V><<<blocks, kComposeWarps * 32, 0, stream>>>(args);
+        else scan_compose_kernel<T, V><<<blocks, kComposeWarps * 32, 0, stream>>>(args);
+        launch_carry(args, backward, stream);
     }
-    scan_apply_kernel<T, V><<<blocks, threads, 0, stream>>>(args);
-}
-template <typename T, int V> void backward_launch(ScanArgs& args, cudaStream_t stream) {
-    args.channel_tiles = (args.in.width + 32 * V - 1) / (32 * V);
-    const unsigned int blocks = unsigned(args.chunks * args.channel_tiles);
-    if (args.chunks > 1) {
-        scan_compose_backward_kernel<T, V><<<blocks, kChunk / kForwardSteps * 32, 0, stream>>>(args);
-        launch_carry(args, args.grad_states, true, stream);
-    }
-    scan_apply_backward_kernel<T, V><<<blocks, kChunk / kBackwardSteps * 32, 0, stream>>>(args);
+    if (backward) scan_apply_backward_kernel<T, V><<<blocks, kApplyWarps * 32, 0, stream>>>(args);
+    else scan_apply_kernel<T, V><<<blocks, kApplyWarps * 32, 0, stream>>>(args);
 }
 
 // Two channels a lane where every row allows it.
@@ -531,15 +538,17 @@ template <typename T> void scan_typed(ScanArgs& a, bool backward, cudaStream_t s
     const bool pairs = a.in.width % 2 == 0 && pairs_possible(a.in.x, a.in.x_stride, rows, e) && pairs_possible(a.in.gate, a.in.gate_stride, rows, e) &&
                        pairs_possible(a.h, a.h_stride, rows, e) && pairs_possible(a.grad_h, a.grad_h_stride, rows, e) &&
                        pairs_possible(a.grad_x, a.grad_x_stride, rows, e) && pairs_possible(a.grad_gate, a.grad_gate_stride, rows, e);
-    if (pairs) { if (backward) backward_launch<T, 2>(a, stream); else forward_launch<T, 2>(a, stream); }
-    else { if (backward) backward_launch<T, 1>(a, stream); else forward_launch<T, 1>(a, stream); }
+    if (pairs) scan_launch<T, 2>(a, backward, stream); else scan_launch<T, 1>(a, backward, stream);
 }
 
+constexpr int64_t kMostStride = 1 << 22;      // elements: 128 rows of it are within 32 bits' worth of bytes
+bool stride_ok(int64_t stride) { return stride >= 0 && stride <= kMostStride; }
+
 int check_scan(const HtgsScan* scan, const char* message) {
-    if (!scan || !known_type(scan->type) || scan->rows < 0 || scan->rows > 0x7fffffff || scan->width < 1 || scan->width > 65536 || scan->n_sequences < 1 ||
+    if (!scan || !known_type(scan->type) || scan->rows < 0 || scan->rows > 0x7fffff00 || !stride_ok(scan->x_stride) || !stride_ok(scan->gate_stride) || scan->width < 1 || scan->width > 65536 || scan->n_sequences < 1 ||
         (!scan->offsets && scan->rows % scan->n_sequences != 0) || (scan->rows > 0 && (!scan->x || !scan->gate)))
         return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
-    if (chunk_count(scan->rows) * ((scan->width + 31) / 32) > 0x7fffffff) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
+    if (pieces(scan->rows, kChunk) * ((scan->width + 31) / 32) > 0x7fffffff) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
     return HTGS_OK;
 }
 
@@ -556,12 +565,12 @@ int pass_states(const float* from, float* to, const HtgsScan* scan, cudaStream_t
 extern "C" {
 
 size_t htgs_gated_scan_state_bytes(int64_t rows, int32_t width) {
-    return rows <= 0 || width <= 0 ? 0 : size_t(htgs::chunk_count(rows)) * size_t(width) * sizeof(float);
+    return rows <= 0 || width <= 0 ? 0 : size_t(htgs::pieces(rows, htgs::kKept)) * size_t(width) * sizeof(float);
 }
 
 size_t htgs_gated_scan_workspace_bytes(int64_t rows, int32_t width) {
     if (rows <= 0 || width <= 0) return 0;
-    const size_t values = size_t(htgs::chunk_count(rows)) * size_t(width);
+    const size_t values = size_t(htgs::pieces(rows, htgs::kChunk)) * size_t(width);
     return htgs::align256(values * sizeof(float2)) + htgs::align256(values * sizeof(float));
 }
 
@@ -572,14 +581,14 @@ int htgs_gated_scan(const HtgsScan* scan, void* h, int64_t h_stride, float* last
     if (!last) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_gated_scan: last must not be null");
     if (scan->rows == 0) return pass_states(scan->initial, last, scan, s);
     if (!h) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_gated_scan: h must not be null");
+    if (!stride_ok(h_stride)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_gated_scan: row strides are from 0 to 2^22");
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < htgs_gated_scan_workspace_bytes(scan->rows, scan->width))
+        return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_gated_scan: workspace too small or not 16-byte aligned");
     ScanArgs a{};
     a.in = *scan;
-    a.chunks = chunk_count(scan->rows);
-    if (a.chunks > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < htgs_gated_scan_workspace_bytes(scan->rows, scan->width)))
-        return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_gated_scan: workspace too small or not 16-byte aligned");
-    const size_t values = size_t(a.chunks) * size_t(scan->width);
     a.composed = static_cast<float2*>(workspace);
-    a.states = states ? states : reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(values * sizeof(float2)));
+    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(pieces(scan->rows, kChunk)) * size_t(scan->width) * sizeof(float2)));
+    a.states = states;
     a.h = h; a.h_stride = h_stride; a.last = last;
     if (scan->type == HTGS_FLOAT32) scan_typed<float>(a, false, s);
     else if (scan->type == HTGS_FLOAT16) scan_typed<__half>(a, false, s);
@@ -595,14 +604,14 @@ int htgs_gated_scan_backward(const HtgsScan* scan, const float* states, const vo
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (scan->rows == 0) return pass_states(grad_last, grad_initial, scan, s);
     if (!states || !grad_h || !grad_x || !grad_gate) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_gated_scan_backward: null pointer");
+    if (!stride_ok(grad_h_stride) || !stride_ok(grad_x_stride) || !stride_ok(grad_gate_stride))
+        return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_gated_scan_backward: row strides are from 0 to 2^22");
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < htgs_gated_scan_workspace_bytes(scan->rows, scan->width))
+        return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_gated_scan_backward: workspace too small or not 16-byte aligned");
     ScanArgs a{};
     a.in = *scan;
-    a.chunks = chunk_count(scan->rows);
-    if (a.chunks > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < htgs_gated_scan_workspace_bytes(scan->rows, scan->width)))
-        return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_gated_scan_backward: workspace too small or not 16-byte aligned");
-    const size_t values = size_t(a.chunks) * size_t(scan->width);
     a.composed = static_cast<float2*>(workspace);
-    a.grad_states = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(values * sizeof(float2)));
+    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(pieces(scan->rows, kChunk)) * size_t(scan->width) * sizeof(float2)));
     a.states = const_cast<float*>(states);
     a.grad_h = grad_h; a.grad_h_stride = grad_h_stride; a.grad_last = grad_last;
     a.grad_x = grad_x; a.grad_x_stride = grad_x_stride; a.grad_gate = grad_gate; a.grad_gate_stride = grad_gate_stride; a.grad_initial = grad_initial;

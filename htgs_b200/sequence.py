@@ -335,6 +335,14 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 # ---- recurrence ----------------------------------------------------------------------------------------------------------------
 
 
+_MOST_STRIDE = 1 << 22      # of a recurrence's rows, in elements
+
+
+def _scan_rows(t: torch.Tensor) -> torch.Tensor:
+    m = _rows(t)
+    return m.clone(memory_format=torch.contiguous_format) if m.stride(0) > _MOST_STRIDE else m
+
+
 def _scan_struct(x, gate, initial, offsets, sequences, reverse) -> HtgsScan:
     return HtgsScan(x.data_ptr(), gate.data_ptr(), None if initial is None else initial.data_ptr(), None if offsets is None else offsets.data_ptr(),
                     x.stride(0), gate.stride(0), x.shape[0], x.shape[1], sequences, _TYPES[x.dtype], int(reverse))
@@ -370,7 +378,7 @@ class _GatedScan(torch.autograd.Function):
         rows, width = x.shape
         if grad_h is None:
             grad_h = torch.zeros((rows, width), dtype=x.dtype, device=x.device)
-        grad_h = _rows(grad_h)
+        grad_h = _scan_rows(grad_h)
         grad_last = None if grad_last is None else grad_last.contiguous()
         grad_x, grad_gate = (torch.empty((rows, width), dtype=x.dtype, device=x.device) for _ in range(2))
         grad_initial = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[2] else None
@@ -415,9 +423,9 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, initial: Optional[torch.Tens
         return torch.empty_like(x), torch.empty((0, shape[-1]), dtype=torch.float32, device=x.device)
     if _wants_grad(x, gate, initial):
         initial = None if initial is None else initial.contiguous()
-        h, last = _GatedScan.apply(_rows(x), _rows(gate), initial, offsets, sequences, bool(reverse))
+        h, last = _GatedScan.apply(_scan_rows(x), _scan_rows(gate), initial, offsets, sequences, bool(reverse))
     else:
-        h, last, _ = _scan_forward(_rows(x), _rows(gate), None if initial is None else initial.contiguous(), offsets, sequences, bool(reverse), False)
+        h, last, _ = _scan_forward(_scan_rows(x), _scan_rows(gate), None if initial is None else initial.contiguous(), offsets, sequences, bool(reverse), False)
     return h.view(shape), last
 
 

@@ -495,7 +495,8 @@ int htgs_fp8_matmul(const HtgsFp8Matrix* a, const HtgsFp8Matrix* b, void* out, i
  * initial [n_sequences, width] is the state in front of each sequence (NULL: zeros), last [n_sequences, width] the one behind it (that of an
  * empty sequence is its initial state).  reverse != 0 goes through each sequence from its last row to its first.
  * states (htgs_gated_scan_state_bytes) keeps what the backward pass needs and may be NULL where there is none.
- * The backward pass takes grad_last == NULL for zeros; grad_initial may be NULL.  1 <= width <= 65536.
+ * The backward pass takes grad_last == NULL for zeros; grad_initial may be NULL.  1 <= width <= 65536; row strides are from 0 to 2^22; workspace as the
+ * size function says, 16-byte aligned.
  * htgs_gated_scan_step does one step for each row and updates state [rows, width] in place.
  */
 typedef struct HtgsScan {

@@ -393,6 +393,19 @@ def test_scan_of_batches_defaults_and_parts_of_the_gradient():
     assert none.shape == (0, 4) and torch.equal(last, torch.ones(2, 4, device="cuda"))
 
 
+def test_scan_of_far_rows():
+    """Rows further apart than the kernels reach are copied first; a single row's stride says nothing."""
+    import torch
+    from htgs_b200 import sequence as seq
+    far = torch.empty(3, (1 << 22) + 8, device="cuda")
+    far[:, :4] = draw((3, 4), 1)
+    x, g = far[:, :4], draw((3, 4), 2)
+    for n in (3, 1):
+        h, last = seq.gated_scan(x[:n], g[:n])
+        want, want_last = seq.gated_scan(x[:n].contiguous() + 0, g[:n] + 0)
+        assert torch.equal(h, want) and torch.equal(last, want_last)
+
+
 @pytest.mark.parametrize("reverse", [False, True])
 def test_scan_keeps_nan_to_its_sequence_and_channel(reverse):
     import torch

@@ -59,7 +59,7 @@ def test_c_entries_check_their_arguments():
         return _native.HtgsScan(*({"x": 64, "gate": 64, "initial": None, "offsets": None, "xs": 8, "gs": 8, "rows": 300, "width": 8, "n": 1, "type": 0,
                                    "reverse": 0} | k).values())
     forward = lambda s, h=64, last=64, ws=64, size=1 << 30: lib.htgs_gated_scan(ctypes.byref(s), h, 8, last, None, ws, size, None)  # noqa: E731
-    for k in ({"x": None}, {"gate": None}, {"rows": -1}, {"rows": 1 << 31}, {"width": 0}, {"width": 65537}, {"n": 0}, {"n": 7}, {"type": 4}):
+    for k in ({"x": None}, {"gate": None}, {"rows": -1}, {"rows": 1 << 31}, {"width": 0}, {"width": 65537}, {"n": 0}, {"n": 7}, {"type": 4}, {"xs": -8}, {"gs": (1 << 22) + 1}):
         _refused(BAD, forward(scan(**k)))
         _refused(BAD, lib.htgs_gated_scan_backward(ctypes.byref(scan(**k)), 64, 64, 8, None, 64, 8, 64, 8, None, 64, 1 << 30, None))
     _refused(BAD, forward(scan(), h=None))
@@ -76,6 +76,5 @@ def test_workspace_sizes():
     lib = _native.lib()
     assert lib.htgs_gated_scan_workspace_bytes(0, 64) == 0 and lib.htgs_gated_scan_state_bytes(-1, 64) == 0
     for rows, width in ((1, 1), (128, 64), (129, 7), (1_000_000, 128)):
-        chunks = -(-rows // 128)
-        assert lib.htgs_gated_scan_state_bytes(rows, width) == chunks * width * 4
-        assert lib.htgs_gated_scan_workspace_bytes(rows, width) >= chunks * width * 12
+        assert lib.htgs_gated_scan_state_bytes(rows, width) == -(-rows // 8) * width * 4            # a state for every eight rows
+        assert lib.htgs_gated_scan_workspace_bytes(rows, width) >= -(-rows // 64) * width * 12      # a map and a state for each chunk
