@@ -23,7 +23,7 @@ constexpr int kComposeSteps = 16, kComposeWarps = kChunk / kComposeSteps;
 constexpr int kApplySteps = 8, kApplyWarps = kChunk / kApplySteps;
 constexpr int kKept = 8;                     // a state for every so many rows is kept for the backward pass
 constexpr int kCarryWarps = 32, kCarryChannels = 8, kCarryRun = 16;
-static_assert(kApplySteps == kKept, "a warp of the backward pass begins with a state that was kept");
+static_assert(kApplySteps == kKept, "a warp keeps one state, and begins with it in the backward pass");
 
 struct ScanArgs {
     HtgsScan in;
@@ -112,6 +112,11 @@ template <int V> __device__ __forceinline__ void leave_map(float2* to, Num<V> A,
 struct Edges { unsigned int first, last; int sequence; };
 template <int STEPS> __device__ __forceinline__ Edges find_edges(const HtgsScan& in, int64_t p0, int lane) {
     const int64_t p = p0 + lane;
+    // one sequence: only its first and last position have an edge
+    if (!in.offsets && in.n_sequences == 1) {
+        const int64_t end = in.rows - 1 - p0;
+        return {p0 == 0 ? 1u : 0u, end >= 0 && end < STEPS ? 1u << end : 0u, 0};
+    }
     bool first = false, last = false;
     int s = 0;
     if (lane < STEPS && p < in.rows) {
@@ -124,8 +129,6 @@ template <int STEPS> __device__ __forceinline__ Edges find_edges(const HtgsScan&
                 if (__ldg(in.offsets + mid) <= row) s = mid; else hi = mid;
             }
             begin = __ldg(in.offsets + s); end = __ldg(in.offsets + s + 1);
-        } else if (in.n_sequences == 1) {
-            begin = 0; end = in.rows;
         } else {
             const int64_t length = in.rows / in.n_sequences;
             s = int(row / length);
@@ -149,48 +152,41 @@ template <int V> __device__ __forceinline__ void store_state(float* states, int6
 }
 
 // Where a thread works: V channels side by side, STEPS rows from position p0 on (positions count rows in the order of the recurrence), `count` of which exist.
-// Addresses are a pointer to the chunk's row i, the same for the whole block, and the thread's own 32-bit offset to its warp's rows and channel.
 template <int V, int STEPS, int WARPS> struct Place {
-    int lane, warp, channel, count, p0, chunk, lowest, row;       // lowest: the chunk's lowest row (it may lie in front of the first); row: the warp's lowest, from there
-    bool inside, reverse;
+    int lane, warp, channel, count, p0, chunk;
+    bool inside;
     __device__ __forceinline__ explicit Place(const ScanArgs& a, bool from_end = false) {
-        constexpr int kRows = STEPS * WARPS;
         lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
         const int at = int(blockIdx.x / unsigned(a.channel_tiles));
         chunk = from_end ? a.chunks - 1 - at : at;
         channel = (int(blockIdx.x % unsigned(a.channel_tiles)) * 32 + lane) * V;
         inside = channel < a.in.width;
-        reverse = a.in.reverse != 0;
-        const int rows = int(a.in.rows), begin = chunk * kRows;
-        p0 = begin + warp * STEPS;
-        count = max(0, min(STEPS, rows - p0));
-        lowest = reverse ? rows - begin - kRows : begin;
-        row = reverse ? kRows - STEPS - warp * STEPS : warp * STEPS;
+        p0 = (chunk * WARPS + warp) * STEPS;
+        count = max(0, min(STEPS, int(a.in.rows) - p0));
     }
     __device__ __forceinline__ bool whole() const { return count == STEPS && inside; }
     __device__ __forceinline__ int64_t state_at(const ScanArgs& a, int sequence) const { return int64_t(sequence) * a.in.width + channel; }
 };
 
-// A matrix's values at a place.
+// A matrix's values at a place: the address at position p0, and the bytes to the next position.  Going from row to row by one addition takes
+// half the instructions of an address computed for each.
 template <typename T, int V> struct Rows {
-    char* chunk;                              // its lowest row
-    int64_t stride;                           // bytes
-    uint32_t offset;                          // of the thread's channel in the warp's lowest row
-    template <typename P> __device__ __forceinline__ Rows(const void* base, int64_t row_stride, const P& at) : stride(row_stride * int64_t(sizeof(T))) {
-        chunk = static_cast<char*>(const_cast<void*>(base)) + at.lowest * stride;
-        offset = uint32_t(at.row) * uint32_t(stride) + uint32_t(at.channel) * uint32_t(sizeof(T));
-    }
-    template <int STEPS> __device__ __forceinline__ Pack<T, V>* at(int i, bool reverse) const {
-        return reinterpret_cast<Pack<T, V>*>(chunk + (reverse ? STEPS - 1 - i : i) * stride + offset);
+    char* first;
+    int64_t step;
+    template <typename P> __device__ __forceinline__ Rows(const void* base, int64_t stride, const HtgsScan& in, const P& at) {
+        const int64_t row = in.reverse ? in.rows - 1 - at.p0 : at.p0;
+        first = static_cast<char*>(const_cast<void*>(base)) + (row * stride + at.channel) * int64_t(sizeof(T));
+        step = (in.reverse ? -stride : stride) * int64_t(sizeof(T));
     }
     template <typename P, int STEPS> __device__ __forceinline__ void load(const P& place, Pack<T, V> (&out)[STEPS]) const {
+        const char* p = first;
         if (place.whole()) {
             #pragma unroll
-            for (int i = 0; i < STEPS; ++i) out[i] = *at<STEPS>(i, place.reverse);
+            for (int i = 0; i < STEPS; ++i, p += step) out[i] = *reinterpret_cast<const Pack<T, V>*>(p);
         } else {
             #pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                if (place.inside && i < place.count) out[i] = *at<STEPS>(i, place.reverse);
+            for (int i = 0; i < STEPS; ++i, p += step) {
+                if (place.inside && i < place.count) out[i] = *reinterpret_cast<const Pack<T, V>*>(p);
                 else {
                     #pragma unroll
                     for (int k = 0; k < V; ++k) out[i].v[k] = from_float<T>(0.0f);
@@ -198,8 +194,8 @@ template <typename T, int V> struct Rows {
             }
         }
     }
-    template <int STEPS> __device__ __forceinline__ void store(int i, bool reverse, Num<V> n) const { store_number<T, V>(reinterpret_cast<T*>(at<STEPS>(i, reverse)), n); }
 };
+template <typename T, int V> __device__ __forceinline__ void store_at(char* p, Num<V> n) { store_number<T, V>(reinterpret_cast<T*>(p), n); }
 
 // The warp's steps as h -> a h + b, and all of them composed (A, H).  The loop for rows in the middle of a sequence asks for nothing else.
 template <typename T, int V, int STEPS, typename P>
@@ -235,24 +231,30 @@ __global__ void __launch_bounds__(kComposeWarps * 32, 8) scan_compose_kernel(con
     __shared__ float2 shared[W][32 * V];
     const Place<V, S, W> at(args);
     Pack<T, V> x[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
-    Rows<T, V>(args.in.x, args.in.x_stride, at).load(at, x);
+    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
+    Rows<T, V>(args.in.x, args.in.x_stride, args.in, at).load(at, x);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
-    const bool plain = edges.first == 0 && at.count == S;
-    #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
-        if (!plain) {
-            if (i >= at.count) continue;
+    if (edges.first == 0 && at.count == S) {
+        #pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
+            H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
+            A = A * gate.a;
+        }
+    } else {
+        #pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (i >= at.count) break;
             if (edges.first >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 A = Num<V>::all(kCut);
                 H = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
             }
+            const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
+            H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
+            A = A * gate.a;
         }
-        H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
-        A = A * gate.a;
     }
     leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
@@ -273,24 +275,30 @@ __global__ void __launch_bounds__(kComposeWarps * 32, 8) scan_compose_backward_k
     __shared__ float2 shared[W][32 * V];
     const Place<V, S, W> at(args);
     Pack<T, V> d[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
-    Rows<T, V>(args.grad_h, args.grad_h_stride, at).load(at, d);
+    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
+    Rows<T, V>(args.grad_h, args.grad_h_stride, args.in, at).load(at, d);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
-    const bool plain = edges.last == 0 && at.count == S;
-    #pragma unroll
-    for (int i = S - 1; i >= 0; --i) {
-        const Num<V> a = gate_of<V>(gate_exp<V>(number<T, V>(g[i]))).a;
-        if (!plain) {
+    if (edges.last == 0 && at.count == S) {
+        #pragma unroll
+        for (int i = S - 1; i >= 0; --i) {
+            const Num<V> a = gate_of<V>(gate_exp<V>(number<T, V>(g[i]))).a;
+            H = a * (H + number<T, V>(d[i]));
+            A = A * a;
+        }
+    } else {
+        #pragma unroll
+        for (int i = S - 1; i >= 0; --i) {
             if (i >= at.count) continue;
             if (edges.last >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 A = Num<V>::all(kCut);
                 H = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
             }
+            const Num<V> a = gate_of<V>(gate_exp<V>(number<T, V>(g[i]))).a;
+            H = a * (H + number<T, V>(d[i]));
+            A = A * a;
         }
-        H = a * (H + number<T, V>(d[i]));
-        A = A * a;
     }
     leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
@@ -378,8 +386,8 @@ __global__ void __launch_bounds__(kApplyWarps * 32, 4) scan_apply_kernel(const S
     __shared__ float2 shared[W][32 * V];
     const Place<V, S, W> at(args, true);
     Pack<T, V> x[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
-    Rows<T, V>(args.in.x, args.in.x_stride, at).load(at, x);
+    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
+    Rows<T, V>(args.in.x, args.in.x_stride, args.in, at).load(at, x);
     Num<V> h = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
     Num<V> a[S], b[S], A, H;
@@ -387,20 +395,22 @@ __global__ void __launch_bounds__(kApplyWarps * 32, 4) scan_apply_kernel(const S
     leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
     for (int w = 0; w < at.warp; ++w) h = follow<V>(&shared[w][at.lane * V], h);
-    const Rows<T, V> to(args.h, args.h_stride, at);
-    if ((edges.first | edges.last) == 0 && at.whole()) {
-        #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (i % kKept == 0 && args.states) store_state<V>(args.states, int64_t((at.p0 + i) / kKept) * args.in.width + at.channel, h);
-            h = madd(a[i], h, b[i]);
-            to.template store<S>(i, at.reverse, h);
+    const Rows<T, V> to(args.h, args.h_stride, args.in, at);
+    char* p = to.first;
+    if (args.states && at.inside && at.count > 0) store_state<V>(args.states, int64_t(at.p0 / kKept) * args.in.width + at.channel, h);
+    if ((edges.first | edges.last) == 0 && at.count == S) {
+        if (at.inside) {
+            #pragma unroll
+            for (int i = 0; i < S; ++i, p += to.step) {
+                h = madd(a[i], h, b[i]);
+                store_at<T, V>(p, h);
+            }
         }
     } else {
         #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (i % kKept == 0 && args.states && at.inside && i < at.count) store_state<V>(args.states, int64_t((at.p0 + i) / kKept) * args.in.width + at.channel, h);
+        for (int i = 0; i < S; ++i, p += to.step) {
             h = edges.first >> i & 1u ? b[i] : madd(a[i], h, b[i]);
-            if (at.inside && i < at.count) to.template store<S>(i, at.reverse, h);
+            if (at.inside && i < at.count) store_at<T, V>(p, h);
             if (edges.last >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 if (at.inside) store_state<V>(args.last, at.state_at(args, s), h);
@@ -417,9 +427,9 @@ __global__ void __launch_bounds__(kApplyWarps * 32, 3) scan_apply_backward_kerne
     __shared__ float2 shared[W][32 * V];
     const Place<V, S, W> at(args, true);
     Pack<T, V> x[S], d[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, at).load(at, g);
-    Rows<T, V>(args.grad_h, args.grad_h_stride, at).load(at, d);
-    Rows<T, V>(args.in.x, args.in.x_stride, at).load(at, x);
+    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
+    Rows<T, V>(args.grad_h, args.grad_h_stride, args.in, at).load(at, d);
+    Rows<T, V>(args.in.x, args.in.x_stride, args.in, at).load(at, x);
     Num<V> h = load_state<V>(at.count > 0 && at.inside ? args.states : nullptr, int64_t(at.p0 / kKept) * args.in.width + at.channel);
     Num<V> E = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
     const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
@@ -449,27 +459,45 @@ __global__ void __launch_bounds__(kApplyWarps * 32, 3) scan_apply_backward_kerne
     }
     leave_map<V>(&shared[at.warp][at.lane * V], P, Q);
     Num<V> slope[S];                          // (h_{t-1} - x) a (1 - a)
-    #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        if (!plain && (edges.first >> i & 1u)) {
-            const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
+    const Num<V> minus = Num<V>::all(-1.0f);
+    if (edges.first == 0) {
+        #pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const Num<V> value = number<T, V>(x[i]);
+            slope[i] = madd(minus, value, h) * (a[i] * rest[i]);
+            h = madd(a[i], h, rest[i] * value);
         }
-        const Num<V> value = number<T, V>(x[i]);
-        slope[i] = madd(Num<V>::all(-1.0f), value, h) * (a[i] * rest[i]);
-        h = madd(a[i], h, rest[i] * value);
+    } else {
+        #pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (edges.first >> i & 1u) {
+                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
+                h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
+            }
+            const Num<V> value = number<T, V>(x[i]);
+            slope[i] = madd(minus, value, h) * (a[i] * rest[i]);
+            h = madd(a[i], h, rest[i] * value);
+        }
     }
     __syncthreads();
     for (int w = W - 1; w > at.warp; --w) E = follow<V>(&shared[w][at.lane * V], E);
-    const Rows<T, V> to_x(args.grad_x, args.grad_x_stride, at), to_gate(args.grad_gate, args.grad_gate_stride, at);
-    #pragma unroll
-    for (int i = S - 1; i >= 0; --i) {
-        if (plain && at.inside) {
-            const Num<V> D = number<T, V>(d[i]) + E;
-            to_x.template store<S>(i, at.reverse, rest[i] * D);
-            to_gate.template store<S>(i, at.reverse, slope[i] * D);
-            E = a[i] * D;
-        } else if (i < at.count) {
+    const Rows<T, V> to_x(args.grad_x, args.grad_x_stride, args.in, at), to_gate(args.grad_gate, args.grad_gate_stride, args.in, at);
+    char* px = to_x.first + (S - 1) * to_x.step;
+    char* pg = to_gate.first + (S - 1) * to_gate.step;
+    if (plain) {
+        if (at.inside) {
+            #pragma unroll
+            for (int i = S - 1; i >= 0; --i, px -= to_x.step, pg -= to_gate.step) {
+                const Num<V> D = number<T, V>(d[i]) + E;
+                store_at<T, V>(px, rest[i] * D);
+                store_at<T, V>(pg, slope[i] * D);
+                E = a[i] * D;
+            }
+        }
+    } else {
+        #pragma unroll
+        for (int i = S - 1; i >= 0; --i, px -= to_x.step, pg -= to_gate.step) {
+            if (i >= at.count) continue;
             const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u;
             int s = 0;
             if (first || last) s = __shfl_sync(0xffffffffu, edges.sequence, i);
@@ -477,8 +505,8 @@ __global__ void __launch_bounds__(kApplyWarps * 32, 3) scan_apply_backward_kerne
             const Num<V> D = number<T, V>(d[i]) + E;
             E = a[i] * D;
             if (at.inside) {
-                to_x.template store<S>(i, at.reverse, rest[i] * D);
-                to_gate.template store<S>(i, at.reverse, slope[i] * D);
+                store_at<T, V>(px, rest[i] * D);
+                store_at<T, V>(pg, slope[i] * D);
                 if (first && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, s), E);
             }
         }
