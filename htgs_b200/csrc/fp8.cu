@@ -76,52 +76,49 @@ __global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const Qua
     }
 }
 
-// One block per 128 x 128 values.  A thread holds eight rows by eight columns: half a warp has the 128 columns of its eight rows, so a row's
-// largest value is found by shuffles, a column's through shared memory.  The transposed codes go through shared memory too, so that they leave as rows of
-// 128: the eight bytes of half-warp h and column c lie in slot h ^ (c / 8 % 16) of the column's sixteen, which spreads the 16
-// lanes of a store over all banks.  PER_TILE: one scale for the whole tile.  VEC: columns a load takes; a thread's eight are (8 / VEC) groups 16 * VEC apart.
-template <typename T, int VEC, bool PER_TILE>
-__global__ void __launch_bounds__(kQuantBlock, 2) quantize_tiles_kernel(const QuantArgs a) {
+// One block per 128 x 128 values, which lie in shared memory as they came: 16 bytes at a time without passing through registers where the rows allow it (WIDE).
+// A thread deals with eight rows by eight columns: half a warp has the 128 columns of its eight rows, so a row's largest value is found by
+// shuffles, a column's through shared memory.  Transposed codes go through shared memory too, in the tile's place, so that they leave as rows of 128: the
+// eight bytes of half-warp h and column c lie in slot h ^ (c / 8 % 16) of the column's sixteen, which spreads the 16 lanes of a store over all
+// banks.  PER_TILE: one scale for the whole tile.
+// (With the tile in registers, 98 a thread, two blocks were on an SM: 32768 x 1024 with its transpose in 26.6 us.)
+template <typename T, bool WIDE, bool PER_TILE>
+__global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const QuantArgs a) {
+    constexpr int VEC = 16 / int(sizeof(T)), G = 8 / VEC;                 // values in 16 bytes, and of those in a thread's eight columns
+    extern __shared__ __align__(16) unsigned char raw[];
+    T (*tile)[kScaleBlock] = reinterpret_cast<T (*)[kScaleBlock]>(raw);
+    uint2 (*turned)[16] = reinterpret_cast<uint2 (*)[16]>(raw);
     __shared__ float column_largest[16][kScaleBlock];
     __shared__ float column_all[kScaleBlock];
-    __shared__ __align__(16) uint2 turned[kScaleBlock][16];
-    constexpr int G = 8 / VEC;
     const int l = threadIdx.x & 15, h = threadIdx.x >> 4;
     const int64_t row0 = int64_t(blockIdx.y) * kScaleBlock, column0 = int64_t(blockIdx.x) * kScaleBlock;
     const int rows = int(min(int64_t(kScaleBlock), a.rows - row0)), columns = int(min(int64_t(kScaleBlock), a.width - column0));
-    const auto column = [&](int c) { return c / VEC * 16 * VEC + l * VEC + c % VEC; };      // of the thread's c-th value in the tile
-    Pack<T, VEC> raw[8][G];
-    const T* x = static_cast<const T*>(a.x) + (row0 + h * 8) * a.x_stride + column0;
-    #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    const T* x = static_cast<const T*>(a.x) + row0 * a.x_stride + column0;
+    if (WIDE) {
+        constexpr int kPieces = kScaleBlock / VEC;                       // of a row
         #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            if (h * 8 + r < rows && column(j * VEC) < columns) raw[r][j] = *reinterpret_cast<const Pack<T, VEC>*>(x + r * a.x_stride + column(j * VEC));
-            else {
-                #pragma unroll
-                for (int i = 0; i < VEC; ++i) raw[r][j].v[i] = from_float<T>(0.0f);
-            }
+        for (int i = 0; i < kScaleBlock * kPieces / kQuantBlock; ++i) {
+            const int at = i * kQuantBlock + int(threadIdx.x), r = at / kPieces, c = at % kPieces * VEC;
+            const bool there = r < rows && c < columns;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&tile[r][c])), "l"(there ? x + r * a.x_stride + c : x), "r"(there ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        #pragma unroll 8
+        for (int i = 0; i < kScaleBlock * kScaleBlock / kQuantBlock; ++i) {
+            const int at = i * kQuantBlock + int(threadIdx.x), r = at / kScaleBlock, c = at % kScaleBlock;
+            tile[r][c] = r < rows && c < columns ? x[r * a.x_stride + c] : from_float<T>(0.0f);
         }
     }
+    __syncthreads();
+    const auto column = [&](int c) { return c / VEC * 16 * VEC + l * VEC + c % VEC; };      // of the thread's c-th value in the tile
     const auto values = [&](int r, float (&v)[8]) {
         #pragma unroll
         for (int j = 0; j < G; ++j) {
             float f[VEC];
-            to_floats<T, VEC>(raw[r][j], f);
+            load_floats<T, VEC>(&tile[h * 8 + r][(j * 16 + l) * VEC], f);
             #pragma unroll
             for (int i = 0; i < VEC; ++i) v[j * VEC + i] = f[i];
-        }
-    };
-    const auto store_row_codes = [&](int r, const float (&v)[8], float inverse, bool careful) {
-        uint8_t* codes = a.codes + (row0 + h * 8 + r) * a.codes_stride + column0;
-        #pragma unroll
-        for (int j = 0; j < G; ++j) {
-            if (column(j * VEC) >= columns) continue;
-            float f[VEC];
-            #pragma unroll
-            for (int i = 0; i < VEC; ++i) f[i] = v[j * VEC + i];
-            if (careful) store_codes<true>(codes + column(j * VEC), f, inverse);
-            else store_codes<false>(codes + column(j * VEC), f, inverse);
         }
     };
     float most[8] = {};                      // of the thread's columns
@@ -136,7 +133,7 @@ __global__ void __launch_bounds__(kQuantBlock, 2) quantize_tiles_kernel(const Qu
     if (careful) {
         #pragma unroll
         for (int c = 0; c < 8; ++c) most[c] = 0.0f;
-        #pragma unroll
+        #pragma unroll 1
         for (int r = 0; r < 8; ++r) {
             float v[8];
             values(r, v);
@@ -144,18 +141,6 @@ __global__ void __launch_bounds__(kQuantBlock, 2) quantize_tiles_kernel(const Qu
             for (int c = 0; c < 8; ++c) most[c] = fmaxf(most[c], finite_magnitude(v[c]));
         }
     }
-    if (!PER_TILE && a.codes) {
-        #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            float v[8];
-            values(r, v);
-            const int e = scale_exponent(lanes_max<16>(careful ? largest_finite(v) : largest_magnitude(v)));
-            if (h * 8 + r >= rows) continue;
-            store_row_codes(r, v, inverse_scale(e), careful);
-            if (l == 0) a.scales[(row0 + h * 8 + r) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
-        }
-    }
-    if (!PER_TILE && !a.codes_t) return;
     #pragma unroll
     for (int c = 0; c < 8; ++c) column_largest[h][column(c)] = most[c];
     __syncthreads();
@@ -165,38 +150,59 @@ __global__ void __launch_bounds__(kQuantBlock, 2) quantize_tiles_kernel(const Qu
         for (int i = 0; i < 16; ++i) largest = fmaxf(largest, column_largest[i][threadIdx.x]);
         if (PER_TILE) largest = lanes_max<32>(largest);
         column_all[threadIdx.x] = largest;
-        if (!PER_TILE && int(threadIdx.x) < columns) a.scales_t[(column0 + threadIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(scale_exponent(largest) + 127);
+        if (!PER_TILE && a.codes_t && int(threadIdx.x) < columns) a.scales_t[(column0 + threadIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(scale_exponent(largest) + 127);
     }
     __syncthreads();
+    int tile_e = 0;
     if (PER_TILE) {
-        const int e = scale_exponent(fmaxf(fmaxf(column_all[0], column_all[32]), fmaxf(column_all[64], column_all[96])));
-        if (a.codes) {
+        tile_e = scale_exponent(fmaxf(fmaxf(column_all[0], column_all[32]), fmaxf(column_all[64], column_all[96])));
+        if (threadIdx.x == 0 && a.codes) a.scales[int64_t(blockIdx.y) * a.scales_stride + blockIdx.x] = uint8_t(tile_e + 127);
+        if (threadIdx.x == 0 && a.codes_t) a.scales_t[int64_t(blockIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(tile_e + 127);
+    }
+    if (a.codes) {
+        const bool together = a.width % VEC == 0 && a.codes_stride % VEC == 0 && reinterpret_cast<uintptr_t>(a.codes) % VEC == 0;
+        #pragma unroll 2
+        for (int r = 0; r < 8; ++r) {
+            float v[8];
+            values(r, v);
+            const int e = PER_TILE ? tile_e : scale_exponent(lanes_max<16>(careful ? largest_finite(v) : largest_magnitude(v)));
+            if (h * 8 + r >= rows) continue;
+            const float inverse = inverse_scale(e);
+            uint8_t* codes = a.codes + (row0 + h * 8 + r) * a.codes_stride + column0;
             #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                if (h * 8 + r >= rows) break;
-                float v[8];
-                values(r, v);
-                store_row_codes(r, v, inverse_scale(e), careful);
+            for (int j = 0; j < G; ++j) {
+                float f[VEC];
+                #pragma unroll
+                for (int i = 0; i < VEC; ++i) f[i] = v[j * VEC + i];
+                if (together) {
+                    if (column(j * VEC) >= columns) continue;
+                    if (careful) store_codes<true>(codes + column(j * VEC), f, inverse);
+                    else store_codes<false>(codes + column(j * VEC), f, inverse);
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        if (column(j * VEC + i) < columns) codes[column(j * VEC + i)] = uint8_t(encode2<true>(f[i], 0.0f, inverse) & 0xffu);
+                }
             }
-            if (threadIdx.x == 0) a.scales[int64_t(blockIdx.y) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
-        }
-        if (!a.codes_t) return;
-        if (threadIdx.x == 0) a.scales_t[int64_t(blockIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(e + 127);
-        #pragma unroll
-        for (int c = 0; c < 8; ++c) most[c] = inverse_scale(e);
-    } else {
-        #pragma unroll
-        for (int c = 0; c < 8; ++c) most[c] = inverse_scale(scale_exponent(column_all[column(c)]));
-    }
-    {
-        const auto one = [&](int r, int c) { return to_float<T>(raw[r][c / VEC].v[c % VEC]); };
-        #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            uint2& to = turned[column(c)][h ^ (column(c) / 8 % 16)];
-            if (careful) to = make_uint2(encode4<true>(one(0, c), one(1, c), one(2, c), one(3, c), most[c]), encode4<true>(one(4, c), one(5, c), one(6, c), one(7, c), most[c]));
-            else to = make_uint2(encode4<false>(one(0, c), one(1, c), one(2, c), one(3, c), most[c]), encode4<false>(one(4, c), one(5, c), one(6, c), one(7, c), most[c]));
+            if (!PER_TILE && l == 0) a.scales[(row0 + h * 8 + r) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
         }
     }
+    if (!a.codes_t) return;
+    #pragma unroll
+    for (int c = 0; c < 8; ++c) most[c] = inverse_scale(PER_TILE ? tile_e : scale_exponent(column_all[column(c)]));
+    uint32_t words[2][8];                    // four rows' codes of each column
+    #pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        float v[4][8];
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) values(4 * q + r, v[r]);
+        #pragma unroll
+        for (int c = 0; c < 8; ++c)
+            words[q][c] = careful ? encode4<true>(v[0][c], v[1][c], v[2][c], v[3][c], most[c]) : encode4<false>(v[0][c], v[1][c], v[2][c], v[3][c], most[c]);
+    }
+    __syncthreads();                         // nothing more is read of the tile
+    #pragma unroll
+    for (int c = 0; c < 8; ++c) turned[column(c)][h ^ (column(c) / 8 % 16)] = make_uint2(words[0][c], words[1][c]);
     __syncthreads();
     const bool whole = rows == kScaleBlock && a.codes_t_stride % 16 == 0 && reinterpret_cast<uintptr_t>(a.codes_t) % 16 == 0;
     for (int i = threadIdx.x; i < columns * 8; i += kQuantBlock) {
@@ -205,8 +211,9 @@ __global__ void __launch_bounds__(kQuantBlock, 2) quantize_tiles_kernel(const Qu
         uint8_t* to = a.codes_t + (column0 + c) * a.codes_t_stride + row0 + 16 * s;
         if (whole) *reinterpret_cast<uint4*>(to) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         else {
-            const uint32_t words[4] = {lo.x, lo.y, hi.x, hi.y};
-            for (int k = 0; k < 16 && 16 * s + k < rows; ++k) to[k] = uint8_t(words[k >> 2] >> (8 * (k & 3)));
+            const uint32_t four[4] = {lo.x, lo.y, hi.x, hi.y};
+            #pragma unroll 1
+            for (int k = 0; k < 16 && 16 * s + k < rows; ++k) to[k] = uint8_t((k < 8 ? k < 4 ? four[0] : four[1] : k < 12 ? four[2] : four[3]) >> (8 * (k & 3)));
         }
     }
 }
@@ -269,16 +276,23 @@ unsigned int blocks_for(int64_t rows, int64_t width, int columns) {
 template <typename T, int VEC> void launch_rows(const QuantArgs& a, cudaStream_t stream) {
     quantize_rows_kernel<T, VEC><<<blocks_for(a.rows, a.width, VEC == 1 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream>>>(a);
 }
-template <typename T, int VEC> void launch_tiles(const QuantArgs& a, int rows_per_scale, cudaStream_t stream) {
+template <typename T, bool WIDE, bool PER_TILE> cudaError_t launch_tiles(const QuantArgs& a, cudaStream_t stream) {
     const dim3 grid(unsigned((a.width + kScaleBlock - 1) / kScaleBlock), unsigned((a.rows + kScaleBlock - 1) / kScaleBlock));
-    if (rows_per_scale == 1) quantize_tiles_kernel<T, VEC, false><<<grid, kQuantBlock, 0, stream>>>(a);
-    else quantize_tiles_kernel<T, VEC, true><<<grid, kQuantBlock, 0, stream>>>(a);
+    constexpr int smem = kScaleBlock * kScaleBlock * int(sizeof(T));
+    static PerDeviceOnce once;
+    const cudaError_t err = once.run([] { return cudaFuncSetAttribute(quantize_tiles_kernel<T, WIDE, PER_TILE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    if (err == cudaSuccess) quantize_tiles_kernel<T, WIDE, PER_TILE><<<grid, kQuantBlock, smem, stream>>>(a);
+    return err;
 }
-template <typename T> void quantize_typed(const QuantArgs& a, int rows_per_scale, cudaStream_t stream) {
+template <typename T> int quantize_typed(const QuantArgs& a, int rows_per_scale, cudaStream_t stream) {
     constexpr int V = 16 / int(sizeof(T));
-    const bool wide = a.width % V == 0 && rows_aligned(a.x, a.x_stride, a.rows, sizeof(T), 16) && rows_aligned(a.codes, a.codes_stride, a.rows, 1, V);
-    if (rows_per_scale == 1 && !a.codes_t) { if (wide) launch_rows<T, V>(a, stream); else launch_rows<T, 1>(a, stream); }
-    else { if (wide) launch_tiles<T, V>(a, rows_per_scale, stream); else launch_tiles<T, 1>(a, rows_per_scale, stream); }
+    const bool wide = a.width % V == 0 && rows_aligned(a.x, a.x_stride, a.rows, sizeof(T), 16);
+    cudaError_t err = cudaSuccess;
+    if (rows_per_scale != 1) err = wide ? launch_tiles<T, true, true>(a, stream) : launch_tiles<T, false, true>(a, stream);
+    else if (a.codes_t) err = wide ? launch_tiles<T, true, false>(a, stream) : launch_tiles<T, false, false>(a, stream);
+    else if (wide && rows_aligned(a.codes, a.codes_stride, a.rows, 1, V)) launch_rows<T, V>(a, stream);
+    else launch_rows<T, 1>(a, stream);
+    return err == cudaSuccess ? sequence_status("htgs_quantize_fp8") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
 template <typename T, int VEC> void launch_dequantize(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
@@ -308,10 +322,9 @@ int htgs_quantize_fp8(const void* x, int64_t x_stride, int type, int64_t rows, i
     if ((codes_t || rows_per_scale != 1) && rows > 65535ll * kScaleBlock) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_quantize_fp8: at most 8388480 rows with tiles or a transpose");
     const QuantArgs a{x, x_stride, rows, width, codes, scales, codes_stride, scales_stride, codes_t, scales_t, codes_t_stride, scales_t_stride};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (type == HTGS_FLOAT32) quantize_typed<float>(a, rows_per_scale, s);
-    else if (type == HTGS_FLOAT16) quantize_typed<__half>(a, rows_per_scale, s);
-    else quantize_typed<__nv_bfloat16>(a, rows_per_scale, s);
-    return sequence_status("htgs_quantize_fp8");
+    if (type == HTGS_FLOAT32) return quantize_typed<float>(a, rows_per_scale, s);
+    if (type == HTGS_FLOAT16) return quantize_typed<__half>(a, rows_per_scale, s);
+    return quantize_typed<__nv_bfloat16>(a, rows_per_scale, s);
 }
 
 int htgs_dequantize_fp8(const HtgsFp8Matrix* matrix, void* out, int64_t out_stride, int out_type, void* stream) {

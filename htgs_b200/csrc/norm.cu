@@ -252,21 +252,22 @@ __global__ void __launch_bounds__(MOST, MOST == kNarrowBlock ? kNarrowBlocks : 1
     }
 }
 
-// Sums the blocks' partial gradients of the weight, always in the same order.  32 columns by 8 slices of the blocks.
-template <typename T> __global__ void __launch_bounds__(kNormBlock) norm_weight_kernel(const float* partial, int blocks, int width, T* grad_weight) {
-    __shared__ float shared[kNormWarps][32];
+// Sums the blocks' partial gradients of the weight, always in the same order.  32 columns by 32 slices of the blocks, four of a slice's on their way at a time.
+template <typename T> __global__ void __launch_bounds__(1024) norm_weight_kernel(const float* partial, int blocks, int width, T* grad_weight) {
+    __shared__ float shared[32][33];
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, column = blockIdx.x * 32 + lane;
-    float total = 0.0f;
-    if (column < width)
-        for (int b = slice; b < blocks; b += kNormWarps) total += partial[int64_t(b) * width + column];
-    shared[slice][lane] = total;
-    __syncthreads();
-    if (slice == 0 && column < width) {
-        total = 0.0f;
-        #pragma unroll
-        for (int s = 0; s < kNormWarps; ++s) total += shared[s][lane];
-        grad_weight[column] = from_float<T>(total);
+    float sum[4] = {};
+    if (column < width) {
+        for (int b = slice; b < blocks; b += 128) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (b + 32 * i < blocks) sum[i] += partial[int64_t(b + 32 * i) * width + column];
+        }
     }
+    shared[slice][lane] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    __syncthreads();
+    const float total = warp_sum(shared[lane][slice]);       // of column `slice`
+    if (lane == 0 && int(blockIdx.x) * 32 + slice < width) grad_weight[blockIdx.x * 32 + slice] = from_float<T>(total);
 }
 
 int backward_threads(int width) { return (width + 32 * kBackwardColumns - 1) / (32 * kBackwardColumns) * 32; }
@@ -317,7 +318,7 @@ template <typename T> void backward_typed(const NormBackwardArgs& a, void* grad_
                       rows_aligned(a.x, a.x_stride, a.rows, e, 16) && rows_aligned(a.residual, a.residual_stride, a.rows, e, 16) && aligned(a.weight, 16) &&
                       rows_aligned(a.grad_x, a.grad_x_stride, a.rows, e, 16);
     if (wide) backward_launch<T, V>(a, stream); else backward_launch<T, 1>(a, stream);
-    norm_weight_kernel<T><<<(a.width + 31) / 32, kNormBlock, 0, stream>>>(a.partial, backward_blocks(a.rows, a.width), a.width, static_cast<T*>(grad_weight));
+    norm_weight_kernel<T><<<(a.width + 31) / 32, 1024, 0, stream>>>(a.partial, backward_blocks(a.rows, a.width), a.width, static_cast<T*>(grad_weight));
 }
 
 }  // namespace
