@@ -19,15 +19,15 @@ namespace {
 
 // A block takes a chunk of 32 or 64 channels; each of its warps takes some rows of it.
 constexpr int kChunk = 64;                                                       // rows
-constexpr int kComposeSteps = 16, kComposeWarps = kChunk / kComposeSteps;
-constexpr int kApplySteps = 8, kApplyWarps = kChunk / kApplySteps;
+constexpr int kSteps = 8, kWarps = kChunk / kSteps;                              // rows of a warp
+constexpr int kScanBlock = kWarps * 32;
 constexpr int kKept = 8;                     // a state for every so many rows is kept for the backward pass
 constexpr int kCarryWarps = 32, kCarryChannels = 8, kCarryRun = 16;
-static_assert(kApplySteps == kKept, "a warp keeps one state, and begins with it in the backward pass");
+static_assert(kSteps == kKept, "a warp keeps one state, and begins with it in the backward pass");
 
 struct ScanArgs {
     HtgsScan in;
-    int chunks, channel_tiles;
+    int chunks;
     float2* composed;                        // [chunks, width]
     float* carried;                          // [chunks, width] state in front of each chunk (backward: E behind it); nothing where there is one chunk
     float* states;                           // [ceil(rows / 8), width] state in front of every eight rows, or null
@@ -151,164 +151,154 @@ template <int V> __device__ __forceinline__ void store_state(float* states, int6
     for (int k = 0; k < V; ++k) states[at + k] = n[k];
 }
 
-// Where a thread works: V channels side by side, STEPS rows from position p0 on (positions count rows in the order of the recurrence), `count` of which exist.
-template <int V, int STEPS, int WARPS> struct Place {
-    int lane, warp, channel, count, p0, chunk;
+// Where a thread works: V channels side by side, kSteps rows from position p0 on (positions count rows in the order of the recurrence), `count` of which exist.
+constexpr int kGridRows = 32768;              // chunks along the grid's y, the rest along z
+template <int V> struct Place {
+    int lane, warp, channel0, channel, count, p0, chunk;
     bool inside;
     __device__ __forceinline__ explicit Place(const ScanArgs& a, bool from_end = false) {
         lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
-        const int at = int(blockIdx.x / unsigned(a.channel_tiles));
+        const int at = int(blockIdx.z * kGridRows + blockIdx.y);
         chunk = from_end ? a.chunks - 1 - at : at;
-        channel = (int(blockIdx.x % unsigned(a.channel_tiles)) * 32 + lane) * V;
+        channel0 = int(blockIdx.x) * 32 * V;
+        channel = channel0 + lane * V;
         inside = channel < a.in.width;
-        p0 = (chunk * WARPS + warp) * STEPS;
-        count = max(0, min(STEPS, int(a.in.rows) - p0));
+        p0 = chunk * kChunk + warp * kSteps;
+        count = max(0, min(kSteps, int(a.in.rows) - p0));
     }
-    __device__ __forceinline__ bool whole() const { return count == STEPS && inside; }
     __device__ __forceinline__ int64_t state_at(const ScanArgs& a, int sequence) const { return int64_t(sequence) * a.in.width + channel; }
 };
 
-// A matrix's values at a place: the address at position p0, and the bytes to the next position.  Going from row to row by one addition takes
-// half the instructions of an address computed for each.
-template <typename T, int V> struct Rows {
-    char* first;
-    int64_t step;
-    template <typename P> __device__ __forceinline__ Rows(const void* base, int64_t stride, const HtgsScan& in, const P& at) {
-        const int64_t row = in.reverse ? in.rows - 1 - at.p0 : at.p0;
-        first = static_cast<char*>(const_cast<void*>(base)) + (row * stride + at.channel) * int64_t(sizeof(T));
-        step = (in.reverse ? -stride : stride) * int64_t(sizeof(T));
-    }
-    template <typename P, int STEPS> __device__ __forceinline__ void load(const P& place, Pack<T, V> (&out)[STEPS]) const {
-        const char* p = first;
-        if (place.whole()) {
-            #pragma unroll
-            for (int i = 0; i < STEPS; ++i, p += step) out[i] = *reinterpret_cast<const Pack<T, V>*>(p);
-        } else {
-            #pragma unroll
-            for (int i = 0; i < STEPS; ++i, p += step) {
-                if (place.inside && i < place.count) out[i] = *reinterpret_cast<const Pack<T, V>*>(p);
-                else {
-                    #pragma unroll
-                    for (int k = 0; k < V; ++k) out[i].v[k] = from_float<T>(0.0f);
-                }
-            }
-        }
-    }
-};
-template <typename T, int V> __device__ __forceinline__ void store_at(char* p, Num<V> n) { store_number<T, V>(reinterpret_cast<T*>(p), n); }
-
-// The warp's steps as h -> a h + b, and all of them composed (A, H).  The loop for rows in the middle of a sequence asks for nothing else.
-template <typename T, int V, int STEPS, typename P>
-__device__ __forceinline__ void forward_steps(const ScanArgs& args, const P& at, const Edges& edges, const Pack<T, V> (&x)[STEPS],
-                                              const Pack<T, V> (&g)[STEPS], Num<V> (&a)[STEPS], Num<V> (&b)[STEPS], Num<V>& A, Num<V>& H) {
-    A = Num<V>::all(1.0f); H = Num<V>::all(0.0f);
-    #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
-        a[i] = gate.a;
-        b[i] = gate.rest * number<T, V>(x[i]);
-    }
-    if (edges.first == 0 && at.count == STEPS) {
+// A chunk of 32 V channels in shared memory, one row per position, brought and taken away PIECE bytes at a time: 16 where every row of the matrix
+// allows it, or 4, or a single 16-bit value.
+template <typename T, int V, int PIECE> struct Tile {
+    static constexpr int kRow = 32 * V, kElements = PIECE / int(sizeof(T)), kPieces = kRow / kElements, kRowsAtOnce = kScanBlock / kPieces, kTrips = kChunk / kRowsAtOnce;
+    static constexpr int bytes = kChunk * kRow * int(sizeof(T));
+    T* data;
+    __device__ __forceinline__ explicit Tile(unsigned char* at) : data(reinterpret_cast<T*>(at)) {}
+    // f(address in the matrix, address here, whether the piece exists), for each of the thread's pieces
+    template <typename F> __device__ __forceinline__ void each(const void* base, int64_t stride, const ScanArgs& a, const Place<V>& at, F f) const {
+        const int r = int(threadIdx.x) / kPieces, c = int(threadIdx.x) % kPieces * kElements, left = int(a.in.rows) - at.chunk * kChunk;
+        const int64_t position = int64_t(at.chunk) * kChunk + r, row = a.in.reverse ? a.in.rows - 1 - position : position;
+        const int64_t step = (a.in.reverse ? -stride : stride) * kRowsAtOnce;
+        T* there = static_cast<T*>(const_cast<void*>(base)) + row * stride + at.channel0 + c;
+        const bool inside = at.channel0 + c < a.in.width;
+        T* here = data + r * kRow + c;
         #pragma unroll
-        for (int i = 0; i < STEPS; ++i) { A = A * a[i]; H = madd(a[i], H, b[i]); }
-        return;
+        for (int i = 0; i < kTrips; ++i, there += step, here += kRowsAtOnce * kRow) f(there, here, inside && r + i * kRowsAtOnce < left);
     }
-    #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        if (i >= at.count) { a[i] = Num<V>::all(1.0f); b[i] = Num<V>::all(0.0f); }
-        if (edges.first >> i & 1u) {
-            const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            b[i] = madd(a[i], load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s)), b[i]);
-            A = a[i] = Num<V>::all(kCut); H = b[i];
-        } else { A = A * a[i]; H = madd(a[i], H, b[i]); }
+    // What does not exist becomes zero.
+    __device__ __forceinline__ void load(const void* base, int64_t stride, const ScanArgs& a, const Place<V>& at) const {
+        each(base, stride, a, at, [&](T* there, T* here, bool exists) {
+            if constexpr (PIECE == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(here)), "l"(exists ? there : base), "r"(exists ? 16 : 0) : "memory");
+            else if constexpr (PIECE == 4)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(here)), "l"(exists ? there : base), "r"(exists ? 4 : 0) : "memory");
+            else *here = exists ? *there : from_float<T>(0.0f);
+        });
     }
+    __device__ __forceinline__ void store(void* base, int64_t stride, const ScanArgs& a, const Place<V>& at) const {
+        each(base, stride, a, at, [&](T* there, T* here, bool exists) {
+            if (exists) *reinterpret_cast<Pack<T, kElements>*>(there) = *reinterpret_cast<const Pack<T, kElements>*>(here);
+        });
+    }
+    __device__ __forceinline__ T* mine(const Place<V>& at) const { return data + at.warp * kSteps * kRow + at.lane * V; }       // the thread's values: every kRow from here
+    __device__ __forceinline__ static Num<V> get(const T* p) { return number<T, V>(*reinterpret_cast<const Pack<T, V>*>(p)); }
+    __device__ __forceinline__ static void put(T* p, Num<V> n) { store_number<T, V>(p, n); }
+};
+__device__ __forceinline__ void tiles_are_here() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 }
+template <typename T, int V> __device__ __forceinline__ Gate<V> gate_at(const T* p) { return gate_of<V>(gate_exp<V>(number<T, V>(*reinterpret_cast<const Pack<T, V>*>(p)))); }
 
 // First pass, forward: the composition of each chunk.
-template <typename T, int V>
-__global__ void __launch_bounds__(kComposeWarps * 32, 8) scan_compose_kernel(const ScanArgs args) {
-    constexpr int S = kComposeSteps, W = kComposeWarps;
-    __shared__ float2 shared[W][32 * V];
-    const Place<V, S, W> at(args);
-    Pack<T, V> x[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
-    Rows<T, V>(args.in.x, args.in.x_stride, args.in, at).load(at, x);
-    const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
+template <typename T, int V, int PIECE>
+__global__ void __launch_bounds__(kScanBlock, 6) scan_compose_kernel(const ScanArgs args) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    __shared__ float2 shared[kWarps][32 * V];
+    using In = Tile<T, V, PIECE>;
+    const Place<V> at(args);
+    if (at.chunk >= args.chunks) return;
+    const In gs(memory), xs(memory + In::bytes);
+    gs.load(args.in.gate, args.in.gate_stride, args, at);
+    xs.load(args.in.x, args.in.x_stride, args, at);
+    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
+    tiles_are_here();
+    const T *g = gs.mine(at), *x = xs.mine(at);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
-    if (edges.first == 0 && at.count == S) {
+    if (edges.first == 0 && at.count == kSteps) {
         #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
-            H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
+        for (int i = 0; i < kSteps; ++i) {
+            const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
+            H = madd(gate.a, H, gate.rest * In::get(x + i * In::kRow));
             A = A * gate.a;
         }
     } else {
-        #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (i >= at.count) break;
+        #pragma unroll 1
+        for (int i = 0; i < at.count; ++i) {
             if (edges.first >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 A = Num<V>::all(kCut);
                 H = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
             }
-            const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
-            H = madd(gate.a, H, gate.rest * number<T, V>(x[i]));
+            const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
+            H = madd(gate.a, H, gate.rest * In::get(x + i * In::kRow));
             A = A * gate.a;
         }
     }
     leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
-    if (at.warp != 0 || !at.inside) return;
-    #pragma unroll
-    for (int k = 0; k < V; ++k) {
+    if (threadIdx.x < 32 * V && at.channel0 + int(threadIdx.x) < args.in.width) {
         float P = 1.0f, Q = 0.0f;
         #pragma unroll
-        for (int w = 0; w < W; ++w) compose(P, Q, shared[w][at.lane * V + k]);
-        args.composed[int64_t(at.chunk) * args.in.width + at.channel + k] = make_float2(P, Q);
+        for (int w = 0; w < kWarps; ++w) compose(P, Q, shared[w][threadIdx.x]);
+        args.composed[int64_t(at.chunk) * args.in.width + at.channel0 + threadIdx.x] = make_float2(P, Q);
     }
 }
 
 // First pass, backward: E in front of a chunk as a map of E behind it.
-template <typename T, int V>
-__global__ void __launch_bounds__(kComposeWarps * 32, 8) scan_compose_backward_kernel(const ScanArgs args) {
-    constexpr int S = kComposeSteps, W = kComposeWarps;
-    __shared__ float2 shared[W][32 * V];
-    const Place<V, S, W> at(args);
-    Pack<T, V> d[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
-    Rows<T, V>(args.grad_h, args.grad_h_stride, args.in, at).load(at, d);
-    const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
+template <typename T, int V, int PIECE>
+__global__ void __launch_bounds__(kScanBlock, 6) scan_compose_backward_kernel(const ScanArgs args) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    __shared__ float2 shared[kWarps][32 * V];
+    using In = Tile<T, V, PIECE>;
+    const Place<V> at(args);
+    if (at.chunk >= args.chunks) return;
+    const In gs(memory), ds(memory + In::bytes);
+    gs.load(args.in.gate, args.in.gate_stride, args, at);
+    ds.load(args.grad_h, args.grad_h_stride, args, at);
+    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
+    tiles_are_here();
+    const T *g = gs.mine(at), *d = ds.mine(at);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
-    if (edges.last == 0 && at.count == S) {
+    if (edges.last == 0 && at.count == kSteps) {
         #pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-            const Num<V> a = gate_of<V>(gate_exp<V>(number<T, V>(g[i]))).a;
-            H = a * (H + number<T, V>(d[i]));
+        for (int i = kSteps - 1; i >= 0; --i) {
+            const Num<V> a = gate_at<T, V>(g + i * In::kRow).a;
+            H = a * (H + In::get(d + i * In::kRow));
             A = A * a;
         }
     } else {
-        #pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-            if (i >= at.count) continue;
+        #pragma unroll 1
+        for (int i = at.count - 1; i >= 0; --i) {
             if (edges.last >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 A = Num<V>::all(kCut);
                 H = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
             }
-            const Num<V> a = gate_of<V>(gate_exp<V>(number<T, V>(g[i]))).a;
-            H = a * (H + number<T, V>(d[i]));
+            const Num<V> a = gate_at<T, V>(g + i * In::kRow).a;
+            H = a * (H + In::get(d + i * In::kRow));
             A = A * a;
         }
     }
     leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
-    if (at.warp != 0 || !at.inside) return;
-    #pragma unroll
-    for (int k = 0; k < V; ++k) {
+    if (threadIdx.x < 32 * V && at.channel0 + int(threadIdx.x) < args.in.width) {
         float P = 1.0f, Q = 0.0f;
         #pragma unroll
-        for (int w = W - 1; w >= 0; --w) compose(P, Q, shared[w][at.lane * V + k]);
-        args.composed[int64_t(at.chunk) * args.in.width + at.channel + k] = make_float2(P, Q);
+        for (int w = kWarps - 1; w >= 0; --w) compose(P, Q, shared[w][threadIdx.x]);
+        args.composed[int64_t(at.chunk) * args.in.width + at.channel0 + threadIdx.x] = make_float2(P, Q);
     }
 }
 
@@ -379,38 +369,58 @@ __device__ __forceinline__ void pass_empty_sequences(const ScanArgs& args, const
             for (int k = 0; k < v; ++k) to[s * args.in.width + channel + k] = from ? from[s * args.in.width + channel + k] : 0.0f;
 }
 
-// Third pass, forward; from the end, where the first pass has left the rows in L2.
-template <typename T, int V>
-__global__ void __launch_bounds__(kApplyWarps * 32, 4) scan_apply_kernel(const ScanArgs args) {
-    constexpr int S = kApplySteps, W = kApplyWarps;
-    __shared__ float2 shared[W][32 * V];
-    const Place<V, S, W> at(args, true);
-    Pack<T, V> x[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
-    Rows<T, V>(args.in.x, args.in.x_stride, args.in, at).load(at, x);
+// Third pass, forward; from the end, where the first pass has left the rows in L2.  h takes the place of x.
+template <typename T, int V, int PIECE>
+__global__ void __launch_bounds__(kScanBlock, 5) scan_apply_kernel(const ScanArgs args) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    __shared__ float2 shared[kWarps][32 * V];
+    using In = Tile<T, V, PIECE>;
+    const Place<V> at(args, true);
+    if (at.chunk < 0) return;
+    const In gs(memory), xs(memory + In::bytes);
+    gs.load(args.in.gate, args.in.gate_stride, args, at);
+    xs.load(args.in.x, args.in.x_stride, args, at);
     Num<V> h = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
-    const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
-    Num<V> a[S], b[S], A, H;
-    forward_steps<T, V, S>(args, at, edges, x, g, a, b, A, H);
+    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
+    tiles_are_here();
+    const T* g = gs.mine(at);
+    T* x = xs.mine(at);
+    Num<V> a[kSteps], b[kSteps], A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
+    #pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
+        a[i] = gate.a;
+        b[i] = gate.rest * In::get(x + i * In::kRow);
+    }
+    if (edges.first == 0 && at.count == kSteps) {
+        #pragma unroll
+        for (int i = 0; i < kSteps; ++i) { A = A * a[i]; H = madd(a[i], H, b[i]); }
+    } else {
+        #pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (i >= at.count) break;
+            if (edges.first >> i & 1u) {
+                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
+                A = Num<V>::all(kCut);
+                H = b[i] = madd(a[i], load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s)), b[i]);
+            } else { A = A * a[i]; H = madd(a[i], H, b[i]); }
+        }
+    }
     leave_map<V>(&shared[at.warp][at.lane * V], A, H);
     __syncthreads();
     for (int w = 0; w < at.warp; ++w) h = follow<V>(&shared[w][at.lane * V], h);
-    const Rows<T, V> to(args.h, args.h_stride, args.in, at);
-    char* p = to.first;
     if (args.states && at.inside && at.count > 0) store_state<V>(args.states, int64_t(at.p0 / kKept) * args.in.width + at.channel, h);
-    if ((edges.first | edges.last) == 0 && at.count == S) {
-        if (at.inside) {
-            #pragma unroll
-            for (int i = 0; i < S; ++i, p += to.step) {
-                h = madd(a[i], h, b[i]);
-                store_at<T, V>(p, h);
-            }
+    if ((edges.first | edges.last) == 0) {
+        #pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            h = madd(a[i], h, b[i]);
+            In::put(x + i * In::kRow, h);
         }
     } else {
         #pragma unroll
-        for (int i = 0; i < S; ++i, p += to.step) {
+        for (int i = 0; i < kSteps; ++i) {
             h = edges.first >> i & 1u ? b[i] : madd(a[i], h, b[i]);
-            if (at.inside && i < at.count) store_at<T, V>(p, h);
+            In::put(x + i * In::kRow, h);
             if (edges.last >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 if (at.inside) store_state<V>(args.last, at.state_at(args, s), h);
@@ -418,100 +428,95 @@ __global__ void __launch_bounds__(kApplyWarps * 32, 4) scan_apply_kernel(const S
         }
     }
     if (at.warp == 0 && at.inside) pass_empty_sequences(args, args.in.initial, args.last, at.chunk, at.channel, V);
+    __syncthreads();
+    xs.store(args.h, args.h_stride, args, at);
 }
 
-// Third pass, backward: each warp goes eight rows forward from the state that was kept, and back from the E that the warps behind it leave.
-template <typename T, int V>
-__global__ void __launch_bounds__(kApplyWarps * 32, 3) scan_apply_backward_kernel(const ScanArgs args) {
-    constexpr int S = kApplySteps, W = kApplyWarps;
-    __shared__ float2 shared[W][32 * V];
-    const Place<V, S, W> at(args, true);
-    Pack<T, V> x[S], d[S], g[S];
-    Rows<T, V>(args.in.gate, args.in.gate_stride, args.in, at).load(at, g);
-    Rows<T, V>(args.grad_h, args.grad_h_stride, args.in, at).load(at, d);
-    Rows<T, V>(args.in.x, args.in.x_stride, args.in, at).load(at, x);
+// Third pass, backward: each warp goes eight rows forward from the state that was kept, and back from the E that the warps behind it leave.  The gradients
+// take the places of x and gate.
+template <typename T, int V, int PIECE>
+__global__ void __launch_bounds__(kScanBlock, 3) scan_apply_backward_kernel(const ScanArgs args) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    __shared__ float2 shared[kWarps][32 * V];
+    using In = Tile<T, V, PIECE>;
+    const Place<V> at(args, true);
+    if (at.chunk < 0) return;
+    const In gs(memory), xs(memory + In::bytes), ds(memory + 2 * In::bytes);
+    gs.load(args.in.gate, args.in.gate_stride, args, at);
+    ds.load(args.grad_h, args.grad_h_stride, args, at);
+    xs.load(args.in.x, args.in.x_stride, args, at);
     Num<V> h = load_state<V>(at.count > 0 && at.inside ? args.states : nullptr, int64_t(at.p0 / kKept) * args.in.width + at.channel);
     Num<V> E = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
-    const Edges edges = find_edges<S>(args.in, at.p0, at.lane);
-    const bool plain = (edges.first | edges.last) == 0 && at.count == S;
-    Num<V> a[S], rest[S];
+    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
+    tiles_are_here();
+    T *g = gs.mine(at), *x = xs.mine(at);
+    const T* d = ds.mine(at);
+    const bool plain = (edges.first | edges.last) == 0 && at.count == kSteps;
+    Num<V> a[kSteps], rest[kSteps];
     Num<V> P = Num<V>::all(1.0f), Q = Num<V>::all(0.0f);             // E in front of the warp's rows is P E + Q
     #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        const Gate<V> gate = gate_of<V>(gate_exp<V>(number<T, V>(g[i])));
+    for (int i = 0; i < kSteps; ++i) {
+        const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
         a[i] = gate.a; rest[i] = gate.rest;
     }
     if (plain) {
         #pragma unroll
-        for (int i = S - 1; i >= 0; --i) { Q = a[i] * (Q + number<T, V>(d[i])); P = P * a[i]; }
+        for (int i = kSteps - 1; i >= 0; --i) { Q = a[i] * (Q + In::get(d + i * In::kRow)); P = P * a[i]; }
     } else {
         #pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
+        for (int i = kSteps - 1; i >= 0; --i) {
             if (i >= at.count) continue;
             if (edges.last >> i & 1u) {
                 const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
                 P = Num<V>::all(kCut);
                 Q = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
             }
-            Q = a[i] * (Q + number<T, V>(d[i]));
+            Q = a[i] * (Q + In::get(d + i * In::kRow));
             P = P * a[i];
         }
     }
     leave_map<V>(&shared[at.warp][at.lane * V], P, Q);
-    Num<V> slope[S];                          // (h_{t-1} - x) a (1 - a)
+    Num<V> slope[kSteps];                     // (h_{t-1} - x) a (1 - a)
     const Num<V> minus = Num<V>::all(-1.0f);
-    if (edges.first == 0) {
-        #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const Num<V> value = number<T, V>(x[i]);
-            slope[i] = madd(minus, value, h) * (a[i] * rest[i]);
-            h = madd(a[i], h, rest[i] * value);
+    #pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        if (edges.first && (edges.first >> i & 1u)) {
+            const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
+            h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
         }
-    } else {
-        #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (edges.first >> i & 1u) {
-                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-                h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
-            }
-            const Num<V> value = number<T, V>(x[i]);
-            slope[i] = madd(minus, value, h) * (a[i] * rest[i]);
-            h = madd(a[i], h, rest[i] * value);
-        }
+        const Num<V> value = In::get(x + i * In::kRow);
+        slope[i] = madd(minus, value, h) * (a[i] * rest[i]);
+        h = madd(a[i], h, rest[i] * value);
     }
     __syncthreads();
-    for (int w = W - 1; w > at.warp; --w) E = follow<V>(&shared[w][at.lane * V], E);
-    const Rows<T, V> to_x(args.grad_x, args.grad_x_stride, args.in, at), to_gate(args.grad_gate, args.grad_gate_stride, args.in, at);
-    char* px = to_x.first + (S - 1) * to_x.step;
-    char* pg = to_gate.first + (S - 1) * to_gate.step;
+    for (int w = kWarps - 1; w > at.warp; --w) E = follow<V>(&shared[w][at.lane * V], E);
     if (plain) {
-        if (at.inside) {
-            #pragma unroll
-            for (int i = S - 1; i >= 0; --i, px -= to_x.step, pg -= to_gate.step) {
-                const Num<V> D = number<T, V>(d[i]) + E;
-                store_at<T, V>(px, rest[i] * D);
-                store_at<T, V>(pg, slope[i] * D);
-                E = a[i] * D;
-            }
+        #pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i) {
+            const Num<V> D = In::get(d + i * In::kRow) + E;
+            In::put(x + i * In::kRow, rest[i] * D);
+            In::put(g + i * In::kRow, slope[i] * D);
+            E = a[i] * D;
         }
     } else {
         #pragma unroll
-        for (int i = S - 1; i >= 0; --i, px -= to_x.step, pg -= to_gate.step) {
+        for (int i = kSteps - 1; i >= 0; --i) {
             if (i >= at.count) continue;
             const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u;
             int s = 0;
             if (first || last) s = __shfl_sync(0xffffffffu, edges.sequence, i);
             if (last) E = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
-            const Num<V> D = number<T, V>(d[i]) + E;
+            const Num<V> D = In::get(d + i * In::kRow) + E;
+            In::put(x + i * In::kRow, rest[i] * D);
+            In::put(g + i * In::kRow, slope[i] * D);
             E = a[i] * D;
-            if (at.inside) {
-                store_at<T, V>(px, rest[i] * D);
-                store_at<T, V>(pg, slope[i] * D);
-                if (first && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, s), E);
-            }
+            if (first && at.inside && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, s), E);
         }
     }
     if (at.warp == 0 && at.inside) pass_empty_sequences(args, args.grad_last, args.grad_initial, at.chunk, at.channel, V);
+    __syncthreads();
+    xs.store(args.grad_x, args.grad_x_stride, args, at);
+    gs.store(args.grad_gate, args.grad_gate_stride, args, at);
 }
 
 // One step for each row, the state updated in place.
@@ -532,8 +537,6 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const T* __restrict__ x,
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 int64_t pieces(int64_t rows, int piece) { return (rows + piece - 1) / piece; }
 
-bool pairs_possible(const void* p, int64_t stride, int64_t rows, size_t element) { return !p || rows_aligned(p, stride, rows, element, 2 * element); }
-
 void launch_carry(const ScanArgs& args, bool from_end, cudaStream_t stream) {
     int parts = 1;                             // eight chunks in a run, and at most eight blocks
     while (parts < 8 && args.chunks > kCarryWarps * (32 / kCarryChannels) * 8 * parts) parts *= 2;
@@ -546,27 +549,43 @@ void launch_carry(const ScanArgs& args, bool from_end, cudaStream_t stream) {
     cudaLaunchKernelEx(&config, scan_carry_kernel, static_cast<const float2*>(args.composed), args.carried, args.chunks, int(args.in.width), from_end, parts);
 }
 
-template <typename T, int V> void scan_launch(ScanArgs& args, bool backward, cudaStream_t stream) {
-    args.channel_tiles = (args.in.width + 32 * V - 1) / (32 * V);
-    args.chunks = int(pieces(args.in.rows, kChunk));
-    const unsigned int blocks = unsigned(int64_t(args.chunks) * args.channel_tiles);
-    if (args.chunks > 1) {
-        if (backward) scan_compose_backward_kernel<T, V><<<blocks, kComposeWarps * 32, 0, stream>>>(args);
-        else scan_compose_kernel<T, V><<<blocks, kComposeWarps * 32, 0, stream>>>(args);
-        launch_carry(args, backward, stream);
-    }
-    if (backward) scan_apply_backward_kernel<T, V><<<blocks, kApplyWarps * 32, 0, stream>>>(args);
-    else scan_apply_kernel<T, V><<<blocks, kApplyWarps * 32, 0, stream>>>(args);
+template <typename K> cudaError_t launch_chunks(K kernel, PerDeviceOnce& once, const ScanArgs& args, int tiles, int smem, cudaStream_t stream) {
+    const cudaError_t err = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    if (err != cudaSuccess) return err;
+    const dim3 grid(unsigned(tiles), unsigned(args.chunks < kGridRows ? args.chunks : kGridRows), unsigned((args.chunks + kGridRows - 1) / kGridRows));
+    kernel<<<grid, kScanBlock, smem, stream>>>(args);
+    return cudaSuccess;
 }
 
-// Two channels a lane where every row allows it.
-template <typename T> void scan_typed(ScanArgs& a, bool backward, cudaStream_t stream) {
-    const int64_t rows = a.in.rows;
-    const size_t e = sizeof(T);
-    const bool pairs = a.in.width % 2 == 0 && pairs_possible(a.in.x, a.in.x_stride, rows, e) && pairs_possible(a.in.gate, a.in.gate_stride, rows, e) &&
-                       pairs_possible(a.h, a.h_stride, rows, e) && pairs_possible(a.grad_h, a.grad_h_stride, rows, e) &&
-                       pairs_possible(a.grad_x, a.grad_x_stride, rows, e) && pairs_possible(a.grad_gate, a.grad_gate_stride, rows, e);
-    if (pairs) scan_launch<T, 2>(a, backward, stream); else scan_launch<T, 1>(a, backward, stream);
+template <typename T, int V, int PIECE> cudaError_t scan_launch(ScanArgs& args, bool backward, cudaStream_t stream) {
+    static PerDeviceOnce compose, apply, compose_backward, apply_backward;
+    constexpr int bytes = Tile<T, V, PIECE>::bytes;
+    const int tiles = (args.in.width + 32 * V - 1) / (32 * V);
+    args.chunks = int(pieces(args.in.rows, kChunk));
+    cudaError_t err = cudaSuccess;
+    if (args.chunks > 1) {
+        err = backward ? launch_chunks(scan_compose_backward_kernel<T, V, PIECE>, compose_backward, args, tiles, 2 * bytes, stream)
+                       : launch_chunks(scan_compose_kernel<T, V, PIECE>, compose, args, tiles, 2 * bytes, stream);
+        if (err == cudaSuccess) launch_carry(args, backward, stream);
+    }
+    if (err != cudaSuccess) return err;
+    return backward ? launch_chunks(scan_apply_backward_kernel<T, V, PIECE>, apply_backward, args, tiles, 3 * bytes, stream)
+                    : launch_chunks(scan_apply_kernel<T, V, PIECE>, apply, args, tiles, 2 * bytes, stream);
+}
+
+// Two channels a lane where every row allows it, in pieces of 16 bytes where they do too.
+template <typename T> int scan_typed(ScanArgs& a, bool backward, cudaStream_t stream) {
+    const auto allow = [&](size_t bytes) {
+        const auto one = [&](const void* p, int64_t stride) { return !p || rows_aligned(p, stride, a.in.rows, sizeof(T), bytes); };
+        return size_t(a.in.width) * sizeof(T) % bytes == 0 && one(a.in.x, a.in.x_stride) && one(a.in.gate, a.in.gate_stride) && one(a.h, a.h_stride) &&
+               one(a.grad_h, a.grad_h_stride) && one(a.grad_x, a.grad_x_stride) && one(a.grad_gate, a.grad_gate_stride);
+    };
+    cudaError_t err;
+    if (allow(16)) err = scan_launch<T, 2, 16>(a, backward, stream);
+    else if constexpr (sizeof(T) == 4) err = scan_launch<T, 1, 4>(a, backward, stream);
+    else if (allow(4)) err = scan_launch<T, 2, 4>(a, backward, stream);
+    else err = scan_launch<T, 1, 2>(a, backward, stream);
+    return err == cudaSuccess ? sequence_status("htgs_gated_scan") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
 constexpr int64_t kMostStride = 1 << 22;      // elements: 128 rows of it are within 32 bits' worth of bytes
@@ -618,10 +637,9 @@ int htgs_gated_scan(const HtgsScan* scan, void* h, int64_t h_stride, float* last
     a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(pieces(scan->rows, kChunk)) * size_t(scan->width) * sizeof(float2)));
     a.states = states;
     a.h = h; a.h_stride = h_stride; a.last = last;
-    if (scan->type == HTGS_FLOAT32) scan_typed<float>(a, false, s);
-    else if (scan->type == HTGS_FLOAT16) scan_typed<__half>(a, false, s);
-    else scan_typed<__nv_bfloat16>(a, false, s);
-    return sequence_status("htgs_gated_scan");
+    if (scan->type == HTGS_FLOAT32) return scan_typed<float>(a, false, s);
+    if (scan->type == HTGS_FLOAT16) return scan_typed<__half>(a, false, s);
+    return scan_typed<__nv_bfloat16>(a, false, s);
 }
 
 int htgs_gated_scan_backward(const HtgsScan* scan, const float* states, const void* grad_h, int64_t grad_h_stride, const float* grad_last, void* grad_x,
@@ -643,10 +661,9 @@ int htgs_gated_scan_backward(const HtgsScan* scan, const float* states, const vo
     a.states = const_cast<float*>(states);
     a.grad_h = grad_h; a.grad_h_stride = grad_h_stride; a.grad_last = grad_last;
     a.grad_x = grad_x; a.grad_x_stride = grad_x_stride; a.grad_gate = grad_gate; a.grad_gate_stride = grad_gate_stride; a.grad_initial = grad_initial;
-    if (scan->type == HTGS_FLOAT32) scan_typed<float>(a, true, s);
-    else if (scan->type == HTGS_FLOAT16) scan_typed<__half>(a, true, s);
-    else scan_typed<__nv_bfloat16>(a, true, s);
-    return sequence_status("htgs_gated_scan_backward");
+    if (scan->type == HTGS_FLOAT32) return scan_typed<float>(a, true, s);
+    if (scan->type == HTGS_FLOAT16) return scan_typed<__half>(a, true, s);
+    return scan_typed<__nv_bfloat16>(a, true, s);
 }
 
 int htgs_gated_scan_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride, float* state, int64_t state_stride, void* h,
