@@ -4,30 +4,30 @@
 //   backward, from the last row to the first:  D_t = grad_h_t + E_{t+1};   E_t = a_t D_t   (E behind the last row: the last state's gradient)
 //       grad_x = (1 - a) D;   grad_gate = D (h_{t-1} - x) a (1 - a);   grad_initial = E at the first row
 //
-// A step is the map h -> A h + H, and steps compose: (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2).  The rows are cut into chunks of
-// 128.  One kernel composes each chunk's rows, one walks from chunk to chunk and leaves the state in front of each, one goes through
-// the chunks again from those states and writes h.  The backward pass does the same from the end; h_{t-1} is computed again from the
-// chunks' states, so it is in 32 bits and h need not be read.  A sequence's first row has A = 0 and takes its initial state into H, so
-// packed sequences need no chunks of their own; that zero is kept as
-// -0 and tested for, so that a NaN or infinity of one sequence does not reach the next.  States, products and sums are 32-bit; 1 - a is exp(-gate) a, which keeps its relative precision
-// where a is close to 1.
+// A step is the map h -> A h + H, and steps compose: (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2).  The rows are cut into chunks of 16 to 64.  One
+// kernel composes each chunk's rows, one walks from chunk to chunk and leaves the state in front of each, one goes through the
+// chunks again from those states and writes h.  The backward pass does the same from the end.  A warp takes a chunk of 32 or 64 channels and goes
+// through it eight rows at a time, the next sixteen on their way into shared memory of its own; warps never wait for one another.  For the backward pass the
+// forward one keeps the state in front of every eight rows: h_{t-1} is computed again from there, so it is in 32 bits and neither h nor the rows
+// before are read.  A sequence's first row has A = 0 and takes its initial state into H, so packed sequences need no chunks of their own; that zero is
+// kept as -0 and tested for, so that a NaN or infinity of one sequence does not reach the next.  States, products and sums are 32-bit; 1 - a is
+// exp(-gate) a, which keeps its relative precision where a is close to 1.
+//
 #include "sequence.cuh"
 
 namespace htgs {
 
 namespace {
 
-// A block takes a chunk of 32 or 64 channels; each of its warps takes some rows of it.
-constexpr int kChunk = 64;                                                       // rows
-constexpr int kSteps = 8, kWarps = kChunk / kSteps;                              // rows of a warp
-constexpr int kScanBlock = kWarps * 32;
-constexpr int kKept = 8;                     // a state for every so many rows is kept for the backward pass
+constexpr int kBatch = 8;                    // rows that a warp deals with at a time; a state in front of each batch is kept for the backward pass
+constexpr int kMostChunk = 64;               // rows
+constexpr int kStages = 3;                   // batches of a warp in shared memory
+constexpr int kScanWarps = 4, kScanBlock = kScanWarps * 32;
 constexpr int kCarryWarps = 32, kCarryChannels = 8, kCarryRun = 16;
-static_assert(kSteps == kKept, "a warp keeps one state, and begins with it in the backward pass");
 
 struct ScanArgs {
     HtgsScan in;
-    int chunks;
+    int chunk, chunks, channel_tiles;        // rows of a chunk, chunks, and warps side by side
     float2* composed;                        // [chunks, width]
     float* carried;                          // [chunks, width] state in front of each chunk (backward: E behind it); nothing where there is one chunk
     float* states;                           // [ceil(rows / 8), width] state in front of every eight rows, or null
@@ -108,37 +108,39 @@ template <int V> __device__ __forceinline__ void leave_map(float2* to, Num<V> A,
     for (int k = 0; k < V; ++k) to[k] = make_float2(A[k], H[k]);
 }
 
-// Which of the warp's `STEPS` steps are the first or last of their sequence (bits), and in lane i the sequence of step i.
-struct Edges { unsigned int first, last; int sequence; };
-template <int STEPS> __device__ __forceinline__ Edges find_edges(const HtgsScan& in, int64_t p0, int lane) {
-    const int64_t p = p0 + lane;
-    // one sequence: only its first and last position have an edge
-    if (!in.offsets && in.n_sequences == 1) {
-        const int64_t end = in.rows - 1 - p0;
-        return {p0 == 0 ? 1u : 0u, end >= 0 && end < STEPS ? 1u << end : 0u, 0};
+// Positions p count the rows in the order of the recurrence: row p, or rows - 1 - p in reverse.
+// The sequence that holds a position, by its first position and the one behind its last.
+struct Span {
+    int sequence, begin, end;
+    __device__ __forceinline__ void set(const HtgsScan& in) {
+        int64_t lo, hi;
+        if (in.offsets) { lo = __ldg(in.offsets + sequence); hi = __ldg(in.offsets + sequence + 1); }
+        else { const int64_t length = in.n_sequences == 1 ? in.rows : in.rows / in.n_sequences; lo = sequence * length; hi = lo + length; }
+        begin = int(in.reverse ? in.rows - hi : lo);
+        end = int(in.reverse ? in.rows - lo : hi);
     }
-    bool first = false, last = false;
-    int s = 0;
-    if (lane < STEPS && p < in.rows) {
+    __device__ __forceinline__ void find(const HtgsScan& in, int p) {
         const int64_t row = in.reverse ? in.rows - 1 - p : p;
-        int64_t begin, end;
+        sequence = 0;
         if (in.offsets) {
             int hi = in.n_sequences;
-            while (hi - s > 1) {
-                const int mid = (s + hi) >> 1;
-                if (__ldg(in.offsets + mid) <= row) s = mid; else hi = mid;
+            while (hi - sequence > 1) {
+                const int mid = (sequence + hi) >> 1;
+                if (__ldg(in.offsets + mid) <= row) sequence = mid; else hi = mid;
             }
-            begin = __ldg(in.offsets + s); end = __ldg(in.offsets + s + 1);
-        } else {
-            const int64_t length = in.rows / in.n_sequences;
-            s = int(row / length);
-            begin = s * length; end = begin + length;
+        } else if (in.n_sequences > 1) {
+            sequence = int(row / (in.rows / in.n_sequences));
         }
-        first = row == begin; last = row + 1 == end;
-        if (in.reverse) { const bool swap = first; first = last; last = swap; }
+        set(in);
     }
-    return {__ballot_sync(0xffffffffu, first), __ballot_sync(0xffffffffu, last), s};
-}
+    // The next sequence that has rows; forward: behind this one in the order of the recurrence, else in front of it.
+    __device__ __forceinline__ void move(const HtgsScan& in, bool forward) {
+        const int step = forward != (in.reverse != 0) ? 1 : -1;
+        do sequence += step; while (sequence >= 0 && sequence < in.n_sequences && in.offsets && __ldg(in.offsets + sequence + 1) <= __ldg(in.offsets + sequence));
+        if (sequence >= 0 && sequence < in.n_sequences) set(in);
+        else { sequence = sequence < 0 ? 0 : in.n_sequences - 1; begin = end = -1; }
+    }
+};
 
 template <int V> __device__ __forceinline__ Num<V> load_state(const float* states, int64_t at) {
     float f[V];
@@ -151,155 +153,184 @@ template <int V> __device__ __forceinline__ void store_state(float* states, int6
     for (int k = 0; k < V; ++k) states[at + k] = n[k];
 }
 
-// Where a thread works: V channels side by side, kSteps rows from position p0 on (positions count rows in the order of the recurrence), `count` of which exist.
-constexpr int kGridRows = 32768;              // chunks along the grid's y, the rest along z
+// Where a thread works: V channels side by side, positions begin to end - 1.
 template <int V> struct Place {
-    int lane, warp, channel0, channel, count, p0, chunk;
+    int lane, warp, channel0, channel, chunk, begin, end;
     bool inside;
     __device__ __forceinline__ explicit Place(const ScanArgs& a, bool from_end = false) {
-        lane = threadIdx.x & 31; warp = threadIdx.x >> 5;
-        const int at = int(blockIdx.z * kGridRows + blockIdx.y);
-        chunk = from_end ? a.chunks - 1 - at : at;
-        channel0 = int(blockIdx.x) * 32 * V;
+        lane = threadIdx.x & 31; warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
+        const unsigned int unit = blockIdx.x * kScanWarps + warp, at = unit / unsigned(a.channel_tiles);     // neighbouring channels of a chunk, then the next chunk's
+        chunk = from_end ? a.chunks - 1 - int(at) : int(at);
+        channel0 = int(unit - at * unsigned(a.channel_tiles)) * 32 * V;
         channel = channel0 + lane * V;
         inside = channel < a.in.width;
-        p0 = chunk * kChunk + warp * kSteps;
-        count = max(0, min(kSteps, int(a.in.rows) - p0));
+        begin = chunk * a.chunk;
+        end = at >= unsigned(a.chunks) ? begin : int(min(int64_t(begin) + a.chunk, a.in.rows));
     }
+    __device__ __forceinline__ bool nothing() const { return end <= begin; }
+    __device__ __forceinline__ int last_batch() const { return begin + (end - 1 - begin) / kBatch * kBatch; }
     __device__ __forceinline__ int64_t state_at(const ScanArgs& a, int sequence) const { return int64_t(sequence) * a.in.width + channel; }
 };
 
-// A chunk of 32 V channels in shared memory, one row per position, brought and taken away PIECE bytes at a time: 16 where every row of the matrix
-// allows it, or 4, or a single 16-bit value.
-template <typename T, int V, int PIECE> struct Tile {
-    static constexpr int kRow = 32 * V, kElements = PIECE / int(sizeof(T)), kPieces = kRow / kElements, kRowsAtOnce = kScanBlock / kPieces, kTrips = kChunk / kRowsAtOnce;
-    static constexpr int bytes = kChunk * kRow * int(sizeof(T));
-    T* data;
-    __device__ __forceinline__ explicit Tile(unsigned char* at) : data(reinterpret_cast<T*>(at)) {}
-    // f(address in the matrix, address here, whether the piece exists), for each of the thread's pieces
-    template <typename F> __device__ __forceinline__ void each(const void* base, int64_t stride, const ScanArgs& a, const Place<V>& at, F f) const {
-        const int r = int(threadIdx.x) / kPieces, c = int(threadIdx.x) % kPieces * kElements, left = int(a.in.rows) - at.chunk * kChunk;
-        const int64_t position = int64_t(at.chunk) * kChunk + r, row = a.in.reverse ? a.in.rows - 1 - position : position;
-        const int64_t step = (a.in.reverse ? -stride : stride) * kRowsAtOnce;
-        T* there = static_cast<T*>(const_cast<void*>(base)) + row * stride + at.channel0 + c;
-        const bool inside = at.channel0 + c < a.in.width;
-        T* here = data + r * kRow + c;
-        #pragma unroll
-        for (int i = 0; i < kTrips; ++i, there += step, here += kRowsAtOnce * kRow) f(there, here, inside && r + i * kRowsAtOnce < left);
+// A matrix's rows at a warp's channels on their way into its shared memory, a batch at a time, PIECE bytes at once: 16 where every row of the matrix allows it, or
+// 4.  PIECE 2 is for 16-bit rows that begin on 2 bytes: the 4-byte words that hold a row are copied, and its values lie 0 or 2 bytes behind the first.
+template <typename T, int V, int PIECE> struct Stream {
+    static constexpr int kRow = PIECE == 2 ? 68 : 32 * V * int(sizeof(T));         // bytes
+    static constexpr int bytes = kBatch * kRow;
+    static constexpr int kPieces = PIECE == 2 ? 17 : kRow / PIECE;
+    const char* first;                        // the channels' first value at position 0
+    int64_t step;                             // bytes from position to position
+    int valid;                                // bytes of a row that exist
+    __device__ __forceinline__ Stream(const void* base, int64_t stride, const ScanArgs& a, const Place<V>& at) {
+        first = static_cast<const char*>(base) + ((a.in.reverse ? (a.in.rows - 1) * stride : 0) + at.channel0) * int64_t(sizeof(T));
+        step = (a.in.reverse ? -stride : stride) * int64_t(sizeof(T));
+        valid = min(32 * V, a.in.width - at.channel0) * int(sizeof(T));
     }
-    // What does not exist becomes zero.
-    __device__ __forceinline__ void load(const void* base, int64_t stride, const ScanArgs& a, const Place<V>& at) const {
-        each(base, stride, a, at, [&](T* there, T* here, bool exists) {
-            if constexpr (PIECE == 16)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(here)), "l"(exists ? there : base), "r"(exists ? 16 : 0) : "memory");
-            else if constexpr (PIECE == 4)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(here)), "l"(exists ? there : base), "r"(exists ? 4 : 0) : "memory");
-            else *here = exists ? *there : from_float<T>(0.0f);
-        });
+    __device__ __forceinline__ void copy(unsigned char* to, int p, int count, int lane) const {
+        if constexpr (PIECE == 2) {
+            #pragma unroll
+            for (int i = 0; i < (kBatch * kPieces + 31) / 32; ++i) {
+                const int q = lane + 32 * i, r = q / kPieces, w = q % kPieces;
+                const uintptr_t row = reinterpret_cast<uintptr_t>(first + (p + r) * step), word = (row & ~uintptr_t(3)) + 4 * w;
+                if (r < count && word < row + valid) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to + r * kRow + 4 * w)), "l"(word) : "memory");
+            }
+        } else {
+            constexpr int kAtOnce = 32 / kPieces;                 // rows
+            const int r = lane / kPieces, c = lane % kPieces * PIECE;
+            const char* from = first + (p + r) * step + c;
+            const uint32_t here = smem_u32(to) + uint32_t(r * kRow + c);
+            const int there = c < valid ? count - r : 0;
+            #pragma unroll
+            for (int i = 0; i < kBatch / kAtOnce; ++i, from += kAtOnce * step) {
+                if (i * kAtOnce >= there) continue;
+                if constexpr (PIECE == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(here + i * kAtOnce * kRow), "l"(from) : "memory");
+                else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(here + i * kAtOnce * kRow), "l"(from) : "memory");
+            }
+        }
     }
-    __device__ __forceinline__ void store(void* base, int64_t stride, const ScanArgs& a, const Place<V>& at) const {
-        each(base, stride, a, at, [&](T* there, T* here, bool exists) {
-            if (exists) *reinterpret_cast<Pack<T, kElements>*>(there) = *reinterpret_cast<const Pack<T, kElements>*>(here);
-        });
+    // The thread's channels of row i of a batch that begins at position p.
+    __device__ __forceinline__ Num<V> get(const unsigned char* stage, int p, int i, int lane) const {
+        if constexpr (PIECE == 2) {
+            const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(first)) + uint32_t(p + i) * uint32_t(step) & 2u;
+            return number<T, V>(*reinterpret_cast<const Pack<T, V>*>(stage + i * kRow + off + lane * V * int(sizeof(T))));
+        } else {
+            return number<T, V>(*reinterpret_cast<const Pack<T, V>*>(stage + i * kRow + lane * V * int(sizeof(T))));
+        }
     }
-    __device__ __forceinline__ T* mine(const Place<V>& at) const { return data + at.warp * kSteps * kRow + at.lane * V; }       // the thread's values: every kRow from here
-    __device__ __forceinline__ static Num<V> get(const T* p) { return number<T, V>(*reinterpret_cast<const Pack<T, V>*>(p)); }
-    __device__ __forceinline__ static void put(T* p, Num<V> n) { store_number<T, V>(p, n); }
 };
-__device__ __forceinline__ void tiles_are_here() {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-}
-template <typename T, int V> __device__ __forceinline__ Gate<V> gate_at(const T* p) { return gate_of<V>(gate_exp<V>(number<T, V>(*reinterpret_cast<const Pack<T, V>*>(p)))); }
+
+// N streams through a ring of stages.  The batches are at positions p, p + kBatch * way, ..., `left` of them.
+template <typename S, int N> struct Feed {
+    const S (&streams)[N];
+    unsigned char* ring;
+    int lane, begin, end, p, left, to = 0, from = 0;
+    bool back;
+    __device__ __forceinline__ void send() {
+        if (left > 0) {
+            #pragma unroll
+            for (int n = 0; n < N; ++n) streams[n].copy(ring + (to * N + n) * S::bytes, p, min(kBatch, end - p), lane);
+            p += back ? -kBatch : kBatch;
+            --left;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        to = to + 1 == kStages ? 0 : to + 1;
+    }
+    __device__ __forceinline__ Feed(const S (&s)[N], unsigned char* memory, int lane_, int begin_, int end_, bool back_)
+        : streams(s), ring(memory), lane(lane_), begin(begin_), end(end_), back(back_) {
+        left = (end - begin + kBatch - 1) / kBatch;
+        p = back ? begin + (left - 1) * kBatch : begin;
+        #pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) send();
+    }
+    // The next batch's place; what was in the stage behind it may be overwritten from here on.
+    __device__ __forceinline__ const unsigned char* next() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        const unsigned char* stage = ring + from * N * S::bytes;
+        from = from + 1 == kStages ? 0 : from + 1;
+        send();
+        return stage;
+    }
+};
+
+template <typename T, int V, int PIECE, int N> constexpr int kFeedBytes = kScanWarps * kStages * N * Stream<T, V, PIECE>::bytes;
 
 // First pass, forward: the composition of each chunk.
 template <typename T, int V, int PIECE>
-__global__ void __launch_bounds__(kScanBlock, 6) scan_compose_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kScanBlock, 10) scan_compose_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ float2 shared[kWarps][32 * V];
-    using In = Tile<T, V, PIECE>;
+    using S = Stream<T, V, PIECE>;
     const Place<V> at(args);
-    if (at.chunk >= args.chunks) return;
-    const In gs(memory), xs(memory + In::bytes);
-    gs.load(args.in.gate, args.in.gate_stride, args, at);
-    xs.load(args.in.x, args.in.x_stride, args, at);
-    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
-    tiles_are_here();
-    const T *g = gs.mine(at), *x = xs.mine(at);
+    if (at.nothing()) return;
+    const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at)};
+    Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, false);
+    Span span;
+    span.find(args.in, at.begin);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
-    if (edges.first == 0 && at.count == kSteps) {
-        #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
-            H = madd(gate.a, H, gate.rest * In::get(x + i * In::kRow));
-            A = A * gate.a;
-        }
-    } else {
-        #pragma unroll 1
-        for (int i = 0; i < at.count; ++i) {
-            if (edges.first >> i & 1u) {
-                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-                A = Num<V>::all(kCut);
-                H = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
+    #pragma unroll 1
+    for (int p = at.begin; p < at.end; p += kBatch) {
+        const unsigned char *g = feed.next(), *x = g + S::bytes;
+        if (at.end - p >= kBatch && span.begin < p && span.end >= p + kBatch) {
+            #pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                H = madd(gate.a, H, gate.rest * streams[1].get(x, p, i, at.lane));
+                A = A * gate.a;
             }
-            const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
-            H = madd(gate.a, H, gate.rest * In::get(x + i * In::kRow));
-            A = A * gate.a;
+        } else {
+            #pragma unroll 1
+            for (int i = 0; i < min(kBatch, at.end - p); ++i) {
+                if (p + i == span.end) span.move(args.in, true);
+                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                if (p + i == span.begin) {
+                    A = Num<V>::all(kCut);
+                    H = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, span.sequence));
+                }
+                H = madd(gate.a, H, gate.rest * streams[1].get(x, p, i, at.lane));
+                A = A * gate.a;
+            }
         }
     }
-    leave_map<V>(&shared[at.warp][at.lane * V], A, H);
-    __syncthreads();
-    if (threadIdx.x < 32 * V && at.channel0 + int(threadIdx.x) < args.in.width) {
-        float P = 1.0f, Q = 0.0f;
-        #pragma unroll
-        for (int w = 0; w < kWarps; ++w) compose(P, Q, shared[w][threadIdx.x]);
-        args.composed[int64_t(at.chunk) * args.in.width + at.channel0 + threadIdx.x] = make_float2(P, Q);
-    }
+    if (at.inside) leave_map<V>(&args.composed[int64_t(at.chunk) * args.in.width + at.channel], A, H);
 }
 
 // First pass, backward: E in front of a chunk as a map of E behind it.
 template <typename T, int V, int PIECE>
-__global__ void __launch_bounds__(kScanBlock, 6) scan_compose_backward_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kScanBlock, 10) scan_compose_backward_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ float2 shared[kWarps][32 * V];
-    using In = Tile<T, V, PIECE>;
+    using S = Stream<T, V, PIECE>;
     const Place<V> at(args);
-    if (at.chunk >= args.chunks) return;
-    const In gs(memory), ds(memory + In::bytes);
-    gs.load(args.in.gate, args.in.gate_stride, args, at);
-    ds.load(args.grad_h, args.grad_h_stride, args, at);
-    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
-    tiles_are_here();
-    const T *g = gs.mine(at), *d = ds.mine(at);
+    if (at.nothing()) return;
+    const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.grad_h, args.grad_h_stride, args, at)};
+    Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, true);
+    Span span;
+    span.find(args.in, at.end - 1);
     Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
-    if (edges.last == 0 && at.count == kSteps) {
-        #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i) {
-            const Num<V> a = gate_at<T, V>(g + i * In::kRow).a;
-            H = a * (H + In::get(d + i * In::kRow));
-            A = A * a;
-        }
-    } else {
-        #pragma unroll 1
-        for (int i = at.count - 1; i >= 0; --i) {
-            if (edges.last >> i & 1u) {
-                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-                A = Num<V>::all(kCut);
-                H = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
+    #pragma unroll 1
+    for (int p = at.last_batch(); p >= at.begin; p -= kBatch) {
+        const unsigned char *g = feed.next(), *d = g + S::bytes;
+        if (at.end - p >= kBatch && span.begin <= p && span.end > p + kBatch) {
+            #pragma unroll
+            for (int i = kBatch - 1; i >= 0; --i) {
+                const Num<V> a = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane))).a;
+                H = a * (H + streams[1].get(d, p, i, at.lane));
+                A = A * a;
             }
-            const Num<V> a = gate_at<T, V>(g + i * In::kRow).a;
-            H = a * (H + In::get(d + i * In::kRow));
-            A = A * a;
+        } else {
+            #pragma unroll 1
+            for (int i = min(kBatch, at.end - p) - 1; i >= 0; --i) {
+                if (p + i < span.begin) span.move(args.in, false);
+                const Num<V> a = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane))).a;
+                if (p + i + 1 == span.end) {
+                    A = Num<V>::all(kCut);
+                    H = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, span.sequence));
+                }
+                H = a * (H + streams[1].get(d, p, i, at.lane));
+                A = A * a;
+            }
         }
     }
-    leave_map<V>(&shared[at.warp][at.lane * V], A, H);
-    __syncthreads();
-    if (threadIdx.x < 32 * V && at.channel0 + int(threadIdx.x) < args.in.width) {
-        float P = 1.0f, Q = 0.0f;
-        #pragma unroll
-        for (int w = kWarps - 1; w >= 0; --w) compose(P, Q, shared[w][threadIdx.x]);
-        args.composed[int64_t(at.chunk) * args.in.width + at.channel0 + threadIdx.x] = make_float2(P, Q);
-    }
+    if (at.inside) leave_map<V>(&args.composed[int64_t(at.chunk) * args.in.width + at.channel], A, H);
 }
 
 // Second pass: the state at each chunk's beginning (from_end: behind each chunk, walking from the last to the first).  A cluster of `parts` blocks takes eight
@@ -369,154 +400,123 @@ __device__ __forceinline__ void pass_empty_sequences(const ScanArgs& args, const
             for (int k = 0; k < v; ++k) to[s * args.in.width + channel + k] = from ? from[s * args.in.width + channel + k] : 0.0f;
 }
 
-// Third pass, forward; from the end, where the first pass has left the rows in L2.  h takes the place of x.
+// Third pass, forward; from the end, where the first pass has left the rows in L2.
 template <typename T, int V, int PIECE>
-__global__ void __launch_bounds__(kScanBlock, 5) scan_apply_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kScanBlock, 8) scan_apply_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ float2 shared[kWarps][32 * V];
-    using In = Tile<T, V, PIECE>;
+    using S = Stream<T, V, PIECE>;
     const Place<V> at(args, true);
-    if (at.chunk < 0) return;
-    const In gs(memory), xs(memory + In::bytes);
-    gs.load(args.in.gate, args.in.gate_stride, args, at);
-    xs.load(args.in.x, args.in.x_stride, args, at);
+    if (at.nothing()) return;
+    const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at)};
+    Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, false);
     Num<V> h = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
-    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
-    tiles_are_here();
-    const T* g = gs.mine(at);
-    T* x = xs.mine(at);
-    Num<V> a[kSteps], b[kSteps], A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
-    #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
-        a[i] = gate.a;
-        b[i] = gate.rest * In::get(x + i * In::kRow);
-    }
-    if (edges.first == 0 && at.count == kSteps) {
-        #pragma unroll
-        for (int i = 0; i < kSteps; ++i) { A = A * a[i]; H = madd(a[i], H, b[i]); }
-    } else {
-        #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            if (i >= at.count) break;
-            if (edges.first >> i & 1u) {
-                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-                A = Num<V>::all(kCut);
-                H = b[i] = madd(a[i], load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s)), b[i]);
-            } else { A = A * a[i]; H = madd(a[i], H, b[i]); }
-        }
-    }
-    leave_map<V>(&shared[at.warp][at.lane * V], A, H);
-    __syncthreads();
-    for (int w = 0; w < at.warp; ++w) h = follow<V>(&shared[w][at.lane * V], h);
-    if (args.states && at.inside && at.count > 0) store_state<V>(args.states, int64_t(at.p0 / kKept) * args.in.width + at.channel, h);
-    if ((edges.first | edges.last) == 0) {
-        #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            h = madd(a[i], h, b[i]);
-            In::put(x + i * In::kRow, h);
-        }
-    } else {
-        #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            h = edges.first >> i & 1u ? b[i] : madd(a[i], h, b[i]);
-            In::put(x + i * In::kRow, h);
-            if (edges.last >> i & 1u) {
-                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-                if (at.inside) store_state<V>(args.last, at.state_at(args, s), h);
+    Span span;
+    span.find(args.in, at.begin);
+    const int64_t step = args.in.reverse ? -args.h_stride : args.h_stride;
+    T* to = static_cast<T*>(args.h) + (args.in.reverse ? args.in.rows - 1 - at.begin : at.begin) * args.h_stride + at.channel;
+    #pragma unroll 1
+    for (int p = at.begin; p < at.end; p += kBatch) {
+        const unsigned char *g = feed.next(), *x = g + S::bytes;
+        if (args.states && at.inside) store_state<V>(args.states, int64_t(p / kBatch) * args.in.width + at.channel, h);
+        if (at.end - p >= kBatch && span.begin < p && span.end > p + kBatch) {
+            #pragma unroll
+            for (int i = 0; i < kBatch; ++i, to += step) {
+                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                h = madd(gate.a, h, gate.rest * streams[1].get(x, p, i, at.lane));
+                if (at.inside) store_number<T, V>(to, h);
+            }
+        } else {
+            #pragma unroll 1
+            for (int i = 0; i < min(kBatch, at.end - p); ++i, to += step) {
+                if (p + i == span.end) span.move(args.in, true);
+                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                if (p + i == span.begin) h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, span.sequence));
+                h = madd(gate.a, h, gate.rest * streams[1].get(x, p, i, at.lane));
+                if (at.inside) {
+                    store_number<T, V>(to, h);
+                    if (p + i + 1 == span.end) store_state<V>(args.last, at.state_at(args, span.sequence), h);
+                }
             }
         }
     }
-    if (at.warp == 0 && at.inside) pass_empty_sequences(args, args.in.initial, args.last, at.chunk, at.channel, V);
-    __syncthreads();
-    xs.store(args.h, args.h_stride, args, at);
+    if (at.inside) pass_empty_sequences(args, args.in.initial, args.last, at.chunk, at.channel, V);
 }
 
-// Third pass, backward: each warp goes eight rows forward from the state that was kept, and back from the E that the warps behind it leave.  The gradients
-// take the places of x and gate.
+// Third pass, backward: eight rows forward from the state that was kept, then back.
 template <typename T, int V, int PIECE>
-__global__ void __launch_bounds__(kScanBlock, 3) scan_apply_backward_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kScanBlock, 6) scan_apply_backward_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ float2 shared[kWarps][32 * V];
-    using In = Tile<T, V, PIECE>;
+    using S = Stream<T, V, PIECE>;
     const Place<V> at(args, true);
-    if (at.chunk < 0) return;
-    const In gs(memory), xs(memory + In::bytes), ds(memory + 2 * In::bytes);
-    gs.load(args.in.gate, args.in.gate_stride, args, at);
-    ds.load(args.grad_h, args.grad_h_stride, args, at);
-    xs.load(args.in.x, args.in.x_stride, args, at);
-    Num<V> h = load_state<V>(at.count > 0 && at.inside ? args.states : nullptr, int64_t(at.p0 / kKept) * args.in.width + at.channel);
+    if (at.nothing()) return;
+    const S streams[3] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at), S(args.grad_h, args.grad_h_stride, args, at)};
+    Feed<S, 3> feed(streams, memory + at.warp * kStages * 3 * S::bytes, at.lane, at.begin, at.end, true);
+    int p = at.last_batch();
+    Num<V> kept = load_state<V>(at.inside ? args.states : nullptr, int64_t(p / kBatch) * args.in.width + at.channel);
     Num<V> E = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
-    const Edges edges = find_edges<kSteps>(args.in, at.p0, at.lane);
-    tiles_are_here();
-    T *g = gs.mine(at), *x = xs.mine(at);
-    const T* d = ds.mine(at);
-    const bool plain = (edges.first | edges.last) == 0 && at.count == kSteps;
-    Num<V> a[kSteps], rest[kSteps];
-    Num<V> P = Num<V>::all(1.0f), Q = Num<V>::all(0.0f);             // E in front of the warp's rows is P E + Q
-    #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const Gate<V> gate = gate_at<T, V>(g + i * In::kRow);
-        a[i] = gate.a; rest[i] = gate.rest;
-    }
-    if (plain) {
-        #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i) { Q = a[i] * (Q + In::get(d + i * In::kRow)); P = P * a[i]; }
-    } else {
-        #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i) {
-            if (i >= at.count) continue;
-            if (edges.last >> i & 1u) {
-                const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-                P = Num<V>::all(kCut);
-                Q = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
-            }
-            Q = a[i] * (Q + In::get(d + i * In::kRow));
-            P = P * a[i];
-        }
-    }
-    leave_map<V>(&shared[at.warp][at.lane * V], P, Q);
-    Num<V> slope[kSteps];                     // (h_{t-1} - x) a (1 - a)
+    Span span;
+    span.find(args.in, at.end - 1);
+    const int64_t step_x = args.in.reverse ? -args.grad_x_stride : args.grad_x_stride, step_gate = args.in.reverse ? -args.grad_gate_stride : args.grad_gate_stride;
+    const int64_t row = args.in.reverse ? args.in.rows - at.end : at.end - 1;
+    T* to_x = static_cast<T*>(args.grad_x) + row * args.grad_x_stride + at.channel;
+    T* to_gate = static_cast<T*>(args.grad_gate) + row * args.grad_gate_stride + at.channel;
     const Num<V> minus = Num<V>::all(-1.0f);
-    #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        if (edges.first && (edges.first >> i & 1u)) {
-            const int s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, s));
+    #pragma unroll 1
+    for (; p >= at.begin; p -= kBatch) {
+        const unsigned char *g = feed.next(), *x = g + S::bytes, *d = x + S::bytes;
+        Num<V> h = kept;
+        if (p > at.begin) kept = load_state<V>(at.inside ? args.states : nullptr, int64_t(p / kBatch - 1) * args.in.width + at.channel);
+        const int count = min(kBatch, at.end - p);
+        Num<V> a[kBatch], rest[kBatch], slope[kBatch];               // slope: (h_{t-1} - x) a (1 - a)
+        if (count == kBatch && span.begin < p && span.end > p + kBatch) {
+            #pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                a[i] = gate.a; rest[i] = gate.rest;
+                const Num<V> value = streams[1].get(x, p, i, at.lane);
+                slope[i] = madd(minus, value, h) * (gate.a * gate.rest);
+                h = madd(gate.a, h, gate.rest * value);
+            }
+            #pragma unroll
+            for (int i = kBatch - 1; i >= 0; --i, to_x -= step_x, to_gate -= step_gate) {
+                const Num<V> D = streams[2].get(d, p, i, at.lane) + E;
+                E = a[i] * D;
+                if (at.inside) {
+                    store_number<T, V>(to_x, rest[i] * D);
+                    store_number<T, V>(to_gate, slope[i] * D);
+                }
+            }
+        } else {
+            Span ahead;
+            ahead.find(args.in, p);
+            #pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (i >= count) break;
+                if (p + i == ahead.end) ahead.move(args.in, true);
+                if (p + i == ahead.begin) h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, ahead.sequence));
+                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                a[i] = gate.a; rest[i] = gate.rest;
+                const Num<V> value = streams[1].get(x, p, i, at.lane);
+                slope[i] = madd(minus, value, h) * (gate.a * gate.rest);
+                h = madd(gate.a, h, gate.rest * value);
+            }
+            #pragma unroll
+            for (int i = kBatch - 1; i >= 0; --i) {
+                if (i >= count) continue;
+                if (p + i < span.begin) span.move(args.in, false);
+                if (p + i + 1 == span.end) E = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, span.sequence));
+                const Num<V> D = streams[2].get(d, p, i, at.lane) + E;
+                E = a[i] * D;
+                if (at.inside) {
+                    store_number<T, V>(to_x, rest[i] * D);
+                    store_number<T, V>(to_gate, slope[i] * D);
+                    if (p + i == span.begin && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, span.sequence), E);
+                }
+                to_x -= step_x; to_gate -= step_gate;
+            }
         }
-        const Num<V> value = In::get(x + i * In::kRow);
-        slope[i] = madd(minus, value, h) * (a[i] * rest[i]);
-        h = madd(a[i], h, rest[i] * value);
     }
-    __syncthreads();
-    for (int w = kWarps - 1; w > at.warp; --w) E = follow<V>(&shared[w][at.lane * V], E);
-    if (plain) {
-        #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i) {
-            const Num<V> D = In::get(d + i * In::kRow) + E;
-            In::put(x + i * In::kRow, rest[i] * D);
-            In::put(g + i * In::kRow, slope[i] * D);
-            E = a[i] * D;
-        }
-    } else {
-        #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i) {
-            if (i >= at.count) continue;
-            const bool first = edges.first >> i & 1u, last = edges.last >> i & 1u;
-            int s = 0;
-            if (first || last) s = __shfl_sync(0xffffffffu, edges.sequence, i);
-            if (last) E = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, s));
-            const Num<V> D = In::get(d + i * In::kRow) + E;
-            In::put(x + i * In::kRow, rest[i] * D);
-            In::put(g + i * In::kRow, slope[i] * D);
-            E = a[i] * D;
-            if (first && at.inside && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, s), E);
-        }
-    }
-    if (at.warp == 0 && at.inside) pass_empty_sequences(args, args.grad_last, args.grad_initial, at.chunk, at.channel, V);
-    __syncthreads();
-    xs.store(args.grad_x, args.grad_x_stride, args, at);
-    gs.store(args.grad_gate, args.grad_gate_stride, args, at);
+    if (at.inside) pass_empty_sequences(args, args.grad_last, args.grad_initial, at.chunk, at.channel, V);
 }
 
 // One step for each row, the state updated in place.
@@ -549,28 +549,37 @@ void launch_carry(const ScanArgs& args, bool from_end, cudaStream_t stream) {
     cudaLaunchKernelEx(&config, scan_carry_kernel, static_cast<const float2*>(args.composed), args.carried, args.chunks, int(args.in.width), from_end, parts);
 }
 
-template <typename K> cudaError_t launch_chunks(K kernel, PerDeviceOnce& once, const ScanArgs& args, int tiles, int smem, cudaStream_t stream) {
+// Rows of a chunk: the most, up to 64, that give every SM 32 warps, but at least 16; a few rows are one chunk, whose state needs no walk.
+int chunk_rows(int64_t rows, int64_t tiles) {
+    if (rows <= kMostChunk) return kMostChunk;
+    int chunk = kMostChunk;
+    while (chunk > 16 && pieces(rows, chunk) * tiles < 148 * 32) chunk /= 2;
+    return chunk;
+}
+// Over both layouts of the channels: with two a lane there are fewer tiles, and so more chunks.
+int64_t most_chunks(int64_t rows, int64_t width) { return pieces(rows, chunk_rows(rows, (width + 63) / 64)); }
+
+template <typename K> cudaError_t launch_chunks(K kernel, PerDeviceOnce& once, const ScanArgs& args, int smem, cudaStream_t stream) {
     const cudaError_t err = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-    if (err != cudaSuccess) return err;
-    const dim3 grid(unsigned(tiles), unsigned(args.chunks < kGridRows ? args.chunks : kGridRows), unsigned((args.chunks + kGridRows - 1) / kGridRows));
-    kernel<<<grid, kScanBlock, smem, stream>>>(args);
-    return cudaSuccess;
+    if (err == cudaSuccess) kernel<<<unsigned(pieces(int64_t(args.chunks) * args.channel_tiles, kScanWarps)), kScanBlock, smem, stream>>>(args);
+    return err;
 }
 
 template <typename T, int V, int PIECE> cudaError_t scan_launch(ScanArgs& args, bool backward, cudaStream_t stream) {
     static PerDeviceOnce compose, apply, compose_backward, apply_backward;
-    constexpr int bytes = Tile<T, V, PIECE>::bytes;
-    const int tiles = (args.in.width + 32 * V - 1) / (32 * V);
-    args.chunks = int(pieces(args.in.rows, kChunk));
+    constexpr int two = kFeedBytes<T, V, PIECE, 2>, three = kFeedBytes<T, V, PIECE, 3>;
+    args.channel_tiles = (args.in.width + 32 * V - 1) / (32 * V);
+    args.chunk = chunk_rows(args.in.rows, args.channel_tiles);
+    args.chunks = int(pieces(args.in.rows, args.chunk));
     cudaError_t err = cudaSuccess;
     if (args.chunks > 1) {
-        err = backward ? launch_chunks(scan_compose_backward_kernel<T, V, PIECE>, compose_backward, args, tiles, 2 * bytes, stream)
-                       : launch_chunks(scan_compose_kernel<T, V, PIECE>, compose, args, tiles, 2 * bytes, stream);
+        err = backward ? launch_chunks(scan_compose_backward_kernel<T, V, PIECE>, compose_backward, args, two, stream)
+                       : launch_chunks(scan_compose_kernel<T, V, PIECE>, compose, args, two, stream);
         if (err == cudaSuccess) launch_carry(args, backward, stream);
     }
     if (err != cudaSuccess) return err;
-    return backward ? launch_chunks(scan_apply_backward_kernel<T, V, PIECE>, apply_backward, args, tiles, 3 * bytes, stream)
-                    : launch_chunks(scan_apply_kernel<T, V, PIECE>, apply, args, tiles, 2 * bytes, stream);
+    return backward ? launch_chunks(scan_apply_backward_kernel<T, V, PIECE>, apply_backward, args, three, stream)
+                    : launch_chunks(scan_apply_kernel<T, V, PIECE>, apply, args, two, stream);
 }
 
 // Two channels a lane where every row allows it, in pieces of 16 bytes where they do too.
@@ -595,7 +604,7 @@ int check_scan(const HtgsScan* scan, const char* message) {
     if (!scan || !known_type(scan->type) || scan->rows < 0 || scan->rows > 0x7fffff00 || !stride_ok(scan->x_stride) || !stride_ok(scan->gate_stride) || scan->width < 1 || scan->width > 65536 || scan->n_sequences < 1 ||
         (!scan->offsets && scan->rows % scan->n_sequences != 0) || (scan->rows > 0 && (!scan->x || !scan->gate)))
         return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
-    if (pieces(scan->rows, kChunk) * ((scan->width + 31) / 32) > 0x7fffffff) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
+    if (pieces(scan->rows, kMostChunk) * ((scan->width + 31) / 32) > 0x7fffffff) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
     return HTGS_OK;
 }
 
@@ -612,12 +621,12 @@ int pass_states(const float* from, float* to, const HtgsScan* scan, cudaStream_t
 extern "C" {
 
 size_t htgs_gated_scan_state_bytes(int64_t rows, int32_t width) {
-    return rows <= 0 || width <= 0 ? 0 : size_t(htgs::pieces(rows, htgs::kKept)) * size_t(width) * sizeof(float);
+    return rows <= 0 || width <= 0 ? 0 : size_t(htgs::pieces(rows, htgs::kBatch)) * size_t(width) * sizeof(float);
 }
 
 size_t htgs_gated_scan_workspace_bytes(int64_t rows, int32_t width) {
     if (rows <= 0 || width <= 0) return 0;
-    const size_t values = size_t(htgs::pieces(rows, htgs::kChunk)) * size_t(width);
+    const size_t values = size_t(htgs::most_chunks(rows, width)) * size_t(width);
     return htgs::align256(values * sizeof(float2)) + htgs::align256(values * sizeof(float));
 }
 
@@ -634,7 +643,7 @@ int htgs_gated_scan(const HtgsScan* scan, void* h, int64_t h_stride, float* last
     ScanArgs a{};
     a.in = *scan;
     a.composed = static_cast<float2*>(workspace);
-    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(pieces(scan->rows, kChunk)) * size_t(scan->width) * sizeof(float2)));
+    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(most_chunks(scan->rows, scan->width)) * size_t(scan->width) * sizeof(float2)));
     a.states = states;
     a.h = h; a.h_stride = h_stride; a.last = last;
     if (scan->type == HTGS_FLOAT32) return scan_typed<float>(a, false, s);
@@ -657,7 +666,7 @@ int htgs_gated_scan_backward(const HtgsScan* scan, const float* states, const vo
     ScanArgs a{};
     a.in = *scan;
     a.composed = static_cast<float2*>(workspace);
-    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(pieces(scan->rows, kChunk)) * size_t(scan->width) * sizeof(float2)));
+    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(most_chunks(scan->rows, scan->width)) * size_t(scan->width) * sizeof(float2)));
     a.states = const_cast<float*>(states);
     a.grad_h = grad_h; a.grad_h_stride = grad_h_stride; a.grad_last = grad_last;
     a.grad_x = grad_x; a.grad_x_stride = grad_x_stride; a.grad_gate = grad_gate; a.grad_gate_stride = grad_gate_stride; a.grad_initial = grad_initial;
