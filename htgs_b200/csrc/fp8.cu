@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(kQuantBlock, 6) dequantize_kernel(const uint8_
     const uint32_t across = uint32_t((width + 32 * VEC - 1) / (32 * VEC)), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
     const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;
     const int64_t column = int64_t(warp % across) * (32 * VEC) + lane * VEC;
+    grid_dependency();
     if (warp >= across * down || column >= width) return;
     for (int64_t row0 = warp / across; row0 < rows; row0 += int64_t(down) * R) {
         Pack<uint8_t, VEC> packed[R];
@@ -296,8 +297,8 @@ template <typename T> int quantize_typed(const QuantArgs& a, int rows_per_scale,
 }
 
 template <typename T, int VEC> void launch_dequantize(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
-    dequantize_kernel<T, VEC><<<blocks_for(m.rows, m.width, 32 * VEC), kQuantBlock, 0, stream>>>(
-        m.codes, m.codes_stride, m.scales, m.scales_stride, m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);
+    (void)launch_after(dequantize_kernel<T, VEC>, blocks_for(m.rows, m.width, 32 * VEC), kQuantBlock, 0, stream, m.codes, m.codes_stride, m.scales, m.scales_stride,
+                       m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);       // the caller asks for the last error
 }
 template <typename T> void dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
     if (m.width % 16 == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, 16) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16)) launch_dequantize<T, 16>(m, out, out_stride, stream);

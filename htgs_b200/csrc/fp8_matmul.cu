@@ -28,6 +28,7 @@ template <typename T, int ROWS>
 __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArgs args) {
     const int lane = threadIdx.x & 31;
     const int64_t n = int64_t(blockIdx.x) * (kRowsBlock / 32) + (threadIdx.x >> 5), m0 = int64_t(blockIdx.y) * ROWS;
+    grid_dependency();
     if (n >= args.b.rows) return;
     const uint8_t* b = args.b.codes + n * args.b.codes_stride;
     const uint8_t* sb = args.b.scales + n / args.b.rows_per_scale * args.b.scales_stride;
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) matmul_tiles_kernel(const __g
     }
     __syncthreads();
     if constexpr (PAIR) cluster_barrier();          // the other block's barriers can be reached from here on
+    grid_dependency();                               // the operands may come from the kernel before
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
     const uint32_t tmem_scales = tmem + kAccumulators * BN;
@@ -569,11 +571,13 @@ template <typename T, int BN, int MODE> int launch_tiles(const MatmulArgs& m, in
     cudaError_t err = once.run([] { return cudaFuncSetAttribute(matmul_tiles_kernel<T, BN, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem); });
     if (err != cudaSuccess) return sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
     cudaLaunchConfig_t config{};
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = unsigned(parts); attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = unsigned(parts); attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
     config.blockDim = kTileThreads; config.dynamicSmemBytes = S::smem; config.stream = stream;
-    config.attrs = &attribute; config.numAttrs = 1;
+    config.attrs = attributes; config.numAttrs = 2;
     config.gridDim = MODE == kSplit ? unsigned(args.tiles) * unsigned(parts) : unsigned(args.tiles < kSms / parts ? args.tiles : kSms / parts) * unsigned(parts);
     err = cudaLaunchKernelEx(&config, matmul_tiles_kernel<T, BN, MODE>, map_a, map_b, map_out, args, parts);
     return err == cudaSuccess ? sequence_status("htgs_fp8_matmul") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
@@ -583,8 +587,8 @@ template <typename T> int matmul_typed(const MatmulArgs& args, cudaStream_t stre
     if (args.a.rows <= 8) {
         constexpr int R = 8;
         const dim3 grid(unsigned((args.b.rows + kRowsBlock / 32 - 1) / (kRowsBlock / 32)), unsigned((args.a.rows + R - 1) / R));
-        matmul_rows_kernel<T, R><<<grid, kRowsBlock, 0, stream>>>(args);
-        return sequence_status("htgs_fp8_matmul");
+        const cudaError_t err = launch_after(matmul_rows_kernel<T, R>, grid, kRowsBlock, 0, stream, args);
+        return err == cudaSuccess ? sequence_status("htgs_fp8_matmul") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
     }
     const auto tiles_of = [&](int rows, int columns) { return (args.a.rows + rows - 1) / rows * ((args.b.rows + columns - 1) / columns); };
     const int64_t blocks_k = (args.a.width + kScaleBlock - 1) / kScaleBlock, tiles128 = tiles_of(128, 128), tiles224 = tiles_of(128, 224);

@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(MOST, MOST == kNarrowBlock ? kNarrowBlocks : 1
 template <typename T> __global__ void __launch_bounds__(1024) norm_weight_kernel(const float* partial, int blocks, int width, T* grad_weight) {
     __shared__ float shared[32][33];
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, column = blockIdx.x * 32 + lane;
+    grid_dependency();
     float sum[4] = {};
     if (column < width) {
         for (int b = slice; b < blocks; b += 128) {
@@ -318,7 +319,8 @@ template <typename T> void backward_typed(const NormBackwardArgs& a, void* grad_
                       rows_aligned(a.x, a.x_stride, a.rows, e, 16) && rows_aligned(a.residual, a.residual_stride, a.rows, e, 16) && aligned(a.weight, 16) &&
                       rows_aligned(a.grad_x, a.grad_x_stride, a.rows, e, 16);
     if (wide) backward_launch<T, V>(a, stream); else backward_launch<T, 1>(a, stream);
-    norm_weight_kernel<T><<<(a.width + 31) / 32, 1024, 0, stream>>>(a.partial, backward_blocks(a.rows, a.width), a.width, static_cast<T*>(grad_weight));
+    (void)launch_after(norm_weight_kernel<T>, (a.width + 31) / 32, 1024, 0, stream, static_cast<const float*>(a.partial), backward_blocks(a.rows, a.width), int(a.width),
+                       static_cast<T*>(grad_weight));      // the caller asks for the last error
 }
 
 }  // namespace

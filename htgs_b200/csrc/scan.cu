@@ -344,14 +344,17 @@ __global__ void __launch_bounds__(kCarryWarps * 32) scan_carry_kernel(const floa
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = lane % kCarryChannels, quarter = lane / kCarryChannels;
     const int channel = int(blockIdx.x) / parts * kCarryChannels + at, part = int(blockIdx.x) % parts;
     const bool inside = channel < width;
+    grid_dependency();
     const int runs = kCarryWarps * kQuarters * parts, run = (chunks + runs - 1) / runs;
     const int begin = int(min(int64_t((part * kCarryWarps + warp) * kQuarters + quarter) * run, int64_t(chunks))), count = inside ? min(run, chunks - begin) : 0;
     const int64_t first = int64_t(from_end ? chunks - 1 - begin : begin) * width + channel, step = from_end ? -int64_t(width) : width;
+    const float2* map = composed + first;
+    float* to = states + first;
     float2 maps[kCarryRun];
     float A = 1.0f, H = 0.0f;
     for (int c0 = 0; c0 < run; c0 += kCarryRun) {
         #pragma unroll
-        for (int c = 0; c < kCarryRun; ++c) maps[c] = c0 + c < count ? composed[first + (c0 + c) * step] : make_float2(1.0f, 0.0f);
+        for (int c = 0; c < kCarryRun; ++c, map += step) maps[c] = c0 + c < count ? *map : make_float2(1.0f, 0.0f);
         #pragma unroll
         for (int c = 0; c < kCarryRun; ++c) compose(A, H, maps[c]);
     }
@@ -379,14 +382,15 @@ __global__ void __launch_bounds__(kCarryWarps * 32) scan_carry_kernel(const floa
     }
     for (int w = 0; w < warp; ++w) state = follow(shared[w][at], state);
     state = follow(before, state);
+    map = composed + first;
     for (int c0 = 0; c0 < run; c0 += kCarryRun) {
         if (run > kCarryRun) {
             #pragma unroll
-            for (int c = 0; c < kCarryRun; ++c) maps[c] = c0 + c < count ? composed[first + (c0 + c) * step] : make_float2(1.0f, 0.0f);
+            for (int c = 0; c < kCarryRun; ++c, map += step) maps[c] = c0 + c < count ? *map : make_float2(1.0f, 0.0f);
         }
         #pragma unroll
-        for (int c = 0; c < kCarryRun; ++c) {
-            if (c0 + c < count) states[first + (c0 + c) * step] = state;
+        for (int c = 0; c < kCarryRun; ++c, to += step) {
+            if (c0 + c < count) *to = state;
             state = follow(maps[c], state);
         }
     }
@@ -409,6 +413,7 @@ __global__ void __launch_bounds__(kScanBlock, 8) scan_apply_kernel(const ScanArg
     if (at.nothing()) return;
     const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at)};
     Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, false);
+    grid_dependency();                        // x and gate are older than the first pass, which ended before the second began
     Num<V> h = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
     Span span;
     span.find(args.in, at.begin);
@@ -444,13 +449,14 @@ __global__ void __launch_bounds__(kScanBlock, 8) scan_apply_kernel(const ScanArg
 
 // Third pass, backward: eight rows forward from the state that was kept, then back.
 template <typename T, int V, int PIECE>
-__global__ void __launch_bounds__(kScanBlock, 6) scan_apply_backward_kernel(const ScanArgs args) {
+__global__ void __launch_bounds__(kScanBlock, 5) scan_apply_backward_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
     using S = Stream<T, V, PIECE>;
     const Place<V> at(args, true);
     if (at.nothing()) return;
     const S streams[3] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at), S(args.grad_h, args.grad_h_stride, args, at)};
     Feed<S, 3> feed(streams, memory + at.warp * kStages * 3 * S::bytes, at.lane, at.begin, at.end, true);
+    grid_dependency();
     int p = at.last_batch();
     Num<V> kept = load_state<V>(at.inside ? args.states : nullptr, int64_t(p / kBatch) * args.in.width + at.channel);
     Num<V> E = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
@@ -537,16 +543,18 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const T* __restrict__ x,
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 int64_t pieces(int64_t rows, int piece) { return (rows + piece - 1) / piece; }
 
-void launch_carry(const ScanArgs& args, bool from_end, cudaStream_t stream) {
+cudaError_t launch_carry(const ScanArgs& args, bool from_end, cudaStream_t stream) {
     int parts = 1;                             // eight chunks in a run, and at most eight blocks
     while (parts < 8 && args.chunks > kCarryWarps * (32 / kCarryChannels) * 8 * parts) parts *= 2;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = unsigned(parts); attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = unsigned(parts); attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = unsigned((args.in.width + kCarryChannels - 1) / kCarryChannels * parts); config.blockDim = kCarryWarps * 32; config.stream = stream;
-    config.attrs = &attribute; config.numAttrs = 1;
-    cudaLaunchKernelEx(&config, scan_carry_kernel, static_cast<const float2*>(args.composed), args.carried, args.chunks, int(args.in.width), from_end, parts);
+    config.attrs = attributes; config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, scan_carry_kernel, static_cast<const float2*>(args.composed), args.carried, args.chunks, int(args.in.width), from_end, parts);
 }
 
 // Rows of a chunk: the most, up to 64, that give every SM 32 warps, but at least 16; a few rows are one chunk, whose state needs no walk.
@@ -559,10 +567,14 @@ int chunk_rows(int64_t rows, int64_t tiles) {
 // Over both layouts of the channels: with two a lane there are fewer tiles, and so more chunks.
 int64_t most_chunks(int64_t rows, int64_t width) { return pieces(rows, chunk_rows(rows, (width + 63) / 64)); }
 
-template <typename K> cudaError_t launch_chunks(K kernel, PerDeviceOnce& once, const ScanArgs& args, int smem, cudaStream_t stream) {
+// `behind`: close behind the kernel before, for which the kernel waits itself.
+template <typename K> cudaError_t launch_chunks(K kernel, PerDeviceOnce& once, const ScanArgs& args, int smem, bool behind, cudaStream_t stream) {
     const cudaError_t err = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-    if (err == cudaSuccess) kernel<<<unsigned(pieces(int64_t(args.chunks) * args.channel_tiles, kScanWarps)), kScanBlock, smem, stream>>>(args);
-    return err;
+    if (err != cudaSuccess) return err;
+    const unsigned int blocks = unsigned(pieces(int64_t(args.chunks) * args.channel_tiles, kScanWarps));
+    if (behind) return launch_after(kernel, blocks, kScanBlock, smem, stream, args);
+    kernel<<<blocks, kScanBlock, smem, stream>>>(args);
+    return cudaSuccess;
 }
 
 template <typename T, int V, int PIECE> cudaError_t scan_launch(ScanArgs& args, bool backward, cudaStream_t stream) {
@@ -573,13 +585,13 @@ template <typename T, int V, int PIECE> cudaError_t scan_launch(ScanArgs& args, 
     args.chunks = int(pieces(args.in.rows, args.chunk));
     cudaError_t err = cudaSuccess;
     if (args.chunks > 1) {
-        err = backward ? launch_chunks(scan_compose_backward_kernel<T, V, PIECE>, compose_backward, args, two, stream)
-                       : launch_chunks(scan_compose_kernel<T, V, PIECE>, compose, args, two, stream);
-        if (err == cudaSuccess) launch_carry(args, backward, stream);
+        err = backward ? launch_chunks(scan_compose_backward_kernel<T, V, PIECE>, compose_backward, args, two, false, stream)
+                       : launch_chunks(scan_compose_kernel<T, V, PIECE>, compose, args, two, false, stream);
+        if (err == cudaSuccess) err = launch_carry(args, backward, stream);
     }
     if (err != cudaSuccess) return err;
-    return backward ? launch_chunks(scan_apply_backward_kernel<T, V, PIECE>, apply_backward, args, three, stream)
-                    : launch_chunks(scan_apply_kernel<T, V, PIECE>, apply, args, two, stream);
+    return backward ? launch_chunks(scan_apply_backward_kernel<T, V, PIECE>, apply_backward, args, three, args.chunks > 1, stream)
+                    : launch_chunks(scan_apply_kernel<T, V, PIECE>, apply, args, two, args.chunks > 1, stream);
 }
 
 // Two channels a lane where every row allows it, in pieces of 16 bytes where they do too.
