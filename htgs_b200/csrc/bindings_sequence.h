@@ -223,9 +223,15 @@ Tensor fp8_matmul(const Tensor& x, const OptTensor& x_scales, int64_t x_rows_per
     TORCH_CHECK(!(c10::GradMode::is_enabled() && x.requires_grad()), "fp8_matmul has no gradient: use fp8_linear in training, or torch.no_grad()");
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor xm = rows_of(x);
-    Matrix q = empty_matrix(xm.size(0), width, 1, x);
-    quantize_into(xm, 1, &q, nullptr);
     Tensor out = torch::empty(with_last(x, codes.size(0)), x.options().dtype(dtype.value_or(x.scalar_type())).requires_grad(false));
+    const int64_t rows = xm.size(0);
+    if (rows >= 1 && rows <= 8 && width >= 1 && rows * up(width, kBlock) <= 32768) {       // one kernel codes and multiplies
+        const HtgsFp8Matrix b = view_of(w);
+        check(htgs_fp8_matmul_values(xm.data_ptr(), xm.stride(0), type_of(x.scalar_type()), rows, &b, out.data_ptr(), codes.size(0), type_of(out.scalar_type()), stream_of(x)));
+        return out;
+    }
+    Matrix q = empty_matrix(rows, width, 1, x);
+    quantize_into(xm, 1, &q, nullptr);
     multiply_into(q, w, out);
     return out;
 }

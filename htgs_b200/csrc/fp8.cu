@@ -245,19 +245,15 @@ __global__ void __launch_bounds__(kQuantBlock, 6) dequantize_kernel(const uint8_
             if (row >= rows) break;
             const float scale = scale_value(exponent[r]);
             T* to = out + row * out_stride + column;
-            if constexpr (VEC == 16) {
-                constexpr int V = 16 / int(sizeof(T));
+            if constexpr (VEC > 1) {
                 const uint32_t* words = reinterpret_cast<const uint32_t*>(&packed[r]);
+                float v[VEC];
                 #pragma unroll
-                for (int i = 0; i < 16; i += V) {
-                    float v[V];
-                    #pragma unroll
-                    for (int k = 0; k < V; k += 2) {
-                        const float2 f = decode2(words[(i + k) / 4] >> ((i + k) % 4 * 8));
-                        v[k] = f.x * scale; v[k + 1] = f.y * scale;
-                    }
-                    store_floats<T, V>(to + i, v);
+                for (int k = 0; k < VEC; k += 2) {
+                    const float2 f = decode2(words[k / 4] >> (k % 4 * 8));
+                    v[k] = f.x * scale; v[k + 1] = f.y * scale;
                 }
+                store_floats<T, VEC>(to, v);
             } else {
                 *to = from_float<T>(decode2(packed[r].v[0]).x * scale);
             }
@@ -301,7 +297,8 @@ template <typename T, int VEC> void launch_dequantize(const HtgsFp8Matrix& m, vo
                        m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);       // the caller asks for the last error
 }
 template <typename T> void dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
-    if (m.width % 16 == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, 16) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16)) launch_dequantize<T, 16>(m, out, out_stride, stream);
+    constexpr int V = 16 / int(sizeof(T));        // 16 bytes to store: with 32 a lane every store would write half sectors
+    if (m.width % V == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, V) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16)) launch_dequantize<T, V>(m, out, out_stride, stream);
     else launch_dequantize<T, 1>(m, out, out_stride, stream);
 }
 

@@ -23,26 +23,52 @@ struct MatmulArgs {
     int64_t out_stride;
 };
 
-// Few rows of a: a warp per row of b, 16 codes of it in a lane at a time, against ROWS rows of a.
-template <typename T, int ROWS>
-__global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArgs args) {
-    const int lane = threadIdx.x & 31;
-    const int64_t n = int64_t(blockIdx.x) * (kRowsBlock / 32) + (threadIdx.x >> 5), m0 = int64_t(blockIdx.y) * ROWS;
+// Sixteen codes from column k on of a row of `width`, without what lies behind its end.
+__device__ __forceinline__ void load_codes(const uint8_t* row, int64_t k, int64_t width, uint32_t (&words)[4]) {
+    const uint4 packed = *reinterpret_cast<const uint4*>(row + k);
+    words[0] = packed.x; words[1] = packed.y; words[2] = packed.z; words[3] = packed.w;
+    if (k + 16 <= width) return;
+    #pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int64_t rest = width - k - 4 * w;
+        words[w] = rest >= 4 ? words[w] : rest <= 0 ? 0u : words[w] & ((1u << (8 * int(rest))) - 1u);
+    }
+}
+
+// Few rows of a: a warp per row of b, 16 codes of it in a lane at a time, against ROWS rows of a.  Bound by reading b, and for small b by the launch.
+// With VALUES a comes as values of type X and each block codes them itself into shared memory, as quantize_rows_kernel would (fp8.cu): a launch less.
+struct ValuesArgs { const void* x; int64_t stride; };
+constexpr int kMostRows = 8, kMostValues = 32768;       // of a
+template <typename T, int ROWS, typename X, bool VALUES>
+__global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArgs args, const ValuesArgs values) {
+    extern __shared__ __align__(16) uint8_t coded[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t n = int64_t(blockIdx.x) * (kRowsBlock / 32) + warp, m0 = int64_t(blockIdx.y) * ROWS, width = args.a.width;
+    const int across = int((width + kScaleBlock - 1) / kScaleBlock);
+    const int pitch = across * kScaleBlock;
+    float* factors = reinterpret_cast<float*>(coded + args.a.rows * pitch);       // with VALUES all rows of a are the block's
     grid_dependency();
+    if (VALUES) {
+        for (int unit = warp; unit < int(args.a.rows) * across; unit += kRowsBlock / 32) {
+            const int row = unit / across, block = unit - row * across;
+            const X* x = static_cast<const X*>(values.x) + row * values.stride + block * kScaleBlock;
+            float v[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = block * kScaleBlock + lane + 32 * i < width ? to_float<X>(x[lane + 32 * i]) : 0.0f;
+            const int e = scale_exponent(lanes_max<32>(largest_finite(v)));
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) coded[row * pitch + block * kScaleBlock + lane + 32 * i] = uint8_t(encode2<true>(v[i], 0.0f, inverse_scale(e)) & 0xffu);
+            if (lane == 0) factors[row * across + block] = scale_value(uint32_t(e + 127));
+        }
+        __syncthreads();
+    }
     if (n >= args.b.rows) return;
     const uint8_t* b = args.b.codes + n * args.b.codes_stride;
     const uint8_t* sb = args.b.scales + n / args.b.rows_per_scale * args.b.scales_stride;
     float acc[ROWS] = {};
-    for (int64_t k = lane * 16; k < args.a.width; k += 512) {
-        const uint4 packed = *reinterpret_cast<const uint4*>(b + k);
-        uint32_t words[4] = {packed.x, packed.y, packed.z, packed.w};
-        if (k + 16 > args.a.width) {           // codes behind the row's end are no part of it
-            #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int64_t rest = args.a.width - k - 4 * w;
-                words[w] = rest >= 4 ? words[w] : rest <= 0 ? 0u : words[w] & ((1u << (8 * int(rest))) - 1u);
-            }
-        }
+    for (int64_t k = lane * 16; k < width; k += 512) {
+        uint32_t words[4];
+        load_codes(b, k, width, words);
         float2 vb[8];
         #pragma unroll
         for (int w = 0; w < 4; ++w) { vb[2 * w] = decode2(words[w]); vb[2 * w + 1] = decode2(words[w] >> 16); }
@@ -51,14 +77,15 @@ __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArg
         for (int r = 0; r < ROWS; ++r) {
             const int64_t m = m0 + r;
             if (m >= args.a.rows) break;
-            const uint4 pa = *reinterpret_cast<const uint4*>(args.a.codes + m * args.a.codes_stride + k);
-            uint32_t wa[4] = {pa.x, pa.y, pa.z, pa.w};
-            if (k + 16 > args.a.width) {
-                #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int64_t rest = args.a.width - k - 4 * w;
-                    wa[w] = rest >= 4 ? wa[w] : rest <= 0 ? 0u : wa[w] & ((1u << (8 * int(rest))) - 1u);
-                }
+            uint32_t wa[4];
+            float scale_a;
+            if (VALUES) {
+                const uint4 packed = *reinterpret_cast<const uint4*>(coded + r * pitch + k);
+                wa[0] = packed.x; wa[1] = packed.y; wa[2] = packed.z; wa[3] = packed.w;
+                scale_a = factors[r * across + k / kScaleBlock];
+            } else {
+                load_codes(args.a.codes + m * args.a.codes_stride, k, width, wa);
+                scale_a = scale_value(args.a.scales[m / args.a.rows_per_scale * args.a.scales_stride + k / kScaleBlock]);
             }
             float sum = 0.0f;
             #pragma unroll
@@ -69,14 +96,31 @@ __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArg
                 sum = fmaf(hi.x, vb[2 * w + 1].x, sum);
                 sum = fmaf(hi.y, vb[2 * w + 1].y, sum);
             }
-            acc[r] = fmaf(sum * scale_value(args.a.scales[m / args.a.rows_per_scale * args.a.scales_stride + k / kScaleBlock]), scale_b, acc[r]);
+            acc[r] = fmaf(sum * scale_a, scale_b, acc[r]);
         }
     }
     #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
+        if (m0 + r >= args.a.rows) break;
         const float total = warp_sum(acc[r]);
-        if (lane == 0 && m0 + r < args.a.rows) static_cast<T*>(args.out)[(m0 + r) * args.out_stride + n] = from_float<T>(total);
+        if (lane == 0) static_cast<T*>(args.out)[(m0 + r) * args.out_stride + n] = from_float<T>(total);
     }
+}
+
+template <typename T, int ROWS, typename X, bool VALUES> int launch_rows(const MatmulArgs& args, const ValuesArgs& values, cudaStream_t stream) {
+    const int across = int((args.a.width + kScaleBlock - 1) / kScaleBlock);
+    const size_t smem = VALUES ? size_t(args.a.rows) * across * (kScaleBlock + sizeof(float)) : 0;
+    const dim3 grid(unsigned((args.b.rows + kRowsBlock / 32 - 1) / (kRowsBlock / 32)), unsigned((args.a.rows + ROWS - 1) / ROWS));
+    const cudaError_t err = launch_after(matmul_rows_kernel<T, ROWS, X, VALUES>, grid, kRowsBlock, smem, stream, args, values);
+    return err == cudaSuccess ? sequence_status("htgs_fp8_matmul") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
+template <typename T, typename X> int matmul_values(const MatmulArgs& args, const ValuesArgs& values, cudaStream_t stream) {
+    return args.a.rows == 1 ? launch_rows<T, 1, X, true>(args, values, stream) : launch_rows<T, kMostRows, X, true>(args, values, stream);
+}
+template <typename T> int matmul_values(const MatmulArgs& args, const ValuesArgs& values, int type, cudaStream_t stream) {
+    if (type == HTGS_FLOAT32) return matmul_values<T, float>(args, values, stream);
+    if (type == HTGS_FLOAT16) return matmul_values<T, __half>(args, values, stream);
+    return matmul_values<T, __nv_bfloat16>(args, values, stream);
 }
 
 // ---- tensor cores ------------------------------------------------------------------------------------------------------------
@@ -584,17 +628,15 @@ template <typename T, int BN, int MODE> int launch_tiles(const MatmulArgs& m, in
 }
 
 template <typename T> int matmul_typed(const MatmulArgs& args, cudaStream_t stream) {
-    if (args.a.rows <= 8) {
-        constexpr int R = 8;
-        const dim3 grid(unsigned((args.b.rows + kRowsBlock / 32 - 1) / (kRowsBlock / 32)), unsigned((args.a.rows + R - 1) / R));
-        const cudaError_t err = launch_after(matmul_rows_kernel<T, R>, grid, kRowsBlock, 0, stream, args);
-        return err == cudaSuccess ? sequence_status("htgs_fp8_matmul") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
-    }
+    if (args.a.rows == 1) return launch_rows<T, 1, T, false>(args, {}, stream);
+    if (args.a.rows <= kMostRows) return launch_rows<T, kMostRows, T, false>(args, {}, stream);
     const auto tiles_of = [&](int rows, int columns) { return (args.a.rows + rows - 1) / rows * ((args.b.rows + columns - 1) / columns); };
     const int64_t blocks_k = (args.a.width + kScaleBlock - 1) / kScaleBlock, tiles128 = tiles_of(128, 128), tiles224 = tiles_of(128, 224);
-    // Few tiles: split the sum until the SMs are used, each part at least one block of 128 columns.
+    // Few tiles and a long sum: split it.  Joining the parts costs 2 to 3 us, ten blocks of 128 columns' worth, so a part has eight blocks at least (us, unsplit /
+    // in 4 / in 8: 128 x 2048 by 2048 7.1 / 7.4 / 14.3, 100 x 4096 by 256 10.7 / 7.7 / 7.5, 1024 x 32768 by 512 65 / 25 / 25).  Sixteen clusters of eight are not on
+    // the SMs at once.
     int parts = 1;
-    while (parts < kMostParts && tiles128 * parts * 2 <= kSms && blocks_k >= 2 * parts) parts *= 2;
+    while (parts < kMostParts && blocks_k >= 32 && blocks_k >= 16 * parts && tiles128 * parts * 2 <= (parts < 4 ? kSms : 64)) parts *= 2;
     if (parts > 1) return launch_tiles<T, 128, kSplit>(args, parts, stream);
     // Many tiles: pairs, from sixteen rounds of all SMs on, so that the last, incomplete one weighs little.  us, pairs of 224 / single blocks of 224 / of 128:
     // 8192 x 8192 by 8192 442 / 478 / 554, 100000 x 1024 by 2048 207 / 213 / 226; with fewer rounds 32768 x 512 by 1024 29 / 24 / 25, 4099 x 1080 by 1008 15 / 13 / 11.
@@ -616,6 +658,23 @@ bool matrix_ok(const HtgsFp8Matrix* m) {
 }  // namespace htgs
 
 extern "C" {
+
+int htgs_fp8_matmul_values(const void* x, int64_t x_stride, int type, int64_t rows, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream) {
+    using namespace htgs;
+    if (!matrix_ok(b) || !known_type(type) || !known_type(out_type)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_values: bad matrix or unknown element type");
+    if (rows < 0 || rows > kMostRows || rows * ((b->width + kScaleBlock - 1) / kScaleBlock * kScaleBlock) > kMostValues)
+        return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_values: at most 8 rows and 32768 values (the width rounded up to 128)");
+    if (rows == 0 || b->rows == 0) return HTGS_OK;
+    if (b->width < 1 || !x || !out || out_stride < b->rows)
+        return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_values: x and out must not be null, the width at least 1, and out's rows must hold b.rows values");
+    const HtgsFp8Matrix a{nullptr, nullptr, rows, b->width, 0, 0, 1};
+    const MatmulArgs args{a, *b, out, out_stride};
+    const ValuesArgs values{x, x_stride};
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (out_type == HTGS_FLOAT32) return matmul_values<float>(args, values, type, s);
+    if (out_type == HTGS_FLOAT16) return matmul_values<__half>(args, values, type, s);
+    return matmul_values<__nv_bfloat16>(args, values, type, s);
+}
 
 int htgs_fp8_matmul(const HtgsFp8Matrix* a, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream) {
     using namespace htgs;

@@ -261,6 +261,11 @@ def quantize_fp8(x: torch.Tensor, rows_per_scale: int = 1, transpose: bool = Fal
     return t if transpose else q
 
 
+def _few(x: torch.Tensor) -> bool:
+    """Whether one kernel codes and multiplies the rows of x."""
+    return 1 <= x.shape[0] <= 8 and x.shape[1] >= 1 and x.shape[0] * -(-x.shape[1] // _BLOCK) * _BLOCK <= 32768
+
+
 def _matmul(a: Fp8Matrix, b: Fp8Matrix, dtype: torch.dtype) -> torch.Tensor:
     out = torch.empty((a.codes.shape[0], b.codes.shape[0]), dtype=dtype, device=a.codes.device)
     _call(out.device, "htgs_fp8_matmul", ctypes.byref(a._struct()), ctypes.byref(b._struct()), out.data_ptr(), out.shape[1], _TYPES[dtype])
@@ -291,8 +296,14 @@ def fp8_matmul(x, weight: Fp8Matrix, dtype: Optional[torch.dtype] = None) -> tor
         raise ValueError(f"x must have a last dimension of {weight.shape[1]} values")
     if _wants_grad(x):
         raise RuntimeError("fp8_matmul has no gradient: use fp8_linear in training, or torch.no_grad()")
-    q, _ = _quantize(_rows(x), 1, True, False)
-    return _matmul(q, weight, dtype or x.dtype).view(*x.shape[:-1], weight.shape[0])
+    xm, dtype = _rows(x), dtype or x.dtype
+    if _few(xm):
+        out = torch.empty((*x.shape[:-1], weight.shape[0]), dtype=dtype, device=x.device)
+        _call(x.device, "htgs_fp8_matmul_values", xm.data_ptr(), xm.stride(0), _TYPES[x.dtype], xm.shape[0], ctypes.byref(weight._struct()), out.data_ptr(),
+              weight.shape[0], _TYPES[dtype])
+        return out
+    q, _ = _quantize(xm, 1, True, False)
+    return _matmul(q, weight, dtype).view(*x.shape[:-1], weight.shape[0])
 
 
 class _Fp8Linear(torch.autograd.Function):

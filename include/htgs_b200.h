@@ -486,6 +486,9 @@ int htgs_dequantize_fp8(const HtgsFp8Matrix* matrix, void* out, int64_t out_stri
  * and have a stride that is a multiple of 16; scales begin on 4 bytes with a stride that is a multiple of 4.
  */
 int htgs_fp8_matmul(const HtgsFp8Matrix* a, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream);
+/* The same for a few rows of values, coded within the kernel as htgs_quantize_fp8 does with one row per scale: at most 8 rows, and 32768 values with the
+ * width rounded up to 128. */
+int htgs_fp8_matmul_values(const void* x, int64_t x_stride, int type, int64_t rows, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream);
 
 /*
  * Gated linear recurrence along the rows, per channel:

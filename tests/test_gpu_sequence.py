@@ -204,7 +204,8 @@ def product_bound(a, b, kind):
 
 
 SIZES = [(1, 1, 1), (1, 8, 16), (1, 1000, 1024), (3, 129, 127), (8, 256, 512), (9, 64, 130), (31, 72, 1100), (64, 136, 384), (100, 300, 640), (128, 128, 128), (129, 257, 129),
-         (200, 520, 2056), (300, 1001, 392), (513, 96, 1536)]
+         (200, 520, 2056), (300, 1001, 392), (513, 96, 1536),
+         (2, 130, 8200), (5, 33, 16500), (40, 300, 8200), (130, 140, 4100), (64, 64, 33000)]
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])

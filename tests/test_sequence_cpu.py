@@ -52,6 +52,12 @@ def test_c_entries_check_their_arguments():
     _refused(BAD, product(matrix(), matrix(), out=None))
     _refused(BAD, product(matrix(), matrix(), stride=3))
     assert product(matrix(rows=0), matrix()) == 0
+    values = lambda b, x=64, t=0, rows=4, out=64, stride=4, o=0: lib.htgs_fp8_matmul_values(x, 200, t, rows, ctypes.byref(b), out, stride, o, None)  # noqa: E731
+    for k in ({"x": None}, {"t": 3}, {"rows": 9}, {"rows": -1}, {"out": None}, {"stride": 3}, {"o": -1}):
+        _refused(BAD, values(matrix(), **k))
+    _refused(BAD, values(matrix(codes=1025)))
+    _refused(BAD, values(matrix(width=9000, cs=9008, ss=72)))
+    assert values(matrix(), rows=0) == 0
     _refused(BAD, lib.htgs_dequantize_fp8(ctypes.byref(matrix(rps=3)), 64, 200, 0, None))
     _refused(BAD, lib.htgs_dequantize_fp8(None, 64, 200, 0, None))
 
