@@ -13,6 +13,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>

@@ -1,0 +1,35 @@
+"""CPU: the order of the Gaussians along the curve, and the refiner's refusals."""
+import pytest
+import torch
+
+from htgs_b200 import refiner
+
+
+def test_curve_order_is_a_permutation_that_keeps_neighbours_together():
+    g = torch.Generator().manual_seed(1)
+    grid = torch.stack(torch.meshgrid(*[torch.arange(8.0)] * 3, indexing="ij"), dim=-1).reshape(-1, 3)
+    shuffled = grid[torch.randperm(512, generator=g)]
+    order = refiner.curve_order(shuffled)
+    assert torch.equal(torch.sort(order).values, torch.arange(512))
+    path = shuffled[order]
+    # the curve goes through each octant before the next: 8 runs of 64
+    octant = (path >= 4).long() @ torch.tensor([1, 2, 4])
+    assert torch.equal(octant, torch.arange(8).repeat_interleave(64))
+
+
+def test_curve_order_of_packed_scenes_stays_in_each():
+    g = torch.Generator().manual_seed(2)
+    positions = torch.rand((100, 3), generator=g)
+    offsets = torch.tensor([0, 30, 30, 100], dtype=torch.int32)
+    order = refiner.curve_order(positions, offsets)
+    assert torch.equal(torch.sort(order[:30]).values, torch.arange(30)) and torch.equal(torch.sort(order[30:]).values, torch.arange(30, 100))
+
+
+def test_order_of_equal_and_of_no_positions():
+    assert torch.equal(refiner.curve_order(torch.ones(5, 3)), torch.arange(5))
+    assert refiner.curve_order(torch.empty(0, 3)).shape == (0,)
+
+
+def test_infer_needs_coded_weights():
+    with pytest.raises(RuntimeError):
+        refiner.GaussianRefiner(32, 1).infer({})
