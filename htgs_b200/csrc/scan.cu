@@ -6,7 +6,7 @@
 //
 // A step is the map h -> A h + H, and steps compose: (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2).  The rows are cut into chunks of 16 to 64.  One
 // kernel composes each chunk's rows, one walks from chunk to chunk and leaves the state in front of each, one goes through the
-// chunks again from those states and writes h.  The backward pass does the same from the end.  A warp takes a chunk of 32 or 64 channels and goes
+// chunks again from those states and writes h.  The backward pass does the same from the end.  A warp takes a chunk of 64 channels and goes
 // through it eight rows at a time, the next sixteen on their way into shared memory of its own; warps never wait for one another.  For the backward pass the
 // forward one keeps the state in front of every eight rows: h_{t-1} is computed again from there, so it is in 32 bits and neither h nor the rows
 // before are read.  A sequence's first row has A = 0 and takes its initial state into H, so packed sequences need no chunks of their own; that zero is
@@ -19,6 +19,7 @@ namespace htgs {
 
 namespace {
 
+constexpr int kChannels = 64;                // of a warp, two a lane
 constexpr int kBatch = 8;                    // rows that a warp deals with at a time; a state in front of each batch is kept for the backward pass
 constexpr int kMostChunk = 64;               // rows
 constexpr int kStages = 3;                   // batches of a warp in shared memory
@@ -36,26 +37,16 @@ struct ScanArgs {
     void* grad_x; int64_t grad_x_stride; void* grad_gate; int64_t grad_gate_stride; float* grad_initial;
 };
 
-// V channels side by side: one float, or two in a register pair (one instruction for both).
-template <int V> struct Num;
-template <> struct Num<1> {
-    float v;
-    __device__ __forceinline__ static Num make(const float (&f)[1]) { return {f[0]}; }
-    __device__ __forceinline__ static Num all(float f) { return {f}; }
-    __device__ __forceinline__ float operator[](int) const { return v; }
-};
-template <> struct Num<2> {
+// Two channels side by side, in a register pair: one instruction for both.
+struct Num {
     f32x2 v;
-    __device__ __forceinline__ static Num make(const float (&f)[2]) { return {pack2(f[0], f[1])}; }
+    __device__ __forceinline__ static Num make(float x, float y) { return {pack2(x, y)}; }
     __device__ __forceinline__ static Num all(float f) { return {pack2(f, f)}; }
-    __device__ __forceinline__ float operator[](int i) const { const float2 f = unpack2(v); return i ? f.y : f.x; }
+    __device__ __forceinline__ float2 get() const { return unpack2(v); }
 };
-__device__ __forceinline__ Num<1> operator*(Num<1> a, Num<1> b) { return {a.v * b.v}; }
-__device__ __forceinline__ Num<1> operator+(Num<1> a, Num<1> b) { return {a.v + b.v}; }
-__device__ __forceinline__ Num<1> madd(Num<1> a, Num<1> b, Num<1> c) { return {fmaf(a.v, b.v, c.v)}; }
-__device__ __forceinline__ Num<2> operator*(Num<2> a, Num<2> b) { return {mul2(a.v, b.v)}; }
-__device__ __forceinline__ Num<2> operator+(Num<2> a, Num<2> b) { return {add2(a.v, b.v)}; }
-__device__ __forceinline__ Num<2> madd(Num<2> a, Num<2> b, Num<2> c) { return {fma2(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Num operator*(Num a, Num b) { return {mul2(a.v, b.v)}; }
+__device__ __forceinline__ Num operator+(Num a, Num b) { return {add2(a.v, b.v)}; }
+__device__ __forceinline__ Num madd(Num a, Num b, Num c) { return {fma2(a.v, b.v, c.v)}; }
 
 // exp(-g), from the hardware's 2^x (2 units); above exp(80), where a < 2e-35 tells nothing from zero, it stays; a NaN stays one.
 __device__ __forceinline__ float exp_negated(float scaled) {        // scaled = -g / ln 2
@@ -65,28 +56,16 @@ __device__ __forceinline__ float exp_negated(float scaled) {        // scaled = 
     return t;
 }
 __device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-template <int V> __device__ __forceinline__ Num<V> gate_exp(Num<V> g) {
-    const Num<V> scaled = g * Num<V>::all(-1.4426950408889634f);
-    float t[V];
-    #pragma unroll
-    for (int k = 0; k < V; ++k) t[k] = exp_negated(scaled[k]);
-    return Num<V>::make(t);
+__device__ __forceinline__ Num gate_exp(Num g) {
+    const float2 scaled = (g * Num::all(-1.4426950408889634f)).get();
+    return Num::make(exp_negated(scaled.x), exp_negated(scaled.y));
 }
-template <int V> struct Gate { Num<V> a, rest; };                    // a and 1 - a
-template <int V> __device__ __forceinline__ Gate<V> gate_of(Num<V> t) {
-    const Num<V> sum = t + Num<V>::all(1.0f);
-    float a[V];
-    #pragma unroll
-    for (int k = 0; k < V; ++k) a[k] = rcp_approx(sum[k]);
-    const Num<V> A = Num<V>::make(a);
-    return {A, t * A};
-}
-template <typename T, int V> __device__ __forceinline__ Num<V> number(const Pack<T, V>& p) { float f[V]; to_floats<T, V>(p, f); return Num<V>::make(f); }
-template <typename T, int V> __device__ __forceinline__ void store_number(T* p, Num<V> n) {
-    float f[V];
-    #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = n[k];
-    store_floats<T, V>(p, f);
+struct Gate { Num a, rest; };                    // a and 1 - a
+__device__ __forceinline__ Gate gate_of(Num g) {
+    const Num t = gate_exp(g);
+    const float2 sum = (t + Num::all(1.0f)).get();
+    const Num a = Num::make(rcp_approx(sum.x), rcp_approx(sum.y));
+    return {a, t * a};
 }
 
 // The map of a sequence's first step takes nothing from the state in front of it: A is -0, which no product of gates is.
@@ -97,17 +76,6 @@ __device__ __forceinline__ void compose(float& A, float& H, float2 next) {
     H = follow(next, H);
     A = is_cut(next.x) ? next.x : A * next.x;
 }
-template <int V> __device__ __forceinline__ Num<V> follow(const float2* maps, Num<V> state) {
-    float f[V];
-    #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = follow(maps[k], state[k]);
-    return Num<V>::make(f);
-}
-template <int V> __device__ __forceinline__ void leave_map(float2* to, Num<V> A, Num<V> H) {
-    #pragma unroll
-    for (int k = 0; k < V; ++k) to[k] = make_float2(A[k], H[k]);
-}
-
 // Positions p count the rows in the order of the recurrence: row p, or rows - 1 - p in reverse.
 // The sequence that holds a position, by its first position and the one behind its last.
 struct Span {
@@ -142,80 +110,99 @@ struct Span {
     }
 };
 
-template <int V> __device__ __forceinline__ Num<V> load_state(const float* states, int64_t at) {
-    float f[V];
-    #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = states ? states[at + k] : 0.0f;
-    return Num<V>::make(f);
-}
-template <int V> __device__ __forceinline__ void store_state(float* states, int64_t at, Num<V> n) {
-    #pragma unroll
-    for (int k = 0; k < V; ++k) states[at + k] = n[k];
-}
-
-// Where a thread works: V channels side by side, positions begin to end - 1.
-template <int V> struct Place {
-    int lane, warp, channel0, channel, chunk, begin, end;
-    bool inside;
+// Where a thread works: two channels side by side, of which `live` exist, positions begin to end - 1.
+struct Place {
+    int lane, warp, channel0, channel, live, chunk, begin, end;
     __device__ __forceinline__ explicit Place(const ScanArgs& a, bool from_end = false) {
         lane = threadIdx.x & 31; warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
         const unsigned int unit = blockIdx.x * kScanWarps + warp, at = unit / unsigned(a.channel_tiles);     // neighbouring channels of a chunk, then the next chunk's
         chunk = from_end ? a.chunks - 1 - int(at) : int(at);
-        channel0 = int(unit - at * unsigned(a.channel_tiles)) * 32 * V;
-        channel = channel0 + lane * V;
-        inside = channel < a.in.width;
+        channel0 = int(unit - at * unsigned(a.channel_tiles)) * kChannels;
+        channel = channel0 + lane * 2;
+        live = max(0, min(2, a.in.width - channel));
         begin = chunk * a.chunk;
         end = at >= unsigned(a.chunks) ? begin : int(min(int64_t(begin) + a.chunk, a.in.rows));
     }
     __device__ __forceinline__ bool nothing() const { return end <= begin; }
     __device__ __forceinline__ int last_batch() const { return begin + (end - 1 - begin) / kBatch * kBatch; }
-    __device__ __forceinline__ int64_t state_at(const ScanArgs& a, int sequence) const { return int64_t(sequence) * a.in.width + channel; }
+    // The thread's channels in row `row` of a matrix of states (null: zeros).
+    __device__ __forceinline__ Num load(const float* states, int64_t row, const ScanArgs& a) const {
+        const float* p = states + row * a.in.width + channel;
+        return Num::make(states && live > 0 ? p[0] : 0.0f, states && live > 1 ? p[1] : 0.0f);
+    }
+    __device__ __forceinline__ void store(float* states, int64_t row, const ScanArgs& a, Num n) const {
+        float* p = states + row * a.in.width + channel;
+        const float2 f = n.get();
+        if (live > 0) p[0] = f.x;
+        if (live > 1) p[1] = f.y;
+    }
+    __device__ __forceinline__ void leave_map(const ScanArgs& a, Num A, Num H) const {
+        float2* p = a.composed + int64_t(chunk) * a.in.width + channel;
+        const float2 f = A.get(), h = H.get();
+        if (live > 0) p[0] = make_float2(f.x, h.x);
+        if (live > 1) p[1] = make_float2(f.y, h.y);
+    }
 };
 
-// A matrix's rows at a warp's channels on their way into its shared memory, a batch at a time, PIECE bytes at once: 16 where every row of the matrix allows it, or
-// 4.  PIECE 2 is for 16-bit rows that begin on 2 bytes: the 4-byte words that hold a row are copied, and its values lie 0 or 2 bytes behind the first.
-template <typename T, int V, int PIECE> struct Stream {
-    static constexpr int kRow = PIECE == 2 ? 68 : 32 * V * int(sizeof(T));         // bytes
-    static constexpr int bytes = kBatch * kRow;
-    static constexpr int kPieces = PIECE == 2 ? 17 : kRow / PIECE;
+// The thread's two values to a matrix; ALIGNED: they begin on a multiple of both, and exist together.
+template <typename T, bool ALIGNED> __device__ __forceinline__ void store_pair(T* to, Num n, int live) {
+    const float2 f = n.get();
+    if (ALIGNED) {
+        const float v[2] = {f.x, f.y};
+        if (live > 0) store_floats<T, 2>(to, v);
+    } else {
+        if (live > 0) to[0] = from_float<T>(f.x);
+        if (live > 1) to[1] = from_float<T>(f.y);
+    }
+}
+
+// A matrix's rows at a warp's channels on their way into its shared memory, a batch at a time, 16 bytes at once.  ALIGNED: every row begins on 16 bytes and has a whole
+// number of such pieces.  Else the pieces that hold a row are copied, and its values lie up to 15 bytes behind the first one's beginning; what else is in
+// those pieces is not looked at (a piece lies in the same 16 bytes of memory as a value that exists, so it can be read).
+template <typename T, bool ALIGNED> struct Stream {
+    static constexpr int kRow = kChannels * int(sizeof(T)) + (ALIGNED ? 0 : 16);     // bytes
+    static constexpr int bytes = kBatch * kRow, kPieces = kRow / 16;
     const char* first;                        // the channels' first value at position 0
     int64_t step;                             // bytes from position to position
     int valid;                                // bytes of a row that exist
-    __device__ __forceinline__ Stream(const void* base, int64_t stride, const ScanArgs& a, const Place<V>& at) {
+    __device__ __forceinline__ Stream(const void* base, int64_t stride, const ScanArgs& a, const Place& at) {
         first = static_cast<const char*>(base) + ((a.in.reverse ? (a.in.rows - 1) * stride : 0) + at.channel0) * int64_t(sizeof(T));
         step = (a.in.reverse ? -stride : stride) * int64_t(sizeof(T));
-        valid = min(32 * V, a.in.width - at.channel0) * int(sizeof(T));
+        valid = min(kChannels, a.in.width - at.channel0) * int(sizeof(T));
+    }
+    __device__ __forceinline__ static void piece(uint32_t to, const char* from) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
     }
     __device__ __forceinline__ void copy(unsigned char* to, int p, int count, int lane) const {
-        if constexpr (PIECE == 2) {
-            #pragma unroll
-            for (int i = 0; i < (kBatch * kPieces + 31) / 32; ++i) {
-                const int q = lane + 32 * i, r = q / kPieces, w = q % kPieces;
-                const uintptr_t row = reinterpret_cast<uintptr_t>(first + (p + r) * step), word = (row & ~uintptr_t(3)) + 4 * w;
-                if (r < count && word < row + valid) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to + r * kRow + 4 * w)), "l"(word) : "memory");
-            }
-        } else {
+        if constexpr (ALIGNED) {
             constexpr int kAtOnce = 32 / kPieces;                 // rows
-            const int r = lane / kPieces, c = lane % kPieces * PIECE;
+            const int r = lane / kPieces, c = lane % kPieces * 16;
             const char* from = first + (p + r) * step + c;
             const uint32_t here = smem_u32(to) + uint32_t(r * kRow + c);
             const int there = c < valid ? count - r : 0;
             #pragma unroll
-            for (int i = 0; i < kBatch / kAtOnce; ++i, from += kAtOnce * step) {
-                if (i * kAtOnce >= there) continue;
-                if constexpr (PIECE == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(here + i * kAtOnce * kRow), "l"(from) : "memory");
-                else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(here + i * kAtOnce * kRow), "l"(from) : "memory");
+            for (int i = 0; i < kBatch / kAtOnce; ++i, from += kAtOnce * step)
+                if (i * kAtOnce < there) piece(here + i * kAtOnce * kRow, from);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < (kBatch * kPieces + 31) / 32; ++i) {
+                const int q = lane + 32 * i, r = q / kPieces, w = q % kPieces;
+                const char* row = first + (p + r) * step;
+                const char* from = row - (reinterpret_cast<uintptr_t>(row) & 15) + 16 * w;
+                if (r < count && from < row + valid) piece(smem_u32(to) + uint32_t(r * kRow + 16 * w), from);
             }
         }
     }
     // The thread's channels of row i of a batch that begins at position p.
-    __device__ __forceinline__ Num<V> get(const unsigned char* stage, int p, int i, int lane) const {
-        if constexpr (PIECE == 2) {
-            const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(first)) + uint32_t(p + i) * uint32_t(step) & 2u;
-            return number<T, V>(*reinterpret_cast<const Pack<T, V>*>(stage + i * kRow + off + lane * V * int(sizeof(T))));
-        } else {
-            return number<T, V>(*reinterpret_cast<const Pack<T, V>*>(stage + i * kRow + lane * V * int(sizeof(T))));
+    __device__ __forceinline__ Num get(const unsigned char* stage, int p, int i, int lane) const {
+        const unsigned char* at = stage + i * kRow + lane * 2 * int(sizeof(T));
+        float f[2];
+        if constexpr (ALIGNED) load_floats<T, 2>(reinterpret_cast<const T*>(at), f);
+        else {
+            const T* v = reinterpret_cast<const T*>(at + ((uint32_t(reinterpret_cast<uintptr_t>(first)) + uint32_t(p + i) * uint32_t(step)) & 15u));
+            f[0] = to_float<T>(v[0]); f[1] = to_float<T>(v[1]);
         }
+        return Num::make(f[0], f[1]);
     }
 };
 
@@ -253,27 +240,27 @@ template <typename S, int N> struct Feed {
     }
 };
 
-template <typename T, int V, int PIECE, int N> constexpr int kFeedBytes = kScanWarps * kStages * N * Stream<T, V, PIECE>::bytes;
+template <typename T, bool ALIGNED, int N> constexpr int kFeedBytes = kScanWarps * kStages * N * Stream<T, ALIGNED>::bytes;
 
 // First pass, forward: the composition of each chunk.
-template <typename T, int V, int PIECE>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kScanBlock, 10) scan_compose_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    using S = Stream<T, V, PIECE>;
-    const Place<V> at(args);
+    using S = Stream<T, ALIGNED>;
+    const Place at(args);
     if (at.nothing()) return;
     const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at)};
     Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, false);
     Span span;
     span.find(args.in, at.begin);
-    Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
+    Num A = Num::all(1.0f), H = Num::all(0.0f);
     #pragma unroll 1
     for (int p = at.begin; p < at.end; p += kBatch) {
         const unsigned char *g = feed.next(), *x = g + S::bytes;
         if (at.end - p >= kBatch && span.begin < p && span.end >= p + kBatch) {
             #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                const Gate gate = gate_of(streams[0].get(g, p, i, at.lane));
                 H = madd(gate.a, H, gate.rest * streams[1].get(x, p, i, at.lane));
                 A = A * gate.a;
             }
@@ -281,38 +268,38 @@ __global__ void __launch_bounds__(kScanBlock, 10) scan_compose_kernel(const Scan
             #pragma unroll 1
             for (int i = 0; i < min(kBatch, at.end - p); ++i) {
                 if (p + i == span.end) span.move(args.in, true);
-                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                const Gate gate = gate_of(streams[0].get(g, p, i, at.lane));
                 if (p + i == span.begin) {
-                    A = Num<V>::all(kCut);
-                    H = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, span.sequence));
+                    A = Num::all(kCut);
+                    H = at.load(args.in.initial, span.sequence, args);
                 }
                 H = madd(gate.a, H, gate.rest * streams[1].get(x, p, i, at.lane));
                 A = A * gate.a;
             }
         }
     }
-    if (at.inside) leave_map<V>(&args.composed[int64_t(at.chunk) * args.in.width + at.channel], A, H);
+    at.leave_map(args, A, H);
 }
 
 // First pass, backward: E in front of a chunk as a map of E behind it.
-template <typename T, int V, int PIECE>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kScanBlock, 10) scan_compose_backward_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    using S = Stream<T, V, PIECE>;
-    const Place<V> at(args);
+    using S = Stream<T, ALIGNED>;
+    const Place at(args);
     if (at.nothing()) return;
     const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.grad_h, args.grad_h_stride, args, at)};
     Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, true);
     Span span;
     span.find(args.in, at.end - 1);
-    Num<V> A = Num<V>::all(1.0f), H = Num<V>::all(0.0f);
+    Num A = Num::all(1.0f), H = Num::all(0.0f);
     #pragma unroll 1
     for (int p = at.last_batch(); p >= at.begin; p -= kBatch) {
         const unsigned char *g = feed.next(), *d = g + S::bytes;
         if (at.end - p >= kBatch && span.begin <= p && span.end > p + kBatch) {
             #pragma unroll
             for (int i = kBatch - 1; i >= 0; --i) {
-                const Num<V> a = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane))).a;
+                const Num a = gate_of(streams[0].get(g, p, i, at.lane)).a;
                 H = a * (H + streams[1].get(d, p, i, at.lane));
                 A = A * a;
             }
@@ -320,17 +307,17 @@ __global__ void __launch_bounds__(kScanBlock, 10) scan_compose_backward_kernel(c
             #pragma unroll 1
             for (int i = min(kBatch, at.end - p) - 1; i >= 0; --i) {
                 if (p + i < span.begin) span.move(args.in, false);
-                const Num<V> a = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane))).a;
+                const Num a = gate_of(streams[0].get(g, p, i, at.lane)).a;
                 if (p + i + 1 == span.end) {
-                    A = Num<V>::all(kCut);
-                    H = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, span.sequence));
+                    A = Num::all(kCut);
+                    H = at.load(args.grad_last, span.sequence, args);
                 }
                 H = a * (H + streams[1].get(d, p, i, at.lane));
                 A = A * a;
             }
         }
     }
-    if (at.inside) leave_map<V>(&args.composed[int64_t(at.chunk) * args.in.width + at.channel], A, H);
+    at.leave_map(args, A, H);
 }
 
 // Second pass: the state at each chunk's beginning (from_end: behind each chunk, walking from the last to the first).  A cluster of `parts` blocks takes eight
@@ -405,16 +392,16 @@ __device__ __forceinline__ void pass_empty_sequences(const ScanArgs& args, const
 }
 
 // Third pass, forward; from the end, where the first pass has left the rows in L2.
-template <typename T, int V, int PIECE>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kScanBlock, 8) scan_apply_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    using S = Stream<T, V, PIECE>;
-    const Place<V> at(args, true);
+    using S = Stream<T, ALIGNED>;
+    const Place at(args, true);
     if (at.nothing()) return;
     const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at)};
     Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, false);
     grid_dependency();                        // x and gate are older than the first pass, which ended before the second began
-    Num<V> h = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
+    Num h = at.load(args.chunks > 1 ? args.carried : nullptr, at.chunk, args);
     Span span;
     span.find(args.in, at.begin);
     const int64_t step = args.in.reverse ? -args.h_stride : args.h_stride;
@@ -422,75 +409,71 @@ __global__ void __launch_bounds__(kScanBlock, 8) scan_apply_kernel(const ScanArg
     #pragma unroll 1
     for (int p = at.begin; p < at.end; p += kBatch) {
         const unsigned char *g = feed.next(), *x = g + S::bytes;
-        if (args.states && at.inside) store_state<V>(args.states, int64_t(p / kBatch) * args.in.width + at.channel, h);
+        if (args.states) at.store(args.states, p / kBatch, args, h);
         if (at.end - p >= kBatch && span.begin < p && span.end > p + kBatch) {
             #pragma unroll
             for (int i = 0; i < kBatch; ++i, to += step) {
-                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                const Gate gate = gate_of(streams[0].get(g, p, i, at.lane));
                 h = madd(gate.a, h, gate.rest * streams[1].get(x, p, i, at.lane));
-                if (at.inside) store_number<T, V>(to, h);
+                store_pair<T, ALIGNED>(to, h, at.live);
             }
         } else {
             #pragma unroll 1
             for (int i = 0; i < min(kBatch, at.end - p); ++i, to += step) {
                 if (p + i == span.end) span.move(args.in, true);
-                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
-                if (p + i == span.begin) h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, span.sequence));
+                const Gate gate = gate_of(streams[0].get(g, p, i, at.lane));
+                if (p + i == span.begin) h = at.load(args.in.initial, span.sequence, args);
                 h = madd(gate.a, h, gate.rest * streams[1].get(x, p, i, at.lane));
-                if (at.inside) {
-                    store_number<T, V>(to, h);
-                    if (p + i + 1 == span.end) store_state<V>(args.last, at.state_at(args, span.sequence), h);
-                }
+                store_pair<T, ALIGNED>(to, h, at.live);
+                if (p + i + 1 == span.end) at.store(args.last, span.sequence, args, h);
             }
         }
     }
-    if (at.inside) pass_empty_sequences(args, args.in.initial, args.last, at.chunk, at.channel, V);
+    pass_empty_sequences(args, args.in.initial, args.last, at.chunk, at.channel, at.live);
 }
 
 // Third pass, backward: eight rows forward from the state that was kept, then back.
-template <typename T, int V, int PIECE>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kScanBlock, 5) scan_apply_backward_kernel(const ScanArgs args) {
     extern __shared__ __align__(16) unsigned char memory[];
-    using S = Stream<T, V, PIECE>;
-    const Place<V> at(args, true);
+    using S = Stream<T, ALIGNED>;
+    const Place at(args, true);
     if (at.nothing()) return;
     const S streams[3] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at), S(args.grad_h, args.grad_h_stride, args, at)};
     Feed<S, 3> feed(streams, memory + at.warp * kStages * 3 * S::bytes, at.lane, at.begin, at.end, true);
     grid_dependency();
     int p = at.last_batch();
-    Num<V> kept = load_state<V>(at.inside ? args.states : nullptr, int64_t(p / kBatch) * args.in.width + at.channel);
-    Num<V> E = load_state<V>(args.chunks > 1 && at.inside ? args.carried : nullptr, int64_t(at.chunk) * args.in.width + at.channel);
+    Num kept = at.load(args.states, p / kBatch, args);
+    Num E = at.load(args.chunks > 1 ? args.carried : nullptr, at.chunk, args);
     Span span;
     span.find(args.in, at.end - 1);
     const int64_t step_x = args.in.reverse ? -args.grad_x_stride : args.grad_x_stride, step_gate = args.in.reverse ? -args.grad_gate_stride : args.grad_gate_stride;
     const int64_t row = args.in.reverse ? args.in.rows - at.end : at.end - 1;
     T* to_x = static_cast<T*>(args.grad_x) + row * args.grad_x_stride + at.channel;
     T* to_gate = static_cast<T*>(args.grad_gate) + row * args.grad_gate_stride + at.channel;
-    const Num<V> minus = Num<V>::all(-1.0f);
+    const Num minus = Num::all(-1.0f);
     #pragma unroll 1
     for (; p >= at.begin; p -= kBatch) {
         const unsigned char *g = feed.next(), *x = g + S::bytes, *d = x + S::bytes;
-        Num<V> h = kept;
-        if (p > at.begin) kept = load_state<V>(at.inside ? args.states : nullptr, int64_t(p / kBatch - 1) * args.in.width + at.channel);
+        Num h = kept;
+        if (p > at.begin) kept = at.load(args.states, p / kBatch - 1, args);
         const int count = min(kBatch, at.end - p);
-        Num<V> a[kBatch], rest[kBatch], slope[kBatch];               // slope: (h_{t-1} - x) a (1 - a)
+        Num a[kBatch], rest[kBatch], slope[kBatch];               // slope: (h_{t-1} - x) a (1 - a)
         if (count == kBatch && span.begin < p && span.end > p + kBatch) {
             #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                const Gate gate = gate_of(streams[0].get(g, p, i, at.lane));
                 a[i] = gate.a; rest[i] = gate.rest;
-                const Num<V> value = streams[1].get(x, p, i, at.lane);
+                const Num value = streams[1].get(x, p, i, at.lane);
                 slope[i] = madd(minus, value, h) * (gate.a * gate.rest);
                 h = madd(gate.a, h, gate.rest * value);
             }
             #pragma unroll
             for (int i = kBatch - 1; i >= 0; --i, to_x -= step_x, to_gate -= step_gate) {
-                const Num<V> D = streams[2].get(d, p, i, at.lane) + E;
+                const Num D = streams[2].get(d, p, i, at.lane) + E;
                 E = a[i] * D;
-                if (at.inside) {
-                    store_number<T, V>(to_x, rest[i] * D);
-                    store_number<T, V>(to_gate, slope[i] * D);
-                }
+                store_pair<T, ALIGNED>(to_x, rest[i] * D, at.live);
+                store_pair<T, ALIGNED>(to_gate, slope[i] * D, at.live);
             }
         } else {
             Span ahead;
@@ -499,10 +482,10 @@ __global__ void __launch_bounds__(kScanBlock, 5) scan_apply_backward_kernel(cons
             for (int i = 0; i < kBatch; ++i) {
                 if (i >= count) break;
                 if (p + i == ahead.end) ahead.move(args.in, true);
-                if (p + i == ahead.begin) h = load_state<V>(at.inside ? args.in.initial : nullptr, at.state_at(args, ahead.sequence));
-                const Gate<V> gate = gate_of<V>(gate_exp<V>(streams[0].get(g, p, i, at.lane)));
+                if (p + i == ahead.begin) h = at.load(args.in.initial, ahead.sequence, args);
+                const Gate gate = gate_of(streams[0].get(g, p, i, at.lane));
                 a[i] = gate.a; rest[i] = gate.rest;
-                const Num<V> value = streams[1].get(x, p, i, at.lane);
+                const Num value = streams[1].get(x, p, i, at.lane);
                 slope[i] = madd(minus, value, h) * (gate.a * gate.rest);
                 h = madd(gate.a, h, gate.rest * value);
             }
@@ -510,19 +493,17 @@ __global__ void __launch_bounds__(kScanBlock, 5) scan_apply_backward_kernel(cons
             for (int i = kBatch - 1; i >= 0; --i) {
                 if (i >= count) continue;
                 if (p + i < span.begin) span.move(args.in, false);
-                if (p + i + 1 == span.end) E = load_state<V>(at.inside ? args.grad_last : nullptr, at.state_at(args, span.sequence));
-                const Num<V> D = streams[2].get(d, p, i, at.lane) + E;
+                if (p + i + 1 == span.end) E = at.load(args.grad_last, span.sequence, args);
+                const Num D = streams[2].get(d, p, i, at.lane) + E;
                 E = a[i] * D;
-                if (at.inside) {
-                    store_number<T, V>(to_x, rest[i] * D);
-                    store_number<T, V>(to_gate, slope[i] * D);
-                    if (p + i == span.begin && args.grad_initial) store_state<V>(args.grad_initial, at.state_at(args, span.sequence), E);
-                }
+                store_pair<T, ALIGNED>(to_x, rest[i] * D, at.live);
+                store_pair<T, ALIGNED>(to_gate, slope[i] * D, at.live);
+                if (p + i == span.begin && args.grad_initial) at.store(args.grad_initial, span.sequence, args, E);
                 to_x -= step_x; to_gate -= step_gate;
             }
         }
     }
-    if (at.inside) pass_empty_sequences(args, args.grad_last, args.grad_initial, at.chunk, at.channel, V);
+    pass_empty_sequences(args, args.grad_last, args.grad_initial, at.chunk, at.channel, at.live);
 }
 
 // One step for each row, the state updated in place.
@@ -532,9 +513,9 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const T* __restrict__ x,
     const int64_t total = rows * width, step = int64_t(gridDim.x) * 256;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
         const int64_t row = i / width, channel = i - row * width;
-        const Gate<1> g = gate_of<1>(gate_exp<1>({to_float<T>(gate[row * gate_stride + channel])}));
+        const Gate g = gate_of(Num::all(to_float<T>(gate[row * gate_stride + channel])));
         float* s = state + row * state_stride + channel;
-        const float next = fmaf(g.a.v, *s, g.rest.v * to_float<T>(x[row * x_stride + channel]));
+        const float next = fmaf(g.a.get().x, *s, g.rest.get().x * to_float<T>(x[row * x_stride + channel]));
         *s = next;
         h[row * h_stride + channel] = from_float<T>(next);
     }
@@ -564,8 +545,7 @@ int chunk_rows(int64_t rows, int64_t tiles) {
     while (chunk > 16 && pieces(rows, chunk) * tiles < 148 * 32) chunk /= 2;
     return chunk;
 }
-// Over both layouts of the channels: with two a lane there are fewer tiles, and so more chunks.
-int64_t most_chunks(int64_t rows, int64_t width) { return pieces(rows, chunk_rows(rows, (width + 63) / 64)); }
+int64_t chunk_count(int64_t rows, int64_t width) { return pieces(rows, chunk_rows(rows, pieces(width, kChannels))); }
 
 // `behind`: close behind the kernel before, for which the kernel waits itself.
 template <typename K> cudaError_t launch_chunks(K kernel, PerDeviceOnce& once, const ScanArgs& args, int smem, bool behind, cudaStream_t stream) {
@@ -577,35 +557,28 @@ template <typename K> cudaError_t launch_chunks(K kernel, PerDeviceOnce& once, c
     return cudaSuccess;
 }
 
-template <typename T, int V, int PIECE> cudaError_t scan_launch(ScanArgs& args, bool backward, cudaStream_t stream) {
+template <typename T, bool ALIGNED> cudaError_t scan_launch(ScanArgs& args, bool backward, cudaStream_t stream) {
     static PerDeviceOnce compose, apply, compose_backward, apply_backward;
-    constexpr int two = kFeedBytes<T, V, PIECE, 2>, three = kFeedBytes<T, V, PIECE, 3>;
-    args.channel_tiles = (args.in.width + 32 * V - 1) / (32 * V);
+    constexpr int two = kFeedBytes<T, ALIGNED, 2>, three = kFeedBytes<T, ALIGNED, 3>;
+    args.channel_tiles = int(pieces(args.in.width, kChannels));
     args.chunk = chunk_rows(args.in.rows, args.channel_tiles);
     args.chunks = int(pieces(args.in.rows, args.chunk));
     cudaError_t err = cudaSuccess;
     if (args.chunks > 1) {
-        err = backward ? launch_chunks(scan_compose_backward_kernel<T, V, PIECE>, compose_backward, args, two, false, stream)
-                       : launch_chunks(scan_compose_kernel<T, V, PIECE>, compose, args, two, false, stream);
+        err = backward ? launch_chunks(scan_compose_backward_kernel<T, ALIGNED>, compose_backward, args, two, false, stream)
+                       : launch_chunks(scan_compose_kernel<T, ALIGNED>, compose, args, two, false, stream);
         if (err == cudaSuccess) err = launch_carry(args, backward, stream);
     }
     if (err != cudaSuccess) return err;
-    return backward ? launch_chunks(scan_apply_backward_kernel<T, V, PIECE>, apply_backward, args, three, args.chunks > 1, stream)
-                    : launch_chunks(scan_apply_kernel<T, V, PIECE>, apply, args, two, args.chunks > 1, stream);
+    return backward ? launch_chunks(scan_apply_backward_kernel<T, ALIGNED>, apply_backward, args, three, args.chunks > 1, stream)
+                    : launch_chunks(scan_apply_kernel<T, ALIGNED>, apply, args, two, args.chunks > 1, stream);
 }
 
-// Two channels a lane where every row allows it, in pieces of 16 bytes where they do too.
 template <typename T> int scan_typed(ScanArgs& a, bool backward, cudaStream_t stream) {
-    const auto allow = [&](size_t bytes) {
-        const auto one = [&](const void* p, int64_t stride) { return !p || rows_aligned(p, stride, a.in.rows, sizeof(T), bytes); };
-        return size_t(a.in.width) * sizeof(T) % bytes == 0 && one(a.in.x, a.in.x_stride) && one(a.in.gate, a.in.gate_stride) && one(a.h, a.h_stride) &&
-               one(a.grad_h, a.grad_h_stride) && one(a.grad_x, a.grad_x_stride) && one(a.grad_gate, a.grad_gate_stride);
-    };
-    cudaError_t err;
-    if (allow(16)) err = scan_launch<T, 2, 16>(a, backward, stream);
-    else if constexpr (sizeof(T) == 4) err = scan_launch<T, 1, 4>(a, backward, stream);
-    else if (allow(4)) err = scan_launch<T, 2, 4>(a, backward, stream);
-    else err = scan_launch<T, 1, 2>(a, backward, stream);
+    const auto one = [&](const void* p, int64_t stride) { return !p || rows_aligned(p, stride, a.in.rows, sizeof(T), 16); };
+    const bool whole = size_t(a.in.width) * sizeof(T) % 16 == 0 && one(a.in.x, a.in.x_stride) && one(a.in.gate, a.in.gate_stride) && one(a.h, a.h_stride) &&
+                       one(a.grad_h, a.grad_h_stride) && one(a.grad_x, a.grad_x_stride) && one(a.grad_gate, a.grad_gate_stride);
+    const cudaError_t err = whole ? scan_launch<T, true>(a, backward, stream) : scan_launch<T, false>(a, backward, stream);
     return err == cudaSuccess ? sequence_status("htgs_gated_scan") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
@@ -638,7 +611,7 @@ size_t htgs_gated_scan_state_bytes(int64_t rows, int32_t width) {
 
 size_t htgs_gated_scan_workspace_bytes(int64_t rows, int32_t width) {
     if (rows <= 0 || width <= 0) return 0;
-    const size_t values = size_t(htgs::most_chunks(rows, width)) * size_t(width);
+    const size_t values = size_t(htgs::chunk_count(rows, width)) * size_t(width);
     return htgs::align256(values * sizeof(float2)) + htgs::align256(values * sizeof(float));
 }
 
@@ -655,7 +628,7 @@ int htgs_gated_scan(const HtgsScan* scan, void* h, int64_t h_stride, float* last
     ScanArgs a{};
     a.in = *scan;
     a.composed = static_cast<float2*>(workspace);
-    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(most_chunks(scan->rows, scan->width)) * size_t(scan->width) * sizeof(float2)));
+    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(chunk_count(scan->rows, scan->width)) * size_t(scan->width) * sizeof(float2)));
     a.states = states;
     a.h = h; a.h_stride = h_stride; a.last = last;
     if (scan->type == HTGS_FLOAT32) return scan_typed<float>(a, false, s);
@@ -678,7 +651,7 @@ int htgs_gated_scan_backward(const HtgsScan* scan, const float* states, const vo
     ScanArgs a{};
     a.in = *scan;
     a.composed = static_cast<float2*>(workspace);
-    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(most_chunks(scan->rows, scan->width)) * size_t(scan->width) * sizeof(float2)));
+    a.carried = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(size_t(chunk_count(scan->rows, scan->width)) * size_t(scan->width) * sizeof(float2)));
     a.states = const_cast<float*>(states);
     a.grad_h = grad_h; a.grad_h_stride = grad_h_stride; a.grad_last = grad_last;
     a.grad_x = grad_x; a.grad_x_stride = grad_x_stride; a.grad_gate = grad_gate; a.grad_gate_stride = grad_gate_stride; a.grad_initial = grad_initial;
