@@ -7,7 +7,7 @@
 // A step is the map h -> A h + H, and steps compose: (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2).  The rows are cut into chunks of 16 to 64.  One
 // kernel composes each chunk's rows, one walks from chunk to chunk and leaves the state in front of each, one goes through the
 // chunks again from those states and writes h.  The backward pass does the same from the end.  A warp takes a chunk of 64 channels and goes
-// through it eight rows at a time, the next sixteen on their way into shared memory of its own; warps never wait for one another.  For the backward pass the
+// through it eight rows at a time, the next on their way into shared memory of its own; warps never wait for one another.  For the backward pass the
 // forward one keeps the state in front of every eight rows: h_{t-1} is computed again from there, so it is in 32 bits and neither h nor the rows
 // before are read.  A sequence's first row has A = 0 and takes its initial state into H, so packed sequences need no chunks of their own; that zero is
 // kept as -0 and tested for, so that a NaN or infinity of one sequence does not reach the next.  States, products and sums are 32-bit; 1 - a is
@@ -22,7 +22,6 @@ namespace {
 constexpr int kChannels = 64;                // of a warp, two a lane
 constexpr int kBatch = 8;                    // rows that a warp deals with at a time; a state in front of each batch is kept for the backward pass
 constexpr int kMostChunk = 64;               // rows
-constexpr int kStages = 3;                   // batches of a warp in shared memory
 constexpr int kScanWarps = 4, kScanBlock = kScanWarps * 32;
 constexpr int kCarryWarps = 32, kCarryChannels = 8, kCarryRun = 16;
 
@@ -162,6 +161,7 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void store_pair(T
 template <typename T, bool ALIGNED> struct Stream {
     static constexpr int kRow = kChannels * int(sizeof(T)) + (ALIGNED ? 0 : 16);     // bytes
     static constexpr int bytes = kBatch * kRow, kPieces = kRow / 16;
+    static constexpr int stages = sizeof(T) == 4 ? 2 : 3;        // batches of a warp in shared memory; with three of 32-bit rows too few warps fit an SM
     const char* first;                        // the channels' first value at position 0
     int64_t step;                             // bytes from position to position
     int valid;                                // bytes of a row that exist
@@ -220,27 +220,27 @@ template <typename S, int N> struct Feed {
             --left;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        to = to + 1 == kStages ? 0 : to + 1;
+        to = to + 1 == S::stages ? 0 : to + 1;
     }
     __device__ __forceinline__ Feed(const S (&s)[N], unsigned char* memory, int lane_, int begin_, int end_, bool back_)
         : streams(s), ring(memory), lane(lane_), begin(begin_), end(end_), back(back_) {
         left = (end - begin + kBatch - 1) / kBatch;
         p = back ? begin + (left - 1) * kBatch : begin;
         #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) send();
+        for (int i = 0; i < S::stages - 1; ++i) send();
     }
     // The next batch's place; what was in the stage behind it may be overwritten from here on.
     __device__ __forceinline__ const unsigned char* next() {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::stages - 2) : "memory");
         __syncwarp();
         const unsigned char* stage = ring + from * N * S::bytes;
-        from = from + 1 == kStages ? 0 : from + 1;
+        from = from + 1 == S::stages ? 0 : from + 1;
         send();
         return stage;
     }
 };
 
-template <typename T, bool ALIGNED, int N> constexpr int kFeedBytes = kScanWarps * kStages * N * Stream<T, ALIGNED>::bytes;
+template <typename T, bool ALIGNED, int N> constexpr int kFeedBytes = kScanWarps * Stream<T, ALIGNED>::stages * N * Stream<T, ALIGNED>::bytes;
 
 // First pass, forward: the composition of each chunk.
 template <typename T, bool ALIGNED>
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kScanBlock, 10) scan_compose_kernel(const Scan
     const Place at(args);
     if (at.nothing()) return;
     const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at)};
-    Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, false);
+    Feed<S, 2> feed(streams, memory + at.warp * S::stages * 2 * S::bytes, at.lane, at.begin, at.end, false);
     Span span;
     span.find(args.in, at.begin);
     Num A = Num::all(1.0f), H = Num::all(0.0f);
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kScanBlock, 10) scan_compose_backward_kernel(c
     const Place at(args);
     if (at.nothing()) return;
     const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.grad_h, args.grad_h_stride, args, at)};
-    Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, true);
+    Feed<S, 2> feed(streams, memory + at.warp * S::stages * 2 * S::bytes, at.lane, at.begin, at.end, true);
     Span span;
     span.find(args.in, at.end - 1);
     Num A = Num::all(1.0f), H = Num::all(0.0f);
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kScanBlock, 8) scan_apply_kernel(const ScanArg
     const Place at(args, true);
     if (at.nothing()) return;
     const S streams[2] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at)};
-    Feed<S, 2> feed(streams, memory + at.warp * kStages * 2 * S::bytes, at.lane, at.begin, at.end, false);
+    Feed<S, 2> feed(streams, memory + at.warp * S::stages * 2 * S::bytes, at.lane, at.begin, at.end, false);
     grid_dependency();                        // x and gate are older than the first pass, which ended before the second began
     Num h = at.load(args.chunks > 1 ? args.carried : nullptr, at.chunk, args);
     Span span;
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kScanBlock, 5) scan_apply_backward_kernel(cons
     const Place at(args, true);
     if (at.nothing()) return;
     const S streams[3] = {S(args.in.gate, args.in.gate_stride, args, at), S(args.in.x, args.in.x_stride, args, at), S(args.grad_h, args.grad_h_stride, args, at)};
-    Feed<S, 3> feed(streams, memory + at.warp * kStages * 3 * S::bytes, at.lane, at.begin, at.end, true);
+    Feed<S, 3> feed(streams, memory + at.warp * S::stages * 3 * S::bytes, at.lane, at.begin, at.end, true);
     grid_dependency();
     int p = at.last_batch();
     Num kept = at.load(args.states, p / kBatch, args);
