@@ -20,12 +20,12 @@ struct QuantArgs {
     uint8_t* codes_t; uint8_t* scales_t; int64_t codes_t_stride, scales_t_stride; // transposed; may be null
 };
 
-// A warp takes 32 * VEC columns, VEC side by side in a lane (VEC 1: 128 columns, four of them 32 apart in a lane), of several rows, four at a
+// A warp takes 32 * VEC columns, VEC side by side in a lane, but 128 at least (VEC 1, 2: in a lane several, 32 * VEC apart), of several rows, four at a
 // time, so that enough loads are on their way.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const QuantArgs a) {
     const int lane = threadIdx.x & 31;
-    constexpr int kColumns = VEC == 1 ? kScaleBlock : 32 * VEC, kValues = VEC == 1 ? 4 : VEC, kLanes = VEC == 8 ? 16 : 32, R = 4;
+    constexpr int kColumns = VEC < 4 ? kScaleBlock : 32 * VEC, kValues = kColumns / 32, kLanes = VEC == 8 ? 16 : 32, R = 4;
     const uint32_t across = uint32_t((a.width + kColumns - 1) / kColumns), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
     const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;        // rows that are begun side by side
     if (warp >= across * down) return;
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const Qua
             const T* x = static_cast<const T*>(a.x) + row * a.x_stride + first + lane * VEC;
             #pragma unroll
             for (int i = 0; i < kValues / VEC; ++i) {
-                if (row < a.rows && first + 32 * i + lane * VEC < a.width) raw[r][i] = *reinterpret_cast<const Pack<T, VEC>*>(x + 32 * i);
+                if (row < a.rows && first + (32 * i + lane) * VEC < a.width) raw[r][i] = *reinterpret_cast<const Pack<T, VEC>*>(x + 32 * VEC * i);
                 else {
                     #pragma unroll
                     for (int k = 0; k < VEC; ++k) raw[r][i].v[k] = from_float<T>(0.0f);
@@ -63,13 +63,15 @@ __global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const Qua
             if (careful) largest = largest_finite(v);
             const int e = scale_exponent(lanes_max<kLanes>(largest));
             const float inverse = inverse_scale(e);
-            if (VEC == 1) {
+            #pragma unroll
+            for (int i = 0; i < kValues / VEC; ++i) {
+                const int64_t column = first + (32 * i + lane) * VEC;
+                if (column >= a.width) continue;
+                float f[VEC];
                 #pragma unroll
-                for (int i = 0; i < kValues; ++i)
-                    if (first + 32 * i + lane < a.width) codes[first + 32 * i + lane] = uint8_t(encode2<true>(v[i], 0.0f, inverse) & 0xffu);
-            } else if (first + lane * VEC < a.width) {
-                if (careful) store_codes<true>(codes + first + lane * VEC, v, inverse);
-                else store_codes<false>(codes + first + lane * VEC, v, inverse);
+                for (int k = 0; k < VEC; ++k) f[k] = v[i * VEC + k];
+                if (careful) store_codes<true>(codes + column, f, inverse);
+                else store_codes<false>(codes + column, f, inverse);
             }
             if (lane % kLanes == 0 && at < a.width) a.scales[row * a.scales_stride + at / kScaleBlock] = uint8_t(e + 127);
         }
@@ -101,6 +103,15 @@ __global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const Qu
             const int at = i * kQuantBlock + int(threadIdx.x), r = at / kPieces, c = at % kPieces * VEC;
             const bool there = r < rows && c < columns;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&tile[r][c])), "l"(there ? x + r * a.x_stride + c : x), "r"(there ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (a.x_stride * sizeof(T) % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 4 == 0 && (sizeof(T) == 4 || columns % 2 == 0)) {
+        constexpr int kTogether = 4 / int(sizeof(T)), kPieces = kScaleBlock / kTogether;
+        #pragma unroll 8
+        for (int i = 0; i < kScaleBlock * kPieces / kQuantBlock; ++i) {
+            const int at = i * kQuantBlock + int(threadIdx.x), r = at / kPieces, c = at % kPieces * kTogether;
+            const bool there = r < rows && c < columns;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(&tile[r][c])), "l"(there ? x + r * a.x_stride + c : x), "r"(there ? 4 : 0) : "memory");
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
@@ -223,20 +234,22 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(kQuantBlock, 6) dequantize_kernel(const uint8_t* codes, int64_t codes_stride, const uint8_t* scales, int64_t scales_stride,
                                                                 int shift, int64_t rows, int64_t width, T* out, int64_t out_stride) {
     const int lane = threadIdx.x & 31;
-    constexpr int R = 4;
-    const uint32_t across = uint32_t((width + 32 * VEC - 1) / (32 * VEC)), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
+    constexpr int kColumns = VEC < 4 ? kScaleBlock : 32 * VEC, G = kColumns / 32 / VEC, R = 4;       // as in quantize_rows_kernel
+    const uint32_t across = uint32_t((width + kColumns - 1) / kColumns), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
     const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;
-    const int64_t column = int64_t(warp % across) * (32 * VEC) + lane * VEC;
+    const int64_t column = int64_t(warp % across) * kColumns + lane * VEC;
     grid_dependency();
     if (warp >= across * down || column >= width) return;
     for (int64_t row0 = warp / across; row0 < rows; row0 += int64_t(down) * R) {
-        Pack<uint8_t, VEC> packed[R];
+        Pack<uint8_t, VEC> packed[R][G];
         uint32_t exponent[R];
         #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + int64_t(down) * r;
             if (row >= rows) break;
-            packed[r] = *reinterpret_cast<const Pack<uint8_t, VEC>*>(codes + row * codes_stride + column);
+            #pragma unroll
+            for (int j = 0; j < G; ++j)
+                if (column + 32 * VEC * j < width) packed[r][j] = *reinterpret_cast<const Pack<uint8_t, VEC>*>(codes + row * codes_stride + column + 32 * VEC * j);
             exponent[r] = scales[(row >> shift) * scales_stride + column / kScaleBlock];
         }
         #pragma unroll
@@ -244,18 +257,25 @@ __global__ void __launch_bounds__(kQuantBlock, 6) dequantize_kernel(const uint8_
             const int64_t row = row0 + int64_t(down) * r;
             if (row >= rows) break;
             const float scale = scale_value(exponent[r]);
-            T* to = out + row * out_stride + column;
-            if constexpr (VEC > 1) {
-                const uint32_t* words = reinterpret_cast<const uint32_t*>(&packed[r]);
+            #pragma unroll
+            for (int j = 0; j < G; ++j) {
+                if (column + 32 * VEC * j >= width) break;
                 float v[VEC];
-                #pragma unroll
-                for (int k = 0; k < VEC; k += 2) {
-                    const float2 f = decode2(words[k / 4] >> (k % 4 * 8));
-                    v[k] = f.x * scale; v[k + 1] = f.y * scale;
+                if constexpr (VEC == 1) v[0] = decode2(packed[r][j].v[0]).x * scale;
+                else {
+                    uint32_t words[(VEC + 3) / 4];
+                    if constexpr (VEC == 2) words[0] = *reinterpret_cast<const uint16_t*>(&packed[r][j]);
+                    else {
+                        #pragma unroll
+                        for (int k = 0; k < VEC / 4; ++k) words[k] = reinterpret_cast<const uint32_t*>(&packed[r][j])[k];
+                    }
+                    #pragma unroll
+                    for (int k = 0; k < VEC; k += 2) {
+                        const float2 f = decode2(words[k / 4] >> (k % 4 * 8));
+                        v[k] = f.x * scale; v[k + 1] = f.y * scale;
+                    }
                 }
-                store_floats<T, VEC>(to, v);
-            } else {
-                *to = from_float<T>(decode2(packed[r].v[0]).x * scale);
+                store_floats<T, VEC>(out + row * out_stride + column + 32 * VEC * j, v);
             }
         }
     }
@@ -271,7 +291,7 @@ unsigned int blocks_for(int64_t rows, int64_t width, int columns) {
 }
 
 template <typename T, int VEC> void launch_rows(const QuantArgs& a, cudaStream_t stream) {
-    quantize_rows_kernel<T, VEC><<<blocks_for(a.rows, a.width, VEC == 1 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream>>>(a);
+    quantize_rows_kernel<T, VEC><<<blocks_for(a.rows, a.width, VEC < 4 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream>>>(a);
 }
 template <typename T, bool WIDE, bool PER_TILE> cudaError_t launch_tiles(const QuantArgs& a, cudaStream_t stream) {
     const dim3 grid(unsigned((a.width + kScaleBlock - 1) / kScaleBlock), unsigned((a.rows + kScaleBlock - 1) / kScaleBlock));
@@ -288,17 +308,23 @@ template <typename T> int quantize_typed(const QuantArgs& a, int rows_per_scale,
     if (rows_per_scale != 1) err = wide ? launch_tiles<T, true, true>(a, stream) : launch_tiles<T, false, true>(a, stream);
     else if (a.codes_t) err = wide ? launch_tiles<T, true, false>(a, stream) : launch_tiles<T, false, false>(a, stream);
     else if (wide && rows_aligned(a.codes, a.codes_stride, a.rows, 1, V)) launch_rows<T, V>(a, stream);
+    else if (sizeof(T) == 2 && a.width % 2 == 0 && rows_aligned(a.x, a.x_stride, a.rows, 2, 4) && rows_aligned(a.codes, a.codes_stride, a.rows, 1, 2))
+        launch_rows<T, sizeof(T) == 2 ? 2 : 1>(a, stream);
     else launch_rows<T, 1>(a, stream);
     return err == cudaSuccess ? sequence_status("htgs_quantize_fp8") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
 template <typename T, int VEC> void launch_dequantize(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
-    (void)launch_after(dequantize_kernel<T, VEC>, blocks_for(m.rows, m.width, 32 * VEC), kQuantBlock, 0, stream, m.codes, m.codes_stride, m.scales, m.scales_stride,
+    (void)launch_after(dequantize_kernel<T, VEC>, blocks_for(m.rows, m.width, VEC < 4 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream, m.codes, m.codes_stride, m.scales, m.scales_stride,
                        m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);       // the caller asks for the last error
 }
 template <typename T> void dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
     constexpr int V = 16 / int(sizeof(T));        // 16 bytes to store: with 32 a lane every store would write half sectors
-    if (m.width % V == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, V) && rows_aligned(out, out_stride, m.rows, sizeof(T), 16)) launch_dequantize<T, V>(m, out, out_stride, stream);
+    const auto allow = [&](int values) {
+        return m.width % values == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, values) && rows_aligned(out, out_stride, m.rows, sizeof(T), values * sizeof(T));
+    };
+    if (allow(V)) launch_dequantize<T, V>(m, out, out_stride, stream);
+    else if (allow(2)) launch_dequantize<T, 2>(m, out, out_stride, stream);
     else launch_dequantize<T, 1>(m, out, out_stride, stream);
 }
 

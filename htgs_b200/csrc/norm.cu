@@ -53,7 +53,7 @@ template <int WPR> __device__ __forceinline__ float row_sum(float v, float* shar
 }
 
 // E values a lane, in groups of VEC side by side; group j of a warp starts at column (32 * j + lane) * VEC of the warp's 32 * E, so
-// that a block of 128 columns is held by 16 or 32 lanes of one group (VEC 8, 4) or by four groups (VEC 1) of one warp.
+// that a block of 128 columns is held by 16 or 32 lanes of one group (VEC 8, 4) or by two or four groups (VEC 2, 1) of one warp.
 template <typename T, int VEC, int E, int WPR, bool FP8>
 __global__ void __launch_bounds__(kNormBlock) norm_kernel(const NormArgs a) {
     __shared__ float shared[kNormWarps];
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kNormBlock) norm_kernel(const NormArgs a) {
     if (FP8) {
         uint8_t* codes = a.codes + row * a.codes_stride;
         uint8_t* scales = a.scales + row * a.scales_stride;
-        constexpr int kGroups = VEC == 1 ? 4 : 1;                    // groups in a block of 128 columns
+        constexpr int kGroups = VEC < 4 ? 4 / VEC : 1;               // groups in a block of 128 columns
         constexpr int kLanes = VEC == 8 ? 16 : 32;                   // lanes
         #pragma unroll
         for (int j = 0; j < G; j += kGroups) {
@@ -139,10 +139,10 @@ __global__ void __launch_bounds__(kNormBlock) norm_kernel(const NormArgs a) {
 
 // A block holds whole rows, eight columns a thread, and takes R of them at a time, so that enough loads are on their way; persistent, with
 // each thread's part of grad_weight in registers until the end.  Groups of VEC columns as in norm_kernel, 256 columns a warp.
-// Blocks of up to 128 threads (1024 columns), four per SM, have registers for four rows of 16-byte groups (two of other types); wider ones take one.
+// Blocks of up to 128 threads (1024 columns), four per SM, have registers for four rows of 16-bit groups (two of others); wider ones take one.
 template <typename T, int VEC, int MOST>
 __global__ void __launch_bounds__(MOST, MOST == kNarrowBlock ? kNarrowBlocks : 1) norm_backward_kernel(const NormBackwardArgs a) {
-    constexpr int G = kBackwardColumns / VEC, R = MOST != kNarrowBlock ? 1 : VEC * sizeof(T) == 16 && sizeof(T) == 2 ? 4 : 2;
+    constexpr int G = kBackwardColumns / VEC, R = MOST != kNarrowBlock ? 1 : VEC > 1 && sizeof(T) == 2 ? 4 : 2;
     __shared__ float shared[2][32][R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int base = warp * 32 * kBackwardColumns;
@@ -303,22 +303,28 @@ template <typename T, int VEC> void backward_launch(const NormBackwardArgs& a, c
     else norm_backward_kernel<T, VEC, kWideBlock><<<blocks, threads, 0, stream>>>(a);
 }
 
-// 16-byte groups where every row of every tensor allows them, single values otherwise.
+// Groups of 16 bytes where every row of every tensor allows them, of 4 where they allow that, single values otherwise.
 template <typename T> void norm_typed(const NormArgs& a, cudaStream_t stream) {
-    constexpr int V = 16 / int(sizeof(T));
-    const size_t e = sizeof(T);
-    const bool wide = a.width % V == 0 && rows_aligned(a.x, a.x_stride, a.rows, e, 16) && rows_aligned(a.residual, a.residual_stride, a.rows, e, 16) &&
-                      aligned(a.weight, 16) && rows_aligned(a.y, a.y_stride, a.rows, e, 16) && rows_aligned(a.sum, a.sum_stride, a.rows, e, 16) &&
-                      rows_aligned(a.codes, a.codes_stride, a.rows, 1, 8);
-    if (wide) norm_widths<T, V>(a, stream); else norm_widths<T, 1>(a, stream);
+    const auto allow = [&](int values) {
+        const size_t e = sizeof(T), bytes = values * e;
+        return a.width % values == 0 && rows_aligned(a.x, a.x_stride, a.rows, e, bytes) && rows_aligned(a.residual, a.residual_stride, a.rows, e, bytes) &&
+               aligned(a.weight, bytes) && rows_aligned(a.y, a.y_stride, a.rows, e, bytes) && rows_aligned(a.sum, a.sum_stride, a.rows, e, bytes) &&
+               rows_aligned(a.codes, a.codes_stride, a.rows, 1, values);
+    };
+    if (allow(16 / int(sizeof(T)))) norm_widths<T, 16 / int(sizeof(T))>(a, stream);
+    else if (sizeof(T) == 2 && allow(2)) norm_widths<T, sizeof(T) == 2 ? 2 : 1>(a, stream);
+    else norm_widths<T, 1>(a, stream);
 }
 template <typename T> void backward_typed(const NormBackwardArgs& a, void* grad_weight, cudaStream_t stream) {
-    constexpr int V = 16 / int(sizeof(T));
-    const size_t e = sizeof(T);
-    const bool wide = a.width % V == 0 && rows_aligned(a.grad_y, a.grad_y_stride, a.rows, e, 16) && rows_aligned(a.grad_sum, a.grad_sum_stride, a.rows, e, 16) &&
-                      rows_aligned(a.x, a.x_stride, a.rows, e, 16) && rows_aligned(a.residual, a.residual_stride, a.rows, e, 16) && aligned(a.weight, 16) &&
-                      rows_aligned(a.grad_x, a.grad_x_stride, a.rows, e, 16);
-    if (wide) backward_launch<T, V>(a, stream); else backward_launch<T, 1>(a, stream);
+    const auto allow = [&](int values) {
+        const size_t e = sizeof(T), bytes = values * e;
+        return a.width % values == 0 && rows_aligned(a.grad_y, a.grad_y_stride, a.rows, e, bytes) && rows_aligned(a.grad_sum, a.grad_sum_stride, a.rows, e, bytes) &&
+               rows_aligned(a.x, a.x_stride, a.rows, e, bytes) && rows_aligned(a.residual, a.residual_stride, a.rows, e, bytes) && aligned(a.weight, bytes) &&
+               rows_aligned(a.grad_x, a.grad_x_stride, a.rows, e, bytes);
+    };
+    if (allow(16 / int(sizeof(T)))) backward_launch<T, 16 / int(sizeof(T))>(a, stream);
+    else if (sizeof(T) == 2 && allow(2)) backward_launch<T, sizeof(T) == 2 ? 2 : 1>(a, stream);
+    else backward_launch<T, 1>(a, stream);
     (void)launch_after(norm_weight_kernel<T>, (a.width + 31) / 32, 1024, 0, stream, static_cast<const float*>(a.partial), backward_blocks(a.rows, a.width), int(a.width),
                        static_cast<T*>(grad_weight));      // the caller asks for the last error
 }

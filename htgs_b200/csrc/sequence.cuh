@@ -91,10 +91,11 @@ template <bool CAREFUL> __device__ __forceinline__ uint32_t encode2(float lo, fl
 template <bool CAREFUL> __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inverse) {
     return encode2<CAREFUL>(a, b, inverse) | encode2<CAREFUL>(c, d, inverse) << 16;
 }
-// N codes side by side (N 1, 4 or 8).
+// N codes side by side (N 1, 2, 4 or 8).
 template <bool CAREFUL, int N> __device__ __forceinline__ void store_codes(uint8_t* to, const float (&v)[N], float inverse) {
     if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(encode4<CAREFUL>(v[0], v[1], v[2], v[3], inverse), encode4<CAREFUL>(v[4], v[5], v[6], v[7], inverse));
     else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = encode4<CAREFUL>(v[0], v[1], v[2], v[3], inverse);
+    else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(to) = uint16_t(encode2<CAREFUL>(v[0], v[1], inverse));
     else *to = uint8_t(encode2<CAREFUL>(v[0], 0.0f, inverse) & 0xffu);
 }
 // Largest magnitude; a NaN says nothing.  Infinite where one is, which is when the maximum is taken again over finite_magnitude, and CAREFUL codes follow.
