@@ -4,8 +4,11 @@
 //
 // `quantize_rows_kernel` codes a matrix as it lies; `quantize_tiles_kernel` codes it, its transpose or both from one
 // read: the two gradients of a product sum over other axes than the product, and their operands' blocks run along those.
-// Both are bound by HBM: 2 bytes read (16-bit input) and 1 written per value and orientation.
+// Both are bound by HBM: 2 bytes read (16-bit input) and 1 written per value and orientation: 100000 x 1024 in bf16 58 us as it lies (5.3 TB/s), 62 us turned (4.9 TB/s);
+// back to bf16 100000 x 512 in 34 us (4.5 TB/s).  Rows that do not begin on 16 bytes: 100000 x 511 46, 63 and 51 us, where instructions are the bound.
 #include "sequence.cuh"
+
+#include <type_traits>
 
 namespace htgs {
 
@@ -20,62 +23,99 @@ struct QuantArgs {
     uint8_t* codes_t; uint8_t* scales_t; int64_t codes_t_stride, scales_t_stride; // transposed; may be null
 };
 
-// A warp takes 32 * VEC columns, VEC side by side in a lane, but 128 at least (VEC 1, 2: in a lane several, 32 * VEC apart), of several rows, four at a
-// time, so that enough loads are on their way.
-template <typename T, int VEC>
+// Rows that begin and end on 16 bytes.  A warp takes 16 bytes a lane of several rows, four at a time, so that enough loads are on their way.
+constexpr int kTogether = 4;
+template <typename T>
 __global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const QuantArgs a) {
     const int lane = threadIdx.x & 31;
-    constexpr int kColumns = VEC < 4 ? kScaleBlock : 32 * VEC, kValues = kColumns / 32, kLanes = VEC == 8 ? 16 : 32, R = 4;
+    constexpr int VEC = 16 / int(sizeof(T)), kColumns = 32 * VEC, kLanes = kScaleBlock / VEC, R = kTogether;
     const uint32_t across = uint32_t((a.width + kColumns - 1) / kColumns), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
     const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;        // rows that are begun side by side
     if (warp >= across * down) return;
-    const int64_t first = int64_t(warp % across) * kColumns, at = first + (lane / kLanes) * kScaleBlock;
+    const int64_t column = int64_t(warp % across) * kColumns + lane * VEC;
     for (int64_t row0 = warp / across; row0 < a.rows; row0 += int64_t(down) * R) {
-        Pack<T, VEC> raw[R][kValues / VEC];          // as they are in memory: half the registers of 32-bit values
+        Pack<T, VEC> raw[R];                         // as they are in memory: half the registers of 32-bit values
         #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + int64_t(down) * r;
-            const T* x = static_cast<const T*>(a.x) + row * a.x_stride + first + lane * VEC;
-            #pragma unroll
-            for (int i = 0; i < kValues / VEC; ++i) {
-                if (row < a.rows && first + (32 * i + lane) * VEC < a.width) raw[r][i] = *reinterpret_cast<const Pack<T, VEC>*>(x + 32 * VEC * i);
-                else {
-                    #pragma unroll
-                    for (int k = 0; k < VEC; ++k) raw[r][i].v[k] = from_float<T>(0.0f);
-                }
+            if (row < a.rows && column < a.width) raw[r] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.x) + row * a.x_stride + column);
+            else {
+                #pragma unroll
+                for (int k = 0; k < VEC; ++k) raw[r].v[k] = from_float<T>(0.0f);
             }
         }
         #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + int64_t(down) * r;
             if (row >= a.rows) break;
-            uint8_t* codes = a.codes + row * a.codes_stride;
-            float v[kValues];
-            #pragma unroll
-            for (int i = 0; i < kValues / VEC; ++i) {
-                float f[VEC];
-                to_floats<T, VEC>(raw[r][i], f);
-                #pragma unroll
-                for (int k = 0; k < VEC; ++k) v[i * VEC + k] = f[k];
-            }
+            float v[VEC];
+            to_floats<T, VEC>(raw[r], v);
             float largest = largest_magnitude(v);
             const bool careful = __any_sync(0xffffffffu, largest > FLT_MAX);
             if (careful) largest = largest_finite(v);
             const int e = scale_exponent(lanes_max<kLanes>(largest));
             const float inverse = inverse_scale(e);
-            #pragma unroll
-            for (int i = 0; i < kValues / VEC; ++i) {
-                const int64_t column = first + (32 * i + lane) * VEC;
-                if (column >= a.width) continue;
-                float f[VEC];
-                #pragma unroll
-                for (int k = 0; k < VEC; ++k) f[k] = v[i * VEC + k];
-                if (careful) store_codes<true>(codes + column, f, inverse);
-                else store_codes<false>(codes + column, f, inverse);
-            }
-            if (lane % kLanes == 0 && at < a.width) a.scales[row * a.scales_stride + at / kScaleBlock] = uint8_t(e + 127);
+            if (column >= a.width) continue;
+            uint8_t* codes = a.codes + row * a.codes_stride + column;
+            if (careful) store_codes<true>(codes, v, inverse);
+            else store_codes<false>(codes, v, inverse);
+            if (lane % kLanes == 0) a.scales[row * a.scales_stride + column / kScaleBlock] = uint8_t(e + 127);
         }
     }
+}
+
+// Rows that begin anywhere, of any width, through shared memory: a warp takes 256 columns of a row while those of the next rows are on their way; a lane has every 32nd
+// column.  Addresses go from row to row by one addition.
+constexpr int kStretch = 256, kOnTheWay = 3;
+template <typename T> constexpr int kStretchSlot = kStretch * int(sizeof(T)) + 16;         // bytes
+template <typename T>
+__global__ void __launch_bounds__(kQuantBlock, 6) quantize_anywhere_kernel(const QuantArgs a) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    constexpr int kSlot = kStretchSlot<T>;
+    const int lane = threadIdx.x & 31;
+    const uint32_t across = uint32_t((a.width + kStretch - 1) / kStretch), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
+    const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;
+    if (warp >= across * down) return;
+    const int64_t first = int64_t(warp % across) * kStretch, row = warp / across;
+    const int count = int(min(int64_t(kStretch), a.width - first)), rows = int((a.rows - row + down - 1) / down);
+    const int64_t step = int64_t(down) * a.x_stride, codes_step = int64_t(down) * a.codes_stride, scales_step = int64_t(down) * a.scales_stride;
+    const T *x = static_cast<const T*>(a.x) + row * a.x_stride + first, *coming = x;
+    uint8_t *codes = a.codes + row * a.codes_stride + first + lane, *scales = a.scales + row * a.scales_stride + first / kScaleBlock;
+    unsigned char* ring = memory + (threadIdx.x >> 5) * (kOnTheWay + 1) * kSlot;
+    #pragma unroll
+    for (int i = 0; i < kOnTheWay; ++i, coming += step) {
+        if (i < rows) bring<kStretch>(ring + i * kSlot, coming, count, lane);
+        copies_begun();
+    }
+    const auto go = [&](auto whole) {               // whole: every lane has all its columns
+        for (int i = 0; i < rows; ++i, x += step, coming += step, codes += codes_step, scales += scales_step) {
+            if (i + kOnTheWay < rows) bring<kStretch>(ring + (i + kOnTheWay) % (kOnTheWay + 1) * kSlot, coming, count, lane);
+            copies_begun();
+            copies_done<kOnTheWay>();
+            const T* from = in_slot(ring + i % (kOnTheWay + 1) * kSlot, x) + lane;
+            #pragma unroll
+            for (int b = 0; b < kStretch / kScaleBlock; ++b) {
+                const int there = count - b * kScaleBlock - lane;
+                if (!whole && b * kScaleBlock >= count) break;
+                float v[4];
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = whole || 32 * j < there ? to_float<T>(from[b * kScaleBlock + 32 * j]) : 0.0f;
+                float largest = largest_magnitude(v);
+                const bool careful = __any_sync(0xffffffffu, largest > FLT_MAX);
+                if (careful) largest = largest_finite(v);
+                const int e = scale_exponent(lanes_max<32>(largest));
+                const float inverse = inverse_scale(e);
+                const uint32_t four = careful ? encode4<true>(v[0], v[1], v[2], v[3], inverse) : encode4<false>(v[0], v[1], v[2], v[3], inverse);
+                #pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (whole || 32 * j < there) codes[b * kScaleBlock + 32 * j] = uint8_t(four >> (8 * j));
+                if (lane == 0) scales[b] = uint8_t(e + 127);
+            }
+            __syncwarp();                           // the slot has been read
+        }
+    };
+    if (count == kStretch) go(std::true_type());
+    else go(std::false_type());
 }
 
 // One block per 128 x 128 values, which lie in shared memory as they came: 16 bytes at a time without passing through registers where the rows allow it (WIDE).
@@ -83,12 +123,16 @@ __global__ void __launch_bounds__(kQuantBlock, 6) quantize_rows_kernel(const Qua
 // shuffles, a column's through shared memory.  Transposed codes go through shared memory too, in the tile's place, so that they leave as rows of 128: the
 // eight bytes of half-warp h and column c lie in slot h ^ (c / 8 % 16) of the column's sixteen, which spreads the 16 lanes of a store over all
 // banks.  PER_TILE: one scale for the whole tile.
+// Rows that do not begin and end on 16 bytes come in pairs of 16-bit values, or as they lie and are moved to the beginning of their slots (in us, coded and turned, pairs
+// and slots: 50000 x 1002 fp16 51 and 55; single values and slots: 50000 x 1001 fp32 78 and 67, 80000 x 499 bf16 53 and 41).
 // (With the tile in registers, 98 a thread, two blocks were on an SM: 32768 x 1024 with its transpose in 26.6 us.)
+template <typename T, bool WIDE> constexpr int kTilePitch = kScaleBlock + (WIDE ? 0 : 16 / int(sizeof(T)));
 template <typename T, bool WIDE, bool PER_TILE>
 __global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const QuantArgs a) {
     constexpr int VEC = 16 / int(sizeof(T)), G = 8 / VEC;                 // values in 16 bytes, and of those in a thread's eight columns
     extern __shared__ __align__(16) unsigned char raw[];
-    T (*tile)[kScaleBlock] = reinterpret_cast<T (*)[kScaleBlock]>(raw);
+    constexpr int kPitch = kTilePitch<T, WIDE>;
+    T (*tile)[kPitch] = reinterpret_cast<T (*)[kPitch]>(raw);
     uint2 (*turned)[16] = reinterpret_cast<uint2 (*)[16]>(raw);
     __shared__ float column_largest[16][kScaleBlock];
     __shared__ float column_all[kScaleBlock];
@@ -105,20 +149,29 @@ __global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const Qu
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&tile[r][c])), "l"(there ? x + r * a.x_stride + c : x), "r"(there ? 16 : 0) : "memory");
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (a.x_stride * sizeof(T) % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 4 == 0 && (sizeof(T) == 4 || columns % 2 == 0)) {
-        constexpr int kTogether = 4 / int(sizeof(T)), kPieces = kScaleBlock / kTogether;
+    } else if (sizeof(T) == 2 && columns % 2 == 0 && a.x_stride % 2 == 0 && reinterpret_cast<uintptr_t>(a.x) % 4 == 0) {
         #pragma unroll 8
-        for (int i = 0; i < kScaleBlock * kPieces / kQuantBlock; ++i) {
-            const int at = i * kQuantBlock + int(threadIdx.x), r = at / kPieces, c = at % kPieces * kTogether;
+        for (int i = 0; i < kScaleBlock * kScaleBlock / 2 / kQuantBlock; ++i) {
+            const int at = i * kQuantBlock + int(threadIdx.x), r = at / (kScaleBlock / 2), c = at % (kScaleBlock / 2) * 2;
             const bool there = r < rows && c < columns;
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(&tile[r][c])), "l"(there ? x + r * a.x_stride + c : x), "r"(there ? 4 : 0) : "memory");
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-        #pragma unroll 8
-        for (int i = 0; i < kScaleBlock * kScaleBlock / kQuantBlock; ++i) {
-            const int at = i * kQuantBlock + int(threadIdx.x), r = at / kScaleBlock, c = at % kScaleBlock;
-            tile[r][c] = r < rows && c < columns ? x[r * a.x_stride + c] : from_float<T>(0.0f);
+        const int lane = threadIdx.x & 31, first = int(threadIdx.x >> 5) * 16;             // of the warp's 16 rows
+        const T zero = from_float<T>(0.0f);
+        for (int r = first; r < min(rows, first + 16); ++r) bring<kScaleBlock>(reinterpret_cast<unsigned char*>(tile[r]), x + r * a.x_stride, columns, lane);
+        copies_begun();
+        copies_done<0>();
+        #pragma unroll 4
+        for (int r = first; r < first + 16; ++r) {
+            const T* from = in_slot(reinterpret_cast<unsigned char*>(tile[r]), x + r * a.x_stride) + lane;
+            T v[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = r < rows && lane + 32 * i < columns ? from[32 * i] : zero;
+            __syncwarp();
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) tile[r][lane + 32 * i] = v[i];
         }
     }
     __syncthreads();
@@ -229,12 +282,13 @@ __global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const Qu
     }
 }
 
-// Codes back to values: exact in every output type, except that what leaves the range of 16-bit floats becomes infinite or zero.
+// Codes back to values: exact in every output type, except that what leaves the range of 16-bit floats becomes infinite or zero.  VEC values side by side in a lane, and 128
+// columns of a warp at least (VEC 1, 2: in a lane several groups, 32 * VEC apart).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kQuantBlock, 6) dequantize_kernel(const uint8_t* codes, int64_t codes_stride, const uint8_t* scales, int64_t scales_stride,
                                                                 int shift, int64_t rows, int64_t width, T* out, int64_t out_stride) {
     const int lane = threadIdx.x & 31;
-    constexpr int kColumns = VEC < 4 ? kScaleBlock : 32 * VEC, G = kColumns / 32 / VEC, R = 4;       // as in quantize_rows_kernel
+    constexpr int kColumns = VEC < 4 ? kScaleBlock : 32 * VEC, G = kColumns / 32 / VEC, R = kTogether;
     const uint32_t across = uint32_t((width + kColumns - 1) / kColumns), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
     const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;
     const int64_t column = int64_t(warp % across) * kColumns + lane * VEC;
@@ -281,21 +335,85 @@ __global__ void __launch_bounds__(kQuantBlock, 6) dequantize_kernel(const uint8_
     }
 }
 
-// Blocks for warps that take `columns` columns of four rows each: as many as the SMs hold at once, and at least one row's worth.
-unsigned int blocks_for(int64_t rows, int64_t width, int columns) {
+// The same for rows that begin anywhere, of any width, through shared memory as in quantize_anywhere_kernel.
+template <typename T> constexpr int kDecodeBytes = (kOnTheWay + 1) * (kStretch + 16) + kStretchSlot<T>;         // of a warp
+template <typename T>
+__global__ void __launch_bounds__(kQuantBlock, 6) dequantize_anywhere_kernel(const uint8_t* codes, int64_t codes_stride, const uint8_t* scales, int64_t scales_stride,
+                                                                         int shift, int64_t rows, int64_t width, T* out, int64_t out_stride) {
+    extern __shared__ __align__(16) unsigned char memory[];
+    constexpr int kSlot = kStretch + 16, kBlocks = kStretch / kScaleBlock;
+    const int lane = threadIdx.x & 31;
+    const uint32_t across = uint32_t((width + kStretch - 1) / kStretch), warp = blockIdx.x * (kQuantBlock / 32) + (threadIdx.x >> 5);
+    const uint32_t down = gridDim.x * (kQuantBlock / 32) / across;
+    grid_dependency();
+    if (warp >= across * down) return;
+    const int64_t first = int64_t(warp % across) * kStretch;
+    const int count = int(min(int64_t(kStretch), width - first)), trips = int((rows - warp / across + down - 1) / down);
+    int64_t row = warp / across;                    // that comes next
+    codes += row * codes_stride + first; out += row * out_stride + first;
+    scales += first / kScaleBlock + (lane * kScaleBlock < count ? lane : 0);
+    const int64_t step = int64_t(down) * codes_stride, out_step = int64_t(down) * out_stride;
+    unsigned char* ring = memory + (threadIdx.x >> 5) * kDecodeBytes<T>;
+    unsigned char* outs = ring + (kOnTheWay + 1) * kSlot;
+    const uint8_t* coming = codes;
+    uint32_t exponents[kOnTheWay + 1];              // lane b has block b's
+    #pragma unroll
+    for (int i = 0; i < kOnTheWay; ++i, coming += step, row += down) {
+        exponents[i] = i < trips ? scales[(row >> shift) * scales_stride] : 0u;
+        if (i < trips) bring<kStretch>(ring + i * kSlot, coming, count, lane);
+        copies_begun();
+    }
+    const auto go = [&](auto whole) {               // whole: every lane has all its columns
+        for (int i = 0; i < trips; ++i, codes += step, coming += step, out += out_step, row += down) {
+            exponents[kOnTheWay] = 0u;
+            if (i + kOnTheWay < trips) {
+                exponents[kOnTheWay] = scales[(row >> shift) * scales_stride];
+                bring<kStretch>(ring + (i + kOnTheWay) % (kOnTheWay + 1) * kSlot, coming, count, lane);
+            }
+            copies_begun();
+            copies_done<kOnTheWay>();               // what the lanes read of the row before, and of its output, lies behind them
+            const uint8_t* from = in_slot(ring + i % (kOnTheWay + 1) * kSlot, codes) + lane;
+            T* to = in_slot(outs, out) + lane;
+            #pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const float scale = scale_value(__shfl_sync(0xffffffffu, exponents[0], b));
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = b * kScaleBlock + 32 * j;
+                    if (whole || lane + c < count) to[c] = from_float<T>(decode2(from[c]).x * scale);
+                }
+            }
+            __syncwarp();
+            send<kStretch>(outs, out, count, lane);
+            #pragma unroll
+            for (int k = 0; k < kOnTheWay; ++k) exponents[k] = exponents[k + 1];
+        }
+    };
+    if (count == kStretch) go(std::true_type());
+    else go(std::false_type());
+}
+
+// Blocks for warps that take `columns` columns of four rows each: as many as the SMs hold at once (six by the kernels' registers), and at least one row's worth.
+constexpr int kSharedBytes = 227 * 1024;        // of an SM; a block takes 1 KB of them besides its own
+unsigned int blocks_for(int64_t rows, int64_t width, int columns, int per_sm = 6) {
+    if (per_sm > 6) per_sm = 6;
     const int64_t across = (width + columns - 1) / columns, per_block = kQuantBlock / 32;
     int64_t blocks = (across * ((rows + 3) / 4) + per_block - 1) / per_block;
-    if (blocks > 148 * 6) blocks = 148 * 6;
+    if (blocks > 148 * per_sm) blocks = 148 * per_sm;
     const int64_t least = (across + per_block - 1) / per_block;
     return unsigned(blocks > least ? blocks : least);
 }
 
-template <typename T, int VEC> void launch_rows(const QuantArgs& a, cudaStream_t stream) {
-    quantize_rows_kernel<T, VEC><<<blocks_for(a.rows, a.width, VEC < 4 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream>>>(a);
+template <typename T> cudaError_t quantize_anywhere(const QuantArgs& a, cudaStream_t stream) {
+    constexpr int smem = kQuantBlock / 32 * (kOnTheWay + 1) * kStretchSlot<T>;
+    static PerDeviceOnce once;
+    const cudaError_t err = once.run([] { return cudaFuncSetAttribute(quantize_anywhere_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    if (err == cudaSuccess) quantize_anywhere_kernel<T><<<blocks_for(a.rows, a.width, kStretch, kSharedBytes / (smem + 1024)), kQuantBlock, smem, stream>>>(a);
+    return err;
 }
 template <typename T, bool WIDE, bool PER_TILE> cudaError_t launch_tiles(const QuantArgs& a, cudaStream_t stream) {
     const dim3 grid(unsigned((a.width + kScaleBlock - 1) / kScaleBlock), unsigned((a.rows + kScaleBlock - 1) / kScaleBlock));
-    constexpr int smem = kScaleBlock * kScaleBlock * int(sizeof(T));
+    constexpr int smem = kScaleBlock * kTilePitch<T, WIDE> * int(sizeof(T));
     static PerDeviceOnce once;
     const cudaError_t err = once.run([] { return cudaFuncSetAttribute(quantize_tiles_kernel<T, WIDE, PER_TILE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     if (err == cudaSuccess) quantize_tiles_kernel<T, WIDE, PER_TILE><<<grid, kQuantBlock, smem, stream>>>(a);
@@ -307,25 +425,36 @@ template <typename T> int quantize_typed(const QuantArgs& a, int rows_per_scale,
     cudaError_t err = cudaSuccess;
     if (rows_per_scale != 1) err = wide ? launch_tiles<T, true, true>(a, stream) : launch_tiles<T, false, true>(a, stream);
     else if (a.codes_t) err = wide ? launch_tiles<T, true, false>(a, stream) : launch_tiles<T, false, false>(a, stream);
-    else if (wide && rows_aligned(a.codes, a.codes_stride, a.rows, 1, V)) launch_rows<T, V>(a, stream);
-    else if (sizeof(T) == 2 && a.width % 2 == 0 && rows_aligned(a.x, a.x_stride, a.rows, 2, 4) && rows_aligned(a.codes, a.codes_stride, a.rows, 1, 2))
-        launch_rows<T, sizeof(T) == 2 ? 2 : 1>(a, stream);
-    else launch_rows<T, 1>(a, stream);
+    else if (wide && rows_aligned(a.codes, a.codes_stride, a.rows, 1, V)) quantize_rows_kernel<T><<<blocks_for(a.rows, a.width, 32 * V), kQuantBlock, 0, stream>>>(a);
+    else err = quantize_anywhere<T>(a, stream);
     return err == cudaSuccess ? sequence_status("htgs_quantize_fp8") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
-template <typename T, int VEC> void launch_dequantize(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
-    (void)launch_after(dequantize_kernel<T, VEC>, blocks_for(m.rows, m.width, VEC < 4 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream, m.codes, m.codes_stride, m.scales, m.scales_stride,
-                       m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);       // the caller asks for the last error
+template <typename T, int VEC> cudaError_t launch_dequantize(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
+    return launch_after(dequantize_kernel<T, VEC>, blocks_for(m.rows, m.width, VEC < 4 ? kScaleBlock : 32 * VEC), kQuantBlock, 0, stream, m.codes, m.codes_stride, m.scales, m.scales_stride,
+                        m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);
 }
-template <typename T> void dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
-    constexpr int V = 16 / int(sizeof(T));        // 16 bytes to store: with 32 a lane every store would write half sectors
+// 16 bytes to store (with 32 a lane every store would write half sectors) or two values where every row allows it; else values of narrow matrices one by one, and those of others
+// through shared memory.  (In us, one by one and through shared memory: 200000 x 101 bf16 32 and 53, x 201 64 and 54, 50000 x 1001 fp32 85 and 53; two by two and
+// through shared memory 60000 x 650 fp16 34 and 46.)
+template <typename T> int dequantize_typed(const HtgsFp8Matrix& m, void* out, int64_t out_stride, cudaStream_t stream) {
+    constexpr int V = 16 / int(sizeof(T));
     const auto allow = [&](int values) {
         return m.width % values == 0 && rows_aligned(m.codes, m.codes_stride, m.rows, 1, values) && rows_aligned(out, out_stride, m.rows, sizeof(T), values * sizeof(T));
     };
-    if (allow(V)) launch_dequantize<T, V>(m, out, out_stride, stream);
-    else if (allow(2)) launch_dequantize<T, 2>(m, out, out_stride, stream);
-    else launch_dequantize<T, 1>(m, out, out_stride, stream);
+    cudaError_t err = cudaSuccess;
+    if (allow(V)) err = launch_dequantize<T, V>(m, out, out_stride, stream);
+    else if (allow(2)) err = launch_dequantize<T, 2>(m, out, out_stride, stream);
+    else if (m.width <= kScaleBlock) err = launch_dequantize<T, 1>(m, out, out_stride, stream);
+    else {
+        constexpr int smem = kQuantBlock / 32 * kDecodeBytes<T>;
+        static PerDeviceOnce once;
+        err = once.run([] { return cudaFuncSetAttribute(dequantize_anywhere_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+        if (err == cudaSuccess)
+            err = launch_after(dequantize_anywhere_kernel<T>, blocks_for(m.rows, m.width, kStretch, kSharedBytes / (smem + 1024)), kQuantBlock, smem, stream, m.codes, m.codes_stride, m.scales,
+                               m.scales_stride, m.rows_per_scale == 1 ? 0 : 7, m.rows, m.width, static_cast<T*>(out), out_stride);
+    }
+    return err == cudaSuccess ? sequence_status("htgs_dequantize_fp8") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
 }  // namespace
@@ -359,10 +488,9 @@ int htgs_dequantize_fp8(const HtgsFp8Matrix* matrix, void* out, int64_t out_stri
     if (matrix->rows == 0 || matrix->width == 0) return HTGS_OK;
     if (!matrix->codes || !matrix->scales || !out) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_dequantize_fp8: null pointer");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (out_type == HTGS_FLOAT32) dequantize_typed<float>(*matrix, out, out_stride, s);
-    else if (out_type == HTGS_FLOAT16) dequantize_typed<__half>(*matrix, out, out_stride, s);
-    else dequantize_typed<__nv_bfloat16>(*matrix, out, out_stride, s);
-    return sequence_status("htgs_dequantize_fp8");
+    if (out_type == HTGS_FLOAT32) return dequantize_typed<float>(*matrix, out, out_stride, s);
+    if (out_type == HTGS_FLOAT16) return dequantize_typed<__half>(*matrix, out, out_stride, s);
+    return dequantize_typed<__nv_bfloat16>(*matrix, out, out_stride, s);
 }
 
 }  // extern "C"

@@ -125,6 +125,41 @@ template <int LANES> __device__ __forceinline__ float lanes_max(float v) {
     return v;
 }
 
+// ---- stretches of a row that begin anywhere ----------------------------------------------------------------------------------------
+// Where rows do not begin on 16 bytes, a warp brings `count` values of a row into shared memory of its own, and sends some out, in the 16-byte pieces of memory that
+// they lie in.  In shared memory they lie as far behind a multiple of 16 as in memory; a slot has 16 bytes more than the values.  What a piece holds beside them is
+// copied (it lies in the same 16 bytes as a value that exists) and not looked at.
+template <typename T> __device__ __forceinline__ uint32_t misplaced(const T* p) { return uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u; }
+template <typename T> __device__ __forceinline__ T* in_slot(unsigned char* slot, const T* at) { return reinterpret_cast<T*>(slot + misplaced(at)); }
+template <int MOST, typename T> __device__ __forceinline__ void bring(unsigned char* slot, const T* from, int count, int lane) {        // at most MOST values
+    const int m = int(misplaced(from)), left = count > 0 ? m + count * int(sizeof(T)) - 16 * lane : 0;
+    const char* at = reinterpret_cast<const char*>(from) + (16 * lane - m);
+    const uint32_t to = smem_u32(slot) + 16 * lane;
+    #pragma unroll
+    for (int i = 0; i < (MOST * int(sizeof(T)) + 15 + 511) / 512; ++i)
+        if (512 * i < left) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * i), "l"(at + 512 * i) : "memory");
+}
+// Whole pieces, then the values of the first and the last one, a lane for each.
+template <int MOST, typename T> __device__ __forceinline__ void send(const unsigned char* slot, T* to, int count, int lane) {
+    constexpr int kSize = int(sizeof(T)), kValues = 16 / kSize;
+    if (count <= 0) return;
+    const int m = int(misplaced(to)), end = m + count * kSize, last = end & ~15;
+    char* at = reinterpret_cast<char*>(to) - m;
+    const bool early = 16 * lane < m;        // lane 0's first piece is not whole
+    #pragma unroll
+    for (int i = 0; i < (MOST * kSize + 15 + 511) / 512; ++i)
+        if (512 * i < last - 16 * lane && !(i == 0 && early)) *reinterpret_cast<uint4*>(at + 16 * lane + 512 * i) = *reinterpret_cast<const uint4*>(slot + 16 * lane + 512 * i);
+    const bool front = lane < kValues;
+    const int b = front ? lane * kSize : last + (lane - kValues) * kSize;
+    if (b < end && (front ? b >= m && m != 0 : lane < 2 * kValues && (last > 0 || m == 0)))
+        *reinterpret_cast<T*>(at + b) = *reinterpret_cast<const T*>(slot + b);
+}
+__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int BEGUN> __device__ __forceinline__ void copies_done() {          // all but the last BEGUN groups, for the whole warp
+    asm volatile("cp.async.wait_group %0;" ::"n"(BEGUN) : "memory");
+    __syncwarp();
+}
+
 // Blocks of a cluster: what block `block` has at this block's shared address `address`, and a barrier of all their threads.
 __device__ __forceinline__ uint32_t peer_address(uint32_t address, uint32_t block) {
     uint32_t there;

@@ -184,6 +184,60 @@ def test_quantize_is_exact(kind, rows_per_scale, rows, width):
         assert np.array_equal(f64(q.dequantize()), values, equal_nan=True)
 
 
+ANYWHERE = [("fp32", 20000, 45), ("bf16", 20000, 131), ("fp16", 6001, 250), ("fp32", 9001, 257), ("bf16", 6001, 383), ("fp16", 5001, 511), ("bf16", 4001, 514), ("fp32", 3001, 777),
+            ("bf16", 3001, 1023), ("fp16", 1501, 1111), ("fp32", 1501, 1111), ("bf16", 1201, 1999), ("fp32", 701, 2051), ("bf16", 701, 5003), ("fp16", 301, 8191)]
+
+
+@pytest.mark.parametrize("kind,rows,width", ANYWHERE)
+def test_norm_of_many_rows_that_begin_anywhere(kind, rows, width):
+    """Rows inside a matrix whose other columns are NaN, on addresses of every kind, and enough of them that a warp deals with several."""
+    import torch
+    from htgs_b200 import sequence as seq
+    def inside(seed, scale):
+        whole = torch.full((rows, width + 3), float("nan"), dtype=dtype(kind), device="cuda")
+        whole[:, 1:-2] = draw((rows, width), seed, kind, scale)
+        return whole[:, 1:-2]
+    x, r, gy, gs = inside(70, 1.0), inside(71, 0.5), inside(72, 1.0), inside(73, 1.0)
+    w = draw((width + 1,), 74, kind, 0.2, 1.0)[1:]
+    y64, u64, rho = ref.norm(f64(x), f64(w), f64(r), 1e-6)
+    y_bound, s_bound = norm_bounds(y64, u64, kind, width)
+    x, r, w = (t.detach().requires_grad_(True) for t in (x, r, w))
+    y, s = seq.add_rms_norm(x, w, r)
+    near(y, y64, y_bound, "y")
+    near(s, u64, s_bound, "stream")
+    gx, gr, gw = torch.autograd.grad((y, s), (x, r, w), (gy, gs))
+    gx64, gw64 = ref.norm_backward(f64(gy), f64(gs), u64, rho, f64(w))
+    unit, z = np.abs(u64 * rho), np.abs(f64(gy) * f64(w))
+    bound = U[kind] * np.abs(gx64) + (U[kind] + (2 * width + 16) * F) * (rho * (z + 2 * unit * np.mean(z * unit, axis=1, keepdims=True)) + np.abs(f64(gs))) + TINY[kind]
+    near(gx, gx64, bound, "grad_x")
+    near(gw, gw64, U[kind] * np.abs(gw64) + (U[kind] + (rows + width + 8) * F) * np.sum(np.abs(f64(gy)) * unit, axis=0) + TINY[kind], "grad_weight")
+    with torch.no_grad():
+        q, s8 = seq.add_rms_norm_fp8(x, w, r)
+        scale = np.exp2(q.scales.view(torch.uint8).cpu().numpy().astype(np.float64) - 127).repeat(128, 1)[:, :width]
+        near(q.dequantize(torch.float32), y64, np.maximum(np.abs(y64) * 2.0 ** -4, scale * 2.0 ** -10) + (width + 16) * F * np.abs(y64), "values")
+        assert torch.equal(s8, s)
+
+
+@pytest.mark.parametrize("kind,rows,width", ANYWHERE)
+def test_quantize_many_rows_that_begin_anywhere(kind, rows, width):
+    import torch
+    from htgs_b200 import sequence as seq
+    whole = torch.full((rows, width + 3), float("inf"), dtype=dtype(kind), device="cuda")
+    whole[:, 1:-2] = draw((rows, width), 75, kind)
+    x = whole[:, 1:-2]
+    x[:, :5] *= 64
+    x[rows // 2, width // 2], x[rows // 3, width - 1] = float("nan"), float("inf")
+    for transpose in (False, True):
+        q = seq.quantize_fp8(x, 1, transpose)
+        codes, exponents = codes_of(q)
+        want = ref.quantize(f64(x).T.copy() if transpose else f64(x))
+        assert np.array_equal(exponents, want[1]) and np.array_equal(codes, want[0], equal_nan=True)
+    q = seq.quantize_fp8(x)
+    values = ref.dequantize(*ref.quantize(f64(x)))
+    assert np.array_equal(f64(q.dequantize()), values, equal_nan=True)
+    assert np.array_equal(f64(q.dequantize(torch.float32)), values, equal_nan=True)
+
+
 def test_quantize_at_the_ends_of_the_range():
     import torch
     from htgs_b200 import sequence as seq
