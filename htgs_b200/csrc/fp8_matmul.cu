@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) matmul_tiles_kernel(const __g
             if (SPLIT) {
                 #pragma unroll
                 for (int j = 0; j < kLoads; ++j) shared[turn][4 * j + warp - 4][lane] = next[j];
+                __syncwarp();                // the barrier is of whole warps
                 asm volatile("bar.sync 1, 128;" ::: "memory");    // one per trip: the other buffer is written before the next one
                 #pragma unroll
                 for (int i = 0; i < 12; ++i) words[i] = shared[turn][i][lane];
@@ -487,6 +488,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) matmul_tiles_kernel(const __g
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) tma_store(&map_out, column0 + c, row0, patch);
+                    __syncwarp();            // the next columns are read by the whole warp (.aligned)
                 } else {                     // rows that begin anywhere: a row's 32 values by the 32 lanes
                     __syncwarp();
                     const int column = column0 + c + lane, rows = min(kPatch, args.rows_a - row0);

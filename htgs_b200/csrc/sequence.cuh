@@ -160,7 +160,8 @@ template <int BEGUN> __device__ __forceinline__ void copies_done() {          //
     __syncwarp();
 }
 
-// Blocks of a cluster: what block `block` has at this block's shared address `address`, and a barrier of all their threads.
+// Blocks of a cluster: what block `block` has at this block's shared address `address`, and a barrier of all their threads.  The barrier's instructions are
+// of whole warps (.aligned), which have to come back together first if they stand behind a branch or a loop that some lanes took.
 __device__ __forceinline__ uint32_t peer_address(uint32_t address, uint32_t block) {
     uint32_t there;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(block));
@@ -177,6 +178,7 @@ __device__ __forceinline__ float4 peer_float4(uint32_t address, uint32_t block) 
     return v;
 }
 __device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
