@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArg
     const int64_t n = int64_t(blockIdx.x) * (kRowsBlock / 32) + warp, m0 = int64_t(blockIdx.y) * ROWS, width = args.a.width;
     const int across = int((width + kScaleBlock - 1) / kScaleBlock);
     const int pitch = across * kScaleBlock;
-    float* factors = reinterpret_cast<float*>(coded + args.a.rows * pitch);       // with VALUES all rows of a are the block's
+    uint8_t* exponents = coded + args.a.rows * pitch;                            // with VALUES all rows of a are the block's
     grid_dependency();
     if (VALUES) {
         for (int unit = warp; unit < int(args.a.rows) * across; unit += kRowsBlock / 32) {
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArg
             const int e = scale_exponent(lanes_max<32>(largest_finite(v)));
             #pragma unroll
             for (int i = 0; i < 4; ++i) coded[row * pitch + block * kScaleBlock + lane + 32 * i] = uint8_t(encode2<true>(v[i], 0.0f, inverse_scale(e)) & 0xffu);
-            if (lane == 0) factors[row * across + block] = scale_value(uint32_t(e + 127));
+            if (lane == 0) exponents[row * across + block] = uint8_t(e + 127);
         }
         __syncthreads();
     }
@@ -72,20 +72,20 @@ __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArg
         float2 vb[8];
         #pragma unroll
         for (int w = 0; w < 4; ++w) { vb[2 * w] = decode2(words[w]); vb[2 * w + 1] = decode2(words[w] >> 16); }
-        const float scale_b = scale_value(sb[k / kScaleBlock]);
+        const uint32_t scale_b = sb[k / kScaleBlock];
         #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const int64_t m = m0 + r;
             if (m >= args.a.rows) break;
             uint32_t wa[4];
-            float scale_a;
+            uint32_t scale_a;
             if (VALUES) {
                 const uint4 packed = *reinterpret_cast<const uint4*>(coded + r * pitch + k);
                 wa[0] = packed.x; wa[1] = packed.y; wa[2] = packed.z; wa[3] = packed.w;
-                scale_a = factors[r * across + k / kScaleBlock];
+                scale_a = exponents[r * across + k / kScaleBlock];
             } else {
                 load_codes(args.a.codes + m * args.a.codes_stride, k, width, wa);
-                scale_a = scale_value(args.a.scales[m / args.a.rows_per_scale * args.a.scales_stride + k / kScaleBlock]);
+                scale_a = args.a.scales[m / args.a.rows_per_scale * args.a.scales_stride + k / kScaleBlock];
             }
             float sum = 0.0f;
             #pragma unroll
@@ -96,7 +96,8 @@ __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArg
                 sum = fmaf(hi.x, vb[2 * w + 1].x, sum);
                 sum = fmaf(hi.y, vb[2 * w + 1].y, sum);
             }
-            acc[r] = fmaf(sum * scale_a, scale_b, acc[r]);
+            const float2 factors = scale_factors(scale_a, scale_b);
+            acc[r] = fmaf(sum * factors.x, factors.y, acc[r]);
         }
     }
     #pragma unroll
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kRowsBlock) matmul_rows_kernel(const MatmulArg
 
 template <typename T, int ROWS, typename X, bool VALUES> int launch_rows(const MatmulArgs& args, const ValuesArgs& values, cudaStream_t stream) {
     const int across = int((args.a.width + kScaleBlock - 1) / kScaleBlock);
-    const size_t smem = VALUES ? size_t(args.a.rows) * across * (kScaleBlock + sizeof(float)) : 0;
+    const size_t smem = VALUES ? size_t(args.a.rows) * across * (kScaleBlock + 1) : 0;
     const dim3 grid(unsigned((args.b.rows + kRowsBlock / 32 - 1) / (kRowsBlock / 32)), unsigned((args.a.rows + ROWS - 1) / ROWS));
     const cudaError_t err = launch_after(matmul_rows_kernel<T, ROWS, X, VALUES>, grid, kRowsBlock, smem, stream, args, values);
     return err == cudaSuccess ? sequence_status("htgs_fp8_matmul") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));

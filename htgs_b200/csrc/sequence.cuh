@@ -79,6 +79,12 @@ __device__ __forceinline__ float inverse_scale(int e) { return __uint_as_float(u
 __device__ __forceinline__ float scale_value(uint32_t byte) {                                                     // 2^(byte - 127); 255 is NaN
     return byte == 255u ? __uint_as_float(0x7fffffffu) : byte == 0u ? __uint_as_float(0x400000u) : __uint_as_float(byte << 23);
 }
+// Two factors whose product is that of two scales: the exponents are added first, so that a sum of codes times one factor and then the other leaves the range of
+// 32 bits only where the result does.  (One scale by itself may be up to 2^127, and a sum of 16 products of codes up to 2^22.)
+__device__ __forceinline__ float2 scale_factors(uint32_t a, uint32_t b) {
+    const uint32_t half = (a + b) >> 1;
+    return a == 255u || b == 255u ? make_float2(scale_value(255u), scale_value(255u)) : make_float2(scale_value(half), scale_value(a + b - half));
+}
 
 // Codes v * 2^-e to the nearest E4M3 value, ties to even; NaN becomes NaN.  CAREFUL: infinities do too (the conversion takes them for 448).
 template <bool CAREFUL> __device__ __forceinline__ uint32_t encode2(float lo, float hi, float inverse) {

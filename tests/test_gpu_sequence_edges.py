@@ -1,0 +1,36 @@
+"""GPU: the sequence operators at the ends of their range, and what autograd knows of them.  (Tolerances as in test_gpu_sequence.py.)"""
+import numpy as np
+import pytest
+
+import sequence_reference as ref
+from test_gpu_sequence import binding, draw, f64, near, product_bound  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,out,width", [(1, 40, 128), (3, 33, 300), (8, 65, 1000), (300, 136, 260)])
+@pytest.mark.parametrize("size_x,size_w", [(1e36, 1e-2), (1e30, 1e-30), (3e37, 1e-25), (1e-37, 1e30), (1e-30, 1e36), (1e-10, 1e-25)])
+def test_product_of_large_and_small_values(kind, rows, out, width, size_x, size_w):
+    """Scales whose product is in range although one of them, times a sum of codes, is not."""
+    import torch
+    from htgs_b200 import sequence as seq
+    x, w = draw((rows, width), 3, kind, size_x / 8), draw((out, width), 4, kind, size_w)
+    a, b = ref.dequantize(*ref.quantize(f64(x))), ref.dequantize(*ref.quantize(f64(w), 128), 128)
+    assert np.isfinite(f64(x)).all() and np.abs(a @ b.T).max() < 1e38
+    q = seq.quantize_fp8(w, 128)
+    near(seq.fp8_matmul(x, q), *product_bound(a, b, kind), "values")
+    near(seq.fp8_matmul(seq.quantize_fp8(x), q, torch.float32), *product_bound(a, b, "fp32"), "codes")
+
+
+def test_product_with_scales_that_are_nan():
+    import torch
+    from htgs_b200 import sequence as seq
+    x, w = draw((4, 300), 1), draw((9, 300), 2)
+    q = seq.quantize_fp8(w, 1)
+    q.scales.view(torch.uint8)[3, 1] = 255
+    want = torch.zeros(4, 9, dtype=torch.bool, device="cuda")
+    want[:, 3] = True
+    for rows in (1, 4):
+        assert torch.equal(torch.isnan(seq.fp8_matmul(x[:rows], q)), want[:rows])
+        assert torch.equal(torch.isnan(seq.fp8_matmul(seq.quantize_fp8(x[:rows]), q)), want[:rows])
