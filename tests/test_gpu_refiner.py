@@ -78,3 +78,18 @@ def test_packed_scenes_do_not_see_one_another():
     for name, _ in PARAMETERS:
         assert torch.equal(first[name][:700], second[name][:700]), name
     assert not torch.equal(first["positions"][700:], second["positions"][700:])
+
+
+def test_packed_scenes_are_refined_as_each_alone_wherever_the_others_lie():
+    import torch
+    from htgs_b200.refiner import PARAMETERS, GaussianRefiner
+    torch.manual_seed(3)
+    (_, one, _), (_, two, _) = raw_scene(700, seed=3), raw_scene(901, seed=4)
+    model = GaussianRefiner(64, 2, step=1.0).cuda().freeze()
+    offsets = torch.tensor([0, 700, 1601], dtype=torch.int32, device="cuda")
+    results = []
+    for factor in (1.0, 1000.0):
+        both = {name: torch.cat([one[name], two[name] * (factor if name == "positions" else 1.0)]) for name, _ in PARAMETERS}
+        results.append(model.infer(both, offsets))
+    for name, _ in PARAMETERS:
+        assert torch.equal(results[0][name][:700], results[1][name][:700]), name

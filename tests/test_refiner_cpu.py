@@ -33,3 +33,20 @@ def test_order_of_equal_and_of_no_positions():
 def test_infer_needs_coded_weights():
     with pytest.raises(RuntimeError):
         refiner.GaussianRefiner(32, 1).infer({})
+
+
+def separate_orders(parts):
+    """The orders that scenes get alone, one behind the other."""
+    begin, orders = 0, []
+    for p in parts:
+        orders.append(refiner.curve_order(p) + begin)
+        begin += p.shape[0]
+    return torch.cat(orders)
+
+
+def test_curve_order_of_packed_scenes_is_that_of_each_alone():
+    g = torch.Generator().manual_seed(3)
+    parts = [torch.rand((500, 3), generator=g), torch.rand((300, 3), generator=g) * 5000.0 - 1000.0, torch.empty(0, 3), torch.rand((1, 3), generator=g) * 1e-6,
+             torch.rand((200, 3), generator=g) * torch.tensor([1e-3, 1.0, 1e4])]
+    offsets = torch.tensor([0, 500, 800, 800, 801, 1001], dtype=torch.int32)
+    assert torch.equal(refiner.curve_order(torch.cat(parts), offsets), separate_orders(parts))
