@@ -24,16 +24,18 @@ CHANNELS = sum(width for _, width in PARAMETERS)
 
 
 def curve_order(positions: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Indices that sort Gaussians along the Morton curve through 2^10 cells a side of their bounding box.  With the `offsets` at which packed scenes begin, each scene
+    """Indices that sort Gaussians along the Morton curve through 2^10 cells a side of the bounding box of their finite positions (others lie at its faces).  With the `offsets` at which packed scenes begin, each scene
     has its own box and its own curve: it gets the order that it has alone."""
     if positions.shape[0] == 0:
         return torch.empty(0, dtype=torch.long, device=positions.device)
+    finite = positions.isfinite()
+    least, most = positions.masked_fill(~finite, float("inf")), positions.masked_fill(~finite, float("-inf"))
     if offsets is None:
-        low, high = positions.amin(dim=0), positions.amax(dim=0)
+        low, high = least.amin(dim=0), most.amax(dim=0)
     else:
         scene = torch.bucketize(torch.arange(positions.shape[0], device=positions.device), offsets[1:-1].long(), right=True)
         box = [torch.zeros((offsets.numel() - 1, 3), dtype=positions.dtype, device=positions.device).scatter_reduce_(
-            0, scene[:, None].expand(-1, 3), positions, reduce, include_self=False) for reduce in ("amin", "amax")]
+            0, scene[:, None].expand(-1, 3), ends, reduce, include_self=False) for ends, reduce in ((least, "amin"), (most, "amax"))]
         low, high = box[0][scene], box[1][scene]
     cell = ((positions - low) / (high - low).clamp(min=1e-12) * 1023.0).nan_to_num().clamp(0, 1023).long()
     code = torch.zeros(positions.shape[0], dtype=torch.long, device=positions.device)

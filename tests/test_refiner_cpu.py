@@ -50,3 +50,19 @@ def test_curve_order_of_packed_scenes_is_that_of_each_alone():
              torch.rand((200, 3), generator=g) * torch.tensor([1e-3, 1.0, 1e4])]
     offsets = torch.tensor([0, 500, 800, 800, 801, 1001], dtype=torch.int32)
     assert torch.equal(refiner.curve_order(torch.cat(parts), offsets), separate_orders(parts))
+
+
+def test_positions_that_are_not_finite_leave_the_others_in_order():
+    g = torch.Generator().manual_seed(4)
+    positions = torch.rand((400, 3), generator=g)
+    alone = refiner.curve_order(positions)
+    for value in (float("nan"), float("inf"), float("-inf")):
+        for axis in range(3):
+            odd = torch.cat((positions, torch.full((1, 3), 0.5)))
+            odd[400, axis] = value
+            order = refiner.curve_order(odd)
+            assert torch.equal(order[order != 400], alone)
+    nothing = torch.full((3, 3), float("nan"))
+    assert torch.equal(refiner.curve_order(nothing), torch.arange(3))
+    parts = [positions, odd]
+    assert torch.equal(refiner.curve_order(torch.cat(parts), torch.tensor([0, 400, 801], dtype=torch.int32)), separate_orders(parts))
