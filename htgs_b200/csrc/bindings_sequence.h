@@ -28,6 +28,11 @@ void check_like(const Tensor& t, const char* name, c10::ScalarType type, const c
 }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
+// A tangent would be dropped without a word: a dual tensor need not want a gradient.
+void no_tangent(const Tensor& t) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "the sequence operators have no forward-mode derivative: unpack dual tensors first");
+}
+void no_tangent(const OptTensor& t) { if (t) no_tangent(*t); }
 
 // `t` as a matrix of its last dimension's rows; a copy only where its rows are not evenly spaced or not dense.
 Tensor rows_of(const Tensor& t) {
@@ -66,6 +71,7 @@ void check_norm(const Tensor& x, const Tensor& weight, const OptTensor& residual
         check_like(*residual, "residual", x.scalar_type(), x.device());
         TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), "residual must have the shape of x, ", x.sizes(), ", got ", residual->sizes());
     }
+    no_tangent(x); no_tangent(weight); no_tangent(residual);
 }
 
 // y or codes and scales; sum where there is a residual.
@@ -222,6 +228,7 @@ Tensor fp8_matmul(const Tensor& x, const OptTensor& x_scales, int64_t x_rows_per
     check_value(x, "x");
     TORCH_CHECK_VALUE(x.device() == codes.device(), "x is on ", x.device(), ", expected ", codes.device());
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == width, "x must have a last dimension of ", width, " values");
+    no_tangent(x);
     TORCH_CHECK(!(c10::GradMode::is_enabled() && x.requires_grad()), "fp8_matmul has no gradient: use fp8_linear in training, or torch.no_grad()");
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor xm = rows_of(x);
@@ -284,6 +291,7 @@ Tensor fp8_linear(const Tensor& x, const Tensor& weight) {
     check_value(x, "x");
     check_like(weight, "weight", x.scalar_type(), x.device());
     TORCH_CHECK_VALUE(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1), "weight must have shape (out, width), and x a last dimension of width values");
+    no_tangent(x); no_tangent(weight);
     const bool grad = c10::GradMode::is_enabled(), need_x = grad && x.requires_grad(), need_weight = grad && weight.requires_grad();
     if (need_x || need_weight) return Fp8Linear::apply(x, weight, need_x, need_weight);
     const c10::cuda::CUDAGuard guard(x.device());
@@ -367,6 +375,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const
         TORCH_CHECK_VALUE(initial->dim() == 2 && initial->size(0) == sequences && initial->size(1) == width, "initial must have shape (", sequences, ", ", width, "), got ",
                           initial->sizes());
     }
+    no_tangent(x); no_tangent(gate); no_tangent(initial);
     if (sequences == 0) return {torch::empty_like(x), floats(x, {0, width})};
     const Tensor start = initial ? *initial : Tensor();
     if (c10::GradMode::is_enabled() && (wants_grad(x) || wants_grad(gate) || wants_grad(start))) {
@@ -386,6 +395,7 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state)
     TORCH_CHECK_VALUE(x.dim() == 2 && gate.sizes() == x.sizes() && state.sizes() == x.sizes() && x.size(1) >= 1, "x, gate and state must have one shape, [rows, width]");
     TORCH_CHECK_VALUE((state.stride(1) == 1 || state.size(1) == 1) && (state.size(0) <= 1 || state.stride(0) >= state.size(1)),
                       "state must have dense rows: it is updated in place");
+    no_tangent(x); no_tangent(gate); no_tangent(state);
     TORCH_CHECK(!(c10::GradMode::is_enabled() && (wants_grad(x) || wants_grad(gate) || wants_grad(state))),
                 "gated_scan_step has no gradient: use gated_scan in training, or torch.no_grad()");
     const c10::cuda::CUDAGuard guard(x.device());

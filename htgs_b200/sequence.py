@@ -7,7 +7,8 @@ each Gaussian in the order of a space-filling curve, 10^5 to 10^6 rows long.
 * `gated_scan`, `gated_scan_step`      - gated linear recurrence over whole sequences (differentiable), and one step of it
 
 Values are float32, float16 or bfloat16; sums, statistics and states are 32-bit.  Everything is queued on the current CUDA stream without a
-host wait, can be captured in a CUDA graph, and gives the same bits for the same inputs.  There is no CPU fallback.  (No counterpart in the reference.)
+host wait, can be captured in a CUDA graph, and gives the same bits for the same inputs.  There is no CPU fallback.  Derivatives
+are reverse-mode: dual tensors of forward-mode differentiation are refused.  (No counterpart in the reference.)
 """
 from __future__ import annotations
 
@@ -69,6 +70,12 @@ def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _no_tangent(*tensors) -> None:
+    """A tangent would be dropped without a word: a dual tensor need not want a gradient."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the sequence operators have no forward-mode derivative: unpack dual tensors first")
+
+
 # ---- norm ------------------------------------------------------------------------------------------------------------------
 
 
@@ -83,6 +90,7 @@ def _check_norm(x, weight, residual):
         _check(residual, "residual", x.dtype, x.device)
         if residual.shape != x.shape:
             raise ValueError(f"residual must have the shape of x, {tuple(x.shape)}, got {tuple(residual.shape)}")
+    _no_tangent(x, weight, residual)
 
 
 def _norm_forward(x, weight, residual, eps, with_rstd, to_codes):
@@ -294,6 +302,7 @@ def fp8_matmul(x, weight: Fp8Matrix, dtype: Optional[torch.dtype] = None) -> tor
     _check(x, "x", None, weight.device)
     if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x must have a last dimension of {weight.shape[1]} values")
+    _no_tangent(x)
     if _wants_grad(x):
         raise RuntimeError("fp8_matmul has no gradient: use fp8_linear in training, or torch.no_grad()")
     xm, dtype = _rows(x), dtype or x.dtype
@@ -338,6 +347,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     _check(weight, "weight", x.dtype, x.device)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError("weight must have shape (out, width), and x a last dimension of width values")
+    _no_tangent(x, weight)
     if _wants_grad(x, weight):
         return _Fp8Linear.apply(x, weight)
     return fp8_matmul(x, quantize_fp8(weight, _BLOCK))
@@ -429,6 +439,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, initial: Optional[torch.Tens
         _check(initial, "initial", torch.float32, x.device)
         if tuple(initial.shape) != (sequences, x.shape[-1]):
             raise ValueError(f"initial must have shape {(sequences, x.shape[-1])}, got {tuple(initial.shape)}")
+    _no_tangent(x, gate, initial)
     shape = x.shape
     if sequences == 0:
         return torch.empty_like(x), torch.empty((0, shape[-1]), dtype=torch.float32, device=x.device)
@@ -453,6 +464,7 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) ->
         raise ValueError("x, gate and state must have one shape, [rows, width]")
     if state.stride(1) != 1 and state.shape[1] != 1 or state.shape[0] > 1 and state.stride(0) < state.shape[1]:
         raise ValueError("state must have dense rows: it is updated in place")
+    _no_tangent(x, gate, state)
     if _wants_grad(x, gate, state):
         raise RuntimeError("gated_scan_step has no gradient: use gated_scan in training, or torch.no_grad()")
     xm, gm = _rows(x), _rows(gate)

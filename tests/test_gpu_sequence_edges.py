@@ -34,3 +34,24 @@ def test_product_with_scales_that_are_nan():
     for rows in (1, 4):
         assert torch.equal(torch.isnan(seq.fp8_matmul(x[:rows], q)), want[:rows])
         assert torch.equal(torch.isnan(seq.fp8_matmul(seq.quantize_fp8(x[:rows]), q)), want[:rows])
+
+
+def test_forward_mode_derivatives_are_refused():
+    """No operator has one, and none drops a tangent without a word."""
+    import torch
+    import torch.autograd.forward_ad as fw
+    from htgs_b200 import sequence as seq
+    x, w, r, square = draw((4, 64), 1), draw((64,), 2), draw((4, 64), 3), draw((64, 64), 4)
+    initial, q = draw((1, 64), 5), seq.quantize_fp8(draw((64, 64), 4), 128)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: seq.add_rms_norm(dual(x), w, r), lambda: seq.add_rms_norm(x, dual(w)), lambda: seq.add_rms_norm(x, w, dual(r)),
+                     lambda: seq.add_rms_norm_fp8(dual(x), w), lambda: seq.fp8_matmul(dual(x), q), lambda: seq.fp8_linear(dual(x), square), lambda: seq.fp8_linear(x, dual(square)),
+                     lambda: seq.gated_scan(dual(x), r), lambda: seq.gated_scan(x, dual(r)), lambda: seq.gated_scan(x, r, dual(initial)),
+                     lambda: seq.gated_scan_step(dual(x), r, torch.zeros_like(x)), lambda: seq.gated_scan_step(x, r, dual(torch.zeros_like(x)))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        seq.add_rms_norm(x, w, r)
+    seq.add_rms_norm(x, w, r)
