@@ -403,6 +403,7 @@ Tensor gated_scan_step(const Tensor& x, const Tensor& gate, const Tensor& state)
     Tensor h = make(x, x.sizes());
     check(htgs_gated_scan_step(xm.data_ptr(), xm.stride(0), gm.data_ptr(), gm.stride(0), state.data_ptr<float>(), state.stride(0), h.data_ptr(), x.size(1),
                                type_of(x.scalar_type()), x.size(0), int32_t(x.size(1)), stream_of(x)));
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();       // autograd learns of it; what inference mode made is kept by no gradient
     return h;
 }
 

@@ -471,4 +471,6 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) ->
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     _call(x.device, "htgs_gated_scan_step", xm.data_ptr(), xm.stride(0), gm.data_ptr(), gm.stride(0), state.data_ptr(), state.stride(0), h.data_ptr(),
           x.shape[1], _TYPES[x.dtype], x.shape[0], x.shape[1])
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)        # autograd learns of it; what inference mode made is kept by no gradient
     return h

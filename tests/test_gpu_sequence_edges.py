@@ -55,3 +55,21 @@ def test_forward_mode_derivatives_are_refused():
                 call()
         seq.add_rms_norm(x, w, r)
     seq.add_rms_norm(x, w, r)
+
+
+def test_step_tells_autograd_of_its_state():
+    """A state that another operator keeps for its gradient: the step overwrites it, and that gradient is refused."""
+    import torch
+    from htgs_b200 import sequence as seq
+    x, g, state = draw((3, 16), 1), draw((3, 16), 2), draw((3, 20), 3)[:, :16]
+    factor = draw((3, 16), 4).requires_grad_(True)
+    y = (factor * state).sum()
+    before = state._version
+    seq.gated_scan_step(x, g, state)
+    assert state._version == before + 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        inner = torch.zeros(3, 16, device="cuda")
+        seq.gated_scan_step(x, g, inner)
+    seq.gated_scan_step(x, g, inner)                       # nothing can have kept it
