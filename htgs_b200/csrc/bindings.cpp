@@ -19,6 +19,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/engine.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 
 #include <atomic>

@@ -56,8 +56,18 @@ Tensor make(const Tensor& like, at::IntArrayRef sizes, c10::ScalarType type) { r
 Tensor make(const Tensor& like, at::IntArrayRef sizes) { return make(like, sizes, like.scalar_type()); }
 Tensor bytes(const Tensor& like, size_t count) { return make(like, {int64_t(count)}, torch::kByte); }
 Tensor floats(const Tensor& like, at::IntArrayRef sizes) { return make(like, sizes, torch::kFloat32); }
-void no_second_derivative() {
-    TORCH_CHECK(!c10::GradMode::is_enabled(), "the sequence operators have no second derivative: create_graph must be false");
+// Runs a backward pass.  Where its graph is created, the gradients hang on a node that raises: a second derivative is an error where one is taken, and only there.
+template <typename F> variable_list first_derivative(F&& backward) {
+    variable_list grads;
+    {
+        const c10::AutoGradMode off(false);
+        grads = backward();
+    }
+    if (!c10::GradMode::is_enabled()) return grads;
+    for (Tensor& grad : grads)
+        if (grad.defined()) grad = grad.detach().set_requires_grad(true);
+    const auto refusal = std::make_shared<torch::autograd::DelayedError>("the sequence operators have no second derivative", int64_t(grads.size()));
+    return (*refusal)(std::move(grads));
 }
 
 // ---- norm ---------------------------------------------------------------------------------------------------------------------
@@ -97,7 +107,9 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
         return residual.defined() ? variable_list{y, sum} : variable_list{y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        no_second_derivative();
+        return first_derivative([&] { return first_backward(ctx, grads); });
+    }
+    static variable_list first_backward(AutogradContext* ctx, const variable_list& grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &residual = saved[2], &rstd = saved[3];
         const Tensor grad_sum = grads.size() > 1 ? grads[1] : Tensor();
@@ -263,7 +275,9 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        no_second_derivative();
+        return first_derivative([&] { return first_backward(ctx, grads); });
+    }
+    static variable_list first_backward(AutogradContext* ctx, const variable_list& grads) {
         const auto saved = ctx->get_saved_variables();
         const Matrix xt{saved[0], saved[1], 1}, wt{saved[2], saved[3], kBlock};
         const Tensor gm = rows_of(grads[0]);
@@ -338,7 +352,9 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
         return {h, last};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        no_second_derivative();
+        return first_derivative([&] { return first_backward(ctx, grads); });
+    }
+    static variable_list first_backward(AutogradContext* ctx, const variable_list& grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &gate = saved[1], &initial = saved[2], &offsets = saved[3], &states = saved[4];
         const auto sizes = ctx->saved_data["sizes"].toIntVector();

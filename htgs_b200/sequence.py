@@ -13,6 +13,7 @@ are reverse-mode: dual tensors of forward-mode differentiation are refused.  (No
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -76,6 +77,30 @@ def _no_tangent(*tensors) -> None:
         raise RuntimeError("the sequence operators have no forward-mode derivative: unpack dual tensors first")
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the sequence operators have no second derivative")
+
+
+def _first_derivative(backward):
+    """A backward pass whose gradients, where its graph is created, hang on a node that raises: a second derivative is an error where one is taken,
+    and only there."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        marked = iter(_NoSecondDerivative.apply(*(g.detach().requires_grad_() for g in out if g is not None)))
+        return tuple(None if g is None else next(marked) for g in out)
+    return run
+
+
 # ---- norm ------------------------------------------------------------------------------------------------------------------
 
 
@@ -123,7 +148,7 @@ class _AddRmsNorm(torch.autograd.Function):
         return (y.view(x.shape), total.view(x.shape)) if residual is not None else y.view(x.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, grad_y, grad_sum=None):
         x, residual, weight, rstd = ctx.saved_tensors
         if grad_y is None:
@@ -327,7 +352,7 @@ class _Fp8Linear(torch.autograd.Function):
         return _matmul(xq, wq, x.dtype).view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, grad_y):
         xt, wt = ctx.kept
         need_x, need_weight = ctx.needs_input_grad
@@ -392,7 +417,7 @@ class _GatedScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, grad_h, grad_last):
         x, gate, initial, offsets, states = ctx.saved_tensors
         sequences, reverse = ctx.rest

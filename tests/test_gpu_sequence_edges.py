@@ -73,3 +73,29 @@ def test_step_tells_autograd_of_its_state():
         inner = torch.zeros(3, 16, device="cuda")
         seq.gated_scan_step(x, g, inner)
     seq.gated_scan_step(x, g, inner)                       # nothing can have kept it
+
+
+def operators_with_gradients():
+    from htgs_b200 import sequence as seq
+    x, other, vector, square = draw((5, 32), 1), draw((5, 32), 2), draw((32,), 3), draw((32, 32), 4)
+    return {"norm": (lambda v: seq.add_rms_norm(v, vector, other)[0], x), "norm's weight": (lambda v: seq.add_rms_norm(x, v)[0], vector),
+            "linear": (lambda v: seq.fp8_linear(v, square), x), "linear's weight": (lambda v: seq.fp8_linear(x, v), square),
+            "scan": (lambda v: seq.gated_scan(v, other)[0], x), "gate": (lambda v: seq.gated_scan(x, v)[0], other)}
+
+
+def test_first_derivatives_with_a_graph_and_no_second_ones():
+    """create_graph=True is no error by itself.  A second derivative is one, also where the first one's gradient wants none itself: it is not left out of a sum."""
+    import torch
+    for name, (f, leaf) in operators_with_gradients().items():
+        v = leaf.clone().requires_grad_(True)
+        want, = torch.autograd.grad(f(v).square().sum(), v)
+        y = f(v)
+        got, = torch.autograd.grad(y.square().sum(), v, create_graph=True)
+        assert torch.equal(got, want), name
+        with pytest.raises(RuntimeError, match="second derivative"):
+            got.sum().backward()
+        assert v.grad is None or torch.equal(v.grad, torch.zeros_like(v))
+        y = f(v)
+        got, = torch.autograd.grad(y.sum(), v, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (y.square().sum() + got.square().sum()).backward()
