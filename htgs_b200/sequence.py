@@ -347,15 +347,16 @@ class _Fp8Linear(torch.autograd.Function):
         xm, wm = _rows(x), _rows(weight)
         xq, xt = _quantize(xm, 1, True, need_weight)          # the gradients sum over other axes, so their blocks run along those
         wq, wt = _quantize(wm, _BLOCK, True, need_x)
-        ctx.kept = (xt, wt)
+        ctx.save_for_backward(*(t for m in (xt, wt) for t in ((None, None) if m is None else (m.codes, m.scales))))
         ctx.types = (x.dtype, weight.dtype)
         return _matmul(xq, wq, x.dtype).view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @_first_derivative
     def backward(ctx, grad_y):
-        xt, wt = ctx.kept
+        x_codes, x_scales, w_codes, w_scales = ctx.saved_tensors
         need_x, need_weight = ctx.needs_input_grad
+        xt, wt = _fp8(x_codes, x_scales, 1), _fp8(w_codes, w_scales, _BLOCK)
         gq, gt = _quantize(_rows(grad_y), 1, need_x, need_weight)
         grad_x = _matmul(gq, wt, ctx.types[0]).view(*grad_y.shape[:-1], wt.shape[0]) if need_x else None
         return grad_x, _matmul(gt, xt, ctx.types[1]) if need_weight else None

@@ -99,3 +99,18 @@ def test_first_derivatives_with_a_graph_and_no_second_ones():
         got, = torch.autograd.grad(y.sum(), v, create_graph=True)
         with pytest.raises(RuntimeError, match="second derivative"):
             (y.square().sum() + got.square().sum()).backward()
+
+
+def test_what_a_gradient_needs_is_kept_as_saved_tensors():
+    """They are freed by the backward pass, which is refused the second time, and hooks on saved tensors see them."""
+    import torch
+    for name, (f, leaf) in operators_with_gradients().items():
+        v = leaf.clone().requires_grad_(True)
+        seen = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.dtype) or t, lambda t: t):
+            y = f(v)
+        assert seen, name
+        y.sum().backward()
+        with pytest.raises(RuntimeError, match="second time"):
+            y.sum().backward()
+    assert torch.float8_e4m3fn not in seen                 # the recurrence keeps its inputs and states
