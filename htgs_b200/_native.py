@@ -200,6 +200,9 @@ def lib():
                 l.htgs_dequantize_fp8.argtypes = [ctypes.POINTER(HtgsFp8Matrix), pointer, i64, i32, pointer]
                 l.htgs_fp8_matmul.argtypes = [ctypes.POINTER(HtgsFp8Matrix)] * 2 + [pointer, i64, i32, pointer]
                 l.htgs_fp8_matmul_values.argtypes = [pointer, i64, i32, i64, ctypes.POINTER(HtgsFp8Matrix), pointer, i64, i32, pointer]
+                l.htgs_fp8_matmul_status.argtypes = [i32]
+                l.htgs_fp8_matmul_error_word.restype = ctypes.POINTER(ctypes.c_uint32)
+                l.htgs_fp8_matmul_error_word.argtypes = [i32]
                 l.htgs_gated_scan_state_bytes.restype = ctypes.c_size_t
                 l.htgs_gated_scan_state_bytes.argtypes = [i64, i32]
                 l.htgs_gated_scan_workspace_bytes.restype = ctypes.c_size_t

@@ -11,6 +11,8 @@
 
 #include <cuda.h>
 
+#include <cstring>
+
 namespace htgs {
 
 namespace {
@@ -138,7 +140,7 @@ template <typename T> int matmul_values(const MatmulArgs& args, const ValuesArgs
 // Measured (bf16 out): 100000 x 1024 by 2048 2029 TFLOP/s, 8192 x 8192 by 8192 2487; without any loads the matrix instructions alone reach 2391 and 3354.
 // Split: with few tiles the sum over the columns is split over the blocks of a cluster; each leaves its 32-bit part in its shared memory, and every
 // block adds up some of the rows, always in the same order.
-// Every wait has a time limit.  A role whose wait runs out reports it (MatmulArgs::error, which the next call returns), and the others follow.
+// Every wait has a time limit.  A role whose wait runs out reports it (TileArgs::error: htgs_fp8_matmul_status), and the others follow.
 
 constexpr int kTileRows = 128;                 // of a block
 constexpr int kSms = 148;
@@ -580,24 +582,42 @@ template <typename T> bool make_out_map(CUtensorMap* map, const MatmulArgs& m) {
                     m.out, m.b.rows, m.a.rows, m.out_stride * int64_t(sizeof(T)), kPatch, kPatch);
 }
 
-// A word in the host's memory that a kernel sets when one of its waits runs out; the next product reports it.  One per process.
-unsigned int* error_word() {
-    static unsigned int* const word = [] {
+// A word for each device in the host's memory, which a kernel sets when one of its waits runs out.  The next product on that device reports it, or who asks.
+constexpr int kMostDevices = 64;
+unsigned int* error_words() {
+    static unsigned int* const words = [] {
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;       // the first call may be inside a capture
         cudaThreadExchangeStreamCaptureMode(&mode);
         void* p = nullptr;
-        if (cudaHostAlloc(&p, sizeof(unsigned int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) p = nullptr;
+        if (cudaHostAlloc(&p, kMostDevices * sizeof(unsigned int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+            p = nullptr;
+            cudaGetLastError();
+        }
         cudaThreadExchangeStreamCaptureMode(&mode);
-        if (p) *static_cast<volatile unsigned int*>(p) = 0;
+        if (p) std::memset(p, 0, kMostDevices * sizeof(unsigned int));
         return static_cast<unsigned int*>(p);
     }();
-    return word;
+    return words;
+}
+unsigned int* error_word(int device) {
+    unsigned int* const words = error_words();
+    return words && device >= 0 && device < kMostDevices ? words + device : nullptr;
+}
+int current_device() {
+    int device = -1;
+    cudaGetDevice(&device);
+    return device;
+}
+// What a word says, once: whoever reads it first clears it.
+int reported(unsigned int* word) {
+    if (!word || !__atomic_load_n(word, __ATOMIC_RELAXED) || !__atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL)) return HTGS_OK;
+    return sequence_fail(HTGS_ERR_DEVICE_FLAG, "htgs_fp8_matmul: a wait in an earlier product on this device ran out, and its result is not complete");
 }
 
 // parts: blocks of a cluster (kSplit), else the mode's own number.
 template <typename T, int BN, int MODE> int launch_tiles(const MatmulArgs& m, int parts, cudaStream_t stream) {
     using S = Tile<T, BN, MODE>;
-    unsigned int* error = error_word();
+    unsigned int* error = error_word(current_device());
     if (!error) return sequence_fail(HTGS_ERR_CUDA, "htgs_fp8_matmul: no host memory for the error word");
     CUtensorMap map_a, map_b, map_out{};
     const bool mapped = rows_aligned(m.out, m.out_stride, 2, sizeof(T), 16);
@@ -662,6 +682,14 @@ bool matrix_ok(const HtgsFp8Matrix* m) {
 
 extern "C" {
 
+unsigned int* htgs_fp8_matmul_error_word(int32_t device) { return htgs::error_word(device); }
+
+int htgs_fp8_matmul_status(int32_t device) {
+    using namespace htgs;
+    if (device < 0 || device >= kMostDevices) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_status: no such device");
+    return reported(error_word(device));
+}
+
 int htgs_fp8_matmul_values(const void* x, int64_t x_stride, int type, int64_t rows, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream) {
     using namespace htgs;
     if (!matrix_ok(b) || !known_type(type) || !known_type(out_type)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_values: bad matrix or unknown element type");
@@ -670,6 +698,7 @@ int htgs_fp8_matmul_values(const void* x, int64_t x_stride, int type, int64_t ro
     if (rows == 0 || b->rows == 0) return HTGS_OK;
     if (b->width < 1 || !x || !out || out_stride < b->rows)
         return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_values: x and out must not be null, the width at least 1, and out's rows must hold b.rows values");
+    if (const int code = reported(error_word(current_device())); code != HTGS_OK) return code;
     const HtgsFp8Matrix a{nullptr, nullptr, rows, b->width, 0, 0, 1};
     const MatmulArgs args{a, *b, out, out_stride};
     const ValuesArgs values{x, x_stride};
@@ -687,10 +716,7 @@ int htgs_fp8_matmul(const HtgsFp8Matrix* a, const HtgsFp8Matrix* b, void* out, i
     if (!known_type(out_type)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul: unknown element type");
     if (a->rows == 0 || b->rows == 0) return HTGS_OK;
     if (!out || out_stride < b->rows) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul: out must not be null, and its rows must hold b.rows values");
-    if (volatile unsigned int* error = error_word(); error && *error) {
-        *error = 0;
-        return sequence_fail(HTGS_ERR_DEVICE_FLAG, "htgs_fp8_matmul: a wait in an earlier product ran out, and its result is not complete");
-    }
+    if (const int code = reported(error_word(current_device())); code != HTGS_OK) return code;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->width == 0) {
         const cudaError_t err = cudaMemset2DAsync(out, size_t(out_stride) * type_bytes(out_type), 0, size_t(b->rows) * type_bytes(out_type), size_t(a->rows), s);

@@ -3,7 +3,7 @@ each Gaussian in the order of a space-filling curve, 10^5 to 10^6 rows long.
 
 * `add_rms_norm`, `add_rms_norm_fp8`   - root-mean-square norm of a residual stream with the residual's addition; the second leaves 8-bit codes
 * `quantize_fp8`, `Fp8Matrix`          - 8-bit matrices with a power-of-two scale for each block of 128
-* `fp8_matmul`, `fp8_linear`           - their matrix product; the second is differentiable and quantises its operands itself
+* `fp8_matmul`, `fp8_linear`           - their matrix product; the second is differentiable and quantises its operands itself; `check_products` asks after their errors
 * `gated_scan`, `gated_scan_step`      - gated linear recurrence over whole sequences (differentiable), and one step of it
 
 Values are float32, float16 or bfloat16; sums, statistics and states are 32-bit.  Everything is queued on the current CUDA stream without a
@@ -21,7 +21,7 @@ import torch
 from . import _native
 from ._native import HtgsFp8Matrix, HtgsScan
 
-__all__ = ["add_rms_norm", "add_rms_norm_fp8", "Fp8Matrix", "quantize_fp8", "fp8_matmul", "fp8_linear", "gated_scan", "gated_scan_step"]
+__all__ = ["add_rms_norm", "add_rms_norm_fp8", "Fp8Matrix", "quantize_fp8", "fp8_matmul", "fp8_linear", "check_products", "gated_scan", "gated_scan_step"]
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _BLOCK = 128
@@ -338,6 +338,13 @@ def fp8_matmul(x, weight: Fp8Matrix, dtype: Optional[torch.dtype] = None) -> tor
         return out
     q, _ = _quantize(xm, 1, True, False)
     return _matmul(q, weight, dtype).view(*x.shape[:-1], weight.shape[0])
+
+
+def check_products(device: Optional[torch.device] = None) -> None:
+    """Raises if a product on `device` (default: the current one) gave up on a wait of its kernel, so that its result is not complete.  The next product there
+    raises by itself; this is for what no product follows: after a synchronisation, at the end of a training step or behind a graph's replay.  Waits for nothing."""
+    index = None if device is None else torch.device(device).index
+    _native.check(_native.lib().htgs_fp8_matmul_status(torch.cuda.current_device() if index is None else index))
 
 
 class _Fp8Linear(torch.autograd.Function):

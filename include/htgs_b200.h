@@ -443,7 +443,7 @@ int htgs_activate_backward(const float* raw_scales, const float* raw_rotations, 
 /*
  * Operators for networks over sequences of Gaussians (no counterpart in the reference): what reads or refines a scene's Gaussians, one
  * row each in the order of a space-filling curve.  All are stream-ordered without host synchronisation, take no context, allocate
- * nothing, and give the same bits for the same inputs.  Matrices are row-major with a stride in elements (codes and scales: bytes) from row to row; `type` is an
+ * no device memory (the first product allocates 256 bytes of host memory, its error words), and give the same bits for the same inputs.  Matrices are row-major with a stride in elements (codes and scales: bytes) from row to row; `type` is an
  * HtgsElementType.  Sums, statistics and states are 32-bit whatever the type.
  */
 enum HtgsElementType { HTGS_FLOAT32 = 0, HTGS_FLOAT16 = 1, HTGS_BFLOAT16 = 2 };
@@ -486,6 +486,14 @@ int htgs_dequantize_fp8(const HtgsFp8Matrix* matrix, void* out, int64_t out_stri
  * and have a stride that is a multiple of 16; scales begin on 4 bytes with a stride that is a multiple of 4.
  */
 int htgs_fp8_matmul(const HtgsFp8Matrix* a, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream);
+/*
+ * The roles of a product's kernel wait for one another, two seconds at most.  If a wait runs out, which nothing but a fault elsewhere can cause, the result is not
+ * complete, and a word of the device's is set, in the host's memory.  The next product on that device, of whatever thread, then returns HTGS_ERR_DEVICE_FLAG and
+ * computes nothing; htgs_fp8_matmul_status returns it without a product, for instance after the synchronisation behind the last one or behind a graph's replay.  It is
+ * returned once.  htgs_fp8_matmul_error_word is the word itself (NULL without a GPU).
+ */
+int htgs_fp8_matmul_status(int32_t device);
+unsigned int* htgs_fp8_matmul_error_word(int32_t device);
 /* The same for a few rows of values, coded within the kernel as htgs_quantize_fp8 does with one row per scale: at most 8 rows, and 32768 values with the
  * width rounded up to 128. */
 int htgs_fp8_matmul_values(const void* x, int64_t x_stride, int type, int64_t rows, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream);

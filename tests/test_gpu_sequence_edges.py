@@ -114,3 +114,28 @@ def test_what_a_gradient_needs_is_kept_as_saved_tensors():
         with pytest.raises(RuntimeError, match="second time"):
             y.sum().backward()
     assert torch.float8_e4m3fn not in seen                 # the recurrence keeps its inputs and states
+
+
+def test_a_wait_that_ran_out_is_reported_once_and_for_its_device():
+    """The word that a kernel sets is set here on the host."""
+    import torch
+    from htgs_b200 import _native, sequence as seq
+    lib = _native.lib()
+    x, w = draw((20, 128), 1), draw((16, 128), 2)
+    q = seq.quantize_fp8(w, 128)
+    want, few = seq.fp8_matmul(x, q), seq.fp8_matmul(x[:2], q)
+    word, other = (lib.htgs_fp8_matmul_error_word(device) for device in (0, 1))
+    for call in (lambda: seq.fp8_matmul(x, q), lambda: seq.fp8_matmul(x[:2], q), lambda: seq.fp8_matmul(seq.quantize_fp8(x[:2]), q), lambda: seq.fp8_linear(x, w),
+                 lambda: seq.check_products(), lambda: seq.check_products(x.device)):
+        word[0] = 1
+        with pytest.raises(RuntimeError, match="wait in an earlier product"):
+            call()
+        assert word[0] == 0
+        seq.check_products()
+        assert torch.equal(seq.fp8_matmul(x, q), want)
+    other[0] = 1                                           # another device's
+    assert torch.equal(seq.fp8_matmul(x, q), want) and torch.equal(seq.fp8_matmul(x[:2], q), few)
+    seq.check_products("cuda:0")
+    assert lib.htgs_fp8_matmul_status(1) == _native.HTGS_ERR_DEVICE_FLAG and lib.htgs_fp8_matmul_status(1) == 0
+    for device in (-1, 64):
+        assert lib.htgs_fp8_matmul_status(device) == _native.HTGS_ERR_INVALID_ARGUMENT and not lib.htgs_fp8_matmul_error_word(device)
