@@ -140,7 +140,8 @@ template <typename T> int matmul_values(const MatmulArgs& args, const ValuesArgs
 // Measured (bf16 out): 100000 x 1024 by 2048 2029 TFLOP/s, 8192 x 8192 by 8192 2487; without any loads the matrix instructions alone reach 2391 and 3354.
 // Split: with few tiles the sum over the columns is split over the blocks of a cluster; each leaves its 32-bit part in its shared memory, and every
 // block adds up some of the rows, always in the same order.
-// Every wait has a time limit.  A role whose wait runs out reports it (TileArgs::error: htgs_fp8_matmul_status), and the others follow.
+// Every wait has a time limit.  A role whose wait runs out reports it (TileArgs::error: htgs_fp8_matmul_status), the others follow,
+// and the block's tiles are left full of NaN.
 
 constexpr int kTileRows = 128;                 // of a block
 constexpr int kSms = 148;
@@ -277,6 +278,19 @@ template <typename T> __device__ __forceinline__ void fill_patch(unsigned char* 
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, int column, int row, const void* from) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;"
                  ::"l"(map), "r"(column), "r"(row), "r"(smem_u32(from)) : "memory");
+}
+
+// After a wait that ran out: NaN in every tile that the block had a part in, so that what it left there cannot pass for a result.  The block's own stores have ended,
+// and where sums are split the cluster's.
+template <typename T> __device__ __noinline__ void leave_nan(T* out, int64_t out_stride, int rows_a, int rows_b, int tiles_n, int tiles, int first_tile, int tile_step,
+                                                            int rows_of_tile, int row_in_tile, int columns) {
+    for (int tile = first_tile; tile < tiles; tile += tile_step) {
+        const int64_t row0 = int64_t(tile / tiles_n) * rows_of_tile + row_in_tile, column0 = int64_t(tile % tiles_n) * columns;
+        for (int i = threadIdx.x; i < kTileRows * columns; i += kTileThreads) {
+            const int64_t row = row0 + i / columns, column = column0 + i % columns;
+            if (row < rows_a && column < rows_b) out[row * out_stride + column] = from_float<T>(__uint_as_float(0x7fffffffu));
+        }
+    }
 }
 
 // kSplit: gridDim.x = tiles * parts in clusters of `parts` blocks, one tile each; kPair: clusters of two blocks, and parts is 2; kSingle: parts is 1.
@@ -545,9 +559,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) matmul_tiles_kernel(const __g
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
-    if (threadIdx.x == 0 && *failed) {
-        *reinterpret_cast<volatile unsigned int*>(args.error) = 1;
-        __threadfence_system();
+    if (*failed) {
+        leave_nan<T>(static_cast<T*>(args.out), args.out_stride, args.rows_a, args.rows_b, args.tiles_n, args.tiles, first_tile, tile_step, kRowsOfTile, row_in_tile, BN);
+        if (threadIdx.x == 0) {
+            *reinterpret_cast<volatile unsigned int*>(args.error) = 1;
+            __threadfence_system();
+        }
     }
 }
 

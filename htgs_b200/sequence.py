@@ -341,7 +341,7 @@ def fp8_matmul(x, weight: Fp8Matrix, dtype: Optional[torch.dtype] = None) -> tor
 
 
 def check_products(device: Optional[torch.device] = None) -> None:
-    """Raises if a product on `device` (default: the current one) gave up on a wait of its kernel, so that its result is not complete.  The next product there
+    """Raises if a product on `device` (default: the current one) gave up on a wait of its kernel, so that its result is not complete: NaN where something is missing.  The next product there
     raises by itself; this is for what no product follows: after a synchronisation, at the end of a training step or behind a graph's replay.  Waits for nothing."""
     index = None if device is None else torch.device(device).index
     _native.check(_native.lib().htgs_fp8_matmul_status(torch.cuda.current_device() if index is None else index))
