@@ -140,7 +140,7 @@ template <typename T> int matmul_values(const MatmulArgs& args, const ValuesArgs
 // Measured (bf16 out): 100000 x 1024 by 2048 2029 TFLOP/s, 8192 x 8192 by 8192 2487; without any loads the matrix instructions alone reach 2391 and 3354.
 // Split: with few tiles the sum over the columns is split over the blocks of a cluster; each leaves its 32-bit part in its shared memory, and every
 // block adds up some of the rows, always in the same order.
-// Every wait has a time limit.  A role whose wait runs out reports it (TileArgs::error: htgs_fp8_matmul_status), the others follow,
+// Every wait has a time limit (WaitLimit).  A role whose wait runs out reports it (TileArgs::error: htgs_fp8_matmul_status), the others follow,
 // and the block's tiles are left full of NaN.
 
 constexpr int kTileRows = 128;                 // of a block
@@ -187,13 +187,13 @@ __device__ __forceinline__ void arrive(uint64_t* bar) {
 }
 // False if the time limit ran out or another role has given up.  Out of line: the roles' loops are single threads whose every instruction counts.
 __device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-    const uint64_t begin = nanoseconds();
+    WaitLimit limit(kWaitNanoseconds, nanoseconds());
     for (;;) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
         if (*failed) return false;
-        if (nanoseconds() - begin > kWaitNanoseconds) { *failed = 1; return false; }
+        if (limit.over(nanoseconds())) { *failed = 1; return false; }
     }
 }
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
@@ -369,13 +369,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) matmul_tiles_kernel(const __g
             }
         }
         if (!ok && PAIR) {      // no copy may be on its way when the block ends; a pair's second block has no barrier to ask
-            const uint64_t begin = nanoseconds();
-            while (nanoseconds() - begin < 20000000ull) {}
+            WaitLimit limit(20000000, nanoseconds());
+            while (!limit.over(nanoseconds())) {}
         }
         if (!ok && !PAIR)
             for (uint32_t u = uses > S::stages ? uses - S::stages : 0; u < uses; ++u) {
-                const uint64_t begin = nanoseconds();
-                while (!mbar_try_wait(full + u % S::stages, u / S::stages & 1) && nanoseconds() - begin < kWaitNanoseconds) {}
+                WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                while (!mbar_try_wait(full + u % S::stages, u / S::stages & 1) && !limit.over(nanoseconds())) {}
             }
     } else if (warp == 1) {
         if (!PAIR || part == 0) {
@@ -415,8 +415,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) matmul_tiles_kernel(const __g
             }
             if (!ok && one) {
                 tmem_commit<MODE>(drained);
-                const uint64_t begin = nanoseconds();
-                while (!mbar_try_wait(drained, 0) && nanoseconds() - begin < kWaitNanoseconds) {}
+                WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                while (!mbar_try_wait(drained, 0) && !limit.over(nanoseconds())) {}
             }
         }
     } else if (warp >= 4 && warp < 8) {

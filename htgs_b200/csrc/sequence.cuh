@@ -166,6 +166,21 @@ template <int BEGUN> __device__ __forceinline__ void copies_done() {          //
     __syncwarp();
 }
 
+// The limit of a wait that polls, in nanoseconds of the time in which it polled: between two polls a hundredth of a second counts at most, so that time in which the
+// kernel did not run at all (the GPU was another process's, or the process was suspended) is not held against it.
+struct WaitLimit {
+    static constexpr uint64_t kMostGap = 10000000;
+    uint64_t left, before;
+    __host__ __device__ __forceinline__ WaitLimit(uint64_t limit, uint64_t now) : left(limit), before(now) {}
+    __host__ __device__ __forceinline__ bool over(uint64_t now) {
+        const uint64_t gap = now - before < kMostGap ? now - before : kMostGap;
+        before = now;
+        if (left <= gap) return true;
+        left -= gap;
+        return false;
+    }
+};
+
 // Blocks of a cluster: what block `block` has at this block's shared address `address`, and a barrier of all their threads.  The barrier's instructions are
 // of whole warps (.aligned), which have to come back together first if they stand behind a branch or a loop that some lanes took.
 __device__ __forceinline__ uint32_t peer_address(uint32_t address, uint32_t block) {

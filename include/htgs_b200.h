@@ -487,7 +487,7 @@ int htgs_dequantize_fp8(const HtgsFp8Matrix* matrix, void* out, int64_t out_stri
  */
 int htgs_fp8_matmul(const HtgsFp8Matrix* a, const HtgsFp8Matrix* b, void* out, int64_t out_stride, int out_type, void* stream);
 /*
- * The roles of a product's kernel wait for one another, two seconds at most.  If a wait runs out, which nothing but a fault elsewhere can cause, the result is not
+ * The roles of a product's kernel wait for one another, two seconds of running time at most.  If a wait runs out, which nothing but a fault elsewhere can cause, the result is not
  * complete (its tiles that lack something are NaN), and a word of the device's is set, in the host's memory.  The next product on that device, of whatever thread, then returns HTGS_ERR_DEVICE_FLAG and
  * computes nothing; htgs_fp8_matmul_status returns it without a product, for instance after the synchronisation behind the last one or behind a graph's replay.  It is
  * returned once.  htgs_fp8_matmul_error_word is the word itself (NULL without a GPU).
