@@ -7,8 +7,9 @@ returns refined ones, which go on into `glue.activate` and the rasterizer.
     image = diff_rasterize(refined["positions"], scales, rotations, opacities, refined["sh_0"], sh_rest, densification_info, settings, False)
 
 Each layer adds to a residual stream what a gated recurrence along the curve makes of it: norm, projection to values and gates, recurrence (forwards and
-backwards in turn), projection back.  In training the norm is 16-bit and the projections code their operands themselves; `freeze()` codes the weights once, and from then on
-`infer` has the norm leave 8-bit codes and the projections take them.  (No counterpart in the reference.)
+backwards in turn), projection back.  The raw parameters go into the first projection in 32 bits: with the three bits of an 8-bit code neighbours
+along the curve would be one number to the network.  The others are 8-bit products: in training the norm is 16-bit and they code their operands themselves; `freeze()` codes their weights
+once, and from then on `infer` has the norm leave 8-bit codes and the projections take them.  (No counterpart in the reference.)
 """
 from __future__ import annotations
 
@@ -65,14 +66,14 @@ class GaussianRefiner(torch.nn.Module):
     def freeze(self) -> "GaussianRefiner":
         """Codes the weights for `infer`; to be called again when they have changed."""
         with torch.no_grad():
-            self._frozen = {"embed": quantize_fp8(self.embed, 128), "head": quantize_fp8(self.head, 128),
-                            "enter": [quantize_fp8(w, 128) for w in self.enter], "leave": [quantize_fp8(w, 128) for w in self.leave]}
+            self._frozen = {"embed": self.embed.detach().to(torch.float32, copy=True), "head": quantize_fp8(self.head, 128), "enter": [quantize_fp8(w, 128) for w in self.enter],
+                            "leave": [quantize_fp8(w, 128) for w in self.leave]}
         return self
 
-    def _read(self, raw: Dict[str, torch.Tensor], offsets):
+    def _read(self, raw: Dict[str, torch.Tensor], offsets, embed):
         flat = torch.cat([raw[name].reshape(-1, width) for name, width in PARAMETERS], dim=1)
         order = curve_order(raw["positions"].detach(), offsets)
-        return flat, order, flat[order].to(self.embed.dtype)
+        return flat, order, torch.nn.functional.linear(flat[order].float(), embed.float()).to(self.embed.dtype)
 
     def _write(self, raw, flat, order, change):
         refined = flat.index_add(0, order, change.to(flat.dtype) * self.step)
@@ -81,8 +82,8 @@ class GaussianRefiner(torch.nn.Module):
 
     def forward(self, raw: Dict[str, torch.Tensor], offsets: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
         """Refined copies of the parameters named in PARAMETERS; `offsets` (int32) where packed scenes begin.  Differentiable."""
-        flat, order, x = self._read(raw, offsets)
-        update, stream = fp8_linear(x, self.embed), None
+        flat, order, update = self._read(raw, offsets, self.embed)
+        stream = None
         for layer in range(self.layers):
             y, stream = add_rms_norm(update, self.norms[layer], stream)
             both = fp8_linear(y, self.enter[layer])
@@ -97,8 +98,8 @@ class GaussianRefiner(torch.nn.Module):
         if self._frozen is None:
             raise RuntimeError("call freeze() before infer()")
         f = self._frozen
-        flat, order, x = self._read(raw, offsets)
-        update, stream = fp8_matmul(x, f["embed"]), None
+        flat, order, update = self._read(raw, offsets, f["embed"])
+        stream = None
         for layer in range(self.layers):
             q, stream = add_rms_norm_fp8(update, self.norms[layer], stream)
             both = fp8_matmul(q, f["enter"][layer], update.dtype)

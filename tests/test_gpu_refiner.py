@@ -93,3 +93,32 @@ def test_packed_scenes_are_refined_as_each_alone_wherever_the_others_lie():
         results.append(model.infer(both, offsets))
     for name, _ in PARAMETERS:
         assert torch.equal(results[0][name][:700], results[1][name][:700]), name
+
+
+def test_near_positions_are_told_apart():
+    """Gaussians a fortieth apart between 1 and 2, with nothing else to tell them by and no recurrence: 8-bit numbers there are an eighth apart, which would leave nine
+    different changes; the coding of the norm's output may take a few of the 41 away."""
+    import torch
+    from htgs_b200.refiner import PARAMETERS, GaussianRefiner
+    torch.manual_seed(4)
+    model = GaussianRefiner(64, 0, step=1.0).cuda()
+    raw = {name: torch.ones(41, *((width,) if name != "sh_0" else (1, 3)), device="cuda") for name, width in PARAMETERS}
+    raw["positions"] = torch.cat((torch.linspace(1.0, 2.0, 41, device="cuda")[:, None], torch.ones(41, 2, device="cuda")), dim=1)
+    with torch.no_grad():
+        for result in (model(raw), model.freeze().infer(raw)):
+            change = torch.cat([(result[name] - raw[name]).reshape(41, -1) for name, _ in PARAMETERS[1:]], dim=1)
+            assert torch.unique(change, dim=0).shape[0] > 20
+
+
+def test_infer_stays_with_the_weights_that_were_coded():
+    import torch
+    from htgs_b200.refiner import GaussianRefiner
+    torch.manual_seed(5)
+    _, raw, _ = raw_scene(300)
+    model = GaussianRefiner(64, 2).cuda().freeze()
+    before = model.infer(raw)
+    with torch.no_grad():
+        for p in (model.embed, model.head, *model.enter, *model.leave):
+            p.mul_(2)
+    assert all(torch.equal(before[name], value) for name, value in model.infer(raw).items())
+    assert not torch.equal(before["positions"], model.freeze().infer(raw)["positions"])
