@@ -137,8 +137,10 @@ __global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const Qu
     __shared__ float column_largest[16][kScaleBlock];
     __shared__ float column_all[kScaleBlock];
     const int l = threadIdx.x & 15, h = threadIdx.x >> 4;
-    const int64_t row0 = int64_t(blockIdx.y) * kScaleBlock, column0 = int64_t(blockIdx.x) * kScaleBlock;
+    const uint32_t right = blockIdx.x, down = blockIdx.z * gridDim.y + blockIdx.y;       // of the tiles; a grid has 65535 blocks in its second direction
+    const int64_t row0 = int64_t(down) * kScaleBlock, column0 = int64_t(right) * kScaleBlock;
     const int rows = int(min(int64_t(kScaleBlock), a.rows - row0)), columns = int(min(int64_t(kScaleBlock), a.width - column0));
+    if (rows <= 0) return;
     const T* x = static_cast<const T*>(a.x) + row0 * a.x_stride + column0;
     if (WIDE) {
         constexpr int kPieces = kScaleBlock / VEC;                       // of a row
@@ -214,14 +216,14 @@ __global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const Qu
         for (int i = 0; i < 16; ++i) largest = fmaxf(largest, column_largest[i][threadIdx.x]);
         if (PER_TILE) largest = lanes_max<32>(largest);
         column_all[threadIdx.x] = largest;
-        if (!PER_TILE && a.codes_t && int(threadIdx.x) < columns) a.scales_t[(column0 + threadIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(scale_exponent(largest) + 127);
+        if (!PER_TILE && a.codes_t && int(threadIdx.x) < columns) a.scales_t[(column0 + threadIdx.x) * a.scales_t_stride + down] = uint8_t(scale_exponent(largest) + 127);
     }
     __syncthreads();
     int tile_e = 0;
     if (PER_TILE) {
         tile_e = scale_exponent(fmaxf(fmaxf(column_all[0], column_all[32]), fmaxf(column_all[64], column_all[96])));
-        if (threadIdx.x == 0 && a.codes) a.scales[int64_t(blockIdx.y) * a.scales_stride + blockIdx.x] = uint8_t(tile_e + 127);
-        if (threadIdx.x == 0 && a.codes_t) a.scales_t[int64_t(blockIdx.x) * a.scales_t_stride + blockIdx.y] = uint8_t(tile_e + 127);
+        if (threadIdx.x == 0 && a.codes) a.scales[int64_t(down) * a.scales_stride + right] = uint8_t(tile_e + 127);
+        if (threadIdx.x == 0 && a.codes_t) a.scales_t[int64_t(right) * a.scales_t_stride + down] = uint8_t(tile_e + 127);
     }
     if (a.codes) {
         const bool together = a.width % VEC == 0 && a.codes_stride % VEC == 0 && reinterpret_cast<uintptr_t>(a.codes) % VEC == 0;
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kQuantBlock, 4) quantize_tiles_kernel(const Qu
                         if (column(j * VEC + i) < columns) codes[column(j * VEC + i)] = uint8_t(encode2<true>(f[i], 0.0f, inverse) & 0xffu);
                 }
             }
-            if (!PER_TILE && l == 0) a.scales[(row0 + h * 8 + r) * a.scales_stride + blockIdx.x] = uint8_t(e + 127);
+            if (!PER_TILE && l == 0) a.scales[(row0 + h * 8 + r) * a.scales_stride + right] = uint8_t(e + 127);
         }
     }
     if (!a.codes_t) return;
@@ -412,7 +414,8 @@ template <typename T> cudaError_t quantize_anywhere(const QuantArgs& a, cudaStre
     return err;
 }
 template <typename T, bool WIDE, bool PER_TILE> cudaError_t launch_tiles(const QuantArgs& a, cudaStream_t stream) {
-    const dim3 grid(unsigned((a.width + kScaleBlock - 1) / kScaleBlock), unsigned((a.rows + kScaleBlock - 1) / kScaleBlock));
+    const unsigned down = unsigned((a.rows + kScaleBlock - 1) / kScaleBlock), deep = (down + 65534) / 65535;
+    const dim3 grid(unsigned((a.width + kScaleBlock - 1) / kScaleBlock), (down + deep - 1) / deep, deep);
     constexpr int smem = kScaleBlock * kTilePitch<T, WIDE> * int(sizeof(T));
     static PerDeviceOnce once;
     const cudaError_t err = once.run([] { return cudaFuncSetAttribute(quantize_tiles_kernel<T, WIDE, PER_TILE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
@@ -472,7 +475,6 @@ int htgs_quantize_fp8(const void* x, int64_t x_stride, int type, int64_t rows, i
     if (rows_per_scale != 1 && rows_per_scale != kScaleBlock) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_quantize_fp8: rows_per_scale must be 1 or 128");
     if (rows == 0 || width == 0) return HTGS_OK;
     if (!x || (!codes && !codes_t) || (codes && !scales) || (codes_t && !scales_t)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_quantize_fp8: null pointer");
-    if ((codes_t || rows_per_scale != 1) && rows > 65535ll * kScaleBlock) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_quantize_fp8: at most 8388480 rows with tiles or a transpose");
     const QuantArgs a{x, x_stride, rows, width, codes, scales, codes_stride, scales_stride, codes_t, scales_t, codes_t_stride, scales_t_stride};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (type == HTGS_FLOAT32) return quantize_typed<float>(a, rows_per_scale, s);

@@ -139,3 +139,26 @@ def test_a_wait_that_ran_out_is_reported_once_and_for_its_device():
     assert lib.htgs_fp8_matmul_status(1) == _native.HTGS_ERR_DEVICE_FLAG and lib.htgs_fp8_matmul_status(1) == 0
     for device in (-1, 64):
         assert lib.htgs_fp8_matmul_status(device) == _native.HTGS_ERR_INVALID_ARGUMENT and not lib.htgs_fp8_matmul_error_word(device)
+
+
+def test_more_rows_than_a_grid_has_in_one_direction():
+    """65536 blocks of 128 rows and a few more: coded by blocks and transposed, and through the linear layer's gradients."""
+    import torch
+    from htgs_b200 import sequence as seq
+    rows, begin = 65536 * 128 + 130, 65536 * 128 - 128           # what is not zero lies at the end
+    x, gy, w = torch.zeros(rows, 16, dtype=torch.bfloat16, device="cuda"), torch.zeros(rows, 24, dtype=torch.bfloat16, device="cuda"), draw((24, 16), 3, "bf16")
+    x[begin:], gy[begin:] = draw((rows - begin, 16), 1, "bf16"), draw((rows - begin, 24), 2, "bf16")
+    blocks, turned = seq.quantize_fp8(x, 128), seq.quantize_fp8(x, 1, True)
+    end = f64(x[begin:])
+    for q, part, want, per in ((blocks, slice(begin, None), ref.quantize(end, 128), 128), (turned, slice(None), ref.quantize(end.T.copy()), 1)):
+        codes = q.codes[part] if per == 128 else q.codes[:, begin:]
+        scales = q.scales[begin // 128:] if per == 128 else q.scales[:, begin // 128:]
+        assert np.array_equal(codes.float().double().cpu().numpy(), want[0])
+        assert np.array_equal(scales.contiguous().view(torch.uint8).cpu().numpy().astype(np.int64) - 127, want[1])
+    assert not blocks.codes[:begin].view(torch.uint8).any() and not turned.codes[:, :begin].view(torch.uint8).any()
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    gx, gw = torch.autograd.grad(seq.fp8_linear(*leaves), leaves, gy)
+    rowwise, tilewise = lambda v: ref.dequantize(*ref.quantize(v)), lambda v: ref.dequantize(*ref.quantize(v, 128), 128)  # noqa: E731
+    g = f64(gy[begin:])
+    near(gw, *product_bound(rowwise(g.T.copy()), rowwise(end.T.copy()), "bf16"), "grad_weight")
+    near(gx[begin:], *product_bound(rowwise(g), tilewise(f64(w)).T, "bf16"), "grad_x")
