@@ -25,8 +25,8 @@ CHANNELS = sum(width for _, width in PARAMETERS)
 
 
 def curve_order(positions: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Indices that sort Gaussians along the Morton curve through 2^10 cells a side of the bounding box of their finite positions (others lie at its faces).  With the `offsets` at which packed scenes begin, each scene
-    has its own box and its own curve: it gets the order that it has alone."""
+    """Indices that sort Gaussians along the Morton curve through cubic cells, 2^20 along the longest side of the bounding box of their finite positions (others
+    lie at its faces).  With the `offsets` at which packed scenes begin, each scene has its own box and its own curve: it gets the order that it has alone."""
     if positions.shape[0] == 0:
         return torch.empty(0, dtype=torch.long, device=positions.device)
     finite = positions.isfinite()
@@ -38,14 +38,13 @@ def curve_order(positions: torch.Tensor, offsets: Optional[torch.Tensor] = None)
         box = [torch.zeros((offsets.numel() - 1, 3), dtype=positions.dtype, device=positions.device).scatter_reduce_(
             0, scene[:, None].expand(-1, 3), ends, reduce, include_self=False) for ends, reduce in ((least, "amin"), (most, "amax"))]
         low, high = box[0][scene], box[1][scene]
-    cell = ((positions - low) / (high - low).clamp(min=1e-12) * 1023.0).nan_to_num().clamp(0, 1023).long()
-    code = torch.zeros(positions.shape[0], dtype=torch.long, device=positions.device)
-    for bit in range(10):
-        for axis in range(3):
-            code |= (cell[:, axis] >> bit & 1) << (3 * bit + axis)
-    if offsets is not None:
-        code |= scene << 30
-    return torch.argsort(code, stable=True)
+    most_cell = 2 ** 20 - 1            # so many, and cubes, that a few Gaussians far from the others leave these enough of them in each direction
+    side = (high - low).amax(dim=-1, keepdim=True).clamp(min=1e-12)
+    cell = ((positions.float() - low) / side * most_cell).nan_to_num().clamp(0, most_cell).long()
+    for shift, mask in ((32, 0x1F00000000FFFF), (16, 0x1F0000FF0000FF), (8, 0x100F00F00F00F00F), (4, 0x10C30C30C30C30C3), (2, 0x1249249249249249)):
+        cell = (cell | cell << shift) & mask                     # bit i goes to bit 3 i
+    order = torch.argsort(cell[:, 0] | cell[:, 1] << 1 | cell[:, 2] << 2, stable=True)
+    return order if offsets is None else order[torch.argsort(scene[order], stable=True)]
 
 
 class GaussianRefiner(torch.nn.Module):

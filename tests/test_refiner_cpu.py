@@ -66,3 +66,24 @@ def test_positions_that_are_not_finite_leave_the_others_in_order():
     assert torch.equal(refiner.curve_order(nothing), torch.arange(3))
     parts = [positions, odd]
     assert torch.equal(refiner.curve_order(torch.cat(parts), torch.tensor([0, 400, 801], dtype=torch.int32)), separate_orders(parts))
+
+
+def test_a_few_far_positions_leave_the_others_near_one_another():
+    """Steps along the curve through 10 000 points of a unit cube are about as long as its cells, without and with one point ten thousand times as far away (in a
+    random order they would be 0.66 on average)."""
+    g = torch.Generator().manual_seed(5)
+    positions = torch.rand((10_000, 3), generator=g)
+    for points in (positions, torch.cat((positions, torch.full((1, 3), 1e4))), torch.cat((torch.tensor([[-1e4, 0.5, 2.0]]), positions))):
+        order = refiner.curve_order(points)
+        path = points[order]
+        path = path[(path.abs() <= 1).all(dim=1)]
+        assert path.shape[0] == 10_000 and (path[1:] - path[:-1]).norm(dim=1).mean().item() < 0.15
+
+
+def test_curve_order_is_that_of_the_interleaved_cells():
+    g = torch.Generator().manual_seed(6)
+    positions = torch.randint(0, 2 ** 20, (2000, 3), generator=g).float()
+    positions[0], positions[1] = 0.0, 2.0 ** 20 - 1
+    cells = [[int(c) for c in p] for p in positions]
+    code = [sum((c >> bit & 1) << (3 * bit + axis) for bit in range(20) for axis, c in enumerate(cell)) for cell in cells]
+    assert refiner.curve_order(positions).tolist() == sorted(range(2000), key=lambda i: code[i])
