@@ -5,8 +5,8 @@
 // The product of two E4M3 codes is exact in 32 bits, and a scale shifts its exponent, so the only roundings are those of the 32-bit
 // sum and the last one to the output's type.
 //
-// Few rows: `matmul_rows_kernel`, a warp per row of b, bound by reading b and, where b is small, by the launch (1 x 1024 by 2048: 4.5 us).  Otherwise `matmul_tiles_kernel` on the tensor cores, which take the
-// scales themselves (kind::mxf8f6f4, one scale per row and 32 columns; a block of 128 uses the same one four times).
+// Up to eight rows: `matmul_rows_kernel`, a warp per row of b.  Otherwise `matmul_tiles_kernel` on the tensor cores, which take the scales themselves (kind::mxf8f6f4, one scale
+// per row and 32 columns; a block of 128 uses the same one four times).
 #include "sequence.cuh"
 
 #include <cuda.h>
@@ -37,7 +37,9 @@ __device__ __forceinline__ void load_codes(const uint8_t* row, int64_t k, int64_
     }
 }
 
-// Few rows of a: a warp per row of b, 16 codes of it in a lane at a time, against ROWS rows of a.  Bound by reading b, and for small b by the launch.
+// Few rows of a: a warp per row of b, 16 codes of it in a lane at a time, against ROWS rows of a.  Bound by the launch for small b, else by instructions: a multiply-add and a part of
+// decoding for each code and row of a.  us, one row / eight rows, and the tensor cores' tiles for either (of codes, calls close behind one another; b up to 2048 x 2048 in L2, beyond it from HBM): 512 x 512 1.9 / 5.8 and 3.4, 1024 x 2048
+// 2.8 / 10.4 and 4.5, 2048 x 2048 5.1 / 18.6 and 6.7, 4096 x 4096 10.6 / 46 and 8.6, 8192 x 8192 34 / 152 and 19.  What it saves is a launch, with VALUES: the coding's.
 // With VALUES a comes as values of type X and each block codes them itself into shared memory, as quantize_rows_kernel would (fp8.cu): a launch less.
 struct ValuesArgs { const void* x; int64_t stride; };
 constexpr int kMostRows = 8, kMostValues = 32768;       // of a

@@ -13,8 +13,8 @@
 // kept as -0 and tested for, so that a NaN or infinity of one sequence does not reach the next.  States, products and sums are 32-bit; 1 - a is
 // exp(-gate) a, which keeps its relative precision where a is close to 1.
 //
-// Bound by HBM, and x and gate are read twice: a look-back from chunk to chunk in one pass would have to advance a chunk every 15 ns at 128 channels, and one takes
-// microseconds.  1000000 x 128 in bf16: 86 us first pass (6.0 TB/s), 17 second, 109 third (7.0 TB/s, what L2 still has counted in); 262144 x 512: 91 + 14 + 134 forward,
+// Bound by HBM, and x and gate are read twice: a look-back from chunk to chunk in one pass would have to advance a chunk of 64 rows every 15 ns at 128 channels, and one takes
+// microseconds.  (Wider rows in longer chunks would give it more time: 120 ns for 256 rows of 512 channels.)  1000000 x 128 in bf16: 86 us first pass (6.0 TB/s), 17 second, 109 third (7.0 TB/s, what L2 still has counted in); 262144 x 512: 91 + 14 + 134 forward,
 // 92 + 14 + 221 backward.  Chunks of 64 rows keep every warp of the GPU busy at these sizes; a third pass over rows in registers, without shared memory, took 159 us.
 #include "sequence.cuh"
 
@@ -509,7 +509,8 @@ __global__ void __launch_bounds__(kScanBlock, 5) scan_apply_backward_kernel(cons
     pass_empty_sequences(args, args.grad_last, args.grad_initial, at.chunk, at.channel, at.live);
 }
 
-// One step for each row, the state updated in place.  Bound by the launch up to thousands of rows.
+// One step for each row, the state updated in place.  Bound by the launch up to some hundred rows (1024 columns in bf16: 64 rows 1.9 us, 256 3.3, 1024 6.0), then by
+// instructions, at about half of what HBM gives: 4096 rows 15.8 us, 16384 63.6 (3.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) scan_step_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ gate, int64_t gate_stride, float* state,
                                                        int64_t state_stride, T* h, int64_t h_stride, int64_t rows, int width) {
