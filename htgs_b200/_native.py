@@ -96,6 +96,26 @@ class HtgsScan(ctypes.Structure):
                 ("n_sequences", ctypes.c_int32), ("type", ctypes.c_int32), ("reverse", ctypes.c_int32)]
 
 
+class HtgsRotary(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p * 2), ("y", ctypes.c_void_p * 2), ("positions", ctypes.c_void_p), ("x_stride", ctypes.c_int64 * 2), ("x_head_stride", ctypes.c_int64 * 2),
+                ("positions_stride", ctypes.c_int64), ("rows", ctypes.c_int64), ("base", ctypes.c_double), ("heads", ctypes.c_int32 * 2), ("sections", ctypes.c_int32 * 4),
+                ("axes", ctypes.c_int32), ("positions_type", ctypes.c_int32), ("width", ctypes.c_int32), ("type", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("inverse", ctypes.c_int32)]
+
+
+class HtgsAttention(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("q", "k", "v", "offsets")] + [(name, ctypes.c_int64) for name in (
+        "q_stride", "k_stride", "v_stride", "q_head_stride", "k_head_stride", "v_head_stride", "rows")] + [(name, ctypes.c_int32) for name in (
+            "heads", "key_heads", "width", "n_sequences", "type", "causal", "window")] + [("scale", ctypes.c_float)]
+
+
+class HtgsAttentionStep(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("q", "k", "v", "keys", "values", "lengths")] + [(name, ctypes.c_int64) for name in (
+        "q_stride", "k_stride", "v_stride", "q_head_stride", "k_head_stride", "v_head_stride", "keys_stride", "values_stride", "keys_row_stride", "values_row_stride",
+        "keys_head_stride", "values_head_stride", "capacity")] + [(name, ctypes.c_int32) for name in ("batch", "heads", "key_heads", "width", "type", "window")] + [
+            ("scale", ctypes.c_float)]
+
+
 class HtgsError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(message)
@@ -211,6 +231,17 @@ def lib():
                 l.htgs_gated_scan_backward.argtypes = [ctypes.POINTER(HtgsScan), pointer, pointer, i64, pointer, pointer, i64, pointer, i64, pointer, pointer,
                                                        ctypes.c_size_t, pointer]
                 l.htgs_gated_scan_step.argtypes = [pointer, i64, pointer, i64, pointer, i64, pointer, i64, i32, i64, i32, pointer]
+                l.htgs_rotary.argtypes = [ctypes.POINTER(HtgsRotary), pointer]
+                l.htgs_attention.argtypes = [ctypes.POINTER(HtgsAttention), pointer, pointer, pointer]
+                l.htgs_attention_backward_workspace_bytes.restype = ctypes.c_size_t
+                l.htgs_attention_backward_workspace_bytes.argtypes = [ctypes.POINTER(HtgsAttention)]
+                l.htgs_attention_backward.argtypes = [ctypes.POINTER(HtgsAttention), pointer, pointer, pointer, i64, i64, pointer, pointer, pointer, pointer, ctypes.c_size_t, pointer]
+                l.htgs_attention_status.argtypes = [i32]
+                l.htgs_attention_error_word.restype = ctypes.POINTER(ctypes.c_uint32)
+                l.htgs_attention_error_word.argtypes = [i32]
+                l.htgs_attention_step_workspace_bytes.restype = ctypes.c_size_t
+                l.htgs_attention_step_workspace_bytes.argtypes = [ctypes.POINTER(HtgsAttentionStep)]
+                l.htgs_attention_step.argtypes = [ctypes.POINTER(HtgsAttentionStep), pointer, pointer, ctypes.c_size_t, pointer]
                 l.htgs_set_profiling.argtypes = [ctypes.c_void_p, ctypes.c_int]
                 l.htgs_set_collect_stats.argtypes = [ctypes.c_void_p, ctypes.c_int]
                 l.htgs_set_fast_deterministic.argtypes = [ctypes.c_void_p, ctypes.c_int]

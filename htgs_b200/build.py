@@ -16,8 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libhtgs_b200.so")
 SOURCES = ["api.cu", "preprocess.cu", "binning.cu", "binning_unordered.cu", "blend.cu", "blend_fast.cu", "train.cu", "noalloc.cu", "filter3d.cu", "weights.cu", "activation.cu", "exchange.cu",
-           "norm.cu", "fp8.cu", "fp8_matmul.cu", "scan.cu"]
-HEADERS = ["common.cuh", "core_buffer.cuh", "kernels.h", "sequence.cuh", os.path.join("..", "..", "include", "htgs_b200.h")]
+           "norm.cu", "fp8.cu", "fp8_matmul.cu", "scan.cu", "rotary.cu", "attention.cu", "attention_tiles.cu", "attention_step.cu"]
+HEADERS = ["common.cuh", "core_buffer.cuh", "kernels.h", "sequence.cuh", "tensor_core.cuh", "attention.cuh", os.path.join("..", "..", "include", "htgs_b200.h")]
 
 # IEEE division / sqrt and no fast-math: the per-fragment arithmetic has to round exactly like
 # the reference's base build (its setup.py adds no fast-math flag to the main extension).
@@ -114,7 +114,7 @@ def build_bindings(force: bool = False) -> tuple:
     targets = binding_paths()
     jobs = []
     for target, name, extra in ((targets[0], "_C", []), (targets[1], "_C_benchmarking", ["-DHTGS_BINDINGS_BENCHMARKING"])):
-        if force or _stale(target, [BINDINGS_SRC, os.path.join(CSRC, "bindings_sequence.h"), lib, os.path.normpath(os.path.join(CSRC, "..", "..", "include", "htgs_b200.h"))]):
+        if force or _stale(target, [BINDINGS_SRC, os.path.join(CSRC, "bindings_sequence.h"), os.path.join(CSRC, "bindings_attention.h"), lib, os.path.normpath(os.path.join(CSRC, "..", "..", "include", "htgs_b200.h"))]):
             jobs.append((name, [cxx] + flags + extra + [f"-DTORCH_EXTENSION_NAME={name}"] + [f"-I{d}" for d in includes] + [BINDINGS_SRC, "-o", target] + link))
     if jobs:
         os.makedirs(PYBIND_DIR, exist_ok=True)

@@ -1,0 +1,293 @@
+// Attention over packed sequences: the entry points, the statistics of the backward pass, and kernels for what the tensor cores' (attention_tiles.cu) do not take: 32-bit
+// values, widths that are no multiple of 8, rows that do not begin on 16 bytes.
+#include "attention.cuh"
+
+namespace htgs {
+
+namespace {
+
+constexpr int kLanesThreads = 256, kLanesRows = 32, kRowsOfWarp = 4, kMostWidth = 128, kColumns = kMostWidth / 32;
+
+// rows first + [0, 32) of a head into shared memory, zeros where there is none.
+template <typename T> __device__ __forceinline__ void fill_rows(float* to, int pitch, const void* from, int64_t stride, int64_t offset, int first, int end, int width) {
+    const T* p = static_cast<const T*>(from) + offset;
+    for (int r = threadIdx.x / 32; r < kLanesRows; r += kLanesThreads / 32)
+        for (int c = threadIdx.x & 31; c < width; c += 32) to[r * pitch + c] = first + r < end ? to_float<T>(p[(first + r) * stride + c]) : 0.0f;
+}
+template <typename T> __device__ __forceinline__ void store_row(T* to, const float (&v)[kColumns], float factor, int width, int lane) {
+    #pragma unroll
+    for (int i = 0; i < kColumns; ++i)
+        if (lane + 32 * i < width) to[lane + 32 * i] = from_float<T>(v[i] * factor);
+}
+
+// 32 rows of a head, four to a warp, against 32 rows at a time of those that they see, a lane for each.  Values that a row does not see meet nothing of it: neither its sums nor, by a
+// product with zero, its output.  Bound by loads from shared memory: five for four multiply-adds.
+template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention_lanes_kernel(const HtgsAttention a, T* out, float* sums) {
+    extern __shared__ float shared[];
+    grid_dependency();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, pitch = a.width | 1;
+    const int head = int(blockIdx.x % a.heads), key_head = head / (a.heads / a.key_heads);
+    const SequenceTile t = find_tile<kLanesRows>(a, int(blockIdx.x / a.heads));
+    if (t.first >= t.end) return;
+    float *const qs = shared, *const ks = qs + kLanesRows * pitch, *const vs = ks + kLanesRows * pitch;
+    const int rows = min(kLanesRows, t.end - t.first);
+    float m[kRowsOfWarp], l[kRowsOfWarp] = {}, o[kRowsOfWarp][kColumns] = {};
+    #pragma unroll
+    for (int r = 0; r < kRowsOfWarp; ++r) m[r] = -infinity();
+    if (!t.outside) {
+        fill_rows<T>(qs, pitch, a.q, a.q_stride, head * a.q_head_stride, t.first, t.end, a.width);
+        const float scale = a.scale * kLog2e;
+        const int low = first_seen(a, t.begin, t.first), high = last_seen(a, t.end, t.first + rows - 1);
+        for (int at = low; at <= high; at += kLanesRows) {
+            __syncthreads();
+            fill_rows<T>(ks, pitch, a.k, a.k_stride, key_head * a.k_head_stride, at, high + 1, a.width);
+            fill_rows<T>(vs, pitch, a.v, a.v_stride, key_head * a.v_head_stride, at, high + 1, a.width);
+            __syncthreads();
+            float s[kRowsOfWarp] = {};
+            for (int c = 0; c < a.width; ++c) {
+                const float k = ks[lane * pitch + c];
+                #pragma unroll
+                for (int r = 0; r < kRowsOfWarp; ++r) s[r] = fmaf(qs[(warp * kRowsOfWarp + r) * pitch + c], k, s[r]);
+            }
+            uint32_t seen[kRowsOfWarp];
+            #pragma unroll
+            for (int r = 0; r < kRowsOfWarp; ++r) {
+                const int i = t.first + warp * kRowsOfWarp + r, j = at + lane;
+                const bool sees = i < t.end && j >= first_seen(a, t.begin, i) && j <= last_seen(a, t.end, i);
+                seen[r] = __ballot_sync(0xffffffffu, sees);
+                const float x = sees ? s[r] * scale : -infinity(), most = fmaxf(m[r], lanes_max<32>(x)), base = most == -infinity() ? 0.0f : most, factor = exp2_approx(m[r] - base);
+                m[r] = most;
+                s[r] = exp2_approx(x - base);
+                l[r] = l[r] * factor + warp_sum(s[r]);
+                #pragma unroll
+                for (int i2 = 0; i2 < kColumns; ++i2) o[r][i2] *= factor;
+            }
+            for (int j = 0; j < kLanesRows; ++j) {
+                float v[kColumns];
+                #pragma unroll
+                for (int i = 0; i < kColumns; ++i) v[i] = lane + 32 * i < a.width ? vs[j * pitch + lane + 32 * i] : 0.0f;
+                #pragma unroll
+                for (int r = 0; r < kRowsOfWarp; ++r) {
+                    const float p = __shfl_sync(0xffffffffu, s[r], j);
+                    if (!(seen[r] >> j & 1)) continue;
+                    #pragma unroll
+                    for (int i = 0; i < kColumns; ++i) o[r][i] = fmaf(p, v[i], o[r][i]);
+                }
+            }
+        }
+    }
+    #pragma unroll
+    for (int r = 0; r < kRowsOfWarp; ++r) {
+        const int i = t.first + warp * kRowsOfWarp + r;
+        if (i >= t.end) break;
+        store_row<T>(out + (int64_t(i) * a.heads + head) * a.width, o[r], t.outside ? 0.0f : 1.0f / l[r], a.width, lane);
+        if (sums && lane == 0) sums[head * a.rows + i] = t.outside ? 0.0f : m[r] + log2f(l[r]);
+    }
+}
+
+// {log2 of the sum, D} of the rows of a tile of 128 and a head; rows that are not there get an infinite sum, which makes their weights zero.
+template <typename T> __global__ void __launch_bounds__(kLanesThreads) statistics_kernel(const HtgsAttention a, const T* out, const float* sums, const T* grad, int64_t grad_stride, int64_t grad_head_stride,
+                                                                                        float2* statistics, int64_t statistics_rows) {
+    grid_dependency();
+    const int lane = threadIdx.x & 31, head = int(blockIdx.x % a.heads);
+    const SequenceTile t = find_tile<kStatisticRows>(a, int(blockIdx.x / a.heads));
+    if (t.first >= t.end) return;
+    float2* to = statistics + head * statistics_rows + statistic_base(a, t) + (t.first - t.begin);
+    for (int r = threadIdx.x / 32; r < kStatisticRows; r += kLanesThreads / 32) {
+        const int64_t i = t.first + r;
+        float sum = 0.0f;
+        if (i < t.end && !t.outside)
+            for (int c = lane; c < a.width; c += 32) sum = fmaf(to_float<T>(out[(i * a.heads + head) * a.width + c]), to_float<T>(grad[i * grad_stride + head * grad_head_stride + c]), sum);
+        sum = warp_sum(sum);
+        if (lane == 0) to[r] = i < t.end && !t.outside ? make_float2(sums[head * a.rows + i], sum) : make_float2(infinity(), 0.0f);
+    }
+}
+
+// Gradients of 32 rows of q and a head (KEYS false), or of k, v and a key head, over its query heads, against 32 rows at a time of the others, a lane for each.
+template <typename T, bool KEYS> __global__ void __launch_bounds__(kLanesThreads) attention_lanes_backward_kernel(const HtgsAttention a, const AttentionBackward b) {
+    extern __shared__ float shared[];
+    __shared__ float2 statistics[kLanesRows];
+    grid_dependency();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, pitch = a.width | 1, group = a.heads / a.key_heads, own_heads = KEYS ? a.key_heads : a.heads;
+    const int own_head = int(blockIdx.x % own_heads);
+    const SequenceTile t = find_tile<kLanesRows>(a, int(blockIdx.x / own_heads));
+    if (t.first >= t.end) return;
+    float *const own1 = shared, *const own2 = own1 + kLanesRows * pitch, *const other1 = own2 + kLanesRows * pitch, *const other2 = other1 + kLanesRows * pitch;
+    const int rows = min(kLanesRows, t.end - t.first);
+    const int64_t base = statistic_base(a, t);
+    const float scale = a.scale * kLog2e;
+    float first[kRowsOfWarp][kColumns] = {}, second[kRowsOfWarp][kColumns] = {};        // of q or k; of v
+    if (!t.outside) {
+        const int key_head = KEYS ? own_head : own_head / group;
+        const auto fill_queries = [&](float* q, float* grad, int head, int at, int end) {
+            fill_rows<T>(q, pitch, a.q, a.q_stride, head * a.q_head_stride, at, end, a.width);
+            fill_rows<T>(grad, pitch, b.grad, b.grad_stride, head * b.grad_head_stride, at, end, a.width);
+            if (threadIdx.x < kLanesRows && at + int(threadIdx.x) < end) statistics[threadIdx.x] = b.statistics[head * b.statistics_rows + base + (at - t.begin) + threadIdx.x];
+        };
+        const auto fill_keys = [&](float* k, float* v, int at, int end) {
+            fill_rows<T>(k, pitch, a.k, a.k_stride, key_head * a.k_head_stride, at, end, a.width);
+            fill_rows<T>(v, pitch, a.v, a.v_stride, key_head * a.v_head_stride, at, end, a.width);
+        };
+        if (KEYS) fill_keys(own1, own2, t.first, t.end);
+        else fill_queries(own1, own2, own_head, t.first, t.end);
+        const int low = KEYS ? first_seeing(a, t.begin, t.first) : first_seen(a, t.begin, t.first);
+        const int high = KEYS ? last_seeing(a, t.end, t.first + rows - 1) : last_seen(a, t.end, t.first + rows - 1);
+        for (int head = KEYS ? own_head * group : own_head; head < (KEYS ? (own_head + 1) * group : own_head + 1); ++head) {
+            for (int at = low; at <= high; at += kLanesRows) {
+                __syncthreads();
+                if (KEYS) fill_queries(other1, other2, head, at, high + 1);
+                else fill_keys(other1, other2, at, high + 1);
+                __syncthreads();
+                float s[kRowsOfWarp] = {}, ds[kRowsOfWarp] = {};
+                for (int c = 0; c < a.width; ++c) {
+                    const float x = other1[lane * pitch + c], y = other2[lane * pitch + c];
+                    #pragma unroll
+                    for (int r = 0; r < kRowsOfWarp; ++r) {
+                        s[r] = fmaf(own1[(warp * kRowsOfWarp + r) * pitch + c], x, s[r]);
+                        ds[r] = fmaf(own2[(warp * kRowsOfWarp + r) * pitch + c], y, ds[r]);
+                    }
+                }
+                uint32_t seen[kRowsOfWarp];
+                #pragma unroll
+                for (int r = 0; r < kRowsOfWarp; ++r) {
+                    const int own = t.first + warp * kRowsOfWarp + r, i = KEYS ? at + lane : own, j = KEYS ? own : at + lane;
+                    const bool sees = i < t.end && j < t.end && j >= first_seen(a, t.begin, i) && j <= last_seen(a, t.end, i);
+                    seen[r] = __ballot_sync(0xffffffffu, sees);
+                    const float2 st = sees ? statistics[KEYS ? lane : warp * kRowsOfWarp + r] : make_float2(0.0f, 0.0f);
+                    s[r] = sees ? exp2_approx(fmaf(s[r], scale, -st.x)) : 0.0f;
+                    ds[r] = sees ? s[r] * (ds[r] - st.y) : 0.0f;
+                }
+                for (int j = 0; j < kLanesRows; ++j) {
+                    float x[kColumns], y[kColumns];
+                    #pragma unroll
+                    for (int i = 0; i < kColumns; ++i) {
+                        x[i] = lane + 32 * i < a.width ? other1[j * pitch + lane + 32 * i] : 0.0f;
+                        if (KEYS) y[i] = lane + 32 * i < a.width ? other2[j * pitch + lane + 32 * i] : 0.0f;
+                    }
+                    #pragma unroll
+                    for (int r = 0; r < kRowsOfWarp; ++r) {
+                        const float w = __shfl_sync(0xffffffffu, ds[r], j), p = KEYS ? __shfl_sync(0xffffffffu, s[r], j) : 0.0f;
+                        if (!(seen[r] >> j & 1)) continue;
+                        #pragma unroll
+                        for (int i = 0; i < kColumns; ++i) {
+                            first[r][i] = fmaf(w, x[i], first[r][i]);
+                            if (KEYS) second[r][i] = fmaf(p, y[i], second[r][i]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    #pragma unroll
+    for (int r = 0; r < kRowsOfWarp; ++r) {
+        const int i = t.first + warp * kRowsOfWarp + r;
+        if (i >= t.end) break;
+        const int64_t at = (int64_t(i) * own_heads + own_head) * a.width;
+        store_row<T>(static_cast<T*>(KEYS ? b.grad_k : b.grad_q) + at, first[r], a.scale, a.width, lane);
+        if (KEYS) store_row<T>(static_cast<T*>(b.grad_v) + at, second[r], 1.0f, a.width, lane);
+    }
+}
+
+template <typename T, typename Kernel, typename... Args>
+int launch_lanes(Kernel kernel, PerDeviceOnce& once, const HtgsAttention& a, int heads, int buffers, cudaStream_t stream, const Args&... args) {
+    const int most = buffers * kLanesRows * (kMostWidth | 1) * int(sizeof(float));
+    cudaError_t err = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most); });
+    if (err == cudaSuccess)
+        err = launch_after(kernel, dim3(unsigned(sequence_tiles(a, kLanesRows) * heads)), kLanesThreads, size_t(buffers) * kLanesRows * (a.width | 1) * sizeof(float), stream, a, args...);
+    return err == cudaSuccess ? sequence_status("htgs_attention") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
+
+template <typename T> int forward_lanes(const HtgsAttention& a, void* out, float* sums, cudaStream_t stream) {
+    static PerDeviceOnce once;
+    return launch_lanes<T>(attention_lanes_kernel<T>, once, a, a.heads, 3, stream, static_cast<T*>(out), sums);
+}
+template <typename T> int backward_lanes(const HtgsAttention& a, const AttentionBackward& b, cudaStream_t stream) {
+    static PerDeviceOnce once, once_keys;
+    const int code = launch_lanes<T>(attention_lanes_backward_kernel<T, false>, once, a, a.heads, 4, stream, b);
+    return code != HTGS_OK ? code : launch_lanes<T>(attention_lanes_backward_kernel<T, true>, once_keys, a, a.key_heads, 4, stream, b);
+}
+template <typename T> int launch_statistics(const HtgsAttention& a, const void* out, const float* sums, const AttentionBackward& b, float2* statistics, cudaStream_t stream) {
+    const cudaError_t err = launch_after(statistics_kernel<T>, dim3(unsigned(sequence_tiles(a, kStatisticRows) * a.heads)), kLanesThreads, 0, stream, a, static_cast<const T*>(out), sums,
+                                         static_cast<const T*>(b.grad), b.grad_stride, b.grad_head_stride, statistics, b.statistics_rows);
+    return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
+
+ErrorWords& error_words() {
+    static ErrorWords words;
+    return words;
+}
+int reported(unsigned int* word) { return htgs::reported(word, "htgs_attention: a wait in an earlier call on this device ran out, and its result is not complete"); }
+
+// What a call may not be; nullptr if all is well.
+const char* wrong(const HtgsAttention* a) {
+    if (!a) return "htgs_attention: no arguments";
+    if (!known_type(a->type)) return "htgs_attention: unknown element type";
+    if (a->rows < 0 || a->rows > 0x7fffff00 || a->n_sequences < 1 || a->n_sequences > 0x7fffff00) return "htgs_attention: rows and n_sequences must be below 2^31 - 256, and n_sequences at least 1";
+    if (!a->offsets && a->rows % a->n_sequences) return "htgs_attention: rows must be a multiple of n_sequences where there are no offsets";
+    if (a->key_heads < 1 || a->heads < 1 || a->heads % a->key_heads || a->heads > 65536) return "htgs_attention: heads must be a multiple of key_heads, at most 65536";
+    if (a->width < 1 || a->width > kMostWidth) return "htgs_attention: heads must be 1 to 128 values wide";
+    if (!(a->scale > 0.0f && a->scale <= FLT_MAX)) return "htgs_attention: scale must be positive and finite";
+    if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0 || a->q_head_stride < 0 || a->k_head_stride < 0 || a->v_head_stride < 0) return "htgs_attention: strides must not be negative";
+    if (a->rows && (!a->q || !a->k || !a->v)) return "htgs_attention: q, k and v must not be null";
+    if (sequence_tiles(*a, kLanesRows) * a->heads > 0x7fffffff) return "htgs_attention: too many rows and heads for one call";
+    return nullptr;
+}
+
+}  // namespace
+
+unsigned int* attention_error_word(int device) { return error_words().of(device); }
+
+}  // namespace htgs
+
+extern "C" {
+
+unsigned int* htgs_attention_error_word(int32_t device) { return htgs::attention_error_word(device); }
+
+int htgs_attention_status(int32_t device) {
+    using namespace htgs;
+    if (device < 0 || device >= ErrorWords::kMostDevices) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_attention_status: no such device");
+    return reported(attention_error_word(device));
+}
+
+int htgs_attention(const HtgsAttention* attention, void* out, float* sums, void* stream) {
+    using namespace htgs;
+    if (const char* message = wrong(attention)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
+    if (attention->rows == 0) return HTGS_OK;
+    if (!out) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_attention: out must not be null");
+    if (const int code = reported(attention_error_word(current_device())); code != HTGS_OK) return code;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const HtgsAttention& a = *attention;
+    if (a.type == HTGS_FLOAT32) return forward_lanes<float>(a, out, sums, s);
+    if (a.type == HTGS_FLOAT16) return forward_lanes<__half>(a, out, sums, s);
+    return forward_lanes<__nv_bfloat16>(a, out, sums, s);
+}
+
+size_t htgs_attention_backward_workspace_bytes(const HtgsAttention* attention) {
+    using namespace htgs;
+    if (wrong(attention) || attention->rows == 0) return 0;
+    return size_t(statistic_rows(*attention)) * attention->heads * sizeof(float2);
+}
+
+int htgs_attention_backward(const HtgsAttention* attention, const void* out, const float* sums, const void* grad_out, int64_t grad_out_stride, int64_t grad_out_head_stride,
+                            void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace htgs;
+    if (const char* message = wrong(attention)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
+    if (attention->rows == 0) return HTGS_OK;
+    if (!out || !sums || !grad_out || !grad_q || !grad_k || !grad_v) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_attention_backward: no pointer may be null");
+    if (grad_out_stride < 0 || grad_out_head_stride < 0) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_attention_backward: strides must not be negative");
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < htgs_attention_backward_workspace_bytes(attention))
+        return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_attention_backward: the workspace is too small or not on 16 bytes");
+    if (const int code = reported(attention_error_word(current_device())); code != HTGS_OK) return code;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const HtgsAttention& a = *attention;
+    float2* statistics = static_cast<float2*>(workspace);
+    const AttentionBackward b{grad_out, grad_out_stride, grad_out_head_stride, grad_q, grad_k, grad_v, statistics, statistic_rows(a)};
+    int code = a.type == HTGS_FLOAT32 ? launch_statistics<float>(a, out, sums, b, statistics, s)
+               : a.type == HTGS_FLOAT16 ? launch_statistics<__half>(a, out, sums, b, statistics, s) : launch_statistics<__nv_bfloat16>(a, out, sums, b, statistics, s);
+    if (code != HTGS_OK) return code;
+    if (a.type == HTGS_FLOAT32) return backward_lanes<float>(a, b, s);
+    if (a.type == HTGS_FLOAT16) return backward_lanes<__half>(a, b, s);
+    return backward_lanes<__nv_bfloat16>(a, b, s);
+}
+
+}  // extern "C"

@@ -22,7 +22,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -411,7 +413,7 @@ struct ReadyEvent {     // what `torch.cuda.Stream.wait_event` needs: an object 
     void synchronize() const { event->synchronize(); }
 };
 
-#include "bindings_sequence.h"
+#include "bindings_attention.h"
 
 #endif  // !HTGS_BINDINGS_BENCHMARKING
 
@@ -466,5 +468,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return out;
     }, py::arg("device") = -1);
     sequence::define(m);
+    sequence::define_attention(m);
 #endif
 }

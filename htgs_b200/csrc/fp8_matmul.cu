@@ -7,11 +7,7 @@
 //
 // Up to eight rows: `matmul_rows_kernel`, a warp per row of b.  Otherwise `matmul_tiles_kernel` on the tensor cores, which take the scales themselves (kind::mxf8f6f4, one scale
 // per row and 32 columns; a block of 128 uses the same one four times).
-#include "sequence.cuh"
-
-#include <cuda.h>
-
-#include <cstring>
+#include "tensor_core.cuh"
 
 namespace htgs {
 
@@ -150,7 +146,6 @@ constexpr int kSms = 148;
 constexpr int kMostParts = 8;
 constexpr int kTileThreads = 384;
 constexpr int kAccumulators = 2, kScaleStages = 4, kScaleColumns = 12;       // 4 columns of a's scales and up to 8 of b's
-constexpr uint64_t kWaitNanoseconds = 2000000000ull;
 
 enum TileMode { kSingle, kSplit, kPair };
 
@@ -182,36 +177,6 @@ struct TileArgs {
     unsigned int* error;
 };
 
-__device__ __forceinline__ uint64_t nanoseconds() { uint64_t t; asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t)); return t; }
-
-__device__ __forceinline__ void arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// False if the time limit ran out or another role has given up.  Out of line: the roles' loops are single threads whose every instruction counts.
-__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-    WaitLimit limit(kWaitNanoseconds, nanoseconds());
-    for (;;) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
-        if (*failed) return false;
-        if (limit.over(nanoseconds())) { *failed = 1; return false; }
-    }
-}
-__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
-    return mbar_try_wait(bar, parity) || wait_longer(smem_u32(bar), parity, failed);
-}
-__device__ __forceinline__ bool elect_one() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-    return one != 0;
-}
-// A place in a ring of N, and the parity of the round it is in.
-template <int N> struct Ring {
-    uint32_t at = 0, round = 0;
-    __device__ __forceinline__ void next() { if (++at == N) { at = 0; round ^= 1; } }
-};
-
 __device__ __forceinline__ void arrive_there(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 // `bar`: in a pair, a barrier of the first block.
@@ -224,8 +189,6 @@ template <int MODE> __device__ __forceinline__ void tma_load(void* to, const CUt
                      ::"r"(smem_u32(to)), "l"(map), "r"(column), "r"(row), "r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // An arrival, once the instructions so far are done; in a pair at both blocks' barriers.
 template <int MODE> __device__ __forceinline__ void tmem_commit(uint64_t* bar) {
     if constexpr (MODE == kPair)
@@ -236,16 +199,6 @@ template <int MODE> __device__ __forceinline__ void tmem_commit(uint64_t* bar) {
 __device__ __forceinline__ void tmem_store4(uint32_t address, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&v)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-                   "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-                 : "r"(address));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 // Shared-memory operands: rows of 128 bytes under the 128-byte swizzle, groups of 8 rows 1024 bytes apart (the leading offset says nothing there).  The
 // lower word of a descriptor has the address in units of 16 bytes, the upper one is the same for all.
 constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
@@ -572,19 +525,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) matmul_tiles_kernel(const __g
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled() {
-    static const EncodeTiled found = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult result;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &result) != cudaSuccess || result != cudaDriverEntryPointSuccess) f = nullptr;
-        return reinterpret_cast<EncodeTiled>(f);
-    }();
-    return found;
-}
-
 bool make_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, int64_t columns, int64_t rows, int64_t stride_bytes, int box_columns,
               int box_rows) {
     const cuuint64_t sizes[2] = {cuuint64_t(columns), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride_bytes)};
@@ -601,37 +541,12 @@ template <typename T> bool make_out_map(CUtensorMap* map, const MatmulArgs& m) {
                     m.out, m.b.rows, m.a.rows, m.out_stride * int64_t(sizeof(T)), kPatch, kPatch);
 }
 
-// A word for each device in the host's memory, which a kernel sets when one of its waits runs out.  The next product on that device reports it, or who asks.
-constexpr int kMostDevices = 64;
-unsigned int* error_words() {
-    static unsigned int* const words = [] {
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;       // the first call may be inside a capture
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        void* p = nullptr;
-        if (cudaHostAlloc(&p, kMostDevices * sizeof(unsigned int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
-            p = nullptr;
-            cudaGetLastError();
-        }
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        if (p) std::memset(p, 0, kMostDevices * sizeof(unsigned int));
-        return static_cast<unsigned int*>(p);
-    }();
+ErrorWords& error_words() {
+    static ErrorWords words;
     return words;
 }
-unsigned int* error_word(int device) {
-    unsigned int* const words = error_words();
-    return words && device >= 0 && device < kMostDevices ? words + device : nullptr;
-}
-int current_device() {
-    int device = -1;
-    cudaGetDevice(&device);
-    return device;
-}
-// What a word says, once: whoever reads it first clears it.
-int reported(unsigned int* word) {
-    if (!word || !__atomic_load_n(word, __ATOMIC_RELAXED) || !__atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL)) return HTGS_OK;
-    return sequence_fail(HTGS_ERR_DEVICE_FLAG, "htgs_fp8_matmul: a wait in an earlier product on this device ran out, and its result is not complete");
-}
+unsigned int* error_word(int device) { return error_words().of(device); }
+int reported(unsigned int* word) { return htgs::reported(word, "htgs_fp8_matmul: a wait in an earlier product on this device ran out, and its result is not complete"); }
 
 // parts: blocks of a cluster (kSplit), else the mode's own number.
 template <typename T, int BN, int MODE> int launch_tiles(const MatmulArgs& m, int parts, cudaStream_t stream) {
@@ -705,7 +620,7 @@ unsigned int* htgs_fp8_matmul_error_word(int32_t device) { return htgs::error_wo
 
 int htgs_fp8_matmul_status(int32_t device) {
     using namespace htgs;
-    if (device < 0 || device >= kMostDevices) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_status: no such device");
+    if (device < 0 || device >= ErrorWords::kMostDevices) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_fp8_matmul_status: no such device");
     return reported(error_word(device));
 }
 

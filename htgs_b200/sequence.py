@@ -5,6 +5,9 @@ each Gaussian in the order of a space-filling curve, 10^5 to 10^6 rows long.
 * `quantize_fp8`, `Fp8Matrix`          - 8-bit matrices with a power-of-two scale for each block of 128
 * `fp8_matmul`, `fp8_linear`           - their matrix product; the second is differentiable and quantises its operands itself; `check_products` asks after their errors
 * `gated_scan`, `gated_scan_step`      - gated linear recurrence over whole sequences (differentiable), and one step of it
+* `rotary`                             - rotary positions with several axes, such as a Gaussian's place in space (differentiable)
+* `attention`, `attention_step`        - attention over whole sequences, causal or within a window or neither (differentiable), and one more row over a cache;
+                                         `check_attention` asks after its errors
 
 Values are float32, float16 or bfloat16; sums, statistics and states are 32-bit.  Everything is queued on the current CUDA stream without a
 host wait, can be captured in a CUDA graph, and gives the same bits for the same inputs.  There is no CPU fallback.  Derivatives
@@ -14,14 +17,16 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Optional, Tuple
+import operator
+from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import _native
-from ._native import HtgsFp8Matrix, HtgsScan
+from ._native import HtgsAttention, HtgsAttentionStep, HtgsFp8Matrix, HtgsRotary, HtgsScan
 
-__all__ = ["add_rms_norm", "add_rms_norm_fp8", "Fp8Matrix", "quantize_fp8", "fp8_matmul", "fp8_linear", "check_products", "gated_scan", "gated_scan_step"]
+__all__ = ["add_rms_norm", "add_rms_norm_fp8", "Fp8Matrix", "quantize_fp8", "fp8_matmul", "fp8_linear", "check_products", "gated_scan", "gated_scan_step",
+           "rotary", "attention", "attention_step", "check_attention"]
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _BLOCK = 128
@@ -507,3 +512,258 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) ->
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)        # autograd learns of it; what inference mode made is kept by no gradient
     return h
+
+
+# ---- rotary positions --------------------------------------------------------------------------------------------------------------
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """`t` as [rows, heads, width]; a copy only where a head's values are not dense, rows or heads lie on one another, or 16-bit heads that could begin on 16 bytes do not."""
+    if t.dim() != 3:
+        t = t.reshape(t.shape[:-2].numel(), *t.shape[-2:])
+    rows, heads, width = t.shape
+    fits = (width == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) >= 1) and (rows == 1 or t.stride(0) >= 1)
+    if fits and t.element_size() == 2 and width % 8 == 0:
+        fits = t.data_ptr() % 16 == 0 and (heads == 1 or t.stride(1) % 8 == 0) and (rows == 1 or t.stride(0) % 8 == 0)
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
+
+
+def _sections(sections, axes: int, width: int):
+    pairs = width // 2
+    if sections is None:
+        return [pairs // axes + (axis < pairs % axes) for axis in range(axes)]
+    sections = [int(n) for n in sections]
+    if len(sections) != axes or min(sections) < 0 or sum(sections) != pairs:
+        raise ValueError(f"sections must hold the pairs of each of {axes} axes, {pairs} in all")
+    return sections
+
+
+def _turn(tensors, positions, sections, base, interleaved, inverse):
+    """One or two tensors [rows, heads, width] turned, dense."""
+    rows, _, width = tensors[0].shape
+    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    r = HtgsRotary()
+    for i, (x, y) in enumerate(zip(tensors, out)):
+        r.x[i], r.y[i], r.x_stride[i], r.x_head_stride[i], r.heads[i] = x.data_ptr(), y.data_ptr(), x.stride(0), x.stride(1), x.shape[1]
+    for i, n in enumerate(sections):
+        r.sections[i] = n
+    r.positions, r.positions_stride, r.rows, r.base = positions.data_ptr(), positions.stride(0), rows, base
+    r.axes, r.positions_type, r.width, r.type = len(sections), int(positions.dtype == torch.int32), width, _TYPES[tensors[0].dtype]
+    r.interleaved, r.inverse = int(interleaved), int(inverse)
+    _call(out[0].device, "htgs_rotary", ctypes.byref(r))
+    return out
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, *rest):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.rest = rest
+        tensors = [t for t in (q, k) if t is not None]
+        out = [y.view(t.shape) for y, t in zip(_turn([_heads(t) for t in tensors], positions, *rest, False), tensors)]
+        return tuple(out) if k is not None else out[0]
+
+    @staticmethod
+    @_first_derivative
+    def backward(ctx, *grads):
+        (positions,) = ctx.saved_tensors
+        there = [g for g in grads if g is not None]
+        out = iter(_turn([_heads(g) for g in there], positions, *ctx.rest, True)) if there else iter(())
+        turned = [None if g is None else next(out).view(g.shape) for g in grads]
+        return (*turned, *(None,) * (3 - len(turned) + len(ctx.rest)))
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, sections: Optional[Sequence[int]] = None, base: float = 10000.0,
+           interleaved: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(q, k) with each head's pairs of values turned by angles that grow with the row's position, so that a product of q and k goes by the difference of their positions.
+
+    q is [..., rows, heads, width] and k (or None) [..., rows, key_heads, width], width even, up to 256; `positions` [..., rows, axes], float32 or int32 with 1 to 4 axes,
+    such as the places of Gaussians.  `sections` is the number of pairs that each axis turns (default: evenly, the first axes one more where that does not come out);
+    the i-th of an axis's n pairs turns by position * base^(-i / n).  Pair j is (j, j + width / 2), or (2 j, 2 j + 1) if `interleaved`.  Angles are computed in 64 bits, so
+    far positions keep theirs.  Differentiable in q and k, not in the positions."""
+    compiled = _compiled()
+    if compiled:
+        return compiled.rotary(q, k, positions, None if sections is None else [int(n) for n in sections], float(base), bool(interleaved))
+    _check(q, "q")
+    if q.dim() < 3 or q.shape[-1] % 2 or not 2 <= q.shape[-1] <= 256 or q.shape[-2] < 1:
+        raise ValueError("q must have shape [..., rows, heads, width], width even and 2 to 256")
+    if k is not None:
+        _check(k, "k", q.dtype, q.device)
+        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.shape[-2] < 1:
+            raise ValueError(f"k must have the rows and width of q, {tuple(q.shape)}, got {tuple(k.shape)}")
+    if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int32:
+        _check(positions, "positions", torch.float32, q.device)
+    else:
+        _check(positions, "positions", torch.int32, q.device)
+    if positions.dim() != q.dim() - 1 or positions.shape[:-1] != q.shape[:-2] or not 1 <= positions.shape[-1] <= 4:
+        raise ValueError("positions must have shape [..., rows, axes], the rows of q and 1 to 4 axes")
+    sections = _sections(sections, positions.shape[-1], q.shape[-1])
+    base = float(base)
+    if not 0.0 < base < float("inf"):
+        raise ValueError("base must be positive and finite")
+    _no_tangent(q, k, positions)
+    if _wants_grad(positions):
+        raise RuntimeError("rotary has no gradient with respect to positions: detach them")
+    positions = _rows(positions)
+    tensors = [t for t in (q, k) if t is not None]
+    if _wants_grad(*tensors):
+        out = _Rotary.apply(q, k, positions, sections, base, bool(interleaved))
+        return out if k is not None else (out, None)
+    out = [y.view(t.shape) for y, t in zip(_turn([_heads(t) for t in tensors], positions, sections, base, interleaved, False), tensors)]
+    return out[0], out[1] if k is not None else None
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------------
+
+
+def _window(window) -> int:
+    if window is None:
+        return -1
+    window = operator.index(window)
+    if window < 0:
+        raise ValueError("window must not be negative")
+    return min(window, 0x7fffffff)
+
+
+def _scale(scale, width: int) -> float:
+    scale = width ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
+    return scale
+
+
+def _attention_struct(q, k, v, offsets, sequences, causal, window, scale) -> HtgsAttention:
+    return HtgsAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), None if offsets is None else offsets.data_ptr(), q.stride(0), k.stride(0), v.stride(0), q.stride(1), k.stride(1),
+                         v.stride(1), q.shape[0], q.shape[1], k.shape[1], q.shape[2], sequences, _TYPES[q.dtype], int(causal), window, scale)
+
+
+def _attend(q, k, v, rest, keep):
+    """(out, sums or None) for tensors [rows, heads, width]."""
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    sums = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if keep else None
+    _call(q.device, "htgs_attention", ctypes.byref(_attention_struct(q, k, v, *rest)), out.data_ptr(), None if sums is None else sums.data_ptr())
+    return out, sums
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, *rest):
+        qh, kh, vh = _heads(q), _heads(k), _heads(v)
+        out, sums = _attend(qh, kh, vh, rest, True)
+        ctx.save_for_backward(qh, kh, vh, out, sums, rest[0])
+        ctx.rest, ctx.shapes = rest[1:], (q.shape, k.shape, v.shape)
+        return out.view(q.shape)
+
+    @staticmethod
+    @_first_derivative
+    def backward(ctx, grad):
+        q, k, v, out, sums, offsets = ctx.saved_tensors
+        grad = _heads(grad)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+        struct = _attention_struct(q, k, v, offsets, *ctx.rest)
+        size = _native.lib().htgs_attention_backward_workspace_bytes(ctypes.byref(struct))
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        _call(q.device, "htgs_attention_backward", ctypes.byref(struct), out.data_ptr(), sums.data_ptr(), grad.data_ptr(), grad.stride(0), grad.stride(1),
+              *(g.data_ptr() for g in grads), workspace.data_ptr(), size)
+        return (*(g.view(shape) for g, shape in zip(grads, ctx.shapes)), *(None,) * (1 + len(ctx.rest)))
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Optional[torch.Tensor] = None, causal: bool = False, window: Optional[int] = None,
+              scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale * q k^T) v over each row's sequence: with `causal` over the rows up to its own, with `window` over rows at most so many before or behind.
+
+    q is [rows, heads, width] and k and v [rows, key_heads, width] (one sequence, or with `offsets` several behind one another), or all with a batch in front; a key head serves
+    heads / key_heads neighbouring heads; width is 1 to 128, scale by default width^-0.5.  `offsets` is an int32 tensor of ascending row numbers that begin the sequences
+    (sequences may be empty; rows of none, before the first and behind the last, get zeros).  Views such as the parts of one projection are read in place.  Scores and sums are
+    32-bit.  float16 and bfloat16 with a width that is a multiple of 8 run on the tensor cores; float32 and other widths do not and are much slower.  What a row does not see never reaches
+    its result, not even infinities and NaN.  Differentiable in q, k and v."""
+    compiled = _compiled()
+    if compiled:
+        return compiled.attention(q, k, v, offsets, bool(causal), None if window is None else operator.index(window), None if scale is None else float(scale))
+    _check(q, "q")
+    _check(k, "k", q.dtype, q.device)
+    _check(v, "v", q.dtype, q.device)
+    if q.dim() not in (3, 4) or not 1 <= q.shape[-1] <= 128 or q.shape[-2] < 1:
+        raise ValueError("q must have shape [rows, heads, width] or [batch, rows, heads, width], width 1 to 128")
+    if k.shape != v.shape or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.shape[-2] < 1 or q.shape[-2] % k.shape[-2]:
+        raise ValueError(f"k and v must have one shape, the rows and width of q, {tuple(q.shape)}, and a number of heads that divides q's")
+    if offsets is not None:
+        _check(offsets, "offsets", torch.int32, q.device)
+        if q.dim() != 3 or offsets.dim() != 1 or offsets.numel() < 2:
+            raise ValueError("offsets must hold sequences + 1 row numbers, for q of shape [rows, heads, width]")
+        offsets = offsets.contiguous()
+    sequences = q.shape[0] if q.dim() == 4 else 1 if offsets is None else offsets.numel() - 1
+    rest = (offsets, sequences, bool(causal), _window(window), _scale(scale, q.shape[-1]))
+    _no_tangent(q, k, v)
+    if q.numel() == 0:
+        return q * 1
+    if _wants_grad(q, k, v):
+        return _Attention.apply(q, k, v, *rest)
+    return _attend(_heads(q), _heads(k), _heads(v), rest, False)[0].view(q.shape)
+
+
+def check_attention(device: Optional[torch.device] = None) -> None:
+    """`check_products` for `attention`: raises if a call on `device` (default: the current one) gave up on a wait of its kernel, so that its result is not complete."""
+    index = None if device is None else torch.device(device).index
+    _native.check(_native.lib().htgs_attention_status(torch.cuda.current_device() if index is None else index))
+
+
+def _check_cache(t: torch.Tensor, name: str, shape) -> None:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape [batch, capacity, key_heads, width], {tuple(shape)}, got {tuple(t.shape)}")
+    extent = 0
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= extent:
+            raise ValueError(f"{name} must not have places that are one in memory: it is updated in place")
+        extent += stride * (size - 1)
+    if t.stride(3) != 1 and t.shape[3] != 1:
+        raise ValueError(f"{name} must have dense heads: it is updated in place")
+
+
+def attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, lengths: torch.Tensor, window: Optional[int] = None,
+                   scale: Optional[float] = None) -> torch.Tensor:
+    """One more row of causal `attention` for each sequence: k and v [batch, key_heads, width] become row `lengths[b]` of the caches `keys` and `values` [batch, capacity, key_heads, width], in
+    place, and the result [batch, heads, width] is the attention of q over the rows up to it (the last window + 1 of them with `window`).
+
+    `lengths` [batch] int32 is the number of rows in each cache before the call; it stays as it is, so that one tensor serves all layers of a network (`lengths += 1` behind
+    the last).  A sequence of negative length is left out: its result is zero and its caches stay.  One whose cache is full gets NaN, and its caches stay.
+    For inference: it refuses inputs that want a gradient."""
+    compiled = _compiled()
+    if compiled:
+        return compiled.attention_step(q, k, v, keys, values, lengths, None if window is None else operator.index(window), None if scale is None else float(scale))
+    _check(q, "q")
+    for t, name in ((k, "k"), (v, "v"), (keys, "keys"), (values, "values")):
+        _check(t, name, q.dtype, q.device)
+    _check(lengths, "lengths", torch.int32, q.device)
+    if q.dim() != 3 or not 1 <= q.shape[2] <= 128 or q.shape[1] < 1:
+        raise ValueError("q must have shape [batch, heads, width], width 1 to 128")
+    if k.shape != v.shape or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"k and v must have one shape, the batch and width of q, {tuple(q.shape)}, and a number of heads that divides q's")
+    if keys.dim() != 4:
+        raise ValueError("keys must have shape [batch, capacity, key_heads, width]")
+    shape = (k.shape[0], keys.shape[1], k.shape[1], k.shape[2])
+    _check_cache(keys, "keys", shape)
+    _check_cache(values, "values", shape)
+    if keys.numel() and keys.data_ptr() == values.data_ptr():
+        raise ValueError("keys and values must not be one tensor")
+    if tuple(lengths.shape) != q.shape[:1]:
+        raise ValueError(f"lengths must have shape ({q.shape[0]},), got {tuple(lengths.shape)}")
+    window, scale = _window(window), _scale(scale, q.shape[2])
+    _no_tangent(q, k, v, keys, values)
+    if _wants_grad(q, k, v, keys, values):
+        raise RuntimeError("attention_step has no gradient: use attention in training, or torch.no_grad()")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if q.shape[0] == 0:
+        return out
+    q, k, v, lengths = _heads(q), _heads(k), _heads(v), lengths.contiguous()
+    step = HtgsAttentionStep(q.data_ptr(), k.data_ptr(), v.data_ptr(), keys.data_ptr(), values.data_ptr(), lengths.data_ptr(), q.stride(0), k.stride(0), v.stride(0), q.stride(1),
+                             k.stride(1), v.stride(1), keys.stride(0), values.stride(0), keys.stride(1), values.stride(1), keys.stride(2), values.stride(2), keys.shape[1], q.shape[0],
+                             q.shape[1], k.shape[1], q.shape[2], _TYPES[q.dtype], window, scale)
+    size = _native.lib().htgs_attention_step_workspace_bytes(ctypes.byref(step))
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    _call(q.device, "htgs_attention_step", ctypes.byref(step), out.data_ptr(), None if workspace is None else workspace.data_ptr(), size)
+    for t in (keys, values):
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+    return out

@@ -527,6 +527,72 @@ int htgs_gated_scan_backward(const HtgsScan* scan, const float* states, const vo
 int htgs_gated_scan_step(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride, float* state, int64_t state_stride, void* h,
                          int64_t h_stride, int type, int64_t rows, int32_t width, void* stream);
 
+/*
+ * Rotary positions: in each head the pair j of values is turned by the angle position[axis(j)] * base^(-i / n), where pair j is the i-th of the n pairs of its axis (`sections`
+ * says how many pairs each axis has, in order; they add up to width / 2).  A pair is (j, j + width / 2), or (2 j, 2 j + 1) if interleaved.  Angles are
+ * computed in 64 bits.  x[0] and x[1] (heads[1] may be 0) are [rows, heads, width] with strides in elements from row to row and from head to head, y[0] and y[1]
+ * are dense and may not overlap them.  positions [rows, axes] are float or int32 (positions_type 0 or 1).  inverse != 0 turns the other way, which is the gradient.  width is even, 2 to 256;
+ * base is positive; 1 to 4 axes.
+ */
+typedef struct HtgsRotary {
+    const void* x[2];
+    void* y[2];
+    const void* positions;
+    int64_t x_stride[2], x_head_stride[2], positions_stride, rows;
+    double base;
+    int32_t heads[2], sections[4];
+    int32_t axes, positions_type, width, type, interleaved, inverse;
+} HtgsRotary;
+int htgs_rotary(const HtgsRotary* rotary, void* stream);
+
+/*
+ * Attention over sequences that lie one behind the other: of rows / n_sequences rows each (offsets == NULL), or from row offsets[s] to offsets[s + 1] (device memory,
+ * n_sequences + 1 ascending numbers; sequences may be empty, rows before the first and behind the last one get zeros).
+ *   out_i = sum over j of softmax_j(scale * q_i . k_j) v_j
+ * over the rows j of i's sequence with j <= i if causal, and |i - j| <= window if window >= 0.  q [rows, heads, width], k and v [rows, key_heads, width] have strides
+ * in elements from row to row and from head to head; heads is a multiple of key_heads, and head h uses key head h / (heads / key_heads).  out [rows, heads, width] is dense.
+ * sums [heads, rows] (log2 of each row's sum of exponentials) is what the backward pass needs, or NULL.  1 <= width <= 128, scale > 0.
+ * 16-bit types with a width that is a multiple of 8 and rows and heads that begin on 16 bytes take the tensor cores, where the weights P and their gradients are rounded to
+ * the type; others do not, and take 10 to 100 times as long.  The backward pass writes dense gradients; workspace as the size function says, 16-byte aligned.
+ * A wait that runs out is reported as with htgs_fp8_matmul, by htgs_attention_status and the next call; what is not complete is NaN.
+ */
+typedef struct HtgsAttention {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int32_t* offsets;
+    int64_t q_stride, k_stride, v_stride, q_head_stride, k_head_stride, v_head_stride, rows;
+    int32_t heads, key_heads, width, n_sequences, type, causal, window;
+    float scale;
+} HtgsAttention;
+int htgs_attention(const HtgsAttention* attention, void* out, float* sums, void* stream);
+size_t htgs_attention_backward_workspace_bytes(const HtgsAttention* attention);
+int htgs_attention_backward(const HtgsAttention* attention, const void* out, const float* sums, const void* grad_out, int64_t grad_out_stride,
+                            int64_t grad_out_head_stride, void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
+int htgs_attention_status(int32_t device);
+unsigned int* htgs_attention_error_word(int32_t device);
+
+/*
+ * One more row for each of `batch` sequences: k and v [batch, key_heads, width] become row lengths[b] of the caches keys and values [batch, capacity, key_heads, width] (in
+ * place), and out [batch, heads, width] (dense) is the attention of q over rows max(0, lengths[b] - window) to lengths[b] (from row 0 if window < 0).  lengths (device memory)
+ * stays as it is.  A sequence with lengths[b] < 0 is left out: zeros, and its caches stay; one whose cache is full (lengths[b] >= capacity) gets NaN, and its caches stay.
+ * Strides in elements: from sequence to sequence, from row to row (caches), from head to head.  workspace as the size function says, 16-byte aligned.
+ */
+typedef struct HtgsAttentionStep {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* keys;
+    void* values;
+    const int32_t* lengths;
+    int64_t q_stride, k_stride, v_stride, q_head_stride, k_head_stride, v_head_stride;
+    int64_t keys_stride, values_stride, keys_row_stride, values_row_stride, keys_head_stride, values_head_stride, capacity;
+    int32_t batch, heads, key_heads, width, type, window;
+    float scale;
+} HtgsAttentionStep;
+size_t htgs_attention_step_workspace_bytes(const HtgsAttentionStep* step);
+int htgs_attention_step(const HtgsAttentionStep* step, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Measurement aids (off by default; they do not change results).
  * Profiling: CUDA events are recorded on the frame's stream between the stages; after the call
  * htgs_get_stage_ms fills out_ms[0..HTGS_N_STAGES) with the device time of each stage in ms.
