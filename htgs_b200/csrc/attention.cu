@@ -85,21 +85,57 @@ template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention
     }
 }
 
-// {log2 of the sum, D} of the rows of a tile of 128 and a head; rows that are not there get an infinite sum, which makes their weights zero.
-template <typename T> __global__ void __launch_bounds__(kLanesThreads) statistics_kernel(const HtgsAttention a, const T* out, const float* sums, const T* grad, int64_t grad_stride, int64_t grad_head_stride,
-                                                                                        float2* statistics, int64_t statistics_rows) {
+// Statistics of the rows of a tile of 128 and a head.  Bound by HBM: reads the output and its gradient once.  LANES lanes have a row, N values of it at a time each.
+template <typename T, int N, int LANES> __global__ void __launch_bounds__(kLanesThreads) statistics_kernel(const HtgsAttention a, const T* out, const float* sums, const AttentionBackward b, float* statistics,
+                                                                                                          uint32_t* largest) {
     grid_dependency();
-    const int lane = threadIdx.x & 31, head = int(blockIdx.x % a.heads);
+    const int lane = threadIdx.x % LANES, head = int(blockIdx.x % a.heads), group = a.heads / a.key_heads, key_head = head / group;
     const SequenceTile t = find_tile<kStatisticRows>(a, int(blockIdx.x / a.heads));
     if (t.first >= t.end) return;
-    float2* to = statistics + head * statistics_rows + statistic_base(a, t) + (t.first - t.begin);
-    for (int r = threadIdx.x / 32; r < kStatisticRows; r += kLanesThreads / 32) {
+    float* to = statistics + (head * b.statistics_rows + statistic_base(a, t) + (t.first - t.begin)) * 2;
+    float grads = 0.0f, values = 0.0f;
+    #pragma unroll 2
+    for (int r = threadIdx.x / LANES; r < kStatisticRows; r += kLanesThreads / LANES) {
         const int64_t i = t.first + r;
-        float sum = 0.0f;
-        if (i < t.end && !t.outside)
-            for (int c = lane; c < a.width; c += 32) sum = fmaf(to_float<T>(out[(i * a.heads + head) * a.width + c]), to_float<T>(grad[i * grad_stride + head * grad_head_stride + c]), sum);
-        sum = warp_sum(sum);
-        if (lane == 0) to[r] = i < t.end && !t.outside ? make_float2(sums[head * a.rows + i], sum) : make_float2(infinity(), 0.0f);
+        const bool there = i < t.end && !t.outside;
+        float mean = 0.0f, grad = 0.0f, value = 0.0f;
+        if (there) {
+            const T *o = out + (i * a.heads + head) * a.width, *g = static_cast<const T*>(b.grad) + i * b.grad_stride + head * b.grad_head_stride;
+            for (int c = lane * N; c < a.width; c += LANES * N) {
+                float x[N], y[N];
+                load_floats<T, N>(o + c, x);
+                load_floats<T, N>(g + c, y);
+                #pragma unroll
+                for (int k = 0; k < N; ++k) { mean = fmaf(x[k], y[k], mean); grad = fmaf(y[k], y[k], grad); }
+            }
+            if (largest && head % group == 0) {
+                const T* v = static_cast<const T*>(a.v) + i * a.v_stride + key_head * a.v_head_stride;
+                for (int c = lane * N; c < a.width; c += LANES * N) {
+                    float x[N];
+                    load_floats<T, N>(v + c, x);
+                    #pragma unroll
+                    for (int k = 0; k < N; ++k) value = fmaf(x[k], x[k], value);
+                }
+            }
+        }
+        #pragma unroll
+        for (int d = LANES / 2; d > 0; d >>= 1) {
+            mean += __shfl_xor_sync(0xffffffffu, mean, d);
+            if (largest) { grad += __shfl_xor_sync(0xffffffffu, grad, d); value += __shfl_xor_sync(0xffffffffu, value, d); }
+        }
+        if (lane == 0) {
+            to[r] = there ? sums[head * a.rows + i] : 0.0f;
+            to[kStatisticRows + r] = mean;
+        }
+        grads = fmaxf(grads, finite_magnitude(grad));
+        values = fmaxf(values, finite_magnitude(value));
+    }
+    if (!largest || t.outside) return;
+    grads = lanes_max<32>(grads);
+    values = lanes_max<32>(values);
+    if ((threadIdx.x & 31) == 0) {
+        atomicMax(largest + 2 * t.sequence, __float_as_uint(grads));
+        atomicMax(largest + 2 * t.sequence + 1, __float_as_uint(values));
     }
 }
 
@@ -122,7 +158,11 @@ template <typename T, bool KEYS> __global__ void __launch_bounds__(kLanesThreads
         const auto fill_queries = [&](float* q, float* grad, int head, int at, int end) {
             fill_rows<T>(q, pitch, a.q, a.q_stride, head * a.q_head_stride, at, end, a.width);
             fill_rows<T>(grad, pitch, b.grad, b.grad_stride, head * b.grad_head_stride, at, end, a.width);
-            if (threadIdx.x < kLanesRows && at + int(threadIdx.x) < end) statistics[threadIdx.x] = b.statistics[head * b.statistics_rows + base + (at - t.begin) + threadIdx.x];
+            if (threadIdx.x < kLanesRows && at + int(threadIdx.x) < end) {
+                const int64_t r = base + (at - t.begin) + threadIdx.x;
+                const float* from = b.statistics + (head * b.statistics_rows + r / kStatisticRows * kStatisticRows) * 2 + r % kStatisticRows;
+                statistics[threadIdx.x] = make_float2(from[0], from[kStatisticRows]);
+            }
         };
         const auto fill_keys = [&](float* k, float* v, int at, int end) {
             fill_rows<T>(k, pitch, a.k, a.k_stride, key_head * a.k_head_stride, at, end, a.width);
@@ -206,10 +246,28 @@ template <typename T> int backward_lanes(const HtgsAttention& a, const Attention
     const int code = launch_lanes<T>(attention_lanes_backward_kernel<T, false>, once, a, a.heads, 4, stream, b);
     return code != HTGS_OK ? code : launch_lanes<T>(attention_lanes_backward_kernel<T, true>, once_keys, a, a.key_heads, 4, stream, b);
 }
-template <typename T> int launch_statistics(const HtgsAttention& a, const void* out, const float* sums, const AttentionBackward& b, float2* statistics, cudaStream_t stream) {
-    const cudaError_t err = launch_after(statistics_kernel<T>, dim3(unsigned(sequence_tiles(a, kStatisticRows) * a.heads)), kLanesThreads, 0, stream, a, static_cast<const T*>(out), sums,
-                                         static_cast<const T*>(b.grad), b.grad_stride, b.grad_head_stride, statistics, b.statistics_rows);
+template <typename T, int N, int LANES>
+int launch_statistics(const HtgsAttention& a, const void* out, const float* sums, const AttentionBackward& b, float* statistics, uint32_t* largest, cudaStream_t stream) {
+    const cudaError_t err = launch_after(statistics_kernel<T, N, LANES>, dim3(unsigned(sequence_tiles(a, kStatisticRows) * a.heads)), kLanesThreads, 0, stream, a, static_cast<const T*>(out), sums, b,
+                                         statistics, largest);
     return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
+template <typename T> int backward_typed(const HtgsAttention& a, const void* out, const float* sums, AttentionBackward b, float* statistics, uint32_t* largest, cudaStream_t stream) {
+    const bool tiles = aligned(out, 16) && attention_tiles_take(a, b);
+    if constexpr (sizeof(T) == 2) {
+        if (tiles) {
+            if (std::is_same<T, __half>::value) {
+                const cudaError_t err = cudaMemsetAsync(largest, 0, (size_t(a.n_sequences) + 2) * 2 * sizeof(uint32_t), stream);
+                if (err != cudaSuccess) return sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+                b.largest = largest;
+            } else largest = nullptr;
+            const int code = a.width <= 32 ? launch_statistics<T, 8, 4>(a, out, sums, b, statistics, largest, stream)
+                             : a.width <= 64 ? launch_statistics<T, 8, 8>(a, out, sums, b, statistics, largest, stream) : launch_statistics<T, 8, 16>(a, out, sums, b, statistics, largest, stream);
+            return code != HTGS_OK ? code : attention_tiles_backward(a, b, stream);
+        }
+    }
+    const int code = launch_statistics<T, 1, 32>(a, out, sums, b, statistics, nullptr, stream);
+    return code != HTGS_OK ? code : backward_lanes<T>(a, b, stream);
 }
 
 ErrorWords& error_words() {
@@ -257,6 +315,7 @@ int htgs_attention(const HtgsAttention* attention, void* out, float* sums, void*
     if (const int code = reported(attention_error_word(current_device())); code != HTGS_OK) return code;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const HtgsAttention& a = *attention;
+    if (attention_tiles_take(a, out)) return attention_tiles_forward(a, out, sums, s);
     if (a.type == HTGS_FLOAT32) return forward_lanes<float>(a, out, sums, s);
     if (a.type == HTGS_FLOAT16) return forward_lanes<__half>(a, out, sums, s);
     return forward_lanes<__nv_bfloat16>(a, out, sums, s);
@@ -265,7 +324,8 @@ int htgs_attention(const HtgsAttention* attention, void* out, float* sums, void*
 size_t htgs_attention_backward_workspace_bytes(const HtgsAttention* attention) {
     using namespace htgs;
     if (wrong(attention) || attention->rows == 0) return 0;
-    return size_t(statistic_rows(*attention)) * attention->heads * sizeof(float2);
+    const size_t largest = attention->type == HTGS_FLOAT16 ? (size_t(attention->n_sequences) + 2) * 2 * sizeof(uint32_t) : 0;
+    return size_t(statistic_rows(*attention)) * attention->heads * 2 * sizeof(float) + largest;
 }
 
 int htgs_attention_backward(const HtgsAttention* attention, const void* out, const float* sums, const void* grad_out, int64_t grad_out_stride, int64_t grad_out_head_stride,
@@ -280,14 +340,13 @@ int htgs_attention_backward(const HtgsAttention* attention, const void* out, con
     if (const int code = reported(attention_error_word(current_device())); code != HTGS_OK) return code;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const HtgsAttention& a = *attention;
-    float2* statistics = static_cast<float2*>(workspace);
-    const AttentionBackward b{grad_out, grad_out_stride, grad_out_head_stride, grad_q, grad_k, grad_v, statistics, statistic_rows(a)};
-    int code = a.type == HTGS_FLOAT32 ? launch_statistics<float>(a, out, sums, b, statistics, s)
-               : a.type == HTGS_FLOAT16 ? launch_statistics<__half>(a, out, sums, b, statistics, s) : launch_statistics<__nv_bfloat16>(a, out, sums, b, statistics, s);
-    if (code != HTGS_OK) return code;
-    if (a.type == HTGS_FLOAT32) return backward_lanes<float>(a, b, s);
-    if (a.type == HTGS_FLOAT16) return backward_lanes<__half>(a, b, s);
-    return backward_lanes<__nv_bfloat16>(a, b, s);
+    float* statistics = static_cast<float*>(workspace);
+    const int64_t rows = statistic_rows(a);
+    uint32_t* largest = reinterpret_cast<uint32_t*>(statistics + rows * a.heads * 2);
+    const AttentionBackward b{grad_out, grad_out_stride, grad_out_head_stride, grad_q, grad_k, grad_v, statistics, rows, nullptr};
+    if (a.type == HTGS_FLOAT32) return backward_typed<float>(a, out, sums, b, statistics, largest, s);
+    if (a.type == HTGS_FLOAT16) return backward_typed<__half>(a, out, sums, b, statistics, largest, s);
+    return backward_typed<__nv_bfloat16>(a, out, sums, b, statistics, largest, s);
 }
 
 }  // extern "C"

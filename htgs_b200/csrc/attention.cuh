@@ -11,7 +11,7 @@
 namespace htgs {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kStatisticRows = 128;
+constexpr int kStatisticRows = 128, kStatisticBytes = kStatisticRows * 2 * 4;
 
 // Sequences and what stands before and behind them (rows of no sequence, with offsets only) share tiles with nobody: sequence v begins at tile bound(v) / ROWS + v.  That leaves
 // room for the tiles of all before it, needs no sum over the sequences, and is found by a search over the offsets alone.
@@ -46,7 +46,8 @@ template <int ROWS> __device__ __forceinline__ SequenceTile find_tile(const Htgs
     return {low, begin, end, begin + (tile - begin / ROWS - low) * ROWS, low == 0 || low == n + 1};
 }
 
-// Statistics of rows for the backward pass, {log2 of the sum, D} in order of tiles of 128 rows, so that a tile's lie on 16 bytes: where those of a sequence begin.
+// Statistics of rows for the backward pass, log2 of the sum and D, in order of tiles of 128 rows: 128 of the one, 128 of the other, so that a tile's lie side by side on 16 bytes.  Where those of a
+// sequence begin, in rows.
 __host__ __device__ __forceinline__ int64_t statistic_rows(const HtgsAttention& a) { return sequence_tiles(a, kStatisticRows) * kStatisticRows; }
 __device__ __forceinline__ int64_t statistic_base(const HtgsAttention& a, const SequenceTile& t) {
     if (a.offsets) return (int64_t(t.begin / kStatisticRows) + t.sequence) * kStatisticRows;
@@ -66,11 +67,12 @@ __device__ __forceinline__ float infinity() { return __uint_as_float(0x7f800000u
 struct AttentionBackward {
     const void* grad; int64_t grad_stride, grad_head_stride;
     void* grad_q; void* grad_k; void* grad_v;
-    const float2* statistics; int64_t statistics_rows;       // of a head
+    const float* statistics; int64_t statistics_rows;        // of a head
+    const uint32_t* largest;                                 // of each sequence (counted as in SequenceTile): the largest finite |dout|^2 and |v|^2 of a row and head, as bits; fp16 only
 };
 
 // attention_tiles.cu: 16-bit types, widths that are a multiple of 8, everything on 16 bytes
-bool attention_tiles_take(const HtgsAttention& a);
+bool attention_tiles_take(const HtgsAttention& a, const void* out);
 int attention_tiles_forward(const HtgsAttention& a, void* out, float* sums, cudaStream_t stream);
 bool attention_tiles_take(const HtgsAttention& a, const AttentionBackward& b);
 int attention_tiles_backward(const HtgsAttention& a, const AttentionBackward& b, cudaStream_t stream);

@@ -1,1 +1,1111 @@
+// Attention over packed sequences on the tensor cores (tcgen05): 16-bit values, heads of 8, 16, ... 128 values, rows and heads that begin on 16 bytes.
+//
+// Tiles are 128 rows by 128 rows.  Operands come by TMA into shared memory as panels of 64 columns under the 128-byte swizzle: [128 rows][128 bytes], which serve as they lie both for
+// products along the columns (q k^T) and along the rows (P v, where a panel is a transposed operand).  Scores, weights (over the scores, in the type) and outputs stay in tensor memory.
 #include "attention.cuh"
+
+namespace htgs {
+
+namespace {
+
+constexpr int kTile = 128, kPanel = 64, kPanelBytes = kTile * kPanel * 2;
+constexpr int kTilesThreads = 384;
+constexpr uint32_t kPanelUnits = kPanelBytes >> 4;
+
+// Operand descriptors.  The upper word is the same for all: groups of 8 rows 1024 bytes apart, 128-byte swizzle.  Lower word, along the columns: the address (the leading offset says
+// nothing); along the rows: the address and the distance from panel to panel.
+constexpr uint32_t kPanelHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t along_columns(uint32_t address) { return (address & 0x3ffffu) >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t along_rows(uint32_t address) { return (address & 0x3ffffu) >> 4 | kPanelUnits << 16; }
+// 32-bit sums of products of T; the second operand along its rows or columns.
+template <typename T> __device__ __forceinline__ uint32_t instruction(int columns, bool second_along_rows) {
+    constexpr uint32_t format = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return 1u << 4 | format << 7 | format << 10 | uint32_t(second_along_rows) << 16 | uint32_t(columns >> 3) << 17 | uint32_t(kTile >> 4) << 24;
+}
+__device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint32_t b, uint32_t instruction, uint32_t add) {                 // a in shared memory
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(instruction), "r"(add), "n"(kPanelHigh) : "memory");
+}
+__device__ __forceinline__ void multiply_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t instruction, uint32_t add) {            // a in tensor memory
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(instruction), "r"(add), "n"(kPanelHigh) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void load_panel(void* to, const CUtensorMap* map, int column, int head, int row, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_u32(to)), "l"(map), "r"(column), "r"(head), "r"(row), "r"(smem_u32(bar)) : "memory");
+}
+// 32 columns of a lane's row; begun, and all done.
+__device__ __forceinline__ void tmem_begin32(uint32_t address, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+                   "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(address));
+}
+__device__ __forceinline__ void tmem_begin16(uint32_t address, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(address));
+}
+__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+                   "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- values that are not finite ------------------------------------------------------------------------------------------------
+// A weight of zero takes a finite value out of a sum, not an infinite one or a NaN.  So in tiles where not every row sees every other the operand is looked through before it is used, by warps that have
+// nothing else to do, and where something is not finite a thread adds up what its row sees itself (some 50 us a tile).  Nothing of this costs the other tiles anything.
+
+// Whether rows [first, first + 64) of a tile hold such values; by a warp.
+template <typename T, int PANELS> __device__ __forceinline__ bool not_finite(const unsigned char* tile, int first, int lane) {
+    using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const uint32_t zero = 0;
+    Two sum = *reinterpret_cast<const Two*>(&zero);
+    #pragma unroll 4
+    for (int i = lane; i < PANELS * 64 * 8; i += 32) {
+        const uint4 piece = *reinterpret_cast<const uint4*>(tile + (i >> 9) * kPanelBytes + first * 128 + (i & 511) * 16);
+        const Two* v = reinterpret_cast<const Two*>(&piece);
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) sum = __hfma2(v[k], *reinterpret_cast<const Two*>(&zero), sum);          // NaN from then on
+    }
+    const float2 both = pair_floats<T>(*reinterpret_cast<const uint32_t*>(&sum));
+    return __any_sync(0xffffffffu, both.x != 0.0f || both.y != 0.0f);
+}
+// Columns [from, to) of a lane's row of sums in tensor memory: plus (add), or set to, its weights times the rows [low, high] of a tile.  Weights: words of two, 64 at `weights`, 64 at weights + second.
+template <typename T> __device__ __forceinline__ void multiply_seen(uint32_t sums, int from, int to, bool add, uint32_t weights, uint32_t second, const unsigned char* tile, int low, int high) {
+    #pragma unroll 1
+    for (int c = from; c < to; c += 16) {
+        uint32_t o[16] = {};
+        if (add) {
+            tmem_begin16(sums + c, o);
+            tmem_loaded();
+        }
+        #pragma unroll 1
+        for (int block = 0; block < 4; ++block) {
+            uint32_t w[16];
+            tmem_begin16(weights + (block >> 1) * second + (block & 1) * 16, w);
+            tmem_loaded();
+            #pragma unroll
+            for (int k = 0; k < 32; ++k) {
+                const int row = block * 32 + k;
+                if (row < low || row > high) continue;
+                const float2 pair = pair_floats<T>(w[k / 2]);
+                const float weight = k & 1 ? pair.y : pair.x;
+                const unsigned char* at = tile + (c >> 6) * kPanelBytes + row * 128;
+                #pragma unroll
+                for (int piece = 0; piece < 2; ++piece) {
+                    float v[8];
+                    load_floats<T, 8>(reinterpret_cast<const T*>(at + (((c >> 3 & 7) + piece) ^ (row & 7)) * 16), v);
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) o[piece * 8 + i] = __float_as_uint(fmaf(weight, v[i], __uint_as_float(o[piece * 8 + i])));
+                }
+            }
+            __syncwarp();
+        }
+        tmem_store16(sums + c, o);
+    }
+    tmem_stored();
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------------
+
+// What an exponent may pass the running maximum by before the output is scaled down to a new one: weights up to 2^8 are as precise as those up to 1, and most tiles then leave the output alone.
+constexpr float kSlack = 8.0f;
+// Weights in fp16 are 2^6 times as large, so that one of 2^-20 of the row's largest is a normal number (and the largest is 2^14).
+template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 6.0f : 0.0f;
+
+template <int PANELS> struct ForwardTile {
+    static constexpr int bytes = PANELS * kPanelBytes, stages = PANELS == 2 ? 5 : 8;
+    static constexpr int barriers = 2 + 3 * stages + 6;
+    static constexpr int smem = 1024 + (2 + stages) * bytes + 512;
+    static_assert(barriers * 8 + 8 + stages * 8 <= 512 && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");       // one block has an SM alone, and with it tensor memory
+};
+
+struct ForwardArgs { HtgsAttention a; void* out; float* sums; unsigned int* error; };
+
+// Two tiles of queries, one behind the other, against tiles of keys.  Warp 0 loads; warp 1 issues the products, for one tile of queries while the other's softmax is computed; warps 2 and 3 look through
+// values of which some are not seen; warps 4 to 7 and 8 to 11 have a tile of queries each, a thread for each row.  Tensor memory: scores (weights over them) at 0 and 128, outputs at 256 and 384.
+template <typename T, int PANELS>
+__global__ void __launch_bounds__(kTilesThreads, 1) attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ForwardArgs args) {
+    using S = ForwardTile<PANELS>;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* const queries = raw + (base - smem_u32(raw));
+    unsigned char* const ring = queries + 2 * S::bytes;
+    uint64_t* const q_full = reinterpret_cast<uint64_t*>(ring + S::stages * S::bytes);
+    uint64_t* const full = q_full + 2;
+    uint64_t* const empty = full + S::stages;
+    uint64_t* const searched = empty + S::stages;        // values have been looked through
+    uint64_t* const scored = searched + S::stages;         // the scores of a tile are there
+    uint64_t* const weighed = scored + 2;                // its weights are
+    uint64_t* const summed = weighed + 2;                // they are in the output
+    uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(summed + 2);
+    volatile uint32_t* const failed = tmem_at + 1;
+    volatile uint32_t* const dirty = failed + 1;         // [stages][2], of halves of a tile of values
+
+    const HtgsAttention& a = args.a;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    grid_dependency();
+    // the last tiles of a sequence first: causal, they have the most keys
+    const int head = int(blockIdx.x % a.heads), key_head = head / (a.heads / a.key_heads);
+    const SequenceTile t = find_tile<2 * kTile>(a, int(gridDim.x / a.heads - 1 - blockIdx.x / a.heads));
+    if (t.first >= t.end) return;
+    T* const out = static_cast<T*>(args.out);
+    if (t.outside) {
+        const int rows = min(2 * kTile, t.end - t.first);
+        for (int i = threadIdx.x; i < rows * (a.width / 8); i += kTilesThreads)
+            *reinterpret_cast<uint4*>(out + (int64_t(t.first + i / (a.width / 8)) * a.heads + head) * a.width + i % (a.width / 8) * 8) = make_uint4(0, 0, 0, 0);
+        if (args.sums)
+            for (int i = threadIdx.x; i < rows; i += kTilesThreads) args.sums[head * a.rows + t.first + i] = 0.0f;
+        return;
+    }
+    // keys low + [0, 128 n) for the block; tile s of queries sees tiles [begin[s], end[s]) of them
+    const int last_row = min(t.first + 2 * kTile, t.end) - 1;
+    const int low = first_seen(a, t.begin, t.first), n = (last_seen(a, t.end, last_row) - low) / kTile + 1;
+    int begin[2], end[2];
+    #pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const int row = t.first + s * kTile;
+        begin[s] = row < t.end ? (first_seen(a, t.begin, row) - low) / kTile : 0;
+        end[s] = row < t.end ? (last_seen(a, t.end, min(row + kTile, t.end) - 1) - low) / kTile + 1 : 0;
+    }
+    // whether all rows of tile s see all keys of tile j
+    const auto whole = [&](int s, int j) {
+        const int first = t.first + s * kTile;
+        return low + j * kTile >= first_seen(a, t.begin, min(first + kTile, t.end) - 1) && low + j * kTile + kTile - 1 <= last_seen(a, t.end, min(first, t.end - 1));
+    };
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) { mbar_init(q_full + i, 1); mbar_init(scored + i, 1); mbar_init(weighed + i, 4); mbar_init(summed + i, 1); }
+        for (int i = 0; i < S::stages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 3); mbar_init(searched + i, 2); }
+        *failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tmem_fence_before();
+    }
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            const bool one = elect_one();
+            if (one) {
+                #pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (end[s] == 0) continue;
+                    mbar_arrive_expect_tx(q_full + s, S::bytes);
+                    for (int p = 0; p < PANELS; ++p) load_panel(queries + s * S::bytes + p * kPanelBytes, &map_q, p * kPanel, head, t.first + s * kTile, q_full + s);
+                }
+            }
+            __syncwarp();
+            Ring<S::stages> stage;
+            uint32_t uses = 0;
+            bool ok = true;
+            for (int i = 0; i < 2 * n; ++i, ++uses, stage.next()) {           // keys and values of a tile by turns
+                ok = __all_sync(0xffffffffu, wait_in_line(empty + stage.at, stage.round ^ 1, failed));
+                if (!ok) break;
+                if (one) {
+                    mbar_arrive_expect_tx(full + stage.at, S::bytes);
+                    for (int p = 0; p < PANELS; ++p) load_panel(ring + stage.at * S::bytes + p * kPanelBytes, i & 1 ? &map_v : &map_k, p * kPanel, key_head, low + (i >> 1) * kTile, full + stage.at);
+                }
+                __syncwarp();
+            }
+            if (!ok) {              // no copy may be on its way when the block ends
+                for (uint32_t u = uses > S::stages ? uses - S::stages : 0; u < uses; ++u) {
+                    WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                    while (!mbar_try_wait(full + u % S::stages, u / S::stages & 1) && !limit.over(nanoseconds())) {}
+                }
+                for (int s = 0; s < 2; ++s) {
+                    WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                    while (end[s] && !mbar_try_wait(q_full + s, 0) && !limit.over(nanoseconds())) {}
+                }
+            }
+        } else if (warp == 1) {
+            const bool one = elect_one();
+            const uint32_t score = instruction<T>(kTile, false), weigh = instruction<T>((a.width + 15) & ~15, true);
+            const int steps = (a.width + 15) / 16;
+            Ring<S::stages> stage;
+            uint32_t weighed_round[2] = {0, 0};
+            bool ok = true;
+            const auto scores = [&](int s, uint32_t slot) {
+                const uint32_t q = along_columns(base + s * S::bytes), k = along_columns(base + 2 * S::bytes + slot * S::bytes);
+                if (one) {
+                    for (int i = 0; i < steps; ++i) {
+                        const uint32_t at = (i >> 2) * kPanelUnits + (i & 3) * 2;
+                        multiply(tmem + s * kTile, q + at, k + at, score, i > 0);
+                    }
+                    commit(scored + s);
+                }
+                __syncwarp();
+            };
+            const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_in_line(bar, parity, failed)); };
+            for (int j = -1; j < n && ok; ++j) {              // the output's part of tile j, then the scores of tile j + 1
+                uint32_t value_slot = 0, key_slot = 0;
+                if (j >= 0) { wait(full + stage.at, stage.round); value_slot = stage.at; stage.next(); }
+                if (j + 1 < n) { key_slot = stage.at; wait(full + stage.at, stage.round); stage.next(); }
+                #pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (j >= begin[s] && j < end[s]) {
+                        wait(weighed + s, weighed_round[s]);
+                        if (!ok) break;
+                        weighed_round[s] ^= 1;
+                        tmem_fence_after();
+                        const uint32_t v = along_rows(base + 2 * S::bytes + value_slot * S::bytes);
+                        const bool added = !whole(s, j) && (dirty[2 * value_slot] | dirty[2 * value_slot + 1]);       // by the softmax's threads
+                        if (one) {
+                            #pragma unroll
+                            for (int i = 0; i < (added ? 0 : kTile / 16); ++i) multiply_tmem(tmem + 2 * kTile + s * kTile, tmem + s * kTile + i * 8, v + i * (2048 >> 4), weigh, j > begin[s] || i > 0);
+                            commit(summed + s);
+                        }
+                        __syncwarp();
+                    }
+                    if (j + 1 >= begin[s] && j + 1 < end[s]) {
+                        if (j + 1 == begin[s]) wait(q_full + s, 0);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        scores(s, key_slot);
+                    }
+                }
+                if (!ok) break;
+                if (one) {
+                    if (j >= 0) commit(empty + value_slot);
+                    if (j + 1 < n) commit(empty + key_slot);
+                }
+                __syncwarp();
+            }
+        } else {
+            Ring<S::stages> stage;
+            for (int i = 0; i < 2 * n; ++i, stage.next()) {
+                if (!__all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed))) break;
+                const int j = i >> 1;
+                const bool seen = !(i & 1) || ((j < begin[0] || j >= end[0] || whole(0, j)) && (j < begin[1] || j >= end[1] || whole(1, j)));
+                const bool found = !seen && not_finite<T, PANELS>(ring + stage.at * S::bytes, (warp - 2) * 64, lane);
+                if (lane == 0) {
+                    dirty[2 * stage.at + warp - 2] = found;
+                    arrive(searched + stage.at);
+                    arrive(empty + stage.at);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int s = (warp >> 2) - 1, quarter = (warp & 3) * 32;
+        const int first = t.first + s * kTile, row = min(first + quarter + lane, t.end - 1);
+        const bool there = first + quarter + lane < t.end;
+        const uint32_t lanes = uint32_t(quarter) << 16, score = tmem + s * kTile + lanes, sum_at = tmem + 2 * kTile + s * kTile + lanes;
+        const float scale = a.scale * kLog2e;
+        const int row_low = first_seen(a, t.begin, row), row_high = last_seen(a, t.end, row);
+        float most = -infinity();
+        f32x2 total = pack2(0.0f, 0.0f);
+        bool ok = true;
+        const int from = s == 0 ? begin[0] : begin[1], to = s == 0 ? end[0] : end[1];
+        for (int j = from; j < to; ++j) {
+            ok = __all_sync(0xffffffffu, wait_in_line(scored + s, (j - from) & 1, failed));
+            if (!ok) break;
+            tmem_fence_after();
+            uint32_t v[128];
+            #pragma unroll
+            for (int c = 0; c < 128; c += 32) tmem_begin32(score + c, v + c);
+            tmem_loaded();
+            const int k0 = low + j * kTile;
+            const bool masked = !whole(s, j);
+            const int from_column = row_low - k0, to_column = row_high - k0;
+            if (masked) {
+                #pragma unroll
+                for (int c = 0; c < 128; ++c) v[c] = c < from_column || c > to_column ? 0xff800000u : v[c];
+            }
+            float m[4];
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) m[c] = __uint_as_float(v[c]);
+            #pragma unroll
+            for (int c = 4; c < 128; c += 8)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) m[i] = c + 4 + i < 128 ? fmaxf(fmaxf(m[i], __uint_as_float(v[c + i])), __uint_as_float(v[c + 4 + i < 128 ? c + 4 + i : 0])) : fmaxf(m[i], __uint_as_float(v[c + i]));
+            const float tile_most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * scale;
+            if (__any_sync(0xffffffffu, tile_most > most + kSlack)) {
+                const float now = fmaxf(most, tile_most), factor = most == now ? 1.0f : exp2_approx(most - now);
+                most = now;
+                total = mul2(total, pack2(factor, factor));
+                if (j > from) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (j - from - 1) & 1, failed));
+                    if (!ok) break;
+                    tmem_fence_after();
+                    #pragma unroll 1
+                    for (int c = 0; c < a.width; c += 16) {
+                        uint32_t o[16];
+                        tmem_begin16(sum_at + c, o);
+                        tmem_loaded();
+                        #pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                        tmem_store16(sum_at + c, o);
+                    }
+                    tmem_stored();
+                }
+            }
+            const float shift = kLift<T> - (most == -infinity() ? 0.0f : most);
+            const f32x2 scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
+            f32x2 sums[2] = {total, pack2(0.0f, 0.0f)};
+            #pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+                uint32_t words[16];
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 x = unpack2(fma2(pack2(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1])), scale2, shift2));
+                    const float p0 = exp2_approx(x.x), p1 = exp2_approx(x.y);
+                    sums[i & 1] = add2(sums[i & 1], pack2(p0, p1));
+                    words[i] = floats_pair<T>(p0, p1);
+                }
+                tmem_store16(score + c / 2, words);
+            }
+            total = add2(sums[0], sums[1]);
+            tmem_stored();
+            if (masked) {
+                const uint32_t at = uint32_t(2 * j + 1) % S::stages, round = uint32_t(2 * j + 1) / S::stages & 1;
+                ok = __all_sync(0xffffffffu, wait_in_line(searched + at, round, failed));
+                if (!ok) break;
+                if (dirty[2 * at] | dirty[2 * at + 1]) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(full + at, round, failed));
+                    if (ok && j > from) ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (j - from - 1) & 1, failed));
+                    if (!ok) break;
+                    tmem_fence_after();
+                    multiply_seen<T>(sum_at, 0, a.width, j > from, score, 32, ring + at * S::bytes, from_column, to_column);
+                }
+            }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(weighed + s);
+        }
+        if (ok && to > from) {
+            ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (to - from - 1) & 1, failed));
+            if (ok) {
+                tmem_fence_after();
+                const float2 parts = unpack2(total);
+                const float sum = parts.x + parts.y, inverse = 1.0f / sum;
+                T* const at = out + (int64_t(row) * a.heads + head) * a.width;
+                for (int c = 0; c < a.width; c += 32) {
+                    uint32_t o[32];
+                    tmem_begin32(sum_at + c, o);
+                    tmem_loaded();
+                    #pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float f[8];
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[i + k]) * inverse;
+                        if (there && c + i < a.width) store_floats<T, 8>(at + c + i, f);
+                    }
+                }
+                if (args.sums && there) args.sums[head * a.rows + row] = most - kLift<T> + log2f(sum);
+            }
+        }
+        tmem_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (*failed) {               // a wait ran out: nothing that looks like a result
+        const int rows = min(2 * kTile, t.end - t.first);
+        for (int i = threadIdx.x; i < rows * a.width; i += kTilesThreads)
+            out[(int64_t(t.first + i / a.width) * a.heads + head) * a.width + i % a.width] = from_float<T>(__uint_as_float(0x7fffffffu));
+        if (threadIdx.x == 0) {
+            *reinterpret_cast<volatile unsigned int*>(args.error) = 1;
+            __threadfence_system();
+        }
+    }
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------------
+// Two kernels, one over tiles of keys (gradients of k and v, over all query heads of the key head) and one over tiles of queries, which compute the weights again from the rows' statistics. Seven products
+// where one kernel could do with five, but that one's sums for q would come from many blocks, in an order of their own or in memory of 32 bits.  Here each sum stays in tensor memory from its first
+// term to its last, in a fixed order.
+//
+// fp16: weights carry 2^14 (they are at most 1), and their gradients c, a power of two by a bound on them for the sequence, |dout| |v| / 2: at most 2^14, where small ones are normal numbers.
+
+constexpr int kBackwardTail = 512;
+template <typename T> constexpr float kWeightLift = std::is_same<T, __half>::value ? 14.0f : 0.0f;
+
+template <int PANELS> struct KeysTile {
+    static constexpr int bytes = PANELS * kPanelBytes, stages = PANELS == 2 ? 2 : 4, stage_bytes = 2 * bytes + kStatisticBytes;
+    static constexpr int smem = 1024 + 2 * bytes + stages * stage_bytes + kBackwardTail;
+    static_assert((7 + 3 * stages) * 8 + 8 + stages * 8 <= kBackwardTail && smem <= 227 * 1024 && smem > 116 * 1024 && stage_bytes % 1024 == 0, "shared memory");
+};
+template <int PANELS> struct QueriesTile {
+    static constexpr int bytes = PANELS * kPanelBytes, stages = PANELS == 2 ? 5 : 8;
+    static constexpr int smem = 1024 + (2 + stages) * bytes + kBackwardTail;
+    static_assert((8 + 3 * stages) * 8 + 8 + stages * 8 <= kBackwardTail && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");
+};
+
+struct BackwardArgs { HtgsAttention a; AttentionBackward b; unsigned int* error; };
+
+// The power of two that a sequence's gradients of scores carry (fp16), and 1.
+template <typename T> __device__ __forceinline__ float gradient_lift(const AttentionBackward& b, int sequence) {
+    if (!std::is_same<T, __half>::value) return 1.0f;
+    const float bound = sqrtf(__uint_as_float(b.largest[2 * sequence])) * sqrtf(__uint_as_float(b.largest[2 * sequence + 1]));
+    if (!(bound >= 1e-30f && bound <= 1e30f)) return 1.0f;
+    return __uint_as_float((254u - (__float_as_uint(bound) >> 23)) << 23) * 16384.0f;           // 2^14 / (the power of two that the bound reaches), which is above half of it
+}
+template <typename T> __device__ __forceinline__ void zero_rows(void* to, const SequenceTile& t, int heads, int head, int width) {
+    const int rows = min(kTile, t.end - t.first), pieces = width / 8;
+    for (int i = threadIdx.x; i < rows * pieces; i += kTilesThreads)
+        *reinterpret_cast<uint4*>(static_cast<T*>(to) + (int64_t(t.first + i / pieces) * heads + head) * width + i % pieces * 8) = make_uint4(0, 0, 0, 0);
+}
+template <typename T> __device__ __forceinline__ void nan_rows(void* to, const SequenceTile& t, int heads, int head, int width) {
+    const int rows = min(kTile, t.end - t.first);
+    for (int i = threadIdx.x; i < rows * width; i += kTilesThreads)
+        static_cast<T*>(to)[(int64_t(t.first + i / width) * heads + head) * width + i % width] = from_float<T>(__uint_as_float(0x7fffffffu));
+}
+// Columns [from, to) of a lane's row of sums, times a factor, rounded, into memory.
+template <typename T> __device__ __forceinline__ void store_sums(uint32_t sums, T* row, int from, int to, float factor, bool there) {
+    #pragma unroll 1
+    for (int c = from; c < to; c += 16) {
+        uint32_t o[16];
+        tmem_begin16(sums + c, o);
+        tmem_loaded();
+        #pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+            float f[8];
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[i + k]) * factor;
+            if (there && c + i < to) store_floats<T, 8>(row + c + i, f);
+        }
+    }
+}
+// A barrier of the eight warps that share a tile's columns, with the limit of every wait.
+__device__ __forceinline__ bool all_meet(uint64_t* met, uint32_t& meetings, int lane, volatile uint32_t* failed) {
+    tmem_fence_before();
+    __syncwarp();
+    if (lane == 0) arrive(met);
+    const bool ok = __all_sync(0xffffffffu, wait_in_line(met, meetings++ & 1, failed));
+    tmem_fence_after();
+    return ok;
+}
+// 64 columns from a column on that only [from, to] of count: whether column c of them does.
+__device__ __forceinline__ bool counts(int c, int from, int to) { return c >= from && c <= to; }
+
+// Gradients of k and v of a tile.  Scores and their gradients are turned round, a row for each key, so that the weights are the first operand from tensor memory.  Warp 0 loads queries, output gradients and
+// statistics of a tile of queries; warp 1 issues the products, [dv, next scores] while the score gradients are computed and [dk, next weight gradients] while the weights are; warps 4 to 7 and 8 to 11
+// have 64 columns each.  Tensor memory: scores (weights) 0, weight gradients (score gradients) 128, dv 256, dk 384.
+template <typename T, int PANELS>
+__global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                         const __grid_constant__ CUtensorMap map_grad, const __grid_constant__ BackwardArgs args) {
+    using S = KeysTile<PANELS>;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* const own = raw + (base - smem_u32(raw));            // k, v
+    unsigned char* const ring = own + 2 * S::bytes;
+    const uint32_t ring_at = base + 2 * S::bytes;
+    uint64_t* const own_full = reinterpret_cast<uint64_t*>(ring + S::stages * S::stage_bytes);
+    uint64_t* const full = own_full + 1;
+    uint64_t* const empty = full + S::stages;
+    uint64_t* const searched = empty + S::stages;
+    uint64_t* const scored = searched + S::stages;       // scores are there
+    uint64_t* const weighed = scored + 1;                // weights are
+    uint64_t* const graded = weighed + 1;                // gradients of the weights are
+    uint64_t* const changed = graded + 1;                // gradients of the scores are
+    uint64_t* const finished = changed + 1;
+    uint64_t* const met = finished + 1;
+    uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(met + 1);
+    volatile uint32_t* const failed = tmem_at + 1;
+    volatile uint32_t* const dirty = failed + 1;         // [stages][2]: output gradients, queries
+
+    const HtgsAttention& a = args.a;
+    const AttentionBackward& b = args.b;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    grid_dependency();
+    // the first tiles of a sequence first: causal, they are seen by the most queries
+    const int key_head = int(blockIdx.x % a.key_heads), group = a.heads / a.key_heads;
+    const SequenceTile t = find_tile<kTile>(a, int(blockIdx.x / a.key_heads));
+    if (t.first >= t.end) return;
+    if (t.outside) {
+        zero_rows<T>(b.grad_k, t, a.key_heads, key_head, a.width);
+        zero_rows<T>(b.grad_v, t, a.key_heads, key_head, a.width);
+        return;
+    }
+    const int last_row = min(t.first + kTile, t.end) - 1;
+    const int first_tile = (first_seeing(a, t.begin, t.first) - t.begin) / kTile, tiles = (last_seeing(a, t.end, last_row) - t.begin) / kTile - first_tile + 1, n = group * tiles;
+    const int whole_low = first_seeing(a, t.begin, last_row), whole_high = last_seeing(a, t.end, t.first);
+    const auto query_row = [&](int i) { return t.begin + (first_tile + i % tiles) * kTile; };
+    const auto whole = [&](int q0) { return q0 >= whole_low && q0 + kTile - 1 <= whole_high; };       // all keys are seen by all queries
+
+    if (threadIdx.x == 0) {
+        mbar_init(own_full, 1); mbar_init(scored, 1); mbar_init(weighed, 8); mbar_init(graded, 1); mbar_init(changed, 8); mbar_init(finished, 1); mbar_init(met, 8);
+        for (int i = 0; i < S::stages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 3); mbar_init(searched + i, 2); }
+        *failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tmem_fence_before();
+    }
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            const bool one = elect_one();
+            if (one) {
+                mbar_arrive_expect_tx(own_full, 2 * S::bytes);
+                for (int p = 0; p < PANELS; ++p) {
+                    load_panel(own + p * kPanelBytes, &map_k, p * kPanel, key_head, t.first, own_full);
+                    load_panel(own + S::bytes + p * kPanelBytes, &map_v, p * kPanel, key_head, t.first, own_full);
+                }
+            }
+            __syncwarp();
+            const float* statistics = b.statistics + (statistic_base(a, t) + first_tile * kTile) * 2;
+            Ring<S::stages> stage;
+            uint32_t uses = 0;
+            bool ok = true;
+            for (int i = 0; i < n; ++i, ++uses, stage.next()) {
+                ok = __all_sync(0xffffffffu, wait_in_line(empty + stage.at, stage.round ^ 1, failed));
+                if (!ok) break;
+                if (one) {
+                    unsigned char* at = ring + stage.at * S::stage_bytes;
+                    const int head = key_head * group + i / tiles, row = query_row(i);
+                    mbar_arrive_expect_tx(full + stage.at, S::stage_bytes);
+                    for (int p = 0; p < PANELS; ++p) load_panel(at + p * kPanelBytes, &map_q, p * kPanel, head, row, full + stage.at);
+                    for (int p = 0; p < PANELS; ++p) load_panel(at + S::bytes + p * kPanelBytes, &map_grad, p * kPanel, head, row, full + stage.at);
+                    bulk_copy_g2s(at + 2 * S::bytes, statistics + (head * b.statistics_rows + i % tiles * kTile) * 2, kStatisticBytes, full + stage.at);
+                }
+                __syncwarp();
+            }
+            if (!ok) {              // no copy may be on its way when the block ends
+                for (uint32_t u = uses > S::stages ? uses - S::stages : 0; u < uses; ++u) {
+                    WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                    while (!mbar_try_wait(full + u % S::stages, u / S::stages & 1) && !limit.over(nanoseconds())) {}
+                }
+                WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                while (!mbar_try_wait(own_full, 0) && !limit.over(nanoseconds())) {}
+            }
+        } else if (warp == 1) {
+            const bool one = elect_one();
+            const uint32_t score = instruction<T>(kTile, false), sum = instruction<T>((a.width + 15) & ~15, true);
+            const int steps = (a.width + 15) / 16;
+            Ring<S::stages> stage, next;
+            bool ok = true;
+            const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_in_line(bar, parity, failed)); };
+            // scores (which 0) of keys and queries, or gradients of weights (1) of values and output gradients
+            const auto product = [&](int which, uint32_t slot, uint64_t* bar) {
+                const uint32_t x = along_columns(base + which * S::bytes), y = along_columns(ring_at + slot * S::stage_bytes + which * S::bytes);
+                if (one) {
+                    for (int i = 0; i < steps; ++i) {
+                        const uint32_t at = (i >> 2) * kPanelUnits + (i & 3) * 2;
+                        multiply(tmem + which * kTile, x + at, y + at, score, i > 0);
+                    }
+                    commit(bar);
+                }
+                __syncwarp();
+            };
+            // dv (1) of weights and output gradients, or dk (0) of score gradients and queries
+            const auto gather = [&](int which, uint32_t slot, bool first, bool added) {
+                const uint32_t w = tmem + (which ? 0 : kTile), y = along_rows(ring_at + slot * S::stage_bytes + which * S::bytes), to = tmem + (which ? 2 : 3) * kTile;
+                if (one) {
+                    #pragma unroll
+                    for (int i = 0; i < (added ? 0 : kTile / 16); ++i) multiply_tmem(to, w + (i >> 2) * 64 + (i & 3) * 8, y + i * (2048 >> 4), sum, !first || i > 0);
+                }
+                __syncwarp();
+            };
+            wait(own_full, 0);
+            wait(full, 0);
+            if (ok) {
+                tmem_fence_after();
+                product(0, 0, scored);
+                product(1, 0, graded);
+                next.next();
+            }
+            for (int i = 0; i < n && ok; ++i, stage.next()) {
+                const bool all = whole(query_row(i));
+                wait(weighed, i & 1);
+                if (!ok) break;
+                tmem_fence_after();
+                gather(1, stage.at, i == 0, !all && dirty[2 * stage.at]);
+                if (i + 1 < n) {
+                    wait(full + next.at, next.round);
+                    if (!ok) break;
+                    product(0, next.at, scored);
+                }
+                wait(changed, i & 1);
+                if (!ok) break;
+                tmem_fence_after();
+                gather(0, stage.at, i == 0, !all && dirty[2 * stage.at + 1]);
+                if (one) commit(empty + stage.at);
+                __syncwarp();
+                if (i + 1 < n) {
+                    product(1, next.at, graded);
+                    next.next();
+                }
+            }
+            if (one && ok) commit(finished);
+            __syncwarp();
+        } else {
+            Ring<S::stages> stage;
+            for (int i = 0; i < n; ++i, stage.next()) {
+                if (!__all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed))) break;
+                bool found = false;
+                if (!whole(query_row(i))) {
+                    const unsigned char* tile = ring + stage.at * S::stage_bytes + (warp == 2 ? S::bytes : 0);
+                    found = not_finite<T, PANELS>(tile, 0, lane);
+                    found = not_finite<T, PANELS>(tile, 64, lane) || found;
+                }
+                if (lane == 0) {
+                    dirty[2 * stage.at + warp - 2] = found;
+                    arrive(searched + stage.at);
+                    arrive(empty + stage.at);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int half = (warp >> 2) - 1, quarter = (warp & 3) * 32;
+        const int row = min(t.first + quarter + lane, t.end - 1);
+        const bool there = t.first + quarter + lane < t.end;
+        const uint32_t lanes = uint32_t(quarter) << 16, score = tmem + lanes + half * 64, grade = score + kTile;
+        const float scale = a.scale * kLog2e, lift = gradient_lift<T>(b, t.sequence);
+        const f32x2 scale2 = pack2(scale, scale), lift2 = pack2(lift * exp2f(-kWeightLift<T>), lift * exp2f(-kWeightLift<T>)), weight_lift2 = pack2(kWeightLift<T>, kWeightLift<T>);
+        const f32x2 minus = pack2(-1.0f, -1.0f);
+        const int seen_low = first_seeing(a, t.begin, row), seen_high = last_seeing(a, t.end, row);
+        const int middle = min((a.width / 2 + 15) & ~15, a.width);                // columns of sums, where the two warpgroups share them
+        uint32_t meetings = 0;
+        const auto meet = [&] { return all_meet(met, meetings, lane, failed); };
+        Ring<S::stages> stage;
+        bool ok = true;
+        for (int i = 0; i < n; ++i, stage.next()) {
+            const int q0 = query_row(i), from = seen_low - q0, to = seen_high - q0;
+            const bool masked = !whole(q0);
+            const unsigned char* place = ring + stage.at * S::stage_bytes;
+            const float4* statistics = reinterpret_cast<const float4*>(place + 2 * S::bytes) + half * 16;
+            ok = __all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed) && wait_in_line(scored, i & 1, failed));
+            if (!ok) break;
+            tmem_fence_after();
+            uint32_t p[64];
+            tmem_begin32(score, p);
+            tmem_begin32(score + 32, p + 32);
+            tmem_loaded();
+            #pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t words[16];
+                #pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 sums = statistics[(c + k) / 4];
+                    #pragma unroll
+                    for (int h = 0; h < 4; h += 2) {
+                        const f32x2 off = fma2(h ? pack2(sums.z, sums.w) : pack2(sums.x, sums.y), minus, weight_lift2);
+                        const float2 x = unpack2(fma2(pack2(__uint_as_float(p[c + k + h]), __uint_as_float(p[c + k + h + 1])), scale2, off));
+                        float p0 = exp2_approx(x.x), p1 = exp2_approx(x.y);
+                        if (masked) {
+                            p0 = counts(c + k + h + half * 64, from, to) ? p0 : 0.0f;
+                            p1 = counts(c + k + h + 1 + half * 64, from, to) ? p1 : 0.0f;
+                        }
+                        p[c + k + h] = __float_as_uint(p0);
+                        p[c + k + h + 1] = __float_as_uint(p1);
+                        words[(k + h) / 2] = floats_pair<T>(p0, p1);
+                    }
+                }
+                tmem_store16(score + c / 2, words);
+            }
+            tmem_stored();
+            uint32_t spoilt[2] = {0, 0};
+            if (masked) {
+                ok = __all_sync(0xffffffffu, wait_in_line(searched + stage.at, stage.round, failed));
+                if (!ok) break;
+                spoilt[0] = dirty[2 * stage.at]; spoilt[1] = dirty[2 * stage.at + 1];
+                if (spoilt[0]) {
+                    ok = meet();             // the other columns' weights
+                    if (!ok) break;
+                    multiply_seen<T>(tmem + lanes + 2 * kTile, half ? middle : 0, half ? a.width : middle, i > 0, tmem + lanes, 64, place + S::bytes, from, to);
+                }
+            }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(weighed);
+            ok = __all_sync(0xffffffffu, wait_in_line(graded, i & 1, failed));
+            if (!ok) break;
+            tmem_fence_after();
+            #pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t g[32], words[16];
+                tmem_begin32(grade + c, g);
+                tmem_loaded();
+                #pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 means = statistics[32 + (c + k) / 4];
+                    #pragma unroll
+                    for (int h = 0; h < 4; h += 2) {
+                        const f32x2 away = fma2(h ? pack2(means.z, means.w) : pack2(means.x, means.y), minus, pack2(__uint_as_float(g[k + h]), __uint_as_float(g[k + h + 1])));
+                        float2 ds = unpack2(mul2(mul2(pack2(__uint_as_float(p[c + k + h]), __uint_as_float(p[c + k + h + 1])), lift2), away));
+                        if (masked) {
+                            ds.x = counts(c + k + h + half * 64, from, to) ? ds.x : 0.0f;
+                            ds.y = counts(c + k + h + 1 + half * 64, from, to) ? ds.y : 0.0f;
+                        }
+                        words[(k + h) / 2] = floats_pair<T>(ds.x, ds.y);
+                    }
+                }
+                tmem_store16(grade + c / 2, words);
+            }
+            tmem_stored();
+            if (spoilt[1]) {
+                ok = meet();
+                if (!ok) break;
+                multiply_seen<T>(tmem + lanes + 3 * kTile, half ? middle : 0, half ? a.width : middle, i > 0, tmem + lanes + kTile, 64, place, from, to);
+            }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(changed);
+        }
+        ok = ok && __all_sync(0xffffffffu, wait_in_line(finished, 0, failed));
+        if (ok) {
+            tmem_fence_after();
+            const int64_t at = (int64_t(row) * a.key_heads + key_head) * a.width;
+            if (half == 0) store_sums<T>(tmem + lanes + 2 * kTile, static_cast<T*>(b.grad_v) + at, 0, a.width, exp2f(-kWeightLift<T>), there);
+            else store_sums<T>(tmem + lanes + 3 * kTile, static_cast<T*>(b.grad_k) + at, 0, a.width, a.scale / lift, there);
+        }
+        tmem_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (*failed) {
+        nan_rows<T>(b.grad_k, t, a.key_heads, key_head, a.width);
+        nan_rows<T>(b.grad_v, t, a.key_heads, key_head, a.width);
+        if (threadIdx.x == 0) {
+            *reinterpret_cast<volatile unsigned int*>(args.error) = 1;
+            __threadfence_system();
+        }
+    }
+}
+
+// Gradient of q of a tile.  Scores are computed a tile ahead.  Tensor memory: scores (score gradients) by turns at 0 and 128, weight gradients 256, dq 384.
+template <typename T, int PANELS>
+__global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                            const __grid_constant__ CUtensorMap map_grad, const __grid_constant__ BackwardArgs args) {
+    using S = QueriesTile<PANELS>;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* const own = raw + (base - smem_u32(raw));            // q, dout
+    unsigned char* const ring = own + 2 * S::bytes;
+    const uint32_t ring_at = base + 2 * S::bytes;
+    uint64_t* const own_full = reinterpret_cast<uint64_t*>(ring + S::stages * S::bytes);
+    uint64_t* const full = own_full + 1;
+    uint64_t* const empty = full + S::stages;
+    uint64_t* const searched = empty + S::stages;
+    uint64_t* const scored = searched + S::stages;       // [2]
+    uint64_t* const graded = scored + 2;
+    uint64_t* const changed = graded + 1;
+    uint64_t* const finished = changed + 1;
+    uint64_t* const met = finished + 1;
+    uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(met + 1);
+    volatile uint32_t* const failed = tmem_at + 1;
+    volatile uint32_t* const dirty = failed + 1;         // [stages][2], of halves of a tile of keys
+
+    const HtgsAttention& a = args.a;
+    const AttentionBackward& b = args.b;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    grid_dependency();
+    const int head = int(blockIdx.x % a.heads), key_head = head / (a.heads / a.key_heads);
+    const SequenceTile t = find_tile<kTile>(a, int(gridDim.x / a.heads - 1 - blockIdx.x / a.heads));
+    if (t.first >= t.end) return;
+    if (t.outside) {
+        zero_rows<T>(b.grad_q, t, a.heads, head, a.width);
+        return;
+    }
+    const int last_row = min(t.first + kTile, t.end) - 1;
+    const int low = first_seen(a, t.begin, t.first), n = (last_seen(a, t.end, last_row) - low) / kTile + 1;
+    const int whole_low = first_seen(a, t.begin, last_row), whole_high = last_seen(a, t.end, t.first);
+    const auto whole = [&](int j) { return low + j * kTile >= whole_low && low + j * kTile + kTile - 1 <= whole_high; };
+
+    if (threadIdx.x == 0) {
+        mbar_init(own_full, 1); mbar_init(scored, 1); mbar_init(scored + 1, 1); mbar_init(graded, 1); mbar_init(changed, 8); mbar_init(finished, 1); mbar_init(met, 8);
+        for (int i = 0; i < S::stages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 3); mbar_init(searched + i, 2); }
+        *failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tmem_fence_before();
+    }
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            const bool one = elect_one();
+            if (one) {
+                mbar_arrive_expect_tx(own_full, 2 * S::bytes);
+                for (int p = 0; p < PANELS; ++p) {
+                    load_panel(own + p * kPanelBytes, &map_q, p * kPanel, head, t.first, own_full);
+                    load_panel(own + S::bytes + p * kPanelBytes, &map_grad, p * kPanel, head, t.first, own_full);
+                }
+            }
+            __syncwarp();
+            Ring<S::stages> stage;
+            uint32_t uses = 0;
+            bool ok = true;
+            for (int i = 0; i < 2 * n; ++i, ++uses, stage.next()) {           // keys and values of a tile by turns
+                ok = __all_sync(0xffffffffu, wait_in_line(empty + stage.at, stage.round ^ 1, failed));
+                if (!ok) break;
+                if (one) {
+                    mbar_arrive_expect_tx(full + stage.at, S::bytes);
+                    for (int p = 0; p < PANELS; ++p) load_panel(ring + stage.at * S::bytes + p * kPanelBytes, i & 1 ? &map_v : &map_k, p * kPanel, key_head, low + (i >> 1) * kTile, full + stage.at);
+                }
+                __syncwarp();
+            }
+            if (!ok) {              // no copy may be on its way when the block ends
+                for (uint32_t u = uses > S::stages ? uses - S::stages : 0; u < uses; ++u) {
+                    WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                    while (!mbar_try_wait(full + u % S::stages, u / S::stages & 1) && !limit.over(nanoseconds())) {}
+                }
+                WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                while (!mbar_try_wait(own_full, 0) && !limit.over(nanoseconds())) {}
+            }
+        } else if (warp == 1) {
+            const bool one = elect_one();
+            const uint32_t score = instruction<T>(kTile, false), sum = instruction<T>((a.width + 15) & ~15, true);
+            const int steps = (a.width + 15) / 16;
+            Ring<S::stages> stage;
+            uint32_t key_slot[2] = {0, 0};
+            bool ok = true;
+            const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_in_line(bar, parity, failed)); };
+            // scores of a tile (which 0), or gradients of its weights (1), from the next place of the ring
+            const auto product = [&](int which, int j) {
+                wait(full + stage.at, stage.round);
+                if (!ok) return;
+                tmem_fence_after();
+                const uint32_t x = along_columns(base + which * S::bytes), y = along_columns(ring_at + stage.at * S::bytes), d = tmem + (which ? 2 * kTile : (j & 1) * kTile);
+                if (one) {
+                    for (int i = 0; i < steps; ++i) {
+                        const uint32_t at = (i >> 2) * kPanelUnits + (i & 3) * 2;
+                        multiply(d, x + at, y + at, score, i > 0);
+                    }
+                    commit(which ? graded : scored + (j & 1));
+                    if (which) commit(empty + stage.at);
+                }
+                __syncwarp();
+                if (!which) key_slot[j & 1] = stage.at;
+                stage.next();
+            };
+            wait(own_full, 0);
+            if (ok) product(0, 0);
+            if (ok) product(1, 0);
+            if (ok && n > 1) product(0, 1);
+            for (int j = 0; j < n && ok; ++j) {
+                wait(changed, j & 1);
+                if (!ok) break;
+                tmem_fence_after();
+                const uint32_t slot = key_slot[j & 1], y = along_rows(ring_at + slot * S::bytes), w = tmem + (j & 1) * kTile;
+                const bool added = !whole(j) && (dirty[2 * slot] | dirty[2 * slot + 1]);
+                if (one) {
+                    #pragma unroll
+                    for (int i = 0; i < (added ? 0 : kTile / 16); ++i) multiply_tmem(tmem + 3 * kTile, w + (i >> 2) * 64 + (i & 3) * 8, y + i * (2048 >> 4), sum, j > 0 || i > 0);
+                    commit(empty + slot);
+                }
+                __syncwarp();
+                if (j + 1 < n) product(1, j + 1);
+                if (ok && j + 2 < n) product(0, j + 2);
+            }
+            if (one && ok) commit(finished);
+            __syncwarp();
+        } else {
+            Ring<S::stages> stage;
+            for (int i = 0; i < 2 * n; ++i, stage.next()) {
+                if (!__all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed))) break;
+                const bool found = !(i & 1) && !whole(i >> 1) && not_finite<T, PANELS>(ring + stage.at * S::bytes, (warp - 2) * 64, lane);
+                if (lane == 0) {
+                    dirty[2 * stage.at + warp - 2] = found;
+                    arrive(searched + stage.at);
+                    arrive(empty + stage.at);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int half = (warp >> 2) - 1, quarter = (warp & 3) * 32;
+        const int row = min(t.first + quarter + lane, t.end - 1);
+        const bool there = t.first + quarter + lane < t.end;
+        const uint32_t lanes = uint32_t(quarter) << 16;
+        const float scale = a.scale * kLog2e, lift = gradient_lift<T>(b, t.sequence);
+        const float* statistics = b.statistics + (head * b.statistics_rows + statistic_base(a, t) + (t.first - t.begin)) * 2 + quarter + lane;
+        const float row_sum = there ? statistics[0] : 0.0f, mean = there ? statistics[kStatisticRows] : 0.0f;
+        const f32x2 scale2 = pack2(scale, scale), off2 = pack2(-row_sum, -row_sum), mean2 = pack2(-mean, -mean), lift2 = pack2(lift, lift);
+        const int row_low = first_seen(a, t.begin, row), row_high = last_seen(a, t.end, row);
+        const int middle = min((a.width / 2 + 15) & ~15, a.width);
+        uint32_t meetings = 0;
+        const auto meet = [&] { return all_meet(met, meetings, lane, failed); };
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const uint32_t score = tmem + lanes + (j & 1) * kTile + half * 64, grade = tmem + lanes + 2 * kTile + half * 64;
+            const int from = row_low - (low + j * kTile), to = row_high - (low + j * kTile);
+            const bool masked = !whole(j);
+            ok = __all_sync(0xffffffffu, wait_in_line(scored + (j & 1), j >> 1 & 1, failed));
+            if (!ok) break;
+            tmem_fence_after();
+            uint32_t p[64];
+            tmem_begin32(score, p);
+            tmem_begin32(score + 32, p + 32);
+            tmem_loaded();
+            #pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+                const float2 x = unpack2(fma2(pack2(__uint_as_float(p[c]), __uint_as_float(p[c + 1])), scale2, off2));
+                p[c] = __float_as_uint(exp2_approx(x.x));
+                p[c + 1] = __float_as_uint(exp2_approx(x.y));
+            }
+            ok = __all_sync(0xffffffffu, wait_in_line(graded, j & 1, failed));
+            if (!ok) break;
+            tmem_fence_after();
+            #pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t g[32], words[16];
+                tmem_begin32(grade + c, g);
+                tmem_loaded();
+                #pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    const f32x2 away = add2(pack2(__uint_as_float(g[k]), __uint_as_float(g[k + 1])), mean2);
+                    float2 ds = unpack2(mul2(mul2(pack2(__uint_as_float(p[c + k]), __uint_as_float(p[c + k + 1])), lift2), away));
+                    if (masked) {
+                        ds.x = counts(c + k + half * 64, from, to) ? ds.x : 0.0f;
+                        ds.y = counts(c + k + 1 + half * 64, from, to) ? ds.y : 0.0f;
+                    }
+                    words[k / 2] = floats_pair<T>(ds.x, ds.y);
+                }
+                tmem_store16(score + c / 2, words);
+            }
+            tmem_stored();
+            if (masked) {
+                const uint32_t at = uint32_t(2 * j) % S::stages, round = uint32_t(2 * j) / S::stages & 1;
+                ok = __all_sync(0xffffffffu, wait_in_line(searched + at, round, failed));
+                if (!ok) break;
+                if (dirty[2 * at] | dirty[2 * at + 1]) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(full + at, round, failed)) && meet();             // the other columns' score gradients
+                    if (!ok) break;
+                    multiply_seen<T>(tmem + lanes + 3 * kTile, half ? middle : 0, half ? a.width : middle, j > 0, tmem + lanes + (j & 1) * kTile, 64, ring + at * S::bytes, from, to);
+                }
+            }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(changed);
+        }
+        ok = ok && __all_sync(0xffffffffu, wait_in_line(finished, 0, failed));
+        if (ok) {
+            tmem_fence_after();
+            store_sums<T>(tmem + lanes + 3 * kTile, static_cast<T*>(b.grad_q) + (int64_t(row) * a.heads + head) * a.width, half ? middle : 0, half ? a.width : middle, a.scale / lift, there);
+        }
+        tmem_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (*failed) {
+        nan_rows<T>(b.grad_q, t, a.heads, head, a.width);
+        if (threadIdx.x == 0) {
+            *reinterpret_cast<volatile unsigned int*>(args.error) = 1;
+            __threadfence_system();
+        }
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------
+
+// [rows, heads, width] in boxes of 128 rows and a panel of one head's columns.
+bool make_rows_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int width, int64_t stride, int64_t head_stride) {
+    const cuuint64_t dense = cuuint64_t(width) * 2;                 // a stride that takes no step says nothing
+    const cuuint64_t sizes[3] = {cuuint64_t(width), cuuint64_t(heads), cuuint64_t(rows)};
+    const cuuint64_t strides[2] = {heads > 1 ? cuuint64_t(head_stride) * 2 : dense, rows > 1 ? cuuint64_t(stride) * 2 : dense * cuuint64_t(heads)};
+    const cuuint32_t box[3] = {kPanel, 1, kTile}, steps[3] = {1, 1, 1};
+    const EncodeTiled encode = encode_tiled();
+    return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool heads_aligned(const void* p, int64_t rows, int heads, int64_t stride, int64_t head_stride) {
+    const auto step = [](int64_t s) { return s > 0 && s % 8 == 0 && s < (int64_t(1) << 38); };
+    return aligned(p, 16) && (rows == 1 || step(stride)) && (heads == 1 || step(head_stride));
+}
+
+template <typename T, int PANELS> int launch_forward(const ForwardArgs& args, cudaStream_t stream) {
+    using S = ForwardTile<PANELS>;
+    const HtgsAttention& a = args.a;
+    CUtensorMap q, k, v;
+    if (!make_rows_map(&q, a.q, a.rows, a.heads, a.width, a.q_stride, a.q_head_stride) || !make_rows_map(&k, a.k, a.rows, a.key_heads, a.width, a.k_stride, a.k_head_stride) ||
+        !make_rows_map(&v, a.v, a.rows, a.key_heads, a.width, a.v_stride, a.v_head_stride))
+        return sequence_fail(HTGS_ERR_CUDA, "htgs_attention: the tensor maps cannot be made");
+    static PerDeviceOnce once;
+    cudaError_t err = once.run([] { return cudaFuncSetAttribute(attention_tiles_kernel<T, PANELS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem); });
+    if (err == cudaSuccess) err = launch_after(attention_tiles_kernel<T, PANELS>, dim3(unsigned(sequence_tiles(a, 2 * kTile) * a.heads)), kTilesThreads, S::smem, stream, q, k, v, args);
+    return err == cudaSuccess ? sequence_status("htgs_attention") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
+template <typename T, int PANELS> int launch_backward(const BackwardArgs& args, cudaStream_t stream) {
+    const HtgsAttention& a = args.a;
+    CUtensorMap q, k, v, grad;
+    if (!make_rows_map(&q, a.q, a.rows, a.heads, a.width, a.q_stride, a.q_head_stride) || !make_rows_map(&k, a.k, a.rows, a.key_heads, a.width, a.k_stride, a.k_head_stride) ||
+        !make_rows_map(&v, a.v, a.rows, a.key_heads, a.width, a.v_stride, a.v_head_stride) || !make_rows_map(&grad, args.b.grad, a.rows, a.heads, a.width, args.b.grad_stride, args.b.grad_head_stride))
+        return sequence_fail(HTGS_ERR_CUDA, "htgs_attention_backward: the tensor maps cannot be made");
+    static PerDeviceOnce once;
+    cudaError_t err = once.run([] {
+        const cudaError_t e = cudaFuncSetAttribute(attention_keys_kernel<T, PANELS>, cudaFuncAttributeMaxDynamicSharedMemorySize, KeysTile<PANELS>::smem);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(attention_queries_kernel<T, PANELS>, cudaFuncAttributeMaxDynamicSharedMemorySize, QueriesTile<PANELS>::smem);
+    });
+    const int64_t tiles = sequence_tiles(a, kTile);
+    if (err == cudaSuccess) err = launch_after(attention_keys_kernel<T, PANELS>, dim3(unsigned(tiles * a.key_heads)), kTilesThreads, KeysTile<PANELS>::smem, stream, q, k, v, grad, args);
+    if (err == cudaSuccess) err = launch_after(attention_queries_kernel<T, PANELS>, dim3(unsigned(tiles * a.heads)), kTilesThreads, QueriesTile<PANELS>::smem, stream, q, k, v, grad, args);
+    return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
+template <typename T> int backward_typed(const BackwardArgs& args, cudaStream_t stream) {
+    return args.a.width <= kPanel ? launch_backward<T, 1>(args, stream) : launch_backward<T, 2>(args, stream);
+}
+template <typename T> int forward_typed(const ForwardArgs& args, cudaStream_t stream) {
+    return args.a.width <= kPanel ? launch_forward<T, 1>(args, stream) : launch_forward<T, 2>(args, stream);
+}
+
+}  // namespace
+
+bool attention_tiles_take(const HtgsAttention& a, const void* out) {
+    return a.type != HTGS_FLOAT32 && a.width % 8 == 0 && aligned(out, 16) && heads_aligned(a.q, a.rows, a.heads, a.q_stride, a.q_head_stride) &&
+           heads_aligned(a.k, a.rows, a.key_heads, a.k_stride, a.k_head_stride) && heads_aligned(a.v, a.rows, a.key_heads, a.v_stride, a.v_head_stride);
+}
+
+bool attention_tiles_take(const HtgsAttention& a, const AttentionBackward& b) {
+    return attention_tiles_take(a, b.grad_q) && aligned(b.grad_k, 16) && aligned(b.grad_v, 16) && heads_aligned(b.grad, a.rows, a.heads, b.grad_stride, b.grad_head_stride);
+}
+
+int attention_tiles_backward(const HtgsAttention& a, const AttentionBackward& b, cudaStream_t stream) {
+    unsigned int* error = attention_error_word(current_device());
+    if (!error) return sequence_fail(HTGS_ERR_CUDA, "htgs_attention_backward: no host memory for the error word");
+    const BackwardArgs args{a, b, error};
+    return a.type == HTGS_FLOAT16 ? backward_typed<__half>(args, stream) : backward_typed<__nv_bfloat16>(args, stream);
+}
+
+int attention_tiles_forward(const HtgsAttention& a, void* out, float* sums, cudaStream_t stream) {
+    unsigned int* error = attention_error_word(current_device());
+    if (!error) return sequence_fail(HTGS_ERR_CUDA, "htgs_attention: no host memory for the error word");
+    const ForwardArgs args{a, out, sums, error};
+    return a.type == HTGS_FLOAT16 ? forward_typed<__half>(args, stream) : forward_typed<__nv_bfloat16>(args, stream);
+}
+
+}  // namespace htgs

@@ -28,6 +28,16 @@ static __device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, v
         if (limit.over(nanoseconds())) { *failed = 1; return false; }
     }
 }
+// The same in line, for kernels that give registers from one warp to another, which may not call.
+__device__ __forceinline__ bool wait_in_line(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
+    if (mbar_try_wait(bar, parity)) return true;
+    WaitLimit limit(kWaitNanoseconds, nanoseconds());
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*failed) return false;
+        if (limit.over(nanoseconds())) { *failed = 1; return false; }
+    }
+}
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
     return mbar_try_wait(bar, parity) || wait_longer(smem_u32(bar), parity, failed);
 }

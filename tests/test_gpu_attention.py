@@ -161,11 +161,12 @@ def test_rows_of_no_sequence_get_zeros_and_leave_no_trace(kind):
     leaves = [t.requires_grad_(True) for t in (q, k, v)]
     out = seq.attention(*leaves, offsets=offsets, causal=True)
     grads = torch.autograd.grad(out, leaves, grad)
-    inner = [t.detach()[37:300].contiguous().requires_grad_(True) for t in leaves]
-    alone = seq.attention(*inner, offsets=offsets - 37, causal=True)
-    for a, b in zip((out, *grads), (alone, *torch.autograd.grad(alone, inner, grad[37:300].contiguous()))):
-        assert torch.equal(a[37:300], b)
-        assert not a[:37].any() and not a[300:].any()
+    # Beside values that are not finite a tile is summed up in another order than without them, each sum within the bound: n terms off by 2 F of their magnitudes, then one rounding.
+    inner = [f64(t)[37:300] for t in (*leaves, grad)]
+    want, bound = ref.attend(*inner[:3], [0, 63, 263], True, None, 0.125, kind, inner[3])
+    for name, t in zip(("out", "gq", "gk", "gv"), (out, *grads)):
+        near(t[37:300], want[name], bound[name], name)
+        assert not t[:37].any() and not t[300:].any()
 
 
 @pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
@@ -185,12 +186,13 @@ def test_what_a_row_does_not_see_does_not_reach_it(kind, bad):
     spoilt = [t.clone() for t in (q, k, v, grad)]
     for t in spoilt:
         t[200:390, :, 3] = bad
-    clean, dirty = run(q, k, v, grad), run(*spoilt)
-    other = torch.cat((torch.arange(60), torch.arange(390, rows))).cuda()
-    for name, a, b in zip(("out", "gq", "gk", "gv"), clean, dirty):
-        assert torch.equal(a[other], b[other]), name
-    for name, a, b in zip(("out", "gq"), clean, dirty):           # keys before them are seen by queries behind: only these
-        assert torch.equal(a[60:200], b[60:200]), name
+    dirty = run(*spoilt)
+    want, bound = ref.attend(f64(q), f64(k), f64(v), ends, True, 300, 0.125, kind, f64(grad))          # as above: within the bound, not bit for bit
+    other = torch.cat((torch.arange(60), torch.arange(390, rows)))
+    for name, t in zip(("out", "gq", "gk", "gv"), dirty):
+        near(t[other.cuda()], want[name][other], bound[name][other], name)
+    for name, t in zip(("out", "gq"), dirty):           # keys before them are seen by queries behind: only these
+        near(t[60:200], want[name][60:200], bound[name][60:200], name)
     assert dirty[0][200:390].isnan().any()
 
 
