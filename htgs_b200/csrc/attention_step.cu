@@ -10,7 +10,7 @@ namespace htgs {
 
 namespace {
 
-constexpr int kStepThreads = 256, kStepWarps = kStepThreads / 32, kMostStepWidth = 128, kStepColumns = kMostStepWidth / 32, kStepPiece = 16, kMostSplits = 256;
+constexpr int kStepThreads = 256, kStepWarps = kStepThreads / 32, kMostStepWidth = 128, kStepColumns = kMostStepWidth / 32, kStepPiece = 32, kMostSplits = 256;
 
 struct StepRows { int low, length; bool left_out, full; };        // rows [low, length], the last one new
 
@@ -96,6 +96,211 @@ template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes
     if (splits > 1 && threadIdx.x == 0) *reinterpret_cast<float2*>(parts + (at * splits + split) * part_floats(a.width)) = make_float2(most, sum);
 }
 
+// ---- 16-bit heads on 16 bytes: matrix instructions of a warp ---------------------------------------------------------------------------
+//
+// A block has the query heads of a key head, up to 16 rows of a matrix, and a split of the sequence.  Each of its warps brings 32 keys and values at a time into places of its own in shared memory, one or two
+// sets on their way while one is used, and goes its own way until the end: no barrier of the block.  Products are m16n8k16; the arithmetic is a tenth of what they could do, so rows that no head fills cost nothing.
+// (tcgen05 takes 128 rows at least, of which 4 to 16 would be used, and its accumulators would have to come out of tensor memory for every 32 keys.)
+
+constexpr int kTileWarps = 4, kTileKeys = 32, kTileStages = 3, kTileHeads = 16;
+// Weights are at most 1: fp16 ones carry 2^15, so that one of 2^-29 is a normal number.
+template <typename T> constexpr float kStepLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
+
+// Where piece `piece` (16 bytes) of a row of W values lies: eight rows of a piece are in banks of their own.
+template <int W> __device__ __forceinline__ uint32_t place_of(int row, int piece) {
+    return uint32_t(row * W * 2 + (W >= 64 ? piece ^ (row & 7) : piece ^ (row >> 1 & 3)) * 16);
+}
+__device__ __forceinline__ void load_matrices(uint32_t address, uint32_t (&v)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void load_turned(uint32_t address, uint32_t (&v)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(address) : "memory");
+}
+template <typename T> __device__ __forceinline__ void multiply_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T, int W>        // W: the width rounded up to 32, 64 or 128
+__global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsAttentionStep a, T* out, float* parts, int splits, int chunks) {
+    constexpr int kSteps = W / 16, kPieces = W / 8, kCopies = kTileKeys * kPieces / 32, kRowsOfCopy = 32 / kPieces, kSetBytes = kTileKeys * W * 2;
+    extern __shared__ __align__(16) unsigned char shared[];
+    grid_dependency();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    int rest = int(blockIdx.x);
+    const int split = rest % splits; rest /= splits;
+    const int chunk = rest % chunks; rest /= chunks;
+    const int key_head = rest % a.key_heads, b = rest / a.key_heads;
+    const int group = a.heads / a.key_heads, first_head = key_head * group + chunk * kTileHeads, heads = min(kTileHeads, group - chunk * kTileHeads);
+    const StepRows r = rows_of(a, b);
+    const bool any = !r.left_out && !r.full;
+    float most[2] = {-infinity(), -infinity()}, sum[2] = {0.0f, 0.0f}, o[kPieces][4] = {};
+    if (any) {
+        const int2 rows = rows_of_split(r, split, splits);
+        unsigned char* const mine = shared + warp * kTileStages * 2 * kSetBytes;
+        const uint32_t mine_at = smem_u32(mine);
+        if (a.width < W) {               // columns that are not there: zeros, which no copy overwrites
+            for (int i = lane; i < kTileStages * 2 * kTileKeys * kPieces; i += 32) {
+                const int row = i / kPieces, piece = i % kPieces;
+                if (piece * 8 >= a.width) *reinterpret_cast<uint4*>(mine + row / kTileKeys * kSetBytes + place_of<W>(row % kTileKeys, piece)) = make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
+        }
+        // a lane copies piece lane % kPieces of every kRowsOfCopy-th row
+        const int piece = lane % kPieces, row0 = lane / kPieces;
+        const T* const keys = static_cast<const T*>(a.keys) + b * a.keys_stride + key_head * a.keys_head_stride + piece * 8;
+        const T* const values = static_cast<const T*>(a.values) + b * a.values_stride + key_head * a.values_head_stride + piece * 8;
+        const T* const new_key = static_cast<const T*>(a.k) + b * a.k_stride + key_head * a.k_head_stride + piece * 8;
+        const T* const new_value = static_cast<const T*>(a.v) + b * a.v_stride + key_head * a.v_head_stride + piece * 8;
+        const bool mine_there = piece * 8 < a.width;
+        const auto begin = [&](int first, int stage) {          // rows first + [0, 32); what lies behind the split's last row is zero
+            const uint32_t to = mine_at + stage * 2 * kSetBytes;
+            if (mine_there && first < rows.y) {
+                #pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    const int row = row0 + i * kRowsOfCopy, j = first + row;
+                    const T* k = j == r.length ? new_key : keys + j * a.keys_row_stride;
+                    const T* v = j == r.length ? new_value : values + j * a.values_row_stride;
+                    const uint32_t bytes = j < rows.y ? 16u : 0u;
+                    if (bytes == 0) { k = new_key; v = new_value; }
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + place_of<W>(row, piece)), "l"(k), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + kSetBytes + place_of<W>(row, piece)), "l"(v), "r"(bytes) : "memory");
+                }
+            }
+            copies_begun();
+        };
+        // queries: rows lane / 4 and 8 more, columns 2 (lane % 4) and 8 more of each step
+        uint32_t q[kSteps][4];
+        #pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int head = lane / 4 + (i & 1) * 8, column = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+                q[k][i] = head < heads && column < a.width ? __ldg(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + b * a.q_stride + (first_head + head) * a.q_head_stride + column)) : 0u;
+            }
+        const float scale = a.scale * kLog2e;
+        int first = rows.x + warp * kTileKeys, stage = 0;
+        #pragma unroll
+        for (int i = 0; i < kTileStages - 1; ++i) begin(first + i * kTileWarps * kTileKeys, i);
+        for (; first < rows.y; first += kTileWarps * kTileKeys) {
+            begin(first + (kTileStages - 1) * kTileWarps * kTileKeys, stage == 0 ? kTileStages - 1 : stage - 1);
+            copies_done<kTileStages - 1>();
+            const uint32_t at = mine_at + stage * 2 * kSetBytes;
+            float s[kTileKeys / 8][4] = {};
+            #pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+                #pragma unroll
+                for (int n = 0; n < kTileKeys / 16; ++n) {
+                    uint32_t m[4];
+                    load_matrices(at + place_of<W>(n * 16 + (lane >> 4) * 8 + (lane & 7), 2 * k + (lane >> 3 & 1)), m);
+                    multiply_add<T>(s[2 * n], q[k], m[0], m[1]);
+                    multiply_add<T>(s[2 * n + 1], q[k], m[2], m[3]);
+                }
+            float now[2] = {most[0], most[1]};
+            #pragma unroll
+            for (int n = 0; n < kTileKeys / 8; ++n)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[n][i] = first + n * 8 + (lane & 3) * 2 + (i & 1) < rows.y ? s[n][i] * scale : -infinity();
+                    now[i >> 1] = fmaxf(now[i >> 1], s[n][i]);
+                }
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                now[i] = fmaxf(now[i], __shfl_xor_sync(0xffffffffu, now[i], 1));
+                now[i] = fmaxf(now[i], __shfl_xor_sync(0xffffffffu, now[i], 2));
+            }
+            if (__any_sync(0xffffffffu, now[0] > most[0] || now[1] > most[1])) {
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float factor = now[i] == most[i] ? 1.0f : exp2_approx(most[i] - now[i]);
+                    most[i] = now[i];
+                    sum[i] *= factor;
+                    #pragma unroll
+                    for (int c = 0; c < kPieces; ++c) { o[c][2 * i] *= factor; o[c][2 * i + 1] *= factor; }
+                }
+            }
+            uint32_t p[kTileKeys / 8][2];
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float base = (most[i] == -infinity() ? 0.0f : most[i]) - kStepLift<T>;
+                #pragma unroll
+                for (int n = 0; n < kTileKeys / 8; ++n) {
+                    const float p0 = exp2_approx(s[n][2 * i] - base), p1 = exp2_approx(s[n][2 * i + 1] - base);
+                    sum[i] += p0 + p1;
+                    p[n][i] = floats_pair<T>(p0, p1);
+                }
+            }
+            #pragma unroll
+            for (int n = 0; n < kTileKeys / 16; ++n) {
+                const uint32_t weights[4] = {p[2 * n][0], p[2 * n][1], p[2 * n + 1][0], p[2 * n + 1][1]};
+                #pragma unroll
+                for (int c = 0; c < kPieces; c += 2) {
+                    uint32_t m[4];
+                    load_turned(at + kSetBytes + place_of<W>(n * 16 + (lane >> 3 & 1) * 8 + (lane & 7), c + (lane >> 4)), m);
+                    multiply_add<T>(o[c], weights, m[0], m[1]);
+                    multiply_add<T>(o[c + 1], weights, m[2], m[3]);
+                }
+            }
+            stage = stage + 1 == kTileStages ? 0 : stage + 1;
+            __syncwarp();                // before the place is filled again
+        }
+        copies_done<0>();
+        if (chunk == 0 && rows.y == r.length + 1 && rows.x < rows.y) append<T>(a, b, key_head, r.length);
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+        }
+    }
+    // the warps' parts, joined: [warp][head]{largest, sum} and [warp][head][W]
+    constexpr int kPitch = W + 4;
+    float2* const tops = reinterpret_cast<float2*>(shared);
+    float* const outputs = reinterpret_cast<float*>(tops + kTileWarps * kTileHeads);
+    __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int head = lane / 4 + 8 * i;
+        if ((lane & 3) == 0) tops[warp * kTileHeads + head] = make_float2(most[i], sum[i]);
+        #pragma unroll
+        for (int c = 0; c < kPieces; ++c)
+            *reinterpret_cast<float2*>(outputs + (warp * kTileHeads + head) * kPitch + c * 8 + (lane & 3) * 2) = make_float2(o[c][2 * i], o[c][2 * i + 1]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * (a.width / 8); i += kTileWarps * 32) {
+        const int head = i / (a.width / 8), c = i % (a.width / 8) * 8;
+        float largest = -infinity(), all = 0.0f, total[8] = {};
+        #pragma unroll
+        for (int w = 0; w < kTileWarps; ++w) largest = fmaxf(largest, tops[w * kTileHeads + head].x);
+        const float base = largest == -infinity() ? 0.0f : largest;
+        #pragma unroll
+        for (int w = 0; w < kTileWarps; ++w) {
+            const float2 top = tops[w * kTileHeads + head];
+            const float factor = exp2_approx(top.x - base);
+            all = fmaf(top.y, factor, all);
+            float v[8];
+            load_floats<float, 4>(outputs + (w * kTileHeads + head) * kPitch + c, *reinterpret_cast<float (*)[4]>(v));
+            load_floats<float, 4>(outputs + (w * kTileHeads + head) * kPitch + c + 4, *reinterpret_cast<float (*)[4]>(v + 4));
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) total[k] = fmaf(v[k], factor, total[k]);
+        }
+        const int64_t at = int64_t(b) * a.heads + first_head + head;
+        if (splits > 1) {
+            float* to = parts + (at * splits + split) * part_floats(a.width);
+            *reinterpret_cast<float4*>(to + 4 + c) = make_float4(total[0], total[1], total[2], total[3]);
+            *reinterpret_cast<float4*>(to + 8 + c) = make_float4(total[4], total[5], total[6], total[7]);
+            if (c == 0) *reinterpret_cast<float2*>(to) = make_float2(largest, all);
+        } else {
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) total[k] = r.left_out ? 0.0f : any ? total[k] / all : __uint_as_float(0x7fffffffu);
+            store_floats<T, 8>(out + at * a.width + c, total);
+        }
+    }
+}
+
 // The splits of a head, joined.
 template <typename T> __global__ void __launch_bounds__(kMostStepWidth) step_join_kernel(const HtgsAttentionStep a, T* out, const float* parts, int splits) {
     __shared__ float factors[kMostSplits];
@@ -139,19 +344,50 @@ const char* wrong(const HtgsAttentionStep* a) {
     return nullptr;
 }
 
-// Blocks for each head (or key head and its query heads): enough to fill the GPU, none with fewer than 256 rows of a full cache.
-int splits_of(const HtgsAttentionStep& a, int64_t blocks) {
-    const int64_t rows = a.window >= 0 && a.window < a.capacity ? a.window + 1 : a.capacity;
-    const int64_t most = (rows + 255) / 256, wanted = (148 * 4 + blocks - 1) / blocks;
-    const int64_t splits = wanted < most ? wanted : most;
-    return int(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
+bool step_aligned(const HtgsAttentionStep& a) {
+    const auto ok = [](const void* p, int64_t n0, int64_t s0, int64_t n1, int64_t s1) { return aligned(p, 16) && (n0 == 1 || s0 % 8 == 0) && (n1 == 1 || s1 % 8 == 0); };
+    return a.type != HTGS_FLOAT32 && a.width % 8 == 0 && ok(a.q, a.batch, a.q_stride, a.heads, a.q_head_stride) && ok(a.k, a.batch, a.k_stride, a.key_heads, a.k_head_stride) &&
+           ok(a.v, a.batch, a.v_stride, a.key_heads, a.v_head_stride) && ok(a.keys, a.batch, a.keys_stride, a.key_heads, a.keys_head_stride) && (a.capacity <= 1 || a.keys_row_stride % 8 == 0) &&
+           ok(a.values, a.batch, a.values_stride, a.key_heads, a.values_head_stride) && (a.capacity <= 1 || a.values_row_stride % 8 == 0);
 }
 
-template <typename T> int step_typed(const HtgsAttentionStep& a, void* out, float* parts, cudaStream_t stream) {
-    const int64_t blocks = int64_t(a.batch) * a.heads;
-    const int splits = splits_of(a, blocks);
-    cudaError_t err = launch_after(step_lanes_kernel<T>, dim3(unsigned(blocks * splits)), kStepThreads, 0, stream, a, static_cast<T*>(out), parts, splits);
-    if (err == cudaSuccess && splits > 1) err = launch_after(step_join_kernel<T>, dim3(unsigned(blocks)), kMostStepWidth, 0, stream, a, static_cast<T*>(out), parts, splits);
+struct StepPlan { bool tiles; int64_t blocks; int chunks, splits; };       // blocks: of one split
+// Splits of a sequence: the rounds of all places for a block, by the rows of a split and what a block costs beside them, about as much as 128 rows.
+StepPlan plan_of(const HtgsAttentionStep& a) {
+    StepPlan p{step_aligned(a), 0, 1, 1};
+    const int group = a.heads / a.key_heads;
+    if (p.tiles) p.chunks = (group + kTileHeads - 1) / kTileHeads;
+    p.blocks = int64_t(a.batch) * (p.tiles ? a.key_heads * p.chunks : a.heads);
+    const int64_t rows = (a.window >= 0 && a.window < a.capacity ? a.window + 1 : a.capacity) + 1, slots = 148 * (p.tiles ? (a.width <= 32 ? 4 : a.width <= 64 ? 2 : 1) : 8);
+    int64_t best = INT64_MAX;
+    for (int splits = 1; splits <= kMostSplits && (splits == 1 || rows >= splits * 128); ++splits) {
+        const int64_t cost = (p.blocks * splits + slots - 1) / slots * (rows / splits + 128) + (splits > 1 ? 128 : 0);
+        if (cost < best) { best = cost; p.splits = splits; }
+    }
+    return p;
+}
+
+template <typename T, int W> cudaError_t launch_step(const HtgsAttentionStep& a, T* out, float* parts, const StepPlan& plan, cudaStream_t stream) {
+    constexpr int smem = kTileWarps * kTileStages * 2 * kTileKeys * W * 2;
+    static_assert(kTileWarps * kTileHeads * (8 + (W + 4) * 4) <= smem, "the warps' parts fit the places of keys and values");
+    static PerDeviceOnce once;
+    const cudaError_t err = once.run([] { return cudaFuncSetAttribute(step_tiles_kernel<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    return err != cudaSuccess ? err : launch_after(step_tiles_kernel<T, W>, dim3(unsigned(plan.blocks * plan.splits)), kTileWarps * 32, smem, stream, a, out, parts, plan.splits, plan.chunks);
+}
+
+template <typename T> int step_typed(const HtgsAttentionStep& a, void* to, float* parts, cudaStream_t stream) {
+    const StepPlan plan = plan_of(a);
+    T* const out = static_cast<T*>(to);
+    cudaError_t err = cudaSuccess;
+    bool done = false;
+    if constexpr (sizeof(T) == 2) {
+        if (plan.tiles && aligned(out, 16)) {
+            err = a.width <= 32 ? launch_step<T, 32>(a, out, parts, plan, stream) : a.width <= 64 ? launch_step<T, 64>(a, out, parts, plan, stream) : launch_step<T, 128>(a, out, parts, plan, stream);
+            done = true;
+        }
+    }
+    if (!done) err = launch_after(step_lanes_kernel<T>, dim3(unsigned(int64_t(a.batch) * a.heads * plan.splits)), kStepThreads, 0, stream, a, out, parts, plan.splits);
+    if (err == cudaSuccess && plan.splits > 1) err = launch_after(step_join_kernel<T>, dim3(unsigned(int64_t(a.batch) * a.heads)), kMostStepWidth, 0, stream, a, out, parts, plan.splits);
     return err == cudaSuccess ? sequence_status("htgs_attention_step") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
@@ -164,9 +400,8 @@ extern "C" {
 size_t htgs_attention_step_workspace_bytes(const HtgsAttentionStep* step) {
     using namespace htgs;
     if (wrong(step) || step->batch == 0) return 0;
-    const int64_t blocks = int64_t(step->batch) * step->heads;
-    const int splits = splits_of(*step, blocks);
-    return splits == 1 ? 0 : size_t(blocks) * splits * part_floats(step->width) * sizeof(float);
+    const int splits = plan_of(*step).splits;
+    return splits == 1 ? 0 : size_t(step->batch) * step->heads * splits * part_floats(step->width) * sizeof(float);
 }
 
 int htgs_attention_step(const HtgsAttentionStep* step, void* out, void* workspace, size_t workspace_bytes, void* stream) {
