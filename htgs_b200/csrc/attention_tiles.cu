@@ -66,14 +66,14 @@ __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.s
 // A weight of zero takes a finite value out of a sum, not an infinite one or a NaN.  So in tiles where not every row sees every other the operand is looked through before it is used, by warps that have
 // nothing else to do, and where something is not finite a thread adds up what its row sees itself (some 50 us a tile).  Nothing of this costs the other tiles anything.
 
-// Whether rows [first, first + 64) of a tile hold such values; by a warp.
-template <typename T, int PANELS> __device__ __forceinline__ bool not_finite(const unsigned char* tile, int first, int lane) {
+// Whether a tile holds such values; by a warp.
+template <typename T, int PANELS> __device__ __forceinline__ bool not_finite(const unsigned char* tile, int lane) {
     using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     const uint32_t zero = 0;
     Two sum = *reinterpret_cast<const Two*>(&zero);
     #pragma unroll 4
-    for (int i = lane; i < PANELS * 64 * 8; i += 32) {
-        const uint4 piece = *reinterpret_cast<const uint4*>(tile + (i >> 9) * kPanelBytes + first * 128 + (i & 511) * 16);
+    for (int i = lane; i < PANELS * kTile * 8; i += 32) {
+        const uint4 piece = *reinterpret_cast<const uint4*>(tile + i * 16);
         const Two* v = reinterpret_cast<const Two*>(&piece);
         #pragma unroll
         for (int k = 0; k < 4; ++k) sum = __hfma2(v[k], *reinterpret_cast<const Two*>(&zero), sum);          // NaN from then on
@@ -119,312 +119,505 @@ template <typename T> __device__ __forceinline__ void multiply_seen(uint32_t sum
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 
+// NaN if one of them is.
+__device__ __forceinline__ float largest3(float a, float b, float c) { float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+__device__ __forceinline__ float largest2(float a, float b) { float d; asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
+
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
+    const float2 v = unpack2(x);
+    return pack2(exp2_approx(v.x), exp2_approx(v.y));
+}
+// 2^x = 2^n 2^r with n = x rounded (by adding 1.5 * 2^23, whose low bits then are n) and -1/2 <= r <= 1/2, where 2^r is a polynomial, 1 at 0, of least maximal relative error (found by linear programming):
+// degree 3 for bf16, 2^-13.2, and 4 for fp16, 2^-18.4, both far below half a step of the type.  From x = -127 down it is exactly zero.  NaN is for the caller to keep out.
+//
+// The unit for exponentials makes 16 a clock and SM, 1024 clocks for a tile, as long as the products of heads of 128 and twice as long as those of 64.  Four pairs of 16 go this way instead, through
+// multiply-adds that would idle (16384 rows, causal, heads of 64: 460 -> 425 us; more of them, or a second copy of the loop without them, cost more in instructions than they give).
+constexpr int kPolynomials = 4;
+template <typename T> __device__ __forceinline__ f32x2 exp2_polynomial(f32x2 x) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const float2 v = unpack2(x);
+    x = pack2(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
+    const f32x2 magic = pack2(12582912.0f, 12582912.0f), back = pack2(-12582912.0f, -12582912.0f), minus = pack2(-1.0f, -1.0f);
+    const f32x2 n = add2(x, magic), r = fma2(add2(n, back), minus, x);
+    const auto both = [](float c) { return pack2(c, c); };
+    f32x2 p = kHalf ? fma2(both(0.009582853876054287f), r, both(0.055906426161527634f)) : both(0.05500892922282219f);
+    p = fma2(p, r, both(kHalf ? 0.24024099111557007f : 0.24221095442771912f));
+    p = fma2(p, r, both(kHalf ? 0.6931241750717163f : 0.6932829022407532f));
+    p = fma2(p, r, both(1.0f));
+    const float2 low = unpack2(p), whole = unpack2(n);
+    return pack2(__uint_as_float(__float_as_uint(low.x) + (__float_as_uint(whole.x) << 23)), __uint_as_float(__float_as_uint(low.y) + (__float_as_uint(whole.y) << 23)));
+}
+
 // What an exponent may pass the running maximum by before the output is scaled down to a new one: weights up to 2^8 are as precise as those up to 1, and most tiles then leave the output alone.
 constexpr float kSlack = 8.0f;
 // Weights in fp16 are 2^6 times as large, so that one of 2^-20 of the row's largest is a normal number (and the largest is 2^14).
 template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 6.0f : 0.0f;
 
-template <int PANELS> struct ForwardTile {
-    static constexpr int bytes = PANELS * kPanelBytes, stages = PANELS == 2 ? 5 : 8;
-    static constexpr int barriers = 2 + 3 * stages + 6;
-    static constexpr int smem = 1024 + (2 + stages) * bytes + 512;
-    static_assert(barriers * 8 + 8 + stages * 8 <= 512 && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");       // one block has an SM alone, and with it tensor memory
+constexpr int kItems = 2;            // pieces of work that a block knows of: the present one and the next
+
+// QUERIES: tiles of queries of a block.  Two have an SM and its tensor memory alone, one shares it with another block.
+template <int PANELS, int QUERIES> struct ForwardTile {
+    static constexpr int threads = 128 + 128 * QUERIES, blocks = 3 - QUERIES, columns = 512 / blocks;      // of an SM; of tensor memory
+    static constexpr int bytes = PANELS * kPanelBytes, stages = 5;
+    static constexpr bool apart = PANELS == 1 && QUERIES == 1;       // weights have columns of their own
+    static constexpr int weights = apart ? kTile : 0, outputs = apart ? kTile + kTile / 2 : QUERIES * kTile;     // where they begin; another tile's 128 further
+    static constexpr int barriers = 2 * kItems + 3 * stages + 7 * QUERIES;
+    static constexpr int smem = 1024 + (QUERIES + stages) * bytes + 1024;
+    static_assert(barriers * 8 + 8 + stages * 4 + kItems * int(sizeof(SequenceTile) + 8) <= 1024 && smem <= 227 * 1024 / blocks - (blocks - 1) * 1024 && smem * (blocks + 1) > 227 * 1024, "shared memory");
 };
+// Registers of the warps that compute, and of the others; together those of the launch.
+template <int GROUPS> __device__ __forceinline__ void take_registers() {
+    if constexpr (GROUPS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+}
+template <int GROUPS> __device__ __forceinline__ void give_registers() {
+    if constexpr (GROUPS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+}
 
 struct ForwardArgs { HtgsAttention a; void* out; float* sums; unsigned int* error; };
 
-// Two tiles of queries, one behind the other, against tiles of keys.  Warp 0 loads; warp 1 issues the products, for one tile of queries while the other's softmax is computed; warps 2 and 3 look through
-// values of which some are not seen; warps 4 to 7 and 8 to 11 have a tile of queries each, a thread for each row.  Tensor memory: scores (weights over them) at 0 and 128, outputs at 256 and 384.
-template <typename T, int PANELS>
-__global__ void __launch_bounds__(kTilesThreads, 1) attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ForwardArgs args) {
-    using S = ForwardTile<PANELS>;
+// Blocks stay and go through pieces of work, a head and one or two tiles of queries, one behind the other, against tiles of keys: a block that began for each lost 9000 clocks on its way in and out (262144
+// rows within 512, 27000 for the tiles themselves).  Warp 0 finds the pieces and loads; warps 1 and 2 issue the products, for one tile of queries while the other's softmax (or the other block's) is
+// computed, and the next piece's first scores while the last one's output is stored; warp 3 looks through values of which some are not seen; warps 4 to 7 and 8 to 11 have a tile of queries each, a thread
+// for each row.  Tensor memory of two tiles: scores (weights over them) at 0 and 128, outputs at 256 and 384.  Of one, up to 64 columns wide: scores 0, weights 128, output 192; the next scores are
+// computed as soon as the softmax has read the last ones.
+template <typename T, int PANELS, int QUERIES>
+__global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ForwardArgs args) {
+    using S = ForwardTile<PANELS, QUERIES>;
     extern __shared__ unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     unsigned char* const queries = raw + (base - smem_u32(raw));
-    unsigned char* const ring = queries + 2 * S::bytes;
-    uint64_t* const q_full = reinterpret_cast<uint64_t*>(ring + S::stages * S::bytes);
-    uint64_t* const full = q_full + 2;
+    unsigned char* const ring = queries + QUERIES * S::bytes;
+    uint64_t* const item_full = reinterpret_cast<uint64_t*>(ring + S::stages * S::bytes);
+    uint64_t* const item_empty = item_full + kItems;
+    uint64_t* const full = item_empty + kItems;
     uint64_t* const empty = full + S::stages;
     uint64_t* const searched = empty + S::stages;        // values have been looked through
-    uint64_t* const scored = searched + S::stages;         // the scores of a tile are there
-    uint64_t* const weighed = scored + 2;                // its weights are
-    uint64_t* const summed = weighed + 2;                // they are in the output
-    uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(summed + 2);
+    uint64_t* const q_full = searched + S::stages;
+    uint64_t* const q_empty = q_full + QUERIES;
+    uint64_t* const scored = q_empty + QUERIES;          // the scores of a tile are there
+    uint64_t* const weighed = scored + QUERIES;          // its weights are
+    uint64_t* const summed = weighed + QUERIES;          // they are in the output
+    uint64_t* const taken = summed + QUERIES;            // the scores have been read (weights apart)
+    uint64_t* const drained = taken + QUERIES;           // the output has been read
+    uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(drained + QUERIES);
     volatile uint32_t* const failed = tmem_at + 1;
-    volatile uint32_t* const dirty = failed + 1;         // [stages][2], of halves of a tile of values
+    volatile uint32_t* const dirty = failed + 1;         // [stages], of tiles of values
+    volatile int* const items = reinterpret_cast<volatile int*>(dirty + S::stages);        // [kItems] of 6 words
 
     const HtgsAttention& a = args.a;
-    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    grid_dependency();
-    // the last tiles of a sequence first: causal, they have the most keys
-    const int head = int(blockIdx.x % a.heads), key_head = head / (a.heads / a.key_heads);
-    const SequenceTile t = find_tile<2 * kTile>(a, int(gridDim.x / a.heads - 1 - blockIdx.x / a.heads));
-    if (t.first >= t.end) return;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, group = a.heads / a.key_heads;
     T* const out = static_cast<T*>(args.out);
-    if (t.outside) {
-        const int rows = min(2 * kTile, t.end - t.first);
-        for (int i = threadIdx.x; i < rows * (a.width / 8); i += kTilesThreads)
-            *reinterpret_cast<uint4*>(out + (int64_t(t.first + i / (a.width / 8)) * a.heads + head) * a.width + i % (a.width / 8) * 8) = make_uint4(0, 0, 0, 0);
-        if (args.sums)
-            for (int i = threadIdx.x; i < rows; i += kTilesThreads) args.sums[head * a.rows + t.first + i] = 0.0f;
-        return;
-    }
-    // keys low + [0, 128 n) for the block; tile s of queries sees tiles [begin[s], end[s]) of them
-    const int last_row = min(t.first + 2 * kTile, t.end) - 1;
-    const int low = first_seen(a, t.begin, t.first), n = (last_seen(a, t.end, last_row) - low) / kTile + 1;
-    int begin[2], end[2];
-    #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const int row = t.first + s * kTile;
-        begin[s] = row < t.end ? (first_seen(a, t.begin, row) - low) / kTile : 0;
-        end[s] = row < t.end ? (last_seen(a, t.end, min(row + kTile, t.end) - 1) - low) / kTile + 1 : 0;
-    }
-    // whether all rows of tile s see all keys of tile j
-    const auto whole = [&](int s, int j) {
-        const int first = t.first + s * kTile;
-        return low + j * kTile >= first_seen(a, t.begin, min(first + kTile, t.end) - 1) && low + j * kTile + kTile - 1 <= last_seen(a, t.end, min(first, t.end - 1));
-    };
-
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) { mbar_init(q_full + i, 1); mbar_init(scored + i, 1); mbar_init(weighed + i, 4); mbar_init(summed + i, 1); }
-        for (int i = 0; i < S::stages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 3); mbar_init(searched + i, 2); }
+        for (int i = 0; i < kItems; ++i) { mbar_init(item_full + i, 1); mbar_init(item_empty + i, (S::apart ? 2 : 1) + 1 + 4 * QUERIES); }
+        for (int i = 0; i < QUERIES; ++i) {
+            mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1); mbar_init(scored + i, 1); mbar_init(weighed + i, 4); mbar_init(summed + i, 1); mbar_init(taken + i, 4); mbar_init(drained + i, 4);
+        }
+        for (int i = 0; i < S::stages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 2); mbar_init(searched + i, 1); }
         *failed = 0;
         mbar_fence_init();
     }
+    grid_dependency();               // before tensor memory is taken, which a block of the kernel before may still have to get
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)), "n"(S::columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tmem_fence_before();
     }
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+    const int total = int(sequence_tiles(a, QUERIES * kTile)) * a.heads;
+    // Piece `item`: the last tiles of a sequence first, as they have the most keys where attention is causal.
+    const auto tile_of = [&](int item) { return find_tile<QUERIES * kTile>(a, (total - 1 - item) / a.heads); };
+    // Rounds there and back, so that a block with a long piece has a short one next.
+    const auto item_of = [&](int round) { return round * int(gridDim.x) + (round & 1 ? int(gridDim.x - 1 - blockIdx.x) : int(blockIdx.x)); };
+    const auto head_of = [&](int item) { return item % a.heads; };
+
+    // What the roles know of a piece: keys low + [0, 128 n) for the block; tile s of queries sees tiles [from(s), to(s)) of them.
+    struct Piece {
+        const HtgsAttention& a;
+        int begin, end, first, head, low, n;
+        __device__ Piece(const HtgsAttention& a_) : a(a_), n(0) {}
+        __device__ void set(int begin_, int end_, int first_, int head_) {
+            begin = begin_; end = end_; first = first_; head = head_;
+            low = first_seen(a, begin, first);
+            n = (last_seen(a, end, min(first + QUERIES * kTile, end) - 1) - low) / kTile + 1;
+        }
+        __device__ int from(int s) const { return QUERIES == 1 ? 0 : first + s * kTile < end ? (first_seen(a, begin, first + s * kTile) - low) / kTile : 0; }
+        __device__ int to(int s) const { return QUERIES == 1 ? n : first + s * kTile < end ? (last_seen(a, end, min(first + (s + 1) * kTile, end) - 1) - low) / kTile + 1 : 0; }
+        // tiles [x, y) of keys are seen by all rows of tile s
+        __device__ int2 whole(int s) const {
+            const int row = first + s * kTile;
+            return make_int2((first_seen(a, begin, min(row + kTile, end) - 1) - low + kTile - 1) / kTile, (last_seen(a, end, min(row, end - 1)) - low + 1) / kTile);
+        }
+    };
+    // The next piece, for a warp of a role that is not the loading one; false behind the last.
+    Ring<kItems> item_at;
+    Piece piece(a);
+    const auto next_piece = [&] {
+        if (!__all_sync(0xffffffffu, wait_in_line(item_full + item_at.at, item_at.round, failed))) return false;
+        volatile int* const from = items + 6 * item_at.at;
+        const bool there = from[4];
+        if (there) piece.set(from[0], from[1], from[2], from[3]);
+        __syncwarp();
+        if (lane == 0) arrive(item_empty + item_at.at);
+        item_at.next();
+        return there;
+    };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        give_registers<QUERIES>();
         if (warp == 0) {
             const bool one = elect_one();
-            if (one) {
-                #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    if (end[s] == 0) continue;
-                    mbar_arrive_expect_tx(q_full + s, S::bytes);
-                    for (int p = 0; p < PANELS; ++p) load_panel(queries + s * S::bytes + p * kPanelBytes, &map_q, p * kPanel, head, t.first + s * kTile, q_full + s);
-                }
-            }
-            __syncwarp();
             Ring<S::stages> stage;
-            uint32_t uses = 0;
+            uint32_t uses = 0, loads[QUERIES] = {};
             bool ok = true;
-            for (int i = 0; i < 2 * n; ++i, ++uses, stage.next()) {           // keys and values of a tile by turns
-                ok = __all_sync(0xffffffffu, wait_in_line(empty + stage.at, stage.round ^ 1, failed));
-                if (!ok) break;
-                if (one) {
-                    mbar_arrive_expect_tx(full + stage.at, S::bytes);
-                    for (int p = 0; p < PANELS; ++p) load_panel(ring + stage.at * S::bytes + p * kPanelBytes, i & 1 ? &map_v : &map_k, p * kPanel, key_head, low + (i >> 1) * kTile, full + stage.at);
+            const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_in_line(bar, parity, failed)); };
+            const auto publish = [&](const SequenceTile& t, int head, int there) {
+                wait(item_empty + item_at.at, item_at.round ^ 1);
+                if (!ok) return;
+                if (lane == 0) {
+                    volatile int* const to = items + 6 * item_at.at;
+                    to[0] = t.begin; to[1] = t.end; to[2] = t.first; to[3] = head; to[4] = there;
+                    arrive(item_full + item_at.at);
                 }
                 __syncwarp();
+                item_at.next();
+            };
+            for (int round = 0; ok && round * int(gridDim.x) < total; ++round) {
+                const int item = item_of(round);
+                if (item >= total) continue;
+                const SequenceTile t = tile_of(item);
+                if (t.first >= t.end) continue;
+                const int head = head_of(item);
+                if (t.outside) {
+                    const int rows = min(QUERIES * kTile, t.end - t.first), pieces = a.width / 8;
+                    for (int i = lane; i < rows * pieces; i += 32)
+                        *reinterpret_cast<uint4*>(out + (int64_t(t.first + i / pieces) * a.heads + head) * a.width + i % pieces * 8) = make_uint4(0, 0, 0, 0);
+                    for (int i = lane; i < rows && args.sums; i += 32) args.sums[head * a.rows + t.first + i] = 0.0f;
+                    __syncwarp();
+                    continue;
+                }
+                publish(t, head, 1);
+                piece.set(t.begin, t.end, t.first, head);
+                #pragma unroll
+                for (int s = 0; s < QUERIES; ++s) {
+                    if (piece.to(s) == 0) continue;
+                    wait(q_empty + s, (loads[s] & 1) ^ 1);
+                    if (!ok) break;
+                    ++loads[s];
+                    if (one) {
+                        mbar_arrive_expect_tx(q_full + s, S::bytes);
+                        for (int p = 0; p < PANELS; ++p) load_panel(queries + s * S::bytes + p * kPanelBytes, &map_q, p * kPanel, head, t.first + s * kTile, q_full + s);
+                    }
+                    __syncwarp();
+                }
+                for (int i = 0; i < 2 * piece.n && ok; ++i) {           // keys and values of a tile by turns
+                    wait(empty + stage.at, stage.round ^ 1);
+                    if (!ok) break;
+                    if (one) {
+                        mbar_arrive_expect_tx(full + stage.at, S::bytes);
+                        for (int p = 0; p < PANELS; ++p) load_panel(ring + stage.at * S::bytes + p * kPanelBytes, i & 1 ? &map_v : &map_k, p * kPanel, head / group, piece.low + (i >> 1) * kTile, full + stage.at);
+                    }
+                    __syncwarp();
+                    ++uses;
+                    stage.next();
+                }
             }
+            if (ok) publish({0, 0, 0, 0, false}, 0, 0);
             if (!ok) {              // no copy may be on its way when the block ends
                 for (uint32_t u = uses > S::stages ? uses - S::stages : 0; u < uses; ++u) {
                     WaitLimit limit(kWaitNanoseconds, nanoseconds());
                     while (!mbar_try_wait(full + u % S::stages, u / S::stages & 1) && !limit.over(nanoseconds())) {}
                 }
-                for (int s = 0; s < 2; ++s) {
+                for (int s = 0; s < QUERIES; ++s) {
                     WaitLimit limit(kWaitNanoseconds, nanoseconds());
-                    while (end[s] && !mbar_try_wait(q_full + s, 0) && !limit.over(nanoseconds())) {}
+                    while (loads[s] && !mbar_try_wait(q_full + s, (loads[s] - 1) & 1) && !limit.over(nanoseconds())) {}
                 }
             }
-        } else if (warp == 1) {
+        } else if (warp == 1 || (S::apart && warp == 2)) {
             const bool one = elect_one();
             const uint32_t score = instruction<T>(kTile, false), weigh = instruction<T>((a.width + 15) & ~15, true);
             const int steps = (a.width + 15) / 16;
             Ring<S::stages> stage;
-            uint32_t weighed_round[2] = {0, 0};
+            int2 all[QUERIES] = {};
+            uint32_t scores_done[QUERIES] = {}, outputs_done[QUERIES] = {}, pieces_done[QUERIES] = {};            // so far, whose lowest bits are the parities
             bool ok = true;
-            const auto scores = [&](int s, uint32_t slot) {
-                const uint32_t q = along_columns(base + s * S::bytes), k = along_columns(base + 2 * S::bytes + slot * S::bytes);
+            const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_in_line(bar, parity, failed)); };
+            // scores of tile s of queries; the piece's last free the place of the queries
+            const auto scores = [&](int s, bool last) {
+                const uint32_t q = along_columns(base + s * S::bytes), k = along_columns(base + QUERIES * S::bytes + stage.at * S::bytes);
                 if (one) {
                     for (int i = 0; i < steps; ++i) {
                         const uint32_t at = (i >> 2) * kPanelUnits + (i & 3) * 2;
                         multiply(tmem + s * kTile, q + at, k + at, score, i > 0);
                     }
                     commit(scored + s);
+                    if (last) commit(q_empty + s);
                 }
                 __syncwarp();
             };
-            const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_in_line(bar, parity, failed)); };
-            for (int j = -1; j < n && ok; ++j) {              // the output's part of tile j, then the scores of tile j + 1
-                uint32_t value_slot = 0, key_slot = 0;
-                if (j >= 0) { wait(full + stage.at, stage.round); value_slot = stage.at; stage.next(); }
-                if (j + 1 < n) { key_slot = stage.at; wait(full + stage.at, stage.round); stage.next(); }
-                #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    if (j >= begin[s] && j < end[s]) {
-                        wait(weighed + s, weighed_round[s]);
-                        if (!ok) break;
-                        weighed_round[s] ^= 1;
-                        tmem_fence_after();
-                        const uint32_t v = along_rows(base + 2 * S::bytes + value_slot * S::bytes);
-                        const bool added = !whole(s, j) && (dirty[2 * value_slot] | dirty[2 * value_slot + 1]);       // by the softmax's threads
-                        if (one) {
-                            #pragma unroll
-                            for (int i = 0; i < (added ? 0 : kTile / 16); ++i) multiply_tmem(tmem + 2 * kTile + s * kTile, tmem + s * kTile + i * 8, v + i * (2048 >> 4), weigh, j > begin[s] || i > 0);
-                            commit(summed + s);
-                        }
-                        __syncwarp();
-                    }
-                    if (j + 1 >= begin[s] && j + 1 < end[s]) {
-                        if (j + 1 == begin[s]) wait(q_full + s, 0);
-                        if (!ok) break;
-                        tmem_fence_after();
-                        scores(s, key_slot);
-                    }
-                }
-                if (!ok) break;
+            const auto outputs = [&](int s, int j, bool first, uint32_t slot) {
+                const bool added = (j < all[s].x || j >= all[s].y) && dirty[slot];       // by the softmax's threads
+                const uint32_t v = along_rows(base + QUERIES * S::bytes + slot * S::bytes);
                 if (one) {
-                    if (j >= 0) commit(empty + value_slot);
-                    if (j + 1 < n) commit(empty + key_slot);
+                    #pragma unroll
+                    for (int i = 0; i < (added ? 0 : kTile / 16); ++i) multiply_tmem(tmem + S::outputs + s * kTile, tmem + S::weights + s * kTile + i * 8, v + i * (2048 >> 4), weigh, !first || i > 0);
+                    commit(summed + s);
                 }
                 __syncwarp();
+            };
+            const auto used = [&](uint32_t slot) {
+                if (one) commit(empty + slot);
+                __syncwarp();
+            };
+            if (S::apart && warp == 2) stage.next();
+            while (ok && next_piece()) {
+                const int n = piece.n;
+                #pragma unroll
+                for (int s = 0; s < QUERIES; ++s) all[s] = piece.whole(s);
+                if constexpr (S::apart) {             // one warp has the scores, the other the output
+                    if (warp == 1) wait(q_full, pieces_done[0] & 1);
+                    else wait(drained, (pieces_done[0] & 1) ^ 1);
+                    ++pieces_done[0];
+                    for (int j = 0; j < n && ok; ++j) {
+                        wait(full + stage.at, stage.round);
+                        if (warp == 1) wait(taken, (scores_done[0] & 1) ^ 1);
+                        else wait(weighed, outputs_done[0] & 1);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        if (warp == 1) { scores(0, j + 1 == n); ++scores_done[0]; }
+                        else { outputs(0, j, j == 0, stage.at); ++outputs_done[0]; }
+                        used(stage.at);
+                        stage.next(); stage.next();
+                    }
+                } else {                              // by turns: two warps would take the tensor cores from each other (32768 rows, causal, heads of 128: 1.73 -> 2.08 ms)
+                    int from[QUERIES], to[QUERIES];
+                    #pragma unroll
+                    for (int s = 0; s < QUERIES; ++s) { from[s] = piece.from(s); to[s] = piece.to(s); }
+                    for (int j = -1; j < n && ok; ++j) {              // the output's part of tile j, then the scores of tile j + 1
+                        uint32_t value_slot = 0;
+                        if (j >= 0) {
+                            wait(full + stage.at, stage.round);
+                            value_slot = stage.at;
+                            stage.next();
+                        }
+                        if (j + 1 < n) wait(full + stage.at, stage.round);
+                        #pragma unroll
+                        for (int s = 0; s < QUERIES; ++s) {
+                            if (j >= from[s] && j < to[s]) {
+                                if (j == from[s]) wait(drained + s, pieces_done[s] & 1);        // pieces_done counts the present one
+                                wait(weighed + s, outputs_done[s] & 1);
+                                if (!ok) break;
+                                ++outputs_done[s];
+                                tmem_fence_after();
+                                outputs(s, j, j == from[s], value_slot);
+                            }
+                            if (j + 1 >= from[s] && j + 1 < to[s]) {
+                                if (j + 1 == from[s]) wait(q_full + s, pieces_done[s]++ & 1);
+                                if (!ok) break;
+                                tmem_fence_after();
+                                scores(s, j + 2 == to[s]);
+                            }
+                        }
+                        if (!ok) break;
+                        if (j >= 0) used(value_slot);
+                        if (j + 1 < n) {
+                            used(stage.at);
+                            stage.next();
+                        }
+                    }
+                }
             }
-        } else {
+        } else if (warp == 3) {
             Ring<S::stages> stage;
-            for (int i = 0; i < 2 * n; ++i, stage.next()) {
-                if (!__all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed))) break;
-                const int j = i >> 1;
-                const bool seen = !(i & 1) || ((j < begin[0] || j >= end[0] || whole(0, j)) && (j < begin[1] || j >= end[1] || whole(1, j)));
-                const bool found = !seen && not_finite<T, PANELS>(ring + stage.at * S::bytes, (warp - 2) * 64, lane);
-                if (lane == 0) {
-                    dirty[2 * stage.at + warp - 2] = found;
-                    arrive(searched + stage.at);
-                    arrive(empty + stage.at);
+            bool ok = true;
+            while (ok && next_piece()) {
+                int2 all[QUERIES], any[QUERIES];
+                #pragma unroll
+                for (int s = 0; s < QUERIES; ++s) { all[s] = piece.whole(s); any[s] = make_int2(piece.from(s), piece.to(s)); }
+                for (int i = 0; i < 2 * piece.n && ok; ++i, stage.next()) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed));
+                    if (!ok) break;
+                    const int j = i >> 1;
+                    bool seen = true;
+                    #pragma unroll
+                    for (int s = 0; s < QUERIES; ++s) seen = seen && (!(i & 1) || j < any[s].x || j >= any[s].y || (j >= all[s].x && j < all[s].y));
+                    const bool found = !seen && not_finite<T, PANELS>(ring + stage.at * S::bytes, lane);
+                    if (lane == 0) {
+                        dirty[stage.at] = found;
+                        arrive(searched + stage.at);
+                        arrive(empty + stage.at);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        take_registers<QUERIES>();
         const int s = (warp >> 2) - 1, quarter = (warp & 3) * 32;
-        const int first = t.first + s * kTile, row = min(first + quarter + lane, t.end - 1);
-        const bool there = first + quarter + lane < t.end;
-        const uint32_t lanes = uint32_t(quarter) << 16, score = tmem + s * kTile + lanes, sum_at = tmem + 2 * kTile + s * kTile + lanes;
+        const uint32_t lanes = uint32_t(quarter) << 16, score = tmem + s * kTile + lanes, weights = score + S::weights, sum_at = tmem + S::outputs + s * kTile + lanes;
         const float scale = a.scale * kLog2e;
-        const int row_low = first_seen(a, t.begin, row), row_high = last_seen(a, t.end, row);
-        float most = -infinity();
-        f32x2 total = pack2(0.0f, 0.0f);
+        const f32x2 scale2 = pack2(scale, scale);
+        uint32_t tiles_done = 0, uses = 0;                     // so far: of this tile of queries; places of the ring, by the block
         bool ok = true;
-        const int from = s == 0 ? begin[0] : begin[1], to = s == 0 ? end[0] : end[1];
-        for (int j = from; j < to; ++j) {
-            ok = __all_sync(0xffffffffu, wait_in_line(scored + s, (j - from) & 1, failed));
+        while (ok && next_piece()) {
+            const int first = piece.first + s * kTile, row = min(first + quarter + lane, piece.end - 1);
+            const bool there = first + quarter + lane < piece.end;
+            const int row_low = first_seen(a, piece.begin, row), row_high = last_seen(a, piece.end, row);
+            const int from = piece.from(s), to = piece.to(s);
+            const int2 all = piece.whole(s);
+            float most = -infinity();
+            f32x2 total2 = pack2(0.0f, 0.0f);
+            for (int j = from; j < to; ++j, ++tiles_done) {
+                ok = __all_sync(0xffffffffu, wait_in_line(scored + s, tiles_done & 1, failed));
+                if (!ok) break;
+                tmem_fence_after();
+                const bool used = S::apart && j > from && mbar_test(summed + s, (tiles_done - 1) & 1);      // the last tile's weights: asked here, where nothing waits for it
+                uint32_t v[128];
+                tmem_begin32(score, v);
+                tmem_begin32(score + 32, v + 32);
+                tmem_loaded();
+                tmem_begin32(score + 64, v + 64);
+                tmem_begin32(score + 96, v + 96);
+                float m[8];
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) m[i] = __uint_as_float(v[i]);
+                const int from_column = row_low - (piece.low + j * kTile), to_column = row_high - (piece.low + j * kTile);
+                const bool masked = j < all.x || j >= all.y;
+                if (masked) {
+                    #pragma unroll
+                    for (int c = 0; c < 64; ++c) v[c] = c < from_column || c > to_column ? 0xff800000u : v[c];
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) m[i] = __uint_as_float(v[i]);
+                }
+                #pragma unroll
+                for (int c = 8; c < 56; c += 16)
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) m[i] = largest3(m[i], __uint_as_float(v[c + i]), __uint_as_float(v[c + 8 + i]));
+                tmem_loaded();
+                if constexpr (S::apart) {
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(taken + s);
+                }
+                if (masked) {
+                    #pragma unroll
+                    for (int c = 64; c < 128; ++c) v[c] = c < from_column || c > to_column ? 0xff800000u : v[c];
+                }
+                #pragma unroll
+                for (int c = 56; c < 120; c += 16)
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) m[i] = largest3(m[i], __uint_as_float(v[c + i]), __uint_as_float(v[c + 8 + i]));
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) m[i] = largest2(m[i], __uint_as_float(v[120 + i]));
+                const float tile_most = largest3(largest3(m[0], m[1], m[2]), largest3(m[3], m[4], m[5]), largest2(m[6], m[7])) * scale;
+                if (__any_sync(0xffffffffu, !(tile_most <= most + kSlack))) {
+                    float now = largest2(most, tile_most);           // NaN makes the row's weights NaN, and so does infinity, which could only be taken from itself
+                    now = now == infinity() ? __uint_as_float(0x7fffffffu) : now;
+                    const float factor = most == now ? 1.0f : exp2_approx(most - now);
+                    most = now;
+                    total2 = mul2(total2, pack2(factor, factor));
+                    if (j > from) {
+                        ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (tiles_done - 1) & 1, failed));
+                        if (!ok) break;
+                        tmem_fence_after();
+                        #pragma unroll 1
+                        for (int c = 0; c < a.width; c += 16) {
+                            uint32_t o[16];
+                            tmem_begin16(sum_at + c, o);
+                            tmem_loaded();
+                            #pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                            tmem_store16(sum_at + c, o);
+                        }
+                        tmem_stored();
+                    }
+                }
+                const float shift = kLift<T> - (most == -infinity() ? 0.0f : most);
+                const f32x2 shift2 = pack2(shift, shift);
+                f32x2 sums[2] = {total2, pack2(0.0f, 0.0f)};
+                #pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t words[16];
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const f32x2 x = fma2(pack2(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1])), scale2, shift2);
+                        const f32x2 p = i * kPolynomials / 16 != (i + 1) * kPolynomials / 16 ? exp2_polynomial<T>(x) : exp2_pair(x);
+                        sums[i & 1] = add2(sums[i & 1], p);
+                        const float2 both = unpack2(p);
+                        words[i] = floats_pair<T>(both.x, both.y);
+                    }
+                    if constexpr (S::apart) {
+                        if (c == 0 && j > from && !used) {
+                            ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (tiles_done - 1) & 1, failed));
+                            tmem_fence_after();
+                        }
+                    }
+                    tmem_store16(weights + c / 2, words);
+                }
+                if (S::apart && !ok) break;
+                total2 = add2(sums[0], sums[1]);
+                tmem_stored();
+                if (masked) {
+                    const uint32_t use = uses + 2 * j + 1, at = use % S::stages, round = use / S::stages & 1;
+                    ok = __all_sync(0xffffffffu, wait_in_line(searched + at, round, failed));
+                    if (!ok) break;
+                    if (dirty[at]) {
+                        ok = __all_sync(0xffffffffu, wait_in_line(full + at, round, failed));
+                        if (ok && j > from) ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (tiles_done - 1) & 1, failed));
+                        if (!ok) break;
+                        tmem_fence_after();
+                        multiply_seen<T>(sum_at, 0, a.width, j > from, weights, 32, ring + at * S::bytes, from_column, to_column);
+                    }
+                }
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(weighed + s);
+            }
+            uses += 2 * piece.n;
+            if (!ok || to <= from) continue;
+            ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (tiles_done - 1) & 1, failed));
             if (!ok) break;
             tmem_fence_after();
-            uint32_t v[128];
-            #pragma unroll
-            for (int c = 0; c < 128; c += 32) tmem_begin32(score + c, v + c);
-            tmem_loaded();
-            const int k0 = low + j * kTile;
-            const bool masked = !whole(s, j);
-            const int from_column = row_low - k0, to_column = row_high - k0;
-            if (masked) {
+            const float2 parts = unpack2(total2);
+            const float sum = parts.x + parts.y, inverse = 1.0f / sum;
+            T* const at = out + (int64_t(row) * a.heads + piece.head) * a.width;
+            for (int c = 0; c < a.width; c += 32) {
+                uint32_t o[32];
+                tmem_begin32(sum_at + c, o);
+                tmem_loaded();
                 #pragma unroll
-                for (int c = 0; c < 128; ++c) v[c] = c < from_column || c > to_column ? 0xff800000u : v[c];
-            }
-            float m[4];
-            #pragma unroll
-            for (int c = 0; c < 4; ++c) m[c] = __uint_as_float(v[c]);
-            #pragma unroll
-            for (int c = 4; c < 128; c += 8)
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) m[i] = c + 4 + i < 128 ? fmaxf(fmaxf(m[i], __uint_as_float(v[c + i])), __uint_as_float(v[c + 4 + i < 128 ? c + 4 + i : 0])) : fmaxf(m[i], __uint_as_float(v[c + i]));
-            const float tile_most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * scale;
-            if (__any_sync(0xffffffffu, tile_most > most + kSlack)) {
-                const float now = fmaxf(most, tile_most), factor = most == now ? 1.0f : exp2_approx(most - now);
-                most = now;
-                total = mul2(total, pack2(factor, factor));
-                if (j > from) {
-                    ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (j - from - 1) & 1, failed));
-                    if (!ok) break;
-                    tmem_fence_after();
-                    #pragma unroll 1
-                    for (int c = 0; c < a.width; c += 16) {
-                        uint32_t o[16];
-                        tmem_begin16(sum_at + c, o);
-                        tmem_loaded();
-                        #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                        tmem_store16(sum_at + c, o);
-                    }
-                    tmem_stored();
-                }
-            }
-            const float shift = kLift<T> - (most == -infinity() ? 0.0f : most);
-            const f32x2 scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
-            f32x2 sums[2] = {total, pack2(0.0f, 0.0f)};
-            #pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-                uint32_t words[16];
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 x = unpack2(fma2(pack2(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1])), scale2, shift2));
-                    const float p0 = exp2_approx(x.x), p1 = exp2_approx(x.y);
-                    sums[i & 1] = add2(sums[i & 1], pack2(p0, p1));
-                    words[i] = floats_pair<T>(p0, p1);
-                }
-                tmem_store16(score + c / 2, words);
-            }
-            total = add2(sums[0], sums[1]);
-            tmem_stored();
-            if (masked) {
-                const uint32_t at = uint32_t(2 * j + 1) % S::stages, round = uint32_t(2 * j + 1) / S::stages & 1;
-                ok = __all_sync(0xffffffffu, wait_in_line(searched + at, round, failed));
-                if (!ok) break;
-                if (dirty[2 * at] | dirty[2 * at + 1]) {
-                    ok = __all_sync(0xffffffffu, wait_in_line(full + at, round, failed));
-                    if (ok && j > from) ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (j - from - 1) & 1, failed));
-                    if (!ok) break;
-                    tmem_fence_after();
-                    multiply_seen<T>(sum_at, 0, a.width, j > from, score, 32, ring + at * S::bytes, from_column, to_column);
+                for (int i = 0; i < 32; i += 8) {
+                    float f[8];
+                    #pragma unroll
+                    for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[i + k]) * inverse;
+                    if (there && c + i < a.width) store_floats<T, 8>(at + c + i, f);
                 }
             }
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) arrive(weighed + s);
-        }
-        if (ok && to > from) {
-            ok = __all_sync(0xffffffffu, wait_in_line(summed + s, (to - from - 1) & 1, failed));
-            if (ok) {
-                tmem_fence_after();
-                const float2 parts = unpack2(total);
-                const float sum = parts.x + parts.y, inverse = 1.0f / sum;
-                T* const at = out + (int64_t(row) * a.heads + head) * a.width;
-                for (int c = 0; c < a.width; c += 32) {
-                    uint32_t o[32];
-                    tmem_begin32(sum_at + c, o);
-                    tmem_loaded();
-                    #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        float f[8];
-                        #pragma unroll
-                        for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[i + k]) * inverse;
-                        if (there && c + i < a.width) store_floats<T, 8>(at + c + i, f);
-                    }
-                }
-                if (args.sums && there) args.sums[head * a.rows + row] = most - kLift<T> + log2f(sum);
-            }
+            if (lane == 0) arrive(drained + s);
+            if (args.sums && there) args.sums[piece.head * a.rows + row] = most - kLift<T> + log2f(sum);
         }
         tmem_fence_before();
     }
     __syncthreads();
     if (warp == 1) {
         tmem_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::columns) : "memory");
     }
     if (*failed) {               // a wait ran out: nothing that looks like a result
-        const int rows = min(2 * kTile, t.end - t.first);
-        for (int i = threadIdx.x; i < rows * a.width; i += kTilesThreads)
-            out[(int64_t(t.first + i / a.width) * a.heads + head) * a.width + i % a.width] = from_float<T>(__uint_as_float(0x7fffffffu));
+        for (int round = 0; round * int(gridDim.x) < total; ++round) {
+            const int item = item_of(round);
+            if (item >= total) continue;
+            const SequenceTile t = tile_of(item);
+            const int rows = min(QUERIES * kTile, t.end - t.first);
+            for (int i = threadIdx.x; i < rows * a.width && !t.outside; i += S::threads)
+                out[(int64_t(t.first + i / a.width) * a.heads + head_of(item)) * a.width + i % a.width] = from_float<T>(__uint_as_float(0x7fffffffu));
+        }
         if (threadIdx.x == 0) {
             *reinterpret_cast<volatile unsigned int*>(args.error) = 1;
             __threadfence_system();
@@ -664,8 +857,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
                 bool found = false;
                 if (!whole(query_row(i))) {
                     const unsigned char* tile = ring + stage.at * S::stage_bytes + (warp == 2 ? S::bytes : 0);
-                    found = not_finite<T, PANELS>(tile, 0, lane);
-                    found = not_finite<T, PANELS>(tile, 64, lane) || found;
+                    found = not_finite<T, PANELS>(tile, lane);
                 }
                 if (lane == 0) {
                     dirty[2 * stage.at + warp - 2] = found;
@@ -934,7 +1126,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(con
             Ring<S::stages> stage;
             for (int i = 0; i < 2 * n; ++i, stage.next()) {
                 if (!__all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed))) break;
-                const bool found = !(i & 1) && !whole(i >> 1) && not_finite<T, PANELS>(ring + stage.at * S::bytes, (warp - 2) * 64, lane);
+                const bool found = warp == 2 && !(i & 1) && !whole(i >> 1) && not_finite<T, PANELS>(ring + stage.at * S::bytes, lane);
                 if (lane == 0) {
                     dirty[2 * stage.at + warp - 2] = found;
                     arrive(searched + stage.at);
@@ -1048,16 +1240,17 @@ bool heads_aligned(const void* p, int64_t rows, int heads, int64_t stride, int64
     return aligned(p, 16) && (rows == 1 || step(stride)) && (heads == 1 || step(head_stride));
 }
 
-template <typename T, int PANELS> int launch_forward(const ForwardArgs& args, cudaStream_t stream) {
-    using S = ForwardTile<PANELS>;
+template <typename T, int PANELS, int QUERIES> int launch_forward(const ForwardArgs& args, cudaStream_t stream) {
+    using S = ForwardTile<PANELS, QUERIES>;
     const HtgsAttention& a = args.a;
     CUtensorMap q, k, v;
     if (!make_rows_map(&q, a.q, a.rows, a.heads, a.width, a.q_stride, a.q_head_stride) || !make_rows_map(&k, a.k, a.rows, a.key_heads, a.width, a.k_stride, a.k_head_stride) ||
         !make_rows_map(&v, a.v, a.rows, a.key_heads, a.width, a.v_stride, a.v_head_stride))
         return sequence_fail(HTGS_ERR_CUDA, "htgs_attention: the tensor maps cannot be made");
     static PerDeviceOnce once;
-    cudaError_t err = once.run([] { return cudaFuncSetAttribute(attention_tiles_kernel<T, PANELS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem); });
-    if (err == cudaSuccess) err = launch_after(attention_tiles_kernel<T, PANELS>, dim3(unsigned(sequence_tiles(a, 2 * kTile) * a.heads)), kTilesThreads, S::smem, stream, q, k, v, args);
+    cudaError_t err = once.run([] { return cudaFuncSetAttribute(attention_tiles_kernel<T, PANELS, QUERIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem); });
+    const int64_t pieces = sequence_tiles(a, QUERIES * kTile) * a.heads;
+    if (err == cudaSuccess) err = launch_after(attention_tiles_kernel<T, PANELS, QUERIES>, dim3(unsigned(pieces < 148 * S::blocks ? pieces : 148 * S::blocks)), S::threads, S::smem, stream, q, k, v, args);
     return err == cudaSuccess ? sequence_status("htgs_attention") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 template <typename T, int PANELS> int launch_backward(const BackwardArgs& args, cudaStream_t stream) {
@@ -1080,7 +1273,7 @@ template <typename T> int backward_typed(const BackwardArgs& args, cudaStream_t 
     return args.a.width <= kPanel ? launch_backward<T, 1>(args, stream) : launch_backward<T, 2>(args, stream);
 }
 template <typename T> int forward_typed(const ForwardArgs& args, cudaStream_t stream) {
-    return args.a.width <= kPanel ? launch_forward<T, 1>(args, stream) : launch_forward<T, 2>(args, stream);
+    return args.a.width <= kPanel ? launch_forward<T, 1, 1>(args, stream) : launch_forward<T, 2, 2>(args, stream);
 }
 
 }  // namespace

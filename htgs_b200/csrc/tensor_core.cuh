@@ -28,9 +28,14 @@ static __device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, v
         if (limit.over(nanoseconds())) { *failed = 1; return false; }
     }
 }
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 // The same in line, for kernels that give registers from one warp to another, which may not call.
 __device__ __forceinline__ bool wait_in_line(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_test(bar, parity)) return true;
     WaitLimit limit(kWaitNanoseconds, nanoseconds());
     for (;;) {
         if (mbar_try_wait(bar, parity)) return true;

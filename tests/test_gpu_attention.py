@@ -196,6 +196,29 @@ def test_what_a_row_does_not_see_does_not_reach_it(kind, bad):
     assert dirty[0][200:390].isnan().any()
 
 
+@pytest.mark.parametrize("kind", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_scores_that_are_not_finite_reach_the_rows_that_see_them(kind, bad):
+    """One key's score is not finite, whichever column of a tile it is: NaN for NaN and plus infinity in every row that sees it, a weight of zero for minus infinity."""
+    from htgs_b200 import sequence as seq
+    rows = 390
+    q, k, v, grad = tensors(rows, 1, 1, 16, kind)
+    q[..., 0] = 1.0
+    for j in (0, 1, 6, 7, 13, 40, 77, 127, 128, 200, 201, 259, 388):
+        spoilt = k.clone()
+        spoilt[j, 0, 0] = bad
+        out = f64(seq.attention(q, spoilt, v, causal=True))
+        want, bound = ref.attend(f64(q), f64(k), f64(v), [0, rows], True, None, 0.25, kind)
+        near(out[:j], want["out"][:j], bound["out"][:j], f"{j}: rows before it")
+        if bad != float("-inf"):
+            assert out[j:].isnan().all(), j
+        elif j:
+            assert out[j:].isfinite().all(), j
+            S = 0.25 * (f64(q)[j:, 0] @ f64(spoilt)[:, 0].t())
+            P = torch.softmax(S.masked_fill(torch.arange(rows)[None] > torch.arange(j, rows)[:, None], -math.inf), dim=1)
+            near(out[j:, 0], P @ f64(v)[:, 0], 2 * bound["out"][j:, 0] + 4 * ref.U[kind] * (P @ f64(v)[:, 0].abs()), f"{j}: rows behind it")        # fewer terms than the bound's, with weights up to twice and more
+
+
 def test_scores_far_apart_and_large():
     """Scores from -2000 to 2000: no overflow, and one row's largest does not take another's."""
     kind = "bf16"
