@@ -62,6 +62,64 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t (&
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---- pieces of work ----------------------------------------------------------------------------------------------------------------
+// The grid has a block for each piece.  A block that runs takes further ones from those that have not begun (clusterlaunchcontrol), so long and short pieces spread by themselves, and its roles go on from
+// one to the next without the 9000 clocks that a block needs on its way in and out.
+constexpr int kRecent = 8;
+struct PieceShared { uint4 response[2]; uint64_t come[2]; int recent[kRecent]; };      // recent: what a failed wait may have left incomplete
+
+// One warp's.  A request is made a piece ahead.
+struct Pieces {
+    PieceShared* shared;
+    volatile uint32_t* failed;
+    uint32_t asked = 0, got = 0, taken = 0;
+    bool one;
+    __device__ __forceinline__ void note(int piece) {
+        if (one) shared->recent[taken % kRecent] = piece;
+        ++taken;
+    }
+    __device__ __forceinline__ void ask() {
+        if (one) {
+            uint64_t* const bar = shared->come + (asked & 1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive_expect_tx(bar, 16);
+            asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(shared->response + (asked & 1))), "r"(smem_u32(bar)) : "memory");
+        }
+        __syncwarp();
+        ++asked;
+    }
+    __device__ __forceinline__ int first() {
+        note(int(blockIdx.x));
+        ask();
+        return int(blockIdx.x);
+    }
+    // The piece asked for last, and -1 if there is none or the answer does not come.
+    __device__ __forceinline__ int next() {
+        if (!__all_sync(0xffffffffu, wait_in_line(shared->come + (got & 1), got >> 1 & 1, failed))) return -1;
+        const uint32_t at = smem_u32(shared->response + (got & 1));
+        uint32_t there, piece;
+        asm volatile("{\n\t.reg .b128 r;\n\t.reg .pred p;\n\tld.shared.b128 r, [%2];\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                     "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}" : "=r"(there), "=r"(piece) : "r"(at) : "memory");
+        ++got;
+        if (!there) return -1;
+        note(int(piece));
+        return int(piece);
+    }
+    __device__ __forceinline__ int following() {
+        const int piece = next();
+        if (piece >= 0) ask();
+        return piece;
+    }
+    // After a failure: an answer that is on its way is still a piece that nobody else will do.
+    __device__ __forceinline__ void finish() {
+        WaitLimit limit(kWaitNanoseconds, nanoseconds());
+        while (got < asked) {
+            if (mbar_try_wait(shared->come + (got & 1), got >> 1 & 1)) { next(); break; }
+            if (limit.over(nanoseconds())) break;
+        }
+    }
+};
+
 // ---- values that are not finite ------------------------------------------------------------------------------------------------
 // A weight of zero takes a finite value out of a sum, not an infinite one or a NaN.  So in tiles where not every row sees every other the operand is looked through before it is used, by warps that have
 // nothing else to do, and where something is not finite a thread adds up what its row sees itself (some 50 us a tile).  Nothing of this costs the other tiles anything.
@@ -163,7 +221,7 @@ template <int PANELS, int QUERIES> struct ForwardTile {
     static constexpr int weights = apart ? kTile : 0, outputs = apart ? kTile + kTile / 2 : QUERIES * kTile;     // where they begin; another tile's 128 further
     static constexpr int barriers = 2 * kItems + 3 * stages + 7 * QUERIES;
     static constexpr int smem = 1024 + (QUERIES + stages) * bytes + 1024;
-    static_assert(barriers * 8 + 8 + stages * 4 + kItems * int(sizeof(SequenceTile) + 8) <= 1024 && smem <= 227 * 1024 / blocks - (blocks - 1) * 1024 && smem * (blocks + 1) > 227 * 1024, "shared memory");
+    static_assert(barriers * 8 + 8 + stages * 4 + kItems * 24 + 16 + int(sizeof(PieceShared)) <= 1024 && smem <= 227 * 1024 / blocks - (blocks - 1) * 1024 && smem * (blocks + 1) > 227 * 1024, "shared memory");
 };
 // Registers of the warps that compute, and of the others; together those of the launch.
 template <int GROUPS> __device__ __forceinline__ void take_registers() {
@@ -177,8 +235,7 @@ template <int GROUPS> __device__ __forceinline__ void give_registers() {
 
 struct ForwardArgs { HtgsAttention a; void* out; float* sums; unsigned int* error; };
 
-// Blocks stay and go through pieces of work, a head and one or two tiles of queries, one behind the other, against tiles of keys: a block that began for each lost 9000 clocks on its way in and out (262144
-// rows within 512, 27000 for the tiles themselves).  Warp 0 finds the pieces and loads; warps 1 and 2 issue the products, for one tile of queries while the other's softmax (or the other block's) is
+// A piece is a head and one or two tiles of queries, one behind the other, against tiles of keys.  Warp 0 finds the pieces and loads; warps 1 and 2 issue the products, for one tile of queries while the other's softmax (or the other block's) is
 // computed, and the next piece's first scores while the last one's output is stored; warp 3 looks through values of which some are not seen; warps 4 to 7 and 8 to 11 have a tile of queries each, a thread
 // for each row.  Tensor memory of two tiles: scores (weights over them) at 0 and 128, outputs at 256 and 384.  Of one, up to 64 columns wide: scores 0, weights 128, output 192; the next scores are
 // computed as soon as the softmax has read the last ones.
@@ -206,11 +263,14 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
     volatile uint32_t* const failed = tmem_at + 1;
     volatile uint32_t* const dirty = failed + 1;         // [stages], of tiles of values
     volatile int* const items = reinterpret_cast<volatile int*>(dirty + S::stages);        // [kItems] of 6 words
+    PieceShared* const shared = reinterpret_cast<PieceShared*>((reinterpret_cast<uintptr_t>(items + kItems * 6) + 15) & ~uintptr_t(15));
 
     const HtgsAttention& a = args.a;
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, group = a.heads / a.key_heads;
     T* const out = static_cast<T*>(args.out);
     if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) mbar_init(shared->come + i, 1);
+        for (int i = 0; i < kRecent; ++i) shared->recent[i] = -1;
         for (int i = 0; i < kItems; ++i) { mbar_init(item_full + i, 1); mbar_init(item_empty + i, (S::apart ? 2 : 1) + 1 + 4 * QUERIES); }
         for (int i = 0; i < QUERIES; ++i) {
             mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1); mbar_init(scored + i, 1); mbar_init(weighed + i, 4); mbar_init(summed + i, 1); mbar_init(taken + i, 4); mbar_init(drained + i, 4);
@@ -228,11 +288,9 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
-    const int total = int(sequence_tiles(a, QUERIES * kTile)) * a.heads;
+    const int total = int(gridDim.x);
     // Piece `item`: the last tiles of a sequence first, as they have the most keys where attention is causal.
     const auto tile_of = [&](int item) { return find_tile<QUERIES * kTile>(a, (total - 1 - item) / a.heads); };
-    // Rounds there and back, so that a block with a long piece has a short one next.
-    const auto item_of = [&](int round) { return round * int(gridDim.x) + (round & 1 ? int(gridDim.x - 1 - blockIdx.x) : int(blockIdx.x)); };
     const auto head_of = [&](int item) { return item % a.heads; };
 
     // What the roles know of a piece: keys low + [0, 128 n) for the block; tile s of queries sees tiles [from(s), to(s)) of them.
@@ -286,9 +344,9 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
                 __syncwarp();
                 item_at.next();
             };
-            for (int round = 0; ok && round * int(gridDim.x) < total; ++round) {
-                const int item = item_of(round);
-                if (item >= total) continue;
+            Pieces pieces{shared, failed};
+            pieces.one = one;
+            for (int item = pieces.first(); item >= 0 && ok; item = pieces.following()) {
                 const SequenceTile t = tile_of(item);
                 if (t.first >= t.end) continue;
                 const int head = head_of(item);
@@ -326,8 +384,10 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
                     stage.next();
                 }
             }
+            ok = ok && !*failed;
             if (ok) publish({0, 0, 0, 0, false}, 0, 0);
             if (!ok) {              // no copy may be on its way when the block ends
+                pieces.finish();
                 for (uint32_t u = uses > S::stages ? uses - S::stages : 0; u < uses; ++u) {
                     WaitLimit limit(kWaitNanoseconds, nanoseconds());
                     while (!mbar_try_wait(full + u % S::stages, u / S::stages & 1) && !limit.over(nanoseconds())) {}
@@ -610,9 +670,9 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::columns) : "memory");
     }
     if (*failed) {               // a wait ran out: nothing that looks like a result
-        for (int round = 0; round * int(gridDim.x) < total; ++round) {
-            const int item = item_of(round);
-            if (item >= total) continue;
+        for (int k = 0; k < kRecent; ++k) {
+            const int item = shared->recent[k];
+            if (item < 0) continue;
             const SequenceTile t = tile_of(item);
             const int rows = min(QUERIES * kTile, t.end - t.first);
             for (int i = threadIdx.x; i < rows * a.width && !t.outside; i += S::threads)
@@ -1249,8 +1309,7 @@ template <typename T, int PANELS, int QUERIES> int launch_forward(const ForwardA
         return sequence_fail(HTGS_ERR_CUDA, "htgs_attention: the tensor maps cannot be made");
     static PerDeviceOnce once;
     cudaError_t err = once.run([] { return cudaFuncSetAttribute(attention_tiles_kernel<T, PANELS, QUERIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem); });
-    const int64_t pieces = sequence_tiles(a, QUERIES * kTile) * a.heads;
-    if (err == cudaSuccess) err = launch_after(attention_tiles_kernel<T, PANELS, QUERIES>, dim3(unsigned(pieces < 148 * S::blocks ? pieces : 148 * S::blocks)), S::threads, S::smem, stream, q, k, v, args);
+    if (err == cudaSuccess) err = launch_after(attention_tiles_kernel<T, PANELS, QUERIES>, dim3(unsigned(sequence_tiles(a, QUERIES * kTile) * a.heads)), S::threads, S::smem, stream, q, k, v, args);
     return err == cudaSuccess ? sequence_status("htgs_attention") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 template <typename T, int PANELS> int launch_backward(const BackwardArgs& args, cudaStream_t stream) {
