@@ -60,6 +60,13 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t (&
                  ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
                    "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
+__device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+                 "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
+                 "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- pieces of work ----------------------------------------------------------------------------------------------------------------
@@ -124,13 +131,13 @@ struct Pieces {
 // A weight of zero takes a finite value out of a sum, not an infinite one or a NaN.  So in tiles where not every row sees every other the operand is looked through before it is used, by warps that have
 // nothing else to do, and where something is not finite a thread adds up what its row sees itself (some 50 us a tile).  Nothing of this costs the other tiles anything.
 
-// Whether a tile holds such values; by a warp.
-template <typename T, int PANELS> __device__ __forceinline__ bool not_finite(const unsigned char* tile, int lane) {
+// Whether so much of a tile holds such values; by a warp.
+template <typename T, int BYTES> __device__ __forceinline__ bool not_finite(const unsigned char* tile, int lane) {
     using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     const uint32_t zero = 0;
     Two sum = *reinterpret_cast<const Two*>(&zero);
     #pragma unroll 4
-    for (int i = lane; i < PANELS * kTile * 8; i += 32) {
+    for (int i = lane; i < BYTES / 16; i += 32) {
         const uint4 piece = *reinterpret_cast<const uint4*>(tile + i * 16);
         const Two* v = reinterpret_cast<const Two*>(&piece);
         #pragma unroll
@@ -140,7 +147,7 @@ template <typename T, int PANELS> __device__ __forceinline__ bool not_finite(con
     return __any_sync(0xffffffffu, both.x != 0.0f || both.y != 0.0f);
 }
 // Columns [from, to) of a lane's row of sums in tensor memory: plus (add), or set to, its weights times the rows [low, high] of a tile.  Weights: words of two, 64 at `weights`, 64 at weights + second.
-template <typename T> __device__ __forceinline__ void multiply_seen(uint32_t sums, int from, int to, bool add, uint32_t weights, uint32_t second, const unsigned char* tile, int low, int high) {
+template <typename T> __device__ __forceinline__ void multiply_seen(uint32_t sums, int from, int to, bool add, uint32_t weights, uint32_t second, const unsigned char* tile, int low, int high, int blocks = 4) {
     #pragma unroll 1
     for (int c = from; c < to; c += 16) {
         uint32_t o[16] = {};
@@ -149,7 +156,7 @@ template <typename T> __device__ __forceinline__ void multiply_seen(uint32_t sum
             tmem_loaded();
         }
         #pragma unroll 1
-        for (int block = 0; block < 4; ++block) {
+        for (int block = 0; block < blocks; ++block) {
             uint32_t w[16];
             tmem_begin16(weights + (block >> 1) * second + (block & 1) * 16, w);
             tmem_loaded();
@@ -505,7 +512,7 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
                     bool seen = true;
                     #pragma unroll
                     for (int s = 0; s < QUERIES; ++s) seen = seen && (!(i & 1) || j < any[s].x || j >= any[s].y || (j >= all[s].x && j < all[s].y));
-                    const bool found = !seen && not_finite<T, PANELS>(ring + stage.at * S::bytes, lane);
+                    const bool found = !seen && not_finite<T, S::bytes>(ring + stage.at * S::bytes, lane);
                     if (lane == 0) {
                         dirty[stage.at] = found;
                         arrive(searched + stage.at);
@@ -715,9 +722,9 @@ template <typename T> __device__ __forceinline__ float gradient_lift(const Atten
     if (!(bound >= 1e-30f && bound <= 1e30f)) return 1.0f;
     return __uint_as_float((254u - (__float_as_uint(bound) >> 23)) << 23) * 16384.0f;           // 2^14 / (the power of two that the bound reaches), which is above half of it
 }
-template <typename T> __device__ __forceinline__ void zero_rows(void* to, const SequenceTile& t, int heads, int head, int width) {
+template <typename T> __device__ __forceinline__ void zero_rows(void* to, const SequenceTile& t, int heads, int head, int width, int thread, int threads) {
     const int rows = min(kTile, t.end - t.first), pieces = width / 8;
-    for (int i = threadIdx.x; i < rows * pieces; i += kTilesThreads)
+    for (int i = thread; i < rows * pieces; i += threads)
         *reinterpret_cast<uint4*>(static_cast<T*>(to) + (int64_t(t.first + i / pieces) * heads + head) * width + i % pieces * 8) = make_uint4(0, 0, 0, 0);
 }
 template <typename T> __device__ __forceinline__ void nan_rows(void* to, const SequenceTile& t, int heads, int head, int width) {
@@ -741,6 +748,12 @@ template <typename T> __device__ __forceinline__ void store_sums(uint32_t sums, 
         }
     }
 }
+// Columns [from, to] of 64, as words of two.  On what is stored and not before, so that what is not seen may be anything; and apart from the arithmetic, which else carried it in every tile (14 clocks a value).
+__device__ __forceinline__ void mask_words(uint32_t (&words)[32], int from, int to) {
+    #pragma unroll
+    for (int k = 0; k < 32; ++k)
+        words[k] &= (2 * k >= from && 2 * k <= to ? 0xffffu : 0u) | (2 * k + 1 >= from && 2 * k + 1 <= to ? 0xffff0000u : 0u);
+}
 // A barrier of the eight warps that share a tile's columns, with the limit of every wait.
 __device__ __forceinline__ bool all_meet(uint64_t* met, uint32_t& meetings, int lane, volatile uint32_t* failed) {
     tmem_fence_before();
@@ -750,8 +763,436 @@ __device__ __forceinline__ bool all_meet(uint64_t* met, uint32_t& meetings, int 
     tmem_fence_after();
     return ok;
 }
-// 64 columns from a column on that only [from, to] of count: whether column c of them does.
-__device__ __forceinline__ bool counts(int c, int from, int to) { return c >= from && c <= to; }
+
+// Heads of up to 64: the gradients of k and v (KEYS) or of q of a piece, 128 rows of a head ("own": k and v, or q and dout), against tiles of 64 of the others (q and dout, or k and v), in turns by two
+// warpgroups, a thread for each own row.  Everything that a warpgroup writes or reads has columns of its own, so its next scores and weight gradients are computed while it works on the last ones, and it never
+// waits for more than its own arithmetic.  Warp 0 finds pieces and loads; warp 1 issues the products for scores and weight gradients; warp 2 those that add up, in the tiles' order; warp 3 looks through tiles that
+// are not seen whole.  Tensor memory: scores 0 and 64, weight gradients 128 and 192, weights 256 and 288, score gradients 320 and 352 (of q at both by turns), the sum for k or q 384, for v 448.
+struct NarrowTile {
+    static constexpr int own_bytes = kPanelBytes, other = 64, bytes = other * 128, statistic_bytes = 2 * other * 4, stage_bytes = 2 * bytes + 1024, stages = 6;
+    static constexpr int smem = 1024 + 2 * 2 * own_bytes + stages * stage_bytes + 1024;
+    static_assert((2 * kItems + 4 + 3 * stages + 22 + 2) * 8 + 8 + stages * 4 + kItems * 24 + 16 + int(sizeof(PieceShared)) <= 1024 && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");
+};
+
+template <typename T, bool KEYS>
+__global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(const __grid_constant__ CUtensorMap map_own1, const __grid_constant__ CUtensorMap map_own2, const __grid_constant__ CUtensorMap map_other1,
+                                                                           const __grid_constant__ CUtensorMap map_other2, const __grid_constant__ BackwardArgs args) {
+    using S = NarrowTile;
+    extern __shared__ unsigned char raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* const own = raw + (base - smem_u32(raw));            // two pieces' own rows, one panel and the other
+    unsigned char* const ring = own + 2 * 2 * S::own_bytes;
+    const uint32_t ring_at = base + 2 * 2 * S::own_bytes;
+    uint64_t* const item_full = reinterpret_cast<uint64_t*>(ring + S::stages * S::stage_bytes);
+    uint64_t* const item_empty = item_full + kItems;
+    uint64_t* const own_full = item_empty + kItems;
+    uint64_t* const own_empty = own_full + 2;
+    uint64_t* const full = own_empty + 2;
+    uint64_t* const empty = full + S::stages;
+    uint64_t* const searched = empty + S::stages;
+    // of each warpgroup
+    uint64_t* const scored = searched + S::stages;       // its scores are there
+    uint64_t* const scores_taken = scored + 2;           // and read
+    uint64_t* const graded = scores_taken + 2;           // the gradients of its weights are there
+    uint64_t* const grades_taken = graded + 2;           // and read
+    uint64_t* const weighed = grades_taken + 2;          // its weights are there
+    uint64_t* const changed = weighed + 2;               // the gradients of its scores are: two, by turns, as a warpgroup may be two tiles ahead of the sums
+    uint64_t* const added = changed + 4;                 // and both are in the sums: two, by turns
+    uint64_t* const granted = added + 4;                 // the sums are its to change
+    uint64_t* const returned = granted + 2;              // and not any more
+    uint64_t* const finished = returned + 2;
+    uint64_t* const drained = finished + 1;
+    uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
+    volatile uint32_t* const failed = tmem_at + 1;
+    volatile uint32_t* const dirty = failed + 1;         // [stages]
+    volatile int* const items = reinterpret_cast<volatile int*>(dirty + S::stages);
+    PieceShared* const shared = reinterpret_cast<PieceShared*>((reinterpret_cast<uintptr_t>(items + kItems * 6) + 15) & ~uintptr_t(15));
+
+    const HtgsAttention& a = args.a;
+    const AttentionBackward& b = args.b;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, group = a.heads / a.key_heads, own_heads = KEYS ? a.key_heads : a.heads;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) mbar_init(shared->come + i, 1);
+        for (int i = 0; i < kRecent; ++i) shared->recent[i] = -1;
+        for (int i = 0; i < kItems; ++i) { mbar_init(item_full + i, 1); mbar_init(item_empty + i, 3 + 8); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(own_full + i, 1); mbar_init(own_empty + i, 1); mbar_init(scored + i, 1); mbar_init(scores_taken + i, 4); mbar_init(graded + i, 1); mbar_init(grades_taken + i, 4);
+            mbar_init(weighed + i, 4); mbar_init(changed + 2 * i, 4); mbar_init(changed + 2 * i + 1, 4); mbar_init(added + 2 * i, 1); mbar_init(added + 2 * i + 1, 1); mbar_init(granted + i, 1); mbar_init(returned + i, 4);
+        }
+        mbar_init(finished, 1);
+        mbar_init(drained, 8);
+        for (int i = 0; i < S::stages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 2); mbar_init(searched + i, 1); }
+        *failed = 0;
+        mbar_fence_init();
+    }
+    grid_dependency();               // before tensor memory is taken, which a block of the kernel before may still have to get
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tmem_fence_before();
+    }
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+    constexpr uint32_t kGrades = 128, kWeights = 256, kChanges = 320, kSums = 384;
+    // Pieces with the most to do first, where attention is causal: the first tiles of keys, the last ones of queries.
+    const auto tile_of = [&](int item) { return find_tile<kTile>(a, KEYS ? item / own_heads : int(gridDim.x - 1 - item) / own_heads); };
+    const auto head_of = [&](int item) { return item % own_heads; };
+
+    // A piece: `tiles` tiles of 64 others from row `low` on, for each of the `turns` query heads of a key head; tiles [whole.x, whole.y) are seen (or see) whole.
+    struct Piece {
+        int begin, end, first, head, sequence, low, tiles, n;
+        int2 whole;
+    };
+    Piece piece;
+    const auto set_piece = [&](int begin, int end, int first, int head, int sequence) {
+        const int last = min(first + kTile, end) - 1;
+        int low, high, all_low, all_high;
+        if (KEYS) {
+            low = begin + (first_seeing(a, begin, first) - begin) / S::other * S::other;      // the statistics' tiles begin with the sequence
+            high = last_seeing(a, end, last); all_low = first_seeing(a, begin, last); all_high = last_seeing(a, end, first);
+        } else {
+            low = first_seen(a, begin, first);
+            high = last_seen(a, end, last); all_low = first_seen(a, begin, last); all_high = last_seen(a, end, first);
+        }
+        const int tiles = (high - low) / S::other + 1;
+        piece = {begin, end, first, head, sequence, low, tiles, KEYS ? group * tiles : tiles, make_int2((all_low - low + S::other - 1) / S::other, (all_high - low + 1) / S::other)};
+    };
+    Ring<kItems> item_at;
+    const auto next_piece = [&] {
+        if (!__all_sync(0xffffffffu, wait_in_line(item_full + item_at.at, item_at.round, failed))) return false;
+        volatile int* const from = items + 6 * item_at.at;
+        const bool there = from[5];
+        if (there) set_piece(from[0], from[1], from[2], from[3], from[4]);
+        __syncwarp();
+        if (lane == 0) arrive(item_empty + item_at.at);
+        item_at.next();
+        return there;
+    };
+    const auto tile_in_turn = [&](uint32_t i) { return KEYS ? int(i % uint32_t(piece.tiles)) : int(i); };
+    const auto seen_whole = [&](int tile) { return tile >= piece.whole.x && tile < piece.whole.y; };
+
+    if (warp < 4) {
+        give_registers<2>();
+        const bool one = elect_one();
+        bool ok = true;
+        const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, wait_in_line(bar, parity, failed)); };
+        uint32_t u = 0, pieces_done = 0;              // tiles of others and pieces so far
+        if (warp == 0) {
+            Ring<S::stages> stage;
+            const auto publish = [&](const SequenceTile& t, int head, int there) {
+                wait(item_empty + item_at.at, item_at.round ^ 1);
+                if (!ok) return;
+                if (lane == 0) {
+                    volatile int* const to = items + 6 * item_at.at;
+                    to[0] = t.begin; to[1] = t.end; to[2] = t.first; to[3] = head; to[4] = t.sequence; to[5] = there;
+                    arrive(item_full + item_at.at);
+                }
+                __syncwarp();
+                item_at.next();
+            };
+            Pieces pieces{shared, failed};
+            pieces.one = one;
+            for (int item = pieces.first(); item >= 0 && ok; item = pieces.following()) {
+                const SequenceTile t = tile_of(item);
+                if (t.first >= t.end) continue;
+                const int head = head_of(item);
+                if (t.outside) {
+                    zero_rows<T>(KEYS ? b.grad_k : b.grad_q, t, own_heads, head, a.width, lane, 32);
+                    if (KEYS) zero_rows<T>(b.grad_v, t, own_heads, head, a.width, lane, 32);
+                    __syncwarp();
+                    continue;
+                }
+                publish(t, head, 1);
+                set_piece(t.begin, t.end, t.first, head, t.sequence);
+                const uint32_t place = pieces_done & 1;
+                wait(own_empty + place, (pieces_done >> 1 & 1) ^ 1);
+                if (!ok) break;
+                if (one) {
+                    mbar_arrive_expect_tx(own_full + place, 2 * S::own_bytes);
+                    load_panel(own + place * 2 * S::own_bytes, &map_own1, 0, head, t.first, own_full + place);
+                    load_panel(own + (place * 2 + 1) * S::own_bytes, &map_own2, 0, head, t.first, own_full + place);
+                }
+                __syncwarp();
+                ++pieces_done;
+                for (int i = 0; i < piece.n && ok; ++i) {
+                    wait(empty + stage.at, stage.round ^ 1);
+                    if (!ok) break;
+                    if (one) {
+                        const int tile = tile_in_turn(i), other_head = KEYS ? head * group + i / piece.tiles : head / group, row = piece.low + tile * S::other;
+                        unsigned char* const at = ring + stage.at * S::stage_bytes;
+                        mbar_arrive_expect_tx(full + stage.at, 2 * S::bytes + (KEYS ? S::statistic_bytes : 0));
+                        load_panel(at, &map_other1, 0, other_head, row, full + stage.at);
+                        load_panel(at + S::bytes, &map_other2, 0, other_head, row, full + stage.at);
+                        if (KEYS) {
+                            const int64_t r = statistic_base(a, t) + (row - t.begin);
+                            const float* from = b.statistics + (other_head * b.statistics_rows + r / kStatisticRows * kStatisticRows) * 2 + r % kStatisticRows;
+                            bulk_copy_g2s(at + 2 * S::bytes, from, S::statistic_bytes / 2, full + stage.at);
+                            bulk_copy_g2s(at + 2 * S::bytes + S::statistic_bytes / 2, from + kStatisticRows, S::statistic_bytes / 2, full + stage.at);
+                        }
+                    }
+                    __syncwarp();
+                    ++u;
+                    stage.next();
+                }
+            }
+            ok = ok && !*failed;
+            if (ok) publish({0, 0, 0, 0, false}, 0, 0);
+            if (!ok) {              // no copy may be on its way when the block ends
+                pieces.finish();
+                for (uint32_t x = u > S::stages ? u - S::stages : 0; x < u; ++x) {
+                    WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                    while (!mbar_try_wait(full + x % S::stages, x / S::stages & 1) && !limit.over(nanoseconds())) {}
+                }
+                for (uint32_t x = pieces_done > 2 ? pieces_done - 2 : 0; x < pieces_done; ++x) {
+                    WaitLimit limit(kWaitNanoseconds, nanoseconds());
+                    while (!mbar_try_wait(own_full + (x & 1), x >> 1 & 1) && !limit.over(nanoseconds())) {}
+                }
+            }
+        } else if (warp == 1) {
+            const uint32_t score = instruction<T>(S::other, false);
+            const int steps = (a.width + 15) / 16;
+            const auto product = [&](uint32_t to, uint32_t x, uint32_t y, uint64_t* bar) {
+                if (one) {
+                    for (int i = 0; i < steps; ++i) multiply(to, x + i * 2, y + i * 2, score, i > 0);
+                    commit(bar);
+                }
+                __syncwarp();
+            };
+            while (ok && next_piece()) {
+                const uint32_t place = pieces_done & 1, x = along_columns(base + place * 2 * S::own_bytes);
+                wait(own_full + place, pieces_done >> 1 & 1);
+                ++pieces_done;
+                for (int i = 0; i < piece.n && ok; ++i, ++u) {
+                    const uint32_t h = u & 1, parity = (u >> 1 & 1) ^ 1, slot = u % S::stages, y = along_columns(ring_at + slot * S::stage_bytes);
+                    wait(full + slot, u / S::stages & 1);
+                    wait(scores_taken + h, parity);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    product(tmem + h * 64, x, y, scored + h);
+                    wait(grades_taken + h, parity);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    product(tmem + kGrades + h * 64, x + (S::own_bytes >> 4), y + (S::bytes >> 4), graded + h);
+                }
+                if (one && ok) commit(own_empty + place);
+                __syncwarp();
+            }
+        } else if (warp == 2) {
+            const uint32_t sum = instruction<T>((a.width + 15) & ~15, true);
+            uint32_t grants[2] = {0, 0};
+            const auto gather = [&](uint32_t to, uint32_t weights, uint32_t y, bool first) {
+                if (one) {
+                    #pragma unroll
+                    for (int i = 0; i < S::other / 16; ++i) multiply_tmem(to, weights + i * 8, y + i * (2048 >> 4), sum, !first || i > 0);
+                }
+                __syncwarp();
+            };
+            while (ok && next_piece()) {
+                wait(drained, (pieces_done & 1) ^ 1);
+                ++pieces_done;
+                for (int i = 0; i < piece.n && ok; ++i, ++u) {
+                    const uint32_t h = u & 1, parity = u >> 1 & 1, slot = u % S::stages, y = along_rows(ring_at + slot * S::stage_bytes);
+                    const bool all = seen_whole(tile_in_turn(i));
+                    if (KEYS) {
+                        wait(weighed + h, parity);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        if (all || !dirty[slot]) gather(tmem + kSums + 64, tmem + kWeights + h * 32, y + (S::bytes >> 4), i == 0);
+                    }
+                    wait(changed + 2 * h + parity, u >> 2 & 1);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    if (all || !dirty[slot]) gather(tmem + kSums, tmem + h * 32 + (KEYS || u >> 1 & 1 ? kChanges : kWeights), y, i == 0);
+                    else {                         // the warpgroup adds them itself, when all before are in and before those behind
+                        if (one) commit(granted + h);
+                        __syncwarp();
+                        wait(returned + h, (h ? grants[1]++ : grants[0]++) & 1);
+                        if (!ok) break;
+                        tmem_fence_after();
+                    }
+                    if (one) { commit(added + 2 * h + parity); commit(empty + slot); }
+                    __syncwarp();
+                }
+                if (one && ok) commit(finished);
+                __syncwarp();
+            }
+        } else {
+            while (ok && next_piece()) {
+                for (int i = 0; i < piece.n && ok; ++i, ++u) {
+                    const uint32_t slot = u % S::stages;
+                    wait(full + slot, u / S::stages & 1);
+                    if (!ok) break;
+                    const unsigned char* const at = ring + slot * S::stage_bytes;
+                    const bool found = !seen_whole(tile_in_turn(i)) && not_finite<T, 2 * S::bytes>(at, lane);
+                    if (lane == 0) {
+                        dirty[slot] = found;
+                        arrive(searched + slot);
+                        arrive(empty + slot);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        take_registers<2>();
+        const uint32_t h = uint32_t(warp >> 2) - 1;
+        const int quarter = (warp & 3) * 32;
+        const uint32_t lanes = uint32_t(quarter) << 16, score = tmem + lanes + h * 64, grade = tmem + lanes + kGrades + h * 64, weights = tmem + lanes + kWeights + h * 32,
+                       sums = tmem + lanes + kSums;
+        const float scale = a.scale * kLog2e;
+        const f32x2 scale2 = pack2(scale, scale), minus = pack2(-1.0f, -1.0f);
+        constexpr float kLifted = KEYS ? kWeightLift<T> : 0.0f;                  // weights of keys go into a product themselves
+        const f32x2 weight_lift2 = pack2(kLifted, kLifted);
+        uint32_t u0 = 0, pieces_done = 0, grants = 0;
+        bool ok = true;
+        while (ok && next_piece()) {
+            const int row = min(piece.first + quarter + lane, piece.end - 1);
+            const bool there = piece.first + quarter + lane < piece.end;
+            const int seen_low = (KEYS ? first_seeing(a, piece.begin, row) : first_seen(a, piece.begin, row)) - piece.low;
+            const int seen_high = (KEYS ? last_seeing(a, piece.end, row) : last_seen(a, piece.end, row)) - piece.low;
+            const float lift = gradient_lift<T>(b, piece.sequence), change_lift = lift * exp2f(-kLifted);
+            const f32x2 lift2 = pack2(change_lift, change_lift);
+            f32x2 row_off2 = weight_lift2, row_mean2 = weight_lift2;
+            if (!KEYS) {
+                const int64_t r = statistic_base(a, {piece.sequence, piece.begin, piece.end, piece.first, false}) + (row - piece.begin);
+                const float* from = b.statistics + (piece.head * b.statistics_rows + r / kStatisticRows * kStatisticRows) * 2 + r % kStatisticRows;
+                row_off2 = pack2(-from[0], -from[0]);
+                row_mean2 = pack2(-from[kStatisticRows], -from[kStatisticRows]);
+            }
+            for (uint32_t u = u0 + ((u0 ^ h) & 1); u < u0 + piece.n; u += 2) {
+                const uint32_t parity = u >> 1 & 1, slot = u % S::stages;
+                const int tile = tile_in_turn(u - u0), from = seen_low - tile * S::other, to = seen_high - tile * S::other;
+                const bool masked = !seen_whole(tile);
+                const float4* const statistics = reinterpret_cast<const float4*>(ring + slot * S::stage_bytes + 2 * S::bytes);
+                ok = __all_sync(0xffffffffu, (!KEYS || wait_in_line(full + slot, u / S::stages & 1, failed)) && wait_in_line(scored + h, parity, failed));
+                if (!ok) break;
+                // What this tile's weights and score gradients write over is in the sums: the last tile's, or of q, whose score gradients have two places, the last but one's.  Asked where nothing waits for it.
+                const uint32_t turn = u >> 1, over = turn - (KEYS ? 1 : 2);
+                uint64_t* const old = added + 2 * h + (over & 1);
+                const bool free = turn < (KEYS ? 1 : 2) || mbar_test(old, over >> 1 & 1);
+                tmem_fence_after();
+                uint32_t p[64];
+                tmem_begin32(score, p);
+                tmem_begin32(score + 32, p + 32);
+                tmem_loaded();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(scores_taken + h);
+                #pragma unroll
+                for (int c = 0; c < 64; c += 4) {
+                    const float4 off = KEYS ? statistics[c / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    #pragma unroll
+                    for (int k = 0; k < 4; k += 2) {
+                        const f32x2 off2 = KEYS ? fma2(k ? pack2(off.z, off.w) : pack2(off.x, off.y), minus, weight_lift2) : row_off2;
+                        const float2 x = unpack2(exp2_pair(fma2(pack2(__uint_as_float(p[c + k]), __uint_as_float(p[c + k + 1])), scale2, off2)));
+                        p[c + k] = __float_as_uint(x.x);
+                        p[c + k + 1] = __float_as_uint(x.y);
+                    }
+                }
+                if (!free) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(old, over >> 1 & 1, failed));
+                    if (!ok) break;
+                }
+                if (KEYS) {
+                    uint32_t words[32];
+                    #pragma unroll
+                    for (int k = 0; k < 32; ++k) words[k] = floats_pair<T>(__uint_as_float(p[2 * k]), __uint_as_float(p[2 * k + 1]));
+                    if (masked) mask_words(words, from, to);
+                    tmem_store32(weights, words);
+                    tmem_stored();
+                    if (masked) {
+                        ok = __all_sync(0xffffffffu, wait_in_line(searched + slot, u / S::stages & 1, failed));
+                        if (!ok) break;
+                    }
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(weighed + h);
+                }
+                ok = __all_sync(0xffffffffu, wait_in_line(graded + h, parity, failed));
+                if (!ok) break;
+                tmem_fence_after();
+                uint32_t g[64];
+                tmem_begin32(grade, g);
+                tmem_begin32(grade + 32, g + 32);
+                tmem_loaded();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(grades_taken + h);
+                const uint32_t changes = tmem + lanes + h * 32 + (KEYS || turn & 1 ? kChanges : kWeights);
+                {
+                    uint32_t words[32];
+                    #pragma unroll
+                    for (int c = 0; c < 64; c += 4) {
+                        const float4 mean = KEYS ? statistics[16 + c / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        #pragma unroll
+                        for (int k = 0; k < 4; k += 2) {
+                            const f32x2 grad = pack2(__uint_as_float(g[c + k]), __uint_as_float(g[c + k + 1])), weight = pack2(__uint_as_float(p[c + k]), __uint_as_float(p[c + k + 1]));
+                            const f32x2 away = KEYS ? fma2(k ? pack2(mean.z, mean.w) : pack2(mean.x, mean.y), minus, grad) : add2(grad, row_mean2);
+                            const float2 ds = unpack2(mul2(std::is_same<T, __half>::value ? mul2(weight, lift2) : weight, away));
+                            words[(c + k) / 2] = floats_pair<T>(ds.x, ds.y);
+                        }
+                    }
+                    if (masked) mask_words(words, from, to);
+                    tmem_store32(changes, words);
+                }
+                tmem_stored();
+                if (!KEYS && masked) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(searched + slot, u / S::stages & 1, failed));
+                    if (!ok) break;
+                }
+                const bool spoilt = masked && dirty[slot];
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(changed + 2 * h + parity);
+                if (spoilt) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(full + slot, u / S::stages & 1, failed) && wait_in_line(granted + h, grants & 1, failed));
+                    if (!ok) break;
+                    ++grants;
+                    tmem_fence_after();
+                    multiply_seen<T>(sums, 0, a.width, u > u0, changes, 0, ring + slot * S::stage_bytes, from, to, 2);
+                    if (KEYS) multiply_seen<T>(sums + 64, 0, a.width, u > u0, weights, 0, ring + slot * S::stage_bytes + S::bytes, from, to, 2);
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(returned + h);
+                }
+            }
+            u0 += piece.n;
+            if (!ok) break;
+            ok = __all_sync(0xffffffffu, wait_in_line(finished, pieces_done & 1, failed));
+            if (!ok) break;
+            ++pieces_done;
+            tmem_fence_after();
+            const int64_t at = (int64_t(row) * own_heads + piece.head) * a.width;
+            const int middle = min((a.width / 2 + 15) & ~15, a.width);
+            if (!KEYS) store_sums<T>(sums, static_cast<T*>(b.grad_q) + at, h ? middle : 0, h ? a.width : middle, a.scale / lift, there);
+            else if (h) store_sums<T>(sums + 64, static_cast<T*>(b.grad_v) + at, 0, a.width, exp2f(-kLifted), there);
+            else store_sums<T>(sums, static_cast<T*>(b.grad_k) + at, 0, a.width, a.scale / lift, there);
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(drained);
+        }
+        tmem_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (*failed) {
+        for (int k = 0; k < kRecent; ++k) {
+            if (shared->recent[k] < 0) continue;
+            const SequenceTile t = tile_of(shared->recent[k]);
+            if (t.outside) continue;
+            nan_rows<T>(KEYS ? b.grad_k : b.grad_q, t, own_heads, head_of(shared->recent[k]), a.width);
+            if (KEYS) nan_rows<T>(b.grad_v, t, own_heads, head_of(shared->recent[k]), a.width);
+        }
+        if (threadIdx.x == 0) {
+            *reinterpret_cast<volatile unsigned int*>(args.error) = 1;
+            __threadfence_system();
+        }
+    }
+}
 
 // Gradients of k and v of a tile.  Scores and their gradients are turned round, a row for each key, so that the weights are the first operand from tensor memory.  Warp 0 loads queries, output gradients and
 // statistics of a tile of queries; warp 1 issues the products, [dv, next scores] while the score gradients are computed and [dk, next weight gradients] while the weights are; warps 4 to 7 and 8 to 11
@@ -788,8 +1229,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
     const SequenceTile t = find_tile<kTile>(a, int(blockIdx.x / a.key_heads));
     if (t.first >= t.end) return;
     if (t.outside) {
-        zero_rows<T>(b.grad_k, t, a.key_heads, key_head, a.width);
-        zero_rows<T>(b.grad_v, t, a.key_heads, key_head, a.width);
+        zero_rows<T>(b.grad_k, t, a.key_heads, key_head, a.width, threadIdx.x, kTilesThreads);
+        zero_rows<T>(b.grad_v, t, a.key_heads, key_head, a.width, threadIdx.x, kTilesThreads);
         return;
     }
     const int last_row = min(t.first + kTile, t.end) - 1;
@@ -917,7 +1358,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
                 bool found = false;
                 if (!whole(query_row(i))) {
                     const unsigned char* tile = ring + stage.at * S::stage_bytes + (warp == 2 ? S::bytes : 0);
-                    found = not_finite<T, PANELS>(tile, lane);
+                    found = not_finite<T, S::bytes>(tile, lane);
                 }
                 if (lane == 0) {
                     dirty[2 * stage.at + warp - 2] = found;
@@ -954,9 +1395,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
             tmem_begin32(score, p);
             tmem_begin32(score + 32, p + 32);
             tmem_loaded();
+            uint32_t words[32];
             #pragma unroll
             for (int c = 0; c < 64; c += 32) {
-                uint32_t words[16];
                 #pragma unroll
                 for (int k = 0; k < 32; k += 4) {
                     const float4 sums = statistics[(c + k) / 4];
@@ -964,18 +1405,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
                     for (int h = 0; h < 4; h += 2) {
                         const f32x2 off = fma2(h ? pack2(sums.z, sums.w) : pack2(sums.x, sums.y), minus, weight_lift2);
                         const float2 x = unpack2(fma2(pack2(__uint_as_float(p[c + k + h]), __uint_as_float(p[c + k + h + 1])), scale2, off));
-                        float p0 = exp2_approx(x.x), p1 = exp2_approx(x.y);
-                        if (masked) {
-                            p0 = counts(c + k + h + half * 64, from, to) ? p0 : 0.0f;
-                            p1 = counts(c + k + h + 1 + half * 64, from, to) ? p1 : 0.0f;
-                        }
+                        const float p0 = exp2_approx(x.x), p1 = exp2_approx(x.y);
                         p[c + k + h] = __float_as_uint(p0);
                         p[c + k + h + 1] = __float_as_uint(p1);
-                        words[(k + h) / 2] = floats_pair<T>(p0, p1);
+                        words[(c + k + h) / 2] = floats_pair<T>(p0, p1);
                     }
                 }
-                tmem_store16(score + c / 2, words);
             }
+            if (masked) mask_words(words, from - half * 64, to - half * 64);
+            tmem_store32(score, words);
             tmem_stored();
             uint32_t spoilt[2] = {0, 0};
             if (masked) {
@@ -996,7 +1434,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
             tmem_fence_after();
             #pragma unroll
             for (int c = 0; c < 64; c += 32) {
-                uint32_t g[32], words[16];
+                uint32_t g[32];
                 tmem_begin32(grade + c, g);
                 tmem_loaded();
                 #pragma unroll
@@ -1005,16 +1443,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
                     #pragma unroll
                     for (int h = 0; h < 4; h += 2) {
                         const f32x2 away = fma2(h ? pack2(means.z, means.w) : pack2(means.x, means.y), minus, pack2(__uint_as_float(g[k + h]), __uint_as_float(g[k + h + 1])));
-                        float2 ds = unpack2(mul2(mul2(pack2(__uint_as_float(p[c + k + h]), __uint_as_float(p[c + k + h + 1])), lift2), away));
-                        if (masked) {
-                            ds.x = counts(c + k + h + half * 64, from, to) ? ds.x : 0.0f;
-                            ds.y = counts(c + k + h + 1 + half * 64, from, to) ? ds.y : 0.0f;
-                        }
-                        words[(k + h) / 2] = floats_pair<T>(ds.x, ds.y);
+                        const f32x2 weight = pack2(__uint_as_float(p[c + k + h]), __uint_as_float(p[c + k + h + 1]));
+                        const float2 ds = unpack2(mul2(std::is_same<T, __half>::value ? mul2(weight, lift2) : weight, away));
+                        words[(c + k + h) / 2] = floats_pair<T>(ds.x, ds.y);
                     }
                 }
-                tmem_store16(grade + c / 2, words);
             }
+            if (masked) mask_words(words, from - half * 64, to - half * 64);
+            tmem_store32(grade, words);
             tmem_stored();
             if (spoilt[1]) {
                 ok = meet();
@@ -1080,7 +1516,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(con
     const SequenceTile t = find_tile<kTile>(a, int(gridDim.x / a.heads - 1 - blockIdx.x / a.heads));
     if (t.first >= t.end) return;
     if (t.outside) {
-        zero_rows<T>(b.grad_q, t, a.heads, head, a.width);
+        zero_rows<T>(b.grad_q, t, a.heads, head, a.width, threadIdx.x, kTilesThreads);
         return;
     }
     const int last_row = min(t.first + kTile, t.end) - 1;
@@ -1186,7 +1622,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(con
             Ring<S::stages> stage;
             for (int i = 0; i < 2 * n; ++i, stage.next()) {
                 if (!__all_sync(0xffffffffu, wait_in_line(full + stage.at, stage.round, failed))) break;
-                const bool found = warp == 2 && !(i & 1) && !whole(i >> 1) && not_finite<T, PANELS>(ring + stage.at * S::bytes, lane);
+                const bool found = warp == 2 && !(i & 1) && !whole(i >> 1) && not_finite<T, S::bytes>(ring + stage.at * S::bytes, lane);
                 if (lane == 0) {
                     dirty[2 * stage.at + warp - 2] = found;
                     arrive(searched + stage.at);
@@ -1230,23 +1666,21 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(con
             ok = __all_sync(0xffffffffu, wait_in_line(graded, j & 1, failed));
             if (!ok) break;
             tmem_fence_after();
+            uint32_t words[32];
             #pragma unroll
             for (int c = 0; c < 64; c += 32) {
-                uint32_t g[32], words[16];
+                uint32_t g[32];
                 tmem_begin32(grade + c, g);
                 tmem_loaded();
                 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
-                    const f32x2 away = add2(pack2(__uint_as_float(g[k]), __uint_as_float(g[k + 1])), mean2);
-                    float2 ds = unpack2(mul2(mul2(pack2(__uint_as_float(p[c + k]), __uint_as_float(p[c + k + 1])), lift2), away));
-                    if (masked) {
-                        ds.x = counts(c + k + half * 64, from, to) ? ds.x : 0.0f;
-                        ds.y = counts(c + k + 1 + half * 64, from, to) ? ds.y : 0.0f;
-                    }
-                    words[k / 2] = floats_pair<T>(ds.x, ds.y);
+                    const f32x2 away = add2(pack2(__uint_as_float(g[k]), __uint_as_float(g[k + 1])), mean2), weight = pack2(__uint_as_float(p[c + k]), __uint_as_float(p[c + k + 1]));
+                    const float2 ds = unpack2(mul2(std::is_same<T, __half>::value ? mul2(weight, lift2) : weight, away));
+                    words[(c + k) / 2] = floats_pair<T>(ds.x, ds.y);
                 }
-                tmem_store16(score + c / 2, words);
             }
+            if (masked) mask_words(words, from - half * 64, to - half * 64);
+            tmem_store32(score, words);
             tmem_stored();
             if (masked) {
                 const uint32_t at = uint32_t(2 * j) % S::stages, round = uint32_t(2 * j) / S::stages & 1;
@@ -1285,12 +1719,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(con
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
-// [rows, heads, width] in boxes of 128 rows and a panel of one head's columns.
-bool make_rows_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int width, int64_t stride, int64_t head_stride) {
+// [rows, heads, width] in boxes of so many rows and a panel of one head's columns.
+bool make_rows_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int width, int64_t stride, int64_t head_stride, int box_rows = kTile) {
     const cuuint64_t dense = cuuint64_t(width) * 2;                 // a stride that takes no step says nothing
     const cuuint64_t sizes[3] = {cuuint64_t(width), cuuint64_t(heads), cuuint64_t(rows)};
     const cuuint64_t strides[2] = {heads > 1 ? cuuint64_t(head_stride) * 2 : dense, rows > 1 ? cuuint64_t(stride) * 2 : dense * cuuint64_t(heads)};
-    const cuuint32_t box[3] = {kPanel, 1, kTile}, steps[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {kPanel, 1, cuuint32_t(box_rows)}, steps[3] = {1, 1, 1};
     const EncodeTiled encode = encode_tiled();
     return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1328,8 +1762,27 @@ template <typename T, int PANELS> int launch_backward(const BackwardArgs& args, 
     if (err == cudaSuccess) err = launch_after(attention_queries_kernel<T, PANELS>, dim3(unsigned(tiles * a.heads)), kTilesThreads, QueriesTile<PANELS>::smem, stream, q, k, v, grad, args);
     return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
+template <typename T> int launch_narrow(const BackwardArgs& args, cudaStream_t stream) {
+    const HtgsAttention& a = args.a;
+    const auto maps = [&](CUtensorMap (&m)[4], int rows) {          // q, k, v, dout
+        return make_rows_map(&m[0], a.q, a.rows, a.heads, a.width, a.q_stride, a.q_head_stride, rows) && make_rows_map(&m[1], a.k, a.rows, a.key_heads, a.width, a.k_stride, a.k_head_stride, rows) &&
+               make_rows_map(&m[2], a.v, a.rows, a.key_heads, a.width, a.v_stride, a.v_head_stride, rows) &&
+               make_rows_map(&m[3], args.b.grad, a.rows, a.heads, a.width, args.b.grad_stride, args.b.grad_head_stride, rows);
+    };
+    CUtensorMap own[4], other[4];
+    if (!maps(own, kTile) || !maps(other, NarrowTile::other)) return sequence_fail(HTGS_ERR_CUDA, "htgs_attention_backward: the tensor maps cannot be made");
+    static PerDeviceOnce once;
+    cudaError_t err = once.run([] {
+        const cudaError_t e = cudaFuncSetAttribute(attention_narrow_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, NarrowTile::smem);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(attention_narrow_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, NarrowTile::smem);
+    });
+    const int64_t tiles = sequence_tiles(a, kTile);
+    if (err == cudaSuccess) err = launch_after(attention_narrow_kernel<T, true>, dim3(unsigned(tiles * a.key_heads)), kTilesThreads, NarrowTile::smem, stream, own[1], own[2], other[0], other[3], args);
+    if (err == cudaSuccess) err = launch_after(attention_narrow_kernel<T, false>, dim3(unsigned(tiles * a.heads)), kTilesThreads, NarrowTile::smem, stream, own[0], own[3], other[1], other[2], args);
+    return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
+}
 template <typename T> int backward_typed(const BackwardArgs& args, cudaStream_t stream) {
-    return args.a.width <= kPanel ? launch_backward<T, 1>(args, stream) : launch_backward<T, 2>(args, stream);
+    return args.a.width <= kPanel ? launch_narrow<T>(args, stream) : launch_backward<T, 2>(args, stream);
 }
 template <typename T> int forward_typed(const ForwardArgs& args, cudaStream_t stream) {
     return args.a.width <= kPanel ? launch_forward<T, 1, 1>(args, stream) : launch_forward<T, 2, 2>(args, stream);
