@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
                 ok = __all_sync(0xffffffffu, wait_in_line(scored + s, tiles_done & 1, failed));
                 if (!ok) break;
                 tmem_fence_after();
-                const bool used = S::apart && j > from && mbar_test(summed + s, (tiles_done - 1) & 1);      // the last tile's weights: asked here, where nothing waits for it
+                const bool used = S::apart && j > from && __all_sync(0xffffffffu, mbar_test(summed + s, (tiles_done - 1) & 1));      // the last tile's weights: asked here, where nothing waits for it
                 uint32_t v[128];
                 tmem_begin32(score, v);
                 tmem_begin32(score + 32, v + 32);
@@ -869,7 +869,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
         item_at.next();
         return there;
     };
-    const auto tile_in_turn = [&](uint32_t i) { return KEYS ? int(i % uint32_t(piece.tiles)) : int(i); };
+    // The tile that comes `step` behind a tile; the tiles begin again with each query head.
+    const auto after = [&](int tile, int step) {
+        tile += step;
+        if (KEYS) while (tile >= piece.tiles) tile -= piece.tiles;
+        return tile;
+    };
     const auto seen_whole = [&](int tile) { return tile >= piece.whole.x && tile < piece.whole.y; };
 
     if (warp < 4) {
@@ -915,11 +920,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                 }
                 __syncwarp();
                 ++pieces_done;
+                int tile = 0, other_head = KEYS ? head * group : head / group;
                 for (int i = 0; i < piece.n && ok; ++i) {
                     wait(empty + stage.at, stage.round ^ 1);
                     if (!ok) break;
                     if (one) {
-                        const int tile = tile_in_turn(i), other_head = KEYS ? head * group + i / piece.tiles : head / group, row = piece.low + tile * S::other;
+                        const int row = piece.low + tile * S::other;
                         unsigned char* const at = ring + stage.at * S::stage_bytes;
                         mbar_arrive_expect_tx(full + stage.at, 2 * S::bytes + (KEYS ? S::statistic_bytes : 0));
                         load_panel(at, &map_other1, 0, other_head, row, full + stage.at);
@@ -934,6 +940,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                     __syncwarp();
                     ++u;
                     stage.next();
+                    if (++tile == piece.tiles) { tile = 0; ++other_head; }
                 }
             }
             ok = ok && !*failed;
@@ -991,9 +998,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
             while (ok && next_piece()) {
                 wait(drained, (pieces_done & 1) ^ 1);
                 ++pieces_done;
-                for (int i = 0; i < piece.n && ok; ++i, ++u) {
+                int tile = 0;
+                for (int i = 0; i < piece.n && ok; ++i, ++u, tile = after(tile, 1)) {
                     const uint32_t h = u & 1, parity = u >> 1 & 1, slot = u % S::stages, y = along_rows(ring_at + slot * S::stage_bytes);
-                    const bool all = seen_whole(tile_in_turn(i));
+                    const bool all = seen_whole(tile);
                     if (KEYS) {
                         wait(weighed + h, parity);
                         if (!ok) break;
@@ -1019,12 +1027,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
             }
         } else {
             while (ok && next_piece()) {
-                for (int i = 0; i < piece.n && ok; ++i, ++u) {
+                int tile = 0;
+                for (int i = 0; i < piece.n && ok; ++i, ++u, tile = after(tile, 1)) {
                     const uint32_t slot = u % S::stages;
                     wait(full + slot, u / S::stages & 1);
                     if (!ok) break;
                     const unsigned char* const at = ring + slot * S::stage_bytes;
-                    const bool found = !seen_whole(tile_in_turn(i)) && not_finite<T, 2 * S::bytes>(at, lane);
+                    const bool found = !seen_whole(tile) && not_finite<T, 2 * S::bytes>(at, lane);
                     if (lane == 0) {
                         dirty[slot] = found;
                         arrive(searched + slot);
@@ -1060,17 +1069,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                 row_off2 = pack2(-from[0], -from[0]);
                 row_mean2 = pack2(-from[kStatisticRows], -from[kStatisticRows]);
             }
-            for (uint32_t u = u0 + ((u0 ^ h) & 1); u < u0 + piece.n; u += 2) {
+            int tile = after(0, (u0 ^ h) & 1);
+            for (uint32_t u = u0 + ((u0 ^ h) & 1); u < u0 + piece.n; u += 2, tile = after(tile, 2)) {
                 const uint32_t parity = u >> 1 & 1, slot = u % S::stages;
-                const int tile = tile_in_turn(u - u0), from = seen_low - tile * S::other, to = seen_high - tile * S::other;
+                const int from = seen_low - tile * S::other, to = seen_high - tile * S::other;
                 const bool masked = !seen_whole(tile);
                 const float4* const statistics = reinterpret_cast<const float4*>(ring + slot * S::stage_bytes + 2 * S::bytes);
-                ok = __all_sync(0xffffffffu, (!KEYS || wait_in_line(full + slot, u / S::stages & 1, failed)) && wait_in_line(scored + h, parity, failed));
-                if (!ok) break;
+                const bool loaded = !KEYS || mbar_test(full + slot, u / S::stages & 1), there_yet = mbar_test(scored + h, parity);          // side by side: each takes a hundred clocks
+                ok = __all_sync(0xffffffffu, loaded && there_yet);
+                if (!ok) {
+                    ok = __all_sync(0xffffffffu, wait_in_line(full + slot, u / S::stages & 1, failed) && wait_in_line(scored + h, parity, failed));
+                    if (!ok) break;
+                }
                 // What this tile's weights and score gradients write over is in the sums: the last tile's, or of q, whose score gradients have two places, the last but one's.  Asked where nothing waits for it.
                 const uint32_t turn = u >> 1, over = turn - (KEYS ? 1 : 2);
                 uint64_t* const old = added + 2 * h + (over & 1);
-                const bool free = turn < (KEYS ? 1 : 2) || mbar_test(old, over >> 1 & 1);
+                const bool free = turn < (KEYS ? 1 : 2) || __all_sync(0xffffffffu, mbar_test(old, over >> 1 & 1));
                 tmem_fence_after();
                 uint32_t p[64];
                 tmem_begin32(score, p);
