@@ -2,6 +2,8 @@
 // values, widths that are no multiple of 8, rows that do not begin on 16 bytes.
 #include "attention.cuh"
 
+#include <algorithm>
+
 namespace htgs {
 
 namespace {
@@ -85,17 +87,20 @@ template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention
     }
 }
 
-// Statistics of the rows of a tile of 128 and a head.  Bound by HBM: reads the output and its gradient once.  LANES lanes have a row, N values of it at a time each.
+// Statistics of the rows of a tile of 128 and some heads.  Bound by HBM: reads the output and its gradient once.  LANES lanes have a row, N values of it at a time each.
 template <typename T, int N, int LANES> __global__ void __launch_bounds__(kLanesThreads) statistics_kernel(const HtgsAttention a, const T* out, const float* sums, const AttentionBackward b, float* statistics,
-                                                                                                          uint32_t* largest) {
+                                                                                                          uint32_t* largest, int heads_of_block) {
     grid_dependency();
-    const int lane = threadIdx.x % LANES, head = int(blockIdx.x % a.heads), group = a.heads / a.key_heads, key_head = head / group;
-    const SequenceTile t = find_tile<kStatisticRows>(a, int(blockIdx.x / a.heads));
+    const int lane = threadIdx.x % LANES, group = a.heads / a.key_heads, blocks = (a.heads + heads_of_block - 1) / heads_of_block;
+    const int first_head = int(blockIdx.x % blocks) * heads_of_block, last_head = min(first_head + heads_of_block, a.heads);
+    const SequenceTile t = find_tile<kStatisticRows>(a, int(blockIdx.x / blocks));
     if (t.first >= t.end) return;
-    float* to = statistics + (head * b.statistics_rows + statistic_base(a, t) + (t.first - t.begin)) * 2;
+    const int64_t base = statistic_base(a, t) + (t.first - t.begin);
     float grads = 0.0f, values = 0.0f;
-    #pragma unroll 2
-    for (int r = threadIdx.x / LANES; r < kStatisticRows; r += kLanesThreads / LANES) {
+    const int count = (last_head - first_head) * kStatisticRows;
+    #pragma unroll 4
+    for (int x = threadIdx.x / LANES; x < count; x += kLanesThreads / LANES) {           // rows of a head, then of the next
+        const int head = first_head + x / kStatisticRows, r = x % kStatisticRows;
         const int64_t i = t.first + r;
         const bool there = i < t.end && !t.outside;
         float mean = 0.0f, grad = 0.0f, value = 0.0f;
@@ -109,7 +114,7 @@ template <typename T, int N, int LANES> __global__ void __launch_bounds__(kLanes
                 for (int k = 0; k < N; ++k) { mean = fmaf(x[k], y[k], mean); grad = fmaf(y[k], y[k], grad); }
             }
             if (largest && head % group == 0) {
-                const T* v = static_cast<const T*>(a.v) + i * a.v_stride + key_head * a.v_head_stride;
+                const T* v = static_cast<const T*>(a.v) + i * a.v_stride + head / group * a.v_head_stride;
                 for (int c = lane * N; c < a.width; c += LANES * N) {
                     float x[N];
                     load_floats<T, N>(v + c, x);
@@ -124,6 +129,7 @@ template <typename T, int N, int LANES> __global__ void __launch_bounds__(kLanes
             if (largest) { grad += __shfl_xor_sync(0xffffffffu, grad, d); value += __shfl_xor_sync(0xffffffffu, value, d); }
         }
         if (lane == 0) {
+            float* to = statistics + (head * b.statistics_rows + base) * 2;
             to[r] = there ? sums[head * a.rows + i] : 0.0f;
             to[kStatisticRows + r] = mean;
         }
@@ -248,8 +254,11 @@ template <typename T> int backward_lanes(const HtgsAttention& a, const Attention
 }
 template <typename T, int N, int LANES>
 int launch_statistics(const HtgsAttention& a, const void* out, const float* sums, const AttentionBackward& b, float* statistics, uint32_t* largest, cudaStream_t stream) {
-    const cudaError_t err = launch_after(statistics_kernel<T, N, LANES>, dim3(unsigned(sequence_tiles(a, kStatisticRows) * a.heads)), kLanesThreads, 0, stream, a, static_cast<const T*>(out), sums, b,
-                                         statistics, largest);
+    // Some heads to a block, as long as there are eight blocks for each SM: the way in costs as much as a head (100003 rows, 8 heads of 32 in 7 sequences: 41 us with one head to a block).
+    const int64_t tiles = sequence_tiles(a, kStatisticRows);
+    const int heads = int(std::max<int64_t>(1, std::min<int64_t>(a.heads, tiles * a.heads / (148 * 8))));
+    const cudaError_t err = launch_after(statistics_kernel<T, N, LANES>, dim3(unsigned(tiles * ((a.heads + heads - 1) / heads))), kLanesThreads, 0, stream, a, static_cast<const T*>(out), sums, b,
+                                         statistics, largest, heads);
     return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 template <typename T> int backward_typed(const HtgsAttention& a, const void* out, const float* sums, AttentionBackward b, float* statistics, uint32_t* largest, cudaStream_t stream) {

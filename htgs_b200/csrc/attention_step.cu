@@ -98,11 +98,12 @@ template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes
 
 // ---- 16-bit heads on 16 bytes: matrix instructions of a warp ---------------------------------------------------------------------------
 //
-// A block has the query heads of a key head, up to 16 rows of a matrix, and a split of the sequence.  Each of its warps brings 32 keys and values at a time into places of its own in shared memory, one or two
+// A block has the query heads of a key head, up to 16 rows of a matrix, and a split of the sequence.  Each of its warps brings 16 or 32 keys and values at a time into places of its own in shared memory, one or two
 // sets on their way while one is used, and goes its own way until the end: no barrier of the block.  Products are m16n8k16; the arithmetic is a tenth of what they could do, so rows that no head fills cost nothing.
 // (tcgen05 takes 128 rows at least, of which 4 to 16 would be used, and its accumulators would have to come out of tensor memory for every 32 keys.)
 
-constexpr int kTileWarps = 4, kTileKeys = 32, kTileStages = 3, kTileHeads = 16;
+constexpr int kTileWarps = 4, kTileStages = 3, kTileHeads = 16, kMostClusters = 8;
+template <int W> constexpr int kKeysOfSet = W == 128 ? 16 : 32;          // two blocks then fit an SM, and one's way in and out is the other's time
 // Weights are at most 1: fp16 ones carry 2^15, so that one of 2^-29 is a normal number.
 template <typename T> constexpr float kStepLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 
@@ -125,9 +126,10 @@ template <typename T> __device__ __forceinline__ void multiply_add(float (&d)[4]
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T, int W>        // W: the width rounded up to 32, 64 or 128
+// W: the width rounded up to 32, 64 or 128.  CLUSTER: the splits of a sequence are a cluster of blocks, which join them through shared memory.
+template <typename T, int W, bool CLUSTER>
 __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsAttentionStep a, T* out, float* parts, int splits, int chunks) {
-    constexpr int kSteps = W / 16, kPieces = W / 8, kCopies = kTileKeys * kPieces / 32, kRowsOfCopy = 32 / kPieces, kSetBytes = kTileKeys * W * 2;
+    constexpr int kTileKeys = kKeysOfSet<W>, kSteps = W / 16, kPieces = W / 8, kCopies = kTileKeys * kPieces / 32, kRowsOfCopy = 32 / kPieces, kSetBytes = kTileKeys * W * 2;
     extern __shared__ __align__(16) unsigned char shared[];
     grid_dependency();
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsA
         const T* const new_key = static_cast<const T*>(a.k) + b * a.k_stride + key_head * a.k_head_stride + piece * 8;
         const T* const new_value = static_cast<const T*>(a.v) + b * a.v_stride + key_head * a.v_head_stride + piece * 8;
         const bool mine_there = piece * 8 < a.width;
-        const auto begin = [&](int first, int stage) {          // rows first + [0, 32); what lies behind the split's last row is zero
+        const auto begin = [&](int first, int stage) {          // rows of a set; what lies behind the split's last row is zero
             const uint32_t to = mine_at + stage * 2 * kSetBytes;
             if (mine_there && first < rows.y) {
                 #pragma unroll
@@ -260,6 +262,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsA
     constexpr int kPitch = W + 4;
     float2* const tops = reinterpret_cast<float2*>(shared);
     float* const outputs = reinterpret_cast<float*>(tops + kTileWarps * kTileHeads);
+    float* const joined = outputs + kTileWarps * kTileHeads * kPitch;
     __syncthreads();
     #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -288,7 +291,11 @@ __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsA
             for (int k = 0; k < 8; ++k) total[k] = fmaf(v[k], factor, total[k]);
         }
         const int64_t at = int64_t(b) * a.heads + first_head + head;
-        if (splits > 1) {
+        if (CLUSTER) {
+            *reinterpret_cast<float4*>(joined + head * kPitch + c) = make_float4(total[0], total[1], total[2], total[3]);
+            *reinterpret_cast<float4*>(joined + head * kPitch + c + 4) = make_float4(total[4], total[5], total[6], total[7]);
+            if (c == 0) *reinterpret_cast<float4*>(joined + head * kPitch + W) = make_float4(largest, all, 0.0f, 0.0f);
+        } else if (splits > 1) {
             float* to = parts + (at * splits + split) * part_floats(a.width);
             *reinterpret_cast<float4*>(to + 4 + c) = make_float4(total[0], total[1], total[2], total[3]);
             *reinterpret_cast<float4*>(to + 8 + c) = make_float4(total[4], total[5], total[6], total[7]);
@@ -299,35 +306,82 @@ __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsA
             store_floats<T, 8>(out + at * a.width + c, total);
         }
     }
+    if constexpr (CLUSTER) {
+        cluster_barrier();
+        const uint32_t joined_at = smem_u32(joined);
+        for (int i = split * kTileWarps * 32 + int(threadIdx.x); i < heads * (a.width / 4); i += splits * kTileWarps * 32) {
+            const int head = i / (a.width / 4), c = i % (a.width / 4) * 4;
+            float4 tops[kMostClusters], v[kMostClusters];
+            float largest = -infinity(), all = 0.0f;
+            #pragma unroll
+            for (int k = 0; k < kMostClusters; ++k) {
+                if (k >= splits) break;
+                tops[k] = peer_float4(joined_at + uint32_t(head * kPitch + W) * 4, k);
+                v[k] = peer_float4(joined_at + uint32_t(head * kPitch + c) * 4, k);
+                largest = fmaxf(largest, tops[k].x);
+            }
+            const float base = largest == -infinity() ? 0.0f : largest;
+            float total[4] = {};
+            #pragma unroll
+            for (int k = 0; k < kMostClusters; ++k) {
+                if (k >= splits) break;
+                const float factor = exp2_approx(tops[k].x - base);
+                all = fmaf(tops[k].y, factor, all);
+                total[0] = fmaf(v[k].x, factor, total[0]);
+                total[1] = fmaf(v[k].y, factor, total[1]);
+                total[2] = fmaf(v[k].z, factor, total[2]);
+                total[3] = fmaf(v[k].w, factor, total[3]);
+            }
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) total[k] = r.left_out ? 0.0f : any ? total[k] / all : __uint_as_float(0x7fffffffu);
+            store_floats<T, 4>(out + (int64_t(b) * a.heads + first_head + head) * a.width + c, total);
+        }
+        cluster_barrier();           // no block's shared memory goes before the others have read it
+    }
 }
 
-// The splits of a head, joined.
-template <typename T> __global__ void __launch_bounds__(kMostStepWidth) step_join_kernel(const HtgsAttentionStep a, T* out, const float* parts, int splits) {
+// The splits of a head, joined: a warp's lanes have four columns each and its splits are every eighth; then the warps' sums.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+template <typename T> __global__ void __launch_bounds__(kJoinThreads) step_join_kernel(const HtgsAttentionStep a, T* out, const float* parts, int splits) {
     __shared__ float factors[kMostSplits];
+    __shared__ float4 sums[kJoinWarps][32];
+    __shared__ float warps[2][kJoinWarps];
     grid_dependency();
     const int64_t at = blockIdx.x;
-    const int pitch = part_floats(a.width), lane = threadIdx.x & 31;
-    const StepRows r = rows_of(a, int(at / a.heads));
+    const int pitch = part_floats(a.width), lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const float* mine = parts + at * splits * pitch;
-    if (threadIdx.x < 32) {
-        float most = -infinity(), sum = 0.0f;
-        for (int s = lane; s < splits; s += 32) most = fmaxf(most, mine[s * pitch]);
-        most = lanes_max<32>(most);
-        const float base = most == -infinity() ? 0.0f : most;
-        for (int s = lane; s < splits; s += 32) {
-            const float2 part = *reinterpret_cast<const float2*>(mine + s * pitch);
-            factors[s] = exp2_approx(part.x - base);
-            sum = fmaf(part.y, factors[s], sum);
+    static_assert(kMostSplits <= kJoinThreads, "a split for each thread");
+    const float2 top = int(threadIdx.x) < splits ? *reinterpret_cast<const float2*>(mine + int64_t(threadIdx.x) * pitch) : make_float2(-infinity(), 0.0f);
+    float most = lanes_max<32>(top.x);
+    if (lane == 0) warps[0][warp] = most;
+    __syncthreads();
+    #pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, warps[0][w]);
+    const float factor = exp2_approx(top.x - (most == -infinity() ? 0.0f : most)), part = warp_sum(top.y * factor);
+    if (int(threadIdx.x) < splits) factors[threadIdx.x] = factor;
+    if (lane == 0) warps[1][warp] = part;
+    __syncthreads();
+    float sum = 0.0f;
+    #pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) sum += warps[1][w];
+    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (lane * 4 < a.width) {
+        #pragma unroll 8
+        for (int s = warp; s < splits; s += kJoinWarps) {
+            const float4 v = *reinterpret_cast<const float4*>(mine + int64_t(s) * pitch + 4 + lane * 4);
+            const float f = factors[s];
+            total.x = fmaf(v.x, f, total.x); total.y = fmaf(v.y, f, total.y); total.z = fmaf(v.z, f, total.z); total.w = fmaf(v.w, f, total.w);
         }
-        sum = warp_sum(sum);
-        for (int s = lane; s < splits; s += 32) factors[s] /= sum;
     }
+    sums[warp][lane] = total;
     __syncthreads();
     const int c = threadIdx.x;
     if (c >= a.width) return;
-    float total = 0.0f;
-    for (int s = 0; s < splits; ++s) total = fmaf(mine[s * pitch + 4 + c], factors[s], total);
-    out[at * a.width + c] = from_float<T>(r.left_out ? 0.0f : r.full ? __uint_as_float(0x7fffffffu) : total);
+    float all = 0.0f;
+    #pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) all += reinterpret_cast<const float*>(sums[w])[c];
+    const StepRows r = rows_of(a, int(at / a.heads));
+    out[at * a.width + c] = from_float<T>(r.left_out ? 0.0f : r.full ? __uint_as_float(0x7fffffffu) : all / sum);
 }
 
 const char* wrong(const HtgsAttentionStep* a) {
@@ -351,28 +405,46 @@ bool step_aligned(const HtgsAttentionStep& a) {
            ok(a.values, a.batch, a.values_stride, a.key_heads, a.values_head_stride) && (a.capacity <= 1 || a.values_row_stride % 8 == 0);
 }
 
-struct StepPlan { bool tiles; int64_t blocks; int chunks, splits; };       // blocks: of one split
-// Splits of a sequence: the rounds of all places for a block, by the rows of a split and what a block costs beside them, about as much as 128 rows.
+struct StepPlan { bool tiles; int64_t blocks; int chunks, splits; bool cluster; };       // blocks: of one split
+// Splits of a sequence.  A block costs about as much as 128 rows beside its own, or 256 while it takes from others.  One sequence: the rounds of all places for a block, by a block's rows.  Several, whose lengths differ: blocks come and go, so all their rows (five
+// eighths of the capacity, say) spread over the places, and then the last block's.  Up to eight splits can be a cluster, whose join costs about 128 rows' time; more are joined by a kernel of its own, about 512.
 StepPlan plan_of(const HtgsAttentionStep& a) {
-    StepPlan p{step_aligned(a), 0, 1, 1};
+    StepPlan p{step_aligned(a), 0, 1, 1, false};
     const int group = a.heads / a.key_heads;
     if (p.tiles) p.chunks = (group + kTileHeads - 1) / kTileHeads;
     p.blocks = int64_t(a.batch) * (p.tiles ? a.key_heads * p.chunks : a.heads);
-    const int64_t rows = (a.window >= 0 && a.window < a.capacity ? a.window + 1 : a.capacity) + 1, slots = 148 * (p.tiles ? (a.width <= 32 ? 4 : a.width <= 64 ? 2 : 1) : 8);
+    const int64_t rows = (a.window >= 0 && a.window < a.capacity ? a.window + 1 : a.capacity) + 1, slots = 148 * (p.tiles ? (a.width <= 32 ? 4 : 2) : 8);
     int64_t best = INT64_MAX;
     for (int splits = 1; splits <= kMostSplits && (splits == 1 || rows >= splits * 128); ++splits) {
-        const int64_t cost = (p.blocks * splits + slots - 1) / slots * (rows / splits + 128) + (splits > 1 ? 128 : 0);
-        if (cost < best) { best = cost; p.splits = splits; }
+        const bool cluster = p.tiles && splits > 1 && splits <= kMostClusters;
+        const int64_t time = a.batch == 1 ? (p.blocks * splits + slots - 1) / slots * (rows / splits + 128) : p.blocks * (rows * 5 / 8 + 256 * splits) / slots + rows / splits;
+        const int64_t cost = time + (splits == 1 ? 0 : cluster ? 128 : 512);
+        if (cost < best) { best = cost; p.splits = splits; p.cluster = cluster; }
     }
     return p;
 }
 
-template <typename T, int W> cudaError_t launch_step(const HtgsAttentionStep& a, T* out, float* parts, const StepPlan& plan, cudaStream_t stream) {
-    constexpr int smem = kTileWarps * kTileStages * 2 * kTileKeys * W * 2;
-    static_assert(kTileWarps * kTileHeads * (8 + (W + 4) * 4) <= smem, "the warps' parts fit the places of keys and values");
+template <typename T, int W, bool CLUSTER> cudaError_t launch_step(const HtgsAttentionStep& a, T* out, float* parts, const StepPlan& plan, cudaStream_t stream) {
+    constexpr int smem = kTileWarps * kTileStages * 2 * kKeysOfSet<W> * W * 2;
+    static_assert(kTileWarps * kTileHeads * (8 + (W + 4) * 4) + kTileHeads * (W + 4) * 4 <= smem, "the warps' parts and the block's fit the places of keys and values");
     static PerDeviceOnce once;
-    const cudaError_t err = once.run([] { return cudaFuncSetAttribute(step_tiles_kernel<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-    return err != cudaSuccess ? err : launch_after(step_tiles_kernel<T, W>, dim3(unsigned(plan.blocks * plan.splits)), kTileWarps * 32, smem, stream, a, out, parts, plan.splits, plan.chunks);
+    const cudaError_t err = once.run([] { return cudaFuncSetAttribute(step_tiles_kernel<T, W, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    if (err != cudaSuccess) return err;
+    const dim3 grid(unsigned(plan.blocks * plan.splits));
+    if (!CLUSTER) return launch_after(step_tiles_kernel<T, W, CLUSTER>, grid, kTileWarps * 32, smem, stream, a, out, parts, plan.splits, plan.chunks);
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = unsigned(plan.splits); attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid; config.blockDim = kTileWarps * 32; config.dynamicSmemBytes = smem; config.stream = stream;
+    config.attrs = attributes; config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, step_tiles_kernel<T, W, CLUSTER>, a, out, parts, plan.splits, plan.chunks);
+}
+template <typename T, bool CLUSTER> cudaError_t launch_step(const HtgsAttentionStep& a, T* out, float* parts, const StepPlan& plan, cudaStream_t stream) {
+    return a.width <= 32 ? launch_step<T, 32, CLUSTER>(a, out, parts, plan, stream) : a.width <= 64 ? launch_step<T, 64, CLUSTER>(a, out, parts, plan, stream)
+                                                                                    : launch_step<T, 128, CLUSTER>(a, out, parts, plan, stream);
 }
 
 template <typename T> int step_typed(const HtgsAttentionStep& a, void* to, float* parts, cudaStream_t stream) {
@@ -381,13 +453,13 @@ template <typename T> int step_typed(const HtgsAttentionStep& a, void* to, float
     cudaError_t err = cudaSuccess;
     bool done = false;
     if constexpr (sizeof(T) == 2) {
-        if (plan.tiles && aligned(out, 16)) {
-            err = a.width <= 32 ? launch_step<T, 32>(a, out, parts, plan, stream) : a.width <= 64 ? launch_step<T, 64>(a, out, parts, plan, stream) : launch_step<T, 128>(a, out, parts, plan, stream);
+        if (plan.tiles) {
+            err = plan.cluster ? launch_step<T, true>(a, out, parts, plan, stream) : launch_step<T, false>(a, out, parts, plan, stream);
             done = true;
         }
     }
     if (!done) err = launch_after(step_lanes_kernel<T>, dim3(unsigned(int64_t(a.batch) * a.heads * plan.splits)), kStepThreads, 0, stream, a, out, parts, plan.splits);
-    if (err == cudaSuccess && plan.splits > 1) err = launch_after(step_join_kernel<T>, dim3(unsigned(int64_t(a.batch) * a.heads)), kMostStepWidth, 0, stream, a, out, parts, plan.splits);
+    if (err == cudaSuccess && plan.splits > 1 && !plan.cluster) err = launch_after(step_join_kernel<T>, dim3(unsigned(int64_t(a.batch) * a.heads)), kJoinThreads, 0, stream, a, out, parts, plan.splits);
     return err == cudaSuccess ? sequence_status("htgs_attention_step") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
@@ -400,15 +472,15 @@ extern "C" {
 size_t htgs_attention_step_workspace_bytes(const HtgsAttentionStep* step) {
     using namespace htgs;
     if (wrong(step) || step->batch == 0) return 0;
-    const int splits = plan_of(*step).splits;
-    return splits == 1 ? 0 : size_t(step->batch) * step->heads * splits * part_floats(step->width) * sizeof(float);
+    const StepPlan plan = plan_of(*step);
+    return plan.splits == 1 || plan.cluster ? 0 : size_t(step->batch) * step->heads * plan.splits * part_floats(step->width) * sizeof(float);
 }
 
 int htgs_attention_step(const HtgsAttentionStep* step, void* out, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace htgs;
     if (const char* message = wrong(step)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
     if (step->batch == 0) return HTGS_OK;
-    if (!out) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_attention_step: out must not be null");
+    if (!out || !aligned(out, 16)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, "htgs_attention_step: out must not be null, and begin on 16 bytes");
     const size_t size = htgs_attention_step_workspace_bytes(step);
     if (size && (!workspace || !aligned(workspace, 16) || workspace_bytes < size)) return sequence_fail(HTGS_ERR_WORKSPACE_TOO_SMALL, "htgs_attention_step: the workspace is too small or not on 16 bytes");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -12,7 +12,7 @@ namespace htgs {
 
 namespace {
 
-constexpr int kRotaryThreads = 256, kMostPairs = 128, kRotaryRows = 8;
+constexpr int kRotaryThreads = 256, kMostPairs = 128, kMostRows = 30, kAhead = 2;
 
 struct RotaryArgs {
     HtgsRotary r;
@@ -20,89 +20,122 @@ struct RotaryArgs {
     uint8_t axis[kMostPairs];
 };
 
-// N pairs of a head: the first values at `a`, the second ones at `b`, or all of them at `a`, neighbours.
-template <typename T, int N, bool INTERLEAVED> __device__ __forceinline__ void turn(const T* x, T* y, int second, const float2* angles) {
-    float a[N], b[N];
-    if constexpr (INTERLEAVED) {
-        float both[2 * N];
-        if constexpr (N * 2 * sizeof(T) <= 16) load_floats<T, 2 * N>(x, both);
+// N pairs of a head: as they lie in memory, and as first and second values.
+template <typename T, int N, bool INTERLEAVED> struct Pairs {
+    static constexpr bool whole = INTERLEAVED && 2 * N * sizeof(T) <= 16;           // in one piece
+    Pack<T, whole ? 2 * N : N> one, two;
+    __device__ __forceinline__ void load(const T* x, int second) {
+        one = *reinterpret_cast<const decltype(one)*>(x);
+        if (!whole) two = *reinterpret_cast<const decltype(two)*>(x + (INTERLEAVED ? N : second));
+    }
+    // cosines of a row from the first pair on, then, `pairs` further each time, sines and minus sines
+    __device__ __forceinline__ void turn(const float* angles, int pairs, T* y, int second) const {
+        float values[2 * N];
+        if constexpr (whole) to_floats<T, 2 * N>(one, values);
         else {
-            float low[N], high[N];
-            load_floats<T, N>(x, low);
-            load_floats<T, N>(x + N, high);
-            #pragma unroll
-            for (int i = 0; i < N; ++i) { both[i] = low[i]; both[N + i] = high[i]; }
+            to_floats<T, N>(one, *reinterpret_cast<float (*)[N]>(values));
+            to_floats<T, N>(two, *reinterpret_cast<float (*)[N]>(values + N));
         }
+        float c[N], d[N], m[N];
+        load_floats<float, N>(angles, c);
+        load_floats<float, N>(angles + pairs, d);
+        load_floats<float, N>(angles + 2 * pairs, m);
+        constexpr int kStep = N == 1 ? 1 : 2;
         #pragma unroll
-        for (int i = 0; i < N; ++i) { a[i] = both[2 * i]; b[i] = both[2 * i + 1]; }
-    } else {
-        load_floats<T, N>(x, a);
-        load_floats<T, N>(x + second, b);
-    }
-    #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float2 w = angles[i];
-        const float u = a[i] * w.x - b[i] * w.y, v = a[i] * w.y + b[i] * w.x;
-        a[i] = u;
-        b[i] = v;
-    }
-    if constexpr (INTERLEAVED) {
-        float both[2 * N];
-        #pragma unroll
-        for (int i = 0; i < N; ++i) { both[2 * i] = a[i]; both[2 * i + 1] = b[i]; }
-        if constexpr (N * 2 * sizeof(T) <= 16) store_floats<T, 2 * N>(y, both);
+        for (int i = 0; i < N; i += kStep) {
+            const int a0 = INTERLEAVED ? 2 * i : i, b0 = INTERLEAVED ? 2 * i + 1 : N + i, a1 = INTERLEAVED ? 2 * i + 2 : i + 1, b1 = INTERLEAVED ? 2 * i + 3 : N + i + 1;
+            if constexpr (N == 1) {
+                const float a = values[a0], b = values[b0];
+                values[a0] = fmaf(b, m[i], a * c[i]);
+                values[b0] = fmaf(a, d[i], b * c[i]);
+            } else {
+                const f32x2 a = pack2(values[a0], values[a1]), b = pack2(values[b0], values[b1]), cosine = pack2(c[i], c[i + 1]);
+                const float2 u = unpack2(fma2(b, pack2(m[i], m[i + 1]), mul2(a, cosine))), v = unpack2(fma2(a, pack2(d[i], d[i + 1]), mul2(b, cosine)));
+                values[a0] = u.x; values[a1] = u.y;
+                values[b0] = v.x; values[b1] = v.y;
+            }
+        }
+        if constexpr (whole) store_floats<T, 2 * N>(y, values);
         else {
-            float low[N], high[N];
-            #pragma unroll
-            for (int i = 0; i < N; ++i) { low[i] = both[i]; high[i] = both[N + i]; }
-            store_floats<T, N>(y, low);
-            store_floats<T, N>(y + N, high);
+            store_floats<T, N>(y, *reinterpret_cast<const float (*)[N]>(values));
+            store_floats<T, N>(y + (INTERLEAVED ? N : second), *reinterpret_cast<const float (*)[N]>(values + N));
         }
-    } else {
-        store_floats<T, N>(y, a);
-        store_floats<T, N>(y + second, b);
     }
+};
+
+// Sine and cosine of z, |z| at most pi / 4: odd and even polynomials of least maximal error for what lies behind z and 1 - z^2 / 2 (found by linear programming), 2^-24 off at most in 32 bits.
+__device__ __forceinline__ void sine_cosine(float z, float& sine, float& cosine) {
+    const float w = z * z;
+    sine = fmaf(z * w, fmaf(fmaf(-0.0001951528392964974f, w, 0.00833216030150652f), w, -0.16666655242443085f), z);
+    cosine = fmaf(fmaf(fmaf(fmaf(2.4438451873720624e-05f, w, -0.001388736767694354f), w, 0.04166664555668831f), w, -0.5f), w, 1.0f);
 }
 
-// A block has a few rows: their cosines and sines first, which all heads share, then all heads of both tensors.
-template <typename T, int N, bool INTERLEAVED> __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs args) {
-    extern __shared__ float2 angles[];                   // [rows][pairs]
+// A block has a few rows: their cosines and sines, which all heads share, while the first values are on their way; then all heads of both tensors.  In 64 bits only what multiplies and adds: rounding is by a large
+// number, whose low bits then are the quarter, and positions are converted once a row, since conversions and roundings are made by a unit that takes longer than all the rest.
+template <typename T, int N, bool INTERLEAVED> __global__ void __launch_bounds__(kRotaryThreads, 5) rotary_kernel(const __grid_constant__ RotaryArgs args, const int rows_of_block) {
+    extern __shared__ __align__(16) float angles[];       // [rows][3][pairs], a row's on 16 bytes
+    __shared__ double positions[kMostRows * 4], turns[kMostPairs];
+    __shared__ uint8_t axis[kMostPairs];
     grid_dependency();
     const HtgsRotary& r = args.r;
-    const int pairs = r.width / 2, heads = r.heads[0] + r.heads[1], chunks = pairs / N;
-    const int64_t first = int64_t(blockIdx.x) * kRotaryRows;
-    const int rows = int(min(int64_t(kRotaryRows), r.rows - first));
-    for (int i = threadIdx.x; i < rows * pairs; i += kRotaryThreads) {
-        const int row = i / pairs, pair = i - row * pairs;
-        const int64_t at = (first + row) * r.positions_stride + args.axis[pair];
-        const double position = r.positions_type == 0 ? double(static_cast<const float*>(r.positions)[at]) : double(static_cast<const int32_t*>(r.positions)[at]);
-        const double t = position * args.turns[pair], whole = t - rint(t), quarter = rint(4.0 * whole);       // whole: -1/2 to 1/2
-        float sine, cosine;
-        sincospif(float(2.0 * (whole - 0.25 * quarter)), &sine, &cosine);
-        const int q = int(quarter) & 3;
-        float2 w = q & 1 ? make_float2(-sine, cosine) : make_float2(cosine, sine);
-        if (q & 2) w = make_float2(-w.x, -w.y);
-        if (r.inverse) w.y = -w.y;
-        angles[i] = w;
+    const int pairs = r.width / 2, heads = r.heads[0] + r.heads[1], chunks = pairs / N, pitch = (3 * pairs + 3) / 4 * 4, of_row = heads * chunks;
+    const int64_t first = int64_t(blockIdx.x) * rows_of_block;
+    const int rows = int(min(int64_t(rows_of_block), r.rows - first)), count = rows * of_row;
+    struct Place { const T* x; T* y; int angle; };
+    const auto place = [&](int i) {
+        const int row = i / of_row, rest = i - row * of_row, all = rest / chunks, chunk = rest - all * chunks, which = all >= r.heads[0], head = all - (which ? r.heads[0] : 0);
+        const int at = INTERLEAVED ? 2 * N * chunk : N * chunk;
+        return Place{static_cast<const T*>(r.x[which]) + (first + row) * r.x_stride[which] + head * r.x_head_stride[which] + at,
+                     static_cast<T*>(r.y[which]) + ((first + row) * r.heads[which] + head) * r.width + at, row * pitch + N * chunk};
+    };
+    for (int i = threadIdx.x; i < rows * r.axes; i += kRotaryThreads) {
+        const int row = i / r.axes;
+        const int64_t at = (first + row) * r.positions_stride + (i - row * r.axes);
+        positions[i] = r.positions_type == 0 ? double(static_cast<const float*>(r.positions)[at]) : double(static_cast<const int32_t*>(r.positions)[at]);
+    }
+    for (int i = threadIdx.x; i < pairs; i += kRotaryThreads) { turns[i] = args.turns[i]; axis[i] = args.axis[i]; }         // arguments are read one address at a time (21 of 70 us)
+    Pairs<T, N, INTERLEAVED> values[kAhead];
+    Place places[kAhead];
+    #pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        const int i = int(threadIdx.x) + k * kRotaryThreads;
+        places[k] = place(i < count ? i : 0);
+        if (i < count) values[k].load(places[k].x, pairs);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * heads * chunks; i += kRotaryThreads) {
-        const int chunk = i % chunks, rest = i / chunks, row = rest / heads;
-        int head = rest - row * heads;
-        const int which = head >= r.heads[0];
-        if (which) head -= r.heads[0];
-        const int at = INTERLEAVED ? 2 * N * chunk : N * chunk;
-        const T* x = static_cast<const T*>(r.x[which]) + (first + row) * r.x_stride[which] + head * r.x_head_stride[which] + at;
-        T* y = static_cast<T*>(r.y[which]) + ((first + row) * r.heads[which] + head) * r.width + at;
-        turn<T, N, INTERLEAVED>(x, y, pairs, angles + row * pairs + N * chunk);
+    for (int i = threadIdx.x; i < rows * pairs; i += kRotaryThreads) {
+        const int row = i / pairs, pair = i - row * pairs;
+        constexpr double kWhole = 6755399441055744.0;          // 1.5 * 2^52
+        const double t = positions[row * r.axes + axis[pair]] * turns[pair], whole = t - ((t + kWhole) - kWhole), quarter = fma(4.0, whole, kWhole);       // whole: -1/2 to 1/2
+        float sine, cosine;
+        sine_cosine(float(6.283185307179586477 * fma(-0.25, quarter - kWhole, whole)), sine, cosine);
+        const int q = __double2loint(quarter);
+        float x = q & 1 ? -sine : cosine, y = q & 1 ? cosine : sine;
+        if (q & 2) { x = -x; y = -y; }
+        if (r.inverse) y = -y;
+        float* const to = angles + row * pitch + pair;
+        to[0] = x; to[pairs] = y; to[2 * pairs] = -y;
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+        if (int(threadIdx.x) + k * kRotaryThreads < count) values[k].turn(angles + places[k].angle, pairs, places[k].y, pairs);
+    for (int i = threadIdx.x + kAhead * kRotaryThreads; i < count; i += kRotaryThreads) {           // one row of many heads
+        const Place p = place(i);
+        Pairs<T, N, INTERLEAVED> v;
+        v.load(p.x, pairs);
+        v.turn(angles + p.angle, pairs, p.y, pairs);
     }
 }
 
 template <typename T, int N> int launch_rotary(const RotaryArgs& args, cudaStream_t stream) {
-    const dim3 grid(unsigned((args.r.rows + kRotaryRows - 1) / kRotaryRows));
-    const size_t smem = size_t(kRotaryRows) * (args.r.width / 2) * sizeof(float2);
-    const cudaError_t err = args.r.interleaved ? launch_after(rotary_kernel<T, N, true>, grid, kRotaryThreads, smem, stream, args)
-                                               : launch_after(rotary_kernel<T, N, false>, grid, kRotaryThreads, smem, stream, args);
+    // Rows whose values the threads of a block load at once.
+    const int items = (args.r.heads[0] + args.r.heads[1]) * (args.r.width / 2 / N), most = kAhead * kRotaryThreads / items, rows = most < 1 ? 1 : most > kMostRows ? kMostRows : most;
+    const dim3 grid(unsigned((args.r.rows + rows - 1) / rows));
+    const size_t smem = size_t(rows) * ((3 * (args.r.width / 2) + 3) / 4 * 4) * sizeof(float);
+    static_assert(kMostRows * 3 * kMostPairs * 4 <= 47 * 1024, "shared memory");
+    const cudaError_t err = args.r.interleaved ? launch_after(rotary_kernel<T, N, true>, grid, kRotaryThreads, smem, stream, args, rows)
+                                               : launch_after(rotary_kernel<T, N, false>, grid, kRotaryThreads, smem, stream, args, rows);
     return err == cudaSuccess ? sequence_status("htgs_rotary") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 

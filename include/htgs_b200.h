@@ -574,7 +574,7 @@ unsigned int* htgs_attention_error_word(int32_t device);
 
 /*
  * One more row for each of `batch` sequences: k and v [batch, key_heads, width] become row lengths[b] of the caches keys and values [batch, capacity, key_heads, width] (in
- * place), and out [batch, heads, width] (dense) is the attention of q over rows max(0, lengths[b] - window) to lengths[b] (from row 0 if window < 0).  lengths (device memory)
+ * place), and out [batch, heads, width] (dense, on 16 bytes) is the attention of q over rows max(0, lengths[b] - window) to lengths[b] (from row 0 if window < 0).  lengths (device memory)
  * stays as it is.  A sequence with lengths[b] < 0 is left out: zeros, and its caches stay; one whose cache is full (lengths[b] >= capacity) gets NaN, and its caches stay.
  * Strides in elements: from sequence to sequence, from row to row (caches), from head to head.  workspace as the size function says, 16-byte aligned.
  */
