@@ -98,11 +98,11 @@ template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes
 
 // ---- 16-bit heads on 16 bytes: matrix instructions of a warp ---------------------------------------------------------------------------
 //
-// A block has the query heads of a key head, up to 16 rows of a matrix, and a split of the sequence.  Each of its warps brings 16 or 32 keys and values at a time into places of its own in shared memory, one or two
-// sets on their way while one is used, and goes its own way until the end: no barrier of the block.  Products are m16n8k16; the arithmetic is a tenth of what they could do, so rows that no head fills cost nothing.
+// A block has the query heads of a key head, up to 16 rows of a matrix, and a split of the sequence.  Each of its warps brings 16 or 32 keys and values at a time into places of its own in shared memory, one
+// set on its way while one is used, and goes its own way until the end: no barrier of the block.  (Two sets on their way, and a block less on an SM: a million rows 49 us instead of 45.)  Products are m16n8k16; the arithmetic is a tenth of what they could do, so rows that no head fills cost nothing.
 // (tcgen05 takes 128 rows at least, of which 4 to 16 would be used, and its accumulators would have to come out of tensor memory for every 32 keys.)
 
-constexpr int kTileWarps = 4, kTileStages = 3, kTileHeads = 16, kMostClusters = 8;
+constexpr int kTileWarps = 4, kTileStages = 2, kTileHeads = 16, kMostClusters = 8;
 template <int W> constexpr int kKeysOfSet = W == 128 ? 16 : 32;          // two blocks then fit an SM, and one's way in and out is the other's time
 // Weights are at most 1: fp16 ones carry 2^15, so that one of 2^-29 is a normal number.
 template <typename T> constexpr float kStepLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
@@ -134,9 +134,14 @@ __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsA
     grid_dependency();
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     int rest = int(blockIdx.x);
-    const int split = rest % splits; rest /= splits;
-    const int chunk = rest % chunks; rest /= chunks;
-    const int key_head = rest % a.key_heads, b = rest / a.key_heads;
+    // a cluster is splits that follow one another; else blocks that run at once read the same rows' heads
+    int split = 0, chunk = 0;
+    if (CLUSTER) { split = rest % splits; rest /= splits; }
+    chunk = rest % chunks; rest /= chunks;
+    const int key_head = rest % a.key_heads;
+    rest /= a.key_heads;
+    if (!CLUSTER) { split = rest % splits; rest /= splits; }
+    const int b = rest;
     const int group = a.heads / a.key_heads, first_head = key_head * group + chunk * kTileHeads, heads = min(kTileHeads, group - chunk * kTileHeads);
     const StepRows r = rows_of(a, b);
     const bool any = !r.left_out && !r.full;
@@ -407,7 +412,8 @@ bool step_aligned(const HtgsAttentionStep& a) {
 
 struct StepPlan { bool tiles; int64_t blocks; int chunks, splits; bool cluster; };       // blocks: of one split
 // Splits of a sequence.  A block costs about as much as 128 rows beside its own, or 256 while it takes from others.  One sequence: the rounds of all places for a block, by a block's rows.  Several, whose lengths differ: blocks come and go, so all their rows (five
-// eighths of the capacity, say) spread over the places, and then the last block's.  Up to eight splits can be a cluster, whose join costs about 128 rows' time; more are joined by a kernel of its own, about 512.
+// eighths of the capacity, say) spread over the places, and then the last block's.  Up to eight splits
+// can be a cluster, whose join costs about 128 rows' time, where half the places are enough for all (32 scenes, 8 splits: 49 us in clusters, 42 without); else a kernel of its own joins them, about 512.
 StepPlan plan_of(const HtgsAttentionStep& a) {
     StepPlan p{step_aligned(a), 0, 1, 1, false};
     const int group = a.heads / a.key_heads;
@@ -416,7 +422,7 @@ StepPlan plan_of(const HtgsAttentionStep& a) {
     const int64_t rows = (a.window >= 0 && a.window < a.capacity ? a.window + 1 : a.capacity) + 1, slots = 148 * (p.tiles ? (a.width <= 32 ? 4 : 2) : 8);
     int64_t best = INT64_MAX;
     for (int splits = 1; splits <= kMostSplits && (splits == 1 || rows >= splits * 128); ++splits) {
-        const bool cluster = p.tiles && splits > 1 && splits <= kMostClusters;
+        const bool cluster = p.tiles && splits > 1 && splits <= kMostClusters && p.blocks * splits <= slots / 2;
         const int64_t time = a.batch == 1 ? (p.blocks * splits + slots - 1) / slots * (rows / splits + 128) : p.blocks * (rows * 5 / 8 + 256 * splits) / slots + rows / splits;
         const int64_t cost = time + (splits == 1 ? 0 : cluster ? 128 : 512);
         if (cost < best) { best = cost; p.splits = splits; p.cluster = cluster; }

@@ -398,3 +398,166 @@ def test_a_captured_forward_and_backward():
     graph.replay()
     for a, b in zip(captured, run()):
         assert torch.equal(a, b)
+
+
+# ---- many pieces, several calls at once, large places, states of failure ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("heads,key_heads,width,causal,window", [(8, 8, 32, False, 100), (4, 2, 64, True, None), (6, 1, 48, False, None), (4, 2, 128, True, None), (2, 2, 96, False, 150)])
+def test_copies_of_a_scene_get_the_same_bits(heads, key_heads, width, causal, window, kind):
+    """So many pieces that every block goes through several: each copy of three sequences, one of them empty, comes out as the first, and the first as alone."""
+    from htgs_b200 import sequence as seq
+    lengths, copies = (431, 0, 130), 60
+    one = [t.cpu() for t in tensors(sum(lengths), heads, key_heads, width, kind)]
+    ends = [0]
+    for _ in range(copies):
+        for n in lengths:
+            ends.append(ends[-1] + n)
+
+    def run(parts, ends):
+        leaves = [t.cuda().requires_grad_(True) for t in parts[:3]]
+        out = seq.attention(*leaves, offsets=torch.tensor(ends, dtype=torch.int32, device="cuda"), causal=causal, window=window)
+        return (out, *torch.autograd.grad(out, leaves, parts[3].cuda()))
+
+    alone = run(one, ends[:4])
+    for _ in range(3):
+        for a, b in zip(alone, run([t.repeat(copies, 1, 1) for t in one], ends)):
+            assert torch.equal(b.view(copies, *a.shape), a.expand(copies, *a.shape))
+    want, bound = ref.attend(*(f64(t) for t in one[:3]), ends[:4], causal, window, width ** -0.5, kind, f64(one[3]))
+    for name, t in zip(("out", "gq", "gk", "gv"), alone):
+        near(t, want[name], bound[name], name)
+
+
+def test_calls_of_several_threads_and_streams_at_once():
+    import threading
+    from htgs_b200 import sequence as seq
+    cases = [(tensors(900, 4, 2, 64, "bf16", seed=1), {"causal": True}), (tensors(700, 2, 2, 128, "fp16", seed=9), {"window": 77})]
+
+    def run(parts, how):
+        leaves = [t.detach().requires_grad_(True) for t in parts[:3]]
+        out = seq.attention(*leaves, **how)
+        return (out, *torch.autograd.grad(out, leaves, parts[3]))
+
+    serial = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(which):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = run(*cases[which])
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, serial[which])):
+                failures.append(which)
+        except Exception as e:  # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+
+
+@pytest.mark.parametrize("factor", [2.0 ** -14, 1.0, 2.0 ** 13])
+def test_half_precision_gradients_of_any_size(factor):
+    """Gradients of scores are 10^-3 of the output's gradient and less; those of small output gradients would be below the smallest number of fp16, those of large ones pass its largest in a sum."""
+    from htgs_b200 import sequence as seq
+    for width in (64, 128):
+        q, k, v, grad = tensors(700, 2, 1, width, "fp16")
+        grad = (grad.float() * factor * 0.25).half()
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+        got = torch.autograd.grad(seq.attention(*leaves), leaves, grad)
+        want, bound = ref.attend(f64(q), f64(k), f64(v), [0, 700], False, None, width ** -0.5, "fp16", f64(grad))
+        for name, t in zip(("gq", "gk", "gv"), got):
+            near(t, want[name], bound[name], name)
+
+
+def test_places_behind_two_to_the_31():
+    """The last rows of a cache of 2.2e9 values, and rows of a projection 2^16 values apart."""
+    from htgs_b200 import sequence as seq
+    capacity, heads, width = 2_200_000, 8, 128
+    keys, values = (torch.empty((1, capacity, heads, width), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q, k, v = (draw((1, heads, width), i, "bf16") for i in range(3))
+    keys[:, -60:], values[:, -60:] = draw((1, 60, heads, width), 4, "bf16"), draw((1, 60, heads, width), 5, "bf16")
+    out = seq.attention_step(q, k, v, keys, values, torch.tensor([capacity - 1], dtype=torch.int32, device="cuda"), window=50)
+    assert torch.equal(keys[0, -1], k[0]) and torch.equal(values[0, -1], v[0])
+    small = keys[:, -51:].clone(), values[:, -51:].clone()
+    assert torch.equal(out, seq.attention_step(q, k, v, *small, torch.tensor([50], dtype=torch.int32, device="cuda")))
+    del keys, values
+    far = torch.empty((40_000, 1 << 16), dtype=torch.bfloat16, device="cuda")[:, :3 * 64]
+    far.copy_(draw((40_000, 192), 6, "bf16"))
+    parts = [t.unflatten(1, (1, 64)) for t in far.split(64, dim=1)]
+    near_by = [t.contiguous() for t in parts]
+    assert torch.equal(seq.attention(*parts, window=30), seq.attention(*near_by, window=30))
+    p = torch.arange(40_000, dtype=torch.int32, device="cuda")[:, None]
+    assert torch.equal(seq.rotary(parts[0], None, p)[0], seq.rotary(near_by[0], None, p)[0])
+
+
+def test_a_wait_that_ran_out_is_reported_once():
+    """The word that a kernel would set is set by hand."""
+    from htgs_b200 import _native, sequence as seq
+    q, k, v, _ = tensors(20, 1, 1, 16, "bf16")
+    device = torch.cuda.current_device()
+    seq.attention(q, k, v)
+    word = _native.lib().htgs_attention_error_word(device)
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        seq.attention(q, k, v)
+    seq.check_attention()
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        seq.check_attention(q.device)
+    assert seq.attention(q, k, v).isfinite().all()
+
+
+def test_refusals():
+    from htgs_b200 import sequence as seq
+    q, k, v, _ = tensors(20, 4, 2, 16, "bf16")
+    n = torch.zeros(20, dtype=torch.int32, device="cuda")
+    p = torch.zeros((20, 2), device="cuda")
+    cache = torch.zeros((20, 5, 2, 16), dtype=torch.bfloat16, device="cuda")
+    other = torch.zeros_like(cache)
+    bad_values = [lambda: seq.attention(q, k[:10], v[:10]), lambda: seq.attention(q, k[:, :1].expand(20, 3, 16), v[:, :1].expand(20, 3, 16)), lambda: seq.attention(q, k, v[..., :8]),
+                  lambda: seq.attention(q, k, v, window=-1), lambda: seq.attention(q, k, v, scale=0.0), lambda: seq.attention(q, k, v, scale=float("nan")),
+                  lambda: seq.attention(q, k, v, offsets=n[:1]), lambda: seq.attention(q[None], k[None], v[None], offsets=n[:2]), lambda: seq.attention(q[:, 0], k[:, 0], v[:, 0]),
+                  lambda: seq.attention(*(torch.zeros((4, 1, 129), device="cuda") for _ in range(3))),
+                  lambda: seq.rotary(q[..., :15], None, p), lambda: seq.rotary(q, k[:10], p), lambda: seq.rotary(q, k, p[:10]), lambda: seq.rotary(q, k, p[:, :0]),
+                  lambda: seq.rotary(q, k, p, sections=[8]), lambda: seq.rotary(q, k, p, sections=[9, -1]), lambda: seq.rotary(q, k, p, sections=[4, 3]), lambda: seq.rotary(q, k, p, base=0.0),
+                  lambda: seq.rotary(q, k, p, base=float("inf")), lambda: seq.attention_step(q, k, v, cache, cache, n), lambda: seq.attention_step(q, k, v, cache[:, :, :1], other[:, :, :1], n),
+                  lambda: seq.attention_step(q, k, v, cache, other, n[:3]), lambda: seq.attention_step(q, k, v, cache, other, n, window=-2),
+                  lambda: seq.attention_step(q, k, v, cache[:, :1].expand(20, 5, 2, 16), other, n), lambda: seq.attention_step(q, k, v, cache.transpose(2, 3).contiguous().transpose(2, 3), other, n)]
+    for i, call in enumerate(bad_values):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    bad_types = [lambda: seq.attention(q, k.half(), v), lambda: seq.attention(q.double(), k.double(), v.double()), lambda: seq.attention(q, k, v, offsets=n.long()), lambda: seq.attention(q, k, v, window=1.5),
+                 lambda: seq.rotary(q, k, p.double()), lambda: seq.rotary(q, k, n.long()[:, None]), lambda: seq.attention_step(q, k, v, cache, other, n.long()), lambda: seq.attention(q, k, None)]
+    for i, call in enumerate(bad_types):
+        with pytest.raises(TypeError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    wants = q.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        seq.attention_step(wants, k, v, cache, other, n)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: seq.attention(dual, k, v), lambda: seq.rotary(dual, k, p), lambda: seq.attention_step(dual, k, v, cache, other, n)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+def test_the_step_advances_the_caches_versions():
+    from htgs_b200 import sequence as seq
+    q, k, v, _ = tensors(3, 2, 2, 16, "bf16")
+    keys, values = (torch.zeros((3, 5, 2, 16), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    before = keys._version, values._version
+    seq.attention_step(q, k, v, keys, values, torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert keys._version > before[0] and values._version > before[1]
+    with torch.inference_mode():
+        inside = torch.zeros_like(keys), torch.zeros_like(values)
+        seq.attention_step(q, k, v, *inside, torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert torch.equal(inside[0], keys)
