@@ -232,10 +232,10 @@ def lib():
                                                        ctypes.c_size_t, pointer]
                 l.htgs_gated_scan_step.argtypes = [pointer, i64, pointer, i64, pointer, i64, pointer, i64, i32, i64, i32, pointer]
                 l.htgs_rotary.argtypes = [ctypes.POINTER(HtgsRotary), pointer]
-                l.htgs_attention.argtypes = [ctypes.POINTER(HtgsAttention), pointer, pointer, pointer]
+                l.htgs_attention.argtypes = [ctypes.POINTER(HtgsAttention), pointer, pointer, pointer, pointer]
                 l.htgs_attention_backward_workspace_bytes.restype = ctypes.c_size_t
                 l.htgs_attention_backward_workspace_bytes.argtypes = [ctypes.POINTER(HtgsAttention)]
-                l.htgs_attention_backward.argtypes = [ctypes.POINTER(HtgsAttention), pointer, pointer, pointer, i64, i64, pointer, pointer, pointer, pointer, ctypes.c_size_t, pointer]
+                l.htgs_attention_backward.argtypes = [ctypes.POINTER(HtgsAttention), pointer, pointer, pointer, pointer, i64, i64, pointer, pointer, pointer, pointer, ctypes.c_size_t, pointer]
                 l.htgs_attention_status.argtypes = [i32]
                 l.htgs_attention_error_word.restype = ctypes.POINTER(ctypes.c_uint32)
                 l.htgs_attention_error_word.argtypes = [i32]

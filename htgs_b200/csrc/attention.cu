@@ -24,7 +24,7 @@ template <typename T> __device__ __forceinline__ void store_row(T* to, const flo
 
 // 32 rows of a head, four to a warp, against 32 rows at a time of those that they see, a lane for each.  Values that a row does not see meet nothing of it: neither its sums nor, by a
 // product with zero, its output.  Bound by loads from shared memory: five for four multiply-adds.
-template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention_lanes_kernel(const HtgsAttention a, T* out, float* sums) {
+template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention_lanes_kernel(const HtgsAttention a, T* out, T* rest, float* sums) {
     extern __shared__ float shared[];
     grid_dependency();
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, pitch = a.width | 1;
@@ -82,13 +82,20 @@ template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention
     for (int r = 0; r < kRowsOfWarp; ++r) {
         const int i = t.first + warp * kRowsOfWarp + r;
         if (i >= t.end) break;
-        store_row<T>(out + (int64_t(i) * a.heads + head) * a.width, o[r], t.outside ? 0.0f : 1.0f / l[r], a.width, lane);
+        const int64_t at = (int64_t(i) * a.heads + head) * a.width;
+        const float factor = t.outside ? 0.0f : 1.0f / l[r];
+        store_row<T>(out + at, o[r], factor, a.width, lane);
+        if (rest) {                    // what the rounding takes away
+            #pragma unroll
+            for (int c = 0; c < kColumns; ++c) o[r][c] = o[r][c] * factor - to_float<T>(from_float<T>(o[r][c] * factor));
+            store_row<T>(rest + at, o[r], 1.0f, a.width, lane);
+        }
         if (sums && lane == 0) sums[head * a.rows + i] = t.outside ? 0.0f : m[r] + log2f(l[r]);
     }
 }
 
 // Statistics of the rows of a tile of 128 and some heads.  Bound by HBM: reads the output and its gradient once.  LANES lanes have a row, N values of it at a time each.
-template <typename T, int N, int LANES> __global__ void __launch_bounds__(kLanesThreads) statistics_kernel(const HtgsAttention a, const T* out, const float* sums, const AttentionBackward b, float* statistics,
+template <typename T, int N, int LANES> __global__ void __launch_bounds__(kLanesThreads) statistics_kernel(const HtgsAttention a, const T* out, const T* rest, const float* sums, const AttentionBackward b, float* statistics,
                                                                                                           uint32_t* largest, int heads_of_block) {
     grid_dependency();
     const int lane = threadIdx.x % LANES, group = a.heads / a.key_heads, blocks = (a.heads + heads_of_block - 1) / heads_of_block;
@@ -112,6 +119,11 @@ template <typename T, int N, int LANES> __global__ void __launch_bounds__(kLanes
                 load_floats<T, N>(g + c, y);
                 #pragma unroll
                 for (int k = 0; k < N; ++k) { mean = fmaf(x[k], y[k], mean); grad = fmaf(y[k], y[k], grad); }
+                if (rest) {
+                    load_floats<T, N>(rest + (o - out) + c, x);
+                    #pragma unroll
+                    for (int k = 0; k < N; ++k) mean = fmaf(x[k], y[k], mean);
+                }
             }
             if (largest && head % group == 0) {
                 const T* v = static_cast<const T*>(a.v) + i * a.v_stride + head / group * a.v_head_stride;
@@ -243,9 +255,9 @@ int launch_lanes(Kernel kernel, PerDeviceOnce& once, const HtgsAttention& a, int
     return err == cudaSuccess ? sequence_status("htgs_attention") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
-template <typename T> int forward_lanes(const HtgsAttention& a, void* out, float* sums, cudaStream_t stream) {
+template <typename T> int forward_lanes(const HtgsAttention& a, void* out, void* rest, float* sums, cudaStream_t stream) {
     static PerDeviceOnce once;
-    return launch_lanes<T>(attention_lanes_kernel<T>, once, a, a.heads, 3, stream, static_cast<T*>(out), sums);
+    return launch_lanes<T>(attention_lanes_kernel<T>, once, a, a.heads, 3, stream, static_cast<T*>(out), static_cast<T*>(rest), sums);
 }
 template <typename T> int backward_lanes(const HtgsAttention& a, const AttentionBackward& b, cudaStream_t stream) {
     static PerDeviceOnce once, once_keys;
@@ -253,16 +265,16 @@ template <typename T> int backward_lanes(const HtgsAttention& a, const Attention
     return code != HTGS_OK ? code : launch_lanes<T>(attention_lanes_backward_kernel<T, true>, once_keys, a, a.key_heads, 4, stream, b);
 }
 template <typename T, int N, int LANES>
-int launch_statistics(const HtgsAttention& a, const void* out, const float* sums, const AttentionBackward& b, float* statistics, uint32_t* largest, cudaStream_t stream) {
+int launch_statistics(const HtgsAttention& a, const void* out, const void* rest, const float* sums, const AttentionBackward& b, float* statistics, uint32_t* largest, cudaStream_t stream) {
     // Some heads to a block, as long as there are eight blocks for each SM: the way in costs as much as a head (100003 rows, 8 heads of 32 in 7 sequences: 41 us with one head to a block).
     const int64_t tiles = sequence_tiles(a, kStatisticRows);
     const int heads = int(std::max<int64_t>(1, std::min<int64_t>(a.heads, tiles * a.heads / (148 * 8))));
-    const cudaError_t err = launch_after(statistics_kernel<T, N, LANES>, dim3(unsigned(tiles * ((a.heads + heads - 1) / heads))), kLanesThreads, 0, stream, a, static_cast<const T*>(out), sums, b,
+    const cudaError_t err = launch_after(statistics_kernel<T, N, LANES>, dim3(unsigned(tiles * ((a.heads + heads - 1) / heads))), kLanesThreads, 0, stream, a, static_cast<const T*>(out), static_cast<const T*>(rest), sums, b,
                                          statistics, largest, heads);
     return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
-template <typename T> int backward_typed(const HtgsAttention& a, const void* out, const float* sums, AttentionBackward b, float* statistics, uint32_t* largest, cudaStream_t stream) {
-    const bool tiles = aligned(out, 16) && attention_tiles_take(a, b);
+template <typename T> int backward_typed(const HtgsAttention& a, const void* out, const void* rest, const float* sums, AttentionBackward b, float* statistics, uint32_t* largest, cudaStream_t stream) {
+    const bool tiles = aligned(out, 16) && aligned(rest, 16) && attention_tiles_take(a, b);
     if constexpr (sizeof(T) == 2) {
         if (tiles) {
             if (std::is_same<T, __half>::value) {
@@ -270,12 +282,12 @@ template <typename T> int backward_typed(const HtgsAttention& a, const void* out
                 if (err != cudaSuccess) return sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
                 b.largest = largest;
             } else largest = nullptr;
-            const int code = a.width <= 32 ? launch_statistics<T, 8, 4>(a, out, sums, b, statistics, largest, stream)
-                             : a.width <= 64 ? launch_statistics<T, 8, 8>(a, out, sums, b, statistics, largest, stream) : launch_statistics<T, 8, 16>(a, out, sums, b, statistics, largest, stream);
+            const int code = a.width <= 32 ? launch_statistics<T, 8, 4>(a, out, rest, sums, b, statistics, largest, stream)
+                             : a.width <= 64 ? launch_statistics<T, 8, 8>(a, out, rest, sums, b, statistics, largest, stream) : launch_statistics<T, 8, 16>(a, out, rest, sums, b, statistics, largest, stream);
             return code != HTGS_OK ? code : attention_tiles_backward(a, b, stream);
         }
     }
-    const int code = launch_statistics<T, 1, 32>(a, out, sums, b, statistics, nullptr, stream);
+    const int code = launch_statistics<T, 1, 32>(a, out, rest, sums, b, statistics, nullptr, stream);
     return code != HTGS_OK ? code : backward_lanes<T>(a, b, stream);
 }
 
@@ -316,7 +328,7 @@ int htgs_attention_status(int32_t device) {
     return reported(attention_error_word(device));
 }
 
-int htgs_attention(const HtgsAttention* attention, void* out, float* sums, void* stream) {
+int htgs_attention(const HtgsAttention* attention, void* out, void* rest, float* sums, void* stream) {
     using namespace htgs;
     if (const char* message = wrong(attention)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
     if (attention->rows == 0) return HTGS_OK;
@@ -324,10 +336,10 @@ int htgs_attention(const HtgsAttention* attention, void* out, float* sums, void*
     if (const int code = reported(attention_error_word(current_device())); code != HTGS_OK) return code;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const HtgsAttention& a = *attention;
-    if (attention_tiles_take(a, out)) return attention_tiles_forward(a, out, sums, s);
-    if (a.type == HTGS_FLOAT32) return forward_lanes<float>(a, out, sums, s);
-    if (a.type == HTGS_FLOAT16) return forward_lanes<__half>(a, out, sums, s);
-    return forward_lanes<__nv_bfloat16>(a, out, sums, s);
+    if (attention_tiles_take(a, out, rest)) return attention_tiles_forward(a, out, rest, sums, s);
+    if (a.type == HTGS_FLOAT32) return forward_lanes<float>(a, out, rest, sums, s);
+    if (a.type == HTGS_FLOAT16) return forward_lanes<__half>(a, out, rest, sums, s);
+    return forward_lanes<__nv_bfloat16>(a, out, rest, sums, s);
 }
 
 size_t htgs_attention_backward_workspace_bytes(const HtgsAttention* attention) {
@@ -337,7 +349,7 @@ size_t htgs_attention_backward_workspace_bytes(const HtgsAttention* attention) {
     return size_t(statistic_rows(*attention)) * attention->heads * 2 * sizeof(float) + largest;
 }
 
-int htgs_attention_backward(const HtgsAttention* attention, const void* out, const float* sums, const void* grad_out, int64_t grad_out_stride, int64_t grad_out_head_stride,
+int htgs_attention_backward(const HtgsAttention* attention, const void* out, const void* rest, const float* sums, const void* grad_out, int64_t grad_out_stride, int64_t grad_out_head_stride,
                             void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace htgs;
     if (const char* message = wrong(attention)) return sequence_fail(HTGS_ERR_INVALID_ARGUMENT, message);
@@ -353,9 +365,9 @@ int htgs_attention_backward(const HtgsAttention* attention, const void* out, con
     const int64_t rows = statistic_rows(a);
     uint32_t* largest = reinterpret_cast<uint32_t*>(statistics + rows * a.heads * 2);
     const AttentionBackward b{grad_out, grad_out_stride, grad_out_head_stride, grad_q, grad_k, grad_v, statistics, rows, nullptr};
-    if (a.type == HTGS_FLOAT32) return backward_typed<float>(a, out, sums, b, statistics, largest, s);
-    if (a.type == HTGS_FLOAT16) return backward_typed<__half>(a, out, sums, b, statistics, largest, s);
-    return backward_typed<__nv_bfloat16>(a, out, sums, b, statistics, largest, s);
+    if (a.type == HTGS_FLOAT32) return backward_typed<float>(a, out, rest, sums, b, statistics, largest, s);
+    if (a.type == HTGS_FLOAT16) return backward_typed<__half>(a, out, rest, sums, b, statistics, largest, s);
+    return backward_typed<__nv_bfloat16>(a, out, rest, sums, b, statistics, largest, s);
 }
 
 }  // extern "C"

@@ -72,8 +72,8 @@ struct AttentionBackward {
 };
 
 // attention_tiles.cu: 16-bit types, widths that are a multiple of 8, everything on 16 bytes
-bool attention_tiles_take(const HtgsAttention& a, const void* out);
-int attention_tiles_forward(const HtgsAttention& a, void* out, float* sums, cudaStream_t stream);
+bool attention_tiles_take(const HtgsAttention& a, const void* out, const void* rest);
+int attention_tiles_forward(const HtgsAttention& a, void* out, void* rest, float* sums, cudaStream_t stream);
 bool attention_tiles_take(const HtgsAttention& a, const AttentionBackward& b);
 int attention_tiles_backward(const HtgsAttention& a, const AttentionBackward& b, cudaStream_t stream);
 unsigned int* attention_error_word(int device);

@@ -240,7 +240,7 @@ template <int GROUPS> __device__ __forceinline__ void give_registers() {
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
 }
 
-struct ForwardArgs { HtgsAttention a; void* out; float* sums; unsigned int* error; };
+struct ForwardArgs { HtgsAttention a; void* out; void* rest; float* sums; unsigned int* error; };
 
 // A piece is a head and one or two tiles of queries, one behind the other, against tiles of keys.  Warp 0 finds the pieces and loads; warps 1 and 2 issue the products, for one tile of queries while the other's softmax (or the other block's) is
 // computed, and the next piece's first scores while the last one's output is stored; warp 3 looks through values of which some are not seen; warps 4 to 7 and 8 to 11 have a tile of queries each, a thread
@@ -661,7 +661,14 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
                     float f[8];
                     #pragma unroll
                     for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[i + k]) * inverse;
-                    if (there && c + i < a.width) store_floats<T, 8>(at + c + i, f);
+                    if (there && c + i < a.width) {
+                        store_floats<T, 8>(at + c + i, f);
+                        if (args.rest) {                    // what the rounding takes away
+                            #pragma unroll
+                            for (int k = 0; k < 8; ++k) f[k] -= to_float<T>(from_float<T>(f[k]));
+                            store_floats<T, 8>(static_cast<T*>(args.rest) + (at - out) + c + i, f);
+                        }
+                    }
                 }
             }
             tmem_fence_before();
@@ -1804,13 +1811,13 @@ template <typename T> int forward_typed(const ForwardArgs& args, cudaStream_t st
 
 }  // namespace
 
-bool attention_tiles_take(const HtgsAttention& a, const void* out) {
-    return a.type != HTGS_FLOAT32 && a.width % 8 == 0 && aligned(out, 16) && heads_aligned(a.q, a.rows, a.heads, a.q_stride, a.q_head_stride) &&
+bool attention_tiles_take(const HtgsAttention& a, const void* out, const void* rest) {
+    return a.type != HTGS_FLOAT32 && a.width % 8 == 0 && aligned(out, 16) && aligned(rest, 16) && heads_aligned(a.q, a.rows, a.heads, a.q_stride, a.q_head_stride) &&
            heads_aligned(a.k, a.rows, a.key_heads, a.k_stride, a.k_head_stride) && heads_aligned(a.v, a.rows, a.key_heads, a.v_stride, a.v_head_stride);
 }
 
 bool attention_tiles_take(const HtgsAttention& a, const AttentionBackward& b) {
-    return attention_tiles_take(a, b.grad_q) && aligned(b.grad_k, 16) && aligned(b.grad_v, 16) && heads_aligned(b.grad, a.rows, a.heads, b.grad_stride, b.grad_head_stride);
+    return attention_tiles_take(a, b.grad_q, nullptr) && aligned(b.grad_k, 16) && aligned(b.grad_v, 16) && heads_aligned(b.grad, a.rows, a.heads, b.grad_stride, b.grad_head_stride);
 }
 
 int attention_tiles_backward(const HtgsAttention& a, const AttentionBackward& b, cudaStream_t stream) {
@@ -1820,10 +1827,10 @@ int attention_tiles_backward(const HtgsAttention& a, const AttentionBackward& b,
     return a.type == HTGS_FLOAT16 ? backward_typed<__half>(args, stream) : backward_typed<__nv_bfloat16>(args, stream);
 }
 
-int attention_tiles_forward(const HtgsAttention& a, void* out, float* sums, cudaStream_t stream) {
+int attention_tiles_forward(const HtgsAttention& a, void* out, void* rest, float* sums, cudaStream_t stream) {
     unsigned int* error = attention_error_word(current_device());
     if (!error) return sequence_fail(HTGS_ERR_CUDA, "htgs_attention: no host memory for the error word");
-    const ForwardArgs args{a, out, sums, error};
+    const ForwardArgs args{a, out, rest, sums, error};
     return a.type == HTGS_FLOAT16 ? forward_typed<__half>(args, stream) : forward_typed<__nv_bfloat16>(args, stream);
 }
 

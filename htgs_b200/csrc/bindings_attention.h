@@ -130,10 +130,11 @@ struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& given_offsets, int64_t sequences, bool causal, int64_t window, double scale) {
         const c10::cuda::CUDAGuard guard(q.device());
         const Tensor qh = heads_of(q), kh = heads_of(k), vh = heads_of(v), offsets = given_offsets ? *given_offsets : Tensor();
-        Tensor out = make(q, q.sizes()), sums = floats(q, {qh.size(1), qh.size(0)});
+        Tensor out = make(q, q.sizes()), sums = floats(q, {qh.size(1), qh.size(0)}), rest;
+        if (q.element_size() == 2) rest = make(q, q.sizes());
         const HtgsAttention a = attention_of(qh, kh, vh, offsets, {sequences, causal, window, scale});
-        check(htgs_attention(&a, out.data_ptr(), sums.data_ptr<float>(), stream_of(q)));
-        ctx->save_for_backward({qh, kh, vh, out, sums, offsets});
+        check(htgs_attention(&a, out.data_ptr(), rest.defined() ? rest.data_ptr() : nullptr, sums.data_ptr<float>(), stream_of(q)));
+        ctx->save_for_backward({qh, kh, vh, out, sums, offsets, rest});
         ctx->saved_data["sequences"] = sequences;
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["window"] = window;
@@ -146,7 +147,7 @@ struct Attention : torch::autograd::Function<Attention> {
     }
     static variable_list first_backward(AutogradContext* ctx, const variable_list& grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &sums = saved[4], &offsets = saved[5];
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &sums = saved[4], &offsets = saved[5], &rest = saved[6];
         const c10::cuda::CUDAGuard guard(q.device());
         const Tensor grad = heads_of(grads[0]);
         const auto keys = ctx->saved_data["keys"].toIntVector();
@@ -155,7 +156,7 @@ struct Attention : torch::autograd::Function<Attention> {
         Tensor grad_q = make(q, grads[0].sizes()), grad_k = make(k, keys), grad_v = make(v, keys);
         const size_t size = htgs_attention_backward_workspace_bytes(&a);
         Tensor workspace = bytes(q, size);
-        check(htgs_attention_backward(&a, out.data_ptr(), sums.data_ptr<float>(), grad.data_ptr(), grad.stride(0), grad.stride(1), grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr(),
+        check(htgs_attention_backward(&a, out.data_ptr(), rest.defined() ? rest.data_ptr() : nullptr, sums.data_ptr<float>(), grad.data_ptr(), grad.stride(0), grad.stride(1), grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr(),
                                       workspace.data_ptr(), size, stream_of(q)));
         return {grad_q, grad_k, grad_v, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
@@ -185,7 +186,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTen
     const Tensor qh = heads_of(q), kh = heads_of(k), vh = heads_of(v);
     Tensor out = make(q, q.sizes());
     const HtgsAttention a = attention_of(qh, kh, vh, off, {sequences, causal, window, scale});
-    check(htgs_attention(&a, out.data_ptr(), nullptr, stream_of(q)));
+    check(htgs_attention(&a, out.data_ptr(), nullptr, nullptr, stream_of(q)));
     return out;
 }
 

@@ -638,35 +638,37 @@ def _attention_struct(q, k, v, offsets, sequences, causal, window, scale) -> Htg
                          v.stride(1), q.shape[0], q.shape[1], k.shape[1], q.shape[2], sequences, _TYPES[q.dtype], int(causal), window, scale)
 
 
-def _attend(q, k, v, rest, keep):
-    """(out, sums or None) for tensors [rows, heads, width]."""
+def _attend(q, k, v, how, keep):
+    """(out, what its rounding took away or None, sums or None) for tensors [rows, heads, width]."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    rest = torch.empty_like(out) if keep and out.element_size() == 2 else None
     sums = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if keep else None
-    _call(q.device, "htgs_attention", ctypes.byref(_attention_struct(q, k, v, *rest)), out.data_ptr(), None if sums is None else sums.data_ptr())
-    return out, sums
+    _call(q.device, "htgs_attention", ctypes.byref(_attention_struct(q, k, v, *how)), out.data_ptr(), None if rest is None else rest.data_ptr(),
+          None if sums is None else sums.data_ptr())
+    return out, rest, sums
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, *rest):
+    def forward(ctx, q, k, v, *how):
         qh, kh, vh = _heads(q), _heads(k), _heads(v)
-        out, sums = _attend(qh, kh, vh, rest, True)
-        ctx.save_for_backward(qh, kh, vh, out, sums, rest[0])
-        ctx.rest, ctx.shapes = rest[1:], (q.shape, k.shape, v.shape)
+        out, rest, sums = _attend(qh, kh, vh, how, True)
+        ctx.save_for_backward(qh, kh, vh, out, rest, sums, how[0])
+        ctx.how, ctx.shapes = how[1:], (q.shape, k.shape, v.shape)
         return out.view(q.shape)
 
     @staticmethod
     @_first_derivative
     def backward(ctx, grad):
-        q, k, v, out, sums, offsets = ctx.saved_tensors
+        q, k, v, out, rest, sums, offsets = ctx.saved_tensors
         grad = _heads(grad)
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-        struct = _attention_struct(q, k, v, offsets, *ctx.rest)
+        struct = _attention_struct(q, k, v, offsets, *ctx.how)
         size = _native.lib().htgs_attention_backward_workspace_bytes(ctypes.byref(struct))
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _call(q.device, "htgs_attention_backward", ctypes.byref(struct), out.data_ptr(), sums.data_ptr(), grad.data_ptr(), grad.stride(0), grad.stride(1),
+        _call(q.device, "htgs_attention_backward", ctypes.byref(struct), out.data_ptr(), None if rest is None else rest.data_ptr(), sums.data_ptr(), grad.data_ptr(), grad.stride(0), grad.stride(1),
               *(g.data_ptr() for g in grads), workspace.data_ptr(), size)
-        return (*(g.view(shape) for g, shape in zip(grads, ctx.shapes)), *(None,) * (1 + len(ctx.rest)))
+        return (*(g.view(shape) for g, shape in zip(grads, ctx.shapes)), *(None,) * (1 + len(ctx.how)))
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Optional[torch.Tensor] = None, causal: bool = False, window: Optional[int] = None,
@@ -694,13 +696,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Option
             raise ValueError("offsets must hold sequences + 1 row numbers, for q of shape [rows, heads, width]")
         offsets = offsets.contiguous()
     sequences = q.shape[0] if q.dim() == 4 else 1 if offsets is None else offsets.numel() - 1
-    rest = (offsets, sequences, bool(causal), _window(window), _scale(scale, q.shape[-1]))
+    how = (offsets, sequences, bool(causal), _window(window), _scale(scale, q.shape[-1]))
     _no_tangent(q, k, v)
     if q.numel() == 0:
         return q * 1
     if _wants_grad(q, k, v):
-        return _Attention.apply(q, k, v, *rest)
-    return _attend(_heads(q), _heads(k), _heads(v), rest, False)[0].view(q.shape)
+        return _Attention.apply(q, k, v, *how)
+    return _attend(_heads(q), _heads(k), _heads(v), how, False)[0].view(q.shape)
 
 
 def check_attention(device: Optional[torch.device] = None) -> None:

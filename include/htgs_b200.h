@@ -551,7 +551,8 @@ int htgs_rotary(const HtgsRotary* rotary, void* stream);
  *   out_i = sum over j of softmax_j(scale * q_i . k_j) v_j
  * over the rows j of i's sequence with j <= i if causal, and |i - j| <= window if window >= 0.  q [rows, heads, width], k and v [rows, key_heads, width] have strides
  * in elements from row to row and from head to head; heads is a multiple of key_heads, and head h uses key head h / (heads / key_heads).  out [rows, heads, width] is dense.
- * sums [heads, rows] (log2 of each row's sum of exponentials) is what the backward pass needs, or NULL.  1 <= width <= 128, scale > 0.
+ * sums [heads, rows] (log2 of each row's sum of exponentials) is what the backward pass needs, or NULL; rest, dense as out and of its type, or NULL, is what out's rounding took away, which keeps the
+ * gradients of q and k from a rounding that all of a row's keys share (NULL for float32).  1 <= width <= 128, scale > 0.
  * 16-bit types with a width that is a multiple of 8 and rows and heads that begin on 16 bytes take the tensor cores, where the weights P and their gradients are rounded to
  * the type; others do not, and take 10 to 100 times as long.  The backward pass writes dense gradients; workspace as the size function says, 16-byte aligned.
  * A wait that runs out is reported as with htgs_fp8_matmul, by htgs_attention_status and the next call; what is not complete is NaN.
@@ -565,9 +566,9 @@ typedef struct HtgsAttention {
     int32_t heads, key_heads, width, n_sequences, type, causal, window;
     float scale;
 } HtgsAttention;
-int htgs_attention(const HtgsAttention* attention, void* out, float* sums, void* stream);
+int htgs_attention(const HtgsAttention* attention, void* out, void* rest, float* sums, void* stream);
 size_t htgs_attention_backward_workspace_bytes(const HtgsAttention* attention);
-int htgs_attention_backward(const HtgsAttention* attention, const void* out, const float* sums, const void* grad_out, int64_t grad_out_stride,
+int htgs_attention_backward(const HtgsAttention* attention, const void* out, const void* rest, const float* sums, const void* grad_out, int64_t grad_out_stride,
                             int64_t grad_out_head_stride, void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
 int htgs_attention_status(int32_t device);
 unsigned int* htgs_attention_error_word(int32_t device);

@@ -55,19 +55,19 @@ def test_attention_checks_its_arguments():
     for k in ({"q": None}, {"k": None}, {"v": None}, {"qs": -1}, {"kh": -1}, {"rows": -1}, {"rows": 1 << 31}, {"heads": 0}, {"heads": 3, "key_heads": 2}, {"key_heads": 0}, {"width": 0},
               {"width": 129}, {"n": 0}, {"n": 7}, {"type": 3}, {"scale": 0.0}, {"scale": -1.0}, {"scale": float("nan")}, {"scale": float("inf")}, {"rows": 0x7fffff00 // 64 * 64, "heads": 65536}):
         a = attention(**k)
-        refused(lib.htgs_attention(ctypes.byref(a), 64, None, None))
-        refused(lib.htgs_attention_backward(ctypes.byref(a), 64, 64, 64, 32, 16, 64, 64, 64, 64, 1 << 40, None))
+        refused(lib.htgs_attention(ctypes.byref(a), 64, None, None, None))
+        refused(lib.htgs_attention_backward(ctypes.byref(a), 64, None, 64, 64, 32, 16, 64, 64, 64, 64, 1 << 40, None))
         assert lib.htgs_attention_backward_workspace_bytes(ctypes.byref(a)) == 0
     a = attention()
-    refused(lib.htgs_attention(ctypes.byref(a), None, None, None))
-    refused(lib.htgs_attention(None, 64, None, None))
+    refused(lib.htgs_attention(ctypes.byref(a), None, None, None, None))
+    refused(lib.htgs_attention(None, 64, None, None, None))
     for at in range(7):
         pointers = [None if i == at else 64 for i in range(7)]
-        refused(lib.htgs_attention_backward(ctypes.byref(a), *pointers[:3], 32, 16, *pointers[3:], 1 << 30, None), SMALL if at == 6 else BAD)
-    refused(lib.htgs_attention_backward(ctypes.byref(a), 64, 64, 64, -1, 16, 64, 64, 64, 64, 1 << 30, None))
-    refused(lib.htgs_attention_backward(ctypes.byref(a), 64, 64, 64, 32, 16, 64, 64, 64, 64, 16, None), SMALL)
-    refused(lib.htgs_attention_backward(ctypes.byref(a), 64, 64, 64, 32, 16, 64, 64, 64, 72, 1 << 30, None), SMALL)
-    assert lib.htgs_attention(ctypes.byref(attention(rows=0)), 64, None, None) == 0
+        refused(lib.htgs_attention_backward(ctypes.byref(a), pointers[0], None, *pointers[1:3], 32, 16, *pointers[3:], 1 << 30, None), SMALL if at == 6 else BAD)
+    refused(lib.htgs_attention_backward(ctypes.byref(a), 64, None, 64, 64, -1, 16, 64, 64, 64, 64, 1 << 30, None))
+    refused(lib.htgs_attention_backward(ctypes.byref(a), 64, None, 64, 64, 32, 16, 64, 64, 64, 64, 16, None), SMALL)
+    refused(lib.htgs_attention_backward(ctypes.byref(a), 64, None, 64, 64, 32, 16, 64, 64, 64, 72, 1 << 30, None), SMALL)
+    assert lib.htgs_attention(ctypes.byref(attention(rows=0)), 64, None, None, None) == 0
     refused(lib.htgs_attention_status(-1))
     refused(lib.htgs_attention_status(64))
 
