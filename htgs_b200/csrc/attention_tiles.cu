@@ -214,6 +214,8 @@ template <typename T> __device__ __forceinline__ f32x2 exp2_polynomial(f32x2 x) 
 }
 
 // What an exponent may pass the running maximum by before the output is scaled down to a new one: weights up to 2^8 are as precise as those up to 1, and most tiles then leave the output alone.
+// (What is lost is that the largest weight is 1, which is not rounded: the output is off by 0.0023 of its size in bf16, where 0.0019 would be possible and its own rounding is 0.0017; a scaling at each new maximum costs 10 % for heads of
+// 64 and up to 30 % for those of 128.  In training with heads of more than 64 it is done all the same: the gradients of q and k, which the output's error reaches through D, have their score gradients rounded once more.)
 constexpr float kSlack = 8.0f;
 // Weights in fp16 are 2^6 times as large, so that one of 2^-20 of the row's largest is a normal number (and the largest is 2^14).
 template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 6.0f : 0.0f;
@@ -528,6 +530,7 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
         const uint32_t lanes = uint32_t(quarter) << 16, score = tmem + s * kTile + lanes, weights = score + S::weights, sum_at = tmem + S::outputs + s * kTile + lanes;
         const float scale = a.scale * kLog2e;
         const f32x2 scale2 = pack2(scale, scale);
+        const float slack = PANELS == 2 && args.rest ? 0.0f : kSlack;
         uint32_t tiles_done = 0, uses = 0;                     // so far: of this tile of queries; places of the ring, by the block
         bool ok = true;
         while (ok && next_piece()) {
@@ -581,7 +584,7 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
                 #pragma unroll
                 for (int i = 0; i < 8; ++i) m[i] = largest2(m[i], __uint_as_float(v[120 + i]));
                 const float tile_most = largest3(largest3(m[0], m[1], m[2]), largest3(m[3], m[4], m[5]), largest2(m[6], m[7])) * scale;
-                if (__any_sync(0xffffffffu, !(tile_most <= most + kSlack))) {
+                if (__any_sync(0xffffffffu, !(tile_most <= most + slack))) {
                     float now = largest2(most, tile_most);           // NaN makes the row's weights NaN, and so does infinity, which could only be taken from itself
                     now = now == infinity() ? __uint_as_float(0x7fffffffu) : now;
                     const float factor = most == now ? 1.0f : exp2_approx(most - now);
@@ -773,12 +776,13 @@ __device__ __forceinline__ bool all_meet(uint64_t* met, uint32_t& meetings, int 
 
 // Heads of up to 64: the gradients of k and v (KEYS) or of q of a piece, 128 rows of a head ("own": k and v, or q and dout), against tiles of 64 of the others (q and dout, or k and v), in turns by two
 // warpgroups, a thread for each own row.  Everything that a warpgroup writes or reads has columns of its own, so its next scores and weight gradients are computed while it works on the last ones, and it never
-// waits for more than its own arithmetic.  Warp 0 finds pieces and loads; warp 1 issues the products for scores and weight gradients; warp 2 those that add up, in the tiles' order; warp 3 looks through tiles that
+// waits for more than its own arithmetic.  Score gradients go into the sum in two parts, what their rounding takes away over the weight gradients that they were made of: the tensor cores have the time, and the gradients
+// of q and k are then rounded where they are stored and nowhere else to speak of (100003 rows within 256, heads of 32: off by 0.0021 of their size, 0.0027 in one part, for 0.0017 of the last rounding alone).  Warp 0 finds pieces and loads; warp 1 issues the products for scores and weight gradients; warp 2 those that add up, in the tiles' order; warp 3 looks through tiles that
 // are not seen whole.  Tensor memory: scores 0 and 64, weight gradients 128 and 192, weights 256 and 288, score gradients 320 and 352 (of q at both by turns), the sum for k or q 384, for v 448.
 struct NarrowTile {
     static constexpr int own_bytes = kPanelBytes, other = 64, bytes = other * 128, statistic_bytes = 2 * other * 4, stage_bytes = 2 * bytes + 1024, stages = 6;
     static constexpr int smem = 1024 + 2 * 2 * own_bytes + stages * stage_bytes + 1024;
-    static_assert((2 * kItems + 4 + 3 * stages + 22 + 2) * 8 + 8 + stages * 4 + kItems * 24 + 16 + int(sizeof(PieceShared)) <= 1024 && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");
+    static_assert((2 * kItems + 4 + 3 * stages + 20 + 2) * 8 + 8 + stages * 4 + kItems * 24 + 16 + int(sizeof(PieceShared)) <= 1024 && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");
 };
 
 template <typename T, bool KEYS>
@@ -801,8 +805,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
     uint64_t* const scored = searched + S::stages;       // its scores are there
     uint64_t* const scores_taken = scored + 2;           // and read
     uint64_t* const graded = scores_taken + 2;           // the gradients of its weights are there
-    uint64_t* const grades_taken = graded + 2;           // and read
-    uint64_t* const weighed = grades_taken + 2;          // its weights are there
+    uint64_t* const weighed = graded + 2;                // its weights are there
     uint64_t* const changed = weighed + 2;               // the gradients of its scores are: two, by turns, as a warpgroup may be two tiles ahead of the sums
     uint64_t* const added = changed + 4;                 // and both are in the sums: two, by turns
     uint64_t* const granted = added + 4;                 // the sums are its to change
@@ -823,7 +826,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
         for (int i = 0; i < kRecent; ++i) shared->recent[i] = -1;
         for (int i = 0; i < kItems; ++i) { mbar_init(item_full + i, 1); mbar_init(item_empty + i, 3 + 8); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(own_full + i, 1); mbar_init(own_empty + i, 1); mbar_init(scored + i, 1); mbar_init(scores_taken + i, 4); mbar_init(graded + i, 1); mbar_init(grades_taken + i, 4);
+            mbar_init(own_full + i, 1); mbar_init(own_empty + i, 1); mbar_init(scored + i, 1); mbar_init(scores_taken + i, 4); mbar_init(graded + i, 1);
             mbar_init(weighed + i, 4); mbar_init(changed + 2 * i, 4); mbar_init(changed + 2 * i + 1, 4); mbar_init(added + 2 * i, 1); mbar_init(added + 2 * i + 1, 1); mbar_init(granted + i, 1); mbar_init(returned + i, 4);
         }
         mbar_init(finished, 1);
@@ -984,7 +987,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                     if (!ok) break;
                     tmem_fence_after();
                     product(tmem + h * 64, x, y, scored + h);
-                    wait(grades_taken + h, parity);
+                    if (u > 1) wait(added + 2 * h + ((u >> 1) - 1 & 1), (u >> 1) - 1 >> 1 & 1);      // where they were lie the last score gradients' lower parts
                     if (!ok) break;
                     tmem_fence_after();
                     product(tmem + kGrades + h * 64, x + (S::own_bytes >> 4), y + (S::bytes >> 4), graded + h);
@@ -1018,7 +1021,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                     wait(changed + 2 * h + parity, u >> 2 & 1);
                     if (!ok) break;
                     tmem_fence_after();
-                    if (all || !dirty[slot]) gather(tmem + kSums, tmem + h * 32 + (KEYS || u >> 1 & 1 ? kChanges : kWeights), y, i == 0);
+                    if (all || !dirty[slot]) {
+                        gather(tmem + kSums, tmem + h * 32 + (KEYS || u >> 1 & 1 ? kChanges : kWeights), y, i == 0);
+                        gather(tmem + kSums, tmem + kGrades + h * 64, y, false);
+                    }
                     else {                         // the warpgroup adds them itself, when all before are in and before those behind
                         if (one) commit(granted + h);
                         __syncwarp();
@@ -1137,12 +1143,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                 tmem_begin32(grade, g);
                 tmem_begin32(grade + 32, g + 32);
                 tmem_loaded();
-                tmem_fence_before();
-                __syncwarp();
-                if (lane == 0) arrive(grades_taken + h);
                 const uint32_t changes = tmem + lanes + h * 32 + (KEYS || turn & 1 ? kChanges : kWeights);
                 {
-                    uint32_t words[32];
+                    uint32_t words[32], lower[32];
                     #pragma unroll
                     for (int c = 0; c < 64; c += 4) {
                         const float4 mean = KEYS ? statistics[16 + c / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1152,10 +1155,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                             const f32x2 away = KEYS ? fma2(k ? pack2(mean.z, mean.w) : pack2(mean.x, mean.y), minus, grad) : add2(grad, row_mean2);
                             const float2 ds = unpack2(mul2(std::is_same<T, __half>::value ? mul2(weight, lift2) : weight, away));
                             words[(c + k) / 2] = floats_pair<T>(ds.x, ds.y);
+                            const float2 upper = pair_floats<T>(words[(c + k) / 2]);
+                            lower[(c + k) / 2] = floats_pair<T>(ds.x - upper.x, ds.y - upper.y);
                         }
                     }
-                    if (masked) mask_words(words, from, to);
+                    if (masked) { mask_words(words, from, to); mask_words(lower, from, to); }
                     tmem_store32(changes, words);
+                    tmem_store32(grade, lower);
                 }
                 tmem_stored();
                 if (!KEYS && masked) {
@@ -1172,6 +1178,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                     ++grants;
                     tmem_fence_after();
                     multiply_seen<T>(sums, 0, a.width, u > u0, changes, 0, ring + slot * S::stage_bytes, from, to, 2);
+                    multiply_seen<T>(sums, 0, a.width, true, grade, 0, ring + slot * S::stage_bytes, from, to, 2);
                     if (KEYS) multiply_seen<T>(sums + 64, 0, a.width, u > u0, weights, 0, ring + slot * S::stage_bytes + S::bytes, from, to, 2);
                     tmem_fence_before();
                     __syncwarp();

@@ -47,14 +47,17 @@ def both_ways(q, k, v, grad, kind, ends=None, causal=False, window=None, scale=N
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
     out = seq.attention(*leaves, offsets=offsets, causal=causal, window=window, scale=scale)
     with torch.no_grad():
-        assert torch.equal(out, seq.attention(q, k, v, offsets=offsets, causal=causal, window=window, scale=scale))
+        inference = seq.attention(q, k, v, offsets=offsets, causal=causal, window=window, scale=scale)
+    if q.shape[-1] <= 64 or kind == "fp32":
+        assert torch.equal(out, inference)
     grads = torch.autograd.grad(out, leaves, grad)
     flat = [f64(t).flatten(0, -3) for t in (q, k, v, grad)]
     rows = flat[0].shape[0]
     if q.dim() == 4:
         ends = list(range(0, rows + 1, q.shape[1]))
     want, bound = ref.attend(*flat[:3], ends or [0, rows], causal, window, q.shape[-1] ** -0.5 if scale is None else scale, kind, flat[3])
-    for name, t in zip(("out", "gq", "gk", "gv"), (out, *grads)):
+    # wider heads take a row's largest weight as 1 in training and as up to 2^8 else: other roundings of the weights, each at most u of them, which the bound has
+    for name, t in zip(("out", "out", "gq", "gk", "gv"), (out, inference, *grads)):
         near(t.flatten(0, -3), want[name], bound[name], name)
     again = torch.autograd.grad(seq.attention(*leaves, offsets=offsets, causal=causal, window=window, scale=scale), leaves, grad)
     assert all(torch.equal(a, b) for a, b in zip(grads, again)), "the same inputs give the same bits"
