@@ -2,7 +2,7 @@
 //
 //   out = sum over cached rows j of softmax_j(scale * q . k_j) v_j,   the new row among them.
 //
-// A cache is read once: bound by HBM where caches are long, by the launch where they are short.  The rows of a sequence are split over blocks, by its length, which only the device knows;
+// A cache is read once: bound by HBM where caches are long (a million rows of 2 key heads of 64: 48 us, 5.4 TB/s; 32 scenes of up to 8192 rows, 2 key heads of 128: 40 us, 4.2 TB/s), by the launch where they are short (7 us).  The rows of a sequence are split over blocks, by its length, which only the device knows;
 // each leaves its largest score, its sum and its unnormalised output, and a second kernel joins them, always in the same order.
 #include "attention.cuh"
 
@@ -35,7 +35,7 @@ template <typename T> __device__ __forceinline__ void append(const HtgsAttention
     }
 }
 
-// One head and split to a block, a row at a time to a warp, columns to its lanes.
+// One head and split to a block, a row at a time to a warp, columns to its lanes.  Bound by a warp's sum for each row (a million rows, 8 heads of 64: 1.07 ms).
 template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes_kernel(const HtgsAttentionStep a, T* out, float* parts, int splits) {
     __shared__ float2 warps[kStepWarps];
     __shared__ float outputs[kStepWarps][kMostStepWidth];

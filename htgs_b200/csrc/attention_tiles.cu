@@ -712,13 +712,15 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
 constexpr int kBackwardTail = 512;
 template <typename T> constexpr float kWeightLift = std::is_same<T, __half>::value ? 14.0f : 0.0f;
 
-template <int PANELS> struct KeysTile {
-    static constexpr int bytes = PANELS * kPanelBytes, stages = PANELS == 2 ? 2 : 4, stage_bytes = 2 * bytes + kStatisticBytes;
+// Heads of more than 64.
+constexpr int kWidePanels = 2;
+struct KeysTile {
+    static constexpr int bytes = kWidePanels * kPanelBytes, stages = 2, stage_bytes = 2 * bytes + kStatisticBytes;
     static constexpr int smem = 1024 + 2 * bytes + stages * stage_bytes + kBackwardTail;
     static_assert((7 + 3 * stages) * 8 + 8 + stages * 8 <= kBackwardTail && smem <= 227 * 1024 && smem > 116 * 1024 && stage_bytes % 1024 == 0, "shared memory");
 };
-template <int PANELS> struct QueriesTile {
-    static constexpr int bytes = PANELS * kPanelBytes, stages = PANELS == 2 ? 5 : 8;
+struct QueriesTile {
+    static constexpr int bytes = kWidePanels * kPanelBytes, stages = 5;
     static constexpr int smem = 1024 + (2 + stages) * bytes + kBackwardTail;
     static_assert((8 + 3 * stages) * 8 + 8 + stages * 8 <= kBackwardTail && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");
 };
@@ -774,7 +776,7 @@ __device__ __forceinline__ bool all_meet(uint64_t* met, uint32_t& meetings, int 
     return ok;
 }
 
-// Heads of up to 64: the gradients of k and v (KEYS) or of q of a piece, 128 rows of a head ("own": k and v, or q and dout), against tiles of 64 of the others (q and dout, or k and v), in turns by two
+// Heads of up to 64 (262144 rows within 512, 4 heads of 64: 950 us for k and v, 740 for q): the gradients of k and v (KEYS) or of q of a piece, 128 rows of a head ("own": k and v, or q and dout), against tiles of 64 of the others (q and dout, or k and v), in turns by two
 // warpgroups, a thread for each own row.  Everything that a warpgroup writes or reads has columns of its own, so its next scores and weight gradients are computed while it works on the last ones, and it never
 // waits for more than its own arithmetic.  Score gradients go into the sum in two parts, what their rounding takes away over the weight gradients that they were made of: the tensor cores have the time, and the gradients
 // of q and k are then rounded where they are stored and nowhere else to speak of (100003 rows within 256, heads of 32: off by 0.0021 of their size, 0.0027 in one part, for 0.0017 of the last rounding alone).  Warp 0 finds pieces and loads; warp 1 issues the products for scores and weight gradients; warp 2 those that add up, in the tiles' order; warp 3 looks through tiles that
@@ -1224,11 +1226,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
 
 // Gradients of k and v of a tile.  Scores and their gradients are turned round, a row for each key, so that the weights are the first operand from tensor memory.  Warp 0 loads queries, output gradients and
 // statistics of a tile of queries; warp 1 issues the products, [dv, next scores] while the score gradients are computed and [dk, next weight gradients] while the weights are; warps 4 to 7 and 8 to 11
-// have 64 columns each.  Tensor memory: scores (weights) 0, weight gradients (score gradients) 128, dv 256, dk 384.
-template <typename T, int PANELS>
+// have 64 columns each.  Tensor memory: scores (weights) 0, weight gradients (score gradients) 128, dv 256, dk 384.  With the kernel behind it 16384 rows, causal, 8 heads of 128 take 1.5 to 1.8 ms, 1.0
+// PFLOP/s of the seven products.
+template <typename T>
 __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                          const __grid_constant__ CUtensorMap map_grad, const __grid_constant__ BackwardArgs args) {
-    using S = KeysTile<PANELS>;
+    using S = KeysTile;
     extern __shared__ unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     unsigned char* const own = raw + (base - smem_u32(raw));            // k, v
@@ -1288,7 +1291,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
             const bool one = elect_one();
             if (one) {
                 mbar_arrive_expect_tx(own_full, 2 * S::bytes);
-                for (int p = 0; p < PANELS; ++p) {
+                for (int p = 0; p < kWidePanels; ++p) {
                     load_panel(own + p * kPanelBytes, &map_k, p * kPanel, key_head, t.first, own_full);
                     load_panel(own + S::bytes + p * kPanelBytes, &map_v, p * kPanel, key_head, t.first, own_full);
                 }
@@ -1305,8 +1308,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
                     unsigned char* at = ring + stage.at * S::stage_bytes;
                     const int head = key_head * group + i / tiles, row = query_row(i);
                     mbar_arrive_expect_tx(full + stage.at, S::stage_bytes);
-                    for (int p = 0; p < PANELS; ++p) load_panel(at + p * kPanelBytes, &map_q, p * kPanel, head, row, full + stage.at);
-                    for (int p = 0; p < PANELS; ++p) load_panel(at + S::bytes + p * kPanelBytes, &map_grad, p * kPanel, head, row, full + stage.at);
+                    for (int p = 0; p < kWidePanels; ++p) load_panel(at + p * kPanelBytes, &map_q, p * kPanel, head, row, full + stage.at);
+                    for (int p = 0; p < kWidePanels; ++p) load_panel(at + S::bytes + p * kPanelBytes, &map_grad, p * kPanel, head, row, full + stage.at);
                     bulk_copy_g2s(at + 2 * S::bytes, statistics + (head * b.statistics_rows + i % tiles * kTile) * 2, kStatisticBytes, full + stage.at);
                 }
                 __syncwarp();
@@ -1514,10 +1517,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_keys_kernel(const 
 }
 
 // Gradient of q of a tile.  Scores are computed a tile ahead.  Tensor memory: scores (score gradients) by turns at 0 and 128, weight gradients 256, dq 384.
-template <typename T, int PANELS>
+template <typename T>
 __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                             const __grid_constant__ CUtensorMap map_grad, const __grid_constant__ BackwardArgs args) {
-    using S = QueriesTile<PANELS>;
+    using S = QueriesTile;
     extern __shared__ unsigned char raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     unsigned char* const own = raw + (base - smem_u32(raw));            // q, dout
@@ -1573,7 +1576,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(con
             const bool one = elect_one();
             if (one) {
                 mbar_arrive_expect_tx(own_full, 2 * S::bytes);
-                for (int p = 0; p < PANELS; ++p) {
+                for (int p = 0; p < kWidePanels; ++p) {
                     load_panel(own + p * kPanelBytes, &map_q, p * kPanel, head, t.first, own_full);
                     load_panel(own + S::bytes + p * kPanelBytes, &map_grad, p * kPanel, head, t.first, own_full);
                 }
@@ -1587,7 +1590,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_queries_kernel(con
                 if (!ok) break;
                 if (one) {
                     mbar_arrive_expect_tx(full + stage.at, S::bytes);
-                    for (int p = 0; p < PANELS; ++p) load_panel(ring + stage.at * S::bytes + p * kPanelBytes, i & 1 ? &map_v : &map_k, p * kPanel, key_head, low + (i >> 1) * kTile, full + stage.at);
+                    for (int p = 0; p < kWidePanels; ++p) load_panel(ring + stage.at * S::bytes + p * kPanelBytes, i & 1 ? &map_v : &map_k, p * kPanel, key_head, low + (i >> 1) * kTile, full + stage.at);
                 }
                 __syncwarp();
             }
@@ -1774,7 +1777,7 @@ template <typename T, int PANELS, int QUERIES> int launch_forward(const ForwardA
     if (err == cudaSuccess) err = launch_after(attention_tiles_kernel<T, PANELS, QUERIES>, dim3(unsigned(sequence_tiles(a, QUERIES * kTile) * a.heads)), S::threads, S::smem, stream, q, k, v, args);
     return err == cudaSuccess ? sequence_status("htgs_attention") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
-template <typename T, int PANELS> int launch_backward(const BackwardArgs& args, cudaStream_t stream) {
+template <typename T> int launch_wide(const BackwardArgs& args, cudaStream_t stream) {
     const HtgsAttention& a = args.a;
     CUtensorMap q, k, v, grad;
     if (!make_rows_map(&q, a.q, a.rows, a.heads, a.width, a.q_stride, a.q_head_stride) || !make_rows_map(&k, a.k, a.rows, a.key_heads, a.width, a.k_stride, a.k_head_stride) ||
@@ -1782,12 +1785,12 @@ template <typename T, int PANELS> int launch_backward(const BackwardArgs& args, 
         return sequence_fail(HTGS_ERR_CUDA, "htgs_attention_backward: the tensor maps cannot be made");
     static PerDeviceOnce once;
     cudaError_t err = once.run([] {
-        const cudaError_t e = cudaFuncSetAttribute(attention_keys_kernel<T, PANELS>, cudaFuncAttributeMaxDynamicSharedMemorySize, KeysTile<PANELS>::smem);
-        return e != cudaSuccess ? e : cudaFuncSetAttribute(attention_queries_kernel<T, PANELS>, cudaFuncAttributeMaxDynamicSharedMemorySize, QueriesTile<PANELS>::smem);
+        const cudaError_t e = cudaFuncSetAttribute(attention_keys_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, KeysTile::smem);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(attention_queries_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, QueriesTile::smem);
     });
     const int64_t tiles = sequence_tiles(a, kTile);
-    if (err == cudaSuccess) err = launch_after(attention_keys_kernel<T, PANELS>, dim3(unsigned(tiles * a.key_heads)), kTilesThreads, KeysTile<PANELS>::smem, stream, q, k, v, grad, args);
-    if (err == cudaSuccess) err = launch_after(attention_queries_kernel<T, PANELS>, dim3(unsigned(tiles * a.heads)), kTilesThreads, QueriesTile<PANELS>::smem, stream, q, k, v, grad, args);
+    if (err == cudaSuccess) err = launch_after(attention_keys_kernel<T>, dim3(unsigned(tiles * a.key_heads)), kTilesThreads, KeysTile::smem, stream, q, k, v, grad, args);
+    if (err == cudaSuccess) err = launch_after(attention_queries_kernel<T>, dim3(unsigned(tiles * a.heads)), kTilesThreads, QueriesTile::smem, stream, q, k, v, grad, args);
     return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 template <typename T> int launch_narrow(const BackwardArgs& args, cudaStream_t stream) {
@@ -1810,7 +1813,7 @@ template <typename T> int launch_narrow(const BackwardArgs& args, cudaStream_t s
     return err == cudaSuccess ? sequence_status("htgs_attention_backward") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 template <typename T> int backward_typed(const BackwardArgs& args, cudaStream_t stream) {
-    return args.a.width <= kPanel ? launch_narrow<T>(args, stream) : launch_backward<T, 2>(args, stream);
+    return args.a.width <= kPanel ? launch_narrow<T>(args, stream) : launch_wide<T>(args, stream);
 }
 template <typename T> int forward_typed(const ForwardArgs& args, cudaStream_t stream) {
     return args.a.width <= kPanel ? launch_forward<T, 1, 1>(args, stream) : launch_forward<T, 2, 2>(args, stream);

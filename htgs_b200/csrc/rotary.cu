@@ -70,6 +70,8 @@ __device__ __forceinline__ void sine_cosine(float z, float& sine, float& cosine)
     cosine = fmaf(fmaf(fmaf(fmaf(2.4438451873720624e-05f, w, -0.001388736767694354f), w, 0.04166664555668831f), w, -0.5f), w, 1.0f);
 }
 
+// Bound by HBM: 100000 rows of 10 heads of 64 in bf16 54 us, 4.8 TB/s (52 without angles); as many rows as two loads of a block's threads hold, five blocks on an SM (four 59 us, six 61).
+//
 // A block has a few rows: their cosines and sines, which all heads share, while the first values are on their way; then all heads of both tensors.  In 64 bits only what multiplies and adds: rounding is by a large
 // number, whose low bits then are the quarter, and positions are converted once a row, since conversions and roundings are made by a unit that takes longer than all the rest.
 template <typename T, int N, bool INTERLEAVED> __global__ void __launch_bounds__(kRotaryThreads, 5) rotary_kernel(const __grid_constant__ RotaryArgs args, const int rows_of_block) {
