@@ -1155,10 +1155,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                         for (int k = 0; k < 4; k += 2) {
                             const f32x2 grad = pack2(__uint_as_float(g[c + k]), __uint_as_float(g[c + k + 1])), weight = pack2(__uint_as_float(p[c + k]), __uint_as_float(p[c + k + 1]));
                             const f32x2 away = KEYS ? fma2(k ? pack2(mean.z, mean.w) : pack2(mean.x, mean.y), minus, grad) : add2(grad, row_mean2);
-                            const float2 ds = unpack2(mul2(std::is_same<T, __half>::value ? mul2(weight, lift2) : weight, away));
+                            const f32x2 change = mul2(std::is_same<T, __half>::value ? mul2(weight, lift2) : weight, away);
+                            const float2 ds = unpack2(change);
                             words[(c + k) / 2] = floats_pair<T>(ds.x, ds.y);
-                            const float2 upper = pair_floats<T>(words[(c + k) / 2]);
-                            lower[(c + k) / 2] = floats_pair<T>(ds.x - upper.x, ds.y - upper.y);
+                            const float2 upper = pair_floats<T>(words[(c + k) / 2]), rest = unpack2(fma2(pack2(upper.x, upper.y), minus, change));
+                            lower[(c + k) / 2] = floats_pair<T>(rest.x, rest.y);
                         }
                     }
                     if (masked) { mask_words(words, from, to); mask_words(lower, from, to); }

@@ -179,7 +179,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTen
     const int64_t sequences = q.dim() == 4 ? q.size(0) : off.defined() ? off.numel() - 1 : 1, window = window_of(given_window);
     const double scale = scale_of(given_scale, q.size(-1));
     no_tangent(q); no_tangent(k); no_tangent(v);
-    if (q.numel() == 0) return q.mul(1);
+    if (q.numel() == 0) return q.add(k.sum().add(v.sum()));               // nothing, and yet of all three
     if (c10::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v)))
         return Attention::apply(q, k, v, off.defined() ? OptTensor(off) : OptTensor(), sequences, causal, window, scale);
     const c10::cuda::CUDAGuard guard(q.device());

@@ -679,10 +679,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Option
     heads / key_heads neighbouring heads; width is 1 to 128, scale by default width^-0.5.  `offsets` is an int32 tensor of ascending row numbers that begin the sequences
     (sequences may be empty; rows of none, before the first and behind the last, get zeros).  Views such as the parts of one projection are read in place.  Scores and sums are
     32-bit.  float16 and bfloat16 with a width that is a multiple of 8 run on the tensor cores; float32 and other widths do not and are much slower.  What a row does not see never reaches
-    its result, not even infinities and NaN.  Differentiable in q, k and v."""
+    its result, not even infinities and NaN.  Differentiable in q, k and v; where a gradient is wanted the weights of heads of more than 64 are rounded otherwise than where none is, so last bits may differ."""
     compiled = _compiled()
     if compiled:
-        return compiled.attention(q, k, v, offsets, bool(causal), None if window is None else operator.index(window), None if scale is None else float(scale))
+        return compiled.attention(q, k, v, offsets, bool(causal), None if window is None else min(operator.index(window), 0x7fffffff), None if scale is None else float(scale))
     _check(q, "q")
     _check(k, "k", q.dtype, q.device)
     _check(v, "v", q.dtype, q.device)
@@ -699,7 +699,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Option
     how = (offsets, sequences, bool(causal), _window(window), _scale(scale, q.shape[-1]))
     _no_tangent(q, k, v)
     if q.numel() == 0:
-        return q * 1
+        return q + (k.sum() + v.sum())               # nothing, and yet of all three
     if _wants_grad(q, k, v):
         return _Attention.apply(q, k, v, *how)
     return _attend(_heads(q), _heads(k), _heads(v), how, False)[0].view(q.shape)
@@ -733,7 +733,7 @@ def attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, keys: torc
     For inference: it refuses inputs that want a gradient."""
     compiled = _compiled()
     if compiled:
-        return compiled.attention_step(q, k, v, keys, values, lengths, None if window is None else operator.index(window), None if scale is None else float(scale))
+        return compiled.attention_step(q, k, v, keys, values, lengths, None if window is None else min(operator.index(window), 0x7fffffff), None if scale is None else float(scale))
     _check(q, "q")
     for t, name in ((k, "k"), (v, "v"), (keys, "keys"), (values, "values")):
         _check(t, name, q.dtype, q.device)

@@ -251,10 +251,11 @@ def test_a_long_row_of_small_weights():
 
 def test_attention_without_rows_and_gradients_of_some_inputs():
     from htgs_b200 import sequence as seq
-    e = torch.empty((0, 2, 16), device="cuda", dtype=torch.bfloat16, requires_grad=True)
-    out = seq.attention(e, e, e)
+    e, f, g = (torch.empty((0, 2, 16), device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(3))
+    out = seq.attention(e, f, g, window=1 << 80)
     assert out.shape == (0, 2, 16)
     out.sum().backward()
+    assert all(t.grad.shape == t.shape for t in (e, f, g))
     q, k, v, grad = tensors(50, 2, 2, 16, "bf16")
     ql = q.clone().requires_grad_(True)
     (gq,) = torch.autograd.grad(seq.attention(ql, k, v), ql, grad)
