@@ -544,8 +544,8 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
             for (int j = from; j < to; ++j, ++tiles_done) {
                 ok = __all_sync(0xffffffffu, wait_in_line(scored + s, tiles_done & 1, failed));
                 if (!ok) break;
-                tmem_fence_after();
                 const bool used = S::apart && j > from && __all_sync(0xffffffffu, mbar_test(summed + s, (tiles_done - 1) & 1));      // the last tile's weights: asked here, where nothing waits for it
+                tmem_fence_after();              // behind both: what the last tile's product read is written over too
                 uint32_t v[128];
                 tmem_begin32(score, v);
                 tmem_begin32(score + 32, v + 32);
@@ -1122,6 +1122,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) attention_narrow_kernel(cons
                 if (!free) {
                     ok = __all_sync(0xffffffffu, wait_in_line(old, over >> 1 & 1, failed));
                     if (!ok) break;
+                    tmem_fence_after();
                 }
                 if (KEYS) {
                     uint32_t words[32];
