@@ -231,6 +231,7 @@ template <int PANELS, int QUERIES> struct ForwardTile {
     static constexpr int barriers = 2 * kItems + 3 * stages + 7 * QUERIES;
     static constexpr int smem = 1024 + (QUERIES + stages) * bytes + 1024;
     static_assert(barriers * 8 + 8 + stages * 4 + kItems * 24 + 16 + int(sizeof(PieceShared)) <= 1024 && smem <= 227 * 1024 / blocks - (blocks - 1) * 1024 && smem * (blocks + 1) > 227 * 1024, "shared memory");
+    static_assert(smem >= kLeastTensorShared && columns * blocks <= 512, "tensor memory");
 };
 // Registers of the warps that compute, and of the others; together those of the launch.
 template <int GROUPS> __device__ __forceinline__ void take_registers() {
@@ -718,11 +719,13 @@ struct KeysTile {
     static constexpr int bytes = kWidePanels * kPanelBytes, stages = 2, stage_bytes = 2 * bytes + kStatisticBytes;
     static constexpr int smem = 1024 + 2 * bytes + stages * stage_bytes + kBackwardTail;
     static_assert((7 + 3 * stages) * 8 + 8 + stages * 8 <= kBackwardTail && smem <= 227 * 1024 && smem > 116 * 1024 && stage_bytes % 1024 == 0, "shared memory");
+    static_assert(smem >= kLeastTensorShared, "tensor memory");
 };
 struct QueriesTile {
     static constexpr int bytes = kWidePanels * kPanelBytes, stages = 5;
     static constexpr int smem = 1024 + (2 + stages) * bytes + kBackwardTail;
     static_assert((8 + 3 * stages) * 8 + 8 + stages * 8 <= kBackwardTail && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");
+    static_assert(smem >= kLeastTensorShared, "tensor memory");
 };
 
 struct BackwardArgs { HtgsAttention a; AttentionBackward b; unsigned int* error; };
@@ -785,6 +788,7 @@ struct NarrowTile {
     static constexpr int own_bytes = kPanelBytes, other = 64, bytes = other * 128, statistic_bytes = 2 * other * 4, stage_bytes = 2 * bytes + 1024, stages = 6;
     static constexpr int smem = 1024 + 2 * 2 * own_bytes + stages * stage_bytes + 1024;
     static_assert((2 * kItems + 4 + 3 * stages + 20 + 2) * 8 + 8 + stages * 4 + kItems * 24 + 16 + int(sizeof(PieceShared)) <= 1024 && smem <= 227 * 1024 && smem > 116 * 1024, "shared memory");
+    static_assert(smem >= kLeastTensorShared, "tensor memory");
 };
 
 template <typename T, bool KEYS>

@@ -164,7 +164,7 @@ template <typename T, int BN, int MODE> struct Tile {
     static constexpr int partial_pitch = BN + 4;                                // floats
     static_assert(barriers * 8 + 16 <= 256 && smem > 116 * 1024 && smem <= 227 * 1024 && stage_bytes % 1024 == 0, "shared memory");
     static_assert(MODE != kSplit || kTileRows * partial_pitch * 4 <= stages * stage_bytes, "a part's sums fit the ring");
-    static_assert(kAccumulators * BN + kScaleStages * kScaleColumns <= 512, "tensor memory");
+    static_assert(kAccumulators * BN + kScaleStages * kScaleColumns <= 512 && smem >= kLeastTensorShared && alone_with_tensor_memory(smem), "tensor memory");
 };
 
 struct TileArgs {

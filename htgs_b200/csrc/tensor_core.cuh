@@ -12,6 +12,12 @@ namespace htgs {
 
 constexpr uint64_t kWaitNanoseconds = 2000000000ull;
 
+// Tensor memory (512 columns of an SM) is waited for without a limit, so a block that holds some may not wait for a block that still has to get its own.  The 8-bit product takes its columns ahead of its
+// wait for the kernel before, attention behind it; what keeps them apart is shared memory: no block that uses tensor memory has less than kLeastTensorShared, and one that takes columns ahead has so much that
+// none of those fits beside it.
+constexpr int kSharedOfSm = 228 * 1024, kSharedOfSystem = 1024, kLeastTensorShared = 98 * 1024;         // of system: in each block, beside its own
+constexpr bool alone_with_tensor_memory(int smem) { return smem + kLeastTensorShared + 2 * kSharedOfSystem > kSharedOfSm; }
+
 __device__ __forceinline__ uint64_t nanoseconds() { uint64_t t; asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t)); return t; }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {

@@ -43,3 +43,22 @@ def test_tensor_memory_is_touched_only_behind_a_fence():
                                         ("if (!free) {\nok = wait_in_line(old, 0, failed);\ntmem_fence_after();\n}\ntmem_store32(weights, words);", [])])
 def test_the_search_finds_what_it_looks_for(text, lines):
     assert unfenced(text) == lines
+
+
+def test_blocks_with_tensor_memory_that_may_wait_for_one_another_never_share_an_sm():
+    """Whoever takes tensor memory asserts, where it is compiled, how much shared memory it has; who takes it ahead of the wait for the kernel before, that it has an SM to itself."""
+    ahead = []
+    for name in sorted(os.listdir(build.CSRC)):
+        if not name.endswith(".cu"):
+            continue
+        with open(os.path.join(build.CSRC, name)) as f:
+            text = f.read()
+        kernels = [k for k in re.split(r"(?=\n__global__|\n(?:template <[^\n]*> )__global__)", text) if "__global__" in k and "tcgen05.alloc" in k]
+        if not kernels:
+            continue
+        tiles = re.findall(r"\nstruct (?:\w*Tile|Tile) \{.*?\n\};|> struct \w*Tile \{.*?\n\};", text, re.S)
+        assert tiles and all("smem >= kLeastTensorShared" in t for t in tiles), name
+        if any(k.index("tcgen05.alloc") < k.index("grid_dependency()") for k in kernels):
+            ahead.append(name)
+            assert all("alone_with_tensor_memory(smem)" in t for t in tiles), name
+    assert ahead == ["fp8_matmul.cu"]
