@@ -23,7 +23,7 @@ template <typename T> __device__ __forceinline__ void store_row(T* to, const flo
 }
 
 // 32 rows of a head, four to a warp, against 32 rows at a time of those that they see, a lane for each.  Values that a row does not see meet nothing of it: neither its sums nor, by a
-// product with zero, its output.  Bound by loads from shared memory, five for four multiply-adds: 11 TFLOP/s (20011 rows in 33 sequences, 8 heads of 64: 4.98 ms).
+// product with zero, its output.  Weights carry `unit`, so little that a row's add up to 1 at most, and no sum of values passes the largest of them.  Bound by loads from shared memory, five for four multiply-adds: 11 TFLOP/s (20011 rows in 33 sequences, 8 heads of 64: 4.98 ms).
 template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention_lanes_kernel(const HtgsAttention a, T* out, T* rest, float* sums) {
     extern __shared__ float shared[];
     grid_dependency();
@@ -33,13 +33,14 @@ template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention
     if (t.first >= t.end) return;
     float *const qs = shared, *const ks = qs + kLanesRows * pitch, *const vs = ks + kLanesRows * pitch;
     const int rows = min(kLanesRows, t.end - t.first);
-    float m[kRowsOfWarp], l[kRowsOfWarp] = {}, o[kRowsOfWarp][kColumns] = {};
+    float unit = 1.0f, m[kRowsOfWarp], l[kRowsOfWarp] = {}, o[kRowsOfWarp][kColumns] = {};
     #pragma unroll
     for (int r = 0; r < kRowsOfWarp; ++r) m[r] = -infinity();
     if (!t.outside) {
         fill_rows<T>(qs, pitch, a.q, a.q_stride, head * a.q_head_stride, t.first, t.end, a.width);
         const float scale = a.scale * kLog2e;
         const int low = first_seen(a, t.begin, t.first), high = last_seen(a, t.end, t.first + rows - 1);
+        unit = __uint_as_float(uint32_t(127 - bits_of(high - low + 1)) << 23);
         for (int at = low; at <= high; at += kLanesRows) {
             __syncthreads();
             fill_rows<T>(ks, pitch, a.k, a.k_stride, key_head * a.k_head_stride, at, high + 1, a.width);
@@ -59,7 +60,7 @@ template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention
                 seen[r] = __ballot_sync(0xffffffffu, sees);
                 const float x = sees ? s[r] * scale : -infinity(), most = fmaxf(m[r], lanes_max<32>(x)), base = most == -infinity() ? 0.0f : most, factor = exp2_approx(m[r] - base);
                 m[r] = most;
-                s[r] = exp2_approx(x - base);
+                s[r] = exp2_approx(x - base) * unit;
                 l[r] = l[r] * factor + warp_sum(s[r]);
                 #pragma unroll
                 for (int i2 = 0; i2 < kColumns; ++i2) o[r][i2] *= factor;
@@ -90,7 +91,7 @@ template <typename T> __global__ void __launch_bounds__(kLanesThreads) attention
             for (int c = 0; c < kColumns; ++c) o[r][c] = o[r][c] * factor - to_float<T>(from_float<T>(o[r][c] * factor));
             store_row<T>(rest + at, o[r], 1.0f, a.width, lane);
         }
-        if (sums && lane == 0) sums[head * a.rows + i] = t.outside ? 0.0f : m[r] + log2f(l[r]);
+        if (sums && lane == 0) sums[head * a.rows + i] = t.outside ? 0.0f : m[r] + log2f(l[r] / unit);
     }
 }
 

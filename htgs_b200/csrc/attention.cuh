@@ -61,6 +61,9 @@ __device__ __forceinline__ int last_seen(const HtgsAttention& a, int end, int i)
 __device__ __forceinline__ int first_seeing(const HtgsAttention& a, int begin, int j) { return a.causal ? j : first_seen(a, begin, j); }
 __device__ __forceinline__ int last_seeing(const HtgsAttention& a, int end, int j) { return a.window < 0 || end - 1 - j <= a.window ? end - 1 : j + a.window; }
 
+// The least b with n <= 2^b, of a positive n.
+__device__ __forceinline__ int bits_of(int n) { return 32 - __clz(n - 1); }
+
 __device__ __forceinline__ float exp2_approx(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float infinity() { return __uint_as_float(0x7f800000u); }
 

@@ -217,8 +217,10 @@ template <typename T> __device__ __forceinline__ f32x2 exp2_polynomial(f32x2 x) 
 // (What is lost is that the largest weight is 1, which is not rounded: the output is off by 0.0023 of its size in bf16, where 0.0019 would be possible and its own rounding is 0.0017; a scaling at each new maximum costs 10 % for heads of
 // 64 and up to 30 % for those of 128.  In training with heads of more than 64 it is done all the same: the gradients of q and k, which the output's error reaches through D, have their score gradients rounded once more.)
 constexpr float kSlack = 8.0f;
-// Weights in fp16 are 2^6 times as large, so that one of 2^-20 of the row's largest is a normal number (and the largest is 2^14).
-template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 6.0f : 0.0f;
+// Powers of two that weights carry.  fp16: 2^6, so that one of 2^-20 of the row's largest is a normal number (and the largest is 2^14); sums of such values are far from the end of 32 bits.  bf16, whose
+// values reach as far as 32 bits do: so little that the weights of n tiles of keys, 2^8 each at most, add up to a half at most, and no sum of values passes the largest of them.  (Without it 1.3e36, or a
+// thousand times 4e35, became infinite.  Exponents lose their last bits by it, 2^-19 of a weight.  By the piece's own tiles, so that a sequence gets the same bits whatever it is packed with.)
+template <typename T> __device__ __forceinline__ float lift_of(int n) { return std::is_same<T, __half>::value ? 6.0f : -(kSlack + 1.0f + float(bits_of(n * kTile))); }
 
 constexpr int kItems = 2;            // pieces of work that a block knows of: the present one and the next
 
@@ -540,6 +542,7 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
             const int row_low = first_seen(a, piece.begin, row), row_high = last_seen(a, piece.end, row);
             const int from = piece.from(s), to = piece.to(s);
             const int2 all = piece.whole(s);
+            const float lift = lift_of<T>(piece.n);
             float most = -infinity();
             f32x2 total2 = pack2(0.0f, 0.0f);
             for (int j = from; j < to; ++j, ++tiles_done) {
@@ -607,7 +610,7 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
                         tmem_stored();
                     }
                 }
-                const float shift = kLift<T> - (most == -infinity() ? 0.0f : most);
+                const float shift = lift - (most == -infinity() ? 0.0f : most);
                 const f32x2 shift2 = pack2(shift, shift);
                 f32x2 sums[2] = {total2, pack2(0.0f, 0.0f)};
                 #pragma unroll
@@ -678,7 +681,7 @@ __global__ void __launch_bounds__(128 + 128 * QUERIES, 3 - QUERIES) attention_ti
             tmem_fence_before();
             __syncwarp();
             if (lane == 0) arrive(drained + s);
-            if (args.sums && there) args.sums[piece.head * a.rows + row] = most - kLift<T> + log2f(sum);
+            if (args.sums && there) args.sums[piece.head * a.rows + row] = most - lift + log2f(sum);
         }
         tmem_fence_before();
     }
