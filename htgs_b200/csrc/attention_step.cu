@@ -18,6 +18,9 @@ __device__ __forceinline__ StepRows rows_of(const HtgsAttentionStep& a, int b) {
     const int n = __ldg(a.lengths + b);
     return {a.window >= 0 && n > a.window ? n - a.window : 0, n, n < 0, n >= a.capacity};
 }
+// Rows of a sequence that is not left out, as a power of two that they do not pass: weights carry its inverse (fp16: see kStepLift), so that a row's add up to 1 at most and no sum of values passes the
+// largest of them.  (Without it some 300 values of 1e36 became infinite.)
+__device__ __forceinline__ int row_bits(const StepRows& r) { return bits_of(r.length + 1 - r.low); }
 // Rows [first, last) of a split, in whole pieces but for the last.
 __device__ __forceinline__ int2 rows_of_split(const StepRows& r, int split, int splits) {
     const int rows = r.length + 1 - r.low, pieces = (rows + kStepPiece - 1) / kStepPiece;
@@ -47,7 +50,7 @@ template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes
     const bool any = !r.left_out && !r.full;
     if (any) {
         const int2 rows = rows_of_split(r, split, splits);
-        const float scale = a.scale * kLog2e;
+        const float scale = a.scale * kLog2e, unit = __uint_as_float(uint32_t(127 - row_bits(r)) << 23);
         float q[kStepColumns];
         #pragma unroll
         for (int i = 0; i < kStepColumns; ++i) {
@@ -67,7 +70,7 @@ template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes
                 value[i] = c < a.width ? to_float<T>(v[c]) : 0.0f;
             }
             s = warp_sum(s) * scale;
-            const float most = fmaxf(m, s), base = most == -infinity() ? 0.0f : most, factor = exp2_approx(m - base), p = exp2_approx(s - base);
+            const float most = fmaxf(m, s), base = most == -infinity() ? 0.0f : most, factor = exp2_approx(m - base), p = exp2_approx(s - base) * unit;
             m = most;
             l = fmaf(l, factor, p);
             #pragma unroll
@@ -104,8 +107,8 @@ template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes
 
 constexpr int kTileWarps = 4, kTileStages = 2, kTileHeads = 16, kMostClusters = 8;
 template <int W> constexpr int kKeysOfSet = W == 128 ? 16 : 32;          // two blocks then fit an SM, and one's way in and out is the other's time
-// Weights are at most 1: fp16 ones carry 2^15, so that one of 2^-29 is a normal number.
-template <typename T> constexpr float kStepLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
+// Weights are at most 1: fp16 ones carry 2^15, so that one of 2^-29 is a normal number (sums of such values are far from the end of 32 bits).
+constexpr float kStepLift = 15.0f;
 
 // Where piece `piece` (16 bytes) of a row of W values lies: eight rows of a piece are in banks of their own.
 template <int W> __device__ __forceinline__ uint32_t place_of(int row, int piece) {
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsA
                 const int head = lane / 4 + (i & 1) * 8, column = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
                 q[k][i] = head < heads && column < a.width ? __ldg(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + b * a.q_stride + (first_head + head) * a.q_head_stride + column)) : 0u;
             }
-        const float scale = a.scale * kLog2e;
+        const float scale = a.scale * kLog2e, lift = std::is_same<T, __half>::value ? kStepLift : -float(row_bits(r) + 1);          // bf16 weights are rounded: a half in all
         int first = rows.x + warp * kTileKeys, stage = 0;
         #pragma unroll
         for (int i = 0; i < kTileStages - 1; ++i) begin(first + i * kTileWarps * kTileKeys, i);
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) step_tiles_kernel(const HtgsA
             uint32_t p[kTileKeys / 8][2];
             #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float base = (most[i] == -infinity() ? 0.0f : most[i]) - kStepLift<T>;
+                const float base = (most[i] == -infinity() ? 0.0f : most[i]) - lift;
                 #pragma unroll
                 for (int n = 0; n < kTileKeys / 8; ++n) {
                     const float p0 = exp2_approx(s[n][2 * i] - base), p1 = exp2_approx(s[n][2 * i + 1] - base);

@@ -11,6 +11,17 @@ pytestmark = pytest.mark.gpu
 LARGE = 0.875 * 2.0 ** 126
 
 
+def step_reference(q, k, v, kind):
+    """The attention of one row of queries [heads, width] over all rows of k and v, and the bound of attention_reference.attend for it."""
+    u, n, width, group = ref.U[kind], k.shape[0], q.shape[1], q.shape[0] // k.shape[1]
+    k, v = k.repeat_interleave(group, dim=1), v.repeat_interleave(group, dim=1)
+    S, largest = (torch.einsum("hd,nhd->hn", a, b) * width ** -0.5 for a, b in ((q, k), (q.abs(), k.abs())))
+    P = torch.softmax(S, dim=1)
+    off = largest.amax(dim=1, keepdim=True) * (width * ref.SUM + 8 * ref.F) * 2 + 2.0 ** -20 + n * ref.SUM
+    want, spread = torch.einsum("hn,nhd->hd", P, v), torch.einsum("hn,nhd->hd", P, v.abs())
+    return want, u * want.abs() + (u + off + n * ref.SUM) * spread + ref.TINY[kind]
+
+
 def values(rows, heads, width, kind, seed):
     """Of one sign in each column, and a factor of two apart."""
     g = torch.Generator().manual_seed(seed)
@@ -59,3 +70,23 @@ def test_small_values_keep_their_bits(kind):
     out = seq.attention(q, k, v)
     want, bound = ref.attend(f64(q), f64(k), f64(v), [0, rows], False, None, 0.125, kind)
     near(out, want["out"], bound["out"])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("flat", [True, False])
+@pytest.mark.parametrize("batch,capacity,heads,key_heads,width,window", [(1, 70, 2, 1, 64, None), (2, 1500, 4, 2, 128, None), (1, 40000, 4, 1, 64, None), (3, 900, 1, 1, 13, None), (2, 60000, 2, 2, 32, 5000),
+                                                                        (9, 6000, 16, 8, 128, None)])
+def test_a_step_over_large_values_stays_finite(batch, capacity, heads, key_heads, width, window, flat, kind):
+    """Alone, in a cluster of splits and in splits that a second kernel joins."""
+    from htgs_b200 import sequence as seq
+    q, k, v = draw((batch, heads, width), 1, kind), draw((batch, key_heads, width), 2, kind), values(batch, key_heads, width, kind, 3)
+    if flat:
+        q.zero_()
+    keys = draw((batch, capacity, key_heads, width), 4, kind)
+    vals = values(batch * capacity, key_heads, width, kind, 5).view(batch, capacity, key_heads, width)
+    lengths = torch.tensor([capacity - 1 - 3 * b for b in range(batch)], dtype=torch.int32, device="cuda")
+    out = seq.attention_step(q, k, v, keys, vals, lengths, window=window)
+    for b, n in enumerate(lengths.tolist()):
+        low = 0 if window is None else max(0, n - window)
+        want, bound = step_reference(f64(q[b]), f64(keys[b, low:n + 1]), f64(vals[b, low:n + 1]), kind)
+        near(out[b], want, bound)
