@@ -414,9 +414,12 @@ bool step_aligned(const HtgsAttentionStep& a) {
 }
 
 struct StepPlan { bool tiles; int64_t blocks; int chunks, splits; bool cluster; };       // blocks: of one split
-// Splits of a sequence.  A block costs about as much as 128 rows beside its own, or 256 while it takes from others.  One sequence: the rounds of all places for a block, by a block's rows.  Several, whose lengths differ: blocks come and go, so all their rows (five
-// eighths of the capacity, say) spread over the places, and then the last block's.  Up to eight splits
-// can be a cluster, whose join costs about 128 rows' time, where half the places are enough for all (32 scenes, 8 splits: 49 us in clusters, 42 without); else a kernel of its own joins them, about 512.
+// Splits of a sequence, for caches that are full: what they hold only the device knows, and the plan has to bear the most.  (Plans for caches half or five eighths full are the same or a few splits apart, and
+// within 4 % in time at an eighth, a half and all of the capacity.)  A block costs about as much as 128 rows beside its own, or 256 while it takes from others.  One sequence: the rounds of all places for a
+// block, by a block's rows.  Several, whose lengths differ: blocks come and go, so all their rows spread over the places, and then the last block's.  Places are two on an SM for heads of more than 32, though
+// three fit: with splits for three a million rows of 2 key heads of 64 take 114 us instead of 108 (caches out of L2), 32 full caches of 8192 rows, 2 of 128, 58 instead of 54, 100 of 3000 rows, 1 of 96, 39
+// instead of 40.  Up to eight splits can be a cluster, whose join costs about 128 rows' time, where half the places are enough for all (32 scenes, 8 splits: 49 us in clusters, 42 without); else a kernel of
+// its own joins them, about 512.
 StepPlan plan_of(const HtgsAttentionStep& a) {
     StepPlan p{step_aligned(a), 0, 1, 1, false};
     const int group = a.heads / a.key_heads;
@@ -426,7 +429,7 @@ StepPlan plan_of(const HtgsAttentionStep& a) {
     int64_t best = INT64_MAX;
     for (int splits = 1; splits <= kMostSplits && (splits == 1 || rows >= splits * 128); ++splits) {
         const bool cluster = p.tiles && splits > 1 && splits <= kMostClusters && p.blocks * splits <= slots / 2;
-        const int64_t time = a.batch == 1 ? (p.blocks * splits + slots - 1) / slots * (rows / splits + 128) : p.blocks * (rows * 5 / 8 + 256 * splits) / slots + rows / splits;
+        const int64_t time = a.batch == 1 ? (p.blocks * splits + slots - 1) / slots * (rows / splits + 128) : p.blocks * (rows + 256 * splits) / slots + rows / splits;
         const int64_t cost = time + (splits == 1 ? 0 : cluster ? 128 : 512);
         if (cost < best) { best = cost; p.splits = splits; p.cluster = cluster; }
     }
