@@ -96,7 +96,7 @@ class GaussianRefiner(torch.nn.Module):
         if positions.shape[0] == 0:
             return positions.float()
         low, side, _ = _boxes(positions, offsets)
-        return ((positions.float() - low) / side * 1024.0).nan_to_num().clamp(0.0, 1024.0)[order]
+        return ((positions.float() - low) / side * 1024.0).nan_to_num().clamp(0.0, 1024.0).float()[order]        # 64-bit positions have a box in 64 bits
 
     def _attend(self, both, places, offsets):
         each = self.width // self.heads
