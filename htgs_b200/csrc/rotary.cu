@@ -20,9 +20,15 @@ struct RotaryArgs {
     uint8_t axis[kMostPairs];
 };
 
+// How pairs lie: first values apart from second ones; side by side; or side by side, but a pair does not begin on a multiple of its size, so that its values come one by one.
+enum PairLayout { kHalves, kInterleaved, kInterleavedAnywhere };
+// Whether N pairs are one load.
+template <typename T, int N, PairLayout LAYOUT> constexpr bool kWholePairs = LAYOUT == kInterleaved && 2 * N * sizeof(T) <= 16;
+
 // N pairs of a head: as they lie in memory, and as first and second values.
-template <typename T, int N, bool INTERLEAVED> struct Pairs {
-    static constexpr bool whole = INTERLEAVED && 2 * N * sizeof(T) <= 16;           // in one piece
+template <typename T, int N, PairLayout LAYOUT> struct Pairs {
+    static constexpr bool INTERLEAVED = LAYOUT != kHalves, whole = kWholePairs<T, N, LAYOUT>;
+    static_assert(LAYOUT != kInterleavedAnywhere || N == 1, "values one by one");
     Pack<T, whole ? 2 * N : N> one, two;
     __device__ __forceinline__ void load(const T* x, int second) {
         one = *reinterpret_cast<const decltype(one)*>(x);
@@ -74,7 +80,7 @@ __device__ __forceinline__ void sine_cosine(float z, float& sine, float& cosine)
 //
 // A block has a few rows: their cosines and sines, which all heads share, while the first values are on their way; then all heads of both tensors.  In 64 bits only what multiplies and adds: rounding is by a large
 // number, whose low bits then are the quarter, and positions are converted once a row, since conversions and roundings are made by a unit that takes longer than all the rest.
-template <typename T, int N, bool INTERLEAVED> __global__ void __launch_bounds__(kRotaryThreads, 5) rotary_kernel(const __grid_constant__ RotaryArgs args, const int rows_of_block) {
+template <typename T, int N, PairLayout LAYOUT> __global__ void __launch_bounds__(kRotaryThreads, 5) rotary_kernel(const __grid_constant__ RotaryArgs args, const int rows_of_block) {
     extern __shared__ __align__(16) float angles[];       // [rows][3][pairs], a row's on 16 bytes
     __shared__ double positions[kMostRows * 4], turns[kMostPairs];
     __shared__ uint8_t axis[kMostPairs];
@@ -86,7 +92,7 @@ template <typename T, int N, bool INTERLEAVED> __global__ void __launch_bounds__
     struct Place { const T* x; T* y; int angle; };
     const auto place = [&](int i) {
         const int row = i / of_row, rest = i - row * of_row, all = rest / chunks, chunk = rest - all * chunks, which = all >= r.heads[0], head = all - (which ? r.heads[0] : 0);
-        const int at = INTERLEAVED ? 2 * N * chunk : N * chunk;
+        const int at = LAYOUT == kHalves ? N * chunk : 2 * N * chunk;
         return Place{static_cast<const T*>(r.x[which]) + (first + row) * r.x_stride[which] + head * r.x_head_stride[which] + at,
                      static_cast<T*>(r.y[which]) + ((first + row) * r.heads[which] + head) * r.width + at, row * pitch + N * chunk};
     };
@@ -96,7 +102,7 @@ template <typename T, int N, bool INTERLEAVED> __global__ void __launch_bounds__
         positions[i] = r.positions_type == 0 ? double(static_cast<const float*>(r.positions)[at]) : double(static_cast<const int32_t*>(r.positions)[at]);
     }
     for (int i = threadIdx.x; i < pairs; i += kRotaryThreads) { turns[i] = args.turns[i]; axis[i] = args.axis[i]; }         // arguments are read one address at a time (21 of 70 us)
-    Pairs<T, N, INTERLEAVED> values[kAhead];
+    Pairs<T, N, LAYOUT> values[kAhead];
     Place places[kAhead];
     #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -124,38 +130,40 @@ template <typename T, int N, bool INTERLEAVED> __global__ void __launch_bounds__
         if (int(threadIdx.x) + k * kRotaryThreads < count) values[k].turn(angles + places[k].angle, pairs, places[k].y, pairs);
     for (int i = threadIdx.x + kAhead * kRotaryThreads; i < count; i += kRotaryThreads) {           // one row of many heads
         const Place p = place(i);
-        Pairs<T, N, INTERLEAVED> v;
+        Pairs<T, N, LAYOUT> v;
         v.load(p.x, pairs);
         v.turn(angles + p.angle, pairs, p.y, pairs);
     }
 }
 
-template <typename T, int N> int launch_rotary(const RotaryArgs& args, cudaStream_t stream) {
+template <typename T, int N, PairLayout LAYOUT> int launch_rotary(const RotaryArgs& args, cudaStream_t stream) {
     // Rows whose values the threads of a block load at once.
     const int items = (args.r.heads[0] + args.r.heads[1]) * (args.r.width / 2 / N), most = kAhead * kRotaryThreads / items, rows = most < 1 ? 1 : most > kMostRows ? kMostRows : most;
     const dim3 grid(unsigned((args.r.rows + rows - 1) / rows));
     const size_t smem = size_t(rows) * ((3 * (args.r.width / 2) + 3) / 4 * 4) * sizeof(float);
     static_assert(kMostRows * 3 * kMostPairs * 4 <= 47 * 1024, "shared memory");
-    const cudaError_t err = args.r.interleaved ? launch_after(rotary_kernel<T, N, true>, grid, kRotaryThreads, smem, stream, args, rows)
-                                               : launch_after(rotary_kernel<T, N, false>, grid, kRotaryThreads, smem, stream, args, rows);
+    const cudaError_t err = launch_after(rotary_kernel<T, N, LAYOUT>, grid, kRotaryThreads, smem, stream, args, rows);
     return err == cudaSuccess ? sequence_status("htgs_rotary") : sequence_fail(HTGS_ERR_CUDA, cudaGetErrorString(err));
 }
 
 // Pairs that a thread turns: as many as lie side by side in 16 bytes, if all rows and heads begin on such.
+template <typename T, int N, PairLayout LAYOUT> bool fits(const HtgsRotary& r) {
+    constexpr int unit = kWholePairs<T, N, LAYOUT> ? 2 * N : N;             // values of one load
+    bool ok = r.width / 2 % N == 0;
+    for (int i = 0; i < 2; ++i)
+        if (r.heads[i])
+            ok = ok && aligned(r.x[i], unit * sizeof(T)) && aligned(r.y[i], unit * sizeof(T)) && (r.rows == 1 || r.x_stride[i] % unit == 0) && (r.heads[i] == 1 || r.x_head_stride[i] % unit == 0);
+    return ok;
+}
+template <typename T, PairLayout LAYOUT> int rotary_laid_out(const RotaryArgs& args, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 2) { if (fits<T, 8, LAYOUT>(args.r)) return launch_rotary<T, 8, LAYOUT>(args, stream); }
+    if (fits<T, 4, LAYOUT>(args.r)) return launch_rotary<T, 4, LAYOUT>(args, stream);
+    if (fits<T, 2, LAYOUT>(args.r)) return launch_rotary<T, 2, LAYOUT>(args, stream);
+    if (fits<T, 1, LAYOUT>(args.r)) return launch_rotary<T, 1, LAYOUT>(args, stream);
+    return launch_rotary<T, 1, LAYOUT == kHalves ? kHalves : kInterleavedAnywhere>(args, stream);
+}
 template <typename T> int rotary_typed(const RotaryArgs& args, cudaStream_t stream) {
-    const HtgsRotary& r = args.r;
-    const auto fits = [&](int n) {
-        const int unit = r.interleaved && 2 * n * int(sizeof(T)) <= 16 ? 2 * n : n;      // values of one load
-        bool ok = r.width / 2 % n == 0;
-        for (int i = 0; i < 2; ++i)
-            if (r.heads[i])
-                ok = ok && aligned(r.x[i], unit * sizeof(T)) && aligned(r.y[i], unit * sizeof(T)) && (r.rows == 1 || r.x_stride[i] % unit == 0) && (r.heads[i] == 1 || r.x_head_stride[i] % unit == 0);
-        return ok;
-    };
-    if constexpr (sizeof(T) == 2) { if (fits(8)) return launch_rotary<T, 8>(args, stream); }
-    if (fits(4)) return launch_rotary<T, 4>(args, stream);
-    if (fits(2)) return launch_rotary<T, 2>(args, stream);
-    return launch_rotary<T, 1>(args, stream);
+    return args.r.interleaved ? rotary_laid_out<T, kInterleaved>(args, stream) : rotary_laid_out<T, kHalves>(args, stream);
 }
 
 }  // namespace
