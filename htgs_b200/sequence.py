@@ -538,10 +538,11 @@ def _sections(sections, axes: int, width: int):
     return sections
 
 
-def _turn(tensors, positions, sections, base, interleaved, inverse):
-    """One or two tensors [rows, heads, width] turned, dense."""
+def _turn(given, positions, sections, base, interleaved, inverse):
+    """One or two tensors [..., rows, heads, width] turned, dense; no views, which autograd would not let be changed in place."""
+    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in given]
+    tensors = [_heads(t) for t in given]
     rows, _, width = tensors[0].shape
-    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
     r = HtgsRotary()
     for i, (x, y) in enumerate(zip(tensors, out)):
         r.x[i], r.y[i], r.x_stride[i], r.x_head_stride[i], r.heads[i] = x.data_ptr(), y.data_ptr(), x.stride(0), x.stride(1), x.shape[1]
@@ -561,7 +562,7 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.rest = rest
         tensors = [t for t in (q, k) if t is not None]
-        out = [y.view(t.shape) for y, t in zip(_turn([_heads(t) for t in tensors], positions, *rest, False), tensors)]
+        out = _turn(tensors, positions, *rest, False)
         return tuple(out) if k is not None else out[0]
 
     @staticmethod
@@ -569,8 +570,8 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, *grads):
         (positions,) = ctx.saved_tensors
         there = [g for g in grads if g is not None]
-        out = iter(_turn([_heads(g) for g in there], positions, *ctx.rest, True)) if there else iter(())
-        turned = [None if g is None else next(out).view(g.shape) for g in grads]
+        out = iter(_turn(there, positions, *ctx.rest, True)) if there else iter(())
+        turned = [None if g is None else next(out) for g in grads]
         return (*turned, *(None,) * (3 - len(turned) + len(ctx.rest)))
 
 
@@ -610,7 +611,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if _wants_grad(*tensors):
         out = _Rotary.apply(q, k, positions, sections, base, bool(interleaved))
         return out if k is not None else (out, None)
-    out = [y.view(t.shape) for y, t in zip(_turn([_heads(t) for t in tensors], positions, sections, base, interleaved, False), tensors)]
+    out = _turn(tensors, positions, sections, base, interleaved, False)
     return out[0], out[1] if k is not None else None
 
 
@@ -638,9 +639,9 @@ def _attention_struct(q, k, v, offsets, sequences, causal, window, scale) -> Htg
                          v.stride(1), q.shape[0], q.shape[1], k.shape[1], q.shape[2], sequences, _TYPES[q.dtype], int(causal), window, scale)
 
 
-def _attend(q, k, v, how, keep):
-    """(out, what its rounding took away or None, sums or None) for tensors [rows, heads, width]."""
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+def _attend(q, k, v, how, keep, shape):
+    """(out, what its rounding took away or None, sums or None) for tensors [rows, heads, width]; `shape`: the output's, which is no view, as autograd would not let it be changed in place."""
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
     rest = torch.empty_like(out) if keep and out.element_size() == 2 else None
     sums = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if keep else None
     _call(q.device, "htgs_attention", ctypes.byref(_attention_struct(q, k, v, *how)), out.data_ptr(), None if rest is None else rest.data_ptr(),
@@ -652,10 +653,10 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, *how):
         qh, kh, vh = _heads(q), _heads(k), _heads(v)
-        out, rest, sums = _attend(qh, kh, vh, how, True)
+        out, rest, sums = _attend(qh, kh, vh, how, True, q.shape)
         ctx.save_for_backward(qh, kh, vh, out, rest, sums, how[0])
         ctx.how, ctx.shapes = how[1:], (q.shape, k.shape, v.shape)
-        return out.view(q.shape)
+        return out
 
     @staticmethod
     @_first_derivative
@@ -702,7 +703,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Option
         return q + (k.sum() + v.sum())               # nothing, and yet of all three
     if _wants_grad(q, k, v):
         return _Attention.apply(q, k, v, *how)
-    return _attend(_heads(q), _heads(k), _heads(v), how, False)[0].view(q.shape)
+    return _attend(_heads(q), _heads(k), _heads(v), how, False, q.shape)[0]
 
 
 def check_attention(device: Optional[torch.device] = None) -> None:
