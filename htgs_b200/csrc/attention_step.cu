@@ -2,7 +2,7 @@
 //
 //   out = sum over cached rows j of softmax_j(scale * q . k_j) v_j,   the new row among them.
 //
-// A cache is read once: bound by HBM where caches are long (a million rows of 2 key heads of 64: 48 us, 5.4 TB/s; 32 scenes of up to 8192 rows, 2 key heads of 128: 40 us, 4.2 TB/s), by the launch where they are short (7 us).  The rows of a sequence are split over blocks, by its length, which only the device knows;
+// A cache is read once: bound by HBM where caches are long (a million rows of 2 key heads of 64: 46 us, 5.6 TB/s; 32 scenes of up to 8192 rows, 2 key heads of 128: 40 us, 4.2 TB/s), by the launch where they are short (7 us).  The rows of a sequence are split over blocks, by its length, which only the device knows;
 // each leaves its largest score, its sum and its unnormalised output, and a second kernel joins them, always in the same order.
 #include "attention.cuh"
 
@@ -102,11 +102,11 @@ template <typename T> __global__ void __launch_bounds__(kStepThreads) step_lanes
 // ---- 16-bit heads on 16 bytes: matrix instructions of a warp ---------------------------------------------------------------------------
 //
 // A block has the query heads of a key head, up to 16 rows of a matrix, and a split of the sequence.  Each of its warps brings 16 or 32 keys and values at a time into places of its own in shared memory, one
-// set on its way while one is used, and goes its own way until the end: no barrier of the block.  (Two sets on their way, and a block less on an SM: a million rows 49 us instead of 45.)  Products are m16n8k16; the arithmetic is a tenth of what they could do, so rows that no head fills cost nothing.
-// (tcgen05 takes 128 rows at least, of which 4 to 16 would be used, and its accumulators would have to come out of tensor memory for every 32 keys.)
+// set on its way while one is used, and goes its own way until the end: no barrier of the block.  (Two sets on their way: a million rows 49 us instead of 46, 32 scenes 44 instead of 40.)  Products are m16n8k16; the arithmetic is a tenth of what they could do, so rows that no head fills cost nothing.
+// (tcgen05 takes 64 rows at least, of which 4 to 16 would be used; its accumulators would have to come out of tensor memory for every 32 keys, and the step is bound by HBM.)
 
 constexpr int kTileWarps = 4, kTileStages = 2, kTileHeads = 16, kMostClusters = 8;
-template <int W> constexpr int kKeysOfSet = W == 128 ? 16 : 32;          // two blocks then fit an SM, and one's way in and out is the other's time
+template <int W> constexpr int kKeysOfSet = W == 128 ? 16 : 32;          // 64 KB to a block at most, so that some fit an SM, and one's way in and out is the others' time
 // Weights are at most 1: fp16 ones carry 2^15, so that one of 2^-29 is a normal number (sums of such values are far from the end of 32 bits).
 constexpr float kStepLift = 15.0f;
 

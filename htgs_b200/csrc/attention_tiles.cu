@@ -214,7 +214,7 @@ template <typename T> __device__ __forceinline__ f32x2 exp2_polynomial(f32x2 x) 
 }
 
 // What an exponent may pass the running maximum by before the output is scaled down to a new one: weights up to 2^8 are as precise as those up to 1, and most tiles then leave the output alone.
-// (What is lost is that the largest weight is 1, which is not rounded: the output is off by 0.0023 of its size in bf16, where 0.0019 would be possible and its own rounding is 0.0017; a scaling at each new maximum costs 10 % for heads of
+// (What is lost is that the largest weight is a power of two, which is not rounded: the output is off by 0.0023 of its size in bf16, where 0.0019 would be possible and its own rounding is 0.0017; a scaling at each new maximum costs 10 % for heads of
 // 64 and up to 30 % for those of 128.  In training with heads of more than 64 it is done all the same: the gradients of q and k, which the output's error reaches through D, have their score gradients rounded once more.)
 constexpr float kSlack = 8.0f;
 // Powers of two that weights carry.  fp16: 2^6, so that one of 2^-20 of the row's largest is a normal number (and the largest is 2^14); sums of such values are far from the end of 32 bits.  bf16, whose

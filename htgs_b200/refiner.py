@@ -12,7 +12,8 @@ along the curve would be one number to the network.  The others are 8-bit produc
 once, and from then on `infer` has the norm leave 8-bit codes and the projections take them.
 
 With `heads` a layer also adds what each Gaussian finds among its neighbours along the curve: norm, projection to queries, keys and values, rotary positions by the Gaussians' places in their
-scene's box, attention to `window` rows on either side, projection back.  (No counterpart in the reference.)
+scene's box, attention to `window` rows on either side, projection back.  Attention is on the tensor cores where `dtype` has 16 bits and width / heads is a multiple of 8; else it is 10 to 100
+times slower.  (No counterpart in the reference.)
 """
 from __future__ import annotations
 

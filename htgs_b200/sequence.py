@@ -679,8 +679,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Option
     q is [rows, heads, width] and k and v [rows, key_heads, width] (one sequence, or with `offsets` several behind one another), or all with a batch in front; a key head serves
     heads / key_heads neighbouring heads; width is 1 to 128, scale by default width^-0.5.  `offsets` is an int32 tensor of ascending row numbers that begin the sequences
     (sequences may be empty; rows of none, before the first and behind the last, get zeros).  Views such as the parts of one projection are read in place.  Scores and sums are
-    32-bit.  float16 and bfloat16 with a width that is a multiple of 8 run on the tensor cores; float32 and other widths do not and are much slower.  What a row does not see never reaches
-    its result, not even infinities and NaN.  Differentiable in q, k and v; where a gradient is wanted the weights of heads of more than 64 are rounded otherwise than where none is, so last bits may differ."""
+    32-bit and stay in range with the values.  float16 and bfloat16 with a width that is a multiple of 8 run on the tensor cores, which take the weights rounded to that type; float32 and other
+    widths do not and are 10 to 100 times slower.  What a row does not see never reaches its result, not even infinities and NaN.
+
+    Differentiable in q, k and v (all three gradients are computed, whichever are wanted).  For them q, k, v, the result and 32 bits for each row and head are kept, and for 16-bit types another tensor of the
+    result's size: what its rounding took away.  Where a gradient is wanted the weights of heads of more than 64 are rounded otherwise than where none is, so last bits may differ."""
     compiled = _compiled()
     if compiled:
         return compiled.attention(q, k, v, offsets, bool(causal), None if window is None else min(operator.index(window), 0x7fffffff), None if scale is None else float(scale))

@@ -553,8 +553,9 @@ int htgs_rotary(const HtgsRotary* rotary, void* stream);
  * in elements from row to row and from head to head; heads is a multiple of key_heads, and head h uses key head h / (heads / key_heads).  out [rows, heads, width] is dense.
  * sums [heads, rows] (log2 of each row's sum of exponentials) is what the backward pass needs, or NULL; rest, dense as out and of its type, or NULL, is what out's rounding took away, which keeps the
  * gradients of q and k from a rounding that all of a row's keys share (NULL for float32).  1 <= width <= 128, scale > 0.
- * 16-bit types with a width that is a multiple of 8 and rows and heads that begin on 16 bytes take the tensor cores, where the weights P and their gradients are rounded to
- * the type; others do not, and take 10 to 100 times as long.  The backward pass writes dense gradients; workspace as the size function says, 16-byte aligned.
+ * Sums are 32-bit and stay in range with the values.
+ * 16-bit types with a width that is a multiple of 8 and rows and heads that begin on 16 bytes take the tensor cores, where the weights P are rounded to the type, and so are their
+ * gradients (those of heads of up to 64 in two parts); others do not, and take 10 to 100 times as long.  The backward pass writes dense gradients; workspace as the size function says, 16-byte aligned.
  * A wait that runs out is reported as with htgs_fp8_matmul, by htgs_attention_status and the next call; what is not complete is NaN.
  */
 typedef struct HtgsAttention {
